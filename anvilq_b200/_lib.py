@@ -16,6 +16,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 F = ctypes.c_float
 SZ = ctypes.c_size_t
+LL = ctypes.c_longlong
 
 # name -> (restype, argtypes); kept in the order of include/anvilq.h
 SIGNATURES = {
@@ -66,6 +67,15 @@ SIGNATURES = {
     "anvilq_lmhead_argmax": (I, [P, P, F, P, P, P, I, I, ctypes.c_uint, P]),
     "anvilq_argmax_commit": (I, [P, P, P, ctypes.c_uint, P]),
     "anvilq_gqa_decode_paged": (I, [P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, SZ, P, P]),
+    "anvilq_paged_kv_append": (I, [P, LL, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, P, ctypes.c_uint, P]),
+    "anvilq_paged_kv_append_q8": (I, [P, LL, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, ctypes.c_uint,
+                                      P]),
+    "anvilq_kv_q8_values": (I, [P, P, P, P, I, P, P, I, I, I, I, ctypes.c_uint, P]),
+    "anvilq_gqa_decode_q8_workspace_size": (SZ, [I, I, I, I, I]),
+    "anvilq_gqa_decode_q8": (I, [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, P, SZ, P, ctypes.c_uint, P]),
+    "anvilq_logits_process_workspace_size": (SZ, [I, I]),
+    "anvilq_logits_process": (I, [P, I, LL, P, LL, P, I, I, P, LL, P, P, I, P, P, P, P, P, P, I, P, LL, P, I, P, SZ, P,
+                                  ctypes.c_uint, P]),
     "anvilq_tree_attention_workspace_size": (SZ, [I, I, I, I, I]),
     "anvilq_tree_attention": (I, [P, P, P, P, I, P, I, I, I, I, I, F, P, SZ, P, P]),
     "anvilq_rmsnorm_rows": (I, [P, P, F, P, I, I, ctypes.c_uint, P]),
@@ -74,6 +84,10 @@ SIGNATURES = {
     "anvilq_legacy_kv_encode": (I, [P, P, P, I, I, I, I, I, P]),
     "anvilq_legacy_kv_decode": (I, [P, P, P, I, I, I, I, I, P, P]),
 }
+
+KV_Q8_BLOCK = 16       # tokens that share a scale of an 8-bit page
+KV_Q8_INT8 = 0
+KV_Q8_E4M3 = 1
 
 GEMV_KERNEL_CLUSTER = 0
 GEMV_KERNEL_STREAM = 1

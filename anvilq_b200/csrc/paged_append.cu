@@ -1,0 +1,423 @@
+// paged_append.cu -- appending the new tokens of a ragged batch to a paged KV
+// cache, with the position rotation of q and k on the way: binary16 pages (the
+// pools of anvilq_gqa_decode_paged) or 8-bit pages (kv_q8.cuh).
+//
+// Mathematics.  Row t of qkv is a new token of sequence b at position p.  With
+// angle_i = fp32(p * theta^(-2i/D)) (binary64 product, as anvilq_rope_kv_append),
+// every q and k head is rotated in split halves,
+//   a' = a cos angle_i - b sin angle_i,  b' = b cos angle_i + a sin angle_i
+// (a = x[i], b = x[i + D/2]; binary32, each operation rounded), q goes to q_out in
+// binary16, k' and v to row p % page_tokens of page page_table[b][p / page_tokens].
+// 8-bit pages: a block of 16 tokens and a head share a scale s,
+//   s = max(s_kept, scale_for(largest |value| of the block's new rows)),
+//   code = round(value * fp32(1 / s)),
+// s_kept being the scale of rows already in the block (0 where the block starts
+// with a new row).  Where s > s_kept the kept rows are re-coded,
+//   code' = round(code * fp32(s_kept / s)).
+// Values are coded from binary32, not from a binary16 rounding of them.
+//
+// What bounds it: bytes (2 B in, 2 or 1 B out for every element; a few binary32
+// operations each), and for a decode step, one token a sequence, the latency of
+// the chain search -> page-table word -> row -> store.
+//
+// Work split: an item is the run of new rows of one sequence inside one block of
+// 16 positions (the unit of a scale; it never leaves a page), and a slice of the
+// heads.  A CTA computes the item's cosines and sines once, into shared memory;
+// its warps then take heads.  A lane holds 8 consecutive dims of both halves of a
+// row, 16-byte loads and stores.
+#include <algorithm>
+#include <cmath>
+
+#include "kv_q8.cuh"
+
+namespace anvilq {
+namespace append {
+
+using q8::kBlock;
+constexpr int kBinary16 = -1;   // the pool's type: binary16, q8::kInt8 or q8::kE4m3
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxPairs = 64;   // D <= 128
+
+struct Freq {
+  double inv[kMaxPairs];   // theta^(-2i/D), binary64, computed on the host
+};
+
+struct Params {
+  const __half* qkv;            // [T] rows of (Hq + 2 Hkv) D, `stride` elements apart
+  long long stride;
+  const int* starts;            // [B + 1]
+  const int* seqlens;           // [B], the new tokens counted
+  const uint32_t* page_table;   // [B][max_pages]
+  __half* q_out;                // [T][Hq][D]
+  void* k;
+  void* v;
+  float* k_scales;
+  float* v_scales;
+  int* dev_err;
+  int T, B, Hq, Hkv, page_tokens, max_pages, num_pages;
+  int by_token;                 // how blockIdx.x names an item, see find_item
+  int heads_per_cta;
+};
+
+// The item of a CTA: rows [row, row + count) of qkv, positions pos .. of sequence b.
+struct Item {
+  int b, row, pos, count;
+};
+
+// The largest b in [0, n) with key(b) <= x, for a non-decreasing key with
+// key(0) <= x (else 0): the whole warp, 32 probes a step.
+template <typename Key>
+__device__ __forceinline__ int warp_search(int n, int x, Key key) {
+  const int lane = threadIdx.x % 32;
+  int lo = 0, span = n;
+  while (span > 1) {
+    const int step = (span + 31) / 32;
+    const int at = lo + lane * step;
+    const bool le = lane * step < span && key(at) <= x;
+    const uint32_t hit = __ballot_sync(0xffffffffu, le);
+    const int k = hit ? 31 - __clz(hit) : 0;
+    span = min(step, span - k * step);
+    lo += k * step;
+  }
+  return lo;
+}
+
+// Two ways to number the items without a pass over the batch, the host taking
+// the one with fewer numbers (a number without an item ends its CTA):
+//   by token: number t names the item whose first row is t, if t is one;
+//   by place: sequence b's items follow from starts[b] / 16 + 2 b on (its n rows
+//             lie in at most n / 16 + 2 blocks, so the ranges are disjoint).
+__device__ __forceinline__ Item find_item(const Params& p, int number) {
+  Item none{0, 0, 0, 0};
+  const int b = p.by_token ? warp_search(p.B, number, [&](int i) { return p.starts[i]; })
+                           : warp_search(p.B, number, [&](int i) { return p.starts[i] / kBlock + 2 * i; });
+  const int s0 = p.starts[b], s1 = p.starts[b + 1], len = p.seqlens[b];
+  if (s1 <= s0) return none;
+  const long long first = (long long)len - ((long long)s1 - s0);   // position of row s0
+  if (s0 < 0 || s1 > p.T || first < 0 || len > (long long)p.page_tokens * p.max_pages) {
+    if (threadIdx.x == 0 && p.dev_err) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+    return none;
+  }
+  const int p0 = (int)first;
+  int pos;
+  if (p.by_token) {
+    if (number < s0 || number >= s1) return none;
+    pos = p0 + (number - s0);
+    if (number != s0 && pos % kBlock) return none;
+  } else {
+    const int k = number - (s0 / kBlock + 2 * b);
+    const int block = p0 / kBlock + k;
+    if (k < 0 || block > (len - 1) / kBlock) return none;
+    pos = max(p0, block * kBlock);
+  }
+  return Item{b, s0 + (pos - p0), pos, min(len, (pos / kBlock + 1) * kBlock) - pos};
+}
+
+__device__ __forceinline__ void unpack8(const uint4& w, float* v) {
+  const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  uint4 w;
+  __half2* h = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+  return w;
+}
+
+template <int D, int TYPE>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ Params p,
+                                                          const __grid_constant__ Freq freq) {
+  constexpr int kHalf = D / 2;
+  constexpr int kLanes = D / 16;              // lanes of a row: 8 dims of each half a lane
+  constexpr int kRows = 32 / kLanes;          // rows of a pass of a warp
+  constexpr int kPasses = kBlock / kRows;
+  __shared__ __align__(16) float s_cos[kBlock][kHalf];
+  __shared__ __align__(16) float s_sin[kBlock][kHalf];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Item it = find_item(p, blockIdx.x);
+  if (it.count <= 0) return;   // the same for the whole CTA
+  const int logical = it.pos / p.page_tokens;
+  const int page = q8::page_of(p.page_table, p.max_pages, p.num_pages, it.b, logical);
+  if (page < 0) {
+    if (threadIdx.x == 0 && p.dev_err) atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
+    return;
+  }
+  for (int i = threadIdx.x; i < it.count * kHalf; i += kThreads) {
+    const int r = i / kHalf, pair = i % kHalf;
+    const float angle = (float)((double)(it.pos + r) * freq.inv[pair]);
+    sincosf(angle, &s_sin[r][pair], &s_cos[r][pair]);
+  }
+  __syncthreads();
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int d0 = 8 * (lane % kLanes);
+  const int heads = p.Hq + 2 * p.Hkv;
+  const int head_end = min(heads, (int)(blockIdx.y + 1) * p.heads_per_cta);
+  const int slot = it.pos % p.page_tokens;    // row of the page of the item's first token
+  for (int head = blockIdx.y * p.heads_per_cta + warp; head < head_end; head += kWarps) {
+    uint4 lo[kPasses], hi[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRows + lane / kLanes;
+      lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+      if (r < it.count) {
+        const __half* src = p.qkv + (size_t)(it.row + r) * p.stride + head * D + d0;
+        lo[i] = *reinterpret_cast<const uint4*>(src);
+        hi[i] = *reinterpret_cast<const uint4*>(src + kHalf);
+      }
+    }
+    const bool is_q = head < p.Hq, turned = head < p.Hq + p.Hkv;
+    const int kvh = is_q ? 0 : (head - p.Hq) % p.Hkv;
+    float x[kPasses][16];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRows + lane / kLanes;
+      float a[8], b[8];
+      unpack8(lo[i], a);
+      unpack8(hi[i], b);
+      if (turned && r < it.count) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float co = s_cos[r][d0 + e], si = s_sin[r][d0 + e];
+          x[i][e] = __fsub_rn(__fmul_rn(a[e], co), __fmul_rn(b[e], si));
+          x[i][8 + e] = __fadd_rn(__fmul_rn(b[e], co), __fmul_rn(a[e], si));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[i][e] = a[e];
+          x[i][8 + e] = b[e];
+        }
+      }
+    }
+    if (is_q || TYPE == kBinary16) {
+      __half* dst;
+      size_t step;   // from a token to the next
+      if (is_q) {
+        dst = p.q_out + ((size_t)it.row * p.Hq + head) * D;
+        step = (size_t)p.Hq * D;
+      } else {
+        dst = static_cast<__half*>(turned ? p.k : p.v) + (((size_t)page * p.page_tokens + slot) * p.Hkv + kvh) * D;
+        step = (size_t)p.Hkv * D;
+      }
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kRows + lane / kLanes;
+        if (r < it.count) {
+          *reinterpret_cast<uint4*>(dst + r * step + d0) = pack8(x[i]);
+          *reinterpret_cast<uint4*>(dst + r * step + d0 + kHalf) = pack8(x[i] + 8);
+        }
+      }
+      continue;
+    }
+    // 8-bit pages
+    float top = 0.0f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        // a value that is not finite has no code: it is stored as 0 and reported
+        if (!(fabsf(x[i][e]) <= 3.4028234664e38f)) {
+          x[i][e] = 0.0f;
+          odd = true;
+        }
+        top = fmaxf(top, fabsf(x[i][e]));
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (odd && p.dev_err) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
+    constexpr int kCode = TYPE == q8::kE4m3 ? q8::kE4m3 : q8::kInt8;
+    const int kept = it.pos % kBlock;         // rows of the block that were there before
+    const size_t run = (size_t)page * p.Hkv + kvh;
+    float* scale_at = (turned ? p.k_scales : p.v_scales) + run * (p.page_tokens / kBlock) + slot / kBlock;
+    uint8_t* rows = static_cast<uint8_t*>(turned ? p.k : p.v) + (run * p.page_tokens + (slot - kept)) * D;
+    const float s_kept = kept ? *scale_at : 0.0f;
+    const float s = fmaxf(s_kept, q8::scale_for<kCode>(top));
+    const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+    if (kept && s > s_kept) {
+      const float ratio = __fdiv_rn(s_kept, s);
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kRows + lane / kLanes;
+        if (r < kept) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint2* at = reinterpret_cast<uint2*>(rows + r * D + d0 + h * kHalf);
+            uint2 w = *at;
+            float v[8];
+            q8::codes_to_float4<kCode>(w.x, v);
+            q8::codes_to_float4<kCode>(w.y, v + 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= ratio;
+            *at = make_uint2(q8::float4_to_codes<kCode>(v), q8::float4_to_codes<kCode>(v + 4));
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRows + lane / kLanes;
+      if (r < it.count) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[i][e] *= inv;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<uint2*>(rows + (kept + r) * D + d0 + h * kHalf) =
+              make_uint2(q8::float4_to_codes<kCode>(x[i] + 8 * h), q8::float4_to_codes<kCode>(x[i] + 8 * h + 4));
+      }
+    }
+    if (lane == 0) *scale_at = s;
+  }
+}
+
+// values[page][head][token][:] = fp16(code * scale), K's pool then V's: a thread
+// takes 16 codes of a row.
+template <int TYPE>
+__global__ void __launch_bounds__(256) values_kernel(const uint8_t* k, const uint8_t* v, const float* ks,
+                                                     const float* vs, __half* ko, __half* vo, long long chunks,
+                                                     int chunks_per_block) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < 2 * chunks;
+       i += (long long)gridDim.x * blockDim.x) {
+    const bool second = i >= chunks;
+    const long long c = second ? i - chunks : i;
+    const uint4 w = reinterpret_cast<const uint4*>(second ? v : k)[c];
+    const float s = (second ? vs : ks)[c / chunks_per_block];
+    float f[16];
+    q8::codes_to_float4<TYPE>(w.x, f);
+    q8::codes_to_float4<TYPE>(w.y, f + 4);
+    q8::codes_to_float4<TYPE>(w.z, f + 8);
+    q8::codes_to_float4<TYPE>(w.w, f + 12);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) f[e] *= s;
+    uint4* out = reinterpret_cast<uint4*>(second ? vo : ko) + 2 * c;
+    out[0] = pack8(f);
+    out[1] = pack8(f + 8);
+  }
+}
+
+static bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename... KArgs, typename... Args>
+static int launch(void (*kernel)(KArgs...), dim3 grid, int threads, cudaStream_t s, unsigned flags, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = (flags & ANVILQ_GEMM_OVERLAP_PRIOR) ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    cudaGetLastError();
+    return ANVILQ_ECUDA;
+  }
+  return ANVILQ_OK;
+}
+
+// type: kBinary16 or an ANVILQ_KV_Q8_* code type (scales then given)
+static int run(const uint16_t* qkv, long long stride, const int32_t* starts, const int32_t* seqlens,
+               const uint32_t* page_table, uint16_t* q_out, void* k, void* v, float* k_scales, float* v_scales,
+               int type, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages, int num_pages,
+               float theta, int* dev_err, unsigned flags, cudaStream_t st) {
+  if (!qkv || !starts || !seqlens || !page_table || !q_out || !k || !v || !dev_err) return ANVILQ_EINVAL;
+  if (type != kBinary16 && (!k_scales || !v_scales)) return ANVILQ_EINVAL;
+  if (flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) return ANVILQ_EINVAL;
+  if (T < 0 || B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || !(theta > 0.0f) || !std::isfinite(theta))
+    return ANVILQ_EINVAL;
+  if (type != kBinary16 && type != q8::kInt8 && type != q8::kE4m3) return ANVILQ_EINVAL;
+  if ((D != 64 && D != 128) || page_tokens < kBlock || page_tokens % kBlock || max_pages < 1 || num_pages < 1 ||
+      (long long)page_tokens * max_pages > (1LL << 30) || B > (1 << 24) || Hq > (1 << 16) || T > (1 << 30))
+    return ANVILQ_ESHAPE;
+  const int heads = Hq + 2 * Hkv;
+  if (stride < (long long)heads * D) return ANVILQ_EINVAL;
+  if (!a16(qkv) || !a16(q_out) || !a16(k) || !a16(v) || stride % 8) return ANVILQ_EALIGN;
+  if (T == 0) return ANVILQ_OK;
+  Params p{};
+  p.qkv = reinterpret_cast<const __half*>(qkv);
+  p.stride = stride;
+  p.starts = starts;
+  p.seqlens = seqlens;
+  p.page_table = page_table;
+  p.q_out = reinterpret_cast<__half*>(q_out);
+  p.k = k;
+  p.v = v;
+  p.k_scales = k_scales;
+  p.v_scales = v_scales;
+  p.dev_err = dev_err;
+  p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
+  p.page_tokens = page_tokens; p.max_pages = max_pages; p.num_pages = num_pages;
+  const long long by_place = T / kBlock + 2LL * B;
+  p.by_token = T <= by_place;
+  const int items = (int)(p.by_token ? (long long)T : by_place);
+  p.heads_per_cta = heads;
+  Freq freq;
+  for (int i = 0; i < D / 2; ++i) freq.inv[i] = std::pow((double)theta, -2.0 * i / D);
+  const dim3 grid(items, (heads + p.heads_per_cta - 1) / p.heads_per_cta);
+  auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, st, flags, p, freq); };
+  if (D == 64)
+    return type == kBinary16 ? go(append_kernel<64, kBinary16>)
+           : type == q8::kInt8 ? go(append_kernel<64, q8::kInt8>) : go(append_kernel<64, q8::kE4m3>);
+  return type == kBinary16 ? go(append_kernel<128, kBinary16>)
+         : type == q8::kInt8 ? go(append_kernel<128, q8::kInt8>) : go(append_kernel<128, q8::kE4m3>);
+}
+
+}  // namespace append
+}  // namespace anvilq
+
+extern "C" {
+
+int anvilq_paged_kv_append(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
+                           const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, uint16_t* k_pool,
+                           uint16_t* v_pool, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages,
+                           int num_pages, float theta, int* dev_err, unsigned flags, anvilq_stream_t stream) {
+  using namespace anvilq::append;
+  return run(qkv, qkv_stride, token_starts, seqlens, page_table, q_out, k_pool, v_pool, nullptr, nullptr, kBinary16,
+             T, B, Hq, Hkv, D, page_tokens, max_pages, num_pages, theta, dev_err, flags,
+             reinterpret_cast<cudaStream_t>(stream));
+}
+
+int anvilq_paged_kv_append_q8(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
+                              const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, void* k_codes,
+                              void* v_codes, float* k_scales, float* v_scales, int code_type, int T, int B, int Hq,
+                              int Hkv, int D, int page_tokens, int max_pages, int num_pages, float theta,
+                              int* dev_err, unsigned flags, anvilq_stream_t stream) {
+  using namespace anvilq::append;
+  if (code_type != ANVILQ_KV_Q8_INT8 && code_type != ANVILQ_KV_Q8_E4M3) return ANVILQ_EINVAL;
+  return run(qkv, qkv_stride, token_starts, seqlens, page_table, q_out, k_codes, v_codes, k_scales, v_scales,
+             code_type, T, B, Hq, Hkv, D, page_tokens, max_pages, num_pages, theta, dev_err, flags,
+             reinterpret_cast<cudaStream_t>(stream));
+}
+
+int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales,
+                        int code_type, uint16_t* k_out, uint16_t* v_out, int num_pages, int Hkv, int page_tokens,
+                        int D, unsigned flags, anvilq_stream_t stream) {
+  using namespace anvilq::append;
+  if (!k_codes || !v_codes || !k_scales || !v_scales || !k_out || !v_out) return ANVILQ_EINVAL;
+  if (code_type != ANVILQ_KV_Q8_INT8 && code_type != ANVILQ_KV_Q8_E4M3) return ANVILQ_EINVAL;
+  if (flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) return ANVILQ_EINVAL;
+  if (num_pages < 1 || Hkv < 1) return ANVILQ_EINVAL;
+  if ((D != 64 && D != 128) || page_tokens < kBlock || page_tokens % kBlock) return ANVILQ_ESHAPE;
+  if (!a16(k_codes) || !a16(v_codes) || !a16(k_out) || !a16(v_out)) return ANVILQ_EALIGN;
+  const long long chunks = (long long)num_pages * Hkv * page_tokens * (D / 16);
+  const int blocks = (int)std::min<long long>((2 * chunks + 255) / 256, 148 * 16);
+  auto go = [&](auto kernel) {
+    return launch(kernel, dim3(blocks), 256, reinterpret_cast<cudaStream_t>(stream), flags,
+                  static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes), k_scales, v_scales,
+                  reinterpret_cast<__half*>(k_out), reinterpret_cast<__half*>(v_out), chunks, kBlock * D / 16);
+  };
+  return code_type == ANVILQ_KV_Q8_INT8 ? go(values_kernel<ANVILQ_KV_Q8_INT8>) : go(values_kernel<ANVILQ_KV_Q8_E4M3>);
+}
+
+}  // extern "C"

@@ -16,6 +16,7 @@ from . import _lib
 _state = threading.local()
 _dev_err = {}          # device index -> int32[1] device error word
 _workspaces = {}       # (device index, stream ptr) -> uint8 workspace
+_outgrown = []         # workspaces that larger ones replaced: captured graphs may still use them
 _lock = threading.Lock()
 
 
@@ -76,6 +77,8 @@ def workspace(device, nbytes: int) -> torch.Tensor:
     with _lock:
         ws = _workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
+            if ws is not None:
+                _outgrown.append(ws)
             ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
             _workspaces[key] = ws
     return ws
@@ -581,3 +584,307 @@ def gqa_decode_int8(q, k_codes, k_meta, v_codes, v_meta, seqlens, k_escape=None,
                                           Tmax, float(scale), _ptr(ws), ws.numel(), _ptr(err),
                                           _stream_ptr(q.device)), "anvilq_gqa_decode_int8")
     return out
+
+
+# ---- a serving batch over a paged cache ------------------------------------------
+
+def _on_device(name, device, *tensors):
+    """Every given tensor (None: skipped) is on `device`, a CUDA device."""
+    if device.type != "cuda":
+        raise ValueError(f"{name}: tensors must be on a CUDA device")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: all tensors must be on {device}")
+
+
+def _call(name, device, *args):
+    """A library call with `device` current (a stream only takes launches of its own device)."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == device.index:
+        _lib.check(fn(*args), name)
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args), name)
+
+
+def _call_workspace(device, nbytes: int, given) -> torch.Tensor:
+    """The call's workspace: the caller's, else the current stream's.  While a
+    graph is captured it is a fresh one whose counters the graph zeroes before
+    the call, so that no two graphs share one and replays may overlap."""
+    if given is not None:
+        if given.dtype != torch.uint8 or given.device != device or given.numel() < nbytes or \
+                not given.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {nbytes} bytes on {device}")
+        return given
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:WORKSPACE_COUNTER_BYTES].zero_()
+        return ws
+    return workspace(device, nbytes)
+
+
+WORKSPACE_COUNTER_BYTES = 65536
+
+
+def _error_word(device, given):
+    """The call's device error word: the caller's, else the device's.  The first one
+    of a device must not come from a graph's memory."""
+    if given is not None:
+        if given.dtype != torch.int32 or given.numel() < 1 or given.device != device:
+            raise ValueError(f"dev_err must be an int32 tensor on {device}")
+        return given
+    if device.index not in _dev_err and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("run an operation on this device once before capturing a graph")
+    return device_error_word(device)
+
+
+def _check_table(name, page_table, seqlens, B=None):
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+        raise ValueError(f"{name}: page_table must be a contiguous int32 tensor [B, max_pages]")
+    B = page_table.shape[0] if B is None else B
+    if page_table.shape[0] != B:
+        raise ValueError(f"{name}: page_table has {page_table.shape[0]} rows for {B} sequences")
+    if seqlens.dtype != torch.int32 or tuple(seqlens.shape) != (B,) or not seqlens.is_contiguous():
+        raise ValueError(f"{name}: seqlens must be a contiguous int32 tensor [{B}]")
+    return B, page_table.shape[1]
+
+
+def _check_q8(name, k_codes, v_codes, k_scales, v_scales):
+    """(pages, heads, page tokens, D, code type) of a pair of 8-bit pools."""
+    if k_codes.dtype not in (torch.int8, torch.float8_e4m3fn) or v_codes.dtype != k_codes.dtype:
+        raise TypeError(f"{name}: codes must both be int8 or both float8_e4m3fn")
+    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
+        raise ValueError(f"{name}: k_codes/v_codes [num_pages, Hkv, page_tokens, D]")
+    pages, Hkv, page, D = k_codes.shape
+    if page % _lib.KV_Q8_BLOCK:
+        raise ValueError(f"{name}: pages must hold a multiple of {_lib.KV_Q8_BLOCK} tokens")
+    for t in (k_scales, v_scales):
+        if t.dtype != torch.float32 or tuple(t.shape) != (pages, Hkv, page // _lib.KV_Q8_BLOCK):
+            raise ValueError(f"{name}: scales must be float32 [{pages}, {Hkv}, {page // _lib.KV_Q8_BLOCK}]")
+    for t in (k_codes, v_codes, k_scales, v_scales):
+        if not t.is_contiguous():
+            raise ValueError(f"{name}: pools must be contiguous")
+    _on_device(name, k_codes.device, v_codes, k_scales, v_scales)
+    return pages, Hkv, page, D, _lib.KV_Q8_INT8 if k_codes.dtype == torch.int8 else _lib.KV_Q8_E4M3
+
+
+def _check_append(name, qkv, Hq, Hkv, D, page_table, seqlens, token_starts, q_out):
+    B, max_pages = _check_table(name, page_table, seqlens)
+    if qkv.dtype != torch.float16 or qkv.dim() != 2 or qkv.shape[1] != (Hq + 2 * Hkv) * D:
+        raise ValueError(f"{name}: qkv must be float16 [T, {(Hq + 2 * Hkv) * D}]")
+    if qkv.stride(1) != 1 or (qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]):
+        raise ValueError(f"{name}: rows of qkv must be contiguous and must not overlap")
+    if token_starts.dtype != torch.int32 or tuple(token_starts.shape) != (B + 1,) or not token_starts.is_contiguous():
+        raise ValueError(f"{name}: token_starts must be a contiguous int32 tensor [{B + 1}]")
+    T = qkv.shape[0]
+    if q_out is None:
+        q_out = torch.empty((T, Hq, D), dtype=torch.float16, device=qkv.device)
+    elif q_out.dtype != torch.float16 or tuple(q_out.shape) != (T, Hq, D) or not q_out.is_contiguous():
+        raise ValueError(f"{name}: q_out must be contiguous float16 [{T}, {Hq}, {D}]")
+    _on_device(name, qkv.device, page_table, seqlens, token_starts, q_out)
+    return T, B, max_pages, (qkv.stride(0) if T > 1 else qkv.shape[1]), q_out
+
+
+def paged_kv_append(qkv, k_pool, v_pool, page_table, seqlens, token_starts, Hq: int, theta: float = 1e6, q_out=None,
+                    dev_err=None, overlap_prior: bool = False):
+    """Append the new tokens of a ragged batch to a paged fp16 cache, rotating q and
+    k on the way.  qkv fp16 [T, (Hq + 2 Hkv) D] (rows may be strided) holds the new
+    tokens' [q | k | v] rows, sequence after sequence: those of sequence b are rows
+    token_starts[b] .. token_starts[b + 1] (int32 [B + 1]) and its last ones, seqlens
+    (int32 [B]) counting them already.  Pools and page_table as for
+    ``gqa_decode_paged``, written in place.  Returns the rotated q, fp16 [T, Hq, D]
+    (rows of no sequence are left as they are).
+
+    The rotation and cache write of FP32Model.token (anvil-q1/tests/official_weights.py:439-449,
+    466-470) for many tokens, over the Anvil-Q4 page table (anvil-q4/design/SPEC.md:205-208);
+    one token of one sequence gives bit for bit what ``anvilq_rope_kv_append`` gives."""
+    name = "paged_kv_append"
+    if k_pool.dtype != torch.float16 or v_pool.dtype != torch.float16:
+        raise TypeError(f"{name}: the KV pools must be float16")
+    if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or not k_pool.is_contiguous() or not v_pool.is_contiguous():
+        raise ValueError(f"{name}: k_pool/v_pool must be contiguous [num_pages, page_tokens, Hkv, D]")
+    pages, page, Hkv, D = k_pool.shape
+    T, B, max_pages, stride, q_out = _check_append(name, qkv, Hq, Hkv, D, page_table, seqlens, token_starts, q_out)
+    dev = qkv.device
+    _on_device(name, dev, k_pool, v_pool)
+    err = _error_word(dev, dev_err)
+    _call("anvilq_paged_kv_append", dev, _ptr(qkv), stride, _ptr(token_starts), _ptr(seqlens), _ptr(page_table),
+          _ptr(q_out), _ptr(k_pool), _ptr(v_pool), T, B, Hq, Hkv, D, page, max_pages, pages, float(theta), _ptr(err),
+          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    return q_out
+
+
+def paged_kv_append_q8(qkv, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, token_starts, Hq: int,
+                       theta: float = 1e6, q_out=None, dev_err=None, overlap_prior: bool = False):
+    """``paged_kv_append`` into 8-bit pages: codes int8 or float8_e4m3fn
+    [num_pages, Hkv, page_tokens, D], scales float32 [num_pages, Hkv, page_tokens / 16],
+    one for each block of 16 tokens and head, all written in place.  A block's scale
+    fits its largest value; when a later token of the block needs a larger one, the
+    block's earlier codes are rounded again to it (anvilq_paged_kv_append_q8 in
+    include/anvilq.h has the formulas).  Values that are not finite set a device error
+    and are stored as 0."""
+    name = "paged_kv_append_q8"
+    pages, Hkv, page, D, code = _check_q8(name, k_codes, v_codes, k_scales, v_scales)
+    T, B, max_pages, stride, q_out = _check_append(name, qkv, Hq, Hkv, D, page_table, seqlens, token_starts, q_out)
+    dev = qkv.device
+    _on_device(name, dev, k_codes)
+    err = _error_word(dev, dev_err)
+    _call("anvilq_paged_kv_append_q8", dev, _ptr(qkv), stride, _ptr(token_starts), _ptr(seqlens), _ptr(page_table),
+          _ptr(q_out), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), code, T, B, Hq, Hkv, D, page,
+          max_pages, pages, float(theta), _ptr(err), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    return q_out
+
+
+def kv_q8_values(k_codes, v_codes, k_scales, v_scales, k_out=None, v_out=None, overlap_prior: bool = False):
+    """The values of whole 8-bit pools, fp16(code * scale), in two fp16 tensors of the codes' shape."""
+    name = "kv_q8_values"
+    pages, Hkv, page, D, code = _check_q8(name, k_codes, v_codes, k_scales, v_scales)
+    dev = k_codes.device
+    k_out = torch.empty(k_codes.shape, dtype=torch.float16, device=dev) if k_out is None else k_out
+    v_out = torch.empty(k_codes.shape, dtype=torch.float16, device=dev) if v_out is None else v_out
+    for t in (k_out, v_out):
+        if t.dtype != torch.float16 or t.shape != k_codes.shape or not t.is_contiguous():
+            raise ValueError(f"{name}: k_out/v_out must be contiguous float16 with the shape of the codes")
+    _on_device(name, dev, k_out, v_out)
+    _call("anvilq_kv_q8_values", dev, _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), code, _ptr(k_out),
+          _ptr(v_out), pages, Hkv, page, D, GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    return k_out, v_out
+
+
+def gqa_decode_q8(q, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, scale: float = 0.0, out=None,
+                  dev_err=None, workspace=None, overlap_prior: bool = False):
+    """GQA attention over 8-bit pages (``paged_kv_append_q8``'s): q fp16 [B, Hq, D], one
+    query token a sequence, or [B, Q, Hq, D], its last Q tokens (drafts to verify, a
+    chunk), each seeing the positions up to its own.  seqlens int32 [B] counts all
+    tokens, the queries' included; a sequence of length 0 gives zeros.  Returns fp16
+    in q's shape.  workspace: a uint8 tensor zero-filled once, for callers that keep
+    their own (default: the current stream's).
+
+    attention(q, keys, values) of anvil-q1-fp/tests/fp64_reference.py:164-170, batched."""
+    name = "gqa_decode_q8"
+    if q.dtype != torch.float16 or q.dim() not in (3, 4) or not q.is_contiguous():
+        raise ValueError(f"{name}: q must be contiguous float16 [B, Hq, D] or [B, Q, Hq, D]")
+    B, Hq, D = q.shape[0], q.shape[-2], q.shape[-1]
+    Q = q.shape[1] if q.dim() == 4 else 1
+    pages, Hkv, page, Dk, code = _check_q8(name, k_codes, v_codes, k_scales, v_scales)
+    if Dk != D:
+        raise ValueError(f"{name}: head_dim of q and the pools differ")
+    _, max_pages = _check_table(name, page_table, seqlens, B)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.dtype != torch.float16 or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError(f"{name}: out must be contiguous float16 in q's shape")
+    dev = q.device
+    _on_device(name, dev, k_codes, page_table, seqlens, out)
+    need = _lib.load().anvilq_gqa_decode_q8_workspace_size(B, Q, Hq, Hkv, D)
+    if need == 0:
+        raise ValueError(f"{name}: unsupported shape B={B} Q={Q} Hq={Hq} Hkv={Hkv} D={D}")
+    ws = _call_workspace(dev, need, workspace)
+    err = _error_word(dev, dev_err)
+    _call("anvilq_gqa_decode_q8", dev, _ptr(q), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), code,
+          _ptr(page_table), _ptr(seqlens), _ptr(out), B, Q, Hq, Hkv, D, page, max_pages, pages, float(scale), _ptr(ws),
+          ws.numel(), _ptr(err), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    return out
+
+
+def logits_process(logits, history=None, history_lens=None, prompt_lens=None, repetition=None, presence=None,
+                   frequency=None, bias_starts=None, bias_ids=None, bias_values=None, allowed=None, allowed_rows=None,
+                   out=None, write_logits: bool = True, choose: bool = True, dev_err=None, workspace=None,
+                   overlap_prior: bool = False):
+    """Penalties for repeated tokens, biases and grammar masks on logits [B, V] (fp32
+    or fp16, rows may be strided), and the greedy choice.  Returns (out fp32 [B, V],
+    tokens int32 [B]); None in the place of what write_logits / choose leave out.
+    out may be the fp32 logits themselves.
+
+    history int32 [B, L] (prompt, then generated tokens), history_lens int32 [B],
+    prompt_lens int32 [B]: repetition (fp32 [B]) divides or multiplies the logit of
+    every token in the history, frequency and presence (fp32 [B]) are taken off for
+    the generated ones.  bias_starts int32 [B + 1], bias_ids int32 [n], bias_values
+    fp32 [n]: each row's list of additions (an id's last entry counts).  allowed
+    int32 [masks, ceil(V / 32)]: bit v % 32 of word v / 32 allows token v; row b uses
+    mask allowed_rows[b] (int32 [B]; negative: none), or b.  A token of -1 says that
+    its row had nothing to choose from.
+
+    The choice is the reference's greedy one, lowest index on ties
+    (anvil-q4/tests/transformer_reference.py:212-217)."""
+    name = "logits_process"
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.float16):
+        raise ValueError(f"{name}: logits must be float32 or float16 [B, V]")
+    B, V = logits.shape
+    if B < 1 or V < 1 or logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
+        raise ValueError(f"{name}: rows of logits must be contiguous and must not overlap")
+    if not write_logits and not choose:
+        raise ValueError(f"{name}: nothing to compute")
+
+    def rows(t, dtype, what, n=B):
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous()):
+            raise ValueError(f"{name}: {what} must be contiguous {dtype} [{n}]")
+
+    L = 0
+    if history is not None:
+        if history.dtype != torch.int32 or history.dim() != 2 or history.shape[0] != B or \
+                (history.shape[1] > 1 and history.stride(1) != 1):
+            raise ValueError(f"{name}: history must be int32 [{B}, L] with contiguous rows")
+        if history_lens is None:
+            raise ValueError(f"{name}: history needs history_lens")
+        L = history.shape[1]
+        if B > 1 and history.stride(0) < L:
+            raise ValueError(f"{name}: rows of history must not overlap")
+    elif any(t is not None for t in (history_lens, prompt_lens, repetition, presence, frequency)):
+        raise ValueError(f"{name}: penalties and lengths need a history")
+    rows(history_lens, torch.int32, "history_lens")
+    rows(prompt_lens, torch.int32, "prompt_lens")
+    rows(repetition, torch.float32, "repetition")
+    rows(presence, torch.float32, "presence")
+    rows(frequency, torch.float32, "frequency")
+    if L == 0:
+        history = None       # no tokens: nothing to penalise
+        history_lens = prompt_lens = repetition = presence = frequency = None
+    n_bias = 0
+    if bias_starts is not None:
+        if bias_ids is None or bias_values is None:
+            raise ValueError(f"{name}: bias_starts needs bias_ids and bias_values")
+        n_bias = bias_ids.numel()
+        rows(bias_starts, torch.int32, "bias_starts", B + 1)
+        rows(bias_ids, torch.int32, "bias_ids", n_bias)
+        rows(bias_values, torch.float32, "bias_values", n_bias)
+    elif bias_ids is not None or bias_values is not None:
+        raise ValueError(f"{name}: a bias list needs bias_starts")
+    masks = 0
+    if allowed is not None:
+        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[1] < (V + 31) // 32 or \
+                (allowed.shape[1] > 1 and allowed.stride(1) != 1):
+            raise ValueError(f"{name}: allowed must be int32 [masks, {(V + 31) // 32}] with contiguous rows")
+        masks = allowed.shape[0]
+        if masks > 1 and allowed.stride(0) < (V + 31) // 32:
+            raise ValueError(f"{name}: rows of allowed must not overlap")
+        if allowed_rows is None and masks != B:
+            raise ValueError(f"{name}: one mask a row, or allowed_rows")
+        rows(allowed_rows, torch.int32, "allowed_rows")
+    elif allowed_rows is not None:
+        raise ValueError(f"{name}: allowed_rows needs allowed")
+    dev = logits.device
+    if not write_logits:
+        if out is not None:
+            raise ValueError(f"{name}: out is not written without write_logits")
+    elif out is None:
+        out = torch.empty((B, V), dtype=torch.float32, device=dev)
+    elif out.dtype != torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or \
+            (B > 1 and out.stride(0) < V):
+        raise ValueError(f"{name}: out must be float32 [{B}, {V}] with contiguous rows")
+    tokens = torch.empty(B, dtype=torch.int32, device=dev) if choose else None
+    _on_device(name, dev, history, history_lens, prompt_lens, repetition, presence, frequency, bias_starts, bias_ids,
+               bias_values, allowed, allowed_rows, out)
+    need = _lib.load().anvilq_logits_process_workspace_size(B, V)
+    if need == 0:
+        raise ValueError(f"{name}: unsupported shape B={B} V={V}")
+    ws = _call_workspace(dev, need, workspace) if choose else None
+    err = _error_word(dev, dev_err)
+    pitch = lambda t, n: 0 if t is None else t.stride(0) if t.shape[0] > 1 else n
+    _call("anvilq_logits_process", dev, _ptr(logits), 1 if logits.dtype == torch.float16 else 0, pitch(logits, V),
+          _ptr(out), pitch(out, V), _ptr(tokens), B, V, _ptr(history), pitch(history, L), _ptr(history_lens),
+          _ptr(prompt_lens), L, _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_starts), _ptr(bias_ids),
+          _ptr(bias_values), n_bias, _ptr(allowed), pitch(allowed, (V + 31) // 32), _ptr(allowed_rows), masks,
+          _ptr(ws), 0 if ws is None else ws.numel(), _ptr(err), GEMM_OVERLAP_PRIOR if overlap_prior else 0,
+          _stream_ptr(dev))
+    return out, tokens

@@ -624,6 +624,121 @@ int anvilq_gqa_decode_paged(const uint16_t* q, const uint16_t* k_pool, const uin
                             int D, int page_tokens, int max_pages, int num_pages, float scale, void* workspace,
                             size_t workspace_bytes, int* dev_err, anvilq_stream_t stream);
 
+/* ---- a serving batch over a paged cache ---------------------------------------
+ *
+ * One step of a ragged batch: the new tokens' rows are rotated and appended to
+ * the pages, attention reads the pages, the logits get their penalties and
+ * masks.  No counterpart function in the reference, whose token() takes one
+ * token of one sequence (official_weights.py:451-509): rotation :439-449, cache
+ * write :470, attention :471-486, and the Q4 page table
+ * (anvil-q4/design/SPEC.md:205-208).
+ * flags of every call here: ANVILQ_GEMM_OVERLAP_PRIOR.
+ *
+ * 8-bit pages.  A block of 16 tokens of a page and a kv head share one scale,
+ * value = code * scale, and a head's rows of a page lie together:
+ *   codes   int8 or e4m3  [num_pages][Hkv][page_tokens][D]
+ *   scales  float         [num_pages][Hkv][page_tokens / 16]
+ * page_tokens % 16 == 0, D in {64, 128}. */
+#define ANVILQ_KV_Q8_BLOCK 16
+#define ANVILQ_KV_Q8_INT8 0   /* codes -127 .. 127 */
+#define ANVILQ_KV_Q8_E4M3 1   /* 8-bit floats: 4 exponent, 3 fraction bits, largest 448 */
+
+/* Appends the new tokens of B sequences to binary16 pages.  Row t of
+ * qkv (fp16 [T] rows of (Hq + 2 Hkv) * D = [q | k | v], qkv_stride elements
+ * apart) is a new token of the sequence b with token_starts[b] <= t <
+ * token_starts[b + 1] (device int32 [B + 1], non-decreasing, first >= 0, last
+ * <= T; rows outside are neither read nor written); sequence b holds
+ * seqlens[b] tokens with the new ones, which are its last.  Every q and k head
+ * is rotated to its token's position exactly as by anvilq_rope_kv_append; q
+ * goes to q_out fp16 [T][Hq][D], k and v to row position % page_tokens of
+ * physical page page_table[b][position / page_tokens] of the pools of
+ * anvilq_gqa_decode_paged.  No two new tokens may share a cache row.
+ * A sequence with more new tokens than seqlens[b], or longer than
+ * page_tokens * max_pages, sets ANVILQ_DEV_ERR_SEQLEN, an absent page of a new
+ * token ANVILQ_DEV_ERR_PAGE; nothing is then written for it (for that page).
+ * D in {64, 128}, page_tokens % 16 == 0, qkv_stride % 8 == 0, 16-byte aligned
+ * qkv, q_out and pools; dev_err required; T == 0 does nothing. */
+int anvilq_paged_kv_append(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
+                           const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, uint16_t* k_pool,
+                           uint16_t* v_pool, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages,
+                           int num_pages, float theta, int* dev_err, unsigned flags, anvilq_stream_t stream);
+
+/* The same into 8-bit pages.  The block's scale becomes
+ *   s = max(s_kept, top / 127)                                    (int8)
+ *   s = max(s_kept, the smallest power of two with top <= 448 s)  (e4m3)
+ * with top the largest magnitude among the block's new rows (before any
+ * rounding to binary16) and s_kept its scale so far, 0 when the block's first
+ * row is among the new ones; new rows are stored as round(value * fp32(1 / s)),
+ * and where s > s_kept the block's earlier rows become
+ * round(code * fp32(s_kept / s)) -- so one int8 code is off by at most half a
+ * step of every scale its block has had.  Rows behind the new ones keep their
+ * codes.  A value that is not finite sets ANVILQ_DEV_ERR_NONFINITE and is
+ * stored as 0.  Two sequences must not append to the same page in one call. */
+int anvilq_paged_kv_append_q8(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
+                              const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, void* k_codes,
+                              void* v_codes, float* k_scales, float* v_scales, int code_type, int T, int B, int Hq,
+                              int Hkv, int D, int page_tokens, int max_pages, int num_pages, float theta,
+                              int* dev_err, unsigned flags, anvilq_stream_t stream);
+
+/* The values of whole 8-bit pools in binary16: out[page][head][token][d] =
+ * fp16(code * scale), same layout as the codes (to move pages into binary16, or
+ * to look at them).  16-byte aligned codes and outputs. */
+int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales,
+                        int code_type, uint16_t* k_out, uint16_t* v_out, int num_pages, int Hkv, int page_tokens,
+                        int D, unsigned flags, anvilq_stream_t stream);
+
+/* Attention of Q query tokens a sequence over 8-bit pages: query i of sequence
+ * b is its token at position seqlens[b] - Q + i and sees every position up to
+ * its own (Q = 1: the decode step; more: drafted tokens or a chunk, appended
+ * before).  q and out fp16 [B][Q][Hq][D], seqlens int32 [B] (device, 0 ..
+ * page_tokens * max_pages).  A query that sees nothing -- an empty sequence, or
+ * a position below 0 -- gives zeros.  Scores and the softmax run in fp32, the
+ * probabilities enter the tensor cores as binary16.  scale <= 0 selects
+ * 1/sqrt(D).  Hq % Hkv == 0, Hq <= 1024, Q <= 64, B <= 65535; 16-byte aligned
+ * q, codes and out; dev_err required.  A length outside its range sets
+ * ANVILQ_DEV_ERR_SEQLEN and counts as 0; an absent live page sets
+ * ANVILQ_DEV_ERR_PAGE (the output is then not to be used).  workspace: at least
+ * anvilq_gqa_decode_q8_workspace_size(...) bytes (0: shape not supported),
+ * layout as described at ANVILQ_WORKSPACE_COUNTER_BYTES. */
+size_t anvilq_gqa_decode_q8_workspace_size(int B, int Q, int Hq, int Hkv, int D);
+int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_codes, const float* k_scales,
+                         const float* v_scales, int code_type, const uint32_t* page_table, const int32_t* seqlens,
+                         uint16_t* out, int B, int Q, int Hq, int Hkv, int D, int page_tokens, int max_pages,
+                         int num_pages, float scale, void* workspace, size_t workspace_bytes, int* dev_err,
+                         unsigned flags, anvilq_stream_t stream);
+
+/* Penalties, biases and grammar masks on B rows of V logits (fp32, or fp16 with
+ * logits_half; logits_stride elements apart), and the greedy choice.  For token
+ * v of row b, in fp32, each operation rounded:
+ *   v in history[b][0 .. history_lens[b]):  l = l > 0 ? l / repetition[b] : l * repetition[b]
+ *   n > 0 occurrences from prompt_lens[b] on (NULL: from 0):
+ *                                           l = (l - frequency[b] * n) - presence[b]
+ *   v in the row's bias list, entries bias_starts[b] .. bias_starts[b + 1] of
+ *   bias_ids / bias_values (of bias_total):  l = l + the value of v's LAST entry
+ *   bit v % 32 of word v / 32 of its mask clear:  l = -inf
+ * out (fp32, out_stride apart; may be the fp32 logits themselves) = l; token[b] =
+ * the lowest v with the largest l > -inf, NaN never chosen, -1 when there is
+ * none.  Either of out and token may be NULL.
+ * history int32 rows of up to L tokens, history_stride apart; penalties fp32
+ * [B], each may be NULL (none); history, bias_starts, allowed may be NULL.
+ * allowed: `masks` rows of words, allowed_stride apart; row b uses mask
+ * allowed_rows[b] (negative: all allowed), or b when allowed_rows is NULL.
+ * A token id outside [0, V) sets ANVILQ_DEV_ERR_TOKEN and is ignored; a
+ * history length outside [0, L], a bias range outside its list (an empty one is
+ * used) or a mask row >= masks (none is used) sets ANVILQ_DEV_ERR_SEQLEN.
+ * B <= 4096; dev_err required; workspace (needed for token):
+ * anvilq_logits_process_workspace_size bytes, 16-byte aligned, layout as
+ * described at ANVILQ_WORKSPACE_COUNTER_BYTES. */
+size_t anvilq_logits_process_workspace_size(int B, int V);
+int anvilq_logits_process(const void* logits, int logits_half, long long logits_stride, float* out,
+                          long long out_stride, int32_t* token, int B, int V, const int32_t* history,
+                          long long history_stride, const int32_t* history_lens, const int32_t* prompt_lens, int L,
+                          const float* repetition, const float* presence, const float* frequency,
+                          const int32_t* bias_starts, const int32_t* bias_ids, const float* bias_values,
+                          int bias_total, const uint32_t* allowed, long long allowed_stride,
+                          const int32_t* allowed_rows, int masks, void* workspace, size_t workspace_bytes,
+                          int* dev_err, unsigned flags, anvilq_stream_t stream);
+
 /* ---- tree attention of speculative draft nodes -----------------------------
  *
  * Replaces the per-node causal tree attention of the batched draft-tree decoder
