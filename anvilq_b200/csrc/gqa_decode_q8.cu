@@ -9,16 +9,17 @@
 //
 // What bounds it: the codes' bytes, read once (4 Hq/Hkv Q flops a byte).
 //
-// Work split.  A tile is a block of 16 tokens of one kv head: 2 KB of K codes and
-// 2 KB of V codes at D = 128, each one contiguous run, one TMA box.  The rows of a
-// tile's products are the Q * Hq/Hkv query rows of its kv head, in groups of 8 or
-// 16 (kRows); a pair is a (sequence, kv head, row group).  All pairs' tiles in a
-// row -- sequence, then pair, then tile -- are cut into equal stretches, one a
-// warp, so that the device is evenly loaded whatever the lengths; the table of
-// lengths is on the device, so every warp finds its stretch from it.  A pair that
-// lies inside one warp's stretch is finished by that warp.  The others' partial
-// softmax states are merged in shared memory, and where a pair spans CTAs, by the
-// CTA that arrives last at the pair's ticket, in CTA order (bit-reproducible).
+// Work split.  A tile is 32 tokens of one kv head, two blocks: 4 KB of K codes and
+// 4 KB of V codes at D = 128, in runs of 2 KB at least.  The rows of a tile's
+// products are the Q * Hq/Hkv query rows of its kv head, in groups of 8 or 16
+// (kRows); a pair is a (sequence, kv head, row group).  All pairs' tiles in a row --
+// sequence, then pair, then tile -- are cut into chunks, one CTA each, and a chunk
+// into equal stretches, one a warp, so that the device is evenly loaded whatever
+// the lengths; the lengths are on the device, so every warp finds its stretch from
+// them.  A pair inside one warp's stretch is finished by that warp.  The others'
+// partial softmax states are merged in shared memory, and where a pair spans
+// chunks, by the CTA that arrives last at the pair's ticket, in chunk order
+// (bit-reproducible).  plan_of has the rules.
 //
 // A warp streams its tiles through its own TMA ring, mbarrier by mbarrier.  The
 // codes never return to memory as binary16: fragments of mma.m16n8k16 are formed
@@ -32,8 +33,10 @@
 //     fragments pair the bytes of two tokens.  Over a long context the sum of p c
 //     is far smaller than the sum of p, so here an offset would cost precision:
 //     int8 codes are made signed first, (1024 + 128 + c) - 1152 in binary16.
-// The tokens of a tile are dealt to fragment columns in an order (token_of) that
-// keeps both reads of the 128-byte-swizzled tile free of bank conflicts.
+// The tokens of a block are dealt to fragment columns in an order (token_of) that
+// keeps both reads of the 128-byte-swizzled block free of bank conflicts.  Two
+// blocks a step share the waits, votes and bookkeeping: one block a step took 480
+// instructions a block and was bound by their issue, not by memory.
 //
 // Softmax: binary32, log2 domain, online.  The running reference m is not the
 // maximum but stays within 12 of it (above: p <= 2^12; m is set 4 below a new
@@ -54,7 +57,11 @@ namespace anvilq {
 namespace attn8 {
 
 using q8::kBlock;
-constexpr int kTile = kBlock;
+constexpr int kTile = 2 * kBlock;   // tokens of a step
+constexpr int kMaxSms = 160;                  // SMs that are used
+constexpr int kMaxChunks = 9 * kMaxSms;       // chunks of a call that pairs may span (plan_of: at most 4.25 a CTA)
+constexpr int kMaxSpan = 2 * kMaxSms;         // chunks of a pair
+constexpr int kTickets = 2;                   // counters before the tickets
 constexpr unsigned long long kWaitLimitNs = 1000000000ull;
 
 struct Params {
@@ -64,10 +71,12 @@ struct Params {
   const uint32_t* page_table;  // [B][max_pages]
   const int* seqlens;          // [B]
   __half* out;                 // [B][Q][Hq][D]
-  int* tickets;                // one a CTA (of the pair that starts in it and ends in a later one)
-  float* partials;             // [CTA][2] states: of the pair begun earlier, of the pair that goes on
+  int* counters;               // next chunk, CTAs done, then a ticket a chunk (of the pair that goes on from it)
+  float* partials;             // [chunk][2] states: of the pair begun earlier, of the pair that goes on
+  float* parked;               // [CTA][warp] states
   int* dev_err;
   int B, Q, Hq, Hkv, group, row_groups, page_tokens, max_pages, num_pages;
+  int wide;                    // pages hold whole tiles: one copy of 32 rows, not two of 16
   float scale_log2;            // softmax scale * log2(e)
 };
 
@@ -76,38 +85,49 @@ template <int D_, int RT_>
 struct Shape {
   static constexpr int D = D_, RT = RT_;
   static constexpr int kRows = 8 * RT;
-  static constexpr int kWarps = RT == 1 ? 8 : 4;
+  static constexpr int kWarps = RT == 1 ? 6 : 4;               // 168 or 255 registers a thread
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kCtas = RT == 1 ? 2 : 3;                // per SM
-  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kCtas = 2;                              // per SM
   static constexpr int kTileBytes = kTile * D;                 // of K or V
   static constexpr int kStageBytes = 2 * kTileBytes;
+  // 16 KB a warp: the copies of all warps in flight are several times what the
+  // memory's latency needs; more of them only queue (half as much again ran 8 %
+  // slower, the page table, scales and q waiting behind them)
+  static constexpr int kStages = 16 * 1024 / kStageBytes;
   static constexpr int kRingBytes = kStages * kStageBytes;     // per warp
   static constexpr int kState = kRows * D;                     // floats of a state's o
-  // a warp's state of a pair begun earlier has its own room (the ring is in use
-  // when it is stored); that of a pair that goes on takes the idle ring
-  static constexpr int kStateOffset = kWarps * kRingBytes;
-  static constexpr int kStatOffset = kStateOffset + kWarps * kState * 4;   // (m, l) [warp][2][row]
+  static constexpr int kSlots = 32;                            // tiles that are described ahead, two batches
+  static constexpr int kStatOffset = kWarps * kRingBytes;      // (m, l) [warp][2][row]
   static constexpr int kMetaOffset = kStatOffset + kWarps * 2 * kRows * 8;
-  static constexpr int kBarOffset = kMetaOffset + kWarps * kStages * 32;
-  static constexpr int kTotal = kBarOffset + kWarps * kStages * 8 + 1024;  // + slack to align the ring
+  static constexpr int kBarOffset = kMetaOffset + kWarps * kSlots * 48;
+  static constexpr int kEnd = kBarOffset + kWarps * kStages * 8;
+  static constexpr int kTotal = kEnd + 1024;                   // + slack to align the rings
   static constexpr int kPartial = kState + 2 * kRows;          // floats of a state in global memory
+  static_assert((kStages & (kStages - 1)) == 0 && kStages <= 4, "a slot's old tile is used by the time it is named again");
   static_assert(kRingBytes >= kState * 4, "a state fits the idle ring");
+  static_assert(kWarps * kRingBytes >= kMaxSpan * kRows * 8, "(m, l) of every chunk of a pair fit the idle rings");
   static_assert(kCtas * (kTotal + 2048) <= 227 * 1024, "CTAs per SM");
 };
 
-struct Meta {        // what a tile's consumer needs beside the codes
-  float ks, vs;      // scales
-  int tile, n;       // tile of the pair, the pair's tiles
-  int b, pair;       // sequence, pair of the sequence
-  int pad[2];
+struct Meta {        // a tile: what its copies and its consumer need
+  float ks[2], vs[2];            // its blocks' scales
+  int tile, n;                   // tile of the pair, the pair's tiles
+  int b, pair;                   // sequence, pair of the sequence
+  int row[2];                    // blocks' first rows in the pools (as matrices of D-byte rows)
+  uint32_t word[2];              // page-table words
 };
-static_assert(sizeof(Meta) == 32, "one 32-byte slot a stage");
+static_assert(sizeof(Meta) == 48, "three 16-byte reads");
 
-struct Part {        // a warp's state of a pair that it did not finish alone
-  long long first;   // the pair's first tile in the row of all tiles
+struct Part {        // a pair that a warp did not finish alone
+  unsigned first;    // its first tile in the row of all tiles
   int n, b, pair;
-  int valid, ends;   // ends: the pair's last tile is in it
+};
+
+// How the work is cut.  Sizes in tiles; a warp's stretch of a chunk is 1 / kWarps of it.
+struct Plan {
+  bool whole;        // a chunk is a pair, whatever its length
+  unsigned total;    // tiles in all
+  unsigned first, rest;   // size of the first gridDim.x chunks, and of the others
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -127,15 +147,24 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// Bounded wait: true when the phase completed, false after ~kWaitLimitNs.
-__device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
+// The warp's bounded wait: true when the phase completed, false after ~kWaitLimitNs.
+__device__ __noinline__ bool warp_wait_long(uint32_t bar, uint32_t parity) {
   const unsigned long long t0 = globaltimer();
   for (uint32_t i = 0;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63u) == 63u && globaltimer() - t0 > kWaitLimitNs) return false;
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((i & 63u) == 63u && __any_sync(0xffffffffu, globaltimer() - t0 > kWaitLimitNs)) return false;
   }
 }
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i)
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return warp_wait_long(bar, parity);
+}
+__device__ __forceinline__ void copy4_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies4_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -146,8 +175,7 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
 // D(16x8, f32) += A(16x16, f16, row) * B(16x8, f16, col)
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -161,16 +189,42 @@ __device__ __forceinline__ float fast_exp2(float x) {   // 2^x, 2 units in the l
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t low16) {
-  uint32_t h;
-  asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(h) : "r"(low16));
-  return h;
+// four e4m3 codes as two pairs of binary16 values (exact)
+__device__ __forceinline__ void e4m3x4_to_half4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
-// The token of a tile at column n (of 16) of S: within eights, even columns keep
+// The token of a block at column n (of 16) of S: within eights, even columns keep
 // their place and odd ones are crossed, so that the two rows of a quarter-warp's
 // K read differ in bit 2 and the four rows of its V read in bits 1 and 2 -- with
 // the swizzle, 8 different 16-byte banks either way.
 __device__ __forceinline__ int token_of(int n) { return (n & 8) | ((n & 1) ? ((n & 6) ^ 5) : (n & 7)); }
+
+// Rules, each measured on a B200 (DESIGN section on this kernel has the cases):
+//   * a CTA a pair, when that costs no CTA more than a few tiles a warp over equal
+//     stretches: it saves the merge across CTAs (tickets and a round trip through
+//     L2, about as long as kMergeTiles tiles).
+//   * equal stretches otherwise; a long row of tiles is cut twice: most of it into
+//     one chunk a CTA, the rest into small chunks that CTAs take as they finish,
+//     because SMs do not get equal shares of the memory's bandwidth.
+constexpr int kMergeTiles = 3;
+constexpr int kLongStretch = 64;    // tiles of a warp from which the end is dealt out
+constexpr int kDealtSpan = 64;      // ... unless a pair would be spread over more chunks than these
+template <int W>
+__device__ __forceinline__ Plan plan_of(unsigned total, int longest, int all_pairs, int ctas) {
+  Plan pl;
+  pl.total = total;
+  const unsigned even = max(1u, (total + ctas * W - 1) / (ctas * W));
+  const unsigned rounds = (all_pairs + ctas - 1) / ctas;
+  pl.whole = rounds * ((longest + W - 1) / W) <= even + kMergeTiles;
+  pl.first = pl.rest = even * W;
+  if (even >= kLongStretch && longest <= kDealtSpan * (even / 16) * W) {
+    pl.rest = (even / 16) * W;
+    pl.first = (even - even / 6) * W;
+  }
+  return pl;
+}
 
 template <int D, int TYPE, int RT>
 __global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
@@ -182,18 +236,21 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
   constexpr int VW = D / 32;        // V words of a lane and token
   constexpr int W = S::kWarps;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ Part s_part[W][2];
-  __shared__ int s_last[2];
+  __shared__ Part s_part[W][2];     // [0] a pair begun before the stretch, [1] one that goes on after it
+  __shared__ int s_flags[W];        // kHas0, kEnds0, kParked0, kHas1
+  __shared__ int s_next, s_last[2];
+  __shared__ float s_sum[S::kRows];
+  __shared__ Plan s_plan;           // out of the registers of the tile loop; every warp writes the same
+  constexpr int kHas0 = 1, kEnds0 = 2, kParked0 = 4, kHas1 = 8;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int g = lane / 4, c = lane % 4;
   unsigned char* ring = smem + warp * S::kRingBytes;
-  Meta* meta = reinterpret_cast<Meta*>(smem + S::kMetaOffset) + warp * S::kStages;
+  Meta* meta = reinterpret_cast<Meta*>(smem + S::kMetaOffset) + warp * S::kSlots;   // of tile j: slot j % kSlots
   const uint32_t bar0 = smem_u32(smem + S::kBarOffset) + warp * S::kStages * 8;
   if (lane == 0) {
     for (int s = 0; s < S::kStages; ++s)
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + 8 * s) : "memory");
-    s_part[warp][0].valid = s_part[warp][1].valid = 0;
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
   }
@@ -202,143 +259,152 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  const long long capacity = (long long)p.page_tokens * p.max_pages;
+  const int capacity = p.page_tokens * p.max_pages;   // <= 2^30
   auto tiles_of = [&](int b) {
     const int n = p.seqlens[b];
     return n < 0 || n > capacity ? 0 : (n + kTile - 1) / kTile;
   };
-  // empty sequences (and lengths that are none) are this loop's
-  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    const int n = p.seqlens[b];
-    if (n >= 1 && n <= capacity) continue;
-    if (n != 0 && threadIdx.x == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
-    uint4* o = reinterpret_cast<uint4*>(p.out + (size_t)b * p.Q * p.Hq * D);
-    for (int i = threadIdx.x; i < p.Q * p.Hq * (D / 8); i += S::kThreads) o[i] = make_uint4(0, 0, 0, 0);
-  }
-
-  // ---- this warp's stretch [begin, end) of all tiles ----
+  // ---- the row of all tiles: its length, its longest pair ----
   const int pairs = p.Hkv * p.row_groups;   // of a sequence
-  long long total = 0;
-  for (int b = lane; b < p.B; b += 32) total += tiles_of(b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  total *= pairs;
-  const long long workers = (long long)gridDim.x * W;
-  const long long chunk = max(1ll, (total + workers - 1) / workers);
-  const long long begin = ((long long)blockIdx.x * W + warp) * chunk;
-  const long long end = min(total, begin + chunk);
-  const int count = (int)max(0ll, end - begin);   // chunk <= 2^30 tiles of 16 tokens
-  // the sequence of the first tile, and where its tiles start
-  int at_b = 0;
-  long long at_base = 0;
-  if (count > 0) {
-    for (int b0 = 0;; b0 += 32) {
-      const long long mine = b0 + lane < p.B ? (long long)tiles_of(b0 + lane) * pairs : 0;
-      long long incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      const uint32_t past = __ballot_sync(0xffffffffu, at_base + incl > begin);
-      if (past) {   // some sequence holds it, as begin < total
-        const int l = __ffs(past) - 1;
-        at_b = b0 + l;
-        at_base += __shfl_sync(0xffffffffu, incl - mine, l);
-        break;
-      }
-      at_base += __shfl_sync(0xffffffffu, incl, 31);
+  {
+    unsigned sum = 0;
+    int longest = 0;
+    for (int b = lane; b < p.B; b += 32) {
+      const int n = tiles_of(b);
+      sum += n;
+      longest = max(longest, n);
     }
-  }
-
-  // ---- producer: lane l of the warp prepares tile j0 + l of every 32 and issues it ----
-  int pr_row = 0;          // row of the pools (as matrices of D-byte rows) of this lane's tile
-  Meta pr_meta;
-  auto prepare = [&](int j0) {
-    const long long x = begin + min(j0 + lane, count - 1);
-    int n = tiles_of(at_b);
-    while (x >= at_base + (long long)n * pairs && at_b + 1 < p.B) {
-      at_base += (long long)n * pairs;
-      n = tiles_of(++at_b);
-    }
-    // the bounds below hold by themselves unless the lengths change under the kernel
-    n = max(n, 1);
-    const unsigned long long rel = (unsigned long long)(x - at_base);
-    pr_meta.b = at_b;
-    pr_meta.n = n;
-    pr_meta.pair = min((int)(rel / (unsigned)n), pairs - 1);
-    pr_meta.tile = (int)min(rel - (unsigned long long)pr_meta.pair * n, (unsigned long long)n - 1);
-    const int t0 = pr_meta.tile * kTile;
-    int page = q8::page_of(p.page_table, p.max_pages, p.num_pages, at_b, t0 / p.page_tokens);
-    if (page < 0) {   // reported; the copies then stay inside the pool
-      atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
-      page = 0;
-    }
-    const size_t run = (size_t)page * p.Hkv + pr_meta.pair / p.row_groups;
-    const int row = t0 % p.page_tokens;
-    pr_row = (int)(run * p.page_tokens + row);
-    const size_t block = run * (p.page_tokens / kBlock) + row / kBlock;
-    pr_meta.ks = p.k_scales[block];
-    pr_meta.vs = p.v_scales[block];
-    // the next 32 start where the last of these is
-    at_b = __shfl_sync(0xffffffffu, at_b, 31);
-    at_base = __shfl_sync(0xffffffffu, at_base, 31);
-  };
-  auto copy = [&](int j) {
-    if (lane == j % 32) {
-      const int st = j % S::kStages;
-      const uint32_t bar = bar0 + 8 * st, dst = smem_u32(ring + st * S::kStageBytes);
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(S::kStageBytes) : "memory");
-      tma_2d(dst, &mk, 0, pr_row, bar);
-      tma_2d(dst + S::kTileBytes, &mv, 0, pr_row, bar);
-    }
-  };
-  auto note = [&](int j) {
-    if (lane == j % 32) meta[j % S::kStages] = pr_meta;
-  };
-  int issued = 0;
-  if (count > 0) {
-    prepare(0);
-    const int ahead = min(S::kStages, count);
-    for (; issued < ahead; ++issued) copy(issued);
-    for (int j = 0; j < ahead; ++j) note(j);   // after the copies: these wait for the scales
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    const Plan plan = plan_of<W>(sum * pairs, longest, p.B * pairs, gridDim.x);
+    if (lane == 0) s_plan = plan;
     __syncwarp();
   }
+  // first tile of chunk k, and the chunk of tile x
+  auto chunk_at = [&](unsigned k) {
+    return k <= gridDim.x ? k * s_plan.first : gridDim.x * s_plan.first + (k - gridDim.x) * s_plan.rest;
+  };
+  auto chunk_of = [&](unsigned x) {
+    const unsigned head = gridDim.x * s_plan.first;
+    return x < head ? x / s_plan.first : gridDim.x + (x - head) / s_plan.rest;
+  };
+  // some chunks are taken as CTAs finish
+  auto dealt = [&] { return !s_plan.whole && s_plan.total > gridDim.x * s_plan.first; };
 
-  // ---- the state of the current pair ----
-  uint32_t qa[KS][2 * RT];   // A fragments: rows g (and g + 8)
-  float start[RT];           // where S's accumulators start
-  float m[RT], l[RT];
-  float o[RT][KS][4];        // O^T: dims g.., rows 8 t + 2 c and + 1
-  float F = 1.0f, F_inv = 1.0f, F_top = 1.0f;
-  int len = 0, sees[RT];     // positions that row g (g + 8) sees
-  bool from_start = false;   // the pair's first tile was in this stretch
+  // the scores' scale in the log2 domain (int8: codes enter S as c 2^-24)
+  const float scale = p.scale_log2 * (TYPE == q8::kInt8 ? 0x1p24f : 1.0f);
+  uint32_t before = 0;   // tiles of earlier chunks: tile j's stage and parity follow from before + j
   bool ok = true;
-
-  for (int j = 0; j < count; ++j) {
-    const int st = j % S::kStages;
-    if (ok) {
-      const bool landed = mbar_wait_bounded(bar0 + 8 * st, (j / S::kStages) & 1);
-      if (!__all_sync(0xffffffffu, landed)) {   // no more tiles are used; the stretch is walked to its end
-        ok = false;
-        if (lane == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TIMEOUT);
+  for (unsigned chunk = blockIdx.x;;) {
+    // ---- this warp's stretch: `count` tiles from `begin` on ----
+    unsigned begin = 0;
+    int count = 0;
+    int b_first = 0;           // the sequence of the first tile, and where its tiles start
+    unsigned base_first = 0;
+    if (s_plan.whole) {
+      if (chunk >= (unsigned)(p.B * pairs)) break;
+      b_first = chunk / pairs;
+      const int n = tiles_of(b_first), share = (n + W - 1) / W;
+      // any row's start will do: nothing refers to tiles of other sequences
+      begin = (chunk - b_first * pairs) * n + warp * share;
+      count = max(0, min(n - warp * share, share));
+    } else {
+      const unsigned from = chunk_at(chunk);
+      if (from >= s_plan.total) break;
+      const unsigned share = (chunk < gridDim.x ? s_plan.first : s_plan.rest) / W;
+      begin = from + warp * share;
+      count = begin < s_plan.total ? (int)min(share, s_plan.total - begin) : 0;
+      if (threadIdx.x == 0 && dealt()) s_next = gridDim.x + atomicAdd(p.counters, 1);
+      for (int b0 = 0; count > 0; b0 += 32) {
+        const unsigned mine = b0 + lane < p.B ? tiles_of(b0 + lane) * pairs : 0;
+        unsigned incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += up;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, base_first + incl > begin);
+        if (past || b0 + 32 >= p.B) {   // some sequence holds it, as begin < total
+          const int l = past ? __ffs(past) - 1 : (p.B - 1) % 32;
+          b_first = b0 + l;
+          base_first += __shfl_sync(0xffffffffu, incl - mine, l);
+          break;
+        }
+        base_first += __shfl_sync(0xffffffffu, incl, 31);
       }
     }
-    if (!ok) break;
-    const Meta md = meta[st];
-    const int t0 = md.tile * kTile;
-    if (j == 0 || md.tile == 0) {
-      // a new pair: its query rows, and an empty state
-      from_start = md.tile == 0;
-      len = p.seqlens[md.b];
+    if (!ok) count = 0;
+
+    // ---- the tiles' slots, 16 at a time, a lane each block: first which tiles they
+    // are (and the page-table word, on its way), later their rows and scales.  b: a
+    // sequence no later than the first tile's, base: where its tiles start ----
+    const int half = lane & 1;
+    auto name_tiles = [&](int j0, int b, unsigned base) {
+      const unsigned x = begin + min(j0 + lane / 2, count - 1);
+      int n = tiles_of(b);
+      while (x - base >= (unsigned)n * pairs && b + 1 < p.B) {
+        base += (unsigned)n * pairs;
+        n = tiles_of(++b);
+      }
+      // the bounds below hold by themselves unless the lengths change under the kernel
+      n = max(n, 1);
+      const unsigned rel = x - base;
+      const unsigned pair = min(rel / (unsigned)n, (unsigned)pairs - 1u), tile = min(rel - pair * n, (unsigned)n - 1u);
+      // a tile without a second block has its first one twice
+      unsigned t = tile * kTile + half * kBlock;
+      if ((int)t >= p.seqlens[b]) t = tile * kTile;
+      const unsigned logical = min(t / (unsigned)p.page_tokens, (unsigned)p.max_pages - 1u);
+      Meta& md = meta[(j0 + lane / 2) & (S::kSlots - 1)];
+      copy4_async(smem_u32(&md.word[half]), p.page_table + (size_t)b * p.max_pages + logical);
+      md.row[half] = t % (unsigned)p.page_tokens;   // of its page, for now
+      if (half == 0) *reinterpret_cast<int4*>(&md.tile) = make_int4(tile, n, b, pair);
+    };
+    auto find_tiles = [&](int j0) {   // after a barrier of the warp since name_tiles
+      Meta& md = meta[(j0 + lane / 2) & (S::kSlots - 1)];
+      copies4_done();   // this lane's own
+      const uint32_t word = md.word[half];
+      unsigned page = word & 0x7FFFFFFFu;
+      if (!(word >> 31) || page >= (unsigned)p.num_pages) {   // the copies then stay inside the pool
+        atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
+        page = 0;
+      }
+      // rows of a pool fit an int
+      const int row = (int)(page * p.Hkv + md.pair / p.row_groups) * p.page_tokens + md.row[half];
+      md.row[half] = row;
+      copy4_async(smem_u32(&md.ks[half]), p.k_scales + row / kBlock);
+      copy4_async(smem_u32(&md.vs[half]), p.v_scales + row / kBlock);
+    };
+    auto copy = [&](int j) {
+      if (lane == 0) {
+        const uint32_t st = (before + j) & (S::kStages - 1);
+        const uint32_t bar = bar0 + 8 * st, dst = smem_u32(ring) + st * S::kStageBytes;
+        const int2 row = *reinterpret_cast<const int2*>(meta[j & (S::kSlots - 1)].row);
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(S::kStageBytes) : "memory");
+        tma_2d(dst, &mk, 0, row.x, bar);
+        tma_2d(dst + S::kTileBytes, &mv, 0, row.x, bar);
+        if (!p.wide) {
+          tma_2d(dst + S::kTileBytes / 2, &mk, 0, row.y, bar);
+          tma_2d(dst + S::kTileBytes * 3 / 2, &mv, 0, row.y, bar);
+        }
+      }
+    };
+
+    // ---- the state of the current pair ----
+    uint32_t qa[KS][2 * RT];   // A fragments: rows g (and g + 8)
+    float start[RT];           // where S's accumulators start (int8)
+    float m[RT], l[RT];
+    float o[RT][KS][4];        // O^T: dims g.., rows 8 t + 2 c and + 1
+    float F = 1.0f, F_inv = 1.0f;
+    int flags = 0;
+
+    auto begin_pair = [&](const Meta& md) {   // its query rows, and an empty state
       const int kvh = md.pair / p.row_groups, r0 = (md.pair % p.row_groups) * S::kRows;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         const int r = r0 + 8 * t + g, i = r / p.group;
         const bool row = i < p.Q;
-        sees[t] = row ? len - p.Q + 1 + i : 0;
-        const __half* src = p.q + (((size_t)md.b * p.Q + (row ? i : 0)) * p.Hq + kvh * p.group + r % p.group) * D + 16 * c;
-        float sum = 0.0f;
+        const __half* src =
+            p.q + (((size_t)md.b * p.Q + (row ? i : 0)) * p.Hq + kvh * p.group + r % p.group) * D + 16 * c;
 #pragma unroll
         for (int h = 0; h < NC; ++h)
 #pragma unroll
@@ -349,341 +415,478 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
             qa[4 * h + 2 * u][RT + t] = w.y;
             qa[4 * h + 2 * u + 1][t] = w.z;
             qa[4 * h + 2 * u + 1][RT + t] = w.w;
-            if (TYPE == q8::kInt8) {
-              const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
-                sum += f.x + f.y;
-              }
-            }
           }
-        if (TYPE == q8::kInt8) {
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        }
-        start[t] = sum * -0x1p-17f;   // -128 2^-24
         m[t] = -1e30f;
         l[t] = 0.0f;
 #pragma unroll
         for (int mt = 0; mt < KS; ++mt) o[t][mt][0] = o[t][mt][1] = o[t][mt][2] = o[t][mt][3] = 0.0f;
       }
-      F = F_inv = F_top = 1.0f;
-    }
-
-    // ---- S = Q K^T: columns token_of(0..7) and token_of(8..15) ----
-    const unsigned char* kt = ring + st * S::kStageBytes;
-    const unsigned char* vt = kt + S::kTileBytes;
-    float s[2][4];
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      s[nt][0] = s[nt][1] = TYPE == q8::kInt8 ? start[0] : 0.0f;
-      s[nt][2] = s[nt][3] = TYPE == q8::kInt8 ? start[RT - 1] : 0.0f;
-      const int row = token_of(8 * nt + g);
-#pragma unroll
-      for (int h = 0; h < NC; ++h) {
-        const int at = D == 128 ? row * 128 + (((c + 4 * h) ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
-        const uint4 w = *reinterpret_cast<const uint4*>(kt + at);
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t b0, b1;
-          if (TYPE == q8::kInt8) {
-            const uint32_t u = v[e] ^ 0x80808080u;
-            b0 = __byte_perm(u, 0, 0x4140);
-            b1 = __byte_perm(u, 0, 0x4342);
-          } else {
-            b0 = e4m3x2_to_half2(v[e]);
-            b1 = e4m3x2_to_half2(v[e] >> 16);
-          }
-          const uint32_t* a = qa[4 * h + e];
-          if (RT == 1) mma16816(s[nt], a[0], 0u, a[1], 0u, b0, b1);
-          else mma16816(s[nt], a[0], a[RT - 1], a[RT], a[2 * RT - 1], b0, b1);
-        }
-      }
-    }
-
-    // ---- softmax: rows g (c0, c1) and, with RT == 2, g + 8 (c2, c3) ----
-    const float ks = md.ks * p.scale_log2 * (TYPE == q8::kInt8 ? 0x1p24f : 1.0f);
-    float x[RT][4];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[t][e] = s[e >> 1][2 * t + (e & 1)] * ks;
-    const bool edge = t0 + kTile > len - p.Q + 1;   // some row does not see all of the tile
-    if (edge) {
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (t0 + token_of(8 * (e >> 1) + 2 * c + (e & 1)) >= sees[t]) x[t][e] = -INFINITY;
-    }
-    float mx[RT];
-    bool above = false;
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      mx[t] = fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3]));
-      above |= mx[t] > m[t] + 12.0f;
-    }
-    if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        mx[t] = fmaxf(mx[t], __shfl_xor_sync(0xffffffffu, mx[t], 1));
-        mx[t] = fmaxf(mx[t], __shfl_xor_sync(0xffffffffu, mx[t], 2));
-        const float m_new = mx[t] > m[t] + 12.0f ? mx[t] - 4.0f : m[t];
-        const float alpha = fast_exp2(m[t] - m_new);
-        m[t] = m_new;
-        l[t] *= alpha;
-        const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * c), a1 = __shfl_sync(0xffffffffu, alpha, 8 * c + 4);
-#pragma unroll
-        for (int mt = 0; mt < KS; ++mt) {
-          o[t][mt][0] *= a0;
-          o[t][mt][1] *= a1;
-          o[t][mt][2] *= a0;
-          o[t][mt][3] *= a1;
-        }
-      }
-    }
-    float vs = md.vs * F_inv;
-    if ((vs > 8.0f || vs < 0.125f) && md.vs > 0.0f) {
-      // 2^-40 of the largest scale so far is below what the binary16 result can
-      // show of it, and keeps o / F inside binary32
-      F_top = fmaxf(F_top, md.vs);
-      const float F_new = fmaxf(md.vs, F_top * 0x1p-40f);
-      const float f = F * (F_inv = 1.0f / F_new);
-      F = F_new;
-      vs = md.vs * F_inv;
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int mt = 0; mt < KS; ++mt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[t][mt][e] *= f;
-    }
-    uint32_t pb[RT][2];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      float pr[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(x[t][e] - m[t]);
-      l[t] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
-      pb[t][0] = pack_half2(pr[0] * vs, pr[1] * vs);
-      pb[t][1] = pack_half2(pr[2] * vs, pr[3] * vs);
-    }
-
-    // ---- O^T += V^T P^T ----
-    uint32_t v[4][VW];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = token_of(8 * (e >> 1) + 2 * c + (e & 1));
-      if (D == 128) {
-        const uint4 w = *reinterpret_cast<const uint4*>(vt + row * 128 + ((g ^ (row & 7)) << 4));
-        v[e][0] = w.x; v[e][1] = w.y; v[e][2 % VW] = w.z; v[e][3 % VW] = w.w;
-      } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(vt + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
-        v[e][0] = w.x; v[e][1] = w.y;
-      }
-      // rows behind the sequence may hold anything: an e4m3 NaN times p = 0 would be a NaN
-      if (TYPE == q8::kE4m3 && edge && t0 + row >= len) {
-#pragma unroll
-        for (int w = 0; w < VW; ++w) v[e][w] = 0u;
-      }
-    }
-    __syncwarp();
-    // the stage is free again
-    if (issued < count) {
-      if (issued % 32 == 0) prepare(issued);
-      copy(issued);
-      note(issued);
-      ++issued;
+      F = F_inv = 1.0f;
+    };
+    int issued = 0, j = 0;
+    if (count > 0) {
+      name_tiles(0, b_first, base_first);
+      __syncwarp();
+      begin_pair(meta[0]);      // q's loads travel with the page-table words
+      find_tiles(0);
+      __syncwarp();
+      const int ahead = min(S::kStages, count);
+      for (; issued < ahead; ++issued) copy(issued);
+      copies4_done();
       __syncwarp();
     }
-#pragma unroll
-    for (int w = 0; w < VW; ++w)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        // dims 4 w + 2 u and + 1 of the lane's chunk: bytes of tokens (0, 1), then (2, 3)
-        const uint32_t p01 = __byte_perm(v[0][w], v[1][w], u ? 0x7362 : 0x5140);
-        const uint32_t p23 = __byte_perm(v[2][w], v[3][w], u ? 0x7362 : 0x5140);
-        uint32_t a[4];
-        if (TYPE == q8::kInt8) {
-          const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
-          const uint32_t s01 = p01 ^ 0x80808080u, s23 = p23 ^ 0x80808080u;
-          a[0] = __byte_perm(s01, 0x64646464u, 0x4140);
-          a[1] = __byte_perm(s01, 0x64646464u, 0x4342);
-          a[2] = __byte_perm(s23, 0x64646464u, 0x4140);
-          a[3] = __byte_perm(s23, 0x64646464u, 0x4342);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&a[e]), off);
-            a[e] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-        } else {
-          a[0] = e4m3x2_to_half2(p01);
-          a[1] = e4m3x2_to_half2(p01 >> 16);
-          a[2] = e4m3x2_to_half2(p23);
-          a[3] = e4m3x2_to_half2(p23 >> 16);
-        }
-#pragma unroll
-        for (int t = 0; t < RT; ++t) mma16816(o[t][2 * w + u], a[0], a[1], a[2], a[3], pb[t][0], pb[t][1]);
-      }
 
-    // ---- the pair's last tile here ----
-    const bool ends = md.tile == md.n - 1;
-    if (ends || j == count - 1) {
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
-        l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
+#pragma unroll 1
+    for (; j < count; ++j) {
+      const uint32_t st = (before + j) & (S::kStages - 1);
+      const Meta& slot = meta[j & (S::kSlots - 1)];
+      const float4 sc = *reinterpret_cast<const float4*>(slot.ks);
+      const struct { int tile, n; } md = {slot.tile, slot.n};
+      const int t0 = md.tile * kTile;
+      const bool fresh = j == 0 || md.tile == 0;
+      if (fresh && j > 0) begin_pair(slot);
+      if (!warp_wait(bar0 + 8 * st, (before + j) / S::kStages & 1)) {   // no tile is used after this
+        ok = false;
+        if (lane == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TIMEOUT);
+        break;
       }
-      if (from_start && ends) {
-        const int kvh = md.pair / p.row_groups, r0 = (md.pair % p.row_groups) * S::kRows;
+      if (TYPE == q8::kInt8 && fresh) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          const float inv = l[t] == 0.0f ? 0.0f : F / l[t];
+          float sum = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float f = __shfl_sync(0xffffffffu, inv, 8 * c + 4 * e);
-            const int r = r0 + 8 * t + 2 * c + e, i = r / p.group;
-            if (i < p.Q) {
-              __half* dst = p.out + (((size_t)md.b * p.Q + i) * p.Hq + kvh * p.group + r % p.group) * D + g * (D / 8);
+          for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-              for (int q = 0; q < NC; ++q) {
-                uint4 w;
-                w.x = pack_half2(o[t][4 * q][e] * f, o[t][4 * q][2 + e] * f);
-                w.y = pack_half2(o[t][4 * q + 1][e] * f, o[t][4 * q + 1][2 + e] * f);
-                w.z = pack_half2(o[t][4 * q + 2][e] * f, o[t][4 * q + 2][2 + e] * f);
-                w.w = pack_half2(o[t][4 * q + 3][e] * f, o[t][4 * q + 3][2 + e] * f);
-                reinterpret_cast<uint4*>(dst)[q] = w;
+            for (int e = 0; e < 2; ++e) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qa[ks][e * RT + t]));
+              sum += f.x + f.y;
+            }
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          start[t] = sum * -0x1p-17f;   // -128 2^-24
+        }
+      }
+
+      // ---- S = Q K^T: of block nt / 2, columns token_of(0..7) or token_of(8..15) ----
+      const unsigned char* kt = ring + st * S::kStageBytes;
+      const unsigned char* vt = kt + S::kTileBytes;
+      float s[4][4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        s[nt][0] = s[nt][1] = TYPE == q8::kInt8 ? start[0] : 0.0f;
+        s[nt][2] = s[nt][3] = TYPE == q8::kInt8 ? start[RT - 1] : 0.0f;
+      }
+#pragma unroll
+      for (int h = 0; h < NC; ++h) {
+        uint4 w[4];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+          const int row = token_of(g) + 8 * nt;
+          const int at = D == 128 ? row * 128 + (((c + 4 * h) ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+          w[nt] = *reinterpret_cast<const uint4*>(kt + at);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int nt = 0; nt < 4; ++nt) {   // four independent accumulators in a row
+            const uint32_t v = e == 0 ? w[nt].x : e == 1 ? w[nt].y : e == 2 ? w[nt].z : w[nt].w;
+            uint32_t b0, b1;
+            if (TYPE == q8::kInt8) {
+              const uint32_t u = v ^ 0x80808080u;
+              b0 = __byte_perm(u, 0, 0x4140);
+              b1 = __byte_perm(u, 0, 0x4342);
+            } else {
+              e4m3x4_to_half4(v, b0, b1);
+            }
+            const uint32_t* a = qa[4 * h + e];
+            if (RT == 1) mma16816(s[nt], a[0], 0u, a[1], 0u, b0, b1);
+            else mma16816(s[nt], a[0], a[RT - 1], a[RT], a[2 * RT - 1], b0, b1);
+          }
+      }
+
+      // ---- softmax: rows g (c0, c1) and, with RT == 2, g + 8 (c2, c3) ----
+      float x[RT][8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float ks = (h ? sc.y : sc.x) * scale;
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[t][4 * h + e] = s[2 * h + (e >> 1)][2 * t + (e & 1)] * ks;
+      }
+      // some row may not see all of the tile: length >= 32 (n - 1) + 1, row 0 sees Q - 1 less
+      const bool edge = t0 + kTile > kTile * (md.n - 1) + 2 - p.Q;
+      int len = 0;
+      if (edge) {
+        len = p.seqlens[slot.b];
+        const int r0 = (slot.pair % p.row_groups) * S::kRows;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const int sees = len - p.Q + 1 + (r0 + 8 * t + g) / p.group - t0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (token_of(8 * ((e >> 1) & 1) + 2 * c + (e & 1)) + 16 * (e >> 2) >= sees) x[t][e] = -INFINITY;
+        }
+      }
+      float mx[RT];
+      bool above = false;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        mx[t] = fmaxf(fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])),
+                      fmaxf(fmaxf(x[t][4], x[t][5]), fmaxf(x[t][6], x[t][7])));
+        above |= mx[t] > m[t] + 12.0f;
+      }
+      if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          mx[t] = fmaxf(mx[t], __shfl_xor_sync(0xffffffffu, mx[t], 1));
+          mx[t] = fmaxf(mx[t], __shfl_xor_sync(0xffffffffu, mx[t], 2));
+          const float m_new = mx[t] > m[t] + 12.0f ? mx[t] - 4.0f : m[t];
+          const float alpha = fast_exp2(m[t] - m_new);
+          m[t] = m_new;
+          l[t] *= alpha;
+          const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * c), a1 = __shfl_sync(0xffffffffu, alpha, 8 * c + 4);
+#pragma unroll
+          for (int mt = 0; mt < KS; ++mt) {
+            o[t][mt][0] *= a0;
+            o[t][mt][1] *= a1;
+            o[t][mt][2] *= a0;
+            o[t][mt][3] *= a1;
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[t][e] = fast_exp2(x[t][e] - m[t]);
+        l[t] += ((x[t][0] + x[t][1]) + (x[t][2] + x[t][3])) + ((x[t][4] + x[t][5]) + (x[t][6] + x[t][7]));
+      }
+
+      // ---- O^T += V^T P^T, a block at a time ----
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float vs = h ? sc.w : sc.z;
+        float rel = vs * F_inv;
+        if ((rel > 8.0f || rel < 0.125f) && vs > 0.0f) {
+          // values of scales below 2^-40 round to nothing in the binary16 result
+          const float F_new = fmaxf(vs, 0x1p-40f);
+          const float f = F * (F_inv = 1.0f / F_new);
+          F = F_new;
+          rel = vs * F_inv;
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[t][mt][e] *= f;
+        }
+        uint32_t pb[RT][2];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          pb[t][0] = pack_half2(x[t][4 * h] * rel, x[t][4 * h + 1] * rel);
+          pb[t][1] = pack_half2(x[t][4 * h + 2] * rel, x[t][4 * h + 3] * rel);
+        }
+        uint32_t v[4][VW];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = token_of(2 * c + (e & 1)) + 8 * (e >> 1) + 16 * h;
+          if (D == 128) {
+            const uint4 w = *reinterpret_cast<const uint4*>(vt + row * 128 + ((g ^ (row & 7)) << 4));
+            v[e][0] = w.x; v[e][1] = w.y; v[e][2 % VW] = w.z; v[e][3 % VW] = w.w;
+          } else {
+            const uint2 w =
+                *reinterpret_cast<const uint2*>(vt + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
+            v[e][0] = w.x; v[e][1] = w.y;
+          }
+          // rows behind the sequence may hold anything: an e4m3 NaN times p = 0 would be a NaN
+          if (TYPE == q8::kE4m3 && edge && t0 + row >= len) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) v[e][w] = 0u;
+          }
+        }
+        if (h == 1) {   // the stage is free again
+          __syncwarp();
+          if (issued < count) {
+            copy(issued);
+            ++issued;
+            // the next 16 tiles' slots, well before they are needed: at 8 the last of
+            // these slots' old tiles have been used (kStages <= 4)
+            if ((issued & 3) == 0) {
+              const int at = issued & 15, upcoming = issued - at + 16;
+              if (at == 8 && upcoming < count) {
+                const Meta& last = meta[(upcoming - 1) & (S::kSlots - 1)];
+                name_tiles(upcoming, last.b, begin + upcoming - 1 - (unsigned)last.pair * last.n - last.tile);
               }
+              if (at == 12 && upcoming < count) find_tiles(upcoming);
+              if (at == 0) copies4_done();
+              __syncwarp();
             }
           }
         }
-      } else {
-        const int slot = from_start ? 1 : 0;
-        float* state = from_start ? reinterpret_cast<float*>(ring)
-                                  : reinterpret_cast<float*>(smem + S::kStateOffset) + warp * S::kState;
-        float2* stat = reinterpret_cast<float2*>(smem + S::kStatOffset) + (warp * 2 + slot) * S::kRows;
-        __syncwarp();
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            // dims 4 w + 2 u and + 1 of the lane's chunk: bytes of tokens (0, 1), then (2, 3)
+            const uint32_t p01 = __byte_perm(v[0][w], v[1][w], u ? 0x7362 : 0x5140);
+            const uint32_t p23 = __byte_perm(v[2][w], v[3][w], u ? 0x7362 : 0x5140);
+            uint32_t a[4];
+            if (TYPE == q8::kInt8) {
+              const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+              const uint32_t s01 = p01 ^ 0x80808080u, s23 = p23 ^ 0x80808080u;
+              a[0] = __byte_perm(s01, 0x64646464u, 0x4140);
+              a[1] = __byte_perm(s01, 0x64646464u, 0x4342);
+              a[2] = __byte_perm(s23, 0x64646464u, 0x4140);
+              a[3] = __byte_perm(s23, 0x64646464u, 0x4342);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __half2 d = __hsub2(*reinterpret_cast<__half2*>(&a[e]), off);
+                a[e] = *reinterpret_cast<const uint32_t*>(&d);
+              }
+            } else {
+              e4m3x4_to_half4(p01, a[0], a[1]);
+              e4m3x4_to_half4(p23, a[2], a[3]);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) mma16816(o[t][2 * w + u], a[0], a[1], a[2], a[3], pb[t][0], pb[t][1]);
+          }
+      }
+
+      // ---- the pair's last tile here ----
+      const bool ends = md.tile == md.n - 1;
+      if (ends || j == count - 1) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          if (c == 0) stat[8 * t + g] = make_float2(m[t], l[t]);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float4* dst = reinterpret_cast<float4*>(state + (8 * t + 2 * c + e) * D + g * (D / 8));
-#pragma unroll
-            for (int q = 0; q < KS / 2; ++q)
-              dst[q] = make_float4(o[t][2 * q][e] * F, o[t][2 * q][2 + e] * F, o[t][2 * q + 1][e] * F,
-                                   o[t][2 * q + 1][2 + e] * F);
-          }
+          l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
+          l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
         }
-        if (lane == 0) {
-          const long long x = begin + j;
-          s_part[warp][slot] = Part{x - md.tile, md.n, md.b, md.pair, 1, ends};
+        const bool from_start = j >= md.tile;   // the pair's first tile is in this stretch
+        const int sb = slot.b, sp = slot.pair;
+        if (from_start && ends) {
+          const int kvh = sp / p.row_groups, r0 = (sp % p.row_groups) * S::kRows;
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            const float inv = l[t] == 0.0f ? 0.0f : F / l[t];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float f = __shfl_sync(0xffffffffu, inv, 8 * c + 4 * e);
+              const int r = r0 + 8 * t + 2 * c + e, i = r / p.group;
+              if (i < p.Q) {
+                __half* dst = p.out + (((size_t)sb * p.Q + i) * p.Hq + kvh * p.group + r % p.group) * D + g * (D / 8);
+#pragma unroll
+                for (int q = 0; q < NC; ++q) {
+                  uint4 w;
+                  w.x = pack_half2(o[t][4 * q][e] * f, o[t][4 * q][2 + e] * f);
+                  w.y = pack_half2(o[t][4 * q + 1][e] * f, o[t][4 * q + 1][2 + e] * f);
+                  w.z = pack_half2(o[t][4 * q + 2][e] * f, o[t][4 * q + 2][2 + e] * f);
+                  w.w = pack_half2(o[t][4 * q + 3][e] * f, o[t][4 * q + 3][2 + e] * f);
+                  reinterpret_cast<uint4*>(dst)[q] = w;
+                }
+              }
+            }
+          }
+        } else {
+          // the state: in the ring where the stretch is over, else (a pair begun
+          // earlier, the ring in use) in this warp's place in global memory
+          const int which = from_start ? 1 : 0;
+          const bool parked = j < count - 1;
+          float* state = parked ? p.parked + ((size_t)blockIdx.x * W + warp) * S::kState : reinterpret_cast<float*>(ring);
+          float2* stat = reinterpret_cast<float2*>(smem + S::kStatOffset) + (warp * 2 + which) * S::kRows;
+          __syncwarp();
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            if (c == 0) stat[8 * t + g] = make_float2(m[t], l[t]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float4* dst = reinterpret_cast<float4*>(state + (8 * t + 2 * c + e) * D + g * (D / 8));
+#pragma unroll
+              for (int q = 0; q < KS / 2; ++q)
+                dst[q] = make_float4(o[t][2 * q][e] * F, o[t][2 * q][2 + e] * F, o[t][2 * q + 1][e] * F,
+                                     o[t][2 * q + 1][2 + e] * F);
+            }
+          }
+          flags |= which ? kHas1 : kHas0 | (ends ? kEnds0 : 0) | (parked ? kParked0 : 0);
+          if (lane == 0) s_part[warp][which] = Part{begin + j - md.tile, md.n, sb, sp};
         }
       }
     }
-  }
-  if (!ok) {
-    // copies in flight land before the shared memory is given up
-    for (int j = max(0, issued - S::kStages); j < issued; ++j)
-      if (j >= 0) mbar_wait_bounded(bar0 + 8 * (j % S::kStages), (j / S::kStages) & 1);
-  }
-  __syncthreads();
+    if (!ok) {
+      // copies in flight land before the shared memory is used for anything else
+      for (; j < issued; ++j)
+        if (!warp_wait(bar0 + 8 * ((before + j) & (S::kStages - 1)), (before + j) / S::kStages & 1)) break;
+    }
+    before += count;
+    if (lane == 0) s_flags[warp] = flags;
+    __syncthreads();
 
-  // ---- merge what the warps left ----
-  // A chain: the states of one pair in consecutive warps.  It begins with a
-  // pair begun earlier in warp 0, or with a warp's pair that goes on.
-  auto weights = [](float M, float mi) { return fast_exp2(mi - M); };
-  auto finish = [&](const Part& pt, int row, int d4, float4 acc, float lsum) {
-    const int kvh = pt.pair / p.row_groups, r = (pt.pair % p.row_groups) * S::kRows + row, i = r / p.group;
-    if (i >= p.Q) return;
-    const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-    __half* dst = p.out + (((size_t)pt.b * p.Q + i) * p.Hq + kvh * p.group + r % p.group) * D + 4 * d4;
-    *reinterpret_cast<uint2*>(dst) =
-        make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
-  };
-  const float2* stats = reinterpret_cast<const float2*>(smem + S::kStatOffset);
-  Part open[2];                       // this CTA's share of pairs that span CTAs
-  open[0].valid = open[1].valid = 0;
-  for (int w = 0; w < W; ++w)
-    for (int slot = w == 0 ? 0 : 1; slot < 2; ++slot) {
-      const Part first = s_part[w][slot];
-      if (!first.valid) continue;
+    // ---- merge what the warps left ----
+    // A chain: the states of one pair in consecutive warps.  It begins with a
+    // pair begun earlier in warp 0, or with a warp's pair that goes on.
+    auto finish = [&](const Part& pt, int at, float4 acc, float lsum) {   // at: float4 of the state
+      const int row = at / (D / 4);
+      const int kvh = pt.pair / p.row_groups, r = (pt.pair % p.row_groups) * S::kRows + row, i = r / p.group;
+      if (i >= p.Q) return;
+      const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+      __half* dst = p.out + (((size_t)pt.b * p.Q + i) * p.Hq + kvh * p.group + r % p.group) * D + 4 * (at % (D / 4));
+      *reinterpret_cast<uint2*>(dst) =
+          make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
+    };
+    constexpr int kVec = S::kRows * (D / 4);                       // float4s of a state
+    constexpr int kMine = (kVec + S::kThreads - 1) / S::kThreads;  // of a thread
+    const float2* stats = reinterpret_cast<const float2*>(smem + S::kStatOffset);
+    int open = 0;        // bit s: the pair of s_part[open_warp[s]][s] spans chunks
+    int open_warp1 = 0;  // (that of slot 0 is warp 0's)
+    for (int w = 0, slot = 0; w < W; slot ? (void)(++w) : (void)0, slot = 1) {
+      int fl = s_flags[w];
+      if (!(fl & (slot ? kHas1 : kHas0))) continue;
       int members = 1;
-      bool ended = first.ends != 0;
-      while (!ended && w + members < W && s_part[w + members][0].valid) {
-        ended = s_part[w + members][0].ends != 0;
+      bool ended = slot == 0 && (fl & kEnds0);
+      while (!ended && w + members < W && ((fl = s_flags[w + members]) & kHas0)) {
+        ended = (fl & kEnds0) != 0;
         ++members;
       }
       const bool whole = slot == 1 && ended;
-      float* out = p.partials + ((size_t)blockIdx.x * 2 + slot) * S::kPartial;
-      for (int i = threadIdx.x; i < S::kRows * (D / 4); i += S::kThreads) {
-        const int row = i / (D / 4), d4 = i % (D / 4);
+      float* out = p.partials + ((size_t)chunk * 2 + slot) * S::kPartial;
+#pragma unroll 1
+      for (int i = 0; i < kMine; ++i) {
+        const int at = threadIdx.x + i * S::kThreads, row = at / (D / 4);
+        if (at >= kVec) break;
         float M = -1e30f, lsum = 0.0f;
+#pragma unroll 4
         for (int k = 0; k < members; ++k) M = fmaxf(M, stats[((w + k) * 2 + (k ? 0 : slot)) * S::kRows + row].x);
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
         for (int k = 0; k < members; ++k) {
           const float2 ml = stats[((w + k) * 2 + (k ? 0 : slot)) * S::kRows + row];
-          const float f = weights(M, ml.x);
-          const float* state = k == 0 && slot == 1 ? reinterpret_cast<const float*>(smem + w * S::kRingBytes)
-                                                   : reinterpret_cast<const float*>(smem + S::kStateOffset) + (w + k) * S::kState;
-          const float4 v = *reinterpret_cast<const float4*>(state + row * D + 4 * d4);
+          const float f = fast_exp2(ml.x - M);
+          const bool parked = (k || !slot) && (s_flags[w + k] & kParked0);
+          const float4* state = parked ? reinterpret_cast<const float4*>(p.parked + ((size_t)blockIdx.x * W + w + k) * S::kState)
+                                       : reinterpret_cast<const float4*>(smem + (w + k) * S::kRingBytes);
+          const float4 v = state[at];
           lsum += f * ml.y;
           acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
         }
         if (whole) {
-          finish(first, row, d4, acc, lsum);
+          finish(s_part[w][1], at, acc, lsum);
         } else {
-          __stcg(reinterpret_cast<float4*>(out + row * D) + d4, acc);
-          if (d4 == 0) __stcg(reinterpret_cast<float2*>(out + S::kState) + row, make_float2(M, lsum));
+          __stcg(reinterpret_cast<float4*>(out) + at, acc);
+          if (at % (D / 4) == 0) __stcg(reinterpret_cast<float2*>(out + S::kState) + row, make_float2(M, lsum));
         }
       }
-      if (!whole) open[slot] = first;
-    }
-  if (!open[0].valid && !open[1].valid) return;
-
-  // ---- pairs that span CTAs: the last CTA to arrive merges, in CTA order ----
-  const long long cta_tiles = chunk * W;
-  int first_cta[2], ctas[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    first_cta[s] = s == 1 ? (int)blockIdx.x : open[0].valid ? (int)(open[0].first / cta_tiles) : 0;
-    ctas[s] = open[s].valid ? (int)((open[s].first + open[s].n - 1) / cta_tiles) - first_cta[s] + 1 : 0;
-  }
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    const int s = threadIdx.x;
-    bool last = false;
-    if (open[s].valid) {
-      last = atomicAdd(p.tickets + first_cta[s], 1) == ctas[s] - 1;
-      if (last) p.tickets[first_cta[s]] = 0;
-    }
-    s_last[s] = last;
-  }
-  __syncthreads();
-  for (int s = 0; s < 2; ++s) {
-    if (!s_last[s]) continue;
-    __threadfence();
-    // the first CTA's state is of a pair that goes on, the others' of one begun earlier
-    auto state_of = [&](int k) { return p.partials + ((size_t)(first_cta[s] + k) * 2 + (k == 0)) * S::kPartial; };
-    for (int i = threadIdx.x; i < S::kRows * (D / 4); i += S::kThreads) {
-      const int row = i / (D / 4), d4 = i % (D / 4);
-      float M = -1e30f, lsum = 0.0f;
-      for (int k = 0; k < ctas[s]; ++k)
-        M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(state_of(k) + S::kState) + row).x);
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-      for (int k = 0; k < ctas[s]; ++k) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(state_of(k) + S::kState) + row);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(state_of(k) + row * D) + d4);
-        const float f = weights(M, ml.x);
-        lsum += f * ml.y;
-        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      if (!whole) {
+        open |= 1 << slot;
+        if (slot) open_warp1 = w;
       }
-      finish(open[s], row, d4, acc, lsum);
     }
+
+    // ---- pairs that span chunks: the last CTA to arrive merges, in chunk order ----
+    __syncthreads();   // the partials are written (and the rings free again)
+    if (open) {
+      if (threadIdx.x < 2) {
+        const int slot = threadIdx.x;
+        bool last = false;
+        if (open >> slot & 1) {
+          const Part pt = s_part[slot ? open_warp1 : 0][slot];
+          const unsigned c0 = chunk_of(pt.first), c1 = chunk_of(pt.first + pt.n - 1);
+          __threadfence();
+          int* ticket = p.counters + kTickets + c0;
+          last = atomicAdd(ticket, 1) == (int)(c1 - c0);
+          if (last) *ticket = 0;
+          __threadfence();
+        }
+        s_last[slot] = last;
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int slot = 0; slot < 2; ++slot) {
+        if (!s_last[slot]) continue;
+        const Part pt = s_part[slot ? open_warp1 : 0][slot];
+        const unsigned c0 = chunk_of(pt.first);
+        const int n = (int)(chunk_of(pt.first + pt.n - 1) - c0) + 1;
+        // the first chunk's state is of a pair that goes on, the others' of one begun earlier
+        auto state_of = [&](int k) { return p.partials + ((size_t)(c0 + k) * 2 + (k == 0)) * S::kPartial; };
+        constexpr int kBatch = kMine > 1 ? 4 : 8;   // chunks whose states a thread loads at a time
+        float4 v[kMine][kBatch];
+        auto load = [&](int k0) {
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+              const int at = threadIdx.x + i * S::kThreads;
+              if (k0 + k < n && at < kVec) v[i][k] = __ldcg(reinterpret_cast<const float4*>(state_of(k0 + k)) + at);
+            }
+        };
+        load(0);
+        // every chunk's (m, l), then the weights 2^(m - M) in their place: a warp a row
+        float2* ml = reinterpret_cast<float2*>(smem);   // [chunk][row], over the rings
+        for (int i = threadIdx.x; i < n * S::kRows; i += S::kThreads)
+          ml[i] = __ldcg(reinterpret_cast<const float2*>(state_of(i / S::kRows) + S::kState) + i % S::kRows);
+        __syncthreads();
+        for (int row = warp; row < S::kRows; row += W) {
+          float M = -1e30f, sum = 0.0f;
+          for (int k = lane; k < n; k += 32) M = fmaxf(M, ml[k * S::kRows + row].x);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+          for (int k = lane; k < n; k += 32) {
+            const float f = fast_exp2(ml[k * S::kRows + row].x - M);
+            ml[k * S::kRows + row].x = f;
+            sum += f * ml[k * S::kRows + row].y;
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (lane == 0) s_sum[row] = sum;
+        }
+        __syncthreads();
+        float4 acc[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+        for (int k0 = 0;;) {
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+              const int at = threadIdx.x + i * S::kThreads;
+              if (k0 + k < n && at < kVec) {
+                const float f = ml[(k0 + k) * S::kRows + at / (D / 4)].x;
+                acc[i].x += f * v[i][k].x; acc[i].y += f * v[i][k].y;
+                acc[i].z += f * v[i][k].z; acc[i].w += f * v[i][k].w;
+              }
+            }
+          k0 += kBatch;
+          if (k0 >= n) break;
+          load(k0);
+        }
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int at = threadIdx.x + i * S::kThreads;
+          if (at < kVec) finish(pt, at, acc[i], s_sum[at / (D / 4)]);
+        }
+        __syncthreads();   // the rings, s_sum and s_part are used again
+      }
+    }
+    // the next chunk: the ring's generic reads and writes end before copies fill it again
+    if (s_plan.whole) {
+      chunk += gridDim.x;
+    } else if (dealt()) {
+      chunk = s_next;
+    } else {
+      break;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && dealt() && atomicAdd(p.counters + 1, 1) == (int)gridDim.x - 1) {
+    p.counters[0] = 0;   // the last CTA: nobody takes a chunk any more
+    p.counters[1] = 0;
+  }
+  // empty sequences (and lengths that are none)
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    const int n = p.seqlens[b];
+    if (n >= 1 && n <= capacity) continue;
+    if (n != 0 && threadIdx.x == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+    uint4* o = reinterpret_cast<uint4*>(p.out + (size_t)b * p.Q * p.Hq * D);
+    for (int i = threadIdx.x; i < p.Q * p.Hq * (D / 8); i += S::kThreads) o[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -725,14 +928,16 @@ static int sm_count() {
 // 8 rows a pair where they suffice, else 16 (the MMA's row count): more rows
 // would leave too few registers for enough warps
 static int row_tiles(int Q, int Hq, int Hkv) { return Q * (Hq / Hkv) <= 8 ? 1 : 2; }
-static int max_ctas(int rt, int sms) { return sms * (rt == 1 ? Shape<128, 1>::kCtas : Shape<128, 2>::kCtas); }
+static int max_ctas(int sms) { return 2 * std::min(sms, kMaxSms); }
+static size_t partial_floats(int rt, int D) { return (size_t)kMaxChunks * 2 * (8 * rt) * (D + 2); }
+static size_t parked_floats(int rt, int D, int sms) { return (size_t)max_ctas(sms) * (rt == 1 ? 6 : 4) * (8 * rt) * D; }
 
 static std::once_flag g_encode_once;
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
-// A pool's codes as a matrix of D-byte rows; one box = a tile's 16 rows, swizzled
-// over the row's length.
-static bool pool_map(CUtensorMap* map, const void* codes, long long rows, int D) {
+// A pool's codes as a matrix of D-byte rows, swizzled over the row's length; one box
+// is a tile where pages hold whole ones, else a block.
+static bool pool_map(CUtensorMap* map, const void* codes, long long rows, int D, int box_rows) {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -744,7 +949,7 @@ static bool pool_map(CUtensorMap* map, const void* codes, long long rows, int D)
   if (!g_encode) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)D};
-  const cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)kTile};
+  const cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
@@ -782,7 +987,7 @@ size_t anvilq_gqa_decode_q8_workspace_size(int B, int Q, int Hq, int Hkv, int D)
   const int sms = sm_count();
   if (sms <= 0) return 0;
   const int rt = row_tiles(Q, Hq, Hkv);
-  return ANVILQ_WORKSPACE_COUNTER_BYTES + (size_t)max_ctas(rt, sms) * 2 * (8 * rt) * (D + 2) * sizeof(float);
+  return ANVILQ_WORKSPACE_COUNTER_BYTES + (partial_floats(rt, D) + parked_floats(rt, D, sms)) * sizeof(float);
 }
 
 int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_codes, const float* k_scales,
@@ -813,8 +1018,9 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   p.page_table = page_table;
   p.seqlens = seqlens;
   p.out = reinterpret_cast<__half*>(out);
-  p.tickets = static_cast<int*>(workspace);
+  p.counters = static_cast<int*>(workspace);
   p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + ANVILQ_WORKSPACE_COUNTER_BYTES);
+  p.parked = p.partials + partial_floats(rt, D);
   p.dev_err = dev_err;
   p.B = B; p.Q = Q; p.Hq = Hq; p.Hkv = Hkv;
   p.group = Hq / Hkv;
@@ -822,11 +1028,13 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   p.page_tokens = page_tokens; p.max_pages = max_pages; p.num_pages = num_pages;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
   // as many CTAs as the device holds, but no more warps than the table has room for tiles
-  const double tiles = (double)B * Hkv * p.row_groups * max_pages * (page_tokens / kTile);
-  const int ctas = (int)std::max(1.0, std::min((double)max_ctas(rt, sms), std::ceil(tiles / warps)));
-  if (tiles / ((double)ctas * warps) > (double)(1 << 30)) return ANVILQ_ESHAPE;   // a warp counts its tiles in an int
+  const double tiles = (double)B * Hkv * p.row_groups * ((double)max_pages * page_tokens / kTile + 1);
+  const int ctas = (int)std::max(1.0, std::min((double)max_ctas(sms), std::ceil(tiles / warps)));
+  if (tiles > (double)(1u << 31)) return ANVILQ_ESHAPE;   // tiles are counted in 32 bits
   CUtensorMap mk, mv;
-  if (!pool_map(&mk, k_codes, rows, D) || !pool_map(&mv, v_codes, rows, D)) return ANVILQ_EALIGN;
+  p.wide = page_tokens % kTile == 0;
+  const int box = p.wide ? kTile : kBlock;
+  if (!pool_map(&mk, k_codes, rows, D, box) || !pool_map(&mv, v_codes, rows, D, box)) return ANVILQ_EALIGN;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool int8 = code_type == ANVILQ_KV_Q8_INT8;
   if (D == 64)

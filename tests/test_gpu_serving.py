@@ -341,6 +341,7 @@ ATTENTIONS = [
     ([70], 64, 4, 4, 64, 16),                       # the widest chunk
     ([33] * 40, 1, 8, 8, 64, 16),                   # more than 32 sequences, many short pairs
     ([20000], 2, 4, 1, 128, 128),                   # one long pair over the whole device
+    ([40000], 3, 4, 1, 64, 32),                     # the same with more than 8 rows
 ]
 
 
