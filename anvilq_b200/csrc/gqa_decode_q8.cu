@@ -60,9 +60,14 @@ using q8::kBlock;
 constexpr int kTile = 2 * kBlock;   // tokens of a step
 constexpr int kMaxSms = 160;                  // SMs that are used
 constexpr int kMaxChunks = 9 * kMaxSms;       // chunks of a call that pairs may span (plan_of: at most 4.25 a CTA)
-constexpr int kMaxSpan = 2 * kMaxSms;         // chunks of a pair
 constexpr int kTickets = 2;                   // counters before the tickets
 constexpr unsigned long long kWaitLimitNs = 1000000000ull;
+
+struct Divisor {     // x / d for 0 <= x < 2^17, 1 <= d < 2^15: the error of m is below d / 2^32
+  int d;
+  unsigned m;        // ceil(2^32 / d); 0 for d = 1
+  __device__ __forceinline__ int quotient(int x) const { return m ? (int)__umulhi((unsigned)x, m) : x; }
+};
 
 struct Params {
   const __half* q;             // [B][Q][Hq][D]
@@ -75,7 +80,8 @@ struct Params {
   float* partials;             // [chunk][2] states: of the pair begun earlier, of the pair that goes on
   float* parked;               // [CTA][warp] states
   int* dev_err;
-  int B, Q, Hq, Hkv, group, row_groups, page_tokens, max_pages, num_pages;
+  int B, Q, Hq, Hkv, page_tokens, max_pages, num_pages;
+  Divisor group, row_groups;   // query heads a kv head; row groups a (sequence, kv head)
   int wide;                    // pages hold whole tiles: one copy of 32 rows, not two of 16
   float scale_log2;            // softmax scale * log2(e)
 };
@@ -87,6 +93,7 @@ struct Shape {
   static constexpr int kRows = 8 * RT;
   static constexpr int kWarps = RT == 1 ? 6 : 4;               // 168 or 255 registers a thread
   static constexpr int kThreads = kWarps * 32;
+  static_assert(kWarps <= 6, "Control has room for their parts");
   static constexpr int kCtas = 2;                              // per SM
   static constexpr int kTileBytes = kTile * D;                 // of K or V
   static constexpr int kStageBytes = 2 * kTileBytes;
@@ -105,7 +112,6 @@ struct Shape {
   static constexpr int kPartial = kState + 2 * kRows;          // floats of a state in global memory
   static_assert((kStages & (kStages - 1)) == 0 && kStages <= 4, "a slot's old tile is used by the time it is named again");
   static_assert(kRingBytes >= kState * 4, "a state fits the idle ring");
-  static_assert(kWarps * kRingBytes >= kMaxSpan * kRows * 8, "(m, l) of every chunk of a pair fit the idle rings");
   static_assert(kCtas * (kTotal + 2048) <= 227 * 1024, "CTAs per SM");
 };
 
@@ -164,7 +170,10 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ void copy4_async(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copies4_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {   // through L2 alone
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -226,270 +235,218 @@ __device__ __forceinline__ Plan plan_of(unsigned total, int longest, int all_pai
   return pl;
 }
 
+// tiles of a pair of sequence b; none for a length outside 0 .. capacity
+__device__ __forceinline__ int tiles_of(const Params& p, int b) {
+  const int n = p.seqlens[b];
+  return n < 0 || n > p.page_tokens * p.max_pages ? 0 : (n + kTile - 1) / kTile;
+}
+
+constexpr int kMaxWarps = 6;
+enum { kHas0 = 1, kEnds0 = 2, kParked0 = 4, kHas1 = 8 };
+struct Control {     // in shared memory
+  Part part[kMaxWarps][2];   // [0] a pair begun before the warp's stretch, [1] one that goes on after it
+  int flags[kMaxWarps];      // kHas0 ...
+  int next, last[2];
+  uint2 open[2];             // first chunk and number of chunks of a pair that spans several
+  Plan plan;                 // out of the registers of the tile loop; every warp writes the same
+  __device__ __forceinline__ unsigned chunk_at(unsigned k) const {   // first tile of chunk k
+    return k <= gridDim.x ? k * plan.first : gridDim.x * plan.first + (k - gridDim.x) * plan.rest;
+  }
+  __device__ __forceinline__ unsigned chunk_of(unsigned x) const {   // the chunk of tile x
+    const unsigned head = gridDim.x * plan.first;
+    return x < head ? x / plan.first : gridDim.x + (x - head) / plan.rest;
+  }
+  // some chunks are taken as CTAs finish
+  __device__ __forceinline__ bool dealt() const { return !plan.whole && plan.total > gridDim.x * plan.first; }
+};
+
+// One warp's stretch: `count` tiles from tile `begin` of the row on, b and base a
+// sequence no later than the first tile's and where its tiles start.  Pairs inside
+// it are finished, the states of others left for merge_chunk.  `before`: tiles of
+// the warp's earlier stretches.  False after a wait that ran out.  A function of
+// its own, as merge_chunk is: in one body the compiler spilled this loop's state
+// (1.6 times the time).
 template <int D, int TYPE, int RT>
-__global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
-    gqa_decode_q8_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                         const __grid_constant__ Params p) {
+__device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,
+                                         unsigned char* smem, Control& ctl, uint32_t before, unsigned begin, int count,
+                                         int b_first, unsigned base_first) {
   using S = Shape<D, RT>;
   constexpr int KS = D / 16;        // k-steps of S, m-tiles of O^T
   constexpr int NC = D / 64;        // 16-byte K chunks of a lane
   constexpr int VW = D / 32;        // V words of a lane and token
   constexpr int W = S::kWarps;
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ Part s_part[W][2];     // [0] a pair begun before the stretch, [1] one that goes on after it
-  __shared__ int s_flags[W];        // kHas0, kEnds0, kParked0, kHas1
-  __shared__ int s_next, s_last[2];
-  __shared__ float s_sum[S::kRows];
-  __shared__ Plan s_plan;           // out of the registers of the tile loop; every warp writes the same
-  constexpr int kHas0 = 1, kEnds0 = 2, kParked0 = 4, kHas1 = 8;
-  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int g = lane / 4, c = lane % 4;
   unsigned char* ring = smem + warp * S::kRingBytes;
   Meta* meta = reinterpret_cast<Meta*>(smem + S::kMetaOffset) + warp * S::kSlots;   // of tile j: slot j % kSlots
   const uint32_t bar0 = smem_u32(smem + S::kBarOffset) + warp * S::kStages * 8;
-  if (lane == 0) {
-    for (int s = 0; s < S::kStages; ++s)
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + 8 * s) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
-  }
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  __syncwarp();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  const int capacity = p.page_tokens * p.max_pages;   // <= 2^30
-  auto tiles_of = [&](int b) {
-    const int n = p.seqlens[b];
-    return n < 0 || n > capacity ? 0 : (n + kTile - 1) / kTile;
-  };
-  // ---- the row of all tiles: its length, its longest pair ----
-  const int pairs = p.Hkv * p.row_groups;   // of a sequence
-  {
-    unsigned sum = 0;
-    int longest = 0;
-    for (int b = lane; b < p.B; b += 32) {
-      const int n = tiles_of(b);
-      sum += n;
-      longest = max(longest, n);
-    }
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    longest = __reduce_max_sync(0xffffffffu, longest);
-    const Plan plan = plan_of<W>(sum * pairs, longest, p.B * pairs, gridDim.x);
-    if (lane == 0) s_plan = plan;
-    __syncwarp();
-  }
-  // first tile of chunk k, and the chunk of tile x
-  auto chunk_at = [&](unsigned k) {
-    return k <= gridDim.x ? k * s_plan.first : gridDim.x * s_plan.first + (k - gridDim.x) * s_plan.rest;
-  };
-  auto chunk_of = [&](unsigned x) {
-    const unsigned head = gridDim.x * s_plan.first;
-    return x < head ? x / s_plan.first : gridDim.x + (x - head) / s_plan.rest;
-  };
-  // some chunks are taken as CTAs finish
-  auto dealt = [&] { return !s_plan.whole && s_plan.total > gridDim.x * s_plan.first; };
-
+  const int pairs = p.Hkv * p.row_groups.d, Q = p.Q;
+  const bool wide = p.wide;
+  const int* seqlens = p.seqlens;
   // the scores' scale in the log2 domain (int8: codes enter S as c 2^-24)
   const float scale = p.scale_log2 * (TYPE == q8::kInt8 ? 0x1p24f : 1.0f);
-  uint32_t before = 0;   // tiles of earlier chunks: tile j's stage and parity follow from before + j
   bool ok = true;
-  for (unsigned chunk = blockIdx.x;;) {
-    // ---- this warp's stretch: `count` tiles from `begin` on ----
-    unsigned begin = 0;
-    int count = 0;
-    int b_first = 0;           // the sequence of the first tile, and where its tiles start
-    unsigned base_first = 0;
-    if (s_plan.whole) {
-      if (chunk >= (unsigned)(p.B * pairs)) break;
-      b_first = chunk / pairs;
-      const int n = tiles_of(b_first), share = (n + W - 1) / W;
-      // any row's start will do: nothing refers to tiles of other sequences
-      begin = (chunk - b_first * pairs) * n + warp * share;
-      count = max(0, min(n - warp * share, share));
-    } else {
-      const unsigned from = chunk_at(chunk);
-      if (from >= s_plan.total) break;
-      const unsigned share = (chunk < gridDim.x ? s_plan.first : s_plan.rest) / W;
-      begin = from + warp * share;
-      count = begin < s_plan.total ? (int)min(share, s_plan.total - begin) : 0;
-      if (threadIdx.x == 0 && dealt()) s_next = gridDim.x + atomicAdd(p.counters, 1);
-      for (int b0 = 0; count > 0; b0 += 32) {
-        const unsigned mine = b0 + lane < p.B ? tiles_of(b0 + lane) * pairs : 0;
-        unsigned incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += up;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, base_first + incl > begin);
-        if (past || b0 + 32 >= p.B) {   // some sequence holds it, as begin < total
-          const int l = past ? __ffs(past) - 1 : (p.B - 1) % 32;
-          b_first = b0 + l;
-          base_first += __shfl_sync(0xffffffffu, incl - mine, l);
-          break;
-        }
-        base_first += __shfl_sync(0xffffffffu, incl, 31);
+
+  // ---- the tiles' slots, 16 at a time, a lane each block: first which tiles they
+  // are (and the page-table word, on its way), later their rows and scales.  b: a
+  // sequence no later than the first tile's, base: where its tiles start ----
+  const int half = lane & 1;
+  auto name_tiles = [&](int j0, int b, unsigned base) {
+    const unsigned x = begin + min(j0 + lane / 2, count - 1);
+    int n = tiles_of(p, b);
+    while (x - base >= (unsigned)n * pairs && b + 1 < p.B) {
+      base += (unsigned)n * pairs;
+      n = tiles_of(p, ++b);
+    }
+    // the bounds below hold by themselves unless the lengths change under the kernel
+    n = max(n, 1);
+    const unsigned rel = x - base;
+    const unsigned pair = min(rel / (unsigned)n, (unsigned)pairs - 1u), tile = min(rel - pair * n, (unsigned)n - 1u);
+    // a tile without a second block has its first one twice
+    unsigned t = tile * kTile + half * kBlock;
+    if ((int)t >= p.seqlens[b]) t = tile * kTile;
+    const unsigned logical = min(t / (unsigned)p.page_tokens, (unsigned)p.max_pages - 1u);
+    Meta& md = meta[(j0 + lane / 2) & (S::kSlots - 1)];
+    copy4_async(smem_u32(&md.word[half]), p.page_table + (size_t)b * p.max_pages + logical);
+    md.row[half] = t % (unsigned)p.page_tokens;   // of its page, for now
+    if (half == 0) *reinterpret_cast<int4*>(&md.tile) = make_int4(tile, n, b, pair);
+  };
+  auto find_tiles = [&](int j0) {   // after a barrier of the warp since name_tiles
+    Meta& md = meta[(j0 + lane / 2) & (S::kSlots - 1)];
+    copies_done();   // this lane's own
+    const uint32_t word = md.word[half];
+    unsigned page = word & 0x7FFFFFFFu;
+    if (!(word >> 31) || page >= (unsigned)p.num_pages) {   // the copies then stay inside the pool
+      atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
+      page = 0;
+    }
+    // rows of a pool fit an int
+    const int row = (int)(page * p.Hkv + p.row_groups.quotient(md.pair)) * p.page_tokens + md.row[half];
+    md.row[half] = row;
+    copy4_async(smem_u32(&md.ks[half]), p.k_scales + row / kBlock);
+    copy4_async(smem_u32(&md.vs[half]), p.v_scales + row / kBlock);
+  };
+  auto copy = [&](int j) {
+    if (lane == 0) {
+      const uint32_t st = (before + j) & (S::kStages - 1);
+      const uint32_t bar = bar0 + 8 * st, dst = smem_u32(ring) + st * S::kStageBytes;
+      const int2 row = *reinterpret_cast<const int2*>(meta[j & (S::kSlots - 1)].row);
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(S::kStageBytes) : "memory");
+      tma_2d(dst, &mk, 0, row.x, bar);
+      tma_2d(dst + S::kTileBytes, &mv, 0, row.x, bar);
+      if (!wide) {
+        tma_2d(dst + S::kTileBytes / 2, &mk, 0, row.y, bar);
+        tma_2d(dst + S::kTileBytes * 3 / 2, &mv, 0, row.y, bar);
       }
     }
-    if (!ok) count = 0;
+  };
 
-    // ---- the tiles' slots, 16 at a time, a lane each block: first which tiles they
-    // are (and the page-table word, on its way), later their rows and scales.  b: a
-    // sequence no later than the first tile's, base: where its tiles start ----
-    const int half = lane & 1;
-    auto name_tiles = [&](int j0, int b, unsigned base) {
-      const unsigned x = begin + min(j0 + lane / 2, count - 1);
-      int n = tiles_of(b);
-      while (x - base >= (unsigned)n * pairs && b + 1 < p.B) {
-        base += (unsigned)n * pairs;
-        n = tiles_of(++b);
-      }
-      // the bounds below hold by themselves unless the lengths change under the kernel
-      n = max(n, 1);
-      const unsigned rel = x - base;
-      const unsigned pair = min(rel / (unsigned)n, (unsigned)pairs - 1u), tile = min(rel - pair * n, (unsigned)n - 1u);
-      // a tile without a second block has its first one twice
-      unsigned t = tile * kTile + half * kBlock;
-      if ((int)t >= p.seqlens[b]) t = tile * kTile;
-      const unsigned logical = min(t / (unsigned)p.page_tokens, (unsigned)p.max_pages - 1u);
-      Meta& md = meta[(j0 + lane / 2) & (S::kSlots - 1)];
-      copy4_async(smem_u32(&md.word[half]), p.page_table + (size_t)b * p.max_pages + logical);
-      md.row[half] = t % (unsigned)p.page_tokens;   // of its page, for now
-      if (half == 0) *reinterpret_cast<int4*>(&md.tile) = make_int4(tile, n, b, pair);
-    };
-    auto find_tiles = [&](int j0) {   // after a barrier of the warp since name_tiles
-      Meta& md = meta[(j0 + lane / 2) & (S::kSlots - 1)];
-      copies4_done();   // this lane's own
-      const uint32_t word = md.word[half];
-      unsigned page = word & 0x7FFFFFFFu;
-      if (!(word >> 31) || page >= (unsigned)p.num_pages) {   // the copies then stay inside the pool
-        atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
-        page = 0;
-      }
-      // rows of a pool fit an int
-      const int row = (int)(page * p.Hkv + md.pair / p.row_groups) * p.page_tokens + md.row[half];
-      md.row[half] = row;
-      copy4_async(smem_u32(&md.ks[half]), p.k_scales + row / kBlock);
-      copy4_async(smem_u32(&md.vs[half]), p.v_scales + row / kBlock);
-    };
-    auto copy = [&](int j) {
-      if (lane == 0) {
-        const uint32_t st = (before + j) & (S::kStages - 1);
-        const uint32_t bar = bar0 + 8 * st, dst = smem_u32(ring) + st * S::kStageBytes;
-        const int2 row = *reinterpret_cast<const int2*>(meta[j & (S::kSlots - 1)].row);
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(S::kStageBytes) : "memory");
-        tma_2d(dst, &mk, 0, row.x, bar);
-        tma_2d(dst + S::kTileBytes, &mv, 0, row.x, bar);
-        if (!p.wide) {
-          tma_2d(dst + S::kTileBytes / 2, &mk, 0, row.y, bar);
-          tma_2d(dst + S::kTileBytes * 3 / 2, &mv, 0, row.y, bar);
+  // ---- the state of the current pair ----
+  uint32_t qa[KS][2 * RT];   // A fragments: rows g (and g + 8)
+  float start[RT];           // where S's accumulators start (int8)
+  float m[RT], l[RT];
+  float o[RT][KS][4];        // O^T: dims g.., rows 8 t + 2 c and + 1
+  float F = 1.0f, F_inv = 1.0f;
+  int flags = 0;
+
+  auto begin_pair = [&](const Meta& md) {   // its query rows, and an empty state
+    const int kvh = p.row_groups.quotient(md.pair), r0 = (md.pair - kvh * p.row_groups.d) * S::kRows;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = r0 + 8 * t + g, i = p.group.quotient(r);
+      const bool row = i < p.Q;
+      const __half* src =
+          p.q + (((size_t)md.b * p.Q + (row ? i : 0)) * p.Hq + kvh * p.group.d + r - i * p.group.d) * D + 16 * c;
+#pragma unroll
+      for (int h = 0; h < NC; ++h)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (row) w = *reinterpret_cast<const uint4*>(src + 64 * h + 8 * u);
+          qa[4 * h + 2 * u][t] = w.x;
+          qa[4 * h + 2 * u][RT + t] = w.y;
+          qa[4 * h + 2 * u + 1][t] = w.z;
+          qa[4 * h + 2 * u + 1][RT + t] = w.w;
         }
-      }
-    };
-
-    // ---- the state of the current pair ----
-    uint32_t qa[KS][2 * RT];   // A fragments: rows g (and g + 8)
-    float start[RT];           // where S's accumulators start (int8)
-    float m[RT], l[RT];
-    float o[RT][KS][4];        // O^T: dims g.., rows 8 t + 2 c and + 1
-    float F = 1.0f, F_inv = 1.0f;
-    int flags = 0;
-
-    auto begin_pair = [&](const Meta& md) {   // its query rows, and an empty state
-      const int kvh = md.pair / p.row_groups, r0 = (md.pair % p.row_groups) * S::kRows;
+      m[t] = -1e30f;
+      l[t] = 0.0f;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const int r = r0 + 8 * t + g, i = r / p.group;
-        const bool row = i < p.Q;
-        const __half* src =
-            p.q + (((size_t)md.b * p.Q + (row ? i : 0)) * p.Hq + kvh * p.group + r % p.group) * D + 16 * c;
-#pragma unroll
-        for (int h = 0; h < NC; ++h)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (row) w = *reinterpret_cast<const uint4*>(src + 64 * h + 8 * u);
-            qa[4 * h + 2 * u][t] = w.x;
-            qa[4 * h + 2 * u][RT + t] = w.y;
-            qa[4 * h + 2 * u + 1][t] = w.z;
-            qa[4 * h + 2 * u + 1][RT + t] = w.w;
-          }
-        m[t] = -1e30f;
-        l[t] = 0.0f;
-#pragma unroll
-        for (int mt = 0; mt < KS; ++mt) o[t][mt][0] = o[t][mt][1] = o[t][mt][2] = o[t][mt][3] = 0.0f;
-      }
-      F = F_inv = 1.0f;
-    };
-    int issued = 0, j = 0;
-    if (count > 0) {
-      name_tiles(0, b_first, base_first);
-      __syncwarp();
-      begin_pair(meta[0]);      // q's loads travel with the page-table words
-      find_tiles(0);
-      __syncwarp();
-      const int ahead = min(S::kStages, count);
-      for (; issued < ahead; ++issued) copy(issued);
-      copies4_done();
-      __syncwarp();
+      for (int mt = 0; mt < KS; ++mt) o[t][mt][0] = o[t][mt][1] = o[t][mt][2] = o[t][mt][3] = 0.0f;
     }
+    F = F_inv = 1.0f;
+  };
+  int issued = 0, j = 0;
+  if (count > 0) {
+    name_tiles(0, b_first, base_first);
+    __syncwarp();
+    begin_pair(meta[0]);      // q's loads travel with the page-table words
+    find_tiles(0);
+    __syncwarp();
+    const int ahead = min(S::kStages, count);
+    for (; issued < ahead; ++issued) copy(issued);
+    copies_done();
+    __syncwarp();
+  }
 
 #pragma unroll 1
-    for (; j < count; ++j) {
-      const uint32_t st = (before + j) & (S::kStages - 1);
-      const Meta& slot = meta[j & (S::kSlots - 1)];
-      const float4 sc = *reinterpret_cast<const float4*>(slot.ks);
-      const struct { int tile, n; } md = {slot.tile, slot.n};
-      const int t0 = md.tile * kTile;
-      const bool fresh = j == 0 || md.tile == 0;
-      if (fresh && j > 0) begin_pair(slot);
-      if (!warp_wait(bar0 + 8 * st, (before + j) / S::kStages & 1)) {   // no tile is used after this
-        ok = false;
-        if (lane == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TIMEOUT);
-        break;
+  for (; j < count; ++j) {
+    const uint32_t st = (before + j) & (S::kStages - 1);
+    const Meta& slot = meta[j & (S::kSlots - 1)];
+    const struct { int tile, n; } md = {slot.tile, slot.n};
+    const bool fresh = j == 0 || md.tile == 0;
+    if (fresh && j > 0) begin_pair(slot);
+    if (!warp_wait(bar0 + 8 * st, (before + j) / S::kStages & 1)) {   // no tile is used after this
+      ok = false;
+      if (lane == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TIMEOUT);
+      break;
+    }
+    if (TYPE == q8::kInt8 && fresh) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qa[ks][e * RT + t]));
+            sum += f.x + f.y;
+          }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        start[t] = sum * -0x1p-17f;   // -128 2^-24
       }
-      if (TYPE == q8::kInt8 && fresh) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          float sum = 0.0f;
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qa[ks][e * RT + t]));
-              sum += f.x + f.y;
-            }
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          start[t] = sum * -0x1p-17f;   // -128 2^-24
-        }
-      }
+    }
 
-      // ---- S = Q K^T: of block nt / 2, columns token_of(0..7) or token_of(8..15) ----
-      const unsigned char* kt = ring + st * S::kStageBytes;
+    // ---- block by block (not unrolled: twice the state would not fit 168 registers) ----
+    const unsigned char* kt = ring + st * S::kStageBytes;
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h, kt += kBlock * D) {
       const unsigned char* vt = kt + S::kTileBytes;
-      float s[4][4];
+      const int t0 = md.tile * kTile + h * kBlock;
+      // ---- S = Q K^T: columns token_of(0..7) and token_of(8..15) ----
+      float s[2][4];
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
+      for (int nt = 0; nt < 2; ++nt) {
         s[nt][0] = s[nt][1] = TYPE == q8::kInt8 ? start[0] : 0.0f;
         s[nt][2] = s[nt][3] = TYPE == q8::kInt8 ? start[RT - 1] : 0.0f;
       }
+      uint4 w[NC][2];
 #pragma unroll
-      for (int h = 0; h < NC; ++h) {
-        uint4 w[4];
+      for (int q = 0; q < NC; ++q)
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
+        for (int nt = 0; nt < 2; ++nt) {
           const int row = token_of(g) + 8 * nt;
-          const int at = D == 128 ? row * 128 + (((c + 4 * h) ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
-          w[nt] = *reinterpret_cast<const uint4*>(kt + at);
+          const int at = D == 128 ? row * 128 + (((c + 4 * q) ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+          w[q][nt] = *reinterpret_cast<const uint4*>(kt + at);
         }
+#pragma unroll
+      for (int q = 0; q < NC; ++q)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int nt = 0; nt < 4; ++nt) {   // four independent accumulators in a row
-            const uint32_t v = e == 0 ? w[nt].x : e == 1 ? w[nt].y : e == 2 ? w[nt].z : w[nt].w;
+          for (int nt = 0; nt < 2; ++nt) {
+            const uint4 k = w[q][nt];
+            const uint32_t v = e == 0 ? k.x : e == 1 ? k.y : e == 2 ? k.z : k.w;
             uint32_t b0, b1;
             if (TYPE == q8::kInt8) {
               const uint32_t u = v ^ 0x80808080u;
@@ -498,42 +455,37 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
             } else {
               e4m3x4_to_half4(v, b0, b1);
             }
-            const uint32_t* a = qa[4 * h + e];
+            const uint32_t* a = qa[4 * q + e];
             if (RT == 1) mma16816(s[nt], a[0], 0u, a[1], 0u, b0, b1);
             else mma16816(s[nt], a[0], a[RT - 1], a[RT], a[2 * RT - 1], b0, b1);
           }
-      }
 
       // ---- softmax: rows g (c0, c1) and, with RT == 2, g + 8 (c2, c3) ----
-      float x[RT][8];
+      const float ks = slot.ks[h] * scale, vs = slot.vs[h];
+      float x[RT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float ks = (h ? sc.y : sc.x) * scale;
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[t][4 * h + e] = s[2 * h + (e >> 1)][2 * t + (e & 1)] * ks;
-      }
-      // some row may not see all of the tile: length >= 32 (n - 1) + 1, row 0 sees Q - 1 less
-      const bool edge = t0 + kTile > kTile * (md.n - 1) + 2 - p.Q;
+        for (int e = 0; e < 4; ++e) x[t][e] = s[e >> 1][2 * t + (e & 1)] * ks;
+      // some row may not see all of the block: length >= 32 (n - 1) + 1, row 0 sees Q - 1 less
+      const bool edge = t0 + kBlock > kTile * (md.n - 1) + 2 - Q;
       int len = 0;
       if (edge) {
-        len = p.seqlens[slot.b];
-        const int r0 = (slot.pair % p.row_groups) * S::kRows;
+        len = seqlens[slot.b];
+        const int r0 = (slot.pair - p.row_groups.quotient(slot.pair) * p.row_groups.d) * S::kRows;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          const int sees = len - p.Q + 1 + (r0 + 8 * t + g) / p.group - t0;
+          const int sees = len - Q + 1 + p.group.quotient(r0 + 8 * t + g) - t0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (token_of(8 * ((e >> 1) & 1) + 2 * c + (e & 1)) + 16 * (e >> 2) >= sees) x[t][e] = -INFINITY;
+          for (int e = 0; e < 4; ++e)
+            if (token_of(2 * c + (e & 1)) + 8 * (e >> 1) >= sees) x[t][e] = -INFINITY;
         }
       }
       float mx[RT];
       bool above = false;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        mx[t] = fmaxf(fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])),
-                      fmaxf(fmaxf(x[t][4], x[t][5]), fmaxf(x[t][6], x[t][7])));
+        mx[t] = fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3]));
         above |= mx[t] > m[t] + 12.0f;
       }
       if (__any_sync(0xffffffffu, above)) {
@@ -555,328 +507,407 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
           }
         }
       }
+      float rel = vs * F_inv;
+      if ((rel > 8.0f || rel < 0.125f) && vs > 0.0f) {
+        // values of scales below 2^-40 round to nothing in the binary16 result
+        const float F_new = fmaxf(vs, 0x1p-40f);
+        const float f = F * (F_inv = 1.0f / F_new);
+        F = F_new;
+        rel = vs * F_inv;
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][mt][e] *= f;
+      }
+      uint32_t pb[RT][2];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[t][e] = fast_exp2(x[t][e] - m[t]);
-        l[t] += ((x[t][0] + x[t][1]) + (x[t][2] + x[t][3])) + ((x[t][4] + x[t][5]) + (x[t][6] + x[t][7]));
+        for (int e = 0; e < 4; ++e) x[t][e] = fast_exp2(x[t][e] - m[t]);
+        l[t] += (x[t][0] + x[t][1]) + (x[t][2] + x[t][3]);
+        pb[t][0] = pack_half2(x[t][0] * rel, x[t][1] * rel);
+        pb[t][1] = pack_half2(x[t][2] * rel, x[t][3] * rel);
       }
 
-      // ---- O^T += V^T P^T, a block at a time ----
+      // ---- O^T += V^T P^T ----
+      uint32_t v[4][VW];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float vs = h ? sc.w : sc.z;
-        float rel = vs * F_inv;
-        if ((rel > 8.0f || rel < 0.125f) && vs > 0.0f) {
-          // values of scales below 2^-40 round to nothing in the binary16 result
-          const float F_new = fmaxf(vs, 0x1p-40f);
-          const float f = F * (F_inv = 1.0f / F_new);
-          F = F_new;
-          rel = vs * F_inv;
-#pragma unroll
-          for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int mt = 0; mt < KS; ++mt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[t][mt][e] *= f;
-        }
-        uint32_t pb[RT][2];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          pb[t][0] = pack_half2(x[t][4 * h] * rel, x[t][4 * h + 1] * rel);
-          pb[t][1] = pack_half2(x[t][4 * h + 2] * rel, x[t][4 * h + 3] * rel);
-        }
-        uint32_t v[4][VW];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = token_of(2 * c + (e & 1)) + 8 * (e >> 1) + 16 * h;
-          if (D == 128) {
-            const uint4 w = *reinterpret_cast<const uint4*>(vt + row * 128 + ((g ^ (row & 7)) << 4));
-            v[e][0] = w.x; v[e][1] = w.y; v[e][2 % VW] = w.z; v[e][3 % VW] = w.w;
-          } else {
-            const uint2 w =
-                *reinterpret_cast<const uint2*>(vt + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
-            v[e][0] = w.x; v[e][1] = w.y;
-          }
-          // rows behind the sequence may hold anything: an e4m3 NaN times p = 0 would be a NaN
-          if (TYPE == q8::kE4m3 && edge && t0 + row >= len) {
-#pragma unroll
-            for (int w = 0; w < VW; ++w) v[e][w] = 0u;
-          }
-        }
-        if (h == 1) {   // the stage is free again
-          __syncwarp();
-          if (issued < count) {
-            copy(issued);
-            ++issued;
-            // the next 16 tiles' slots, well before they are needed: at 8 the last of
-            // these slots' old tiles have been used (kStages <= 4)
-            if ((issued & 3) == 0) {
-              const int at = issued & 15, upcoming = issued - at + 16;
-              if (at == 8 && upcoming < count) {
-                const Meta& last = meta[(upcoming - 1) & (S::kSlots - 1)];
-                name_tiles(upcoming, last.b, begin + upcoming - 1 - (unsigned)last.pair * last.n - last.tile);
-              }
-              if (at == 12 && upcoming < count) find_tiles(upcoming);
-              if (at == 0) copies4_done();
-              __syncwarp();
-            }
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < VW; ++w)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            // dims 4 w + 2 u and + 1 of the lane's chunk: bytes of tokens (0, 1), then (2, 3)
-            const uint32_t p01 = __byte_perm(v[0][w], v[1][w], u ? 0x7362 : 0x5140);
-            const uint32_t p23 = __byte_perm(v[2][w], v[3][w], u ? 0x7362 : 0x5140);
-            uint32_t a[4];
-            if (TYPE == q8::kInt8) {
-              const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
-              const uint32_t s01 = p01 ^ 0x80808080u, s23 = p23 ^ 0x80808080u;
-              a[0] = __byte_perm(s01, 0x64646464u, 0x4140);
-              a[1] = __byte_perm(s01, 0x64646464u, 0x4342);
-              a[2] = __byte_perm(s23, 0x64646464u, 0x4140);
-              a[3] = __byte_perm(s23, 0x64646464u, 0x4342);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __half2 d = __hsub2(*reinterpret_cast<__half2*>(&a[e]), off);
-                a[e] = *reinterpret_cast<const uint32_t*>(&d);
-              }
-            } else {
-              e4m3x4_to_half4(p01, a[0], a[1]);
-              e4m3x4_to_half4(p23, a[2], a[3]);
-            }
-#pragma unroll
-            for (int t = 0; t < RT; ++t) mma16816(o[t][2 * w + u], a[0], a[1], a[2], a[3], pb[t][0], pb[t][1]);
-          }
-      }
-
-      // ---- the pair's last tile here ----
-      const bool ends = md.tile == md.n - 1;
-      if (ends || j == count - 1) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
-          l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
-        }
-        const bool from_start = j >= md.tile;   // the pair's first tile is in this stretch
-        const int sb = slot.b, sp = slot.pair;
-        if (from_start && ends) {
-          const int kvh = sp / p.row_groups, r0 = (sp % p.row_groups) * S::kRows;
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            const float inv = l[t] == 0.0f ? 0.0f : F / l[t];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float f = __shfl_sync(0xffffffffu, inv, 8 * c + 4 * e);
-              const int r = r0 + 8 * t + 2 * c + e, i = r / p.group;
-              if (i < p.Q) {
-                __half* dst = p.out + (((size_t)sb * p.Q + i) * p.Hq + kvh * p.group + r % p.group) * D + g * (D / 8);
-#pragma unroll
-                for (int q = 0; q < NC; ++q) {
-                  uint4 w;
-                  w.x = pack_half2(o[t][4 * q][e] * f, o[t][4 * q][2 + e] * f);
-                  w.y = pack_half2(o[t][4 * q + 1][e] * f, o[t][4 * q + 1][2 + e] * f);
-                  w.z = pack_half2(o[t][4 * q + 2][e] * f, o[t][4 * q + 2][2 + e] * f);
-                  w.w = pack_half2(o[t][4 * q + 3][e] * f, o[t][4 * q + 3][2 + e] * f);
-                  reinterpret_cast<uint4*>(dst)[q] = w;
-                }
-              }
-            }
-          }
+      for (int e = 0; e < 4; ++e) {
+        const int row = token_of(2 * c + (e & 1)) + 8 * (e >> 1);
+        if (D == 128) {
+          const uint4 k = *reinterpret_cast<const uint4*>(vt + row * 128 + ((g ^ (row & 7)) << 4));
+          v[e][0] = k.x; v[e][1] = k.y; v[e][2 % VW] = k.z; v[e][3 % VW] = k.w;
         } else {
-          // the state: in the ring where the stretch is over, else (a pair begun
-          // earlier, the ring in use) in this warp's place in global memory
-          const int which = from_start ? 1 : 0;
-          const bool parked = j < count - 1;
-          float* state = parked ? p.parked + ((size_t)blockIdx.x * W + warp) * S::kState : reinterpret_cast<float*>(ring);
-          float2* stat = reinterpret_cast<float2*>(smem + S::kStatOffset) + (warp * 2 + which) * S::kRows;
-          __syncwarp();
+          const uint2 k =
+              *reinterpret_cast<const uint2*>(vt + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
+          v[e][0] = k.x; v[e][1] = k.y;
+        }
+        // rows behind the sequence may hold anything: an e4m3 NaN times p = 0 would be a NaN
+        if (TYPE == q8::kE4m3 && edge && t0 + row >= len) {
 #pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            if (c == 0) stat[8 * t + g] = make_float2(m[t], l[t]);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float4* dst = reinterpret_cast<float4*>(state + (8 * t + 2 * c + e) * D + g * (D / 8));
-#pragma unroll
-              for (int q = 0; q < KS / 2; ++q)
-                dst[q] = make_float4(o[t][2 * q][e] * F, o[t][2 * q][2 + e] * F, o[t][2 * q + 1][e] * F,
-                                     o[t][2 * q + 1][2 + e] * F);
-            }
-          }
-          flags |= which ? kHas1 : kHas0 | (ends ? kEnds0 : 0) | (parked ? kParked0 : 0);
-          if (lane == 0) s_part[warp][which] = Part{begin + j - md.tile, md.n, sb, sp};
+          for (int w = 0; w < VW; ++w) v[e][w] = 0u;
         }
       }
+#pragma unroll
+      for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          // dims 4 w + 2 u and + 1 of the lane's chunk: bytes of tokens (0, 1), then (2, 3)
+          const uint32_t p01 = __byte_perm(v[0][w], v[1][w], u ? 0x7362 : 0x5140);
+          const uint32_t p23 = __byte_perm(v[2][w], v[3][w], u ? 0x7362 : 0x5140);
+          uint32_t a[4];
+          if (TYPE == q8::kInt8) {
+            const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+            const uint32_t s01 = p01 ^ 0x80808080u, s23 = p23 ^ 0x80808080u;
+            a[0] = __byte_perm(s01, 0x64646464u, 0x4140);
+            a[1] = __byte_perm(s01, 0x64646464u, 0x4342);
+            a[2] = __byte_perm(s23, 0x64646464u, 0x4140);
+            a[3] = __byte_perm(s23, 0x64646464u, 0x4342);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __half2 d = __hsub2(*reinterpret_cast<__half2*>(&a[e]), off);
+              a[e] = *reinterpret_cast<const uint32_t*>(&d);
+            }
+          } else {
+            e4m3x4_to_half4(p01, a[0], a[1]);
+            e4m3x4_to_half4(p23, a[2], a[3]);
+          }
+#pragma unroll
+          for (int t = 0; t < RT; ++t) mma16816(o[t][2 * w + u], a[0], a[1], a[2], a[3], pb[t][0], pb[t][1]);
+        }
     }
-    if (!ok) {
-      // copies in flight land before the shared memory is used for anything else
-      for (; j < issued; ++j)
-        if (!warp_wait(bar0 + 8 * ((before + j) & (S::kStages - 1)), (before + j) / S::kStages & 1)) break;
-    }
-    before += count;
-    if (lane == 0) s_flags[warp] = flags;
-    __syncthreads();
-
-    // ---- merge what the warps left ----
-    // A chain: the states of one pair in consecutive warps.  It begins with a
-    // pair begun earlier in warp 0, or with a warp's pair that goes on.
-    auto finish = [&](const Part& pt, int at, float4 acc, float lsum) {   // at: float4 of the state
-      const int row = at / (D / 4);
-      const int kvh = pt.pair / p.row_groups, r = (pt.pair % p.row_groups) * S::kRows + row, i = r / p.group;
-      if (i >= p.Q) return;
-      const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-      __half* dst = p.out + (((size_t)pt.b * p.Q + i) * p.Hq + kvh * p.group + r % p.group) * D + 4 * (at % (D / 4));
-      *reinterpret_cast<uint2*>(dst) =
-          make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
-    };
-    constexpr int kVec = S::kRows * (D / 4);                       // float4s of a state
-    constexpr int kMine = (kVec + S::kThreads - 1) / S::kThreads;  // of a thread
-    const float2* stats = reinterpret_cast<const float2*>(smem + S::kStatOffset);
-    int open = 0;        // bit s: the pair of s_part[open_warp[s]][s] spans chunks
-    int open_warp1 = 0;  // (that of slot 0 is warp 0's)
-    for (int w = 0, slot = 0; w < W; slot ? (void)(++w) : (void)0, slot = 1) {
-      int fl = s_flags[w];
-      if (!(fl & (slot ? kHas1 : kHas0))) continue;
-      int members = 1;
-      bool ended = slot == 0 && (fl & kEnds0);
-      while (!ended && w + members < W && ((fl = s_flags[w + members]) & kHas0)) {
-        ended = (fl & kEnds0) != 0;
-        ++members;
+    __syncwarp();
+    // the stage is free again
+    if (issued < count) {
+      copy(issued);
+      ++issued;
+      // the next 16 tiles' slots, well before they are needed: at 8 the last of
+      // these slots' old tiles have been used (kStages <= 4)
+      if ((issued & 3) == 0) {
+        const int at = issued & 15, upcoming = issued - at + 16;
+        if (at == 8 && upcoming < count) {
+          const Meta& last = meta[(upcoming - 1) & (S::kSlots - 1)];
+          name_tiles(upcoming, last.b, begin + upcoming - 1 - (unsigned)last.pair * last.n - last.tile);
+        }
+        if (at == 12 && upcoming < count) find_tiles(upcoming);
+        if (at == 0) copies_done();
+        __syncwarp();
       }
-      const bool whole = slot == 1 && ended;
-      float* out = p.partials + ((size_t)chunk * 2 + slot) * S::kPartial;
+    }
+
+    // ---- the pair's last tile here ----
+    const bool ends = md.tile == md.n - 1;
+    if (ends || j == count - 1) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
+        l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
+      }
+      const bool from_start = j >= md.tile;   // the pair's first tile is in this stretch
+      const int sb = slot.b, sp = slot.pair;
+      if (from_start && ends) {
+        const int kvh = p.row_groups.quotient(sp), r0 = (sp - kvh * p.row_groups.d) * S::kRows;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const float inv = l[t] == 0.0f ? 0.0f : F / l[t];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float f = __shfl_sync(0xffffffffu, inv, 8 * c + 4 * e);
+            const int r = r0 + 8 * t + 2 * c + e, i = p.group.quotient(r);
+            if (i < p.Q) {
+              __half* dst = p.out + (((size_t)sb * p.Q + i) * p.Hq + kvh * p.group.d + r - i * p.group.d) * D + g * (D / 8);
+#pragma unroll
+              for (int q = 0; q < NC; ++q) {
+                uint4 w;
+                w.x = pack_half2(o[t][4 * q][e] * f, o[t][4 * q][2 + e] * f);
+                w.y = pack_half2(o[t][4 * q + 1][e] * f, o[t][4 * q + 1][2 + e] * f);
+                w.z = pack_half2(o[t][4 * q + 2][e] * f, o[t][4 * q + 2][2 + e] * f);
+                w.w = pack_half2(o[t][4 * q + 3][e] * f, o[t][4 * q + 3][2 + e] * f);
+                reinterpret_cast<uint4*>(dst)[q] = w;
+              }
+            }
+          }
+        }
+      } else {
+        // the state: in the ring where the stretch is over, else (a pair begun
+        // earlier, the ring in use) in this warp's place in global memory
+        const int which = from_start ? 1 : 0;
+        const bool parked = j < count - 1;
+        float* state = parked ? p.parked + ((size_t)blockIdx.x * W + warp) * S::kState : reinterpret_cast<float*>(ring);
+        float2* stat = reinterpret_cast<float2*>(smem + S::kStatOffset) + (warp * 2 + which) * S::kRows;
+        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          if (c == 0) stat[8 * t + g] = make_float2(m[t], l[t]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float4* dst = reinterpret_cast<float4*>(state + (8 * t + 2 * c + e) * D + g * (D / 8));
+#pragma unroll
+            for (int q = 0; q < KS / 2; ++q)
+              dst[q] = make_float4(o[t][2 * q][e] * F, o[t][2 * q][2 + e] * F, o[t][2 * q + 1][e] * F,
+                                   o[t][2 * q + 1][2 + e] * F);
+          }
+        }
+        flags |= which ? kHas1 : kHas0 | (ends ? kEnds0 : 0) | (parked ? kParked0 : 0);
+        if (lane == 0) ctl.part[warp][which] = Part{begin + j - md.tile, md.n, sb, sp};
+      }
+    }
+  }
+  if (!ok) {
+    // copies in flight land before the shared memory is used for anything else
+    for (; j < issued; ++j)
+      if (!warp_wait(bar0 + 8 * ((before + j) & (S::kStages - 1)), (before + j) / S::kStages & 1)) break;
+  }
+  if (lane == 0) ctl.flags[warp] = flags;
+  return ok;
+}
+
+// Merges what the warps left of a chunk (frugal with registers: the tile loop's
+// share the kernel's with this).
+template <int D, int RT>
+__device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem, Control& ctl, unsigned chunk) {
+  using S = Shape<D, RT>;
+  constexpr int W = S::kWarps;
+  constexpr int kVec = S::kRows * (D / 4);   // float4s of a state
+  auto finish = [&](const Part& pt, int at, float4 acc, float lsum) {   // at: float4 of the state
+    const int row = at / (D / 4);
+    const int kvh = p.row_groups.quotient(pt.pair), r = (pt.pair - kvh * p.row_groups.d) * S::kRows + row;
+    const int i = p.group.quotient(r);
+    if (i >= p.Q) return;
+    const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+    __half* dst = p.out + (((size_t)pt.b * p.Q + i) * p.Hq + kvh * p.group.d + r - i * p.group.d) * D + 4 * (at % (D / 4));
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
+  };
+  auto add_state = [](float M, float& lsum, float4& acc, float2 ml, float4 v) {   // M: at least ml.x
+    const float f = fast_exp2(ml.x - M);
+    lsum += f * ml.y;
+    acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+  };
+  // A chain: the states of one pair in consecutive warps.  It begins with a
+  // pair begun earlier in warp 0, or with a warp's pair that goes on.
+  const float2* stats = reinterpret_cast<const float2*>(smem + S::kStatOffset);
+  unsigned has0, ends0, parked0, starts;   // bit w: warp w's
+  {
+    const int lane = threadIdx.x % 32, fl = lane < W ? ctl.flags[lane] : 0;
+    has0 = __ballot_sync(0xffffffffu, fl & kHas0);
+    ends0 = __ballot_sync(0xffffffffu, fl & kEnds0);
+    parked0 = __ballot_sync(0xffffffffu, fl & kParked0);
+    starts = __ballot_sync(0xffffffffu, fl & kHas1) << 1 | (has0 & 1);   // bit 0: slot 0 of warp 0; bit w + 1: slot 1 of w
+  }
+  int open = 0;        // bit s: the pair of ctl.part[open warp][s] spans chunks
+  int open_warp1 = 0;  // (that of slot 0 is warp 0's)
 #pragma unroll 1
+  for (; starts; starts &= starts - 1) {
+    const int slot = (starts & 1) ? 0 : 1, w = max(__ffs(starts) - 2, 0);
+    int members = 1;
+    bool ended = slot == 0 && (ends0 & 1);
+    while (!ended && (has0 >> (w + members) & 1)) {
+      ended = ends0 >> (w + members) & 1;
+      ++members;
+    }
+    const bool whole = slot == 1 && ended;
+    float* out = p.partials + ((size_t)chunk * 2 + slot) * S::kPartial;
+    const float2* stat = stats + (w * 2 + slot) * S::kRows;   // of members after the first: slot 0 of their warps
+#pragma unroll 1
+    for (int at = threadIdx.x; at < kVec; at += S::kThreads) {
+      const int row = at / (D / 4);
+      float M = stat[row].x, lsum = 0.0f;
+#pragma unroll 2
+      for (int k = 1; k < members; ++k) M = fmaxf(M, stats[(w + k) * 2 * S::kRows + row].x);
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+      for (int k = 0; k < members; ++k) {
+        const bool parked = (k || !slot) && (parked0 >> (w + k) & 1);
+        const float4* state = parked ? reinterpret_cast<const float4*>(p.parked + ((size_t)blockIdx.x * W + w + k) * S::kState)
+                                     : reinterpret_cast<const float4*>(smem + (w + k) * S::kRingBytes);
+        add_state(M, lsum, acc, k ? stats[(w + k) * 2 * S::kRows + row] : stat[row], state[at]);
+      }
+      if (whole) {
+        finish(ctl.part[w][1], at, acc, lsum);
+      } else {
+        __stcg(reinterpret_cast<float4*>(out) + at, acc);
+        if (at % (D / 4) == 0) __stcg(reinterpret_cast<float2*>(out + S::kState) + row, make_float2(M, lsum));
+      }
+    }
+    if (!whole) {
+      open |= 1 << slot;
+      if (slot) open_warp1 = w;
+    }
+  }
+
+  // ---- pairs that span chunks: the last CTA to arrive merges, in chunk order ----
+  __syncthreads();   // the partials are written (and the rings free again)
+  if (!open) return;
+  if (threadIdx.x < 2) {
+    const int slot = threadIdx.x;
+    bool last = false;
+    if (open >> slot & 1) {
+      const Part pt = ctl.part[slot ? open_warp1 : 0][slot];
+      const unsigned c0 = ctl.chunk_of(pt.first), c1 = ctl.chunk_of(pt.first + pt.n - 1);
+      int* ticket = p.counters + kTickets + c0;
+      __threadfence();
+      last = atomicAdd(ticket, 1) == (int)(c1 - c0);
+      if (last) *ticket = 0;
+      __threadfence();
+      ctl.open[slot] = make_uint2(c0, c1 - c0 + 1);
+    }
+    ctl.last[slot] = last;
+  }
+  __syncthreads();
+  constexpr int kFit = W * S::kRingBytes / (S::kPartial * 4);          // states that fit the rings
+  constexpr int kMine = (kVec + S::kThreads - 1) / S::kThreads;        // float4s of a thread
+#pragma unroll 1
+  for (int slot = 0; slot < 2; ++slot) {
+    if (!ctl.last[slot]) continue;
+    const unsigned c0 = ctl.open[slot].x;
+    const int n = (int)ctl.open[slot].y;
+    float M[kMine], lsum[kMine];
+    float4 acc[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      M[i] = -1e30f;
+      lsum[i] = 0.0f;
+      acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll 1
+    for (int k0 = 0; k0 < n; k0 += kFit) {
+      const int m = min(kFit, n - k0);
+      // the states of m chunks, all on their way at once
+      for (int i = threadIdx.x; i < m * (S::kPartial / 4); i += S::kThreads) {
+        const int k = i / (S::kPartial / 4), at = i % (S::kPartial / 4);
+        // the first chunk's state is of a pair that goes on, the others' of one begun earlier
+        copy16_async(smem_u32(smem) + 16 * i,
+                     p.partials + ((size_t)(c0 + k0 + k) * 2 + (k0 + k == 0)) * S::kPartial + 4 * at);
+      }
+      copies_done();
+      __syncthreads();
+      const float* state = reinterpret_cast<const float*>(smem);
+#pragma unroll
       for (int i = 0; i < kMine; ++i) {
         const int at = threadIdx.x + i * S::kThreads, row = at / (D / 4);
         if (at >= kVec) break;
-        float M = -1e30f, lsum = 0.0f;
+        float top = M[i];
 #pragma unroll 4
-        for (int k = 0; k < members; ++k) M = fmaxf(M, stats[((w + k) * 2 + (k ? 0 : slot)) * S::kRows + row].x);
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < m; ++k) top = fmaxf(top, state[k * S::kPartial + S::kState + 2 * row]);
+        const float old = fast_exp2(M[i] - top);
+        M[i] = top;
+        lsum[i] *= old;
+        acc[i].x *= old; acc[i].y *= old; acc[i].z *= old; acc[i].w *= old;
 #pragma unroll 4
-        for (int k = 0; k < members; ++k) {
-          const float2 ml = stats[((w + k) * 2 + (k ? 0 : slot)) * S::kRows + row];
-          const float f = fast_exp2(ml.x - M);
-          const bool parked = (k || !slot) && (s_flags[w + k] & kParked0);
-          const float4* state = parked ? reinterpret_cast<const float4*>(p.parked + ((size_t)blockIdx.x * W + w + k) * S::kState)
-                                       : reinterpret_cast<const float4*>(smem + (w + k) * S::kRingBytes);
-          const float4 v = state[at];
-          lsum += f * ml.y;
-          acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-        }
-        if (whole) {
-          finish(s_part[w][1], at, acc, lsum);
-        } else {
-          __stcg(reinterpret_cast<float4*>(out) + at, acc);
-          if (at % (D / 4) == 0) __stcg(reinterpret_cast<float2*>(out + S::kState) + row, make_float2(M, lsum));
-        }
+        for (int k = 0; k < m; ++k)
+          add_state(top, lsum[i], acc[i], reinterpret_cast<const float2*>(state + k * S::kPartial + S::kState)[row],
+                    reinterpret_cast<const float4*>(state + k * S::kPartial)[at]);
       }
-      if (!whole) {
-        open |= 1 << slot;
-        if (slot) open_warp1 = w;
-      }
+      __syncthreads();   // the rings are used again
     }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int at = threadIdx.x + i * S::kThreads;
+      if (at < kVec) finish(ctl.part[slot ? open_warp1 : 0][slot], at, acc[i], lsum[i]);
+    }
+  }
+}
 
-    // ---- pairs that span chunks: the last CTA to arrive merges, in chunk order ----
-    __syncthreads();   // the partials are written (and the rings free again)
-    if (open) {
-      if (threadIdx.x < 2) {
-        const int slot = threadIdx.x;
-        bool last = false;
-        if (open >> slot & 1) {
-          const Part pt = s_part[slot ? open_warp1 : 0][slot];
-          const unsigned c0 = chunk_of(pt.first), c1 = chunk_of(pt.first + pt.n - 1);
-          __threadfence();
-          int* ticket = p.counters + kTickets + c0;
-          last = atomicAdd(ticket, 1) == (int)(c1 - c0);
-          if (last) *ticket = 0;
-          __threadfence();
+template <int D, int TYPE, int RT>
+__global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
+    gqa_decode_q8_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                         const __grid_constant__ Params p) {
+  using S = Shape<D, RT>;
+  constexpr int W = S::kWarps;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ Control ctl;
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t bar0 = smem_u32(smem + S::kBarOffset) + warp * S::kStages * 8;
+  if (lane == 0) {
+    for (int s = 0; s < S::kStages; ++s)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + 8 * s) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+  }
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncwarp();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int capacity = p.page_tokens * p.max_pages;   // <= 2^30
+  // ---- the row of all tiles: its length, its longest pair ----
+  const int pairs = p.Hkv * p.row_groups.d;   // of a sequence
+  {
+    unsigned sum = 0;
+    int longest = 0;
+    for (int b = lane; b < p.B; b += 32) {
+      const int n = tiles_of(p, b);
+      sum += n;
+      longest = max(longest, n);
+    }
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    const Plan plan = plan_of<W>(sum * pairs, longest, p.B * pairs, gridDim.x);
+    if (lane == 0) ctl.plan = plan;
+    __syncwarp();
+  }
+  uint32_t before = 0;   // tiles of earlier chunks: tile j's stage and parity follow from before + j
+  bool ok = true;
+  for (unsigned chunk = blockIdx.x;;) {
+    // ---- this warp's stretch: `count` tiles from `begin` on ----
+    unsigned begin = 0;
+    int count = 0;
+    int b_first = 0;           // the sequence of the first tile, and where its tiles start
+    unsigned base_first = 0;
+    if (ctl.plan.whole) {
+      if (chunk >= (unsigned)(p.B * pairs)) break;
+      b_first = chunk / pairs;
+      const int n = tiles_of(p, b_first), share = (n + W - 1) / W;
+      // any row's start will do: nothing refers to tiles of other sequences
+      begin = (chunk - b_first * pairs) * n + warp * share;
+      count = max(0, min(n - warp * share, share));
+    } else {
+      const unsigned from = ctl.chunk_at(chunk);
+      if (from >= ctl.plan.total) break;
+      const unsigned share = (chunk < gridDim.x ? ctl.plan.first : ctl.plan.rest) / W;
+      begin = from + warp * share;
+      count = begin < ctl.plan.total ? (int)min(share, ctl.plan.total - begin) : 0;
+      if (threadIdx.x == 0 && ctl.dealt()) ctl.next = gridDim.x + atomicAdd(p.counters, 1);
+      for (int b0 = 0; count > 0; b0 += 32) {
+        const unsigned mine = b0 + lane < p.B ? tiles_of(p, b0 + lane) * pairs : 0;
+        unsigned incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += up;
         }
-        s_last[slot] = last;
-      }
-      __syncthreads();
-#pragma unroll 1
-      for (int slot = 0; slot < 2; ++slot) {
-        if (!s_last[slot]) continue;
-        const Part pt = s_part[slot ? open_warp1 : 0][slot];
-        const unsigned c0 = chunk_of(pt.first);
-        const int n = (int)(chunk_of(pt.first + pt.n - 1) - c0) + 1;
-        // the first chunk's state is of a pair that goes on, the others' of one begun earlier
-        auto state_of = [&](int k) { return p.partials + ((size_t)(c0 + k) * 2 + (k == 0)) * S::kPartial; };
-        constexpr int kBatch = kMine > 1 ? 4 : 8;   // chunks whose states a thread loads at a time
-        float4 v[kMine][kBatch];
-        auto load = [&](int k0) {
-#pragma unroll
-          for (int k = 0; k < kBatch; ++k)
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-              const int at = threadIdx.x + i * S::kThreads;
-              if (k0 + k < n && at < kVec) v[i][k] = __ldcg(reinterpret_cast<const float4*>(state_of(k0 + k)) + at);
-            }
-        };
-        load(0);
-        // every chunk's (m, l), then the weights 2^(m - M) in their place: a warp a row
-        float2* ml = reinterpret_cast<float2*>(smem);   // [chunk][row], over the rings
-        for (int i = threadIdx.x; i < n * S::kRows; i += S::kThreads)
-          ml[i] = __ldcg(reinterpret_cast<const float2*>(state_of(i / S::kRows) + S::kState) + i % S::kRows);
-        __syncthreads();
-        for (int row = warp; row < S::kRows; row += W) {
-          float M = -1e30f, sum = 0.0f;
-          for (int k = lane; k < n; k += 32) M = fmaxf(M, ml[k * S::kRows + row].x);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-          for (int k = lane; k < n; k += 32) {
-            const float f = fast_exp2(ml[k * S::kRows + row].x - M);
-            ml[k * S::kRows + row].x = f;
-            sum += f * ml[k * S::kRows + row].y;
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          if (lane == 0) s_sum[row] = sum;
+        const uint32_t past = __ballot_sync(0xffffffffu, base_first + incl > begin);
+        if (past || b0 + 32 >= p.B) {   // some sequence holds it, as begin < total
+          const int l = past ? __ffs(past) - 1 : (p.B - 1) % 32;
+          b_first = b0 + l;
+          base_first += __shfl_sync(0xffffffffu, incl - mine, l);
+          break;
         }
-        __syncthreads();
-        float4 acc[kMine];
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 1
-        for (int k0 = 0;;) {
-#pragma unroll
-          for (int k = 0; k < kBatch; ++k)
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-              const int at = threadIdx.x + i * S::kThreads;
-              if (k0 + k < n && at < kVec) {
-                const float f = ml[(k0 + k) * S::kRows + at / (D / 4)].x;
-                acc[i].x += f * v[i][k].x; acc[i].y += f * v[i][k].y;
-                acc[i].z += f * v[i][k].z; acc[i].w += f * v[i][k].w;
-              }
-            }
-          k0 += kBatch;
-          if (k0 >= n) break;
-          load(k0);
-        }
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int at = threadIdx.x + i * S::kThreads;
-          if (at < kVec) finish(pt, at, acc[i], s_sum[at / (D / 4)]);
-        }
-        __syncthreads();   // the rings, s_sum and s_part are used again
+        base_first += __shfl_sync(0xffffffffu, incl, 31);
       }
     }
+    if (ok) ok = run_stretch<D, TYPE, RT>(mk, mv, p, smem, ctl, before, begin, count, b_first, base_first);
+    else if (threadIdx.x % 32 == 0) ctl.flags[warp] = 0;
+    before += count;
+    __syncthreads();
+
+    merge_chunk<D, RT>(p, smem, ctl, chunk);
     // the next chunk: the ring's generic reads and writes end before copies fill it again
-    if (s_plan.whole) {
+    if (ctl.plan.whole) {
       chunk += gridDim.x;
-    } else if (dealt()) {
-      chunk = s_next;
+    } else if (ctl.dealt()) {
+      chunk = ctl.next;
     } else {
       break;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
   }
-  if (threadIdx.x == 0 && dealt() && atomicAdd(p.counters + 1, 1) == (int)gridDim.x - 1) {
+  if (threadIdx.x == 0 && ctl.dealt() && atomicAdd(p.counters + 1, 1) == (int)gridDim.x - 1) {
     p.counters[0] = 0;   // the last CTA: nobody takes a chunk any more
     p.counters[1] = 0;
   }
@@ -1023,12 +1054,13 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   p.parked = p.partials + partial_floats(rt, D);
   p.dev_err = dev_err;
   p.B = B; p.Q = Q; p.Hq = Hq; p.Hkv = Hkv;
-  p.group = Hq / Hkv;
-  p.row_groups = (Q * p.group + 8 * rt - 1) / (8 * rt);
+  auto divisor = [](int d) { return Divisor{d, d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d)}; };
+  p.group = divisor(Hq / Hkv);
+  p.row_groups = divisor((Q * (Hq / Hkv) + 8 * rt - 1) / (8 * rt));
   p.page_tokens = page_tokens; p.max_pages = max_pages; p.num_pages = num_pages;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
   // as many CTAs as the device holds, but no more warps than the table has room for tiles
-  const double tiles = (double)B * Hkv * p.row_groups * ((double)max_pages * page_tokens / kTile + 1);
+  const double tiles = (double)B * Hkv * p.row_groups.d * ((double)max_pages * page_tokens / kTile + 1);
   const int ctas = (int)std::max(1.0, std::min((double)max_ctas(sms), std::ceil(tiles / warps)));
   if (tiles > (double)(1u << 31)) return ANVILQ_ESHAPE;   // tiles are counted in 32 bits
   CUtensorMap mk, mv;
