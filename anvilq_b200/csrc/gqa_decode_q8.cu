@@ -748,66 +748,71 @@ __device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem
       const Part pt = ctl.part[slot ? open_warp1 : 0][slot];
       const unsigned c0 = ctl.chunk_of(pt.first), c1 = ctl.chunk_of(pt.first + pt.n - 1);
       int* ticket = p.counters + kTickets + c0;
-      __threadfence();
-      last = atomicAdd(ticket, 1) == (int)(c1 - c0);
+      // releases the CTA's partials (through the barrier above) and acquires the others'
+      int arrived;
+      asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(arrived) : "l"(ticket) : "memory");
+      last = arrived == (int)(c1 - c0);
       if (last) *ticket = 0;
-      __threadfence();
       ctl.open[slot] = make_uint2(c0, c1 - c0 + 1);
     }
     ctl.last[slot] = last;
   }
   __syncthreads();
-  constexpr int kFit = W * S::kRingBytes / (S::kPartial * 4);          // states that fit the rings
-  constexpr int kMine = (kVec + S::kThreads - 1) / S::kThreads;        // float4s of a thread
+  // Both merges at once where there are two, each by half of the warps with half
+  // of the rings: their time is latency.
+  const int both = ctl.last[0] + ctl.last[1];
+  if (!both) return;
+  static_assert(W % 2 == 0, "two halves");
+  const int threads = both == 2 ? S::kThreads / 2 : S::kThreads;
+  const int slot = both == 2 ? (int)threadIdx.x / threads : ctl.last[1], me = both == 2 ? threadIdx.x % threads : threadIdx.x;
+  unsigned char* room = smem + (both == 2 ? slot * (W / 2) * S::kRingBytes : 0);
+  constexpr int kFit = W / 2 * S::kRingBytes / (S::kPartial * 4);         // states that fit half of the rings
+  constexpr int kMine = (2 * kVec + S::kThreads - 1) / S::kThreads;       // float4s of a thread, at most
+  auto sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(threads) : "memory"); };
+  const unsigned c0 = ctl.open[slot].x;
+  const int n = (int)ctl.open[slot].y;
+  float M[kMine], lsum[kMine];
+  float4 acc[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    M[i] = -1e30f;
+    lsum[i] = 0.0f;
+    acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
 #pragma unroll 1
-  for (int slot = 0; slot < 2; ++slot) {
-    if (!ctl.last[slot]) continue;
-    const unsigned c0 = ctl.open[slot].x;
-    const int n = (int)ctl.open[slot].y;
-    float M[kMine], lsum[kMine];
-    float4 acc[kMine];
+  for (int k0 = 0; k0 < n; k0 += kFit) {
+    const int m = min(kFit, n - k0);
+    // the states of m chunks, all on their way at once
+    for (int i = me; i < m * (S::kPartial / 4); i += threads) {
+      const int k = i / (S::kPartial / 4), at = i % (S::kPartial / 4);
+      // the first chunk's state is of a pair that goes on, the others' of one begun earlier
+      copy16_async(smem_u32(room) + 16 * i, p.partials + ((size_t)(c0 + k0 + k) * 2 + (k0 + k == 0)) * S::kPartial + 4 * at);
+    }
+    copies_done();
+    sync();
+    const float* state = reinterpret_cast<const float*>(room);
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      M[i] = -1e30f;
-      lsum[i] = 0.0f;
-      acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-#pragma unroll 1
-    for (int k0 = 0; k0 < n; k0 += kFit) {
-      const int m = min(kFit, n - k0);
-      // the states of m chunks, all on their way at once
-      for (int i = threadIdx.x; i < m * (S::kPartial / 4); i += S::kThreads) {
-        const int k = i / (S::kPartial / 4), at = i % (S::kPartial / 4);
-        // the first chunk's state is of a pair that goes on, the others' of one begun earlier
-        copy16_async(smem_u32(smem) + 16 * i,
-                     p.partials + ((size_t)(c0 + k0 + k) * 2 + (k0 + k == 0)) * S::kPartial + 4 * at);
-      }
-      copies_done();
-      __syncthreads();
-      const float* state = reinterpret_cast<const float*>(smem);
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int at = threadIdx.x + i * S::kThreads, row = at / (D / 4);
-        if (at >= kVec) break;
-        float top = M[i];
+      const int at = me + i * threads, row = at / (D / 4);
+      if (at >= kVec) break;
+      float top = M[i];
 #pragma unroll 4
-        for (int k = 0; k < m; ++k) top = fmaxf(top, state[k * S::kPartial + S::kState + 2 * row]);
-        const float old = fast_exp2(M[i] - top);
-        M[i] = top;
-        lsum[i] *= old;
-        acc[i].x *= old; acc[i].y *= old; acc[i].z *= old; acc[i].w *= old;
+      for (int k = 0; k < m; ++k) top = fmaxf(top, state[k * S::kPartial + S::kState + 2 * row]);
+      const float old = fast_exp2(M[i] - top);
+      M[i] = top;
+      lsum[i] *= old;
+      acc[i].x *= old; acc[i].y *= old; acc[i].z *= old; acc[i].w *= old;
 #pragma unroll 4
-        for (int k = 0; k < m; ++k)
-          add_state(top, lsum[i], acc[i], reinterpret_cast<const float2*>(state + k * S::kPartial + S::kState)[row],
-                    reinterpret_cast<const float4*>(state + k * S::kPartial)[at]);
-      }
-      __syncthreads();   // the rings are used again
+      for (int k = 0; k < m; ++k)
+        add_state(top, lsum[i], acc[i], reinterpret_cast<const float2*>(state + k * S::kPartial + S::kState)[row],
+                  reinterpret_cast<const float4*>(state + k * S::kPartial)[at]);
     }
+    if (k0 + kFit < n) sync();   // the room is used again
+  }
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int at = threadIdx.x + i * S::kThreads;
-      if (at < kVec) finish(ctl.part[slot ? open_warp1 : 0][slot], at, acc[i], lsum[i]);
-    }
+  for (int i = 0; i < kMine; ++i) {
+    const int at = me + i * threads;
+    if (at < kVec) finish(ctl.part[slot ? open_warp1 : 0][slot], at, acc[i], lsum[i]);
   }
 }
 

@@ -20,7 +20,12 @@ _outgrown = []         # workspaces that larger ones replaced: captured graphs m
 _lock = threading.Lock()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the handle without a Stream object around it
+
+
 def _stream_ptr(device):
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -601,10 +606,12 @@ def _call(name, device, *args):
     """A library call with `device` current (a stream only takes launches of its own device)."""
     fn = getattr(_lib.load(), name)
     if torch.cuda.current_device() == device.index:
-        _lib.check(fn(*args), name)
+        rc = fn(*args)
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args), name)
+            rc = fn(*args)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _call_workspace(device, nbytes: int, given) -> torch.Tensor:
@@ -620,7 +627,8 @@ def _call_workspace(device, nbytes: int, given) -> torch.Tensor:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         ws[:WORKSPACE_COUNTER_BYTES].zero_()
         return ws
-    return workspace(device, nbytes)
+    ws = _workspaces.get((device.index, _stream_ptr(device)))
+    return ws if ws is not None and ws.numel() >= nbytes else workspace(device, nbytes)
 
 
 WORKSPACE_COUNTER_BYTES = 65536
@@ -633,56 +641,61 @@ def _error_word(device, given):
         if given.dtype != torch.int32 or given.numel() < 1 or given.device != device:
             raise ValueError(f"dev_err must be an int32 tensor on {device}")
         return given
-    if device.index not in _dev_err and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("run an operation on this device once before capturing a graph")
-    return device_error_word(device)
+    w = _dev_err.get(device.index)
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("run an operation on this device once before capturing a graph")
+        w = device_error_word(device)
+    return w
 
 
 def _check_table(name, page_table, seqlens, B=None):
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+    shape = page_table.shape
+    if page_table.dtype != torch.int32 or len(shape) != 2 or not page_table.is_contiguous():
         raise ValueError(f"{name}: page_table must be a contiguous int32 tensor [B, max_pages]")
-    B = page_table.shape[0] if B is None else B
-    if page_table.shape[0] != B:
-        raise ValueError(f"{name}: page_table has {page_table.shape[0]} rows for {B} sequences")
-    if seqlens.dtype != torch.int32 or tuple(seqlens.shape) != (B,) or not seqlens.is_contiguous():
+    B = shape[0] if B is None else B
+    if shape[0] != B:
+        raise ValueError(f"{name}: page_table has {shape[0]} rows for {B} sequences")
+    if seqlens.dtype != torch.int32 or seqlens.shape != (B,) or not seqlens.is_contiguous():
         raise ValueError(f"{name}: seqlens must be a contiguous int32 tensor [{B}]")
-    return B, page_table.shape[1]
+    return B, shape[1]
 
 
 def _check_q8(name, k_codes, v_codes, k_scales, v_scales):
     """(pages, heads, page tokens, D, code type) of a pair of 8-bit pools."""
-    if k_codes.dtype not in (torch.int8, torch.float8_e4m3fn) or v_codes.dtype != k_codes.dtype:
+    kind, shape = k_codes.dtype, k_codes.shape
+    if (kind != torch.int8 and kind != torch.float8_e4m3fn) or v_codes.dtype != kind:
         raise TypeError(f"{name}: codes must both be int8 or both float8_e4m3fn")
-    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
+    if len(shape) != 4 or v_codes.shape != shape:
         raise ValueError(f"{name}: k_codes/v_codes [num_pages, Hkv, page_tokens, D]")
-    pages, Hkv, page, D = k_codes.shape
+    pages, Hkv, page, D = shape
     if page % _lib.KV_Q8_BLOCK:
         raise ValueError(f"{name}: pages must hold a multiple of {_lib.KV_Q8_BLOCK} tokens")
-    for t in (k_scales, v_scales):
-        if t.dtype != torch.float32 or tuple(t.shape) != (pages, Hkv, page // _lib.KV_Q8_BLOCK):
-            raise ValueError(f"{name}: scales must be float32 [{pages}, {Hkv}, {page // _lib.KV_Q8_BLOCK}]")
-    for t in (k_codes, v_codes, k_scales, v_scales):
-        if not t.is_contiguous():
-            raise ValueError(f"{name}: pools must be contiguous")
-    _on_device(name, k_codes.device, v_codes, k_scales, v_scales)
-    return pages, Hkv, page, D, _lib.KV_Q8_INT8 if k_codes.dtype == torch.int8 else _lib.KV_Q8_E4M3
+    blocks = (pages, Hkv, page // _lib.KV_Q8_BLOCK)
+    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.shape != blocks or \
+            v_scales.shape != blocks:
+        raise ValueError(f"{name}: scales must be float32 {list(blocks)}")
+    if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_scales.is_contiguous()
+            and v_scales.is_contiguous()):
+        raise ValueError(f"{name}: pools must be contiguous")
+    return pages, Hkv, page, D, _lib.KV_Q8_INT8 if kind == torch.int8 else _lib.KV_Q8_E4M3
 
 
 def _check_append(name, qkv, Hq, Hkv, D, page_table, seqlens, token_starts, q_out):
     B, max_pages = _check_table(name, page_table, seqlens)
     if qkv.dtype != torch.float16 or qkv.dim() != 2 or qkv.shape[1] != (Hq + 2 * Hkv) * D:
         raise ValueError(f"{name}: qkv must be float16 [T, {(Hq + 2 * Hkv) * D}]")
-    if qkv.stride(1) != 1 or (qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]):
+    T, width = qkv.shape
+    stride, inner = qkv.stride()
+    if inner != 1 or (T > 1 and stride < width):
         raise ValueError(f"{name}: rows of qkv must be contiguous and must not overlap")
-    if token_starts.dtype != torch.int32 or tuple(token_starts.shape) != (B + 1,) or not token_starts.is_contiguous():
+    if token_starts.dtype != torch.int32 or token_starts.shape != (B + 1,) or not token_starts.is_contiguous():
         raise ValueError(f"{name}: token_starts must be a contiguous int32 tensor [{B + 1}]")
-    T = qkv.shape[0]
     if q_out is None:
         q_out = torch.empty((T, Hq, D), dtype=torch.float16, device=qkv.device)
-    elif q_out.dtype != torch.float16 or tuple(q_out.shape) != (T, Hq, D) or not q_out.is_contiguous():
+    elif q_out.dtype != torch.float16 or q_out.shape != (T, Hq, D) or not q_out.is_contiguous():
         raise ValueError(f"{name}: q_out must be contiguous float16 [{T}, {Hq}, {D}]")
-    _on_device(name, qkv.device, page_table, seqlens, token_starts, q_out)
-    return T, B, max_pages, (qkv.stride(0) if T > 1 else qkv.shape[1]), q_out
+    return T, B, max_pages, (stride if T > 1 else width), q_out
 
 
 def paged_kv_append(qkv, k_pool, v_pool, page_table, seqlens, token_starts, Hq: int, theta: float = 1e6, q_out=None,
@@ -706,7 +719,7 @@ def paged_kv_append(qkv, k_pool, v_pool, page_table, seqlens, token_starts, Hq: 
     pages, page, Hkv, D = k_pool.shape
     T, B, max_pages, stride, q_out = _check_append(name, qkv, Hq, Hkv, D, page_table, seqlens, token_starts, q_out)
     dev = qkv.device
-    _on_device(name, dev, k_pool, v_pool)
+    _on_device(name, dev, k_pool, v_pool, page_table, seqlens, token_starts, q_out)
     err = _error_word(dev, dev_err)
     _call("anvilq_paged_kv_append", dev, _ptr(qkv), stride, _ptr(token_starts), _ptr(seqlens), _ptr(page_table),
           _ptr(q_out), _ptr(k_pool), _ptr(v_pool), T, B, Hq, Hkv, D, page, max_pages, pages, float(theta), _ptr(err),
@@ -727,7 +740,7 @@ def paged_kv_append_q8(qkv, k_codes, v_codes, k_scales, v_scales, page_table, se
     pages, Hkv, page, D, code = _check_q8(name, k_codes, v_codes, k_scales, v_scales)
     T, B, max_pages, stride, q_out = _check_append(name, qkv, Hq, Hkv, D, page_table, seqlens, token_starts, q_out)
     dev = qkv.device
-    _on_device(name, dev, k_codes)
+    _on_device(name, dev, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, token_starts, q_out)
     err = _error_word(dev, dev_err)
     _call("anvilq_paged_kv_append_q8", dev, _ptr(qkv), stride, _ptr(token_starts), _ptr(seqlens), _ptr(page_table),
           _ptr(q_out), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), code, T, B, Hq, Hkv, D, page,
@@ -745,7 +758,7 @@ def kv_q8_values(k_codes, v_codes, k_scales, v_scales, k_out=None, v_out=None, o
     for t in (k_out, v_out):
         if t.dtype != torch.float16 or t.shape != k_codes.shape or not t.is_contiguous():
             raise ValueError(f"{name}: k_out/v_out must be contiguous float16 with the shape of the codes")
-    _on_device(name, dev, k_out, v_out)
+    _on_device(name, dev, v_codes, k_scales, v_scales, k_out, v_out)
     _call("anvilq_kv_q8_values", dev, _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), code, _ptr(k_out),
           _ptr(v_out), pages, Hkv, page, D, GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return k_out, v_out
@@ -775,7 +788,7 @@ def gqa_decode_q8(q, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, 
     elif out.dtype != torch.float16 or out.shape != q.shape or not out.is_contiguous():
         raise ValueError(f"{name}: out must be contiguous float16 in q's shape")
     dev = q.device
-    _on_device(name, dev, k_codes, page_table, seqlens, out)
+    _on_device(name, dev, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, out)
     need = _lib.load().anvilq_gqa_decode_q8_workspace_size(B, Q, Hq, Hkv, D)
     if need == 0:
         raise ValueError(f"{name}: unsupported shape B={B} Q={Q} Hq={Hq} Hkv={Hkv} D={D}")
@@ -808,35 +821,45 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
     The choice is the reference's greedy one, lowest index on ties
     (anvil-q4/tests/transformer_reference.py:212-217)."""
     name = "logits_process"
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.float16):
+    half = logits.dtype == torch.float16
+    if logits.dim() != 2 or not (half or logits.dtype == torch.float32):
         raise ValueError(f"{name}: logits must be float32 or float16 [B, V]")
     B, V = logits.shape
-    if B < 1 or V < 1 or logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
+    pitch, inner = logits.stride()
+    if B < 1 or V < 1 or inner != 1 or (B > 1 and pitch < V):
         raise ValueError(f"{name}: rows of logits must be contiguous and must not overlap")
     if not write_logits and not choose:
         raise ValueError(f"{name}: nothing to compute")
+    dev = logits.device
 
-    def rows(t, dtype, what, n=B):
-        if t is not None and (t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous()):
+    def rows(t, dtype, what, n):
+        if t is not None and (t.dtype != dtype or t.shape != (n,) or not t.is_contiguous()):
             raise ValueError(f"{name}: {what} must be contiguous {dtype} [{n}]")
 
-    L = 0
+    def matrix(t, dtype, n, cols, what):   # rows of at least `cols`, contiguous, apart; their distance
+        if t.dtype != dtype or t.dim() != 2 or (n is not None and t.shape[0] != n) or t.shape[1] < cols:
+            raise ValueError(f"{name}: {what} must be {dtype} [{'masks' if n is None else n}, {cols}]")
+        apart, inner = t.stride()
+        if (inner != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and apart < cols):
+            raise ValueError(f"{name}: rows of {what} must be contiguous and must not overlap")
+        return apart if t.shape[0] > 1 else t.shape[1]
+
+    L = history_pitch = 0
     if history is not None:
-        if history.dtype != torch.int32 or history.dim() != 2 or history.shape[0] != B or \
-                (history.shape[1] > 1 and history.stride(1) != 1):
-            raise ValueError(f"{name}: history must be int32 [{B}, L] with contiguous rows")
         if history_lens is None:
             raise ValueError(f"{name}: history needs history_lens")
+        history_pitch = matrix(history, torch.int32, B, 0, "history")
         L = history.shape[1]
-        if B > 1 and history.stride(0) < L:
+        if B > 1 and history_pitch < L:
             raise ValueError(f"{name}: rows of history must not overlap")
-    elif any(t is not None for t in (history_lens, prompt_lens, repetition, presence, frequency)):
+    elif history_lens is not None or prompt_lens is not None or repetition is not None or presence is not None or \
+            frequency is not None:
         raise ValueError(f"{name}: penalties and lengths need a history")
-    rows(history_lens, torch.int32, "history_lens")
-    rows(prompt_lens, torch.int32, "prompt_lens")
-    rows(repetition, torch.float32, "repetition")
-    rows(presence, torch.float32, "presence")
-    rows(frequency, torch.float32, "frequency")
+    rows(history_lens, torch.int32, "history_lens", B)
+    rows(prompt_lens, torch.int32, "prompt_lens", B)
+    rows(repetition, torch.float32, "repetition", B)
+    rows(presence, torch.float32, "presence", B)
+    rows(frequency, torch.float32, "frequency", B)
     if L == 0:
         history = None       # no tokens: nothing to penalise
         history_lens = prompt_lens = repetition = presence = frequency = None
@@ -844,34 +867,31 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
     if bias_starts is not None:
         if bias_ids is None or bias_values is None:
             raise ValueError(f"{name}: bias_starts needs bias_ids and bias_values")
-        n_bias = bias_ids.numel()
+        n_bias = bias_ids.shape[0] if bias_ids.dim() == 1 else -1
         rows(bias_starts, torch.int32, "bias_starts", B + 1)
         rows(bias_ids, torch.int32, "bias_ids", n_bias)
         rows(bias_values, torch.float32, "bias_values", n_bias)
     elif bias_ids is not None or bias_values is not None:
         raise ValueError(f"{name}: a bias list needs bias_starts")
-    masks = 0
+    masks = mask_pitch = 0
     if allowed is not None:
-        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[1] < (V + 31) // 32 or \
-                (allowed.shape[1] > 1 and allowed.stride(1) != 1):
-            raise ValueError(f"{name}: allowed must be int32 [masks, {(V + 31) // 32}] with contiguous rows")
+        mask_pitch = matrix(allowed, torch.int32, None, (V + 31) // 32, "allowed")
         masks = allowed.shape[0]
-        if masks > 1 and allowed.stride(0) < (V + 31) // 32:
-            raise ValueError(f"{name}: rows of allowed must not overlap")
         if allowed_rows is None and masks != B:
             raise ValueError(f"{name}: one mask a row, or allowed_rows")
-        rows(allowed_rows, torch.int32, "allowed_rows")
+        rows(allowed_rows, torch.int32, "allowed_rows", B)
     elif allowed_rows is not None:
         raise ValueError(f"{name}: allowed_rows needs allowed")
-    dev = logits.device
+    out_pitch = V
     if not write_logits:
         if out is not None:
             raise ValueError(f"{name}: out is not written without write_logits")
     elif out is None:
         out = torch.empty((B, V), dtype=torch.float32, device=dev)
-    elif out.dtype != torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or \
-            (B > 1 and out.stride(0) < V):
-        raise ValueError(f"{name}: out must be float32 [{B}, {V}] with contiguous rows")
+    else:
+        out_pitch = matrix(out, torch.float32, B, V, "out")
+        if out.shape[1] != V:
+            raise ValueError(f"{name}: out must be float32 [{B}, {V}]")
     tokens = torch.empty(B, dtype=torch.int32, device=dev) if choose else None
     _on_device(name, dev, history, history_lens, prompt_lens, repetition, presence, frequency, bias_starts, bias_ids,
                bias_values, allowed, allowed_rows, out)
@@ -880,11 +900,9 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
         raise ValueError(f"{name}: unsupported shape B={B} V={V}")
     ws = _call_workspace(dev, need, workspace) if choose else None
     err = _error_word(dev, dev_err)
-    pitch = lambda t, n: 0 if t is None else t.stride(0) if t.shape[0] > 1 else n
-    _call("anvilq_logits_process", dev, _ptr(logits), 1 if logits.dtype == torch.float16 else 0, pitch(logits, V),
-          _ptr(out), pitch(out, V), _ptr(tokens), B, V, _ptr(history), pitch(history, L), _ptr(history_lens),
-          _ptr(prompt_lens), L, _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_starts), _ptr(bias_ids),
-          _ptr(bias_values), n_bias, _ptr(allowed), pitch(allowed, (V + 31) // 32), _ptr(allowed_rows), masks,
-          _ptr(ws), 0 if ws is None else ws.numel(), _ptr(err), GEMM_OVERLAP_PRIOR if overlap_prior else 0,
-          _stream_ptr(dev))
+    _call("anvilq_logits_process", dev, _ptr(logits), half, pitch if B > 1 else V, _ptr(out), out_pitch, _ptr(tokens),
+          B, V, _ptr(history), history_pitch, _ptr(history_lens), _ptr(prompt_lens), L, _ptr(repetition),
+          _ptr(presence), _ptr(frequency), _ptr(bias_starts), _ptr(bias_ids), _ptr(bias_values), n_bias, _ptr(allowed),
+          mask_pitch, _ptr(allowed_rows), masks, _ptr(ws), 0 if ws is None else ws.numel(), _ptr(err),
+          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return out, tokens
