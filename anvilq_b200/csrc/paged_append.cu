@@ -22,9 +22,12 @@
 //
 // Work split: an item is the run of new rows of one sequence inside one block of
 // 16 positions (the unit of a scale; it never leaves a page), and a slice of the
-// heads.  A CTA computes the item's cosines and sines once, into shared memory;
-// its warps then take heads.  A lane holds 8 consecutive dims of both halves of a
-// row, 16-byte loads and stores.
+// heads.  A CTA computes the item's cosines and sines once, into shared memory.
+// Rows that are copied or rotated into binary16 are then dealt to the threads in
+// the order of memory, 8 consecutive dims of both halves of a head a thread; a
+// block that is coded needs its largest value first, so a warp takes all of a
+// head's rows, keeps them as they came (binary16) and rotates them twice, which
+// costs fewer registers than it saves time to keep them rotated.
 #include <algorithm>
 #include <cmath>
 
@@ -65,38 +68,40 @@ struct Item {
   int b, row, pos, count;
 };
 
-// The largest b in [0, n) with key(b) <= x, for a non-decreasing key with
-// key(0) <= x (else 0): the whole warp, 32 probes a step.
-template <typename Key>
-__device__ __forceinline__ int warp_search(int n, int x, Key key) {
-  const int lane = threadIdx.x % 32;
-  int lo = 0, span = n;
-  while (span > 1) {
-    const int step = (span + 31) / 32;
-    const int at = lo + lane * step;
-    const bool le = lane * step < span && key(at) <= x;
-    const uint32_t hit = __ballot_sync(0xffffffffu, le);
-    const int k = hit ? 31 - __clz(hit) : 0;
-    span = min(step, span - k * step);
-    lo += k * step;
-  }
-  return lo;
-}
-
 // Two ways to number the items without a pass over the batch, the host taking
 // the one with fewer numbers (a number without an item ends its CTA):
 //   by token: number t names the item whose first row is t, if t is one;
 //   by place: sequence b's items follow from starts[b] / 16 + 2 b on (its n rows
 //             lie in at most n / 16 + 2 blocks, so the ranges are disjoint).
+// The whole warp looks for the largest b with key(b) <= number, key non-decreasing:
+// 32 probes a step, and with the last step's probes come every candidate's lengths.
 __device__ __forceinline__ Item find_item(const Params& p, int number) {
-  Item none{0, 0, 0, 0};
-  const int b = p.by_token ? warp_search(p.B, number, [&](int i) { return p.starts[i]; })
-                           : warp_search(p.B, number, [&](int i) { return p.starts[i] / kBlock + 2 * i; });
-  const int s0 = p.starts[b], s1 = p.starts[b + 1], len = p.seqlens[b];
+  const int lane = threadIdx.x % 32;
+  const Item none{0, 0, 0, 0};
+  int lo = 0, span = p.B;
+  while (span > 31) {
+    const int step = (span + 31) / 32, at = lane * step;
+    bool le = false;
+    if (at < span) {
+      const int s = p.starts[lo + at];
+      le = (p.by_token ? s : s / kBlock + 2 * (lo + at)) <= number;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, le);
+    const int k = hit ? 31 - __clz(hit) : 0;
+    lo += k * step;
+    span = min(step, span - k * step);
+  }
+  const int mine = lane <= span ? p.starts[lo + lane] : 0;   // span <= 31: the end of the last one too
+  const int my_len = lane < span ? p.seqlens[lo + lane] : 0;
+  const bool le = lane < span && (p.by_token ? mine : mine / kBlock + 2 * (lo + lane)) <= number;
+  const uint32_t hit = __ballot_sync(0xffffffffu, le);
+  const int k = hit ? 31 - __clz(hit) : 0, b = lo + k;
+  const int s0 = __shfl_sync(0xffffffffu, mine, k), s1 = __shfl_sync(0xffffffffu, mine, k + 1);
+  const int len = __shfl_sync(0xffffffffu, my_len, k);
   if (s1 <= s0) return none;
   const long long first = (long long)len - ((long long)s1 - s0);   // position of row s0
   if (s0 < 0 || s1 > p.T || first < 0 || len > (long long)p.page_tokens * p.max_pages) {
-    if (threadIdx.x == 0 && p.dev_err) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+    if (threadIdx.x == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
     return none;
   }
   const int p0 = (int)first;
@@ -106,9 +111,9 @@ __device__ __forceinline__ Item find_item(const Params& p, int number) {
     pos = p0 + (number - s0);
     if (number != s0 && pos % kBlock) return none;
   } else {
-    const int k = number - (s0 / kBlock + 2 * b);
-    const int block = p0 / kBlock + k;
-    if (k < 0 || block > (len - 1) / kBlock) return none;
+    const int nth = number - (s0 / kBlock + 2 * b);
+    const int block = p0 / kBlock + nth;
+    if (nth < 0 || block > (len - 1) / kBlock) return none;
     pos = max(p0, block * kBlock);
   }
   return Item{b, s0 + (pos - p0), pos, min(len, (pos / kBlock + 1) * kBlock) - pos};
@@ -131,149 +136,177 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
   return w;
 }
 
+// 8 dims of both halves of a row, rotated: (a, b) -> (a cos - b sin, b cos + a sin)
+__device__ __forceinline__ void rotate8(float* a, float* b, const float* co, const float* si) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 4) {
+    const float4 c4 = *reinterpret_cast<const float4*>(co + e), s4 = *reinterpret_cast<const float4*>(si + e);
+    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float u = a[e + k], v = b[e + k];
+      a[e + k] = __fsub_rn(__fmul_rn(u, c[k]), __fmul_rn(v, s[k]));
+      b[e + k] = __fadd_rn(__fmul_rn(v, c[k]), __fmul_rn(u, s[k]));
+    }
+  }
+}
+
 template <int D, int TYPE>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ Params p,
-                                                          const __grid_constant__ Freq freq) {
+__global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 4 : 3)
+    append_kernel(const __grid_constant__ Params p, const __grid_constant__ Freq freq) {
   constexpr int kHalf = D / 2;
-  constexpr int kLanes = D / 16;              // lanes of a row: 8 dims of each half a lane
-  constexpr int kRows = 32 / kLanes;          // rows of a pass of a warp
-  constexpr int kPasses = kBlock / kRows;
+  constexpr int kLanes = D / 16;              // threads of a row: 8 dims of each half a thread
   __shared__ __align__(16) float s_cos[kBlock][kHalf];
   __shared__ __align__(16) float s_sin[kBlock][kHalf];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Item it = find_item(p, blockIdx.x);
   if (it.count <= 0) return;   // the same for the whole CTA
-  const int logical = it.pos / p.page_tokens;
-  const int page = q8::page_of(p.page_table, p.max_pages, p.num_pages, it.b, logical);
-  if (page < 0) {
-    if (threadIdx.x == 0 && p.dev_err) atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
-    return;
-  }
+  const int page = q8::page_of(p.page_table, p.max_pages, p.num_pages, it.b, it.pos / p.page_tokens);
   for (int i = threadIdx.x; i < it.count * kHalf; i += kThreads) {
     const int r = i / kHalf, pair = i % kHalf;
     const float angle = (float)((double)(it.pos + r) * freq.inv[pair]);
     sincosf(angle, &s_sin[r][pair], &s_cos[r][pair]);
   }
+  if (page < 0) {
+    if (threadIdx.x == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
+    return;
+  }
   __syncthreads();
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int d0 = 8 * (lane % kLanes);
-  const int heads = p.Hq + 2 * p.Hkv;
-  const int head_end = min(heads, (int)(blockIdx.y + 1) * p.heads_per_cta);
   const int slot = it.pos % p.page_tokens;    // row of the page of the item's first token
-  for (int head = blockIdx.y * p.heads_per_cta + warp; head < head_end; head += kWarps) {
-    uint4 lo[kPasses], hi[kPasses];
+  const int heads = p.Hq + 2 * p.Hkv;
+  const int head0 = blockIdx.y * p.heads_per_cta, head1 = min(heads, head0 + p.heads_per_cta);
+
+  // ---- rows into binary16: q, and with binary16 pages k and v ----
+  const int end16 = TYPE == kBinary16 ? head1 : min(head1, p.Hq);
+  if (head0 < end16) {
+    const int per_row = (end16 - head0) * kLanes, total = it.count * per_row;
+    const __half* src = p.qkv + (size_t)it.row * p.stride + head0 * D;
+    constexpr int kAhead = 2;   // pieces a thread loads at a time
+#pragma unroll 1
+    for (int i = threadIdx.x; i < total; i += kAhead * kThreads) {
+      uint4 lo[kAhead], hi[kAhead];
+      int row[kAhead], at[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int x = i + k * kThreads;
+        row[k] = x / per_row;
+        at[k] = x - row[k] * per_row;
+        if (x < total) {
+          const __half* s = src + (size_t)row[k] * p.stride + (at[k] / kLanes) * D + 8 * (at[k] % kLanes);
+          lo[k] = *reinterpret_cast<const uint4*>(s);
+          hi[k] = *reinterpret_cast<const uint4*>(s + kHalf);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (i + k * kThreads >= total) break;
+        const int head = head0 + at[k] / kLanes, d0 = 8 * (at[k] % kLanes);
+        if (TYPE != kBinary16 || head < p.Hq + p.Hkv) {
+          float a[8], b[8];
+          unpack8(lo[k], a);
+          unpack8(hi[k], b);
+          rotate8(a, b, s_cos[row[k]] + d0, s_sin[row[k]] + d0);
+          lo[k] = pack8(a);
+          hi[k] = pack8(b);
+        }
+        __half* dst;
+        if (TYPE != kBinary16 || head < p.Hq) {
+          dst = p.q_out + ((size_t)(it.row + row[k]) * p.Hq + head) * D + d0;
+        } else {
+          const int kvh = head - p.Hq < p.Hkv ? head - p.Hq : head - p.Hq - p.Hkv;
+          dst = static_cast<__half*>(kvh == head - p.Hq ? p.k : p.v) +
+                (((size_t)page * p.page_tokens + slot + row[k]) * p.Hkv + kvh) * D + d0;
+        }
+        *reinterpret_cast<uint4*>(dst) = lo[k];
+        *reinterpret_cast<uint4*>(dst + kHalf) = hi[k];
+      }
+    }
+  }
+  if (TYPE == kBinary16) return;
+
+  // ---- blocks into codes ----
+  constexpr int kCode = TYPE == q8::kE4m3 ? q8::kE4m3 : q8::kInt8;
+  constexpr int kRows = 32 / kLanes;          // rows of a pass of a warp
+  constexpr int kPasses = kBlock / kRows;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r0 = lane / kLanes, d0 = 8 * (lane % kLanes);
+#pragma unroll 1
+  for (int head = max(head0, p.Hq) + warp; head < head1; head += kWarps) {
+    const bool is_k = head < p.Hq + p.Hkv;
+    const int kvh = head - p.Hq - (is_k ? 0 : p.Hkv);
+    uint4 raw[kPasses][2];
+    const __half* src = p.qkv + (size_t)(it.row + r0) * p.stride + head * D + d0;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const int r = i * kRows + lane / kLanes;
-      lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
-      if (r < it.count) {
-        const __half* src = p.qkv + (size_t)(it.row + r) * p.stride + head * D + d0;
-        lo[i] = *reinterpret_cast<const uint4*>(src);
-        hi[i] = *reinterpret_cast<const uint4*>(src + kHalf);
+      raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+      if (i * kRows + r0 < it.count) {
+        raw[i][0] = *reinterpret_cast<const uint4*>(src + (size_t)i * kRows * p.stride);
+        raw[i][1] = *reinterpret_cast<const uint4*>(src + (size_t)i * kRows * p.stride + kHalf);
       }
     }
-    const bool is_q = head < p.Hq, turned = head < p.Hq + p.Hkv;
-    const int kvh = is_q ? 0 : (head - p.Hq) % p.Hkv;
-    float x[kPasses][16];
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int r = i * kRows + lane / kLanes;
-      float a[8], b[8];
-      unpack8(lo[i], a);
-      unpack8(hi[i], b);
-      if (turned && r < it.count) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float co = s_cos[r][d0 + e], si = s_sin[r][d0 + e];
-          x[i][e] = __fsub_rn(__fmul_rn(a[e], co), __fmul_rn(b[e], si));
-          x[i][8 + e] = __fadd_rn(__fmul_rn(b[e], co), __fmul_rn(a[e], si));
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[i][e] = a[e];
-          x[i][8 + e] = b[e];
-        }
-      }
-    }
-    if (is_q || TYPE == kBinary16) {
-      __half* dst;
-      size_t step;   // from a token to the next
-      if (is_q) {
-        dst = p.q_out + ((size_t)it.row * p.Hq + head) * D;
-        step = (size_t)p.Hq * D;
-      } else {
-        dst = static_cast<__half*>(turned ? p.k : p.v) + (((size_t)page * p.page_tokens + slot) * p.Hkv + kvh) * D;
-        step = (size_t)p.Hkv * D;
-      }
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int r = i * kRows + lane / kLanes;
-        if (r < it.count) {
-          *reinterpret_cast<uint4*>(dst + r * step + d0) = pack8(x[i]);
-          *reinterpret_cast<uint4*>(dst + r * step + d0 + kHalf) = pack8(x[i] + 8);
-        }
-      }
-      continue;
-    }
-    // 8-bit pages
-    float top = 0.0f;
+    // values of pass i, 0 where they are not finite (those have no code, and are reported)
     bool odd = false;
+    auto values = [&](int i, float* x) {
+      unpack8(raw[i][0], x);
+      unpack8(raw[i][1], x + 8);
+      if (is_k && i * kRows + r0 < it.count) rotate8(x, x + 8, s_cos[i * kRows + r0] + d0, s_sin[i * kRows + r0] + d0);
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        // a value that is not finite has no code: it is stored as 0 and reported
-        if (!(fabsf(x[i][e]) <= 3.4028234664e38f)) {
-          x[i][e] = 0.0f;
+      for (int e = 0; e < 16; ++e)
+        if (!(fabsf(x[e]) <= 3.4028234664e38f)) {
+          x[e] = 0.0f;
           odd = true;
         }
-        top = fmaxf(top, fabsf(x[i][e]));
-      }
+    };
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      if (i * kRows >= it.count) break;
+      float x[16];
+      values(i, x);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (odd && p.dev_err) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
-    constexpr int kCode = TYPE == q8::kE4m3 ? q8::kE4m3 : q8::kInt8;
+    if (odd) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
     const int kept = it.pos % kBlock;         // rows of the block that were there before
     const size_t run = (size_t)page * p.Hkv + kvh;
-    float* scale_at = (turned ? p.k_scales : p.v_scales) + run * (p.page_tokens / kBlock) + slot / kBlock;
-    uint8_t* rows = static_cast<uint8_t*>(turned ? p.k : p.v) + (run * p.page_tokens + (slot - kept)) * D;
+    float* scale_at = (is_k ? p.k_scales : p.v_scales) + run * (p.page_tokens / kBlock) + slot / kBlock;
+    uint8_t* rows = static_cast<uint8_t*>(is_k ? p.k : p.v) + (run * p.page_tokens + (slot - kept)) * D;
     const float s_kept = kept ? *scale_at : 0.0f;
     const float s = fmaxf(s_kept, q8::scale_for<kCode>(top));
     const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
     if (kept && s > s_kept) {
       const float ratio = __fdiv_rn(s_kept, s);
+#pragma unroll 1
+      for (int r = r0; r < kept; r += kRows) {
 #pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int r = i * kRows + lane / kLanes;
-        if (r < kept) {
+        for (int h = 0; h < 2; ++h) {
+          uint2* at = reinterpret_cast<uint2*>(rows + r * D + d0 + h * kHalf);
+          uint2 w = *at;
+          float v[8];
+          q8::codes_to_float4<kCode>(w.x, v);
+          q8::codes_to_float4<kCode>(w.y, v + 4);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint2* at = reinterpret_cast<uint2*>(rows + r * D + d0 + h * kHalf);
-            uint2 w = *at;
-            float v[8];
-            q8::codes_to_float4<kCode>(w.x, v);
-            q8::codes_to_float4<kCode>(w.y, v + 4);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= ratio;
-            *at = make_uint2(q8::float4_to_codes<kCode>(v), q8::float4_to_codes<kCode>(v + 4));
-          }
+          for (int e = 0; e < 8; ++e) v[e] *= ratio;
+          *at = make_uint2(q8::float4_to_codes<kCode>(v), q8::float4_to_codes<kCode>(v + 4));
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const int r = i * kRows + lane / kLanes;
-      if (r < it.count) {
+      const int r = i * kRows + r0;
+      if (i * kRows >= it.count) break;
+      float x[16];
+      values(i, x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[i][e] *= inv;
+      for (int e = 0; e < 16; ++e) x[e] *= inv;
+      if (r < it.count)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           *reinterpret_cast<uint2*>(rows + (kept + r) * D + d0 + h * kHalf) =
-              make_uint2(q8::float4_to_codes<kCode>(x[i] + 8 * h), q8::float4_to_codes<kCode>(x[i] + 8 * h + 4));
-      }
+              make_uint2(q8::float4_to_codes<kCode>(x + 8 * h), q8::float4_to_codes<kCode>(x + 8 * h + 4));
     }
     if (lane == 0) *scale_at = s;
   }
@@ -361,7 +394,12 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   const long long by_place = T / kBlock + 2LL * B;
   p.by_token = T <= by_place;
   const int items = (int)(p.by_token ? (long long)T : by_place);
-  p.heads_per_cta = heads;
+  // slices of the heads until the device has a few CTAs an SM: a decode step has
+  // few items, and a prompt's tail then weighs less (at least 8 heads a slice,
+  // which share the cosines)
+  int slices = 1;
+  while (slices * 8 < heads && (long long)items * slices < 148 * 12) slices *= 2;
+  p.heads_per_cta = (heads + slices - 1) / slices;
   Freq freq;
   for (int i = 0; i < D / 2; ++i) freq.inv[i] = std::pow((double)theta, -2.0 * i / D);
   const dim3 grid(items, (heads + p.heads_per_cta - 1) / p.heads_per_cta);
