@@ -23,8 +23,11 @@
 // Work split: an item is the run of new rows of one sequence inside one block of
 // 16 positions (the unit of a scale; it never leaves a page), and a slice of the
 // heads.  A CTA computes the item's cosines and sines once, into shared memory.
-// Rows that are copied or rotated into binary16 are then dealt to the threads in
-// the order of memory, 8 consecutive dims of both halves of a head a thread; a
+// For rows that are copied or rotated into binary16 a thread keeps one row and 8
+// consecutive dims of both halves, their cosines and sines in registers, and goes
+// from head to head, several heads' loads ahead (dealing rows to threads in the
+// order of memory instead, cosines read from shared memory each time, took 1.9
+// times the instructions and was bound by them).  A
 // block that is coded needs its largest value first, so a warp takes all of a
 // head's rows, keeps them as they came (binary16) and rotates them twice, which
 // costs fewer registers than it saves time to keep them rotated.
@@ -136,18 +139,18 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
   return w;
 }
 
+__device__ __forceinline__ void load8(const float* src, float* v) {   // 16-byte aligned
+  const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
 // 8 dims of both halves of a row, rotated: (a, b) -> (a cos - b sin, b cos + a sin)
 __device__ __forceinline__ void rotate8(float* a, float* b, const float* co, const float* si) {
 #pragma unroll
-  for (int e = 0; e < 8; e += 4) {
-    const float4 c4 = *reinterpret_cast<const float4*>(co + e), s4 = *reinterpret_cast<const float4*>(si + e);
-    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float u = a[e + k], v = b[e + k];
-      a[e + k] = __fsub_rn(__fmul_rn(u, c[k]), __fmul_rn(v, s[k]));
-      b[e + k] = __fadd_rn(__fmul_rn(v, c[k]), __fmul_rn(u, s[k]));
-    }
+  for (int e = 0; e < 8; ++e) {
+    const float u = a[e], v = b[e];
+    a[e] = __fsub_rn(__fmul_rn(u, co[e]), __fmul_rn(v, si[e]));
+    b[e] = __fadd_rn(__fmul_rn(v, co[e]), __fmul_rn(u, si[e]));
   }
 }
 
@@ -180,47 +183,49 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 4 : 3)
 
   // ---- rows into binary16: q, and with binary16 pages k and v ----
   const int end16 = TYPE == kBinary16 ? head1 : min(head1, p.Hq);
-  if (head0 < end16) {
-    const int per_row = (end16 - head0) * kLanes, total = it.count * per_row;
-    const __half* src = p.qkv + (size_t)it.row * p.stride + head0 * D;
-    constexpr int kAhead = 2;   // pieces a thread loads at a time
+  {
+    // the threads of a head: a power of two of rows; the other threads take other heads
+    const int log_rows = 32 - __clz(it.count - 1);   // 0 for one row
+    const int d0 = 8 * (threadIdx.x % kLanes), r = (threadIdx.x / kLanes) & ((1 << log_rows) - 1);
+    const int step = (kThreads / kLanes) >> log_rows;
+    float co[8], si[8];
+    load8(s_cos[r] + d0, co);   // of a row behind the item's: not used
+    load8(s_sin[r] + d0, si);
+    const __half* src = p.qkv + (size_t)(it.row + r) * p.stride + d0;
+    constexpr int kAhead = 3;   // heads a thread loads at a time
+    if (r < it.count) {
 #pragma unroll 1
-    for (int i = threadIdx.x; i < total; i += kAhead * kThreads) {
-      uint4 lo[kAhead], hi[kAhead];
-      int row[kAhead], at[kAhead];
+      for (int h0 = head0 + ((threadIdx.x / kLanes) >> log_rows); h0 < end16; h0 += kAhead * step) {
+        uint4 lo[kAhead], hi[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int x = i + k * kThreads;
-        row[k] = x / per_row;
-        at[k] = x - row[k] * per_row;
-        if (x < total) {
-          const __half* s = src + (size_t)row[k] * p.stride + (at[k] / kLanes) * D + 8 * (at[k] % kLanes);
-          lo[k] = *reinterpret_cast<const uint4*>(s);
-          hi[k] = *reinterpret_cast<const uint4*>(s + kHalf);
-        }
-      }
+        for (int k = 0; k < kAhead; ++k)
+          if (h0 + k * step < end16) {
+            lo[k] = *reinterpret_cast<const uint4*>(src + (h0 + k * step) * D);
+            hi[k] = *reinterpret_cast<const uint4*>(src + (h0 + k * step) * D + kHalf);
+          }
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if (i + k * kThreads >= total) break;
-        const int head = head0 + at[k] / kLanes, d0 = 8 * (at[k] % kLanes);
-        if (TYPE != kBinary16 || head < p.Hq + p.Hkv) {
-          float a[8], b[8];
-          unpack8(lo[k], a);
-          unpack8(hi[k], b);
-          rotate8(a, b, s_cos[row[k]] + d0, s_sin[row[k]] + d0);
-          lo[k] = pack8(a);
-          hi[k] = pack8(b);
+        for (int k = 0; k < kAhead; ++k) {
+          const int head = h0 + k * step;
+          if (head >= end16) break;
+          if (TYPE != kBinary16 || head < p.Hq + p.Hkv) {
+            float a[8], b[8];
+            unpack8(lo[k], a);
+            unpack8(hi[k], b);
+            rotate8(a, b, co, si);
+            lo[k] = pack8(a);
+            hi[k] = pack8(b);
+          }
+          __half* dst;
+          if (TYPE != kBinary16 || head < p.Hq) {
+            dst = p.q_out + ((size_t)(it.row + r) * p.Hq + head) * D + d0;
+          } else {
+            const bool is_k = head < p.Hq + p.Hkv;
+            dst = static_cast<__half*>(is_k ? p.k : p.v) +
+                  (((size_t)page * p.page_tokens + slot + r) * p.Hkv + head - p.Hq - (is_k ? 0 : p.Hkv)) * D + d0;
+          }
+          *reinterpret_cast<uint4*>(dst) = lo[k];
+          *reinterpret_cast<uint4*>(dst + kHalf) = hi[k];
         }
-        __half* dst;
-        if (TYPE != kBinary16 || head < p.Hq) {
-          dst = p.q_out + ((size_t)(it.row + row[k]) * p.Hq + head) * D + d0;
-        } else {
-          const int kvh = head - p.Hq < p.Hkv ? head - p.Hq : head - p.Hq - p.Hkv;
-          dst = static_cast<__half*>(kvh == head - p.Hq ? p.k : p.v) +
-                (((size_t)page * p.page_tokens + slot + row[k]) * p.Hkv + kvh) * D + d0;
-        }
-        *reinterpret_cast<uint4*>(dst) = lo[k];
-        *reinterpret_cast<uint4*>(dst + kHalf) = hi[k];
       }
     }
   }
@@ -250,7 +255,12 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 4 : 3)
     auto values = [&](int i, float* x) {
       unpack8(raw[i][0], x);
       unpack8(raw[i][1], x + 8);
-      if (is_k && i * kRows + r0 < it.count) rotate8(x, x + 8, s_cos[i * kRows + r0] + d0, s_sin[i * kRows + r0] + d0);
+      if (is_k && i * kRows + r0 < it.count) {
+        float co[8], si[8];
+        load8(s_cos[i * kRows + r0] + d0, co);
+        load8(s_sin[i * kRows + r0] + d0, si);
+        rotate8(x, x + 8, co, si);
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (!(fabsf(x[e]) <= 3.4028234664e38f)) {
@@ -313,29 +323,44 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 4 : 3)
 }
 
 // values[page][head][token][:] = fp16(code * scale), K's pool then V's: a thread
-// takes 16 codes of a row.
+// takes 16 codes of a row at a time, four such pieces on their way.
 template <int TYPE>
 __global__ void __launch_bounds__(256) values_kernel(const uint8_t* k, const uint8_t* v, const float* ks,
                                                      const float* vs, __half* ko, __half* vo, long long chunks,
                                                      int chunks_per_block) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < 2 * chunks;
-       i += (long long)gridDim.x * blockDim.x) {
-    const bool second = i >= chunks;
-    const long long c = second ? i - chunks : i;
-    const uint4 w = reinterpret_cast<const uint4*>(second ? v : k)[c];
-    const float s = (second ? vs : ks)[c / chunks_per_block];
-    float f[16];
-    q8::codes_to_float4<TYPE>(w.x, f);
-    q8::codes_to_float4<TYPE>(w.y, f + 4);
-    q8::codes_to_float4<TYPE>(w.z, f + 8);
-    q8::codes_to_float4<TYPE>(w.w, f + 12);
+  constexpr int kAhead = 4;
+  const bool second = blockIdx.y != 0;
+  const uint4* codes = reinterpret_cast<const uint4*>(second ? v : k);
+  const float* scales = second ? vs : ks;
+  uint4* out = reinterpret_cast<uint4*>(second ? vo : ko);
+  for (long long i0 = (long long)blockIdx.x * (kAhead * 256) + threadIdx.x; i0 < chunks;
+       i0 += (long long)gridDim.x * (kAhead * 256)) {
+    uint4 w[kAhead];
+    float s[kAhead];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) f[e] *= s;
-    uint4* out = reinterpret_cast<uint4*>(second ? vo : ko) + 2 * c;
-    out[0] = pack8(f);
-    out[1] = pack8(f + 8);
+    for (int a = 0; a < kAhead; ++a) {
+      const long long c = i0 + 256 * a;
+      if (c < chunks) {
+        w[a] = __ldcs(codes + c);
+        s[a] = scales[c / chunks_per_block];
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const long long c = i0 + 256 * a;
+      if (c >= chunks) break;
+      float f[16];
+      q8::codes_to_float4<TYPE>(w[a].x, f);
+      q8::codes_to_float4<TYPE>(w[a].y, f + 4);
+      q8::codes_to_float4<TYPE>(w[a].z, f + 8);
+      q8::codes_to_float4<TYPE>(w[a].w, f + 12);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) f[e] *= s[a];
+      out[2 * c] = pack8(f);
+      out[2 * c + 1] = pack8(f + 8);
+    }
   }
 }
 
@@ -398,7 +423,7 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   // few items, and a prompt's tail then weighs less (at least 8 heads a slice,
   // which share the cosines)
   int slices = 1;
-  while (slices * 8 < heads && (long long)items * slices < 148 * 12) slices *= 2;
+  while (slices * 8 < heads && (long long)items * slices < 148 * 4) slices *= 2;
   p.heads_per_cta = (heads + slices - 1) / slices;
   Freq freq;
   for (int i = 0; i < D / 2; ++i) freq.inv[i] = std::pow((double)theta, -2.0 * i / D);
@@ -449,9 +474,9 @@ int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k
   if ((D != 64 && D != 128) || page_tokens < kBlock || page_tokens % kBlock) return ANVILQ_ESHAPE;
   if (!a16(k_codes) || !a16(v_codes) || !a16(k_out) || !a16(v_out)) return ANVILQ_EALIGN;
   const long long chunks = (long long)num_pages * Hkv * page_tokens * (D / 16);
-  const int blocks = (int)std::min<long long>((2 * chunks + 255) / 256, 148 * 16);
+  const int blocks = (int)std::min<long long>((chunks + 1023) / 1024, 148 * 8);
   auto go = [&](auto kernel) {
-    return launch(kernel, dim3(blocks), 256, reinterpret_cast<cudaStream_t>(stream), flags,
+    return launch(kernel, dim3(blocks, 2), 256, reinterpret_cast<cudaStream_t>(stream), flags,
                   static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes), k_scales, v_scales,
                   reinterpret_cast<__half*>(k_out), reinterpret_cast<__half*>(v_out), chunks, kBlock * D / 16);
   };
