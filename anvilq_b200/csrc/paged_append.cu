@@ -41,7 +41,7 @@ namespace append {
 
 using q8::kBlock;
 constexpr int kBinary16 = -1;   // the pool's type: binary16, q8::kInt8 or q8::kE4m3
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxPairs = 64;   // D <= 128
 
@@ -155,7 +155,7 @@ __device__ __forceinline__ void rotate8(float* a, float* b, const float* co, con
 }
 
 template <int D, int TYPE>
-__global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 4 : 3)
+__global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 6)
     append_kernel(const __grid_constant__ Params p, const __grid_constant__ Freq freq) {
   constexpr int kHalf = D / 2;
   constexpr int kLanes = D / 16;              // threads of a row: 8 dims of each half a thread
@@ -165,6 +165,28 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 4 : 3)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Item it = find_item(p, blockIdx.x);
   if (it.count <= 0) return;   // the same for the whole CTA
+  const int heads = p.Hq + 2 * p.Hkv;
+  const int head0 = blockIdx.y * p.heads_per_cta, head1 = min(heads, head0 + p.heads_per_cta);
+  // rows into binary16: q, and with binary16 pages k and v.  The threads of a head
+  // are a power of two of rows; the other threads take other heads.
+  const int end16 = TYPE == kBinary16 ? head1 : min(head1, p.Hq);
+  const int log_rows = 32 - __clz(it.count - 1);   // 0 for one row
+  const int d16 = 8 * (threadIdx.x % kLanes), r16 = (threadIdx.x / kLanes) & ((1 << log_rows) - 1);
+  const int step = (kThreads / kLanes) >> log_rows;
+  const __half* src16 = p.qkv + (size_t)(it.row + r16) * p.stride + d16;
+  constexpr int kAhead = 3;   // heads a thread loads at a time
+  uint4 lo[kAhead], hi[kAhead];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (r16 < it.count && h0 + k * step < end16) {
+        lo[k] = *reinterpret_cast<const uint4*>(src16 + (h0 + k * step) * D);
+        hi[k] = *reinterpret_cast<const uint4*>(src16 + (h0 + k * step) * D + kHalf);
+      }
+  };
+  int h0 = head0 + ((threadIdx.x / kLanes) >> log_rows);
+  load(h0);   // the first heads' rows travel with the page-table word, while the cosines are computed
+
   const int page = q8::page_of(p.page_table, p.max_pages, p.num_pages, it.b, it.pos / p.page_tokens);
   for (int i = threadIdx.x; i < it.count * kHalf; i += kThreads) {
     const int r = i / kHalf, pair = i % kHalf;
@@ -176,57 +198,37 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 4 : 3)
     return;
   }
   __syncthreads();
-
   const int slot = it.pos % p.page_tokens;    // row of the page of the item's first token
-  const int heads = p.Hq + 2 * p.Hkv;
-  const int head0 = blockIdx.y * p.heads_per_cta, head1 = min(heads, head0 + p.heads_per_cta);
-
-  // ---- rows into binary16: q, and with binary16 pages k and v ----
-  const int end16 = TYPE == kBinary16 ? head1 : min(head1, p.Hq);
   {
-    // the threads of a head: a power of two of rows; the other threads take other heads
-    const int log_rows = 32 - __clz(it.count - 1);   // 0 for one row
-    const int d0 = 8 * (threadIdx.x % kLanes), r = (threadIdx.x / kLanes) & ((1 << log_rows) - 1);
-    const int step = (kThreads / kLanes) >> log_rows;
     float co[8], si[8];
-    load8(s_cos[r] + d0, co);   // of a row behind the item's: not used
-    load8(s_sin[r] + d0, si);
-    const __half* src = p.qkv + (size_t)(it.row + r) * p.stride + d0;
-    constexpr int kAhead = 3;   // heads a thread loads at a time
-    if (r < it.count) {
+    load8(s_cos[r16] + d16, co);   // of a row behind the item's: not used
+    load8(s_sin[r16] + d16, si);
 #pragma unroll 1
-      for (int h0 = head0 + ((threadIdx.x / kLanes) >> log_rows); h0 < end16; h0 += kAhead * step) {
-        uint4 lo[kAhead], hi[kAhead];
+    for (; h0 < end16; h0 += kAhead * step) {
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-          if (h0 + k * step < end16) {
-            lo[k] = *reinterpret_cast<const uint4*>(src + (h0 + k * step) * D);
-            hi[k] = *reinterpret_cast<const uint4*>(src + (h0 + k * step) * D + kHalf);
-          }
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          const int head = h0 + k * step;
-          if (head >= end16) break;
-          if (TYPE != kBinary16 || head < p.Hq + p.Hkv) {
-            float a[8], b[8];
-            unpack8(lo[k], a);
-            unpack8(hi[k], b);
-            rotate8(a, b, co, si);
-            lo[k] = pack8(a);
-            hi[k] = pack8(b);
-          }
-          __half* dst;
-          if (TYPE != kBinary16 || head < p.Hq) {
-            dst = p.q_out + ((size_t)(it.row + r) * p.Hq + head) * D + d0;
-          } else {
-            const bool is_k = head < p.Hq + p.Hkv;
-            dst = static_cast<__half*>(is_k ? p.k : p.v) +
-                  (((size_t)page * p.page_tokens + slot + r) * p.Hkv + head - p.Hq - (is_k ? 0 : p.Hkv)) * D + d0;
-          }
-          *reinterpret_cast<uint4*>(dst) = lo[k];
-          *reinterpret_cast<uint4*>(dst + kHalf) = hi[k];
+      for (int k = 0; k < kAhead; ++k) {
+        const int head = h0 + k * step;
+        if (r16 >= it.count || head >= end16) break;
+        if (TYPE != kBinary16 || head < p.Hq + p.Hkv) {
+          float a[8], b[8];
+          unpack8(lo[k], a);
+          unpack8(hi[k], b);
+          rotate8(a, b, co, si);
+          lo[k] = pack8(a);
+          hi[k] = pack8(b);
         }
+        __half* dst;
+        if (TYPE != kBinary16 || head < p.Hq) {
+          dst = p.q_out + ((size_t)(it.row + r16) * p.Hq + head) * D + d16;
+        } else {
+          const bool is_k = head < p.Hq + p.Hkv;
+          dst = static_cast<__half*>(is_k ? p.k : p.v) +
+                (((size_t)page * p.page_tokens + slot + r16) * p.Hkv + head - p.Hq - (is_k ? 0 : p.Hkv)) * D + d16;
+        }
+        *reinterpret_cast<uint4*>(dst) = lo[k];
+        *reinterpret_cast<uint4*>(dst + kHalf) = hi[k];
       }
+      load(h0 + kAhead * step);
     }
   }
   if (TYPE == kBinary16) return;
@@ -423,7 +425,7 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   // few items, and a prompt's tail then weighs less (at least 8 heads a slice,
   // which share the cosines)
   int slices = 1;
-  while (slices * 8 < heads && (long long)items * slices < 148 * 4) slices *= 2;
+  while (slices * 8 < heads && (long long)items * slices < 148 * 8) slices *= 2;
   p.heads_per_cta = (heads + slices - 1) / slices;
   Freq freq;
   for (int i = 0; i < D / 2; ++i) freq.inv[i] = std::pow((double)theta, -2.0 * i / D);
