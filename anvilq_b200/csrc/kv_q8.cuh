@@ -37,8 +37,10 @@ __device__ __forceinline__ int page_of(const uint32_t* table, int max_pages, int
 template <int TYPE>
 __device__ __forceinline__ void codes_to_float4(uint32_t w, float* v) {
   if (TYPE == kInt8) {
+    // (code + 128) in the last byte of 2^23, made signed by one exact subtraction
+    const uint32_t u = w ^ 0x80808080u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)((w >> (8 * i)) & 0xFFu);
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + i)) - 8388736.0f;
   } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -50,18 +52,17 @@ __device__ __forceinline__ void codes_to_float4(uint32_t w, float* v) {
   }
 }
 
-// four binary32 values as codes, each rounded to the nearest (ties to even) and
-// held inside the type's range (int8 uses -127 .. 127)
+// four binary32 values as codes, each rounded to the nearest (ties to even).  They
+// are within the type's range but for their own rounding: |value| <= largest code
+// times a few (1 + 2^-24), which rounds to the largest code (int8 uses -127 .. 127).
 template <int TYPE>
 __device__ __forceinline__ uint32_t float4_to_codes(const float* v) {
   if (TYPE == kInt8) {
-    uint32_t w = 0;
+    // the sum's last bits are the rounded value's (two's complement)
+    uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = max(-127, min(127, __float2int_rn(v[i])));
-      w |= (uint32_t)(c & 0xFF) << (8 * i);
-    }
-    return w;
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(v[i], 12582912.0f));   // 1.5 2^23
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3);

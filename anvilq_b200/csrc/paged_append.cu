@@ -252,9 +252,7 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 6)
         raw[i][1] = *reinterpret_cast<const uint4*>(src + (size_t)i * kRows * p.stride + kHalf);
       }
     }
-    // values of pass i, 0 where they are not finite (those have no code, and are reported)
-    bool odd = false;
-    auto values = [&](int i, float* x) {
+    auto values = [&](int i, float* x) {   // of pass i
       unpack8(raw[i][0], x);
       unpack8(raw[i][1], x + 8);
       if (is_k && i * kRows + r0 < it.count) {
@@ -263,25 +261,35 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 6)
         load8(s_sin[i * kRows + r0] + d0, si);
         rotate8(x, x + 8, co, si);
       }
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (!(fabsf(x[e]) <= 3.4028234664e38f)) {
-          x[e] = 0.0f;
-          odd = true;
-        }
     };
-    float top = 0.0f;
+    auto finite = [](float v) { return fabsf(v) <= 3.4028234664e38f ? v : 0.0f; };
+    float top = 0.0f, probe = 0.0f;   // probe: NaN after a value that is not finite
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       if (i * kRows >= it.count) break;
       float x[16];
       values(i, x);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
+      for (int e = 0; e < 16; ++e) {
+        top = fmaxf(top, fabsf(x[e]));
+        probe = fmaf(x[e], 0.0f, probe);
+      }
+    }
+    // such a value has no code: it is stored as 0, and reported
+    const bool odd = __any_sync(0xffffffffu, probe != 0.0f);
+    if (odd) {
+      if (lane == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
+      top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        float x[16];
+        values(i, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(finite(x[e])));
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (odd) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
     const int kept = it.pos % kBlock;         // rows of the block that were there before
     const size_t run = (size_t)page * p.Hkv + kvh;
     float* scale_at = (is_k ? p.k_scales : p.v_scales) + run * (p.page_tokens / kBlock) + slot / kBlock;
@@ -312,6 +320,9 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 6)
       if (i * kRows >= it.count) break;
       float x[16];
       values(i, x);
+      if (odd)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = finite(x[e]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] *= inv;
       if (r < it.count)
@@ -421,11 +432,12 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   const long long by_place = T / kBlock + 2LL * B;
   p.by_token = T <= by_place;
   const int items = (int)(p.by_token ? (long long)T : by_place);
-  // slices of the heads until the device has a few CTAs an SM: a decode step has
-  // few items, and a prompt's tail then weighs less (at least 8 heads a slice,
-  // which share the cosines)
+  // slices of the heads (at least 8 heads each) only until there are two CTAs an SM:
+  // every slice looks up its tokens and computes their cosines again.  A prompt of
+  // 15.8k tokens (14/2 heads of 64) takes 16.3 us in one slice, 17.7 in two; 8.5k
+  // tokens (32/8 of 128, 8-bit) 38.5 in one, 41.6 in two; a step of 64 tokens 3.2 either way.
   int slices = 1;
-  while (slices * 8 < heads && (long long)items * slices < 148 * 8) slices *= 2;
+  while (slices * 8 < heads && (long long)items * slices < 148 * 2) slices *= 2;
   p.heads_per_cta = (heads + slices - 1) / slices;
   Freq freq;
   for (int i = 0; i < D / 2; ++i) freq.inv[i] = std::pow((double)theta, -2.0 * i / D);
