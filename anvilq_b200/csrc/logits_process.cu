@@ -14,14 +14,17 @@
 // What bounds it: bytes -- each logit in and out once (the history, the lists and
 // the mask's bits are small beside them).
 //
-// Work split: a CTA takes a stretch of the vocabulary of one row.  Its logits are
-// loaded first; while they travel it scans the row's history and bias list for the
-// tokens of its stretch, into tables in shared memory (occurrences; list index).
-// The tables are cleared and read densely: a word a token each way costs less than
-// a second scan of the history for the cells that matter.  One pass then applies
-// everything.  The choice is a maximum over orderable (value, index) keys, combined
-// over a row's CTAs with an integer atomicMax, so its result does not depend on
-// their order.
+// Work split: a CTA takes some consecutive stretches of the vocabulary of one row.
+// It keeps the row's history in registers (its first 2048 tokens; longer ones are
+// read again) and for each stretch, while the stretch's logits travel, enters the
+// tokens that lie in it -- of the history and of the bias list -- into tables in
+// shared memory: occurrences, list indexes, a bitmap, and a list of the different
+// tokens.  Then a dense pass masks and writes the logits outside the bitmap, and a
+// sparse one computes the listed tokens, each by one thread, which cleans their
+// cells.  (One pass that looks every token up took 55 instructions a logit: nearly
+// every warp has some lane with a penalty.)  The choice is a maximum over orderable
+// (value, index) keys, combined over a row's CTAs with an integer atomicMax, so
+// its result does not depend on their order.
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -61,15 +64,14 @@ struct Params {
   unsigned long long* keys;
   int* tickets;
   int* dev_err;
-  int V, L, bias_total, masks, stretch;
+  int V, L, bias_total, masks, stretch, per_cta;
   int wide_out;                  // out's rows start on 16-byte boundaries
 };
 
-// larger value first, then the lower index; above 0 for v > -inf
-__device__ __forceinline__ unsigned long long choice_key(float v, int index) {
-  uint32_t b = __float_as_uint(v + 0.0f);   // -0 as +0
-  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return ((unsigned long long)b << 32) | (unsigned long long)(0xFFFFFFFFu - (uint32_t)index);
+// ascending with the value, above that of -inf for every other number; -0 as +0
+__device__ __forceinline__ unsigned orderable(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
 constexpr int kPiece = 8;                                // logits of a thread at a time
@@ -105,86 +107,63 @@ template <> struct Raw8<__half> {
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 
+constexpr int kIds = 8;                                  // tokens of the history that a thread keeps
+
 // WIDE: rows start on 16-byte boundaries; a thread's piece is 8 consecutive logits.
 // Otherwise its 8 logits lie kThreads apart, so that a warp's loads still are whole
 // sectors.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) int tables[];
-  __shared__ unsigned long long s_best[kThreads / 32];
+  __shared__ uint32_t s_map[2][kMaxStretch / 32];   // the listed tokens; of even and odd stretches
+  __shared__ int s_listed[2];
+  __shared__ unsigned s_best[kThreads / 32];
+  __shared__ int s_at;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int b = blockIdx.y;
-  const int v0 = blockIdx.x * p.stretch, v1 = min(p.V, v0 + p.stretch);
+  const int row_end = min((long long)p.V, ((long long)blockIdx.x + 1) * p.per_cta * p.stretch);
+  int v0 = blockIdx.x * p.per_cta * p.stretch;
   const bool lead = blockIdx.x == 0 && threadIdx.x == 0;
   const T* x = static_cast<const T*>(p.x) + b * p.ld;
   constexpr int kAcross = kThreads * kPiece;
-  const int mine = v0 + (int)threadIdx.x * (WIDE ? kPiece : 1), apart = WIDE ? 1 : kThreads;   // of a piece's logits
-  Raw8<T> raw[kPieces];
-  float loose[kPieces][kPiece];
-  // whole pieces only: the row's last logits may not fill one
-  auto whole = [&](int i) { return WIDE && mine + i * kAcross + kPiece <= v1; };
+  constexpr int kApart = WIDE ? 1 : kThreads;             // between a piece's logits
+  const int first = (int)threadIdx.x * (WIDE ? kPiece : 1);
+  Raw8<T> raw[kPieces];       // whole pieces
+  auto load = [&](int v0) {
+    const int v1 = min(row_end, v0 + p.stretch);
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int v = mine + i * kAcross;
-    if (whole(i)) {
-      raw[i].load(x + v);
-    } else {
+    for (int i = 0; i < kPieces; ++i) {
+      const int v = v0 + first + i * kAcross;
+      if (WIDE && v + kPiece <= v1) raw[i].load(x + v);   // others are loaded when they are used
+    }
+  };
+  load(v0);
+  // ---- what the row brings ----
+  const int32_t* history = p.history + b * p.history_ld;
+  int ids[kIds];
+  int hist = 0, prompt = 0, bias0 = 0, bias1 = 0;
+  if (p.history) {
 #pragma unroll
-      for (int e = 0; e < kPiece; ++e)
-        loose[i][e] = v + e * apart < v1 ? to_float(x[v + e * apart]) : -INFINITY;
+    for (int k = 0; k < kIds; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      ids[k] = i < p.L ? history[i] : -1;
+    }
+    hist = p.history_lens[b];
+    prompt = p.prompt_lens ? p.prompt_lens[b] : 0;
+    if (hist < 0 || hist > p.L) {
+      if (lead) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+      hist = max(0, min(hist, p.L));
     }
   }
-
-  // ---- the tables: occurrences (top bit: only before the generated part), list indexes ----
-  int* count = tables;
-  int* entry = tables + (p.history ? p.stretch : 0);
-  if (p.history || p.bias_starts) {
-    if (p.history)
-      for (int i = threadIdx.x; i < p.stretch / 4; i += kThreads) reinterpret_cast<int4*>(count)[i] = make_int4(0, 0, 0, 0);
-    if (p.bias_starts)
-      for (int i = threadIdx.x; i < p.stretch / 4; i += kThreads) reinterpret_cast<int4*>(entry)[i] = make_int4(-1, -1, -1, -1);
-    int hist = 0, prompt = 0, bias0 = 0, bias1 = 0;
-    if (p.history) {
-      hist = p.history_lens[b];
-      prompt = p.prompt_lens ? p.prompt_lens[b] : 0;
-      if (hist < 0 || hist > p.L) {
-        if (lead) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
-        hist = max(0, min(hist, p.L));
-      }
+  if (p.bias_starts) {
+    bias0 = p.bias_starts[b];
+    bias1 = p.bias_starts[b + 1];
+    if (bias0 < 0 || bias1 > p.bias_total || bias0 > bias1) {
+      if (lead) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+      bias0 = bias1 = 0;
     }
-    if (p.bias_starts) {
-      bias0 = p.bias_starts[b];
-      bias1 = p.bias_starts[b + 1];
-      if (bias0 < 0 || bias1 > p.bias_total || bias0 > bias1) {
-        if (lead) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
-        bias0 = bias1 = 0;
-      }
-    }
-    __syncthreads();
-    auto place = [&](int id) {   // in the stretch, or -1
-      if ((unsigned)id >= (unsigned)p.V) {
-        if (blockIdx.x == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TOKEN);
-        return -1;
-      }
-      return id >= v0 && id < v1 ? id - v0 : -1;
-    };
-    const int32_t* history = p.history + b * p.history_ld;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < hist; i += kThreads) {
-      const int at = place(history[i]);
-      if (at >= 0) {
-        if (i >= prompt) atomicAdd(count + at, 1);
-        else atomicOr(reinterpret_cast<unsigned*>(count + at), 0x80000000u);
-      }
-    }
-    for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) {
-      const int at = place(p.bias_ids[i]);
-      if (at >= 0) atomicMax(entry + at, i);   // the last entry of an id
-    }
-    __syncthreads();
   }
-
   const float rep = p.repetition ? p.repetition[b] : 1.0f;
   const float pres = p.presence ? p.presence[b] : 0.0f;
   const float freq = p.frequency ? p.frequency[b] : 0.0f;
@@ -198,86 +177,172 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     }
   }
   float* out = p.out ? p.out + b * p.out_ld : nullptr;
-  float best = -INFINITY;   // the thread's logits come in ascending order: the first of equals stays
-  int best_at = -1;
+  const bool special = p.history || p.bias_starts;
+  int* count = tables;                                            // occurrences in the generated part
+  int* entry = tables + (p.history ? p.stretch : 0);              // last index of the bias list, or -1
+  uint16_t* listed = reinterpret_cast<uint16_t*>(entry + (p.bias_starts ? p.stretch : 0));
+  static_assert(kMaxStretch <= 0x10000, "a place fits 16 bits");
+  if (special) {
+    if (p.history)
+      for (int i = threadIdx.x; i < p.stretch / 4; i += kThreads) reinterpret_cast<int4*>(count)[i] = make_int4(0, 0, 0, 0);
+    if (p.bias_starts)
+      for (int i = threadIdx.x; i < p.stretch / 4; i += kThreads) reinterpret_cast<int4*>(entry)[i] = make_int4(-1, -1, -1, -1);
+    for (int i = threadIdx.x; i < kMaxStretch / 32; i += kThreads) s_map[0][i] = s_map[1][i] = 0u;
+    if (threadIdx.x < 2) s_listed[threadIdx.x] = 0;
+  }
+  if (threadIdx.x == 0) s_at = 0x7FFFFFFF;
+  // an id outside the vocabulary is reported (by the row's first CTA) and ignored
+  auto report = [&](int id) {
+    if (blockIdx.x == 0 && (unsigned)id >= (unsigned)p.V) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TOKEN);
+  };
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int v = mine + i * kAcross, at = v - v0;
-    if (v >= v1) break;
-    float l[kPiece];
-    if (whole(i)) {
-      raw[i].get(l);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kPiece; ++e) l[e] = loose[i][e];
-    }
-    if (p.history) {
-      int n[kPiece];
-      if (WIDE) {   // the stretch is a multiple of a piece
-        *reinterpret_cast<int4*>(n) = *reinterpret_cast<const int4*>(count + at);
-        *reinterpret_cast<int4*>(n + 4) = *reinterpret_cast<const int4*>(count + at + 4);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kPiece; ++e) n[e] = v + e * apart < v1 ? count[at + e * apart] : 0;
-      }
-#pragma unroll
-      for (int e = 0; e < kPiece; ++e)
-        if (n[e]) {
-          l[e] = l[e] > 0.0f ? __fdiv_rn(l[e], rep) : __fmul_rn(l[e], rep);
-          const int said = n[e] & 0x7FFFFFFF;
-          if (said) l[e] = __fsub_rn(__fsub_rn(l[e], __fmul_rn(freq, (float)said)), pres);
+  for (int k = 0; k < kIds; ++k) {
+    const int i = threadIdx.x + k * kThreads;
+    if (p.history && i < hist) report(ids[k]);
+    else ids[k] = -1;
+  }
+  for (int i = kIds * kThreads + threadIdx.x; i < hist; i += kThreads) report(history[i]);
+  for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) report(p.bias_ids[i]);
+
+  float best = -INFINITY;
+  int best_at = 0x7FFFFFFF;   // the lowest of equals
+  int parity = 0;
+#pragma unroll 1
+  for (; v0 < row_end; v0 += p.stretch, parity ^= 1) {
+    const int v1 = min(row_end, v0 + p.stretch);
+    uint32_t* map = s_map[parity];
+    if (special) {
+      __syncthreads();      // the tables are clean
+      auto enter = [&](int at) {   // the first of a token's threads lists it
+        const uint32_t bit = 1u << (at % 32);
+        if (!(atomicOr(map + at / 32, bit) & bit)) listed[atomicAdd(&s_listed[parity], 1)] = (uint16_t)at;
+      };
+      auto occurs = [&](int id, int i) {
+        if (id >= v0 && id < v1) {
+          enter(id - v0);
+          // bit 31: in the history at all
+          if (i >= prompt) atomicAdd(count + (id - v0), 1);
+          else atomicOr(reinterpret_cast<unsigned*>(count + (id - v0)), 0x80000000u);
         }
+      };
+      if (p.history) {
+#pragma unroll
+        for (int k = 0; k < kIds; ++k) occurs(ids[k], threadIdx.x + k * kThreads);
+        for (int i = kIds * kThreads + threadIdx.x; i < hist; i += kThreads) occurs(history[i], i);
+      }
+      for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) {
+        const int id = p.bias_ids[i];
+        if (id >= v0 && id < v1) {
+          enter(id - v0);
+          atomicMax(entry + (id - v0), i);   // the last entry of an id
+        }
+      }
+      __syncthreads();
     }
-    if (p.bias_starts) {
-      int n[kPiece];
+
+    // ---- dense: what is not listed ----
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int v = v0 + first + i * kAcross, at = v - v0;
+      if (v >= v1) break;
+      const bool whole = v + (kPiece - 1) * kApart < v1;
+      float l[kPiece];
+      uint32_t skip = 0u;     // bit e: listed
       if (WIDE) {
-        *reinterpret_cast<int4*>(n) = *reinterpret_cast<const int4*>(entry + at);
-        *reinterpret_cast<int4*>(n + 4) = *reinterpret_cast<const int4*>(entry + at + 4);
+        if (special) skip = map[at / 32] >> (at % 32) & 0xFFu;
+        if (whole) {
+          raw[i].get(l);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kPiece; ++e) l[e] = v + e < v1 ? to_float(x[v + e]) : -INFINITY;
+        }
+        if (allowed) {
+          const uint32_t bits = allowed[v / 32] >> (v % 32);
+#pragma unroll
+          for (int e = 0; e < kPiece; ++e)
+            if (!(bits >> e & 1u)) l[e] = -INFINITY;
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e) n[e] = v + e * apart < v1 ? entry[at + e * apart] : -1;
+        for (int e = 0; e < kPiece; ++e) {
+          const int u = v + e * kApart;
+          l[e] = -INFINITY;
+          if (u < v1) {
+            l[e] = to_float(x[u]);
+            if (special) skip |= (map[(u - v0) / 32] >> ((u - v0) % 32) & 1u) << e;
+            if (allowed && !(allowed[u / 32] >> (u % 32) & 1u)) l[e] = -INFINITY;
+          }
+        }
       }
+      if (out) {
+        if (WIDE && whole && p.wide_out && !skip) {
+          reinterpret_cast<float4*>(out + v)[0] = make_float4(l[0], l[1], l[2], l[3]);
+          reinterpret_cast<float4*>(out + v)[1] = make_float4(l[4], l[5], l[6], l[7]);
+        } else {
 #pragma unroll
-      for (int e = 0; e < kPiece; ++e)
-        if (n[e] >= 0) l[e] = __fadd_rn(l[e], p.bias_values[n[e]]);
-    }
-    if (allowed) {
-      const uint32_t bits = WIDE ? allowed[v / 32] >> (v % 32) : 0u;
-#pragma unroll
-      for (int e = 0; e < kPiece; ++e) {
-        const int u = v + e * apart;
-        if (WIDE ? !(bits >> e & 1u) : u < v1 && !(allowed[u / 32] >> (u % 32) & 1u)) l[e] = -INFINITY;
+          for (int e = 0; e < kPiece; ++e)
+            if (v + e * kApart < v1 && !(skip >> e & 1u)) out[v + e * kApart] = l[e];
+        }
       }
-    }
-#pragma unroll
-    for (int e = 0; e < kPiece; ++e)
-      if (l[e] > best && v + e * apart < v1) {
-        best = l[e];
-        best_at = v + e * apart;
-      }
-    if (out) {
-      if (whole(i) && p.wide_out) {
-        reinterpret_cast<float4*>(out + v)[0] = make_float4(l[0], l[1], l[2], l[3]);
-        reinterpret_cast<float4*>(out + v)[1] = make_float4(l[4], l[5], l[6], l[7]);
-      } else {
+      if (skip)
 #pragma unroll
         for (int e = 0; e < kPiece; ++e)
-          if (v + e * apart < v1) out[v + e * apart] = l[e];
+          if (skip >> e & 1u) l[e] = -INFINITY;
+      const float top = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), fmaxf(fmaxf(l[4], l[5]), fmaxf(l[6], l[7])));
+      if (top > best) {       // a thread's places ascend: an equal one later is not lower
+        best = top;
+#pragma unroll
+        for (int e = kPiece - 1; e >= 0; --e)
+          if (l[e] == top) best_at = v + e * kApart;
       }
+    }
+    load(v0 + p.stretch);     // nothing behind row_end
+
+    // ---- sparse: the listed tokens ----
+    if (special) {
+      const int n = s_listed[parity];
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int at = listed[i], v = v0 + at;
+        float l = to_float(x[v]);
+        if (p.history) {
+          const int said = count[at];
+          count[at] = 0;
+          if (said) {
+            l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
+            if (said & 0x7FFFFFFF) l = __fsub_rn(__fsub_rn(l, __fmul_rn(freq, (float)(said & 0x7FFFFFFF))), pres);
+          }
+        }
+        if (p.bias_starts) {
+          const int k = entry[at];
+          entry[at] = -1;
+          if (k >= 0) l = __fadd_rn(l, p.bias_values[k]);
+        }
+        if (allowed && !(allowed[v / 32] >> (v % 32) & 1u)) l = -INFINITY;
+        if (out) out[v] = l;
+        if (l > best || (l == best && v < best_at && l > -INFINITY)) {
+          best = l;
+          best_at = v;
+        }
+      }
+      // the other stretches' map and length, not used before the next barrier
+      for (int i = threadIdx.x; i < kMaxStretch / 32; i += kThreads) s_map[parity ^ 1][i] = 0u;
+      if (threadIdx.x == 0) s_listed[parity ^ 1] = 0;
     }
   }
   if (!p.token) return;
-  unsigned long long key = best_at >= 0 ? choice_key(best, best_at) : 0ull;
+  // the CTA's best value, then the lowest index that has it
+  const unsigned mine = orderable(best);
+  const unsigned warp_best = __reduce_max_sync(0xffffffffu, mine);
+  if (threadIdx.x % 32 == 0) s_best[threadIdx.x / 32] = warp_best;
+  __syncthreads();
+  unsigned top = 0u;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
-    key = other > key ? other : key;
-  }
-  if (threadIdx.x % 32 == 0) s_best[threadIdx.x / 32] = key;
+  for (int w = 0; w < kThreads / 32; ++w) top = max(top, s_best[w]);
+  if (mine == top && best > -INFINITY) atomicMin(&s_at, best_at);
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) key = s_best[w] > key ? s_best[w] : key;
-    if (key) atomicMax(p.keys + b, key);
+    if (s_at != 0x7FFFFFFF)
+      atomicMax(p.keys + b, (unsigned long long)top << 32 | (unsigned long long)(0xFFFFFFFFu - (unsigned)s_at));
     __threadfence();
     if (atomicAdd(p.tickets + b, 1) == (int)gridDim.x - 1) {   // the row's last CTA
       __threadfence();
@@ -288,12 +353,14 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
   }
 }
 
-// The stretch of a CTA: few CTAs a row scan the history fewer times, many fill
-// the device.
-static int stretch_for(int B, int V) {
+// A CTA's stretches: short ones, one a CTA, until few rows fill the device; then
+// as many a CTA as leave it full (four CTAs an SM), so that the history is read rarely.
+static void cut(int B, int V, int* stretch, int* per_cta) {
   int s = kMaxStretch;
   while (s > 512 && (long long)B * ((V + s - 1) / s) < 296) s /= 2;
-  return s;
+  const int n = (V + s - 1) / s, ctas = std::max(1, std::min(n, 592 / B));
+  *stretch = s;
+  *per_cta = (n + ctas - 1) / ctas;
 }
 
 static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -353,12 +420,12 @@ int anvilq_logits_process(const void* logits, int logits_half, long long logits_
   p.tickets = token ? reinterpret_cast<int*>(static_cast<char*>(workspace) + kTicketOffset) : nullptr;
   p.dev_err = dev_err;
   p.V = V; p.L = L; p.bias_total = bias_total; p.masks = masks;
-  p.stretch = stretch_for(B, V);
-  const size_t smem = (size_t)p.stretch * 4 * ((history ? 1 : 0) + (bias_starts ? 1 : 0));
+  cut(B, V, &p.stretch, &p.per_cta);
+  const size_t smem = history || bias_starts ? (size_t)p.stretch * (4 * ((history ? 1 : 0) + (bias_starts ? 1 : 0)) + 2) : 0;
   const bool wide = aligned(logits, 16) && logits_stride % (logits_half ? 8 : 4) == 0;
   p.wide_out = out && aligned(out, 16) && out_stride % 4 == 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((V + p.stretch - 1) / p.stretch, B);
+  cfg.gridDim = dim3((V + p.stretch * p.per_cta - 1) / (p.stretch * p.per_cta), B);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
