@@ -14,17 +14,18 @@
 // What bounds it: bytes -- each logit in and out once (the history, the lists and
 // the mask's bits are small beside them).
 //
-// Work split: a CTA takes some consecutive stretches of the vocabulary of one row.
-// It keeps the row's history in registers (its first 2048 tokens; longer ones are
-// read again) and for each stretch, while the stretch's logits travel, enters the
-// tokens that lie in it -- of the history and of the bias list -- into tables in
-// shared memory: occurrences, list indexes, a bitmap, and a list of the different
-// tokens.  Then a dense pass masks and writes the logits outside the bitmap, and a
-// sparse one computes the listed tokens, each by one thread, which cleans their
-// cells.  (One pass that looks every token up took 55 instructions a logit: nearly
-// every warp has some lane with a penalty.)  The choice is a maximum over orderable
-// (value, index) keys, combined over a row's CTAs with an integer atomicMax, so
-// its result does not depend on their order.
+// Work split: a CTA takes a span of the vocabulary of one row.  While its first
+// logits travel it marks the span's special tokens -- of the row's history and of
+// its bias list -- in a bitmap, counts the marks up to each word, and so gives every
+// special token a place in short tables (occurrences, last bias index).  A dense
+// pass then masks and writes all logits, taking the largest of the others; behind a
+// barrier the special ones are computed from their tables, a thread each, and
+// written over.  More special tokens than the tables hold take further rounds over
+// the history.  (One pass that looks every token up took 55 instructions a logit,
+// as nearly every warp has some lane with a penalty; tables as long as the
+// vocabulary, stretch by stretch, spent their time in barriers.)  The choice is a
+// maximum over orderable (value, index) keys, combined over a row's CTAs with an
+// integer atomicMax, so its result does not depend on their order.
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -64,7 +65,7 @@ struct Params {
   unsigned long long* keys;
   int* tickets;
   int* dev_err;
-  int V, L, bias_total, masks, stretch, per_cta;
+  int V, L, bias_total, masks, span;
   int wide_out;                  // out's rows start on 16-byte boundaries
 };
 
@@ -74,9 +75,14 @@ __device__ __forceinline__ unsigned orderable(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-constexpr int kPiece = 8;                                // logits of a thread at a time
-constexpr int kPieces = 2;
-constexpr int kMaxStretch = kThreads * kPiece * kPieces;
+constexpr int kPiece = 8;                      // logits of a thread at a time
+constexpr int kAhead = 2;                      // pieces loaded ahead
+constexpr int kAcross = kThreads * kPiece;
+constexpr int kMaxSpan = 32768;
+constexpr int kWords = kMaxSpan / 32;          // of the bitmap
+constexpr int kTable = 2048;                   // special tokens of a round
+constexpr int kIds = 8;                        // tokens of the history that a thread keeps
+static_assert(kWords == 4 * kThreads && kMaxSpan <= 0x10000, "four words a thread; a place fits 16 bits");
 
 // eight consecutive logits, 16-byte aligned, as they are stored
 template <typename T> struct Raw8;
@@ -107,66 +113,27 @@ template <> struct Raw8<__half> {
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 
-constexpr int kIds = 8;                                  // tokens of the history that a thread keeps
-
 // WIDE: rows start on 16-byte boundaries; a thread's piece is 8 consecutive logits.
 // Otherwise its 8 logits lie kThreads apart, so that a warp's loads still are whole
 // sectors.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_constant__ Params p) {
-  extern __shared__ __align__(16) int tables[];
-  __shared__ uint32_t s_map[2][kMaxStretch / 32];   // the listed tokens; of even and odd stretches
-  __shared__ int s_listed[2];
+  __shared__ uint32_t s_map[kWords];    // bit: a special token
+  __shared__ int s_rank[kWords];        // special tokens before the word's
+  __shared__ int s_count[kTable];       // occurrences in the generated part; bit 31: in the history at all
+  __shared__ int s_entry[kTable];       // last index in the bias list, or -1
+  __shared__ uint16_t s_token[kTable];
+  __shared__ int s_sum[kThreads / 32];
   __shared__ unsigned s_best[kThreads / 32];
   __shared__ int s_at;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int b = blockIdx.y;
-  const int row_end = min((long long)p.V, ((long long)blockIdx.x + 1) * p.per_cta * p.stretch);
-  int v0 = blockIdx.x * p.per_cta * p.stretch;
+  const int b = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int v0 = blockIdx.x * p.span, v1 = min(p.V, v0 + p.span);
   const bool lead = blockIdx.x == 0 && threadIdx.x == 0;
   const T* x = static_cast<const T*>(p.x) + b * p.ld;
-  constexpr int kAcross = kThreads * kPiece;
   constexpr int kApart = WIDE ? 1 : kThreads;             // between a piece's logits
-  const int first = (int)threadIdx.x * (WIDE ? kPiece : 1);
-  Raw8<T> raw[kPieces];       // whole pieces
-  auto load = [&](int v0) {
-    const int v1 = min(row_end, v0 + p.stretch);
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int v = v0 + first + i * kAcross;
-      if (WIDE && v + kPiece <= v1) raw[i].load(x + v);   // others are loaded when they are used
-    }
-  };
-  load(v0);
-  // ---- what the row brings ----
-  const int32_t* history = p.history + b * p.history_ld;
-  int ids[kIds];
-  int hist = 0, prompt = 0, bias0 = 0, bias1 = 0;
-  if (p.history) {
-#pragma unroll
-    for (int k = 0; k < kIds; ++k) {
-      const int i = threadIdx.x + k * kThreads;
-      ids[k] = i < p.L ? history[i] : -1;
-    }
-    hist = p.history_lens[b];
-    prompt = p.prompt_lens ? p.prompt_lens[b] : 0;
-    if (hist < 0 || hist > p.L) {
-      if (lead) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
-      hist = max(0, min(hist, p.L));
-    }
-  }
-  if (p.bias_starts) {
-    bias0 = p.bias_starts[b];
-    bias1 = p.bias_starts[b + 1];
-    if (bias0 < 0 || bias1 > p.bias_total || bias0 > bias1) {
-      if (lead) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
-      bias0 = bias1 = 0;
-    }
-  }
-  const float rep = p.repetition ? p.repetition[b] : 1.0f;
-  const float pres = p.presence ? p.presence[b] : 0.0f;
-  const float freq = p.frequency ? p.frequency[b] : 0.0f;
+  const int first = v0 + (int)threadIdx.x * (WIDE ? kPiece : 1);
   const uint32_t* allowed = nullptr;
   if (p.allowed) {
     const int row = p.allowed_rows ? p.allowed_rows[b] : b;   // negative: the row has no mask
@@ -176,80 +143,132 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
       allowed = p.allowed + row * p.allowed_ld;
     }
   }
-  float* out = p.out ? p.out + b * p.out_ld : nullptr;
-  const bool special = p.history || p.bias_starts;
-  int* count = tables;                                            // occurrences in the generated part
-  int* entry = tables + (p.history ? p.stretch : 0);              // last index of the bias list, or -1
-  uint16_t* listed = reinterpret_cast<uint16_t*>(entry + (p.bias_starts ? p.stretch : 0));
-  static_assert(kMaxStretch <= 0x10000, "a place fits 16 bits");
-  if (special) {
-    if (p.history)
-      for (int i = threadIdx.x; i < p.stretch / 4; i += kThreads) reinterpret_cast<int4*>(count)[i] = make_int4(0, 0, 0, 0);
-    if (p.bias_starts)
-      for (int i = threadIdx.x; i < p.stretch / 4; i += kThreads) reinterpret_cast<int4*>(entry)[i] = make_int4(-1, -1, -1, -1);
-    for (int i = threadIdx.x; i < kMaxStretch / 32; i += kThreads) s_map[0][i] = s_map[1][i] = 0u;
-    if (threadIdx.x < 2) s_listed[threadIdx.x] = 0;
-  }
-  if (threadIdx.x == 0) s_at = 0x7FFFFFFF;
-  // an id outside the vocabulary is reported (by the row's first CTA) and ignored
-  auto report = [&](int id) {
-    if (blockIdx.x == 0 && (unsigned)id >= (unsigned)p.V) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TOKEN);
+  Raw8<T> raw[kAhead];       // whole pieces, and their words of the mask
+  uint32_t bits[kAhead];
+  auto load = [&](int i, int v) {
+    if (WIDE && v + kPiece <= v1) raw[i].load(x + v);     // others are loaded when they are used
+    if (WIDE && allowed && v < v1) bits[i] = allowed[v / 32];
   };
 #pragma unroll
-  for (int k = 0; k < kIds; ++k) {
-    const int i = threadIdx.x + k * kThreads;
-    if (p.history && i < hist) report(ids[k]);
-    else ids[k] = -1;
-  }
-  for (int i = kIds * kThreads + threadIdx.x; i < hist; i += kThreads) report(history[i]);
-  for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) report(p.bias_ids[i]);
+  for (int i = 0; i < kAhead; ++i) load(i, first + i * kAcross);
 
-  float best = -INFINITY;
-  int best_at = 0x7FFFFFFF;   // the lowest of equals
-  int parity = 0;
-#pragma unroll 1
-  for (; v0 < row_end; v0 += p.stretch, parity ^= 1) {
-    const int v1 = min(row_end, v0 + p.stretch);
-    uint32_t* map = s_map[parity];
-    if (special) {
-      __syncthreads();      // the tables are clean
-      auto enter = [&](int at) {   // the first of a token's threads lists it
-        const uint32_t bit = 1u << (at % 32);
-        if (!(atomicOr(map + at / 32, bit) & bit)) listed[atomicAdd(&s_listed[parity], 1)] = (uint16_t)at;
-      };
-      auto occurs = [&](int id, int i) {
-        if (id >= v0 && id < v1) {
-          enter(id - v0);
-          // bit 31: in the history at all
-          if (i >= prompt) atomicAdd(count + (id - v0), 1);
-          else atomicOr(reinterpret_cast<unsigned*>(count + (id - v0)), 0x80000000u);
-        }
-      };
-      if (p.history) {
-#pragma unroll
-        for (int k = 0; k < kIds; ++k) occurs(ids[k], threadIdx.x + k * kThreads);
-        for (int i = kIds * kThreads + threadIdx.x; i < hist; i += kThreads) occurs(history[i], i);
-      }
-      for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) {
-        const int id = p.bias_ids[i];
-        if (id >= v0 && id < v1) {
-          enter(id - v0);
-          atomicMax(entry + (id - v0), i);   // the last entry of an id
-        }
-      }
-      __syncthreads();
+  // ---- the special tokens ----
+  int hist = 0, prompt = 0, bias0 = 0, bias1 = 0, specials = 0;
+  const int32_t* history = p.history + b * p.history_ld;
+  constexpr int kNone = 0x7FFFFFFF;   // in no span
+  int ids[kIds];
+  const bool special = p.history || p.bias_starts;
+  auto clear = [&] {
+    for (int i = threadIdx.x; i < kTable; i += kThreads) {
+      s_count[i] = 0;
+      s_entry[i] = -1;
     }
-
-    // ---- dense: what is not listed ----
+  };
+  if (special) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int v = v0 + first + i * kAcross, at = v - v0;
+    for (int k = 0; k < kIds; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      ids[k] = p.history && i < p.L ? history[i] : kNone;
+    }
+    if (p.history) {
+      hist = p.history_lens[b];
+      prompt = p.prompt_lens ? p.prompt_lens[b] : 0;
+      if (hist < 0 || hist > p.L) {
+        if (lead) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+        hist = max(0, min(hist, p.L));
+      }
+    }
+    if (p.bias_starts) {
+      bias0 = p.bias_starts[b];
+      bias1 = p.bias_starts[b + 1];
+      if (bias0 < 0 || bias1 > p.bias_total || bias0 > bias1) {
+        if (lead) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+        bias0 = bias1 = 0;
+      }
+    }
+    for (int i = threadIdx.x; i < kWords; i += kThreads) s_map[i] = 0u;
+    clear();
+    __syncthreads();
+    // an id outside the vocabulary is reported (by the row's first CTA) and ignored
+    auto mark = [&](int id) {
+      if (blockIdx.x == 0 && (unsigned)id >= (unsigned)p.V) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TOKEN);
+      if (id >= v0 && id < v1) atomicOr(s_map + (id - v0) / 32, 1u << ((id - v0) % 32));
+    };
+#pragma unroll
+    for (int k = 0; k < kIds; ++k) {
+      if ((int)threadIdx.x + k * kThreads < hist) mark(ids[k]);
+      else ids[k] = kNone;
+    }
+    for (int i = kIds * kThreads + threadIdx.x; i < hist; i += kThreads) mark(history[i]);
+    for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) mark(p.bias_ids[i]);
+    __syncthreads();
+    // marks before each word: a thread's four words, the warp's threads, the warps
+    const uint4 mine = reinterpret_cast<const uint4*>(s_map)[threadIdx.x];
+    const int n0 = __popc(mine.x), n1 = n0 + __popc(mine.y), n2 = n1 + __popc(mine.z), n3 = n2 + __popc(mine.w);
+    int upto = n3;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    int before = upto - n3;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const int n = s_sum[w];
+      specials += n;
+      if (w < warp) before += n;
+    }
+    reinterpret_cast<int4*>(s_rank)[threadIdx.x] = make_int4(before, before + n0, before + n1, before + n2);
+    __syncthreads();
+  }
+  // the occurrences of the special tokens from rank r0 on, as many as the tables hold
+  auto tally = [&](int r0) {
+    auto place = [&](int id) {
+      if (id < v0 || id >= v1) return -1;
+      const int at = id - v0;
+      const int i = s_rank[at / 32] + __popc(s_map[at / 32] & ((1u << (at % 32)) - 1u)) - r0;
+      if (i < 0 || i >= kTable) return -1;
+      s_token[i] = (uint16_t)at;
+      return i;
+    };
+    auto occurs = [&](int at, int i) {
+      if (at < 0) return;
+      if (i >= prompt) atomicAdd(s_count + at, 1);
+      else atomicOr(reinterpret_cast<unsigned*>(s_count + at), 0x80000000u);
+    };
+    if (r0 == 0)
+#pragma unroll
+      for (int k = 0; k < kIds; ++k) occurs(place(ids[k]), threadIdx.x + k * kThreads);
+    // (later rounds read all of it again: its tokens in registers would cost the dense pass)
+    for (int i = (r0 == 0 ? kIds * kThreads : 0) + threadIdx.x; i < hist; i += kThreads) occurs(place(history[i]), i);
+    for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) {
+      const int at = place(p.bias_ids[i]);
+      if (at >= 0) atomicMax(s_entry + at, i);   // the last entry of an id
+    }
+  };
+  if (threadIdx.x == 0) s_at = kNone;
+  if (specials > 0) tally(0);
+
+  // ---- dense: all logits masked and written, the largest of those that are not special ----
+  const float rep = p.repetition ? p.repetition[b] : 1.0f;
+  const float pres = p.presence ? p.presence[b] : 0.0f;
+  const float freq = p.frequency ? p.frequency[b] : 0.0f;
+  float* out = p.out ? p.out + b * p.out_ld : nullptr;
+  float best = -INFINITY;
+  int best_at = kNone;        // the lowest of equals
+#pragma unroll 1
+  for (int vb = first; vb < v1; vb += kAhead * kAcross) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int v = vb + i * kAcross;
       if (v >= v1) break;
       const bool whole = v + (kPiece - 1) * kApart < v1;
       float l[kPiece];
-      uint32_t skip = 0u;     // bit e: listed
+      uint32_t skip = 0u;     // bit e: special
       if (WIDE) {
-        if (special) skip = map[at / 32] >> (at % 32) & 0xFFu;
+        if (special) skip = s_map[(v - v0) / 32] >> (v % 32) & 0xFFu;   // a span starts with a word
         if (whole) {
           raw[i].get(l);
         } else {
@@ -257,10 +276,10 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
           for (int e = 0; e < kPiece; ++e) l[e] = v + e < v1 ? to_float(x[v + e]) : -INFINITY;
         }
         if (allowed) {
-          const uint32_t bits = allowed[v / 32] >> (v % 32);
+          const uint32_t a = bits[i] >> (v % 32);
 #pragma unroll
           for (int e = 0; e < kPiece; ++e)
-            if (!(bits >> e & 1u)) l[e] = -INFINITY;
+            if (!(a >> e & 1u)) l[e] = -INFINITY;
         }
       } else {
 #pragma unroll
@@ -269,19 +288,20 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
           l[e] = -INFINITY;
           if (u < v1) {
             l[e] = to_float(x[u]);
-            if (special) skip |= (map[(u - v0) / 32] >> ((u - v0) % 32) & 1u) << e;
+            if (special) skip |= (s_map[(u - v0) / 32] >> (u % 32) & 1u) << e;
             if (allowed && !(allowed[u / 32] >> (u % 32) & 1u)) l[e] = -INFINITY;
           }
         }
       }
+      load(i, v + kAhead * kAcross);
       if (out) {
-        if (WIDE && whole && p.wide_out && !skip) {
+        if (WIDE && whole && p.wide_out) {
           reinterpret_cast<float4*>(out + v)[0] = make_float4(l[0], l[1], l[2], l[3]);
           reinterpret_cast<float4*>(out + v)[1] = make_float4(l[4], l[5], l[6], l[7]);
         } else {
 #pragma unroll
           for (int e = 0; e < kPiece; ++e)
-            if (v + e * kApart < v1 && !(skip >> e & 1u)) out[v + e * kApart] = l[e];
+            if (v + e * kApart < v1) out[v + e * kApart] = l[e];
         }
       }
       if (skip)
@@ -296,44 +316,41 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
           if (l[e] == top) best_at = v + e * kApart;
       }
     }
-    load(v0 + p.stretch);     // nothing behind row_end
+  }
 
-    // ---- sparse: the listed tokens ----
-    if (special) {
-      const int n = s_listed[parity];
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const int at = listed[i], v = v0 + at;
-        float l = to_float(x[v]);
-        if (p.history) {
-          const int said = count[at];
-          count[at] = 0;
-          if (said) {
-            l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
-            if (said & 0x7FFFFFFF) l = __fsub_rn(__fsub_rn(l, __fmul_rn(freq, (float)(said & 0x7FFFFFFF))), pres);
-          }
-        }
-        if (p.bias_starts) {
-          const int k = entry[at];
-          entry[at] = -1;
-          if (k >= 0) l = __fadd_rn(l, p.bias_values[k]);
-        }
-        if (allowed && !(allowed[v / 32] >> (v % 32) & 1u)) l = -INFINITY;
-        if (out) out[v] = l;
-        if (l > best || (l == best && v < best_at && l > -INFINITY)) {
-          best = l;
-          best_at = v;
-        }
+  // ---- the special tokens, over what the dense pass wrote ----
+  // (Out may be the logits themselves: the dense pass then leaves an allowed one as
+  // it is, and a masked one ends as -inf whatever it is computed from.)
+#pragma unroll 1
+  for (int r0 = 0; r0 < specials; r0 += kTable) {
+    if (r0 > 0) {
+      __syncthreads();
+      clear();
+      __syncthreads();
+      tally(r0);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(kTable, specials - r0); i += kThreads) {
+      const int v = v0 + s_token[i], said = s_count[i], k = s_entry[i];
+      float l = to_float(x[v]);
+      if (said) {
+        l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
+        if (said & 0x7FFFFFFF) l = __fsub_rn(__fsub_rn(l, __fmul_rn(freq, (float)(said & 0x7FFFFFFF))), pres);
       }
-      // the other stretches' map and length, not used before the next barrier
-      for (int i = threadIdx.x; i < kMaxStretch / 32; i += kThreads) s_map[parity ^ 1][i] = 0u;
-      if (threadIdx.x == 0) s_listed[parity ^ 1] = 0;
+      if (k >= 0) l = __fadd_rn(l, p.bias_values[k]);
+      if (allowed && !(allowed[v / 32] >> (v % 32) & 1u)) l = -INFINITY;
+      if (out) out[v] = l;
+      if (l > best || (l == best && v < best_at && l > -INFINITY)) {
+        best = l;
+        best_at = v;
+      }
     }
   }
   if (!p.token) return;
   // the CTA's best value, then the lowest index that has it
   const unsigned mine = orderable(best);
   const unsigned warp_best = __reduce_max_sync(0xffffffffu, mine);
-  if (threadIdx.x % 32 == 0) s_best[threadIdx.x / 32] = warp_best;
+  if (lane == 0) s_best[warp] = warp_best;
   __syncthreads();
   unsigned top = 0u;
 #pragma unroll
@@ -341,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   if (mine == top && best > -INFINITY) atomicMin(&s_at, best_at);
   __syncthreads();
   if (threadIdx.x == 0) {
-    if (s_at != 0x7FFFFFFF)
+    if (s_at != kNone)
       atomicMax(p.keys + b, (unsigned long long)top << 32 | (unsigned long long)(0xFFFFFFFFu - (unsigned)s_at));
     __threadfence();
     if (atomicAdd(p.tickets + b, 1) == (int)gridDim.x - 1) {   // the row's last CTA
@@ -353,14 +370,12 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   }
 }
 
-// A CTA's stretches: short ones, one a CTA, until few rows fill the device; then
-// as many a CTA as leave it full (four CTAs an SM), so that the history is read rarely.
-static void cut(int B, int V, int* stretch, int* per_cta) {
-  int s = kMaxStretch;
-  while (s > 512 && (long long)B * ((V + s - 1) / s) < 296) s /= 2;
-  const int n = (V + s - 1) / s, ctas = std::max(1, std::min(n, 592 / B));
-  *stretch = s;
-  *per_cta = (n + ctas - 1) / ctas;
+// The span of a CTA: one wave of CTAs (four an SM) over the rows, each at least a
+// few hundred logits and at most what the bitmap holds.
+static int span_for(int B, int V) {
+  const int ctas = std::max(1, 592 / B);
+  const int span = ((V + ctas - 1) / ctas + 511) / 512 * 512;
+  return std::min(span, kMaxSpan);
 }
 
 static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -420,14 +435,12 @@ int anvilq_logits_process(const void* logits, int logits_half, long long logits_
   p.tickets = token ? reinterpret_cast<int*>(static_cast<char*>(workspace) + kTicketOffset) : nullptr;
   p.dev_err = dev_err;
   p.V = V; p.L = L; p.bias_total = bias_total; p.masks = masks;
-  cut(B, V, &p.stretch, &p.per_cta);
-  const size_t smem = history || bias_starts ? (size_t)p.stretch * (4 * ((history ? 1 : 0) + (bias_starts ? 1 : 0)) + 2) : 0;
+  p.span = span_for(B, V);
   const bool wide = aligned(logits, 16) && logits_stride % (logits_half ? 8 : 4) == 0;
   p.wide_out = out && aligned(out, 16) && out_stride % 4 == 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((V + p.stretch * p.per_cta - 1) / (p.stretch * p.per_cta), B);
+  cfg.gridDim = dim3((V + p.span - 1) / p.span, B);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

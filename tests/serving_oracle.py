@@ -1,4 +1,6 @@
 """Plain 64-bit forms of the paged-cache serving operators, and case makers (CPU)."""
+from collections import Counter
+
 import numpy as np
 import torch
 
@@ -83,10 +85,11 @@ def logits(x, history, lens, prompts, rep, pres, freq, bias, allowed, real=np.fl
             h = [int(t) for t in history[b, :lens[b]]]
             said = h[max(0, 0 if prompts is None else int(prompts[b])):]
             r, p, f = one(rep, b), one(pres, b), one(freq, b)
+            count = Counter(said)
             for t in set(h):
                 if r is not None:
                     y[b, t] = y[b, t] / r if y[b, t] > 0 else y[b, t] * r
-                n = said.count(t)
+                n = count[t]
                 if n:
                     y[b, t] = (y[b, t] - (real(0) if f is None else f * real(n))) - (real(0) if p is None else p)
         if bias is not None:

@@ -484,6 +484,29 @@ def test_logits(dev, B, V, L, biases, grammar, half):
     assert rest[1] is None and torch.equal(rest[0], out)
 
 
+def test_logits_long_histories(dev):
+    """A row a CTA, with more special tokens than its tables hold at a time, and a
+    history longer than a CTA keeps; in place and not."""
+    rng = np.random.default_rng(19)
+    B, V, L, n = 600, 5000, 4500, 300
+    x, history, lens, prompts, rep, pres, freq = logits_case(rng, B, V, L, False, zipf=False)
+    lens[:] = L - np.arange(B) % 7
+    prompts = np.minimum(prompts, lens)
+    d = lambda a: to(a, dev)
+    ids, w = rng.integers(0, V, (B, n)).astype(np.int32), rng.standard_normal((B, n)).astype(np.float32)
+    allowed = rng.random((B, V)) < 0.7
+    kw = dict(history=d(history), history_lens=d(lens), prompt_lens=d(prompts), repetition=d(rep), presence=d(pres),
+              frequency=d(freq), bias_starts=d(np.arange(0, B * n + 1, n, dtype=np.int32)), bias_ids=d(ids.ravel()),
+              bias_values=d(w.ravel()), allowed=d(so.pack_mask(allowed)))
+    out, tokens = ops.logits_process(d(x), **kw)
+    ops.raise_device_errors(dev)
+    bias = [[(int(t), float(v)) for t, v in zip(ids[b], w[b])] for b in range(B)]
+    check_logits(dev, x, out, tokens, (history, lens, prompts, rep, pres, freq, bias, allowed))
+    same = d(x)
+    again, tokens2 = ops.logits_process(same, out=same, **kw)
+    assert torch.equal(again, out) and torch.equal(tokens2, tokens)
+
+
 @pytest.mark.parametrize("given", [(), ("repetition",), ("presence",), ("frequency",), ("allowed",), ("bias",)])
 def test_logits_parts_alone(dev, given):
     """Each part without the others; rows that share masks or have none; prompt lengths left out."""
