@@ -13,13 +13,12 @@
 // 4 KB of V codes at D = 128, in runs of 2 KB at least.  The rows of a tile's
 // products are the Q * Hq/Hkv query rows of its kv head, in groups of 8 or 16
 // (kRows); a pair is a (sequence, kv head, row group).  All pairs' tiles in a row --
-// sequence, then pair, then tile -- are cut into chunks, one CTA each, and a chunk
-// into equal stretches, one a warp, so that the device is evenly loaded whatever
-// the lengths; the lengths are on the device, so every warp finds its stretch from
-// them.  A pair inside one warp's stretch is finished by that warp.  The others'
-// partial softmax states are merged in shared memory, and where a pair spans
-// chunks, by the CTA that arrives last at the pair's ticket, in chunk order
-// (bit-reproducible).  plan_of has the rules.
+// sequence, then pair, then tile -- are cut into equal stretches, one a warp, so that
+// the device is evenly loaded whatever the lengths; the lengths are on the device,
+// so every warp finds its stretch from them.  A pair inside one warp's stretch is
+// finished by that warp.  The others' partial softmax states are merged in shared
+// memory, and where a pair spans CTAs, by the CTA that arrives last at the pair's
+// ticket, in CTA order (bit-reproducible).  plan_of has the rules.
 //
 // A warp streams its tiles through its own TMA ring, mbarrier by mbarrier.  The
 // codes never return to memory as binary16: fragments of mma.m16n8k16 are formed
@@ -58,9 +57,7 @@ namespace attn8 {
 
 using q8::kBlock;
 constexpr int kTile = 2 * kBlock;   // tokens of a step
-constexpr int kMaxSms = 160;                  // SMs that are used
-constexpr int kMaxChunks = 9 * kMaxSms;       // chunks of a call that pairs may span (plan_of: at most 4.25 a CTA)
-constexpr int kTickets = 2;                   // counters before the tickets
+constexpr int kMaxSms = 160;        // SMs that are used, one CTA each
 constexpr unsigned long long kWaitLimitNs = 1000000000ull;
 
 struct Divisor {     // x / d for 0 <= x < 2^17, 1 <= d < 2^15: the error of m is below d / 2^32
@@ -76,8 +73,8 @@ struct Params {
   const uint32_t* page_table;  // [B][max_pages]
   const int* seqlens;          // [B]
   __half* out;                 // [B][Q][Hq][D]
-  int* counters;               // next chunk, CTAs done, then a ticket a chunk (of the pair that goes on from it)
-  float* partials;             // [chunk][2] states: of the pair begun earlier, of the pair that goes on
+  int* tickets;                // one a CTA, of the pair that goes on from it
+  float* partials;             // [CTA][2] states: of the pair begun earlier, of the pair that goes on
   float* parked;               // [CTA][warp] states
   int* dev_err;
   int B, Q, Hq, Hkv, page_tokens, max_pages, num_pages;
@@ -91,10 +88,9 @@ template <int D_, int RT_>
 struct Shape {
   static constexpr int D = D_, RT = RT_;
   static constexpr int kRows = 8 * RT;
-  static constexpr int kWarps = RT == 1 ? 6 : 4;               // 168 or 255 registers a thread
+  static constexpr int kWarps = RT == 1 ? 12 : 8;              // one CTA an SM: 168 or 255 registers a thread
   static constexpr int kThreads = kWarps * 32;
-  static_assert(kWarps <= 6, "Control has room for their parts");
-  static constexpr int kCtas = 2;                              // per SM
+  static_assert(kWarps <= 12, "Control has room for their parts");
   static constexpr int kTileBytes = kTile * D;                 // of K or V
   static constexpr int kStageBytes = 2 * kTileBytes;
   // 16 KB a warp: the copies of all warps in flight are several times what the
@@ -112,7 +108,7 @@ struct Shape {
   static constexpr int kPartial = kState + 2 * kRows;          // floats of a state in global memory
   static_assert((kStages & (kStages - 1)) == 0 && kStages <= 4, "a slot's old tile is used by the time it is named again");
   static_assert(kRingBytes >= kState * 4, "a state fits the idle ring");
-  static_assert(kCtas * (kTotal + 2048) <= 227 * 1024, "CTAs per SM");
+  static_assert(kTotal + 4096 <= 227 * 1024, "one CTA an SM");
 };
 
 struct Meta {        // a tile: what its copies and its consumer need
@@ -129,11 +125,11 @@ struct Part {        // a pair that a warp did not finish alone
   int n, b, pair;
 };
 
-// How the work is cut.  Sizes in tiles; a warp's stretch of a chunk is 1 / kWarps of it.
+// How the work is cut: a warp's stretch is 1 / kWarps of a CTA's tiles.
 struct Plan {
-  bool whole;        // a chunk is a pair, whatever its length
+  bool whole;        // CTAs take whole pairs in turn
   unsigned total;    // tiles in all
-  unsigned first, rest;   // size of the first gridDim.x chunks, and of the others
+  unsigned chunk;    // else: tiles of a CTA
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -210,28 +206,21 @@ __device__ __forceinline__ void e4m3x4_to_half4(uint32_t w, uint32_t& lo, uint32
 // the swizzle, 8 different 16-byte banks either way.
 __device__ __forceinline__ int token_of(int n) { return (n & 8) | ((n & 1) ? ((n & 6) ^ 5) : (n & 7)); }
 
-// Rules, each measured on a B200 (DESIGN section on this kernel has the cases):
-//   * a CTA a pair, when that costs no CTA more than a few tiles a warp over equal
-//     stretches: it saves the merge across CTAs (tickets and a round trip through
-//     L2, about as long as kMergeTiles tiles).
-//   * equal stretches otherwise; a long row of tiles is cut twice: most of it into
-//     one chunk a CTA, the rest into small chunks that CTAs take as they finish,
-//     because SMs do not get equal shares of the memory's bandwidth.
-constexpr int kMergeTiles = 3;
-constexpr int kLongStretch = 64;    // tiles of a warp from which the end is dealt out
-constexpr int kDealtSpan = 64;      // ... unless a pair would be spread over more chunks than these
+// A CTA a pair, when no warp then has more tiles than with equal shares: it saves
+// the merge across CTAs (tickets and a round trip through L2).  One sequence of 150
+// tokens, 14/2 heads of 64: 6.7 us against 12.0.  With a few tiles more than equal
+// shares it already loses: 1500 tokens 12.7 us against 10.3.  Equal shares otherwise:
+// 32 sequences x 32768 tokens, 32/8 heads of 128, 332 us; with the last sixth of the
+// work dealt out in small chunks as CTAs finish 351 us (each chunk drains a CTA's
+// pipeline), and two CTAs an SM instead of one larger 364 us.
 template <int W>
 __device__ __forceinline__ Plan plan_of(unsigned total, int longest, int all_pairs, int ctas) {
   Plan pl;
   pl.total = total;
   const unsigned even = max(1u, (total + ctas * W - 1) / (ctas * W));
   const unsigned rounds = (all_pairs + ctas - 1) / ctas;
-  pl.whole = rounds * ((longest + W - 1) / W) <= even + kMergeTiles;
-  pl.first = pl.rest = even * W;
-  if (even >= kLongStretch && longest <= kDealtSpan * (even / 16) * W) {
-    pl.rest = (even / 16) * W;
-    pl.first = (even - even / 6) * W;
-  }
+  pl.whole = rounds * ((longest + W - 1) / W) <= even;
+  pl.chunk = even * W;
   return pl;
 }
 
@@ -241,30 +230,21 @@ __device__ __forceinline__ int tiles_of(const Params& p, int b) {
   return n < 0 || n > p.page_tokens * p.max_pages ? 0 : (n + kTile - 1) / kTile;
 }
 
-constexpr int kMaxWarps = 6;
+constexpr int kMaxWarps = 12;
 enum { kHas0 = 1, kEnds0 = 2, kParked0 = 4, kHas1 = 8 };
 struct Control {     // in shared memory
   Part part[kMaxWarps][2];   // [0] a pair begun before the warp's stretch, [1] one that goes on after it
   int flags[kMaxWarps];      // kHas0 ...
-  int next, last[2];
-  uint2 open[2];             // first chunk and number of chunks of a pair that spans several
+  int last[2];
+  uint2 open[2];             // first CTA and number of CTAs of a pair that spans several
   Plan plan;                 // out of the registers of the tile loop; every warp writes the same
-  __device__ __forceinline__ unsigned chunk_at(unsigned k) const {   // first tile of chunk k
-    return k <= gridDim.x ? k * plan.first : gridDim.x * plan.first + (k - gridDim.x) * plan.rest;
-  }
-  __device__ __forceinline__ unsigned chunk_of(unsigned x) const {   // the chunk of tile x
-    const unsigned head = gridDim.x * plan.first;
-    return x < head ? x / plan.first : gridDim.x + (x - head) / plan.rest;
-  }
-  // some chunks are taken as CTAs finish
-  __device__ __forceinline__ bool dealt() const { return !plan.whole && plan.total > gridDim.x * plan.first; }
 };
 
 // One warp's stretch: `count` tiles from tile `begin` of the row on, b and base a
 // sequence no later than the first tile's and where its tiles start.  Pairs inside
-// it are finished, the states of others left for merge_chunk.  `before`: tiles of
+// it are finished, the states of others left for merge_states.  `before`: tiles of
 // the warp's earlier stretches.  False after a wait that ran out.  A function of
-// its own, as merge_chunk is: in one body the compiler spilled this loop's state
+// its own, as merge_states is: in one body the compiler spilled this loop's state
 // (1.6 times the time).
 template <int D, int TYPE, int RT>
 __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,
@@ -664,10 +644,10 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
   return ok;
 }
 
-// Merges what the warps left of a chunk (frugal with registers: the tile loop's
+// Merges what the warps left (frugal with registers: the tile loop's
 // share the kernel's with this).
 template <int D, int RT>
-__device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem, Control& ctl, unsigned chunk) {
+__device__ __forceinline__ void merge_states(const Params& p, unsigned char* smem, Control& ctl) {
   using S = Shape<D, RT>;
   constexpr int W = S::kWarps;
   constexpr int kVec = S::kRows * (D / 4);   // float4s of a state
@@ -697,7 +677,7 @@ __device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem
     parked0 = __ballot_sync(0xffffffffu, fl & kParked0);
     starts = __ballot_sync(0xffffffffu, fl & kHas1) << 1 | (has0 & 1);   // bit 0: slot 0 of warp 0; bit w + 1: slot 1 of w
   }
-  int open = 0;        // bit s: the pair of ctl.part[open warp][s] spans chunks
+  int open = 0;        // bit s: the pair of ctl.part[open warp][s] spans CTAs
   int open_warp1 = 0;  // (that of slot 0 is warp 0's)
 #pragma unroll 1
   for (; starts; starts &= starts - 1) {
@@ -709,7 +689,7 @@ __device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem
       ++members;
     }
     const bool whole = slot == 1 && ended;
-    float* out = p.partials + ((size_t)chunk * 2 + slot) * S::kPartial;
+    float* out = p.partials + ((size_t)blockIdx.x * 2 + slot) * S::kPartial;
     const float2* stat = stats + (w * 2 + slot) * S::kRows;   // of members after the first: slot 0 of their warps
 #pragma unroll 1
     for (int at = threadIdx.x; at < kVec; at += S::kThreads) {
@@ -738,7 +718,7 @@ __device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem
     }
   }
 
-  // ---- pairs that span chunks: the last CTA to arrive merges, in chunk order ----
+  // ---- pairs that span CTAs: the last CTA to arrive merges, in CTA order ----
   __syncthreads();   // the partials are written (and the rings free again)
   if (!open) return;
   if (threadIdx.x < 2) {
@@ -746,8 +726,8 @@ __device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem
     bool last = false;
     if (open >> slot & 1) {
       const Part pt = ctl.part[slot ? open_warp1 : 0][slot];
-      const unsigned c0 = ctl.chunk_of(pt.first), c1 = ctl.chunk_of(pt.first + pt.n - 1);
-      int* ticket = p.counters + kTickets + c0;
+      const unsigned c0 = pt.first / ctl.plan.chunk, c1 = (pt.first + pt.n - 1) / ctl.plan.chunk;
+      int* ticket = p.tickets + c0;
       // releases the CTA's partials (through the barrier above) and acquires the others'
       int arrived;
       asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(arrived) : "l"(ticket) : "memory");
@@ -766,7 +746,8 @@ __device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem
   const int threads = both == 2 ? S::kThreads / 2 : S::kThreads;
   const int slot = both == 2 ? (int)threadIdx.x / threads : ctl.last[1], me = both == 2 ? threadIdx.x % threads : threadIdx.x;
   unsigned char* room = smem + (both == 2 ? slot * (W / 2) * S::kRingBytes : 0);
-  constexpr int kFit = W / 2 * S::kRingBytes / (S::kPartial * 4);         // states that fit half of the rings
+  constexpr int kFitAll = W * S::kRingBytes / (S::kPartial * 4), kFitHalf = W / 2 * S::kRingBytes / (S::kPartial * 4);
+  const int fit = both == 2 ? kFitHalf : kFitAll;                         // states that fit the room
   constexpr int kMine = (2 * kVec + S::kThreads - 1) / S::kThreads;       // float4s of a thread, at most
   auto sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(threads) : "memory"); };
   const unsigned c0 = ctl.open[slot].x;
@@ -780,13 +761,16 @@ __device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem
     acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
 #pragma unroll 1
-  for (int k0 = 0; k0 < n; k0 += kFit) {
-    const int m = min(kFit, n - k0);
-    // the states of m chunks, all on their way at once
-    for (int i = me; i < m * (S::kPartial / 4); i += threads) {
-      const int k = i / (S::kPartial / 4), at = i % (S::kPartial / 4);
-      // the first chunk's state is of a pair that goes on, the others' of one begun earlier
-      copy16_async(smem_u32(room) + 16 * i, p.partials + ((size_t)(c0 + k0 + k) * 2 + (k0 + k == 0)) * S::kPartial + 4 * at);
+  for (int k0 = 0; k0 < n; k0 += fit) {
+    const int m = min(fit, n - k0);
+    // the states of m CTAs, all on their way at once
+#pragma unroll 1
+    for (int k = 0; k < m; ++k) {
+      // the first CTA's state is of a pair that goes on, the others' of one begun earlier
+      const float* from = p.partials + ((size_t)(c0 + k0 + k) * 2 + (k0 + k == 0)) * S::kPartial;
+#pragma unroll 2
+      for (int at = me; at < S::kPartial / 4; at += threads)
+        copy16_async(smem_u32(room) + (k * (S::kPartial / 4) + at) * 16, from + 4 * at);
     }
     copies_done();
     sync();
@@ -807,7 +791,7 @@ __device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem
         add_state(top, lsum[i], acc[i], reinterpret_cast<const float2*>(state + k * S::kPartial + S::kState)[row],
                   reinterpret_cast<const float4*>(state + k * S::kPartial)[at]);
     }
-    if (k0 + kFit < n) sync();   // the room is used again
+    if (k0 + fit < n) sync();   // the room is used again
   }
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
@@ -817,7 +801,7 @@ __device__ __forceinline__ void merge_chunk(const Params& p, unsigned char* smem
 }
 
 template <int D, int TYPE, int RT>
-__global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
+__global__ void __launch_bounds__(Shape<D, RT>::kThreads, 1)
     gqa_decode_q8_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                          const __grid_constant__ Params p) {
   using S = Shape<D, RT>;
@@ -855,31 +839,30 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
     if (lane == 0) ctl.plan = plan;
     __syncwarp();
   }
-  uint32_t before = 0;   // tiles of earlier chunks: tile j's stage and parity follow from before + j
+  uint32_t before = 0;   // tiles of earlier rounds: tile j's stage and parity follow from before + j
   bool ok = true;
-  for (unsigned chunk = blockIdx.x;;) {
+  for (unsigned mine = blockIdx.x;; mine += gridDim.x) {   // pair, or chunk
     // ---- this warp's stretch: `count` tiles from `begin` on ----
     unsigned begin = 0;
     int count = 0;
     int b_first = 0;           // the sequence of the first tile, and where its tiles start
     unsigned base_first = 0;
     if (ctl.plan.whole) {
-      if (chunk >= (unsigned)(p.B * pairs)) break;
-      b_first = chunk / pairs;
+      if (mine >= (unsigned)(p.B * pairs)) break;
+      b_first = mine / pairs;
       const int n = tiles_of(p, b_first), share = (n + W - 1) / W;
       // any row's start will do: nothing refers to tiles of other sequences
-      begin = (chunk - b_first * pairs) * n + warp * share;
+      begin = (mine - b_first * pairs) * n + warp * share;
       count = max(0, min(n - warp * share, share));
     } else {
-      const unsigned from = ctl.chunk_at(chunk);
-      if (from >= ctl.plan.total) break;
-      const unsigned share = (chunk < gridDim.x ? ctl.plan.first : ctl.plan.rest) / W;
+      const unsigned from = mine * ctl.plan.chunk;
+      if (mine >= gridDim.x || from >= ctl.plan.total) break;
+      const unsigned share = ctl.plan.chunk / W;
       begin = from + warp * share;
       count = begin < ctl.plan.total ? (int)min(share, ctl.plan.total - begin) : 0;
-      if (threadIdx.x == 0 && ctl.dealt()) ctl.next = gridDim.x + atomicAdd(p.counters, 1);
       for (int b0 = 0; count > 0; b0 += 32) {
-        const unsigned mine = b0 + lane < p.B ? tiles_of(p, b0 + lane) * pairs : 0;
-        unsigned incl = mine;
+        const unsigned tiles = b0 + lane < p.B ? tiles_of(p, b0 + lane) * pairs : 0;
+        unsigned incl = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
@@ -889,32 +872,21 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, Shape<D, RT>::kCtas)
         if (past || b0 + 32 >= p.B) {   // some sequence holds it, as begin < total
           const int l = past ? __ffs(past) - 1 : (p.B - 1) % 32;
           b_first = b0 + l;
-          base_first += __shfl_sync(0xffffffffu, incl - mine, l);
+          base_first += __shfl_sync(0xffffffffu, incl - tiles, l);
           break;
         }
         base_first += __shfl_sync(0xffffffffu, incl, 31);
       }
     }
     if (ok) ok = run_stretch<D, TYPE, RT>(mk, mv, p, smem, ctl, before, begin, count, b_first, base_first);
-    else if (threadIdx.x % 32 == 0) ctl.flags[warp] = 0;
+    else if (lane == 0) ctl.flags[warp] = 0;
     before += count;
     __syncthreads();
-
-    merge_chunk<D, RT>(p, smem, ctl, chunk);
-    // the next chunk: the ring's generic reads and writes end before copies fill it again
-    if (ctl.plan.whole) {
-      chunk += gridDim.x;
-    } else if (ctl.dealt()) {
-      chunk = ctl.next;
-    } else {
-      break;
-    }
+    merge_states<D, RT>(p, smem, ctl);
+    if (!ctl.plan.whole) break;
+    // the next pair: the ring's generic reads and writes end before copies fill it again
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-  }
-  if (threadIdx.x == 0 && ctl.dealt() && atomicAdd(p.counters + 1, 1) == (int)gridDim.x - 1) {
-    p.counters[0] = 0;   // the last CTA: nobody takes a chunk any more
-    p.counters[1] = 0;
   }
   // empty sequences (and lengths that are none)
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
@@ -964,9 +936,9 @@ static int sm_count() {
 // 8 rows a pair where they suffice, else 16 (the MMA's row count): more rows
 // would leave too few registers for enough warps
 static int row_tiles(int Q, int Hq, int Hkv) { return Q * (Hq / Hkv) <= 8 ? 1 : 2; }
-static int max_ctas(int sms) { return 2 * std::min(sms, kMaxSms); }
-static size_t partial_floats(int rt, int D) { return (size_t)kMaxChunks * 2 * (8 * rt) * (D + 2); }
-static size_t parked_floats(int rt, int D, int sms) { return (size_t)max_ctas(sms) * (rt == 1 ? 6 : 4) * (8 * rt) * D; }
+static int max_ctas(int sms) { return std::min(sms, kMaxSms); }
+static size_t partial_floats(int rt, int D, int sms) { return (size_t)max_ctas(sms) * 2 * (8 * rt) * (D + 2); }
+static size_t parked_floats(int rt, int D, int sms) { return (size_t)max_ctas(sms) * (rt == 1 ? 12 : 8) * (8 * rt) * D; }
 
 static std::once_flag g_encode_once;
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
@@ -1023,7 +995,7 @@ size_t anvilq_gqa_decode_q8_workspace_size(int B, int Q, int Hq, int Hkv, int D)
   const int sms = sm_count();
   if (sms <= 0) return 0;
   const int rt = row_tiles(Q, Hq, Hkv);
-  return ANVILQ_WORKSPACE_COUNTER_BYTES + (partial_floats(rt, D) + parked_floats(rt, D, sms)) * sizeof(float);
+  return ANVILQ_WORKSPACE_COUNTER_BYTES + (partial_floats(rt, D, sms) + parked_floats(rt, D, sms)) * sizeof(float);
 }
 
 int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_codes, const float* k_scales,
@@ -1054,9 +1026,9 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   p.page_table = page_table;
   p.seqlens = seqlens;
   p.out = reinterpret_cast<__half*>(out);
-  p.counters = static_cast<int*>(workspace);
+  p.tickets = static_cast<int*>(workspace);
   p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + ANVILQ_WORKSPACE_COUNTER_BYTES);
-  p.parked = p.partials + partial_floats(rt, D);
+  p.parked = p.partials + partial_floats(rt, D, sms);
   p.dev_err = dev_err;
   p.B = B; p.Q = Q; p.Hq = Hq; p.Hkv = Hkv;
   auto divisor = [](int d) { return Divisor{d, d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d)}; };
@@ -1064,9 +1036,11 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   p.row_groups = divisor((Q * (Hq / Hkv) + 8 * rt - 1) / (8 * rt));
   p.page_tokens = page_tokens; p.max_pages = max_pages; p.num_pages = num_pages;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
-  // as many CTAs as the device holds, but no more warps than the table has room for tiles
+  // as many CTAs as the device holds, but no more than there can be work for: a pair
+  // each, or a tile a warp of what the table has room for
   const double tiles = (double)B * Hkv * p.row_groups.d * ((double)max_pages * page_tokens / kTile + 1);
-  const int ctas = (int)std::max(1.0, std::min((double)max_ctas(sms), std::ceil(tiles / warps)));
+  const double all_pairs = (double)B * Hkv * p.row_groups.d;
+  const int ctas = (int)std::min((double)max_ctas(sms), std::max(all_pairs, std::ceil(tiles / warps)));
   if (tiles > (double)(1u << 31)) return ANVILQ_ESHAPE;   // tiles are counted in 32 bits
   CUtensorMap mk, mv;
   p.wide = page_tokens % kTile == 0;

@@ -57,11 +57,11 @@ def pool_values(codes: torch.Tensor, scales: torch.Tensor) -> np.ndarray:
 
 def attention(q, k, v, len_, Q, scale, ks=None):
     """One sequence: q [Q, Hq, D], k / v [len, Hkv, D] -> out [Q, Hq, D], and the sums the
-    error bound needs: sum p |v| and the largest sum |q| |k| over what a row sees."""
+    error bound needs: sum p |v|, the largest sum |q| |k| and sum |v| over what a row sees."""
     Hq, D = q.shape[1:]
     Hkv = k.shape[1] if len_ else 1
     g = Hq // Hkv
-    out, mass, reach = np.zeros((Q, Hq, D)), np.zeros((Q, Hq, D)), np.zeros((Q, Hq, 1))
+    out, mass, reach, size = np.zeros((Q, Hq, D)), np.zeros((Q, Hq, D)), np.zeros((Q, Hq, 1)), np.zeros((Q, Hq, D))
     for i in range(Q):
         n = len_ - Q + 1 + i
         if n < 1:
@@ -73,7 +73,8 @@ def attention(q, k, v, len_, Q, scale, ks=None):
             out[i, h] = p @ v[:n, h // g]
             mass[i, h] = p @ np.abs(v[:n, h // g])
             reach[i, h] = (np.abs(k[:n, h // g]).max() * np.abs(q[i, h]).sum()) * scale
-    return out, mass, reach
+            size[i, h] = np.abs(v[:n, h // g]).sum(axis=0)
+    return out, mass, reach, size
 
 
 def logits(x, history, lens, prompts, rep, pres, freq, bias, allowed, real=np.float64):

@@ -9,7 +9,11 @@ all of it.  Attention: the probabilities enter the tensor cores in binary16, 2^-
 sum p |v|; the scores' binary32 sums of D products of at most 2 |q| max |k| each (codes
 are summed with an offset that at most doubles them; 8 accumulation steps of at most
 2^-22 each) move a probability by a relative 2^-18 sum |q| max |k|, at most twice (in the
-sum and in the product)."""
+sum and in the product).  What a probability times its block's scale loses below
+binary16's normal range: it enters as p s / F with F at most 8 times the scale s (or the
+scale is 0) and p taken against a reference at least 4 (log2) below the stretch's largest
+score, so that the sum of p is at least 2^4.  Its rounding there is at most 2^-25, of the
+result 2^-25 8 / 2^4 sum |v| = 2^-26 sum |v|; merging stretches averages these."""
 import numpy as np
 import pytest
 import torch
@@ -321,8 +325,8 @@ def check_attention(out, q, k, v, ks, vs, table, lens, scale=0.0):
     for b, n in enumerate(lens):
         at = [so.physical(e) for e in table[b, :-(-n // page)]]
         flat = lambda p: p[at].transpose(0, 2, 1, 3).reshape(-1, Hkv, D)[:n]
-        ref, mass, reach = so.attention(q[b].astype(np.float64), flat(kv), flat(vv), n, Q, scale)
-        tol = HALF * np.abs(ref) + mass * (HALF * (1 + 2.0 ** -6) + 2 * 2.0 ** -18 * reach) + 2.0 ** -24
+        ref, mass, reach, size = so.attention(q[b].astype(np.float64), flat(kv), flat(vv), n, Q, scale)
+        tol = HALF * np.abs(ref) + mass * (HALF * (1 + 2.0 ** -6) + 2 * 2.0 ** -18 * reach) + 2.0 ** -24 + 2.0 ** -26 * size
         bad = np.abs(out[b].astype(np.float64) - ref) > tol
         assert not bad.any(), (b, n, np.argwhere(bad)[:4], np.abs(out[b] - ref).max())
 
@@ -699,7 +703,7 @@ def test_binary16_pages_append_then_attend(dev):
     for b in range(2):
         at = [so.physical(e) for e in table[b, :-(-lens[b] // page)]]
         flat = lambda p: p.cpu().numpy()[at].reshape(-1, Hkv, D)[:lens[b]].astype(np.float64)
-        ref, mass, reach = so.attention(last[b:b + 1].cpu().numpy().astype(np.float64), flat(k), flat(v), int(lens[b]), 1,
+        ref, mass, reach, _ = so.attention(last[b:b + 1].cpu().numpy().astype(np.float64), flat(k), flat(v), int(lens[b]), 1,
                                         1 / np.sqrt(D))
         tol = HALF * np.abs(ref) + mass * (HALF * (1 + 2.0 ** -6) + 2 * 2.0 ** -18 * reach) + 2.0 ** -24
         assert (np.abs(out[b] - ref[0]) <= tol[0]).all()
