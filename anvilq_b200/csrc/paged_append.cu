@@ -439,10 +439,17 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   int slices = 1;
   while (slices * 8 < heads && (long long)items * slices < 148 * 2) slices *= 2;
   p.heads_per_cta = (heads + slices - 1) / slices;
-  Freq freq;
-  for (int i = 0; i < D / 2; ++i) freq.inv[i] = std::pow((double)theta, -2.0 * i / D);
+  // the frequencies of the thread's last theta and D (64 powers cost the host 3 us)
+  thread_local Freq freq;
+  thread_local float freq_theta = 0.0f;
+  thread_local int freq_d = 0;
+  if (theta != freq_theta || D != freq_d) {
+    for (int i = 0; i < D / 2; ++i) freq.inv[i] = std::pow((double)theta, -2.0 * i / D);
+    freq_theta = theta;
+    freq_d = D;
+  }
   const dim3 grid(items, (heads + p.heads_per_cta - 1) / p.heads_per_cta);
-  auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, st, flags, p, freq); };
+  auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, st, flags, p, Freq(freq)); };
   if (D == 64)
     return type == kBinary16 ? go(append_kernel<64, kBinary16>)
            : type == q8::kInt8 ? go(append_kernel<64, q8::kInt8>) : go(append_kernel<64, q8::kE4m3>);

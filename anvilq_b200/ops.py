@@ -7,6 +7,7 @@ stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 
 import torch
@@ -602,10 +603,14 @@ def _on_device(name, device, *tensors):
             raise ValueError(f"{name}: all tensors must be on {device}")
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
 def _call(name, device, *args):
     """A library call with `device` current (a stream only takes launches of its own device)."""
     fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == device.index:
         rc = fn(*args)
     else:
         with torch.cuda.device(device):
@@ -623,7 +628,7 @@ def _call_workspace(device, nbytes: int, given) -> torch.Tensor:
                 not given.is_contiguous():
             raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {nbytes} bytes on {device}")
         return given
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         ws[:WORKSPACE_COUNTER_BYTES].zero_()
         return ws
@@ -643,7 +648,7 @@ def _error_word(device, given):
         return given
     w = _dev_err.get(device.index)
     if w is None:
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             raise RuntimeError("run an operation on this device once before capturing a graph")
         w = device_error_word(device)
     return w
@@ -721,9 +726,9 @@ def paged_kv_append(qkv, k_pool, v_pool, page_table, seqlens, token_starts, Hq: 
     dev = qkv.device
     _on_device(name, dev, k_pool, v_pool, page_table, seqlens, token_starts, q_out)
     err = _error_word(dev, dev_err)
-    _call("anvilq_paged_kv_append", dev, _ptr(qkv), stride, _ptr(token_starts), _ptr(seqlens), _ptr(page_table),
-          _ptr(q_out), _ptr(k_pool), _ptr(v_pool), T, B, Hq, Hkv, D, page, max_pages, pages, float(theta), _ptr(err),
-          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    _call("anvilq_paged_kv_append", dev, qkv.data_ptr(), stride, token_starts.data_ptr(), seqlens.data_ptr(),
+          page_table.data_ptr(), q_out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), T, B, Hq, Hkv, D, page,
+          max_pages, pages, float(theta), err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return q_out
 
 
@@ -742,9 +747,9 @@ def paged_kv_append_q8(qkv, k_codes, v_codes, k_scales, v_scales, page_table, se
     dev = qkv.device
     _on_device(name, dev, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, token_starts, q_out)
     err = _error_word(dev, dev_err)
-    _call("anvilq_paged_kv_append_q8", dev, _ptr(qkv), stride, _ptr(token_starts), _ptr(seqlens), _ptr(page_table),
-          _ptr(q_out), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), code, T, B, Hq, Hkv, D, page,
-          max_pages, pages, float(theta), _ptr(err), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    _call("anvilq_paged_kv_append_q8", dev, qkv.data_ptr(), stride, token_starts.data_ptr(), seqlens.data_ptr(),
+          page_table.data_ptr(), q_out.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(),
+          v_scales.data_ptr(), code, T, B, Hq, Hkv, D, page, max_pages, pages, float(theta), err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return q_out
 
 
@@ -759,9 +764,15 @@ def kv_q8_values(k_codes, v_codes, k_scales, v_scales, k_out=None, v_out=None, o
         if t.dtype != torch.float16 or t.shape != k_codes.shape or not t.is_contiguous():
             raise ValueError(f"{name}: k_out/v_out must be contiguous float16 with the shape of the codes")
     _on_device(name, dev, v_codes, k_scales, v_scales, k_out, v_out)
-    _call("anvilq_kv_q8_values", dev, _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), code, _ptr(k_out),
-          _ptr(v_out), pages, Hkv, page, D, GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    _call("anvilq_kv_q8_values", dev, k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+          code, k_out.data_ptr(), v_out.data_ptr(), pages, Hkv, page, D, GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return k_out, v_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _q8_workspace_size(index, *shape):
+    with torch.cuda.device(index):     # by its number of SMs
+        return _lib.load().anvilq_gqa_decode_q8_workspace_size(*shape)
 
 
 def gqa_decode_q8(q, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, scale: float = 0.0, out=None,
@@ -789,14 +800,14 @@ def gqa_decode_q8(q, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, 
         raise ValueError(f"{name}: out must be contiguous float16 in q's shape")
     dev = q.device
     _on_device(name, dev, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, out)
-    need = _lib.load().anvilq_gqa_decode_q8_workspace_size(B, Q, Hq, Hkv, D)
+    need = _q8_workspace_size(dev.index, B, Q, Hq, Hkv, D)
     if need == 0:
         raise ValueError(f"{name}: unsupported shape B={B} Q={Q} Hq={Hq} Hkv={Hkv} D={D}")
     ws = _call_workspace(dev, need, workspace)
     err = _error_word(dev, dev_err)
-    _call("anvilq_gqa_decode_q8", dev, _ptr(q), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), code,
-          _ptr(page_table), _ptr(seqlens), _ptr(out), B, Q, Hq, Hkv, D, page, max_pages, pages, float(scale), _ptr(ws),
-          ws.numel(), _ptr(err), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    _call("anvilq_gqa_decode_q8", dev, q.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(),
+          v_scales.data_ptr(), code, page_table.data_ptr(), seqlens.data_ptr(), out.data_ptr(), B, Q, Hq, Hkv, D, page,
+          max_pages, pages, float(scale), ws.data_ptr(), ws.numel(), err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return out
 
 
