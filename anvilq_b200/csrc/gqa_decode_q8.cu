@@ -23,16 +23,21 @@
 // A warp streams its tiles through its own TMA ring, mbarrier by mbarrier.  The
 // codes never return to memory as binary16: fragments of mma.m16n8k16 are formed
 // in registers.
-//   S = Q K^T: a lane's B fragment is a token's 16-byte chunks (the contraction's
-//     order over d is free, so q is loaded in the same order).  An int8 code c
-//     enters as the binary16 subnormal (c + 128) 2^-24 -- a byte beside a zero
+//   S^T = K Q^T: a lane's A fragment is chunks of 16 bytes of two tokens (the
+//     contraction's order over d is free, so q is loaded in the same order).  An int8
+//     code c enters as the binary16 subnormal (c + 128) 2^-24 -- a byte beside a zero
 //     byte, no arithmetic -- and the accumulator starts at -128 2^-24 sum q.  An
 //     e4m3 code is converted (exactly) by the cvt instruction.
-//   O^T += V^T P^T: the accumulator layout of S is the B fragment of P^T; V^T's
-//     fragments pair the bytes of two tokens.  Over a long context the sum of p c
-//     is far smaller than the sum of p, so here an offset would cost precision:
-//     int8 codes are made signed first, (1024 + 128 + c) - 1152 in binary16.
-// The tokens of a block are dealt to fragment columns in an order (token_of) that
+//   O^T += V^T P^T: P^T's B fragment is the accumulator of S^T, packed and
+//     transposed (movmatrix), so a lane holds the same query rows' scores, softmax
+//     statistics and outputs.  V^T's fragments pair the bytes of two tokens.  Over a
+//     long context the sum of p c is far smaller than the sum of p, so here an offset
+//     would cost precision: int8 codes are made signed first,
+//     (1024 + 128 + c) - 1152 in binary16.
+//   (With S = Q K^T instead, eight rows as a 16-row operand, the empty half took as
+//   many MMAs again and its zero registers a move each: 389 instructions a block of
+//   16 tokens.)
+// The tokens of a block are dealt to fragment rows in an order (token_of) that
 // keeps both reads of the 128-byte-swizzled block free of bank conflicts.  Two
 // blocks a step share the waits, votes and bookkeeping: one block a step took 480
 // instructions a block and was bound by their issue, not by memory.
@@ -189,6 +194,12 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// an 8x8 matrix of binary16 values (row lane / 4, columns 2 (lane % 4) and + 1), transposed
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 __device__ __forceinline__ float fast_exp2(float x) {   // 2^x, 2 units in the last place; 0 for -inf
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -200,7 +211,7 @@ __device__ __forceinline__ void e4m3x4_to_half4(uint32_t w, uint32_t& lo, uint32
       : "=r"(lo), "=r"(hi)
       : "r"(w));
 }
-// The token of a block at column n (of 16) of S: within eights, even columns keep
+// The token of a block at row n (of 16) of S^T: within eights, even rows keep
 // their place and odd ones are crossed, so that the two rows of a quarter-warp's
 // K read differ in bit 2 and the four rows of its V read in bits 1 and 2 -- with
 // the swizzle, 8 different 16-byte banks either way.
@@ -322,10 +333,11 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
   };
 
   // ---- the state of the current pair ----
-  uint32_t qa[KS][2 * RT];   // A fragments: rows g (and g + 8)
-  float start[RT];           // where S's accumulators start (int8)
-  float m[RT], l[RT];
-  float o[RT][KS][4];        // O^T: dims g.., rows 8 t + 2 c and + 1
+  uint32_t qb[KS][RT][2];    // B fragments of Q^T: row 8 t + g
+  // of rows 8 t + 2 c and + 1, as all that follows:
+  float start[RT][2];        // where S^T's accumulators start (int8)
+  float m[RT][2], l[RT][2];  // the softmax's reference; the lane's share of its sum
+  float o[RT][KS][4];        // O^T: two dims, two rows
   float F = 1.0f, F_inv = 1.0f;
   int flags = 0;
 
@@ -343,13 +355,13 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
         for (int u = 0; u < 2; ++u) {
           uint4 w = make_uint4(0, 0, 0, 0);
           if (row) w = *reinterpret_cast<const uint4*>(src + 64 * h + 8 * u);
-          qa[4 * h + 2 * u][t] = w.x;
-          qa[4 * h + 2 * u][RT + t] = w.y;
-          qa[4 * h + 2 * u + 1][t] = w.z;
-          qa[4 * h + 2 * u + 1][RT + t] = w.w;
+          qb[4 * h + 2 * u][t][0] = w.x;
+          qb[4 * h + 2 * u][t][1] = w.y;
+          qb[4 * h + 2 * u + 1][t][0] = w.z;
+          qb[4 * h + 2 * u + 1][t][1] = w.w;
         }
-      m[t] = -1e30f;
-      l[t] = 0.0f;
+      m[t][0] = m[t][1] = -1e30f;
+      l[t][0] = l[t][1] = 0.0f;
 #pragma unroll
       for (int mt = 0; mt < KS; ++mt) o[t][mt][0] = o[t][mt][1] = o[t][mt][2] = o[t][mt][3] = 0.0f;
     }
@@ -388,12 +400,14 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qa[ks][e * RT + t]));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qb[ks][t][e]));
             sum += f.x + f.y;
           }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        start[t] = sum * -0x1p-17f;   // -128 2^-24
+        sum *= -0x1p-17f;   // -128 2^-24
+        start[t][0] = __shfl_sync(0xffffffffu, sum, 8 * c);
+        start[t][1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
       }
     }
 
@@ -403,50 +417,53 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
     for (int h = 0; h < 2; ++h, kt += kBlock * D) {
       const unsigned char* vt = kt + S::kTileBytes;
       const int t0 = md.tile * kTile + h * kBlock;
-      // ---- S = Q K^T: columns token_of(0..7) and token_of(8..15) ----
-      float s[2][4];
+      // ---- S^T = K Q^T: tokens token_of(g) and + 8, rows 8 t + 2 c and + 1 ----
+      float s[2][RT][4];   // two sums: an accumulator's next MMA waits for its last
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        s[nt][0] = s[nt][1] = TYPE == q8::kInt8 ? start[0] : 0.0f;
-        s[nt][2] = s[nt][3] = TYPE == q8::kInt8 ? start[RT - 1] : 0.0f;
-      }
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[0][t][e] = TYPE == q8::kInt8 ? start[t][e & 1] : 0.0f;
+          s[1][t][e] = 0.0f;
+        }
       uint4 w[NC][2];
 #pragma unroll
       for (int q = 0; q < NC; ++q)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const int row = token_of(g) + 8 * nt;
+        for (int z = 0; z < 2; ++z) {
+          const int row = token_of(g) + 8 * z;
           const int at = D == 128 ? row * 128 + (((c + 4 * q) ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
-          w[q][nt] = *reinterpret_cast<const uint4*>(kt + at);
+          w[q][z] = *reinterpret_cast<const uint4*>(kt + at);
         }
 #pragma unroll
       for (int q = 0; q < NC; ++q)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e) {
+          uint32_t a[2][2];   // [token][pair of dims]
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const uint4 k = w[q][nt];
+          for (int z = 0; z < 2; ++z) {
+            const uint4 k = w[q][z];
             const uint32_t v = e == 0 ? k.x : e == 1 ? k.y : e == 2 ? k.z : k.w;
-            uint32_t b0, b1;
             if (TYPE == q8::kInt8) {
               const uint32_t u = v ^ 0x80808080u;
-              b0 = __byte_perm(u, 0, 0x4140);
-              b1 = __byte_perm(u, 0, 0x4342);
+              a[z][0] = __byte_perm(u, 0, 0x4140);
+              a[z][1] = __byte_perm(u, 0, 0x4342);
             } else {
-              e4m3x4_to_half4(v, b0, b1);
+              e4m3x4_to_half4(v, a[z][0], a[z][1]);
             }
-            const uint32_t* a = qa[4 * q + e];
-            if (RT == 1) mma16816(s[nt], a[0], 0u, a[1], 0u, b0, b1);
-            else mma16816(s[nt], a[0], a[RT - 1], a[RT], a[2 * RT - 1], b0, b1);
           }
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+            mma16816(s[e & 1][t], a[0][0], a[1][0], a[0][1], a[1][1], qb[4 * q + e][t][0], qb[4 * q + e][t][1]);
+        }
 
-      // ---- softmax: rows g (c0, c1) and, with RT == 2, g + 8 (c2, c3) ----
+      // ---- softmax ----
       const float ks = slot.ks[h] * scale, vs = slot.vs[h];
-      float x[RT][4];
+      float x[RT][4];   // tokens token_of(g), then + 8; two rows each
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[t][e] = s[e >> 1][2 * t + (e & 1)] * ks;
+        for (int e = 0; e < 4; ++e) x[t][e] = (s[0][t][e] + s[1][t][e]) * ks;
       // some row may not see all of the block: length >= 32 (n - 1) + 1, row 0 sees Q - 1 less
       const bool edge = t0 + kBlock > kTile * (md.n - 1) + 2 - Q;
       int len = 0;
@@ -454,38 +471,39 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
         len = seqlens[slot.b];
         const int r0 = (slot.pair - p.row_groups.quotient(slot.pair) * p.row_groups.d) * S::kRows;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const int sees = len - Q + 1 + p.group.quotient(r0 + 8 * t + g) - t0;
+        for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (token_of(2 * c + (e & 1)) + 8 * (e >> 1) >= sees) x[t][e] = -INFINITY;
-        }
+          for (int e = 0; e < 4; ++e) {
+            const int sees = len - Q + 1 + p.group.quotient(r0 + 8 * t + 2 * c + (e & 1)) - t0;
+            if (token_of(g) + 8 * (e >> 1) >= sees) x[t][e] = -INFINITY;
+          }
       }
-      float mx[RT];
+      float mx[RT][2];
       bool above = false;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        mx[t] = fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3]));
-        above |= mx[t] > m[t] + 12.0f;
-      }
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mx[t][e] = fmaxf(x[t][e], x[t][2 + e]);
+          above |= mx[t][e] > m[t][e] + 12.0f;
+        }
       if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          mx[t] = fmaxf(mx[t], __shfl_xor_sync(0xffffffffu, mx[t], 1));
-          mx[t] = fmaxf(mx[t], __shfl_xor_sync(0xffffffffu, mx[t], 2));
-          const float m_new = mx[t] > m[t] + 12.0f ? mx[t] - 4.0f : m[t];
-          const float alpha = fast_exp2(m[t] - m_new);
-          m[t] = m_new;
-          l[t] *= alpha;
-          const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * c), a1 = __shfl_sync(0xffffffffu, alpha, 8 * c + 4);
+        for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int mt = 0; mt < KS; ++mt) {
-            o[t][mt][0] *= a0;
-            o[t][mt][1] *= a1;
-            o[t][mt][2] *= a0;
-            o[t][mt][3] *= a1;
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int z = 4; z < 32; z <<= 1) mx[t][e] = fmaxf(mx[t][e], __shfl_xor_sync(0xffffffffu, mx[t][e], z));
+            const float m_new = mx[t][e] > m[t][e] + 12.0f ? mx[t][e] - 4.0f : m[t][e];
+            const float alpha = fast_exp2(m[t][e] - m_new);
+            m[t][e] = m_new;
+            l[t][e] *= alpha;
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt) {
+              o[t][mt][e] *= alpha;
+              o[t][mt][2 + e] *= alpha;
+            }
           }
-        }
       }
       float rel = vs * F_inv;
       if ((rel > 8.0f || rel < 0.125f) && vs > 0.0f) {
@@ -505,10 +523,11 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[t][e] = fast_exp2(x[t][e] - m[t]);
-        l[t] += (x[t][0] + x[t][1]) + (x[t][2] + x[t][3]);
-        pb[t][0] = pack_half2(x[t][0] * rel, x[t][1] * rel);
-        pb[t][1] = pack_half2(x[t][2] * rel, x[t][3] * rel);
+        for (int e = 0; e < 4; ++e) x[t][e] = fast_exp2(x[t][e] - m[t][e & 1]);
+        l[t][0] += x[t][0] + x[t][2];
+        l[t][1] += x[t][1] + x[t][3];
+        pb[t][0] = transpose8x8(pack_half2(x[t][0] * rel, x[t][1] * rel));
+        pb[t][1] = transpose8x8(pack_half2(x[t][2] * rel, x[t][3] * rel));
       }
 
       // ---- O^T += V^T P^T ----
@@ -581,20 +600,20 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
     const bool ends = md.tile == md.n - 1;
     if (ends || j == count - 1) {
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
-        l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
-      }
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int z = 4; z < 32; z <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], z);
       const bool from_start = j >= md.tile;   // the pair's first tile is in this stretch
       const int sb = slot.b, sp = slot.pair;
       if (from_start && ends) {
         const int kvh = p.row_groups.quotient(sp), r0 = (sp - kvh * p.row_groups.d) * S::kRows;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          const float inv = l[t] == 0.0f ? 0.0f : F / l[t];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float f = __shfl_sync(0xffffffffu, inv, 8 * c + 4 * e);
+            const float f = l[t][e] == 0.0f ? 0.0f : F / l[t][e];
             const int r = r0 + 8 * t + 2 * c + e, i = p.group.quotient(r);
             if (i < p.Q) {
               __half* dst = p.out + (((size_t)sb * p.Q + i) * p.Hq + kvh * p.group.d + r - i * p.group.d) * D + g * (D / 8);
@@ -620,9 +639,9 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
         __syncwarp();
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          if (c == 0) stat[8 * t + g] = make_float2(m[t], l[t]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
+            if (g == 0) stat[8 * t + 2 * c + e] = make_float2(m[t][e], l[t][e]);
             float4* dst = reinterpret_cast<float4*>(state + (8 * t + 2 * c + e) * D + g * (D / 8));
 #pragma unroll
             for (int q = 0; q < KS / 2; ++q)
