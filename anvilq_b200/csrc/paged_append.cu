@@ -336,43 +336,41 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 6)
 }
 
 // values[page][head][token][:] = fp16(code * scale), K's pool then V's: a thread
-// takes 16 codes of a row at a time, four such pieces on their way.
+// takes 8 codes of a row at a time, so that a warp stores whole sectors, eight such
+// pieces on their way.
 template <int TYPE>
 __global__ void __launch_bounds__(256) values_kernel(const uint8_t* k, const uint8_t* v, const float* ks,
-                                                     const float* vs, __half* ko, __half* vo, long long chunks,
-                                                     int chunks_per_block) {
+                                                     const float* vs, __half* ko, __half* vo, long long pieces,
+                                                     int pieces_per_block) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 8;
   const bool second = blockIdx.y != 0;
-  const uint4* codes = reinterpret_cast<const uint4*>(second ? v : k);
+  const uint2* codes = reinterpret_cast<const uint2*>(second ? v : k);
   const float* scales = second ? vs : ks;
   uint4* out = reinterpret_cast<uint4*>(second ? vo : ko);
-  for (long long i0 = (long long)blockIdx.x * (kAhead * 256) + threadIdx.x; i0 < chunks;
+  for (long long i0 = (long long)blockIdx.x * (kAhead * 256) + threadIdx.x; i0 < pieces;
        i0 += (long long)gridDim.x * (kAhead * 256)) {
-    uint4 w[kAhead];
+    uint2 w[kAhead];
     float s[kAhead];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       const long long c = i0 + 256 * a;
-      if (c < chunks) {
+      if (c < pieces) {
         w[a] = __ldcs(codes + c);
-        s[a] = scales[c / chunks_per_block];
+        s[a] = scales[c / pieces_per_block];
       }
     }
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       const long long c = i0 + 256 * a;
-      if (c >= chunks) break;
-      float f[16];
+      if (c >= pieces) break;
+      float f[8];
       q8::codes_to_float4<TYPE>(w[a].x, f);
       q8::codes_to_float4<TYPE>(w[a].y, f + 4);
-      q8::codes_to_float4<TYPE>(w[a].z, f + 8);
-      q8::codes_to_float4<TYPE>(w[a].w, f + 12);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) f[e] *= s[a];
-      out[2 * c] = pack8(f);
-      out[2 * c + 1] = pack8(f + 8);
+      for (int e = 0; e < 8; ++e) f[e] *= s[a];
+      out[c] = pack8(f);
     }
   }
 }
@@ -494,12 +492,12 @@ int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k
   if (num_pages < 1 || Hkv < 1) return ANVILQ_EINVAL;
   if ((D != 64 && D != 128) || page_tokens < kBlock || page_tokens % kBlock) return ANVILQ_ESHAPE;
   if (!a16(k_codes) || !a16(v_codes) || !a16(k_out) || !a16(v_out)) return ANVILQ_EALIGN;
-  const long long chunks = (long long)num_pages * Hkv * page_tokens * (D / 16);
-  const int blocks = (int)std::min<long long>((chunks + 1023) / 1024, 148 * 8);
+  const long long pieces = (long long)num_pages * Hkv * page_tokens * (D / 8);
+  const int blocks = (int)std::min<long long>((pieces + 2047) / 2048, 148 * 8);
   auto go = [&](auto kernel) {
     return launch(kernel, dim3(blocks, 2), 256, reinterpret_cast<cudaStream_t>(stream), flags,
                   static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(v_codes), k_scales, v_scales,
-                  reinterpret_cast<__half*>(k_out), reinterpret_cast<__half*>(v_out), chunks, kBlock * D / 16);
+                  reinterpret_cast<__half*>(k_out), reinterpret_cast<__half*>(v_out), pieces, kBlock * D / 8);
   };
   return code_type == ANVILQ_KV_Q8_INT8 ? go(values_kernel<ANVILQ_KV_Q8_INT8>) : go(values_kernel<ANVILQ_KV_Q8_E4M3>);
 }
