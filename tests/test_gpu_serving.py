@@ -750,3 +750,110 @@ def test_caller_workspace(dev):
     with pytest.raises(ValueError):
         ops.gqa_decode_q8(*a, workspace=ws[:need - 1])
     ops.raise_device_errors(dev)
+
+
+def test_two_streams_at_once(dev):
+    """Eager calls on two streams, each stream with its own workspace."""
+    rng = np.random.default_rng(16)
+    q, k, v, ks, vs, table = attention_case(dev, rng, [3000, 700], 1, 8, 2, 128, 16, True)
+    a = [to(q, dev)] + [t.to(dev) for t in (k, v, ks, vs)] + [to(table, dev), to(np.array([3000, 700], np.int32), dev)]
+    x, history, lens, prompts, rep, pres, freq = logits_case(rng, 3, 30000, 200, True)
+    d = lambda t: to(t, dev)
+    kw = dict(history=d(history), history_lens=d(lens), prompt_lens=d(prompts), repetition=d(rep), presence=d(pres),
+              frequency=d(freq))
+    logits = d(x)
+    out, (log, tok) = ops.gqa_decode_q8(*a), ops.logits_process(logits, **kw)
+    torch.cuda.synchronize(dev)
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = []
+    for _ in range(15):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((ops.gqa_decode_q8(*a), *ops.logits_process(logits, **kw)))
+    torch.cuda.synchronize(dev)
+    ops.raise_device_errors(dev)
+    for o, l, t in got:
+        assert torch.equal(o, out) and torch.equal(l, log) and torch.equal(t, tok)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_overlapped_launches_give_the_same(dev, fp8):
+    """A chain of steps under programmatic dependent launch."""
+    rng = np.random.default_rng(17)
+    B, Hq, Hkv, D, page, width = 5, 8, 2, 64, 16, 8
+    pages = B * width
+    table, one = to(so.make_table([width] * B, pages, rng), dev), to(np.arange(B + 1, dtype=np.int32), dev)
+    rows = [to(rng.standard_normal((B, (Hq + 2 * Hkv) * D)).astype(np.float16), dev) for _ in range(60)]
+    lens = [to(np.full(B, i + 1, np.int32), dev) for i in range(60)]
+    ends = []
+    for overlap in (False, True):
+        k = torch.zeros((pages, Hkv, page, D), device=dev).to(code_dtype(fp8))
+        v, ks, vs = k.clone(), *(torch.zeros((pages, Hkv, page // BLOCK), device=dev) for _ in range(2))
+        k16, v16 = (torch.zeros((pages, page, Hkv, D), dtype=torch.float16, device=dev) for _ in range(2))
+        outs = []
+        for x, n in zip(rows, lens):
+            q = ops.paged_kv_append_q8(x, k, v, ks, vs, table, n, one, Hq, overlap_prior=overlap)
+            out = ops.gqa_decode_q8(q, k, v, ks, vs, table, n, overlap_prior=overlap)
+            ops.paged_kv_append(x, k16, v16, table, n, one, Hq, overlap_prior=overlap)
+            raw, token = ops.logits_process(out.view(B, -1), overlap_prior=overlap)
+            outs += [out, raw, token]
+        values = ops.kv_q8_values(k, v, ks, vs, overlap_prior=overlap)
+        ends.append([*outs, *values, k16, v16])
+    torch.cuda.synchronize(dev)
+    ops.raise_device_errors(dev)
+    for x, y in zip(*ends):
+        assert torch.equal(x, y)
+
+
+def test_pools_beyond_31_bits(dev):
+    """Codes and rows whose offsets do not fit 31 bits: the last pages of 2.2 GB pools."""
+    rng = np.random.default_rng(18)
+    Hq, Hkv, D, page = 4, 2, 128, 256
+    pages = 2 ** 31 // (Hkv * page * D) + 1500
+    k = torch.zeros((pages, Hkv, page, D), dtype=torch.int8, device=dev)
+    v, ks, vs = torch.zeros_like(k), *(torch.zeros((pages, Hkv, page // BLOCK), device=dev) for _ in range(2))
+    need = [2, 1]
+    table = np.array([[so.word(pages - 1), so.word(pages - 3)], [so.word(pages - 2), 0]], np.int32)
+    new = [300, 77]
+    starts = np.array([0, 300, 377], np.int32)
+    lens = np.array(new, np.int32)
+    x = rng.standard_normal((377, (Hq + 2 * Hkv) * D)).astype(np.float16)
+    q = ops.paged_kv_append_q8(to(x, dev), k, v, ks, vs, to(table, dev), to(lens, dev), to(starts, dev), Hq)
+    last = q[torch.tensor([299, 376], device=dev)].contiguous()
+    out = ops.gqa_decode_q8(last, k, v, ks, vs, to(table, dev), to(lens, dev))
+    ops.raise_device_errors(dev)
+    assert not k[:pages - 3].any() and not vs[:pages - 3].any()
+    small = [so.word(2), so.word(0)], [so.word(1), 0]
+    check_attention(out.cpu().numpy()[:, None], last.cpu().numpy()[:, None], k[pages - 3:], v[pages - 3:], ks[pages - 3:],
+                    vs[pages - 3:], np.array(small, np.int32), new)
+    k16 = torch.zeros((pages, page, Hkv, D), dtype=torch.float16, device=dev)
+    v16 = torch.zeros_like(k16)
+    assert torch.equal(ops.paged_kv_append(to(x, dev), k16, v16, to(table, dev), to(lens, dev), to(starts, dev), Hq), q)
+    assert torch.equal(v16[pages - 2, :77].reshape(77, -1), to(x, dev)[300:, (Hq + Hkv) * D:])
+    assert not v16[:pages - 3].any()
+
+
+@pytest.mark.parametrize("lens,Q,Hq,Hkv,D,page,fp8", [
+    ([80, 200], 2, 64, 1, 64, 16, False),      # 128 query rows on one kv head
+    ([64], 1, 128, 128, 64, 16, True),         # many kv heads; a table without a spare place
+    ([1] * 300, 1, 2, 1, 64, 16, True),        # many sequences of one token
+    ([17, 0] * 40, 3, 6, 2, 128, 32, False),
+])
+def test_attention_q8_head_layouts(dev, lens, Q, Hq, Hkv, D, page, fp8):
+    rng = np.random.default_rng(len(lens) + Hq)
+    q, k, v, ks, vs, table = attention_case(dev, rng, lens, Q, Hq, Hkv, D, page, fp8)
+    out = ops.gqa_decode_q8(to(q, dev), *(t.to(dev) for t in (k, v, ks, vs)), to(table, dev),
+                            to(np.array(lens, np.int32), dev))
+    ops.raise_device_errors(dev)
+    check_attention(out.cpu().numpy(), q, k, v, ks, vs, table, lens)
+
+
+def test_logits_most_rows(dev):
+    rng = np.random.default_rng(20)
+    x = rng.standard_normal((4096, 70)).astype(np.float32)
+    allowed = rng.random((4096, 70)) < 0.03
+    out, tokens = ops.logits_process(to(x, dev), allowed=to(so.pack_mask(allowed), dev))
+    ops.raise_device_errors(dev)
+    want = np.where(allowed, x, -np.inf)
+    assert np.array_equal(out.cpu().numpy(), want)
+    assert np.array_equal(tokens.cpu().numpy(), np.where(allowed.any(axis=1), want.argmax(axis=1), -1))
