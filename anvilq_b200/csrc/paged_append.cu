@@ -155,7 +155,7 @@ __device__ __forceinline__ void rotate8(float* a, float* b, const float* co, con
 }
 
 template <int D, int TYPE>
-__global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 6)
+__global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
     append_kernel(const __grid_constant__ Params p, const __grid_constant__ Freq freq) {
   constexpr int kHalf = D / 2;
   constexpr int kLanes = D / 16;              // threads of a row: 8 dims of each half a thread
@@ -430,12 +430,14 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   const long long by_place = T / kBlock + 2LL * B;
   p.by_token = T <= by_place;
   const int items = (int)(p.by_token ? (long long)T : by_place);
-  // slices of the heads (at least 8 heads each) only until there are two CTAs an SM:
-  // every slice looks up its tokens and computes their cosines again.  A prompt of
-  // 15.8k tokens (14/2 heads of 64) takes 16.3 us in one slice, 17.7 in two; 8.5k
-  // tokens (32/8 of 128, 8-bit) 38.5 in one, 41.6 in two; a step of 64 tokens 3.2 either way.
+  // Slices of the heads, at least 8 heads each, only until there are four CTAs an SM
+  // (three with 8-bit pages, whose CTAs take more registers): every slice looks up
+  // its tokens and computes their cosines again.  32/8 heads of 128, one slice and
+  // two: 560 items into binary16 47.5 and 39.9 us, 350 items into 8 bits 32.0 and
+  // 24.8, but 538 items into 8 bits 38.1 and 41.8.
+  const long long enough = 148 * (type == kBinary16 ? 4 : 3);
   int slices = 1;
-  while (slices * 8 < heads && (long long)items * slices < 148 * 2) slices *= 2;
+  while (slices * 8 < heads && (long long)items * slices < enough) slices *= 2;
   p.heads_per_cta = (heads + slices - 1) / slices;
   // the frequencies of the thread's last theta and D (64 powers cost the host 3 us)
   thread_local Freq freq;
