@@ -308,12 +308,14 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
 #pragma unroll
         for (int e = 0; e < kPiece; ++e)
           if (skip >> e & 1u) l[e] = -INFINITY;
-      const float top = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), fmaxf(fmaxf(l[4], l[5]), fmaxf(l[6], l[7])));
+      const float t01 = fmaxf(l[0], l[1]), t23 = fmaxf(l[2], l[3]), t45 = fmaxf(l[4], l[5]), t67 = fmaxf(l[6], l[7]);
+      const float t03 = fmaxf(t01, t23), top = fmaxf(t03, fmaxf(t45, t67));
       if (top > best) {       // a thread's places ascend: an equal one later is not lower
         best = top;
-#pragma unroll
-        for (int e = kPiece - 1; e >= 0; --e)
-          if (l[e] == top) best_at = v + e * kApart;
+        // the first that has it, by halves
+        const bool e4 = t03 != top, e2 = (e4 ? t45 : t01) != top;
+        const bool e1 = (e4 ? (e2 ? l[6] : l[4]) : (e2 ? l[2] : l[0])) != top;
+        best_at = v + (4 * e4 + 2 * e2 + e1) * kApart;
       }
     }
   }
