@@ -598,8 +598,9 @@ def _on_device(name, device, *tensors):
     """Every given tensor (None: skipped) is on `device`, a CUDA device."""
     if device.type != "cuda":
         raise ValueError(f"{name}: tensors must be on a CUDA device")
+    index = device.index
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"{name}: all tensors must be on {device}")
 
 
@@ -697,7 +698,7 @@ def _check_append(name, qkv, Hq, Hkv, D, page_table, seqlens, token_starts, q_ou
     if token_starts.dtype != torch.int32 or token_starts.shape != (B + 1,) or not token_starts.is_contiguous():
         raise ValueError(f"{name}: token_starts must be a contiguous int32 tensor [{B + 1}]")
     if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=torch.float16, device=qkv.device)
+        q_out = qkv.new_empty((T, Hq, D))
     elif q_out.dtype != torch.float16 or q_out.shape != (T, Hq, D) or not q_out.is_contiguous():
         raise ValueError(f"{name}: q_out must be contiguous float16 [{T}, {Hq}, {D}]")
     return T, B, max_pages, (stride if T > 1 else width), q_out
@@ -758,8 +759,8 @@ def kv_q8_values(k_codes, v_codes, k_scales, v_scales, k_out=None, v_out=None, o
     name = "kv_q8_values"
     pages, Hkv, page, D, code = _check_q8(name, k_codes, v_codes, k_scales, v_scales)
     dev = k_codes.device
-    k_out = torch.empty(k_codes.shape, dtype=torch.float16, device=dev) if k_out is None else k_out
-    v_out = torch.empty(k_codes.shape, dtype=torch.float16, device=dev) if v_out is None else v_out
+    k_out = torch.empty_like(k_codes, dtype=torch.float16) if k_out is None else k_out
+    v_out = torch.empty_like(k_codes, dtype=torch.float16) if v_out is None else v_out
     for t in (k_out, v_out):
         if t.dtype != torch.float16 or t.shape != k_codes.shape or not t.is_contiguous():
             raise ValueError(f"{name}: k_out/v_out must be contiguous float16 with the shape of the codes")
@@ -844,16 +845,19 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
     dev = logits.device
 
     def rows(t, dtype, what, n):
-        if t is not None and (t.dtype != dtype or t.shape != (n,) or not t.is_contiguous()):
+        if t is None:
+            return
+        if t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
             raise ValueError(f"{name}: {what} must be contiguous {dtype} [{n}]")
 
     def matrix(t, dtype, n, cols, what):   # rows of at least `cols`, contiguous, apart; their distance
-        if t.dtype != dtype or t.dim() != 2 or (n is not None and t.shape[0] != n) or t.shape[1] < cols:
+        shape = t.shape
+        if t.dtype != dtype or len(shape) != 2 or (n is not None and shape[0] != n) or shape[1] < cols:
             raise ValueError(f"{name}: {what} must be {dtype} [{'masks' if n is None else n}, {cols}]")
         apart, inner = t.stride()
-        if (inner != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and apart < cols):
+        if (inner != 1 and shape[1] > 1) or (shape[0] > 1 and apart < cols):
             raise ValueError(f"{name}: rows of {what} must be contiguous and must not overlap")
-        return apart if t.shape[0] > 1 else t.shape[1]
+        return apart if shape[0] > 1 else shape[1]
 
     L = history_pitch = 0
     if history is not None:
@@ -898,18 +902,17 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
         if out is not None:
             raise ValueError(f"{name}: out is not written without write_logits")
     elif out is None:
-        out = torch.empty((B, V), dtype=torch.float32, device=dev)
+        out = torch.empty_like(logits, dtype=torch.float32, memory_format=torch.contiguous_format)
     else:
         out_pitch = matrix(out, torch.float32, B, V, "out")
         if out.shape[1] != V:
             raise ValueError(f"{name}: out must be float32 [{B}, {V}]")
-    tokens = torch.empty(B, dtype=torch.int32, device=dev) if choose else None
+    tokens = logits.new_empty(B, dtype=torch.int32) if choose else None
     _on_device(name, dev, history, history_lens, prompt_lens, repetition, presence, frequency, bias_starts, bias_ids,
                bias_values, allowed, allowed_rows, out)
-    need = _lib.load().anvilq_logits_process_workspace_size(B, V)
-    if need == 0:
+    if B > 4096 or V > 1 << 30:
         raise ValueError(f"{name}: unsupported shape B={B} V={V}")
-    ws = _call_workspace(dev, need, workspace) if choose else None
+    ws = _call_workspace(dev, WORKSPACE_COUNTER_BYTES, workspace) if choose else None
     err = _error_word(dev, dev_err)
     _call("anvilq_logits_process", dev, _ptr(logits), half, pitch if B > 1 else V, _ptr(out), out_pitch, _ptr(tokens),
           B, V, _ptr(history), history_pitch, _ptr(history_lens), _ptr(prompt_lens), L, _ptr(repetition),
