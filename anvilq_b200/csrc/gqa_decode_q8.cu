@@ -254,9 +254,7 @@ struct Control {     // in shared memory
 // One warp's stretch: `count` tiles from tile `begin` of the row on, b and base a
 // sequence no later than the first tile's and where its tiles start.  Pairs inside
 // it are finished, the states of others left for merge_states.  `before`: tiles of
-// the warp's earlier stretches.  False after a wait that ran out.  A function of
-// its own, as merge_states is: in one body the compiler spilled this loop's state
-// (1.6 times the time).
+// the warp's earlier stretches.  False after a wait that ran out.
 template <int D, int TYPE, int RT>
 __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,
                                          unsigned char* smem, Control& ctl, uint32_t before, unsigned begin, int count,
@@ -663,8 +661,9 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
   return ok;
 }
 
-// Merges what the warps left (frugal with registers: the tile loop's
-// share the kernel's with this).
+// Merges what the warps left.  Its loops keep few values at a time: the tile loop
+// lives within the same registers, and a merge that held a state's sums of all
+// members in registers made it spill (1.6 times the time).
 template <int D, int RT>
 __device__ __forceinline__ void merge_states(const Params& p, unsigned char* smem, Control& ctl) {
   using S = Shape<D, RT>;
@@ -1031,13 +1030,18 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   if (!shape_ok(B, Q, Hq, Hkv, D) || page_tokens < kBlock || page_tokens % kBlock || max_pages < 1 || num_pages < 1 ||
       (long long)page_tokens * max_pages > (1LL << 30))
     return ANVILQ_ESHAPE;
-  const long long rows = (long long)num_pages * page_tokens * Hkv;   // a TMA coordinate is an int
-  if ((long long)num_pages * page_tokens > (1LL << 31) || rows > 0x7FFFFFFFLL) return ANVILQ_ESHAPE;
+  const long long positions = (long long)num_pages * page_tokens;
+  if (positions > 0x7FFFFFFFLL / Hkv) return ANVILQ_ESHAPE;   // a TMA coordinate is an int
+  const long long rows = positions * Hkv;
+  const int rt = row_tiles(Q, Hq, Hkv), warps = rt == 1 ? Shape<128, 1>::kWarps : Shape<128, 2>::kWarps;
+  const int row_groups = (Q * (Hq / Hkv) + 8 * rt - 1) / (8 * rt);
+  const double all_pairs = (double)B * Hkv * row_groups;
+  const double tiles = all_pairs * ((double)max_pages * page_tokens / kTile + 1);   // that the table has room for
+  if (tiles > (double)(1u << 31)) return ANVILQ_ESHAPE;   // they are counted in 32 bits
   if (!a16(q) || !a16(k_codes) || !a16(v_codes) || !a16(out) || !a16(workspace)) return ANVILQ_EALIGN;
   const int sms = sm_count();
   if (sms <= 0) return ANVILQ_ECUDA;
   if (!workspace || workspace_bytes < anvilq_gqa_decode_q8_workspace_size(B, Q, Hq, Hkv, D)) return ANVILQ_EWORKSPACE;
-  const int rt = row_tiles(Q, Hq, Hkv), warps = rt == 1 ? Shape<128, 1>::kWarps : Shape<128, 2>::kWarps;
   Params p{};
   p.q = reinterpret_cast<const __half*>(q);
   p.k_scales = k_scales;
@@ -1052,15 +1056,12 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   p.B = B; p.Q = Q; p.Hq = Hq; p.Hkv = Hkv;
   auto divisor = [](int d) { return Divisor{d, d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d)}; };
   p.group = divisor(Hq / Hkv);
-  p.row_groups = divisor((Q * (Hq / Hkv) + 8 * rt - 1) / (8 * rt));
+  p.row_groups = divisor(row_groups);
   p.page_tokens = page_tokens; p.max_pages = max_pages; p.num_pages = num_pages;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
   // as many CTAs as the device holds, but no more than there can be work for: a pair
-  // each, or a tile a warp of what the table has room for
-  const double tiles = (double)B * Hkv * p.row_groups.d * ((double)max_pages * page_tokens / kTile + 1);
-  const double all_pairs = (double)B * Hkv * p.row_groups.d;
+  // each, or a tile a warp
   const int ctas = (int)std::min((double)max_ctas(sms), std::max(all_pairs, std::ceil(tiles / warps)));
-  if (tiles > (double)(1u << 31)) return ANVILQ_ESHAPE;   // tiles are counted in 32 bits
   CUtensorMap mk, mv;
   p.wide = page_tokens % kTile == 0;
   const int box = p.wide ? kTile : kBlock;

@@ -14,10 +14,13 @@
 // What bounds it: bytes -- each logit in and out once (the history, the lists and
 // the mask's bits are small beside them).
 //
-// Work split: a CTA takes a span of the vocabulary of one row.  While its first
-// logits travel it marks the span's special tokens -- of the row's history and of
-// its bias list -- in a bitmap, counts the marks up to each word, and so gives every
-// special token a place in short tables (occurrences, last bias index).  A dense
+// Work split: the vocabulary is cut into chunks of 256, dealt in turn to a row's
+// CTAs (the tokens of a history crowd at one end of a vocabulary: with a contiguous
+// span a CTA, the first one's took several rounds -- below -- while the others
+// waited; 64 rows with 32768 tokens of history 141 us, dealt out 99 us).
+// While its first logits travel a CTA marks its special tokens -- of the row's
+// history and of its bias list -- in a bitmap, counts the marks up to each word, and
+// so gives every one a place in short tables (occurrences, last bias index).  A dense
 // pass then masks and writes all logits, taking the largest of the others; behind a
 // barrier the special ones are computed from their tables, a thread each, and
 // written over.  More special tokens than the tables hold take further rounds over
@@ -65,7 +68,8 @@ struct Params {
   unsigned long long* keys;
   int* tickets;
   int* dev_err;
-  int V, L, bias_total, masks, span;
+  int V, L, bias_total, masks;
+  unsigned magic, shift;         // chunk / CTAs of a row = umulhi(2 chunk, magic) >> shift
   int wide_out;                  // out's rows start on 16-byte boundaries
 };
 
@@ -78,11 +82,13 @@ __device__ __forceinline__ unsigned orderable(float v) {
 constexpr int kPiece = 8;                      // logits of a thread at a time
 constexpr int kAhead = 2;                      // pieces loaded ahead
 constexpr int kAcross = kThreads * kPiece;
-constexpr int kMaxSpan = 32768;
+constexpr int kChunk = 32 * kPiece;            // logits of a warp at a time
+constexpr int kMaxSpan = 32768;                // logits of a CTA
 constexpr int kWords = kMaxSpan / 32;          // of the bitmap
 constexpr int kTable = 2048;                   // special tokens of a round
 constexpr int kIds = 8;                        // tokens of the history that a thread keeps
-static_assert(kWords == 4 * kThreads && kMaxSpan <= 0x10000, "four words a thread; a place fits 16 bits");
+constexpr int kScan = 8;                       // further ones, loaded at a time
+static_assert(kWords == 4 * kThreads && kMaxSpan <= 0x8000, "four words a thread; an `at` has 15 bits");
 
 // eight consecutive logits, 16-byte aligned, as they are stored
 template <typename T> struct Raw8;
@@ -114,26 +120,28 @@ __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 
 // WIDE: rows start on 16-byte boundaries; a thread's piece is 8 consecutive logits.
-// Otherwise its 8 logits lie kThreads apart, so that a warp's loads still are whole
-// sectors.
+// Otherwise its 8 logits lie 32 apart, so that a warp's loads still are whole sectors.
+// A CTA numbers the logits of its chunks, one after the other, by `at`.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_constant__ Params p) {
-  __shared__ uint32_t s_map[kWords];    // bit: a special token
+  __shared__ uint32_t s_map[kWords];    // bit: a special token (at first: of the bias list)
+  __shared__ uint32_t s_seen[kWords];   // bit: a token of the history
   __shared__ int s_rank[kWords];        // special tokens before the word's
-  __shared__ int s_count[kTable];       // occurrences in the generated part; bit 31: in the history at all
+  __shared__ int s_count[kTable];       // occurrences in the generated part
   __shared__ int s_entry[kTable];       // last index in the bias list, or -1
-  __shared__ uint16_t s_token[kTable];
+  __shared__ uint16_t s_token[kTable];  // its `at`; bit 15: of the history
   __shared__ int s_sum[kThreads / 32];
   __shared__ unsigned s_best[kThreads / 32];
   __shared__ int s_at;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int b = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int v0 = blockIdx.x * p.span, v1 = min(p.V, v0 + p.span);
+  const int nth = blockIdx.x, ctas = gridDim.x;
   const bool lead = blockIdx.x == 0 && threadIdx.x == 0;
   const T* x = static_cast<const T*>(p.x) + b * p.ld;
-  constexpr int kApart = WIDE ? 1 : kThreads;             // between a piece's logits
-  const int first = v0 + (int)threadIdx.x * (WIDE ? kPiece : 1);
+  constexpr int kApart = WIDE ? 1 : 32;                   // between a piece's logits
+  const int first_at = WIDE ? threadIdx.x * kPiece : warp * kChunk + lane;
+  const int first = (warp * ctas + nth) * kChunk + first_at % kChunk, across = kAcross * ctas;
   const uint32_t* allowed = nullptr;
   if (p.allowed) {
     const int row = p.allowed_rows ? p.allowed_rows[b] : b;   // negative: the row has no mask
@@ -146,18 +154,33 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   Raw8<T> raw[kAhead];       // whole pieces, and their words of the mask
   uint32_t bits[kAhead];
   auto load = [&](int i, int v) {
-    if (WIDE && v + kPiece <= v1) raw[i].load(x + v);     // others are loaded when they are used
-    if (WIDE && allowed && v < v1) bits[i] = allowed[v / 32];
+    if (WIDE && v + kPiece <= p.V) raw[i].load(x + v);    // others are loaded when they are used
+    if (WIDE && allowed && v < p.V) bits[i] = allowed[v / 32];
   };
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) load(i, first + i * kAcross);
+  for (int i = 0; i < kAhead; ++i) load(i, first + i * across);
 
   // ---- the special tokens ----
   int hist = 0, prompt = 0, bias0 = 0, bias1 = 0, specials = 0;
   const int32_t* history = p.history + b * p.history_ld;
-  constexpr int kNone = 0x7FFFFFFF;   // in no span
-  int ids[kIds];
+  constexpr int kNone = 0x7FFFFFFF;   // no token
+  int ids[kIds];                      // then: their `at`, or -1
+  auto at_of = [&](int id) {          // -1: in another CTA's chunks
+    const unsigned chunk = (unsigned)id / kChunk, q = __umulhi(2 * chunk, p.magic) >> p.shift;
+    return (unsigned)id < (unsigned)p.V && chunk - q * ctas == nth ? (int)(q * kChunk + (unsigned)id % kChunk) : -1;
+  };
   const bool special = p.history || p.bias_starts;
+  // the history from `from` on, kScan tokens of a thread on their way at a time (kNone
+  // behind its end)
+  auto scan = [&](int from, auto each) {
+#pragma unroll 1
+    for (int i = from + threadIdx.x; i < hist; i += kScan * kThreads) {
+      int id[kScan];
+#pragma unroll
+      for (int k = 0; k < kScan; ++k) id[k] = i + k * kThreads < hist ? history[i + k * kThreads] : kNone;
+      each(id, i);
+    }
+  };
   auto clear = [&] {
     for (int i = threadIdx.x; i < kTable; i += kThreads) {
       s_count[i] = 0;
@@ -177,6 +200,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
         if (lead) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
         hist = max(0, min(hist, p.L));
       }
+      prompt = max(0, min(prompt, hist));
     }
     if (p.bias_starts) {
       bias0 = p.bias_starts[b];
@@ -186,26 +210,47 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
         bias0 = bias1 = 0;
       }
     }
-    for (int i = threadIdx.x; i < kWords; i += kThreads) s_map[i] = 0u;
+    for (int i = threadIdx.x; i < kWords; i += kThreads) s_map[i] = s_seen[i] = 0u;
     clear();
     __syncthreads();
     // an id outside the vocabulary is reported (by the row's first CTA) and ignored
-    auto mark = [&](int id) {
-      if (blockIdx.x == 0 && (unsigned)id >= (unsigned)p.V) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TOKEN);
-      if (id >= v0 && id < v1) atomicOr(s_map + (id - v0) / 32, 1u << ((id - v0) % 32));
+    auto report = [&](int id) {
+      if (nth == 0 && (unsigned)id >= (unsigned)p.V) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TOKEN);
+    };
+    // (most tokens of a long history are marked already: reading first keeps their
+    // lanes from queueing at one word)
+    auto mark = [](uint32_t* map, int at) {
+      if (at >= 0 && !(map[at / 32] >> (at % 32) & 1u)) atomicOr(map + at / 32, 1u << (at % 32));
     };
 #pragma unroll
     for (int k = 0; k < kIds; ++k) {
-      if ((int)threadIdx.x + k * kThreads < hist) mark(ids[k]);
-      else ids[k] = kNone;
+      const bool live = (int)threadIdx.x + k * kThreads < hist;
+      if (live) report(ids[k]);
+      ids[k] = live ? at_of(ids[k]) : -1;
+      mark(s_seen, ids[k]);
     }
-    for (int i = kIds * kThreads + threadIdx.x; i < hist; i += kThreads) mark(history[i]);
-    for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) mark(p.bias_ids[i]);
+    scan(kIds * kThreads, [&](const int* id, int i) {
+#pragma unroll
+      for (int k = 0; k < kScan; ++k) {
+        if (i + k * kThreads < hist) report(id[k]);
+        mark(s_seen, at_of(id[k]));
+      }
+    });
+    for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) {
+      report(p.bias_ids[i]);
+      mark(s_map, at_of(p.bias_ids[i]));
+    }
     __syncthreads();
-    // marks before each word: a thread's four words, the warp's threads, the warps
-    const uint4 mine = reinterpret_cast<const uint4*>(s_map)[threadIdx.x];
-    const int n0 = __popc(mine.x), n1 = n0 + __popc(mine.y), n2 = n1 + __popc(mine.z), n3 = n2 + __popc(mine.w);
-    int upto = n3;
+    // Marks before each word, in the order of threads (a thread's words lie apart, so
+    // that crowded neighbours are several threads'), its four words, its warp, the warps.
+    int n[4], mine = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int w = threadIdx.x + k * kThreads;
+      n[k] = __popc(s_map[w] |= s_seen[w]);
+      mine += n[k];
+    }
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, upto, o);
@@ -213,39 +258,64 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
     }
     if (lane == 31) s_sum[warp] = upto;
     __syncthreads();
-    int before = upto - n3;
+    int before = upto - mine;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-      const int n = s_sum[w];
-      specials += n;
-      if (w < warp) before += n;
+      const int sum = s_sum[w];
+      specials += sum;
+      if (w < warp) before += sum;
     }
-    reinterpret_cast<int4*>(s_rank)[threadIdx.x] = make_int4(before, before + n0, before + n1, before + n2);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s_rank[threadIdx.x + k * kThreads] = before;
+      before += n[k];
+    }
     __syncthreads();
   }
-  // the occurrences of the special tokens from rank r0 on, as many as the tables hold
+  // the special tokens from rank r0 on, as many as the tables hold: which they are,
+  // and their occurrences
   auto tally = [&](int r0) {
-    auto place = [&](int id) {
-      if (id < v0 || id >= v1) return -1;
-      const int at = id - v0;
+    auto place = [&](int at) {   // in the tables, of a special token
       const int i = s_rank[at / 32] + __popc(s_map[at / 32] & ((1u << (at % 32)) - 1u)) - r0;
-      if (i < 0 || i >= kTable) return -1;
-      s_token[i] = (uint16_t)at;
-      return i;
+      return i >= 0 && i < kTable ? i : -1;
     };
-    auto occurs = [&](int at, int i) {
-      if (at < 0) return;
-      if (i >= prompt) atomicAdd(s_count + at, 1);
-      else atomicOr(reinterpret_cast<unsigned*>(s_count + at), 0x80000000u);
-    };
+    // Of a short history, all in registers, each token names itself; of a longer one
+    // the bitmap's bits are walked, as then only its generated part is read again (by
+    // later rounds all of that: the tokens in registers would cost the dense pass).
+    const bool counts = p.presence || p.frequency, direct = r0 == 0 && hist <= kIds * kThreads;
+    if (!direct) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int w = threadIdx.x + k * kThreads;
+        const uint32_t seen = s_seen[w];
+        int i = s_rank[w] - r0;
+        for (uint32_t m = s_map[w]; m; m &= m - 1, ++i) {
+          const int bit = __ffs(m) - 1;
+          if (i >= 0 && i < kTable) s_token[i] = (uint16_t)(w * 32 + bit | (seen >> bit & 1u) << 15);
+        }
+      }
+    }
     if (r0 == 0)
 #pragma unroll
-      for (int k = 0; k < kIds; ++k) occurs(place(ids[k]), threadIdx.x + k * kThreads);
-    // (later rounds read all of it again: its tokens in registers would cost the dense pass)
-    for (int i = (r0 == 0 ? kIds * kThreads : 0) + threadIdx.x; i < hist; i += kThreads) occurs(place(history[i]), i);
+      for (int k = 0; k < kIds; ++k) {
+        const int i = ids[k] >= 0 ? place(ids[k]) : -1;
+        if (i < 0) continue;
+        if (direct) s_token[i] = (uint16_t)(ids[k] | 0x8000);
+        if ((int)threadIdx.x + k * kThreads >= prompt) atomicAdd(s_count + i, 1);
+      }
+    if (counts)
+      scan(max(prompt, r0 == 0 ? kIds * kThreads : 0), [&](const int* id, int) {
+#pragma unroll
+        for (int k = 0; k < kScan; ++k) {
+          const int at = at_of(id[k]), i = at >= 0 ? place(at) : -1;
+          if (i >= 0) atomicAdd(s_count + i, 1);
+        }
+      });
     for (int i = bias0 + threadIdx.x; i < bias1; i += kThreads) {
-      const int at = place(p.bias_ids[i]);
-      if (at >= 0) atomicMax(s_entry + at, i);   // the last entry of an id
+      const int at = at_of(p.bias_ids[i]), j = at >= 0 ? place(at) : -1;
+      if (j < 0) continue;
+      s_token[j] = (uint16_t)(at | (s_seen[at / 32] >> (at % 32) & 1u) << 15);
+      atomicMax(s_entry + j, i);   // the last entry of an id
     }
   };
   if (threadIdx.x == 0) s_at = kNone;
@@ -259,21 +329,21 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   float best = -INFINITY;
   int best_at = kNone;        // the lowest of equals
 #pragma unroll 1
-  for (int vb = first; vb < v1; vb += kAhead * kAcross) {
+  for (int vb = first, at = first_at; vb < p.V; vb += kAhead * across) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int v = vb + i * kAcross;
-      if (v >= v1) break;
-      const bool whole = v + (kPiece - 1) * kApart < v1;
+      const int v = vb + i * across;
+      if (v >= p.V) break;
+      const bool whole = v + (kPiece - 1) * kApart < p.V;
       float l[kPiece];
       uint32_t skip = 0u;     // bit e: special
       if (WIDE) {
-        if (special) skip = s_map[(v - v0) / 32] >> (v % 32) & 0xFFu;   // a span starts with a word
+        if (special) skip = s_map[at / 32] >> (at % 32) & 0xFFu;
         if (whole) {
           raw[i].get(l);
         } else {
 #pragma unroll
-          for (int e = 0; e < kPiece; ++e) l[e] = v + e < v1 ? to_float(x[v + e]) : -INFINITY;
+          for (int e = 0; e < kPiece; ++e) l[e] = v + e < p.V ? to_float(x[v + e]) : -INFINITY;
         }
         if (allowed) {
           const uint32_t a = bits[i] >> (v % 32);
@@ -286,14 +356,15 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
         for (int e = 0; e < kPiece; ++e) {
           const int u = v + e * kApart;
           l[e] = -INFINITY;
-          if (u < v1) {
+          if (u < p.V) {
             l[e] = to_float(x[u]);
-            if (special) skip |= (s_map[(u - v0) / 32] >> (u % 32) & 1u) << e;
+            if (special) skip |= (s_map[at / 32 + e] >> lane & 1u) << e;
             if (allowed && !(allowed[u / 32] >> (u % 32) & 1u)) l[e] = -INFINITY;
           }
         }
       }
-      load(i, v + kAhead * kAcross);
+      load(i, v + kAhead * across);
+      at += kAcross;
       if (out) {
         if (WIDE && whole && p.wide_out) {
           reinterpret_cast<float4*>(out + v)[0] = make_float4(l[0], l[1], l[2], l[3]);
@@ -301,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
         } else {
 #pragma unroll
           for (int e = 0; e < kPiece; ++e)
-            if (v + e * kApart < v1) out[v + e * kApart] = l[e];
+            if (v + e * kApart < p.V) out[v + e * kApart] = l[e];
         }
       }
       if (skip)
@@ -333,12 +404,11 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
     }
     __syncthreads();
     for (int i = threadIdx.x; i < min(kTable, specials - r0); i += kThreads) {
-      const int v = v0 + s_token[i], said = s_count[i], k = s_entry[i];
+      const int token = s_token[i], at = token & 0x7FFF, count = s_count[i], k = s_entry[i];
+      const int v = (at / kChunk * ctas + nth) * kChunk + at % kChunk;
       float l = to_float(x[v]);
-      if (said) {
-        l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
-        if (said & 0x7FFFFFFF) l = __fsub_rn(__fsub_rn(l, __fmul_rn(freq, (float)(said & 0x7FFFFFFF))), pres);
-      }
+      if (token >> 15) l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
+      if (count) l = __fsub_rn(__fsub_rn(l, __fmul_rn(freq, (float)count)), pres);
       if (k >= 0) l = __fadd_rn(l, p.bias_values[k]);
       if (allowed && !(allowed[v / 32] >> (v % 32) & 1u)) l = -INFINITY;
       if (out) out[v] = l;
@@ -372,12 +442,25 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   }
 }
 
-// The span of a CTA: one wave of CTAs (four an SM) over the rows, each at least a
-// few hundred logits and at most what the bitmap holds.
-static int span_for(int B, int V) {
-  const int ctas = std::max(1, 592 / B);
-  const int span = ((V + ctas - 1) / ctas + 511) / 512 * 512;
-  return std::min(span, kMaxSpan);
+// The CTAs of a row: one wave (four an SM) over the rows, each with two chunks at
+// least and at most what the bitmap holds.
+static int ctas_for(int B, int V) {
+  const int chunks = (V + kChunk - 1) / kChunk, ctas = std::max(1, 592 / B);
+  const int each = std::min((std::max(2, (chunks + ctas - 1) / ctas) + 1) / 2 * 2, kMaxSpan / kChunk);
+  return (chunks + each - 1) / each;
+}
+
+// Whether out can be written while the logits are read: it is the logits, or no row
+// of it touches one of theirs (rows of both may take turns in one buffer).
+static bool apart(const void* logits, size_t each, long long stride, const float* out, long long out_stride, int B,
+                  int V) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(logits), y = reinterpret_cast<uintptr_t>(out);
+  const size_t xs = (size_t)stride * each, ys = (size_t)out_stride * 4, xn = V * each, yn = (size_t)V * 4;
+  if (x == y) return each == 4 && (B == 1 || xs == ys);
+  if (x + (B - 1) * xs + xn <= y || y + (B - 1) * ys + yn <= x) return true;
+  if (B == 1 || xs != ys) return false;
+  const size_t d = y > x ? (y - x) % xs : (xs - (x - y) % xs) % xs;
+  return d >= xn && xs - d >= yn;
 }
 
 static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -410,7 +493,9 @@ int anvilq_logits_process(const void* logits, int logits_half, long long logits_
     return ANVILQ_EINVAL;   // a penalty needs a history
   if (bias_starts && (bias_total < 0 || (bias_total > 0 && (!bias_ids || !bias_values)))) return ANVILQ_EINVAL;
   if (allowed && (masks < 1 || allowed_stride < (V + 31) / 32 || (!allowed_rows && masks < B))) return ANVILQ_EINVAL;
-  if (B > kMaxRows || V > (1 << 30)) return ANVILQ_ESHAPE;
+  if (out && !apart(logits, logits_half ? 2 : 4, logits_stride, out, out_stride, B, V)) return ANVILQ_EINVAL;
+  if (B > kMaxRows || V > (1 << 30) || (history && L > (1 << 30)) || (bias_starts && bias_total > (1 << 30)))
+    return ANVILQ_ESHAPE;
   if (token && (!workspace || workspace_bytes < ANVILQ_WORKSPACE_COUNTER_BYTES)) return ANVILQ_EWORKSPACE;
   if (token && !aligned(workspace, 16)) return ANVILQ_EALIGN;
   if (!aligned(logits, logits_half ? 2 : 4) || !aligned(out, 4)) return ANVILQ_EALIGN;
@@ -437,11 +522,15 @@ int anvilq_logits_process(const void* logits, int logits_half, long long logits_
   p.tickets = token ? reinterpret_cast<int*>(static_cast<char*>(workspace) + kTicketOffset) : nullptr;
   p.dev_err = dev_err;
   p.V = V; p.L = L; p.bias_total = bias_total; p.masks = masks;
-  p.span = span_for(B, V);
+  const int ctas = ctas_for(B, V);
+  // with shift = floor(log2 ctas) and magic = ceil(2^(31 + shift) / ctas) <= 2^31 the
+  // quotient is exact below 2^30, and a chunk's number is below 2^24 even of a bad id
+  while (ctas >> (p.shift + 1)) ++p.shift;
+  p.magic = (unsigned)(((1ull << (31 + p.shift)) + ctas - 1) / ctas);
   const bool wide = aligned(logits, 16) && logits_stride % (logits_half ? 8 : 4) == 0;
   p.wide_out = out && aligned(out, 16) && out_stride % 4 == 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((V + p.span - 1) / p.span, B);
+  cfg.gridDim = dim3(ctas, B);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];

@@ -400,7 +400,7 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
                const uint32_t* page_table, uint16_t* q_out, void* k, void* v, float* k_scales, float* v_scales,
                int type, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages, int num_pages,
                float theta, int* dev_err, unsigned flags, cudaStream_t st) {
-  if (!qkv || !starts || !seqlens || !page_table || !q_out || !k || !v || !dev_err) return ANVILQ_EINVAL;
+  if ((T != 0 && (!qkv || !q_out)) || !starts || !seqlens || !page_table || !k || !v || !dev_err) return ANVILQ_EINVAL;
   if (type != kBinary16 && (!k_scales || !v_scales)) return ANVILQ_EINVAL;
   if (flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) return ANVILQ_EINVAL;
   if (T < 0 || B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || !(theta > 0.0f) || !std::isfinite(theta))

@@ -859,7 +859,7 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
             raise ValueError(f"{name}: rows of {what} must be contiguous and must not overlap")
         return apart if shape[0] > 1 else shape[1]
 
-    L = history_pitch = 0
+    L = history_pitch = 0    # (of a history without columns nothing is read: any address will do)
     if history is not None:
         if history_lens is None:
             raise ValueError(f"{name}: history needs history_lens")
@@ -875,9 +875,6 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
     rows(repetition, torch.float32, "repetition", B)
     rows(presence, torch.float32, "presence", B)
     rows(frequency, torch.float32, "frequency", B)
-    if L == 0:
-        history = None       # no tokens: nothing to penalise
-        history_lens = prompt_lens = repetition = presence = frequency = None
     n_bias = 0
     if bias_starts is not None:
         if bias_ids is None or bias_values is None:
@@ -915,7 +912,7 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
     ws = _call_workspace(dev, WORKSPACE_COUNTER_BYTES, workspace) if choose else None
     err = _error_word(dev, dev_err)
     _call("anvilq_logits_process", dev, _ptr(logits), half, pitch if B > 1 else V, _ptr(out), out_pitch, _ptr(tokens),
-          B, V, _ptr(history), history_pitch, _ptr(history_lens), _ptr(prompt_lens), L, _ptr(repetition),
+          B, V, _ptr(history) if L else _ptr(history_lens), history_pitch, _ptr(history_lens), _ptr(prompt_lens), L, _ptr(repetition),
           _ptr(presence), _ptr(frequency), _ptr(bias_starts), _ptr(bias_ids), _ptr(bias_values), n_bias, _ptr(allowed),
           mask_pitch, _ptr(allowed_rows), masks, _ptr(ws), 0 if ws is None else ws.numel(), _ptr(err),
           GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))

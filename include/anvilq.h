@@ -657,7 +657,8 @@ int anvilq_gqa_decode_paged(const uint16_t* q, const uint16_t* k_pool, const uin
  * page_tokens * max_pages, sets ANVILQ_DEV_ERR_SEQLEN, an absent page of a new
  * token ANVILQ_DEV_ERR_PAGE; nothing is then written for it (for that page).
  * D in {64, 128}, page_tokens % 16 == 0, qkv_stride % 8 == 0, 16-byte aligned
- * qkv, q_out and pools; dev_err required; T == 0 does nothing. */
+ * qkv, q_out and pools; dev_err required; T == 0 does nothing (qkv and q_out
+ * may then be NULL). */
 int anvilq_paged_kv_append(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
                            const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, uint16_t* k_pool,
                            uint16_t* v_pool, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages,
@@ -691,11 +692,13 @@ int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k
  * b is its token at position seqlens[b] - Q + i and sees every position up to
  * its own (Q = 1: the decode step; more: drafted tokens or a chunk, appended
  * before).  q and out fp16 [B][Q][Hq][D], seqlens int32 [B] (device, 0 ..
- * page_tokens * max_pages).  A query that sees nothing -- an empty sequence, or
+ * page_tokens * max_pages <= 2^30).  A query that sees nothing -- an empty sequence, or
  * a position below 0 -- gives zeros.  Scores and the softmax run in fp32, the
  * probabilities enter the tensor cores as binary16.  scale <= 0 selects
- * 1/sqrt(D).  Hq % Hkv == 0, Hq <= 1024, Q <= 64, B <= 65535; 16-byte aligned
- * q, codes and out; dev_err required.  A length outside its range sets
+ * 1/sqrt(D).  Hq % Hkv == 0, Hq <= 1024, Q <= 64, B <= 65535, at most 2^31 - 1
+ * rows (num_pages * page_tokens * Hkv) in a pool; the tables' positions over
+ * 32, times Hkv and the groups of 8 or 16 query rows of a head, at most 2^31;
+ * 16-byte aligned q, codes and out; dev_err required.  A length outside its range sets
  * ANVILQ_DEV_ERR_SEQLEN and counts as 0; an absent live page sets
  * ANVILQ_DEV_ERR_PAGE (the output is then not to be used).  workspace: at least
  * anvilq_gqa_decode_q8_workspace_size(...) bytes (0: shape not supported),
@@ -716,9 +719,9 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
  *   v in the row's bias list, entries bias_starts[b] .. bias_starts[b + 1] of
  *   bias_ids / bias_values (of bias_total):  l = l + the value of v's LAST entry
  *   bit v % 32 of word v / 32 of its mask clear:  l = -inf
- * out (fp32, out_stride apart; may be the fp32 logits themselves) = l; token[b] =
- * the lowest v with the largest l > -inf, NaN never chosen, -1 when there is
- * none.  Either of out and token may be NULL.
+ * out (fp32, out_stride apart; may be the fp32 logits themselves, else no row of
+ * it may touch theirs) = l; token[b] = the lowest v with the largest l > -inf,
+ * NaN never chosen, -1 when there is none.  Either of out and token may be NULL.
  * history int32 rows of up to L tokens, history_stride apart; penalties fp32
  * [B], each may be NULL (none); history, bias_starts, allowed may be NULL.
  * allowed: `masks` rows of words, allowed_stride apart; row b uses mask
@@ -726,7 +729,7 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
  * A token id outside [0, V) sets ANVILQ_DEV_ERR_TOKEN and is ignored; a
  * history length outside [0, L], a bias range outside its list (an empty one is
  * used) or a mask row >= masks (none is used) sets ANVILQ_DEV_ERR_SEQLEN.
- * B <= 4096; dev_err required; workspace (needed for token):
+ * B <= 4096; V, L, bias_total <= 2^30; dev_err required; workspace (needed for token):
  * anvilq_logits_process_workspace_size bytes, 16-byte aligned, layout as
  * described at ANVILQ_WORKSPACE_COUNTER_BYTES. */
 size_t anvilq_logits_process_workspace_size(int B, int V);

@@ -511,6 +511,71 @@ def test_logits_long_histories(dev):
     assert torch.equal(again, out) and torch.equal(tokens2, tokens)
 
 
+@pytest.mark.parametrize("B,V,L", [(1, 33000, 9000), (3, 70001, 5000), (2, 151936, 20000)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_logits_histories_of_several_ctas(dev, B, V, L, bias):
+    """More tokens of history than a CTA keeps, most of them at one end of the vocabulary,
+    over several CTAs of a row; prompts that are all of it, none, or out of range."""
+    rng = np.random.default_rng(L)
+    x, history, lens, prompts, rep, pres, freq = logits_case(rng, B, V, L, B == 3)
+    lens[:] = [L, L - 77, 2049][:B]
+    d = lambda a: to(a, dev)
+    lists = [[(int(t), float(w)) for t, w in zip(rng.integers(0, V, 50), rng.standard_normal(50).astype(np.float32))]
+             for _ in range(B)] if bias else None
+    kw = dict(bias_starts=d(np.arange(0, 50 * B + 1, 50, dtype=np.int32)),
+              bias_ids=d(np.array([t for r in lists for t, _ in r], np.int32)),
+              bias_values=d(np.array([w for r in lists for _, w in r], np.float32))) if bias else {}
+    for prompts in ([L, 0, 2048], [-5, 2**31 - 1, 2049], [L - 1, 3000, -2**31]):
+        prompts = np.array(prompts[:B], np.int64).astype(np.int32)
+        out, tokens = ops.logits_process(d(x), history=d(history), history_lens=d(lens), prompt_lens=d(prompts),
+                                         repetition=d(rep), presence=d(pres), frequency=d(freq), **kw)
+        ops.raise_device_errors(dev)
+        check_logits(dev, x, out, tokens, (history, lens, prompts, rep, pres, freq, lists, None))
+    out, tokens = ops.logits_process(d(x), history=d(history), history_lens=d(lens), repetition=d(rep), **kw)
+    check_logits(dev, x, out, tokens, (history, lens, None, rep, None, None, lists, None))
+
+
+def test_logits_rows_that_take_turns_or_overlap(dev):
+    rng = np.random.default_rng(20)
+    x = rng.standard_normal((3, 64)).astype(np.float32)
+    both = torch.zeros((3, 128), device=dev)
+    both[:, :64] = to(x, dev)
+    out, _ = ops.logits_process(both[:, :64], out=both[:, 64:])
+    assert np.array_equal(out.cpu().numpy(), x) and np.array_equal(both[:, :64].cpu().numpy(), x)
+    flat = torch.zeros(300, device=dev)
+    rows = flat[:192].view(3, 64)
+    for logits, bad in ((rows, flat[4:196].view(3, 64)), (rows, flat[:228].view(3, 76)[:, :64]),
+                        (both[:, :64], both[:, 32:96])):
+        with pytest.raises(AnvilqError):
+            ops.logits_process(logits, out=bad)
+    with pytest.raises(AnvilqError):                       # binary16 logits under their own results
+        ops.logits_process(flat[:192].view(torch.float16).view(3, 128)[:, :64], out=rows)
+    ops.raise_device_errors(dev)
+
+
+def test_logits_empty_history(dev):
+    x = torch.ones((2, 40), device=dev)
+    none = torch.zeros((2, 0), dtype=torch.int32, device=dev)
+    lens = torch.zeros(2, dtype=torch.int32, device=dev)
+    out, _ = ops.logits_process(x, history=none, history_lens=lens, presence=torch.ones(2, device=dev))
+    assert torch.equal(out, x)
+    ops.raise_device_errors(dev)
+    ops.logits_process(x, history=none, history_lens=lens + 1)
+    with pytest.raises(AnvilqError, match="length"):
+        ops.raise_device_errors(dev)
+
+
+def test_append_without_tokens(dev):
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
+    qkv = torch.zeros((0, 6 * 64), dtype=torch.float16, device=dev)
+    pool = torch.zeros((2, 16, 1, 64), dtype=torch.float16, device=dev)
+    table = torch.zeros((1, 1), dtype=torch.int32, device=dev)
+    assert ops.paged_kv_append(qkv, pool, pool.clone(), table, i32(3), i32(0, 0), 4).shape == (0, 4, 64)
+    codes, scales = torch.zeros((2, 1, 16, 64), dtype=torch.int8, device=dev), torch.zeros((2, 1, 1), device=dev)
+    assert ops.paged_kv_append_q8(qkv, codes, codes.clone(), scales, scales.clone(), table, i32(3), i32(0, 0), 4).shape == (0, 4, 64)
+    ops.raise_device_errors(dev)
+
+
 @pytest.mark.parametrize("given", [(), ("repetition",), ("presence",), ("frequency",), ("allowed",), ("bias",)])
 def test_logits_parts_alone(dev, given):
     """Each part without the others; rows that share masks or have none; prompt lengths left out."""

@@ -43,13 +43,21 @@ CASES = [
     ("anvilq_gqa_decode_q8", ATTN, EINVAL, [dict(q=None), dict(k=None), dict(vs=None), dict(table=None),
      dict(lens=None), dict(out=None), dict(err=None), dict(code=3), dict(flags=8)]),
     ("anvilq_gqa_decode_q8", ATTN, ESHAPE, [dict(B=0), dict(Q=0), dict(Q=65), dict(Hq=9), dict(Hkv=0), dict(D=80),
-     dict(page=8), dict(pages=0), dict(max_pages=0), dict(page=1 << 20, max_pages=2000)]),
+     dict(page=8), dict(pages=0), dict(max_pages=0), dict(page=1 << 20, max_pages=2000),
+     dict(pages=1 << 26), dict(pages=2**31 - 1, page=2**31 - 16, max_pages=1),
+     dict(B=65535, Hq=1024, Hkv=1024, max_pages=1 << 20)]),
     ("anvilq_gqa_decode_q8", ATTN, EALIGN, [dict(q=ODD), dict(k=ODD), dict(v=ODD), dict(out=ODD), dict(ws=ODD)]),
     ("anvilq_logits_process", LOGITS, EINVAL, [dict(x=None), dict(out=None, token=None), dict(err=None), dict(B=0),
      dict(V=0), dict(half=2), dict(stride=999), dict(out_stride=999), dict(hist_lens=None), dict(L=-1),
      dict(hist_stride=9), dict(history=None), dict(bias_total=-1), dict(bias_ids=None), dict(bias=None),
-     dict(masks=0), dict(masks=1), dict(allowed_stride=31), dict(flags=2)]),
-    ("anvilq_logits_process", LOGITS, ESHAPE, [dict(B=4097, masks=4097)]),
+     dict(masks=0), dict(masks=1), dict(allowed_stride=31), dict(flags=2),
+     # results over logits that are still to be read
+     dict(out=ctypes.c_void_p((1 << 20) + 4000)), dict(out=ctypes.c_void_p((1 << 20) - 4)), dict(half=1),
+     dict(out_stride=1001), dict(stride=2000, out_stride=2000, out=ctypes.c_void_p((1 << 20) + 3996)),
+     dict(stride=2000, out_stride=2000, out=ctypes.c_void_p((1 << 20) - 8000 + 4004))]),
+    ("anvilq_logits_process", LOGITS, ESHAPE, [dict(B=4097, masks=4097), dict(V=(1 << 30) + 32, stride=1 << 40,
+     out_stride=1 << 40, allowed_stride=1 << 30), dict(L=(1 << 30) + 1, hist_stride=1 << 31),
+     dict(bias_total=(1 << 30) + 1)]),
     ("anvilq_logits_process", LOGITS, EWORKSPACE, [dict(ws=None), dict(bytes=65535)]),
     ("anvilq_logits_process", LOGITS, EALIGN, [dict(ws=ODD)]),
 ]
