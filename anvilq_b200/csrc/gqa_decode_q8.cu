@@ -63,6 +63,7 @@ namespace attn8 {
 using q8::kBlock;
 constexpr int kTile = 2 * kBlock;   // tokens of a step
 constexpr int kMaxSms = 160;        // SMs that are used, one CTA each
+constexpr int kMaxBatch = 65536;
 constexpr unsigned long long kWaitLimitNs = 1000000000ull;
 
 struct Divisor {     // x / d for 0 <= x < 2^17, 1 <= d < 2^15: the error of m is below d / 2^32
@@ -108,7 +109,8 @@ struct Shape {
   static constexpr int kStatOffset = kWarps * kRingBytes;      // (m, l) [warp][2][row]
   static constexpr int kMetaOffset = kStatOffset + kWarps * 2 * kRows * 8;
   static constexpr int kBarOffset = kMetaOffset + kWarps * kSlots * 48;
-  static constexpr int kEnd = kBarOffset + kWarps * kStages * 8;
+  static constexpr int kGroupOffset = kBarOffset + kWarps * kStages * 8;   // tiles of 32 sequences each
+  static constexpr int kEnd = kGroupOffset + kMaxBatch / 32 * 4;
   static constexpr int kTotal = kEnd + 1024;                   // + slack to align the rings
   static constexpr int kPartial = kState + 2 * kRows;          // floats of a state in global memory
   static_assert((kStages & (kStages - 1)) == 0 && kStages <= 4, "a slot's old tile is used by the time it is named again");
@@ -230,7 +232,7 @@ __device__ __forceinline__ Plan plan_of(unsigned total, int longest, int all_pai
   pl.total = total;
   const unsigned even = max(1u, (total + ctas * W - 1) / (ctas * W));
   const unsigned rounds = (all_pairs + ctas - 1) / ctas;
-  pl.whole = rounds * ((longest + W - 1) / W) <= even;
+  pl.whole = rounds * ((longest + W - 1) / W) <= even + 1;
   pl.chunk = even * W;
   return pl;
 }
@@ -246,6 +248,7 @@ enum { kHas0 = 1, kEnds0 = 2, kParked0 = 4, kHas1 = 8 };
 struct Control {     // in shared memory
   Part part[kMaxWarps][2];   // [0] a pair begun before the warp's stretch, [1] one that goes on after it
   int flags[kMaxWarps];      // kHas0 ...
+  int longest[kMaxWarps];    // tiles of a pair that the warp has seen
   int last[2];
   uint2 open[2];             // first CTA and number of CTAs of a pair that spans several
   Plan plan;                 // out of the registers of the tile loop; every warp writes the same
@@ -842,17 +845,34 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, 1)
 
   const int capacity = p.page_tokens * p.max_pages;   // <= 2^30
   // ---- the row of all tiles: its length, its longest pair ----
+  // Up to 32 sequences every warp counts for itself (no barrier).  More: the warps
+  // share the counting, 32 sequences a group.  (Every warp counting all: 1024 sequences of 1 .. 64 tokens, 32/8 heads of 128, OLD
+  // us against NEW.)
   const int pairs = p.Hkv * p.row_groups.d;   // of a sequence
+  unsigned* group_tiles = reinterpret_cast<unsigned*>(smem + S::kGroupOffset);
   {
+    const int groups = (p.B + 31) / 32;
     unsigned sum = 0;
     int longest = 0;
-    for (int b = lane; b < p.B; b += 32) {
-      const int n = tiles_of(p, b);
-      sum += n;
-      longest = max(longest, n);
+    if (groups == 1) {
+      const int n = lane < p.B ? tiles_of(p, lane) : 0;
+      sum = __reduce_add_sync(0xffffffffu, (unsigned)n);
+      longest = __reduce_max_sync(0xffffffffu, n);
+    } else {
+#pragma unroll 4
+      for (int i = warp; i < groups; i += W) {
+        const int b = 32 * i + lane, n = b < p.B ? tiles_of(p, b) : 0;
+        const unsigned tiles = __reduce_add_sync(0xffffffffu, (unsigned)n);
+        if (lane == 0) group_tiles[i] = tiles;
+        longest = max(longest, n);
+      }
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      if (lane == 0) ctl.longest[warp] = longest;
+      __syncthreads();
+      for (int i = lane; i < groups; i += 32) sum += group_tiles[i];
+      sum = __reduce_add_sync(0xffffffffu, sum);
+      longest = __reduce_max_sync(0xffffffffu, lane < W ? ctl.longest[lane] : 0);
     }
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    longest = __reduce_max_sync(0xffffffffu, longest);
     const Plan plan = plan_of<W>(sum * pairs, longest, p.B * pairs, gridDim.x);
     if (lane == 0) ctl.plan = plan;
     __syncwarp();
@@ -878,8 +898,9 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, 1)
       const unsigned share = ctl.plan.chunk / W;
       begin = from + warp * share;
       count = begin < ctl.plan.total ? (int)min(share, ctl.plan.total - begin) : 0;
-      for (int b0 = 0; count > 0; b0 += 32) {
-        const unsigned tiles = b0 + lane < p.B ? tiles_of(p, b0 + lane) * pairs : 0;
+      // of 32 runs of tiles, the next from base_first on, the one that holds `begin`
+      // (moving base_first there); 32 where none does
+      auto holds = [&](unsigned tiles) {
         unsigned incl = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -887,13 +908,18 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, 1)
           if (lane >= o) incl += up;
         }
         const uint32_t past = __ballot_sync(0xffffffffu, base_first + incl > begin);
-        if (past || b0 + 32 >= p.B) {   // some sequence holds it, as begin < total
-          const int l = past ? __ffs(past) - 1 : (p.B - 1) % 32;
-          b_first = b0 + l;
-          base_first += __shfl_sync(0xffffffffu, incl - tiles, l);
-          break;
-        }
-        base_first += __shfl_sync(0xffffffffu, incl, 31);
+        const int l = past ? __ffs(past) - 1 : 32;
+        base_first += __shfl_sync(0xffffffffu, past ? incl - tiles : incl, min(l, 31));
+        return l;
+      };
+      if (count > 0) {   // some sequence holds it, as begin < total
+        int group = 0;
+        const int groups = (p.B + 31) / 32;
+        for (int l = 32; groups > 1 && l == 32 && group < groups; group += l)
+          l = holds(group + lane < groups ? group_tiles[group + lane] * pairs : 0);
+        const int b = 32 * group + lane;
+        b_first = 32 * group + holds(b < p.B ? tiles_of(p, b) * pairs : 0);
+        b_first = min(b_first, p.B - 1);
       }
     }
     if (ok) ok = run_stretch<D, TYPE, RT>(mk, mv, p, smem, ctl, before, begin, count, b_first, base_first);
@@ -907,12 +933,13 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, 1)
     __syncthreads();
   }
   // empty sequences (and lengths that are none)
-  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    const int n = p.seqlens[b];
-    if (n >= 1 && n <= capacity) continue;
-    if (n != 0 && threadIdx.x == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
-    uint4* o = reinterpret_cast<uint4*>(p.out + (size_t)b * p.Q * p.Hq * D);
-    for (int i = threadIdx.x; i < p.Q * p.Hq * (D / 8); i += S::kThreads) o[i] = make_uint4(0, 0, 0, 0);
+  for (int b0 = blockIdx.x; b0 < p.B; b0 += 32 * gridDim.x) {   // a lane each, 32 at a time
+    const int b = b0 + lane * gridDim.x, len = b < p.B ? p.seqlens[b] : 1;
+    if (warp == 0 && (len < 0 || len > capacity)) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+    for (uint32_t none = __ballot_sync(0xffffffffu, len < 1 || len > capacity); none; none &= none - 1) {
+      uint4* o = reinterpret_cast<uint4*>(p.out + (size_t)(b0 + (__ffs(none) - 1) * gridDim.x) * p.Q * p.Hq * D);
+      for (int i = threadIdx.x; i < p.Q * p.Hq * (D / 8); i += S::kThreads) o[i] = make_uint4(0, 0, 0, 0);
+    }
   }
 }
 
@@ -921,7 +948,7 @@ static bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) =
 
 constexpr int kMaxQueries = 64;   // query tokens of a sequence
 static bool shape_ok(int B, int Q, int Hq, int Hkv, int D) {
-  return B >= 1 && B <= 65535 && Q >= 1 && Q <= kMaxQueries && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 &&
+  return B >= 1 && B < kMaxBatch && Q >= 1 && Q <= kMaxQueries && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 &&
          Hq <= 1024 && (D == 64 || D == 128);
 }
 

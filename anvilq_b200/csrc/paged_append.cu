@@ -436,8 +436,11 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   // two: 560 items into binary16 47.5 and 39.9 us, 350 items into 8 bits 32.0 and
   // 24.8, but 538 items into 8 bits 38.1 and 41.8.
   const long long enough = 148 * (type == kBinary16 ? 4 : 3);
+  // (Items are counted as if every sequence had one more than its rows fill, since
+  // the lengths are on the device.)
+  const long long likely = std::min<long long>(items, T / kBlock + B);
   int slices = 1;
-  while (slices * 8 < heads && (long long)items * slices < enough) slices *= 2;
+  while (slices * 8 < heads && likely * slices < enough) slices *= 2;
   p.heads_per_cta = (heads + slices - 1) / slices;
   // the frequencies of the thread's last theta and D (64 powers cost the host 3 us)
   thread_local Freq freq;
