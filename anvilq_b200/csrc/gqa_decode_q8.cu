@@ -220,10 +220,10 @@ __device__ __forceinline__ void e4m3x4_to_half4(uint32_t w, uint32_t& lo, uint32
 // the swizzle, 8 different 16-byte banks either way.
 __device__ __forceinline__ int token_of(int n) { return (n & 8) | ((n & 1) ? ((n & 6) ^ 5) : (n & 7)); }
 
-// A CTA a pair, when no warp then has more tiles than with equal shares: it saves
-// the merge across CTAs (tickets and a round trip through L2).  One sequence of 150
-// tokens, 14/2 heads of 64: 6.7 us against 12.0.  With a few tiles more than equal
-// shares it already loses: 1500 tokens 12.7 us against 10.3.  Equal shares otherwise:
+// A CTA a pair, when no warp then has more than one tile more than with equal shares:
+// it saves the merge across CTAs (tickets and a round trip through L2).  One sequence,
+// 14/2 heads of 64: 150 tokens 6.7 us against 12.0, 500 tokens (a tile more) 9.0
+// against 10.7, but 1500 tokens (three more) 12.7 against 10.3.  Equal shares otherwise:
 // 32 sequences x 32768 tokens, 32/8 heads of 128, 332 us; with the last sixth of the
 // work dealt out in small chunks as CTAs finish 351 us (each chunk drains a CTA's
 // pipeline), and two CTAs an SM instead of one larger 364 us.
@@ -878,8 +878,8 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, 1)
   const int capacity = p.page_tokens * p.max_pages;   // <= 2^30
   // ---- the row of all tiles: its length, its longest pair ----
   // Up to 32 sequences every warp counts for itself (no barrier).  More: the warps
-  // share the counting, 32 sequences a group.  (Every warp counting all: 1024 sequences of 1 .. 64 tokens, 32/8 heads of 128, OLD
-  // us against NEW.)
+  // share the counting, 32 sequences a group.  (Every warp counting all:
+  // 1024 sequences of 1 .. 64 tokens, 32/8 heads of 128, 40.0 us against 35.4.)
   const int pairs = p.Hkv * p.row_groups.d;   // of a sequence
   unsigned* group_tiles = reinterpret_cast<unsigned*>(smem + S::kGroupOffset);
   {

@@ -78,6 +78,7 @@ APPENDS = [
     ([32700, 9], [60, 300], 14, 2, 64, 48),                   # far positions, pages of three blocks
     ([0] * 70, [1] * 70, 4, 2, 128, 16),                      # more than 32 sequences
     ([i % 23 for i in range(40)], [i % 5 for i in range(40)], 2, 1, 64, 16),   # many empty ones
+    ([i % 40 for i in range(150)], [1 + i % 9 for i in range(150)], 32, 8, 128, 16),   # heads in slices
 ]
 
 
@@ -363,6 +364,26 @@ def test_attention_q8(dev, lens, Q, Hq, Hkv, D, page, fp8):
     check_attention(out.cpu().numpy(), q, k, v, ks, vs, table, lens)
     if Q == 1:
         assert torch.equal(ops.gqa_decode_q8(qd[:, 0], *a, scale=float(1 / np.sqrt(D))), out[:, 0])
+
+
+@pytest.mark.parametrize("B,top,Hq,Hkv,D", [(33, 60, 4, 2, 64), (200, 90, 16, 2, 128), (2500, 20, 2, 1, 64)])
+def test_attention_q8_many_sequences(dev, B, top, Hq, Hkv, D):
+    """More sequences than a warp looks over at once, idle slots and lengths out of range among them."""
+    rng = np.random.default_rng(B)
+    lens = rng.integers(0, top + 1, B)
+    lens[rng.integers(0, B, B // 5)] = 0
+    q, k, v, ks, vs, table = attention_case(dev, rng, [int(n) for n in lens], 1, Hq, Hkv, D, 16, False)
+    a = [t.to(dev) for t in (k, v, ks, vs)] + [to(table, dev)]
+    out = ops.gqa_decode_q8(to(q, dev), *a, to(lens.astype(np.int32), dev), out=torch.full(q.shape, float("nan"), dtype=torch.float16, device=dev))
+    ops.raise_device_errors(dev)
+    check_attention(out.cpu().numpy(), q, k, v, ks, vs, table, [int(n) for n in lens])
+    bad = rng.choice(B, 3, replace=False)
+    lens[bad] = [-7, 16 * table.shape[1] + 1, 2 ** 31 - 1]
+    out = ops.gqa_decode_q8(to(q, dev), *a, to(lens.astype(np.int32), dev))
+    with pytest.raises(AnvilqError, match="length"):
+        ops.raise_device_errors(dev)
+    lens[bad] = 0
+    check_attention(out.cpu().numpy(), q, k, v, ks, vs, table, [int(n) for n in lens])
 
 
 @pytest.mark.parametrize("fp8", [False, True])
