@@ -1085,7 +1085,7 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   if (!q || !k_codes || !v_codes || !k_scales || !v_scales || !page_table || !seqlens || !out || !dev_err)
     return ANVILQ_EINVAL;
   if (code_type != ANVILQ_KV_Q8_INT8 && code_type != ANVILQ_KV_Q8_E4M3) return ANVILQ_EINVAL;
-  if (flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) return ANVILQ_EINVAL;
+  if ((flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) || !(scale < INFINITY)) return ANVILQ_EINVAL;
   if (!shape_ok(B, Q, Hq, Hkv, D) || page_tokens < kBlock || page_tokens % kBlock || max_pages < 1 || num_pages < 1 ||
       (long long)page_tokens * max_pages > (1LL << 30))
     return ANVILQ_ESHAPE;

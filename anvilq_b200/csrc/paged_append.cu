@@ -375,6 +375,10 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* k, const uin
   }
 }
 
+static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + nb && y < x + na;
+}
 static bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename... KArgs, typename... Args>
@@ -413,6 +417,9 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   if (stride < (long long)heads * D) return ANVILQ_EINVAL;
   if (!a16(qkv) || !a16(q_out) || !a16(k) || !a16(v) || stride % 8) return ANVILQ_EALIGN;
   if (T == 0) return ANVILQ_OK;
+  // an item's q is written while others' rows are still to be read
+  if (overlap(qkv, ((size_t)(T - 1) * stride + (size_t)heads * D) * 2, q_out, (size_t)T * Hq * D * 2))
+    return ANVILQ_EINVAL;
   Params p{};
   p.qkv = reinterpret_cast<const __half*>(qkv);
   p.stride = stride;
@@ -497,7 +504,14 @@ int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k
   if (num_pages < 1 || Hkv < 1) return ANVILQ_EINVAL;
   if ((D != 64 && D != 128) || page_tokens < kBlock || page_tokens % kBlock) return ANVILQ_ESHAPE;
   if (!a16(k_codes) || !a16(v_codes) || !a16(k_out) || !a16(v_out)) return ANVILQ_EALIGN;
-  const long long pieces = (long long)num_pages * Hkv * page_tokens * (D / 8);
+  const long long rows = (long long)num_pages * page_tokens;
+  if (rows > (1LL << 40) / Hkv) return ANVILQ_ESHAPE;
+  const long long pieces = rows * Hkv * (D / 8);
+  const size_t values = pieces * 16, codes = pieces * 8;
+  if (overlap(k_out, values, v_out, values) || overlap(k_out, values, k_codes, codes) ||
+      overlap(k_out, values, v_codes, codes) || overlap(v_out, values, k_codes, codes) ||
+      overlap(v_out, values, v_codes, codes))
+    return ANVILQ_EINVAL;
   const int blocks = (int)std::min<long long>((pieces + 2047) / 2048, 148 * 8);
   auto go = [&](auto kernel) {
     return launch(kernel, dim3(blocks, 2), 256, reinterpret_cast<cudaStream_t>(stream), flags,

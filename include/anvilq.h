@@ -658,7 +658,7 @@ int anvilq_gqa_decode_paged(const uint16_t* q, const uint16_t* k_pool, const uin
  * token ANVILQ_DEV_ERR_PAGE; nothing is then written for it (for that page).
  * D in {64, 128}, page_tokens % 16 == 0, qkv_stride % 8 == 0, 16-byte aligned
  * qkv, q_out and pools; dev_err required; T == 0 does nothing (qkv and q_out
- * may then be NULL). */
+ * may then be NULL); q_out lies outside the span of qkv's rows. */
 int anvilq_paged_kv_append(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
                            const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, uint16_t* k_pool,
                            uint16_t* v_pool, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages,
@@ -683,7 +683,7 @@ int anvilq_paged_kv_append_q8(const uint16_t* qkv, long long qkv_stride, const i
 
 /* The values of whole 8-bit pools in binary16: out[page][head][token][d] =
  * fp16(code * scale), same layout as the codes (to move pages into binary16, or
- * to look at them).  16-byte aligned codes and outputs. */
+ * to look at them).  16-byte aligned codes and outputs, which do not overlap. */
 int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales,
                         int code_type, uint16_t* k_out, uint16_t* v_out, int num_pages, int Hkv, int page_tokens,
                         int D, unsigned flags, anvilq_stream_t stream);
@@ -694,7 +694,7 @@ int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k
  * before).  q and out fp16 [B][Q][Hq][D], seqlens int32 [B] (device, 0 ..
  * page_tokens * max_pages <= 2^30).  A query that sees nothing -- an empty sequence, or
  * a position below 0 -- gives zeros.  Scores and the softmax run in fp32, the
- * probabilities enter the tensor cores as binary16.  scale <= 0 selects
+ * probabilities enter the tensor cores as binary16.  scale (finite) <= 0 selects
  * 1/sqrt(D).  Hq % Hkv == 0, Hq <= 1024, Q <= 64, B <= 65535, at most 2^31 - 1
  * rows (num_pages * page_tokens * Hkv) in a pool; the tables' positions over
  * 32, times Hkv and the groups of 8 or 16 query rows of a head, at most 2^31;

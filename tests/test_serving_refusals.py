@@ -10,12 +10,19 @@ EINVAL, EALIGN, EWORKSPACE, ESHAPE = -1, -2, -4, -5
 FAKE = ctypes.c_void_p(1 << 20)   # never dereferenced: every call here is rejected
 ODD = ctypes.c_void_p((1 << 20) + 8)
 
-APPEND = dict(qkv=FAKE, stride=1536, starts=FAKE, lens=FAKE, table=FAKE, q=FAKE, k=FAKE, v=FAKE, T=4, B=2, Hq=8,
+
+def at(byte):
+    return ctypes.c_void_p((1 << 20) + byte)
+
+
+QKV, OUT, OUT2 = FAKE, at(1 << 24), at(1 << 25)
+
+APPEND = dict(qkv=QKV, stride=1536, starts=FAKE, lens=FAKE, table=FAKE, q=OUT, k=FAKE, v=FAKE, T=4, B=2, Hq=8,
               Hkv=2, D=128, page=16, max_pages=4, pages=8, theta=1e6, err=FAKE, flags=0, stream=None)
-APPEND_Q8 = dict(qkv=FAKE, stride=1536, starts=FAKE, lens=FAKE, table=FAKE, q=FAKE, k=FAKE, v=FAKE, ks=FAKE, vs=FAKE,
+APPEND_Q8 = dict(qkv=QKV, stride=1536, starts=FAKE, lens=FAKE, table=FAKE, q=OUT, k=FAKE, v=FAKE, ks=FAKE, vs=FAKE,
                  code=0, T=4, B=2, Hq=8, Hkv=2, D=128, page=16, max_pages=4, pages=8, theta=1e6, err=FAKE, flags=0,
                  stream=None)
-VALUES = dict(k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, code=0, ko=FAKE, vo=FAKE, pages=4, Hkv=2, page=16, D=128, flags=0,
+VALUES = dict(k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, code=0, ko=OUT, vo=OUT2, pages=4, Hkv=2, page=16, D=128, flags=0,
               stream=None)
 ATTN = dict(q=FAKE, k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, code=0, table=FAKE, lens=FAKE, out=FAKE, B=2, Q=1, Hq=8, Hkv=2,
             D=128, page=16, max_pages=4, pages=8, scale=0.0, ws=FAKE, bytes=1 << 30, err=FAKE, flags=0, stream=None)
@@ -27,7 +34,9 @@ LOGITS = dict(x=FAKE, half=0, stride=1000, out=FAKE, out_stride=1000, token=FAKE
 CASES = [
     ("anvilq_paged_kv_append", APPEND, EINVAL, [dict(qkv=None), dict(starts=None), dict(lens=None), dict(table=None),
      dict(q=None), dict(k=None), dict(v=None), dict(err=None), dict(T=-1), dict(B=0), dict(Hq=0), dict(Hq=9),
-     dict(theta=0.0), dict(theta=float("nan")), dict(theta=float("inf")), dict(flags=2), dict(stride=1528)]),
+     dict(theta=0.0), dict(theta=float("nan")), dict(theta=float("inf")), dict(flags=2), dict(stride=1528),
+     # q's rows among those that are still to be read
+     dict(q=QKV), dict(q=at(6144)), dict(q=at(-8192 + 16)), dict(q=at(4 * 3088 - 32), stride=1544)]),
     ("anvilq_paged_kv_append", APPEND, ESHAPE, [dict(D=96), dict(page=8), dict(page=24), dict(page=0),
      dict(max_pages=0), dict(pages=0), dict(page=1 << 20, max_pages=1 << 20)]),
     ("anvilq_paged_kv_append", APPEND, EALIGN, [dict(qkv=ODD), dict(q=ODD), dict(k=ODD), dict(v=ODD),
@@ -37,11 +46,13 @@ CASES = [
     ("anvilq_paged_kv_append_q8", APPEND_Q8, ESHAPE, [dict(D=256), dict(page=20)]),
     ("anvilq_paged_kv_append_q8", APPEND_Q8, EALIGN, [dict(k=ODD), dict(v=ODD)]),
     ("anvilq_kv_q8_values", VALUES, EINVAL, [dict(k=None), dict(ks=None), dict(ko=None), dict(code=7), dict(pages=0),
-     dict(Hkv=0), dict(flags=2)]),
+     dict(Hkv=0), dict(flags=2), dict(ko=FAKE), dict(vo=FAKE), dict(ko=OUT2), dict(vo=at(16368)),
+     dict(ko=at(-32752))]),
     ("anvilq_kv_q8_values", VALUES, ESHAPE, [dict(D=32), dict(page=17)]),
     ("anvilq_kv_q8_values", VALUES, EALIGN, [dict(ko=ODD), dict(v=ODD)]),
     ("anvilq_gqa_decode_q8", ATTN, EINVAL, [dict(q=None), dict(k=None), dict(vs=None), dict(table=None),
-     dict(lens=None), dict(out=None), dict(err=None), dict(code=3), dict(flags=8)]),
+     dict(lens=None), dict(out=None), dict(err=None), dict(code=3), dict(flags=8),
+     dict(scale=float("inf")), dict(scale=float("nan"))]),
     ("anvilq_gqa_decode_q8", ATTN, ESHAPE, [dict(B=0), dict(Q=0), dict(Q=65), dict(Hq=9), dict(Hkv=0), dict(D=80),
      dict(page=8), dict(pages=0), dict(max_pages=0), dict(page=1 << 20, max_pages=2000),
      dict(pages=1 << 26), dict(pages=2**31 - 1, page=2**31 - 16, max_pages=1),
@@ -52,9 +63,9 @@ CASES = [
      dict(hist_stride=9), dict(history=None), dict(bias_total=-1), dict(bias_ids=None), dict(bias=None),
      dict(masks=0), dict(masks=1), dict(allowed_stride=31), dict(flags=2),
      # results over logits that are still to be read
-     dict(out=ctypes.c_void_p((1 << 20) + 4000)), dict(out=ctypes.c_void_p((1 << 20) - 4)), dict(half=1),
-     dict(out_stride=1001), dict(stride=2000, out_stride=2000, out=ctypes.c_void_p((1 << 20) + 3996)),
-     dict(stride=2000, out_stride=2000, out=ctypes.c_void_p((1 << 20) - 8000 + 4004))]),
+     dict(out=at(4000)), dict(out=at(-4)), dict(half=1),
+     dict(out_stride=1001), dict(stride=2000, out_stride=2000, out=at(3996)),
+     dict(stride=2000, out_stride=2000, out=at(-8000 + 4004))]),
     ("anvilq_logits_process", LOGITS, ESHAPE, [dict(B=4097, masks=4097), dict(V=(1 << 30) + 32, stride=1 << 40,
      out_stride=1 << 40, allowed_stride=1 << 30), dict(L=(1 << 30) + 1, hist_stride=1 << 31),
      dict(bias_total=(1 << 30) + 1)]),
