@@ -891,6 +891,48 @@ def test_overlapped_launches_give_the_same(dev, fp8):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_captured_step_replayed_as_the_sequences_grow(dev, fp8):
+    """One captured step, its lengths and history counted up on the device, against eager steps."""
+    rng = np.random.default_rng(21)
+    B, Hq, Hkv, D, page, width, steps = 6, 14, 2, 64, 32, 5, 40
+    pages = B * width
+    table, one = to(so.make_table([width] * B, pages, rng), dev), to(np.arange(B + 1, dtype=np.int32), dev)
+    rows = [to(rng.standard_normal((B, (Hq + 2 * Hkv) * D)).astype(np.float16), dev) for _ in range(steps)]
+    start = to(rng.integers(0, 100, B).astype(np.int32), dev)
+    history = to(rng.integers(0, Hq * D, (B, width * page)).astype(np.int32), dev)
+    presence = torch.full((B,), 0.25, device=dev)
+    ends = []
+    for captured in (False, True):
+        k = torch.zeros((pages, Hkv, page, D), device=dev).to(code_dtype(fp8))
+        v, ks, vs = k.clone(), *(torch.zeros((pages, Hkv, page // BLOCK), device=dev) for _ in range(2))
+        x, lens = rows[0].clone(), start.clone()
+
+        def step():
+            lens.add_(1)
+            q = ops.paged_kv_append_q8(x, k, v, ks, vs, table, lens, one, Hq)
+            out = ops.gqa_decode_q8(q, k, v, ks, vs, table, lens)
+            return (out, *ops.logits_process(out.view(B, -1), history=history, history_lens=lens, presence=presence))
+
+        if captured:
+            g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream(dev)
+            with torch.cuda.graph(g, stream=s):
+                results = step()
+        seen = []
+        for row in rows:
+            x.copy_(row)
+            if captured:
+                g.replay()
+            else:
+                results = step()
+            seen += [t.clone() for t in results]
+        ends.append([*seen, k.view(torch.uint8), v.view(torch.uint8), ks, vs, lens])
+    torch.cuda.synchronize(dev)
+    ops.raise_device_errors(dev)
+    for a, b in zip(*ends):
+        assert torch.equal(a, b)
+
+
 def test_pools_beyond_31_bits(dev):
     """Codes and rows whose offsets do not fit 31 bits: the last pages of 2.2 GB pools."""
     rng = np.random.default_rng(18)
