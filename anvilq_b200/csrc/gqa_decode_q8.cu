@@ -114,7 +114,8 @@ struct Shape {
   static constexpr int kEnd = kGroupOffset + kMaxBatch / 32 * 4;
   static constexpr int kTotal = kEnd + 1024;                   // + slack to align the rings
   static constexpr int kPartial = kState + 2 * kRows;          // floats of a state in global memory
-  static_assert((kStages & (kStages - 1)) == 0 && kStages <= 4, "a slot's old tile is used by the time it is named again");
+  static_assert((kStages & (kStages - 1)) == 0 && kStages <= 4,
+                "a slot's old tile is used by the time it is named again");
   static_assert(kRingBytes >= kState * 4, "a state fits the idle ring");
   static_assert(kTotal + 4096 <= 227 * 1024, "one CTA an SM");
 };
@@ -434,7 +435,8 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           const int row = token_of(g) + 8 * z;
-          const int at = D == 128 ? row * 128 + (((c + 4 * q) ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+          const int at =
+              D == 128 ? row * 128 + (((c + 4 * q) ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
           w[q][z] = *reinterpret_cast<const uint4*>(kt + at);
         }
 #pragma unroll
@@ -618,7 +620,8 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
             const float f = l[t][e] == 0.0f ? 0.0f : F / l[t][e];
             const int r = r0 + 8 * t + 2 * c + e, i = p.group.quotient(r);
             if (i < p.Q) {
-              __half* dst = p.out + (((size_t)sb * p.Q + i) * p.Hq + kvh * p.group.d + r - i * p.group.d) * D + g * (D / 8);
+              __half* dst =
+                  p.out + (((size_t)sb * p.Q + i) * p.Hq + kvh * p.group.d + r - i * p.group.d) * D + g * (D / 8);
 #pragma unroll
               for (int q = 0; q < NC; ++q) {
                 uint4 w;
@@ -679,7 +682,8 @@ __device__ __forceinline__ void merge_states(const Params& p, unsigned char* sme
     const int i = p.group.quotient(r);
     if (i >= p.Q) return;
     const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-    __half* dst = p.out + (((size_t)pt.b * p.Q + i) * p.Hq + kvh * p.group.d + r - i * p.group.d) * D + 4 * (at % (D / 4));
+    __half* dst =
+        p.out + (((size_t)pt.b * p.Q + i) * p.Hq + kvh * p.group.d + r - i * p.group.d) * D + 4 * (at % (D / 4));
     *reinterpret_cast<uint2*>(dst) =
         make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
   };
@@ -691,13 +695,14 @@ __device__ __forceinline__ void merge_states(const Params& p, unsigned char* sme
   // A chain: the states of one pair in consecutive warps.  It begins with a
   // pair begun earlier in warp 0, or with a warp's pair that goes on.
   const float2* stats = reinterpret_cast<const float2*>(smem + S::kStatOffset);
-  unsigned has0, ends0, parked0, starts;   // bit w: warp w's
+  // bit w: warp w's; of starts bit 0: slot 0 of warp 0, bit w + 1: slot 1 of w
+  unsigned has0, ends0, parked0, starts;
   {
     const int lane = threadIdx.x % 32, fl = lane < W ? ctl.flags[lane] : 0;
     has0 = __ballot_sync(0xffffffffu, fl & kHas0);
     ends0 = __ballot_sync(0xffffffffu, fl & kEnds0);
     parked0 = __ballot_sync(0xffffffffu, fl & kParked0);
-    starts = __ballot_sync(0xffffffffu, fl & kHas1) << 1 | (has0 & 1);   // bit 0: slot 0 of warp 0; bit w + 1: slot 1 of w
+    starts = __ballot_sync(0xffffffffu, fl & kHas1) << 1 | (has0 & 1);
   }
   int open = 0;        // bit s: the pair of ctl.part[open warp][s] spans CTAs
   int open_warp1 = 0;  // (that of slot 0 is warp 0's)
@@ -729,8 +734,9 @@ __device__ __forceinline__ void merge_states(const Params& p, unsigned char* sme
 #pragma unroll (U == 1 ? 2 : 1)
       for (int k = 0; k < members; ++k) {
         const bool parked = (k || !slot) && (parked0 >> (w + k) & 1);
-        const float4* state = parked ? reinterpret_cast<const float4*>(p.parked + ((size_t)blockIdx.x * W + w + k) * S::kState)
-                                     : reinterpret_cast<const float4*>(smem + (w + k) * S::kRingBytes);
+        const float4* state =
+            parked ? reinterpret_cast<const float4*>(p.parked + ((size_t)blockIdx.x * W + w + k) * S::kState)
+                   : reinterpret_cast<const float4*>(smem + (w + k) * S::kRingBytes);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int at = at0 + u * threads, row = at / (D / 4);
@@ -797,7 +803,8 @@ __device__ __forceinline__ void merge_states(const Params& p, unsigned char* sme
   if (!both) return;
   static_assert(W % 2 == 0, "two halves");
   const int threads = both == 2 ? S::kThreads / 2 : S::kThreads;
-  const int slot = both == 2 ? (int)threadIdx.x / threads : ctl.last[1], me = both == 2 ? threadIdx.x % threads : threadIdx.x;
+  const int slot = both == 2 ? (int)threadIdx.x / threads : ctl.last[1];
+  const int me = both == 2 ? threadIdx.x % threads : threadIdx.x;
   unsigned char* room = smem + (both == 2 ? slot * (W / 2) * S::kRingBytes : 0);
   constexpr int kFitAll = W * S::kRingBytes / (S::kPartial * 4), kFitHalf = W / 2 * S::kRingBytes / (S::kPartial * 4);
   const int fit = both == 2 ? kFitHalf : kFitAll;                         // states that fit the room
@@ -1015,7 +1022,9 @@ static int sm_count() {
 static int row_tiles(int Q, int Hq, int Hkv) { return Q * (Hq / Hkv) <= 8 ? 1 : 2; }
 static int max_ctas(int sms) { return std::min(sms, kMaxSms); }
 static size_t partial_floats(int rt, int D, int sms) { return (size_t)max_ctas(sms) * 2 * (8 * rt) * (D + 2); }
-static size_t parked_floats(int rt, int D, int sms) { return (size_t)max_ctas(sms) * (rt == 1 ? 12 : 8) * (8 * rt) * D; }
+static size_t parked_floats(int rt, int D, int sms) {
+  return (size_t)max_ctas(sms) * (rt == 1 ? Shape<64, 1>::kWarps : Shape<64, 2>::kWarps) * (8 * rt) * D;
+}
 
 static std::once_flag g_encode_once;
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;

@@ -605,7 +605,15 @@ def _on_device(name, device, *tensors):
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+_current_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+def _capturing(device):
+    """Whether `device`'s current stream is being captured."""
+    if _current_device() == device.index:
+        return _current_capturing()
+    with torch.cuda.device(device):
+        return _current_capturing()
 
 
 def _call(name, device, *args):
@@ -629,7 +637,7 @@ def _call_workspace(device, nbytes: int, given) -> torch.Tensor:
                 not given.is_contiguous():
             raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {nbytes} bytes on {device}")
         return given
-    if _capturing():
+    if _capturing(device):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         ws[:WORKSPACE_COUNTER_BYTES].zero_()
         return ws
@@ -649,7 +657,7 @@ def _error_word(device, given):
         return given
     w = _dev_err.get(device.index)
     if w is None:
-        if _capturing():
+        if _capturing(device):
             raise RuntimeError("run an operation on this device once before capturing a graph")
         w = device_error_word(device)
     return w
@@ -750,7 +758,8 @@ def paged_kv_append_q8(qkv, k_codes, v_codes, k_scales, v_scales, page_table, se
     err = _error_word(dev, dev_err)
     _call("anvilq_paged_kv_append_q8", dev, qkv.data_ptr(), stride, token_starts.data_ptr(), seqlens.data_ptr(),
           page_table.data_ptr(), q_out.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(),
-          v_scales.data_ptr(), code, T, B, Hq, Hkv, D, page, max_pages, pages, float(theta), err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+          v_scales.data_ptr(), code, T, B, Hq, Hkv, D, page, max_pages, pages, float(theta), err.data_ptr(),
+          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return q_out
 
 
@@ -766,7 +775,8 @@ def kv_q8_values(k_codes, v_codes, k_scales, v_scales, k_out=None, v_out=None, o
             raise ValueError(f"{name}: k_out/v_out must be contiguous float16 with the shape of the codes")
     _on_device(name, dev, v_codes, k_scales, v_scales, k_out, v_out)
     _call("anvilq_kv_q8_values", dev, k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
-          code, k_out.data_ptr(), v_out.data_ptr(), pages, Hkv, page, D, GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+          code, k_out.data_ptr(), v_out.data_ptr(), pages, Hkv, page, D,
+          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return k_out, v_out
 
 
@@ -808,7 +818,8 @@ def gqa_decode_q8(q, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, 
     err = _error_word(dev, dev_err)
     _call("anvilq_gqa_decode_q8", dev, q.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(),
           v_scales.data_ptr(), code, page_table.data_ptr(), seqlens.data_ptr(), out.data_ptr(), B, Q, Hq, Hkv, D, page,
-          max_pages, pages, float(scale), ws.data_ptr(), ws.numel(), err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+          max_pages, pages, float(scale), ws.data_ptr(), ws.numel(), err.data_ptr(),
+          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return out
 
 
@@ -912,8 +923,8 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
     ws = _call_workspace(dev, WORKSPACE_COUNTER_BYTES, workspace) if choose else None
     err = _error_word(dev, dev_err)
     _call("anvilq_logits_process", dev, _ptr(logits), half, pitch if B > 1 else V, _ptr(out), out_pitch, _ptr(tokens),
-          B, V, _ptr(history) if L else _ptr(history_lens), history_pitch, _ptr(history_lens), _ptr(prompt_lens), L, _ptr(repetition),
-          _ptr(presence), _ptr(frequency), _ptr(bias_starts), _ptr(bias_ids), _ptr(bias_values), n_bias, _ptr(allowed),
-          mask_pitch, _ptr(allowed_rows), masks, _ptr(ws), 0 if ws is None else ws.numel(), _ptr(err),
-          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+          B, V, _ptr(history) if L else _ptr(history_lens), history_pitch, _ptr(history_lens), _ptr(prompt_lens), L,
+          _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_starts), _ptr(bias_ids), _ptr(bias_values),
+          n_bias, _ptr(allowed), mask_pitch, _ptr(allowed_rows), masks, _ptr(ws), 0 if ws is None else ws.numel(),
+          _ptr(err), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return out, tokens
