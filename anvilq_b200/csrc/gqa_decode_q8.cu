@@ -136,7 +136,7 @@ struct Part {        // a pair that a warp did not finish alone
 
 // How the work is cut: a warp's stretch is 1 / kWarps of a CTA's tiles.
 struct Plan {
-  bool whole;        // CTAs take whole pairs in turn
+  bool whole;        // a CTA takes a whole pair
   unsigned total;    // tiles in all
   unsigned chunk;    // else: tiles of a CTA
 };
@@ -221,20 +221,22 @@ __device__ __forceinline__ void e4m3x4_to_half4(uint32_t w, uint32_t& lo, uint32
 // the swizzle, 8 different 16-byte banks either way.
 __device__ __forceinline__ int token_of(int n) { return (n & 8) | ((n & 1) ? ((n & 6) ^ 5) : (n & 7)); }
 
-// A CTA a pair, when no warp then has more than one tile more than with equal shares:
-// it saves the merge across CTAs (tickets and a round trip through L2).  One sequence,
-// 14/2 heads of 64: 150 tokens 6.7 us against 12.0, 500 tokens (a tile more) 9.0
-// against 10.7, but 1500 tokens (three more) 12.7 against 10.3.  Equal shares otherwise:
-// 32 sequences x 32768 tokens, 32/8 heads of 128, 332 us; with the last sixth of the
-// work dealt out in small chunks as CTAs finish 351 us (each chunk drains a CTA's
-// pipeline), and two CTAs an SM instead of one larger 364 us.
+// A CTA a pair, where there are enough CTAs and no warp then has more than one tile
+// more than with equal shares: it saves the merge across CTAs (tickets and a round
+// trip through L2).  One sequence, 14/2 heads of 64: 150 tokens 6.7 us against 12.0,
+// 500 tokens (a tile more) 9.0 against 10.7, but 1500 tokens (three more) 12.7 against
+// 10.3; several pairs a CTA one after the other, 64 sequences of 256 tokens, 32/8 heads
+// of 128, 25.7 against 19.2.  Equal shares otherwise: 32 sequences x 32768 tokens, 32/8
+// heads of 128, 332 us; with the last sixth of the work dealt out in small chunks as
+// CTAs finish 351 us (each chunk drains a CTA's pipeline), and two CTAs an SM instead
+// of one larger 364 us.
 template <int W>
 __device__ __forceinline__ Plan plan_of(unsigned total, int longest, int all_pairs, int ctas) {
   Plan pl;
   pl.total = total;
   const unsigned even = max(1u, (total + ctas * W - 1) / (ctas * W));
   const unsigned rounds = (all_pairs + ctas - 1) / ctas;
-  pl.whole = rounds * ((longest + W - 1) / W) <= even + 1;
+  pl.whole = rounds == 1 && (longest + W - 1) / W <= even + 1;
   pl.chunk = even * W;
   return pl;
 }
@@ -258,11 +260,10 @@ struct Control {     // in shared memory
 
 // One warp's stretch: `count` tiles from tile `begin` of the row on, b and base a
 // sequence no later than the first tile's and where its tiles start.  Pairs inside
-// it are finished, the states of others left for merge_states.  `before`: tiles of
-// the warp's earlier stretches.  False after a wait that ran out.
+// it are finished, the states of others left for merge_states.
 template <int D, int TYPE, int RT>
-__device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,
-                                         unsigned char* smem, Control& ctl, uint32_t before, unsigned begin, int count,
+__device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,
+                                         unsigned char* smem, Control& ctl, unsigned begin, int count,
                                          int b_first, unsigned base_first) {
   using S = Shape<D, RT>;
   constexpr int KS = D / 16;        // k-steps of S, m-tiles of O^T
@@ -322,7 +323,7 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
   };
   auto copy = [&](int j) {
     if (lane == 0) {
-      const uint32_t st = (before + j) & (S::kStages - 1);
+      const uint32_t st = j & (S::kStages - 1);
       const uint32_t bar = bar0 + 8 * st, dst = smem_u32(ring) + st * S::kStageBytes;
       const int2 row = *reinterpret_cast<const int2*>(meta[j & (S::kSlots - 1)].row);
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(S::kStageBytes) : "memory");
@@ -385,12 +386,12 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
 
 #pragma unroll 1
   for (; j < count; ++j) {
-    const uint32_t st = (before + j) & (S::kStages - 1);
+    const uint32_t st = j & (S::kStages - 1);
     const Meta& slot = meta[j & (S::kSlots - 1)];
     const struct { int tile, n; } md = {slot.tile, slot.n};
     const bool fresh = j == 0 || md.tile == 0;
     if (fresh && j > 0) begin_pair(slot);
-    if (!warp_wait(bar0 + 8 * st, (before + j) / S::kStages & 1)) {   // no tile is used after this
+    if (!warp_wait(bar0 + 8 * st, j / S::kStages & 1)) {   // no tile is used after this
       ok = false;
       if (lane == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TIMEOUT);
       break;
@@ -662,10 +663,9 @@ __device__ __forceinline__ bool run_stretch(const CUtensorMap& mk, const CUtenso
   if (!ok) {
     // copies in flight land before the shared memory is used for anything else
     for (; j < issued; ++j)
-      if (!warp_wait(bar0 + 8 * ((before + j) & (S::kStages - 1)), (before + j) / S::kStages & 1)) break;
+      if (!warp_wait(bar0 + 8 * (j & (S::kStages - 1)), j / S::kStages & 1)) break;
   }
   if (lane == 0) ctl.flags[warp] = flags;
-  return ok;
 }
 
 // Merges what the warps left.  Its loops keep few values at a time: the tile loop
@@ -916,61 +916,50 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, 1)
     if (lane == 0) ctl.plan = plan;
     __syncwarp();
   }
-  uint32_t before = 0;   // tiles of earlier rounds: tile j's stage and parity follow from before + j
-  bool ok = true;
-  for (unsigned mine = blockIdx.x;; mine += gridDim.x) {   // pair, or chunk
-    // ---- this warp's stretch: `count` tiles from `begin` on ----
-    unsigned begin = 0;
-    int count = 0;
-    int b_first = 0;           // the sequence of the first tile, and where its tiles start
-    unsigned base_first = 0;
-    if (ctl.plan.whole) {
-      if (mine >= (unsigned)(p.B * pairs)) break;
-      b_first = mine / pairs;
+  // ---- this warp's stretch: `count` tiles from `begin` on ----
+  unsigned begin = 0;
+  int count = 0;
+  int b_first = 0;           // the sequence of the first tile, and where its tiles start
+  unsigned base_first = 0;
+  if (ctl.plan.whole) {
+    if (blockIdx.x < (unsigned)(p.B * pairs)) {
+      b_first = blockIdx.x / pairs;
       const int n = tiles_of(p, b_first), share = (n + W - 1) / W;
       // any row's start will do: nothing refers to tiles of other sequences
-      begin = (mine - b_first * pairs) * n + warp * share;
+      begin = (blockIdx.x - b_first * pairs) * n + warp * share;
       count = max(0, min(n - warp * share, share));
-    } else {
-      const unsigned from = mine * ctl.plan.chunk;
-      if (mine >= gridDim.x || from >= ctl.plan.total) break;
-      const unsigned share = ctl.plan.chunk / W;
-      begin = from + warp * share;
-      count = begin < ctl.plan.total ? (int)min(share, ctl.plan.total - begin) : 0;
-      // of 32 runs of tiles, the next from base_first on, the one that holds `begin`
-      // (moving base_first there); 32 where none does
-      auto holds = [&](unsigned tiles) {
-        unsigned incl = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += up;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, base_first + incl > begin);
-        const int l = past ? __ffs(past) - 1 : 32;
-        base_first += __shfl_sync(0xffffffffu, past ? incl - tiles : incl, min(l, 31));
-        return l;
-      };
-      if (count > 0) {   // some sequence holds it, as begin < total
-        int group = 0;
-        const int groups = (p.B + 31) / 32;
-        for (int l = 32; groups > 1 && l == 32 && group < groups; group += l)
-          l = holds(group + lane < groups ? group_tiles[group + lane] * pairs : 0);
-        const int b = 32 * group + lane;
-        b_first = 32 * group + holds(b < p.B ? tiles_of(p, b) * pairs : 0);
-        b_first = min(b_first, p.B - 1);
-      }
     }
-    if (ok) ok = run_stretch<D, TYPE, RT>(mk, mv, p, smem, ctl, before, begin, count, b_first, base_first);
-    else if (lane == 0) ctl.flags[warp] = 0;
-    before += count;
-    __syncthreads();
-    merge_states<D, RT>(p, smem, ctl);
-    if (!ctl.plan.whole) break;
-    // the next pair: the ring's generic reads and writes end before copies fill it again
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
+  } else {
+    const unsigned share = ctl.plan.chunk / W;
+    begin = blockIdx.x * ctl.plan.chunk + warp * share;
+    count = begin < ctl.plan.total ? (int)min(share, ctl.plan.total - begin) : 0;
+    // of 32 runs of tiles, the next from base_first on, the one that holds `begin`
+    // (moving base_first there); 32 where none does
+    auto holds = [&](unsigned tiles) {
+      unsigned incl = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, base_first + incl > begin);
+      const int l = past ? __ffs(past) - 1 : 32;
+      base_first += __shfl_sync(0xffffffffu, past ? incl - tiles : incl, min(l, 31));
+      return l;
+    };
+    if (count > 0) {   // some sequence holds it, as begin < total
+      int group = 0;
+      const int groups = (p.B + 31) / 32;
+      for (int l = 32; groups > 1 && l == 32 && group < groups; group += l)
+        l = holds(group + lane < groups ? group_tiles[group + lane] * pairs : 0);
+      const int b = 32 * group + lane;
+      b_first = 32 * group + holds(b < p.B ? tiles_of(p, b) * pairs : 0);
+      b_first = min(b_first, p.B - 1);
+    }
   }
+  run_stretch<D, TYPE, RT>(mk, mv, p, smem, ctl, begin, count, b_first, base_first);
+  __syncthreads();
+  merge_states<D, RT>(p, smem, ctl);
   // empty sequences (and lengths that are none)
   for (int b0 = blockIdx.x; b0 < p.B; b0 += 32 * gridDim.x) {   // a lane each, 32 at a time
     const int b = b0 + lane * gridDim.x, len = b < p.B ? p.seqlens[b] : 1;
