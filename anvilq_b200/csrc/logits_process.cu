@@ -30,6 +30,7 @@
 // maximum over orderable (value, index) keys, combined over a row's CTAs with an
 // integer atomicMax, so its result does not depend on their order.
 #include <algorithm>
+#include <cmath>
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -442,11 +443,18 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   }
 }
 
-// The CTAs of a row: one wave (four an SM) over the rows, each with two chunks at
-// least and at most what the bitmap holds.
+// The CTAs of a row.  A CTA's time grows with its span, about 0.18 us for 1000 logits;
+// the launch's with the CTAs in all, about 4 ns each, so the sum is least at
+// sqrt(V / 20 B) CTAs a row.  8 rows of 32000: 16 CTAs a row 5.6 us, 4 6.5, 74 6.8; one
+// row of 151936: 100 CTAs 5.3 us, 16 6.5; 297 as much as 74, but of two rows 7.7 against
+// 5.8.  Where one wave (four an SM) holds a CTA a row at least, they stay within it: 64
+// rows of 151936, 9 a row 20.5 us, 10 25.8.  (600 rows of 32000: 2 a row 40.2, 1 46.9.)
 static int ctas_for(int B, int V) {
-  const int chunks = (V + kChunk - 1) / kChunk, ctas = std::max(1, 592 / B);
-  const int each = std::min((std::max(2, (chunks + ctas - 1) / ctas) + 1) / 2 * 2, kMaxSpan / kChunk);
+  constexpr int kWave = 4 * 148;
+  const int chunks = (V + kChunk - 1) / kChunk;
+  int ctas = std::max(1, (int)(std::sqrt(V / (20.0 * B)) + 0.5));
+  if (B <= kWave) ctas = std::min(ctas, kWave / B);
+  const int each = std::min(std::max(2, (chunks + ctas - 1) / ctas), kMaxSpan / kChunk);
   return (chunks + each - 1) / each;
 }
 
