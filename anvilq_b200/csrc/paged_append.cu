@@ -30,7 +30,8 @@
 // times the instructions and was bound by them).  A
 // block that is coded needs its largest value first, so a warp takes all of a
 // head's rows, keeps them as they came (binary16) and rotates them twice, which
-// costs fewer registers than it saves time to keep them rotated.
+// costs fewer registers than it saves time to keep them rotated; of a decode step's
+// items, a row or two, it takes several heads at once.
 #include <algorithm>
 #include <cmath>
 
@@ -154,7 +155,8 @@ __device__ __forceinline__ void rotate8(float* a, float* b, const float* co, con
   }
 }
 
-template <int D, int TYPE>
+// FEW: with a path for items of a row or two (run has the rule)
+template <int D, int TYPE, bool FEW>
 __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
     append_kernel(const __grid_constant__ Params p, const __grid_constant__ Freq freq) {
   constexpr int kHalf = D / 2;
@@ -238,6 +240,87 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
   constexpr int kRows = 32 / kLanes;          // rows of a pass of a warp
   constexpr int kPasses = kBlock / kRows;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r0 = lane / kLanes, d0 = 8 * (lane % kLanes);
+  const int kept = it.pos % kBlock;           // rows of the block that were there before
+  auto finite = [](float v) { return fabsf(v) <= 3.4028234664e38f ? v : 0.0f; };
+  // the block's earlier codes in the lane's dims, rows first, first + step ..., times ratio
+  auto recode = [&](uint8_t* rows, int first, int step, float ratio) {
+#pragma unroll 1
+    for (int r = first; r < kept; r += step) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint2* at = reinterpret_cast<uint2*>(rows + r * D + d0 + h * kHalf);
+        uint2 w = *at;
+        float v[8];
+        q8::codes_to_float4<kCode>(w.x, v);
+        q8::codes_to_float4<kCode>(w.y, v + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= ratio;
+        *at = make_uint2(q8::float4_to_codes<kCode>(v), q8::float4_to_codes<kCode>(v + 4));
+      }
+    }
+  };
+  if (FEW && 2 * it.count <= kRows) {
+    // A new token or two, as in a decode step: the lanes that share a pass's rows below
+    // share heads here.
+    const int row = r0 & ((1 << log_rows) - 1), heads_per_warp = kRows >> log_rows;
+#pragma unroll 1
+    for (int h0 = max(head0, p.Hq) + warp * heads_per_warp; h0 < head1; h0 += kWarps * heads_per_warp) {
+      const int head = h0 + (r0 >> log_rows);
+      const bool live = head < head1, mine = live && row < it.count, is_k = head < p.Hq + p.Hkv;
+      const size_t run = (size_t)page * p.Hkv + head - p.Hq - (is_k ? 0 : p.Hkv);
+      float* scale_at = (is_k ? p.k_scales : p.v_scales) + run * (p.page_tokens / kBlock) + slot / kBlock;
+      uint8_t* rows = static_cast<uint8_t*>(is_k ? p.k : p.v) + (run * p.page_tokens + (slot - kept)) * D;
+      uint4 a = make_uint4(0, 0, 0, 0), b = a;
+      float s_kept = 0.0f;
+      if (mine) {
+        const __half* src = p.qkv + (size_t)(it.row + row) * p.stride + head * D + d0;
+        a = *reinterpret_cast<const uint4*>(src);
+        b = *reinterpret_cast<const uint4*>(src + kHalf);
+      }
+      if (live && kept) s_kept = *scale_at;
+      float x[16];
+      unpack8(a, x);
+      unpack8(b, x + 8);
+      if (is_k && mine) {
+        float co[8], si[8];
+        load8(s_cos[row] + d0, co);
+        load8(s_sin[row] + d0, si);
+        rotate8(x, x + 8, co, si);
+      }
+      float top = 0.0f, probe = 0.0f;   // probe: NaN after a value that is not finite
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        top = fmaxf(top, fabsf(x[e]));
+        probe = fmaf(x[e], 0.0f, probe);
+      }
+      if (__any_sync(0xffffffffu, probe != 0.0f)) {   // stored as 0, and reported
+        if (lane == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
+        top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          x[e] = finite(x[e]);
+          top = fmaxf(top, fabsf(x[e]));
+        }
+      }
+#pragma unroll
+      for (int o = kRows * kLanes / 4; o > 0; o >>= 1)
+        if (o < kLanes << log_rows) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (live) {
+        const float s = fmaxf(s_kept, q8::scale_for<kCode>(top));
+        const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+        if (kept && s > s_kept) recode(rows, row, 1 << log_rows, __fdiv_rn(s_kept, s));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] *= inv;
+        if (mine)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<uint2*>(rows + (kept + row) * D + d0 + h * kHalf) =
+                make_uint2(q8::float4_to_codes<kCode>(x + 8 * h), q8::float4_to_codes<kCode>(x + 8 * h + 4));
+        if (row == 0 && d0 == 0) *scale_at = s;
+      }
+    }
+    return;
+  }
 #pragma unroll 1
   for (int head = max(head0, p.Hq) + warp; head < head1; head += kWarps) {
     const bool is_k = head < p.Hq + p.Hkv;
@@ -262,7 +345,6 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
         rotate8(x, x + 8, co, si);
       }
     };
-    auto finite = [](float v) { return fabsf(v) <= 3.4028234664e38f ? v : 0.0f; };
     float top = 0.0f, probe = 0.0f;   // probe: NaN after a value that is not finite
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
@@ -290,30 +372,13 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int kept = it.pos % kBlock;         // rows of the block that were there before
     const size_t run = (size_t)page * p.Hkv + kvh;
     float* scale_at = (is_k ? p.k_scales : p.v_scales) + run * (p.page_tokens / kBlock) + slot / kBlock;
     uint8_t* rows = static_cast<uint8_t*>(is_k ? p.k : p.v) + (run * p.page_tokens + (slot - kept)) * D;
     const float s_kept = kept ? *scale_at : 0.0f;
     const float s = fmaxf(s_kept, q8::scale_for<kCode>(top));
     const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
-    if (kept && s > s_kept) {
-      const float ratio = __fdiv_rn(s_kept, s);
-#pragma unroll 1
-      for (int r = r0; r < kept; r += kRows) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint2* at = reinterpret_cast<uint2*>(rows + r * D + d0 + h * kHalf);
-          uint2 w = *at;
-          float v[8];
-          q8::codes_to_float4<kCode>(w.x, v);
-          q8::codes_to_float4<kCode>(w.y, v + 4);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= ratio;
-          *at = make_uint2(q8::float4_to_codes<kCode>(v), q8::float4_to_codes<kCode>(v + 4));
-        }
-      }
-    }
+    if (kept && s > s_kept) recode(rows, r0, kRows, __fdiv_rn(s_kept, s));
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int r = i * kRows + r0;
@@ -460,11 +525,18 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   }
   const dim3 grid(items, (heads + p.heads_per_cta - 1) / p.heads_per_cta);
   auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, st, flags, p, Freq(freq)); };
+  // Up to two tokens a sequence on average: the kernel that gives a warp several heads
+  // of an item of few rows.  32/32 heads of 128: 1024 sequences of one token 16.4 us
+  // against 50.3, of two 30.2 against 58.  It takes 10 % longer where items are full (4096
+  // tokens of one sequence 44.2 against 38.6), though those items go the same way in both.
+  const bool few = T <= 2LL * B;
+  if (type == kBinary16)
+    return D == 64 ? go(append_kernel<64, kBinary16, false>) : go(append_kernel<128, kBinary16, false>);
   if (D == 64)
-    return type == kBinary16 ? go(append_kernel<64, kBinary16>)
-           : type == q8::kInt8 ? go(append_kernel<64, q8::kInt8>) : go(append_kernel<64, q8::kE4m3>);
-  return type == kBinary16 ? go(append_kernel<128, kBinary16>)
-         : type == q8::kInt8 ? go(append_kernel<128, q8::kInt8>) : go(append_kernel<128, q8::kE4m3>);
+    return type == q8::kInt8 ? (few ? go(append_kernel<64, q8::kInt8, true>) : go(append_kernel<64, q8::kInt8, false>))
+                             : (few ? go(append_kernel<64, q8::kE4m3, true>) : go(append_kernel<64, q8::kE4m3, false>));
+  return type == q8::kInt8 ? (few ? go(append_kernel<128, q8::kInt8, true>) : go(append_kernel<128, q8::kInt8, false>))
+                           : (few ? go(append_kernel<128, q8::kE4m3, true>) : go(append_kernel<128, q8::kE4m3, false>));
 }
 
 }  // namespace append

@@ -79,6 +79,8 @@ APPENDS = [
     ([0] * 70, [1] * 70, 4, 2, 128, 16),                      # more than 32 sequences
     ([i % 23 for i in range(40)], [i % 5 for i in range(40)], 2, 1, 64, 16),   # many empty ones
     ([i % 40 for i in range(150)], [1 + i % 9 for i in range(150)], 32, 8, 128, 16),   # heads in slices
+    ([(7 * i) % 50 for i in range(24)], [1 + i % 3 for i in range(24)], 9, 3, 128, 32),    # a token or two, odd heads
+    ([3] * 9, [2, 1, 4, 0, 1, 3, 2, 1, 2], 7, 7, 64, 16),                                  # the same over block edges
 ]
 
 
@@ -304,6 +306,31 @@ def test_append_q8_not_finite(dev):
     assert v[pg, 0, 1, 5] == 0 and v[pg, 0, 2, 6] == 0
     x = qkv[:, (Hq + Hkv) * D:].astype(np.float32)
     assert vs[pg, 0, 0].item() == np.abs(x[np.isfinite(x)]).max() / np.float32(127)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_append_q8_step_not_finite(dev, fp8):
+    """Of a decode step's tokens only the values that are not finite are lost."""
+    rng = np.random.default_rng(22)
+    B, Hq, Hkv, D, page = 4, 3, 3, 128, 16
+    qkv, table, starts, lens, pages = append_case(rng, [0, 3, 15, 16], [1] * B, Hq, Hkv, D, page, spare_rows=0)
+    clean = qkv.copy()
+    at = (Hq + Hkv) * D + 130                                 # head 1 of V, dim 2
+    for b, bad in ((1, np.inf), (2, np.nan), (3, -np.inf)):
+        qkv[b, at] = bad
+        clean[b, at] = 0
+    ends = []
+    for x in (qkv, clean):
+        k = torch.zeros((pages, Hkv, page, D), device=dev).to(code_dtype(fp8))
+        v, ks, vs = k.clone(), *(torch.zeros((pages, Hkv, 1), device=dev) for _ in range(2))
+        q = ops.paged_kv_append_q8(to(x, dev), k, v, ks, vs, to(table, dev), to(lens, dev), to(starts, dev), Hq)
+        if x is qkv:
+            with pytest.raises(AnvilqError):
+                ops.raise_device_errors(dev)
+        ends.append([q, k.view(torch.uint8), v.view(torch.uint8), ks, vs])
+    ops.raise_device_errors(dev)
+    for a, b in zip(*ends):
+        assert torch.equal(a, b)
 
 
 # ---- attention ----------------------------------------------------------------
