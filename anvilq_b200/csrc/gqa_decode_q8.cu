@@ -415,11 +415,13 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
       }
     }
 
-    // ---- block by block (unrolled: 1 % on a long batch, 2 % on drafts) ----
-    const unsigned char* kt = ring + st * S::kStageBytes;
-#pragma unroll 2
-    for (int h = 0; h < 2; ++h, kt += kBlock * D) {
-      const unsigned char* vt = kt + S::kTileBytes;
+    const unsigned char* tile = ring + st * S::kStageBytes;
+    float x[2][RT][4];   // scores of both blocks: tokens token_of(g), then + 8; two rows each
+    bool edge[2];
+    int len = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned char* kt = tile + h * kBlock * D;
       const int t0 = md.tile * kTile + h * kBlock;
       // ---- S^T = K Q^T: tokens token_of(g) and + 8, rows 8 t + 2 c and + 1 ----
       float s[2][RT][4];   // two sums: an accumulator's next MMA waits for its last
@@ -462,17 +464,14 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
             mma16816(s[e & 1][t], a[0][0], a[1][0], a[0][1], a[1][1], qb[4 * q + e][t][0], qb[4 * q + e][t][1]);
         }
 
-      // ---- softmax ----
-      const float ks = slot.ks[h] * scale, vs = slot.vs[h];
-      float x[RT][4];   // tokens token_of(g), then + 8; two rows each
+      const float ks = slot.ks[h] * scale;
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[t][e] = (s[0][t][e] + s[1][t][e]) * ks;
+        for (int e = 0; e < 4; ++e) x[h][t][e] = (s[0][t][e] + s[1][t][e]) * ks;
       // some row may not see all of the block: length >= 32 (n - 1) + 1, row 0 sees Q - 1 less
-      const bool edge = t0 + kBlock > kTile * (md.n - 1) + 2 - Q;
-      int len = 0;
-      if (edge) {
+      edge[h] = t0 + kBlock > kTile * (md.n - 1) + 2 - Q;
+      if (edge[h]) {
         len = seqlens[slot.b];
         const int r0 = (slot.pair - p.row_groups.quotient(slot.pair) * p.row_groups.d) * S::kRows;
 #pragma unroll
@@ -480,16 +479,19 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int sees = len - Q + 1 + p.group.quotient(r0 + 8 * t + 2 * c + (e & 1)) - t0;
-            if (token_of(g) + 8 * (e >> 1) >= sees) x[t][e] = -INFINITY;
+            if (token_of(g) + 8 * (e >> 1) >= sees) x[h][t][e] = -INFINITY;
           }
       }
+    }
+    // ---- softmax: the reference for both blocks ----
+    {
       float mx[RT][2];
       bool above = false;
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          mx[t][e] = fmaxf(x[t][e], x[t][2 + e]);
+          mx[t][e] = fmaxf(fmaxf(x[0][t][e], x[0][t][2 + e]), fmaxf(x[1][t][e], x[1][t][2 + e]));
           above |= mx[t][e] > m[t][e] + 12.0f;
         }
       if (__any_sync(0xffffffffu, above)) {
@@ -510,6 +512,12 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
             }
           }
       }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned char* vt = tile + S::kTileBytes + h * kBlock * D;
+      const int t0 = md.tile * kTile + h * kBlock;
+      const float vs = slot.vs[h];
       float rel = vs * F_inv;
       if ((rel > 8.0f || rel < 0.125f) && vs > 0.0f) {
         // values of scales below 2^-40 round to nothing in the binary16 result
@@ -528,11 +536,11 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[t][e] = fast_exp2(x[t][e] - m[t][e & 1]);
-        l[t][0] += x[t][0] + x[t][2];
-        l[t][1] += x[t][1] + x[t][3];
-        pb[t][0] = transpose8x8(pack_half2(x[t][0] * rel, x[t][1] * rel));
-        pb[t][1] = transpose8x8(pack_half2(x[t][2] * rel, x[t][3] * rel));
+        for (int e = 0; e < 4; ++e) x[h][t][e] = fast_exp2(x[h][t][e] - m[t][e & 1]);
+        l[t][0] += x[h][t][0] + x[h][t][2];
+        l[t][1] += x[h][t][1] + x[h][t][3];
+        pb[t][0] = transpose8x8(pack_half2(x[h][t][0] * rel, x[h][t][1] * rel));
+        pb[t][1] = transpose8x8(pack_half2(x[h][t][2] * rel, x[h][t][3] * rel));
       }
 
       // ---- O^T += V^T P^T ----
@@ -549,7 +557,7 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
           v[e][0] = k.x; v[e][1] = k.y;
         }
         // rows behind the sequence may hold anything: an e4m3 NaN times p = 0 would be a NaN
-        if (TYPE == q8::kE4m3 && edge && t0 + row >= len) {
+        if (TYPE == q8::kE4m3 && edge[h] && t0 + row >= len) {
 #pragma unroll
           for (int w = 0; w < VW; ++w) v[e][w] = 0u;
         }
