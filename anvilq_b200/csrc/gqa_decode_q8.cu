@@ -87,6 +87,7 @@ struct Params {
   int B, Q, Hq, Hkv, page_tokens, max_pages, num_pages;
   Divisor group, row_groups;   // query heads a kv head; row groups a (sequence, kv head)
   int wide;                    // pages hold whole tiles: one copy of 32 rows, not two of 16
+  unsigned expire;             // ANVILQ_EXPIRE_WAITS: bits of the waits that give up at once
   float scale_log2;            // softmax scale * log2(e)
 };
 
@@ -391,7 +392,8 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
     const struct { int tile, n; } md = {slot.tile, slot.n};
     const bool fresh = j == 0 || md.tile == 0;
     if (fresh && j > 0) begin_pair(slot);
-    if (!warp_wait(bar0 + 8 * st, j / S::kStages & 1)) {   // no tile is used after this
+    if ((p.expire && (p.expire >> ((blockIdx.x + warp + j) & 15) & 1u)) ||
+        !warp_wait(bar0 + 8 * st, j / S::kStages & 1)) {   // no tile is used after this
       ok = false;
       if (lane == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_TIMEOUT);
       break;
@@ -669,9 +671,35 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
     }
   }
   if (!ok) {
-    // copies in flight land before the shared memory is used for anything else
-    for (; j < issued; ++j)
-      if (!warp_wait(bar0 + 8 * (j & (S::kStages - 1)), j / S::kStages & 1)) break;
+    // Copies in flight land before the shared memory is used for anything else.
+    for (int i = j; i < issued; ++i)
+      if (!warp_wait(bar0 + 8 * (i & (S::kStages - 1)), i / S::kStages & 1)) break;
+    // The output is lost, but not the accounts: empty states stand for what is left of
+    // the stretch, so that every pair has all of its members, every ticket all of its
+    // arrivals, and the workspace's counters are zero after this call as after any other.
+    copies_done();
+    __syncwarp();
+    const Meta at = meta[j & (S::kSlots - 1)];
+    __syncwarp();
+    name_tiles(count - 1, at.b, begin + j - (unsigned)at.pair * at.n - at.tile);
+    copies_done();
+    __syncwarp();
+    const Meta end = meta[(count - 1) & (S::kSlots - 1)];
+    float4* state = reinterpret_cast<float4*>(ring);
+    for (int i = lane; i < S::kState / 4; i += 32) state[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto leave_empty = [&](int which, const Meta& md, int k) {   // of the pair of tile k
+      float2* stat = reinterpret_cast<float2*>(smem + S::kStatOffset) + (warp * 2 + which) * S::kRows;
+      if (lane < S::kRows) stat[lane] = make_float2(-1e30f, 0.0f);
+      if (lane == 0) ctl.part[warp][which] = Part{begin + k - md.tile, md.n, md.b, md.pair};
+    };
+    if (at.tile > j) {                                    // begun earlier
+      leave_empty(0, at, j);
+      flags |= kHas0 | (at.n - at.tile <= count - j ? kEnds0 : 0);
+    }
+    if (end.tile < count && end.tile < end.n - 1) {       // begun here, goes on
+      leave_empty(1, end, count - 1);
+      flags |= kHas1;
+    }
   }
   if (lane == 0) ctl.flags[warp] = flags;
 }
@@ -1091,7 +1119,7 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   if (!q || !k_codes || !v_codes || !k_scales || !v_scales || !page_table || !seqlens || !out || !dev_err)
     return ANVILQ_EINVAL;
   if (code_type != ANVILQ_KV_Q8_INT8 && code_type != ANVILQ_KV_Q8_E4M3) return ANVILQ_EINVAL;
-  if ((flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) || !(scale < INFINITY)) return ANVILQ_EINVAL;
+  if ((flags & ~(ANVILQ_GEMM_OVERLAP_PRIOR | ANVILQ_EXPIRE_WAITS(0xFFFF))) || !(scale < INFINITY)) return ANVILQ_EINVAL;
   if (!shape_ok(B, Q, Hq, Hkv, D) || page_tokens < kBlock || page_tokens % kBlock || max_pages < 1 || num_pages < 1 ||
       (long long)page_tokens * max_pages > (1LL << 30))
     return ANVILQ_ESHAPE;
@@ -1123,6 +1151,7 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   p.group = divisor(Hq / Hkv);
   p.row_groups = divisor(row_groups);
   p.page_tokens = page_tokens; p.max_pages = max_pages; p.num_pages = num_pages;
+  p.expire = flags >> 16;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
   // as many CTAs as the device holds, but no more than there can be work for: a pair
   // each, or a tile a warp

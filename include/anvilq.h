@@ -702,7 +702,13 @@ int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k
  * ANVILQ_DEV_ERR_SEQLEN and counts as 0; an absent live page sets
  * ANVILQ_DEV_ERR_PAGE (the output is then not to be used).  workspace: at least
  * anvilq_gqa_decode_q8_workspace_size(...) bytes (0: shape not supported),
- * layout as described at ANVILQ_WORKSPACE_COUNTER_BYTES. */
+ * layout as described at ANVILQ_WORKSPACE_COUNTER_BYTES.
+ * The waits for a tile's copies are bounded by ~1 s each; one that expires sets
+ * ANVILQ_DEV_ERR_TIMEOUT, and the output is not to be used (the counters are zero
+ * all the same).  With ANVILQ_EXPIRE_WAITS(mask) among the flags some of them expire
+ * at once, those whose bit (CTA + warp + tile) % 16 of the mask is set: for trying out
+ * how a program takes that error. */
+#define ANVILQ_EXPIRE_WAITS(mask) ((unsigned)(mask) << 16)   /* mask: 16 bits */
 size_t anvilq_gqa_decode_q8_workspace_size(int B, int Q, int Hq, int Hkv, int D);
 int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_codes, const float* k_scales,
                          const float* v_scales, int code_type, const uint32_t* page_table, const int32_t* seqlens,

@@ -1012,3 +1012,41 @@ def test_logits_most_rows(dev):
     want = np.where(allowed, x, -np.inf)
     assert np.array_equal(out.cpu().numpy(), want)
     assert np.array_equal(tokens.cpu().numpy(), np.where(allowed.any(axis=1), want.argmax(axis=1), -1))
+
+
+# ---- waits that expire ------------------------------------------------------------
+
+@pytest.mark.parametrize("lens,Q,Hq,Hkv,D,fp8", [
+    ([5000, 0, 40, 3000], 1, 8, 2, 128, False),      # pairs over several CTAs, one inside a warp's stretch
+    ([700, 650, 720], 4, 8, 2, 128, True),           # 16 rows a pair
+    ([30000], 1, 14, 2, 64, False),                  # two pairs over the whole device
+    ([300], 1, 14, 2, 64, True),                     # a CTA a pair
+    ([1 + 7 * i % 90 for i in range(300)], 1, 8, 8, 64, False),   # many pairs a warp
+])
+def test_attention_q8_after_expired_waits(dev, lens, Q, Hq, Hkv, D, fp8):
+    """Waits that give up, all of them or some warps': the error is reported once, the
+    workspace's counters are zero behind the call, and the next call on it is right."""
+    rng = np.random.default_rng(len(lens) + D)
+    q, k, v, ks, vs, table = attention_case(dev, rng, lens, Q, Hq, Hkv, D, 16, fp8)
+    a = [to(q, dev)] + [t.to(dev) for t in (k, v, ks, vs)] + [to(table, dev), to(np.array(lens, np.int32), dev)]
+    lib = _lib.load()
+    ws = torch.zeros(lib.anvilq_gqa_decode_q8_workspace_size(len(lens), Q, Hq, Hkv, D), dtype=torch.uint8, device=dev)
+    ref = ops.gqa_decode_q8(*a, workspace=ws)
+    ops.raise_device_errors(dev)
+    check_attention(ref.cpu().numpy(), q, k, v, ks, vs, table, lens)
+    out, word = torch.empty_like(ref), ops.device_error_word(dev)
+    for mask in (0xFFFF, 0x0001, 0x8421, 0x5555, 0x00F0, 0x0003):
+        flags = mask << 16                           # ANVILQ_EXPIRE_WAITS; CTA 0's first wait is bit 0's
+        ptr = lambda t: t.data_ptr()
+        assert lib.anvilq_gqa_decode_q8(*map(ptr, a[:5]), int(fp8), ptr(a[5]), ptr(a[6]), ptr(out), len(lens), Q, Hq,
+                                        Hkv, D, 16, table.shape[1], k.shape[0], 0.0, ptr(ws), ws.numel(), ptr(word),
+                                        flags, torch.cuda.current_stream(dev).cuda_stream) == 0
+        if mask & 1:
+            with pytest.raises(AnvilqError, match="wait"):
+                ops.raise_device_errors(dev)
+        else:
+            torch.cuda.synchronize(dev)
+            word.zero_()
+        assert not ws[:65536].any(), hex(mask)
+        assert torch.equal(ops.gqa_decode_q8(*a, workspace=ws), ref), hex(mask)
+    ops.raise_device_errors(dev)
