@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
 #pragma unroll
       for (int o = kRows * kLanes / 4; o > 0; o >>= 1)
         if (o < kLanes << log_rows) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      __syncwarp();   // every lane has read its head's scale, which one of them replaces
       if (live) {
         const float s = fmaxf(s_kept, q8::scale_for<kCode>(top));
         const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
@@ -396,6 +397,7 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
           *reinterpret_cast<uint2*>(rows + (kept + r) * D + d0 + h * kHalf) =
               make_uint2(q8::float4_to_codes<kCode>(x + 8 * h), q8::float4_to_codes<kCode>(x + 8 * h + 4));
     }
+    __syncwarp();   // every lane has read the scale
     if (lane == 0) *scale_at = s;
   }
 }

@@ -1050,3 +1050,54 @@ def test_attention_q8_after_expired_waits(dev, lens, Q, Hq, Hkv, D, fp8):
         assert not ws[:65536].any(), hex(mask)
         assert torch.equal(ops.gqa_decode_q8(*a, workspace=ws), ref), hex(mask)
     ops.raise_device_errors(dev)
+
+
+# ---- blocks whose scale grows, sequences that are cut back, other rotations -----------
+
+def step_codes(x, kept, codes, scale, dtype):
+    """A block of one head after new rows x [n, D] behind `kept` ones, each operation in
+    binary32: (codes [kept + n, D], scale)."""
+    top = x.abs().max()
+    if dtype == torch.int8:
+        want, round_ = top / 127, lambda y: y.round().clamp(-127, 127).to(dtype)
+    else:
+        want = (2.0 ** torch.ceil(torch.log2(top.double() / 448))).float() if top > 0 else top
+        round_ = lambda y: y.clamp(-448, 448).to(dtype)
+    s = torch.maximum(scale, want) if kept else want
+    old = codes[:kept]
+    if kept and s > scale:
+        old = round_(old.float() * (scale / s))
+    new = round_(x * (1 / s)) if s > 0 else torch.zeros(x.shape).to(dtype)
+    return torch.cat([old.float(), new.float()]).to(dtype), s
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_append_q8_growing_blocks_bit_for_bit(dev, D, fp8):
+    """Blocks with 1 to 15 rows whose scale an appended run of 1 to 15 rows raises, by all
+    lanes alike: kept rows, new rows and scales of V are the formulas' in binary32."""
+    rng = np.random.default_rng(41)
+    Hq, Hkv, page, dtype = 3, 3, 16, code_dtype(fp8)
+    runs = [(kept, n) for kept in range(1, 16) for n in range(1, 17 - kept)]
+    B = len(runs)
+    table = to(so.make_table([1] * B, B, rng), dev)
+    for group in (runs, [r for r in runs if r[1] <= 2]):        # chunks; a token or two a sequence
+        kept, new = [k for k, _ in group], [n for _, n in group]
+        n_seq = len(group)
+        codes = random_codes(rng, (B, Hkv, page, D), fp8)
+        scales = random_scales(rng, (B, Hkv, 1), fp8)
+        k, v, ks, vs = codes.to(dev), codes.to(dev), scales.to(dev), scales.to(dev)
+        starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        size = 8.0 ** rng.integers(-1, 3, size=(starts[-1], 1))
+        qkv = (rng.standard_normal((starts[-1], (Hq + 2 * Hkv) * D)) * size).astype(np.float16)
+        lens = np.array([a + b for a, b in group], np.int32)
+        ops.paged_kv_append_q8(to(qkv, dev), k, v, ks, vs, table[:n_seq].contiguous(), to(lens, dev), to(starts, dev), Hq)
+        ops.raise_device_errors(dev)
+        x = torch.from_numpy(qkv.astype(np.float32)).view(-1, Hq + 2 * Hkv, D)[:, Hq + Hkv:]
+        got, got_s, t = v.cpu(), vs.cpu(), table.cpu().numpy()
+        for b in range(n_seq):
+            pg = so.physical(t[b, 0])
+            for h in range(Hkv):
+                want, s = step_codes(x[starts[b]:starts[b + 1], h], kept[b], codes[pg, h], scales[pg, h, 0], dtype)
+                assert got_s[pg, h, 0] == s, (b, h)
+                assert torch.equal(got[pg, h, :lens[b]].float(), want.float()), (group[b], h)
