@@ -279,6 +279,7 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
   const int pairs = p.Hkv * p.row_groups.d, Q = p.Q;
   const bool wide = p.wide;
   const int* seqlens = p.seqlens;
+  const unsigned* group_tiles = reinterpret_cast<const unsigned*>(smem + S::kGroupOffset);   // of B > 32 sequences
   // the scores' scale in the log2 domain (int8: codes enter S as c 2^-24)
   const float scale = p.scale_log2 * (TYPE == q8::kInt8 ? 0x1p24f : 1.0f);
   bool ok = true;
@@ -292,7 +293,11 @@ __device__ __forceinline__ void run_stretch(const CUtensorMap& mk, const CUtenso
     int n = tiles_of(p, b);
     while (x - base >= (unsigned)n * pairs && b + 1 < p.B) {
       base += (unsigned)n * pairs;
-      n = tiles_of(p, ++b);
+      // whole groups at a time where idle slots leave many without a tile (two sequences of
+      // 8000 tokens, 4094 slots between them: 38 us; stepping over each slot 284)
+      for (++b; b % 32 == 0 && b + 32 < p.B && x - base >= group_tiles[b / 32] * pairs; b += 32)
+        base += group_tiles[b / 32] * pairs;
+      n = tiles_of(p, b);
     }
     // the bounds below hold by themselves unless the lengths change under the kernel
     n = max(n, 1);

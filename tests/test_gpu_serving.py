@@ -1101,3 +1101,54 @@ def test_append_q8_growing_blocks_bit_for_bit(dev, D, fp8):
                 want, s = step_codes(x[starts[b]:starts[b + 1], h], kept[b], codes[pg, h], scales[pg, h, 0], dtype)
                 assert got_s[pg, h, 0] == s, (b, h)
                 assert torch.equal(got[pg, h, :lens[b]].float(), want.float()), (group[b], h)
+
+
+# ---- idle slots ---------------------------------------------------------------------
+
+def idle_slots_case(dev, rng, B, live, tokens, Hq=8, Hkv=2, D=64, page=64):
+    """B slots of which those of `live` hold `tokens` tokens, the others none."""
+    lens = np.zeros(B, np.int32)
+    lens[list(live)] = tokens
+    q, k, v, ks, vs, table = attention_case(dev, rng, [int(n) for n in lens], 1, Hq, Hkv, D, page, False)
+    a = [to(q, dev)] + [t.to(dev) for t in (k, v, ks, vs)] + [to(table, dev), to(lens, dev)]
+    return a, (q, k, v, ks, vs, table, lens)
+
+
+@pytest.mark.parametrize("B,live", [
+    (33, (0, 32)), (64, (31, 32)), (200, (0, 63, 64, 199)), (1024, (31, 1023)), (1025, (0, 992, 1024)),
+    (3000, (5, 6, 1500, 2999)), (5000, (4999,)), (20000, (0, 31, 32, 10016, 19999)),
+])
+def test_attention_q8_live_slots_far_apart(dev, B, live):
+    rng = np.random.default_rng(B)
+    a, (q, k, v, ks, vs, table, lens) = idle_slots_case(dev, rng, B, live, 1500)
+    out = ops.gqa_decode_q8(*a, out=torch.full_like(a[0].squeeze(1), float("nan")).unsqueeze(1))
+    ops.raise_device_errors(dev)
+    got = out.cpu().numpy()
+    idle = np.ones(B, bool)
+    idle[list(live)] = False
+    assert not got[idle].any()
+    pick = list(live)
+    check_attention(got[pick], q[pick], k, v, ks, vs, table[pick], [int(n) for n in lens[pick]])
+
+
+def test_attention_q8_idle_slots_cost_no_walk(dev):
+    """Two sequences in the first and the last of 8192 slots take about as long as in the
+    first two: no warp steps over the idle slots between them one by one (which took ten
+    times as long)."""
+    rng = np.random.default_rng(0)
+    times = []
+    for live in ((0, 1), (0, 8191)):
+        a, _ = idle_slots_case(dev, rng, 8192, live, 8000)
+        out = torch.empty_like(a[0])
+        runs = []
+        for i in range(12):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            for _ in range(10):
+                ops.gqa_decode_q8(*a, out=out)
+            end.record()
+            end.synchronize()
+            runs.append(begin.elapsed_time(end))
+        times.append(min(runs[2:]))
+    ops.raise_device_errors(dev)
+    assert times[1] < 3 * times[0], times
