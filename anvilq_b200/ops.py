@@ -84,6 +84,8 @@ def workspace(device, nbytes: int) -> torch.Tensor:
         ws = _workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
             if ws is not None:
+                # at least twice as large, so that all the outgrown ones are smaller than it
+                nbytes = max(nbytes, 2 * ws.numel())
                 _outgrown.append(ws)
             ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
             _workspaces[key] = ws
