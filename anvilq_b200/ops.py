@@ -17,7 +17,8 @@ from . import _lib
 _state = threading.local()
 _dev_err = {}          # device index -> int32[1] device error word
 _workspaces = {}       # (device index, stream ptr) -> uint8 workspace
-_outgrown = []         # workspaces that larger ones replaced: captured graphs may still use them
+_of_graphs = set()     # keys of workspaces made while a graph was captured: only its replays zero them
+_outgrown = []         # workspaces that others replaced: captured graphs may still use them
 _lock = threading.Lock()
 
 
@@ -76,19 +77,39 @@ def raise_device_errors(device=None):
         raise _lib.AnvilqError(f"device error bits 0x{value:x}: " + "; ".join(what))
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+def _capturing(device):
+    """Whether `device`'s current stream is being captured."""
+    if device.type != "cuda":
+        return False
+    if _current_device() == device.index:
+        return _current_capturing()
+    with torch.cuda.device(device):
+        return _current_capturing()
+
+
 def workspace(device, nbytes: int) -> torch.Tensor:
-    """Zero-filled scratch reused by calls on the current stream (kernels leave it zeroed)."""
-    idx = torch.device(device).index
-    key = (idx, _stream_ptr(device))
+    """Zero-filled scratch reused by calls on the current stream (kernels leave it zeroed).
+    One made while a graph was captured lies in the graph's memory and is zero only in its
+    replays: the stream's next eager call replaces it."""
+    device = torch.device(device)
+    key = (device.index, _stream_ptr(device))
     with _lock:
         ws = _workspaces.get(key)
-        if ws is None or ws.numel() < nbytes:
+        if ws is None or ws.numel() < nbytes or (key in _of_graphs and not _capturing(device)):
             if ws is not None:
                 # at least twice as large, so that all the outgrown ones are smaller than it
                 nbytes = max(nbytes, 2 * ws.numel())
                 _outgrown.append(ws)
             ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
             _workspaces[key] = ws
+            if _capturing(device):
+                _of_graphs.add(key)
+            else:
+                _of_graphs.discard(key)
     return ws
 
 
@@ -606,18 +627,6 @@ def _on_device(name, device, *tensors):
             raise ValueError(f"{name}: all tensors must be on {device}")
 
 
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_current_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
-
-
-def _capturing(device):
-    """Whether `device`'s current stream is being captured."""
-    if _current_device() == device.index:
-        return _current_capturing()
-    with torch.cuda.device(device):
-        return _current_capturing()
-
-
 def _call(name, device, *args):
     """A library call with `device` current (a stream only takes launches of its own device)."""
     fn = getattr(_lib.load(), name)
@@ -643,8 +652,9 @@ def _call_workspace(device, nbytes: int, given) -> torch.Tensor:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         ws[:WORKSPACE_COUNTER_BYTES].zero_()
         return ws
-    ws = _workspaces.get((device.index, _stream_ptr(device)))
-    return ws if ws is not None and ws.numel() >= nbytes else workspace(device, nbytes)
+    key = (device.index, _stream_ptr(device))
+    ws = _workspaces.get(key)
+    return ws if ws is not None and ws.numel() >= nbytes and key not in _of_graphs else workspace(device, nbytes)
 
 
 WORKSPACE_COUNTER_BYTES = 65536

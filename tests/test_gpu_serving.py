@@ -1152,3 +1152,35 @@ def test_attention_q8_idle_slots_cost_no_walk(dev):
         times.append(min(runs[2:]))
     ops.raise_device_errors(dev)
     assert times[1] < 3 * times[0], times
+
+
+# ---- workspaces -----------------------------------------------------------------------
+
+def test_eager_calls_behind_a_capture_have_their_own_workspace(dev):
+    """A stream whose first call was captured: its workspace is the graph's, zero only in
+    replays, and eager serving calls there do not use it."""
+    rng = np.random.default_rng(61)
+    q, k, v, ks, vs, table = attention_case(dev, rng, [3000, 700], 1, 8, 2, 128, 16, False)
+    a = [to(q, dev)] + [t.to(dev) for t in (k, v, ks, vs)] + [to(table, dev), to(np.array([3000, 700], np.int32), dev)]
+    ref = ops.gqa_decode_q8(*a)
+    kc = torch.randn((2, 900, 2, 128), device=dev).half()
+    vc, q16 = torch.randn_like(kc), torch.randn((2, 8, 128), device=dev).half()
+    lens = torch.tensor([900, 33], dtype=torch.int32, device=dev)
+    old = ops.gqa_decode(q16, kc, vc, lens)
+    torch.cuda.synchronize(dev)
+    s = torch.cuda.Stream(dev)
+    key = (dev.index, s.cuda_stream)
+    earlier = ops._workspaces.pop(key, None)         # streams come from a pool
+    ops._of_graphs.discard(key)
+    g, out = torch.cuda.CUDAGraph(), torch.empty_like(old)
+    with torch.cuda.graph(g, stream=s):
+        out.copy_(ops.gqa_decode(q16, kc, vc, lens))
+    of_graph = ops._workspaces[key]
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            assert torch.equal(ops.gqa_decode_q8(*a), ref)
+            g.replay()
+            assert torch.equal(out, old)
+    assert ops._workspaces[key] is not of_graph
+    s.synchronize()
+    ops.raise_device_errors(dev)
