@@ -1015,6 +1015,9 @@ __global__ void __launch_bounds__(Shape<D, RT>::kThreads, 1)
 // ---------------------------------------------------------------------------
 static bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// A block's scale (at most 729, of a rotated binary16 65504) times the softmax scale times
+// 2^24 log2(e) stays below binary32's largest value.
+constexpr float kMaxScale = 0x1p64f;
 constexpr int kMaxQueries = 64;   // query tokens of a sequence
 static bool shape_ok(int B, int Q, int Hq, int Hkv, int D) {
   return B >= 1 && B < kMaxBatch && Q >= 1 && Q <= kMaxQueries && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 &&
@@ -1124,7 +1127,8 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   if (!q || !k_codes || !v_codes || !k_scales || !v_scales || !page_table || !seqlens || !out || !dev_err)
     return ANVILQ_EINVAL;
   if (code_type != ANVILQ_KV_Q8_INT8 && code_type != ANVILQ_KV_Q8_E4M3) return ANVILQ_EINVAL;
-  if ((flags & ~(ANVILQ_GEMM_OVERLAP_PRIOR | ANVILQ_EXPIRE_WAITS(0xFFFF))) || !(scale < INFINITY)) return ANVILQ_EINVAL;
+  if (flags & ~(ANVILQ_GEMM_OVERLAP_PRIOR | ANVILQ_EXPIRE_WAITS(0xFFFF))) return ANVILQ_EINVAL;
+  if (!std::isfinite(scale) || scale > kMaxScale) return ANVILQ_EINVAL;
   if (!shape_ok(B, Q, Hq, Hkv, D) || page_tokens < kBlock || page_tokens % kBlock || max_pages < 1 || num_pages < 1 ||
       (long long)page_tokens * max_pages > (1LL << 30))
     return ANVILQ_ESHAPE;

@@ -803,7 +803,8 @@ def gqa_decode_q8(q, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, 
     """GQA attention over 8-bit pages (``paged_kv_append_q8``'s): q fp16 [B, Hq, D], one
     query token a sequence, or [B, Q, Hq, D], its last Q tokens (drafts to verify, a
     chunk), each seeing the positions up to its own.  seqlens int32 [B] counts all
-    tokens, the queries' included; a sequence of length 0 gives zeros.  Returns fp16
+    tokens, the queries' included; a sequence of length 0 gives zeros.  scale (finite, at
+    most 2^64): of the scores, 0 or less for 1/sqrt(D).  Returns fp16
     in q's shape.  workspace: a uint8 tensor zero-filled once, for callers that keep
     their own (default: the current stream's).
 

@@ -694,8 +694,8 @@ int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k
  * before).  q and out fp16 [B][Q][Hq][D], seqlens int32 [B] (device, 0 ..
  * page_tokens * max_pages <= 2^30).  A query that sees nothing -- an empty sequence, or
  * a position below 0 -- gives zeros.  Scores and the softmax run in fp32, the
- * probabilities enter the tensor cores as binary16.  scale (finite) <= 0 selects
- * 1/sqrt(D).  Hq % Hkv == 0, Hq <= 1024, Q <= 64, B <= 65535, at most 2^31 - 1
+ * probabilities enter the tensor cores as binary16.  scale (finite, at most
+ * 2^64) <= 0 selects 1/sqrt(D).  Hq % Hkv == 0, Hq <= 1024, Q <= 64, B <= 65535, at most 2^31 - 1
  * rows (num_pages * page_tokens * Hkv) in a pool; the tables' positions over
  * 32, times Hkv and the groups of 8 or 16 query rows of a head, at most 2^31;
  * 16-byte aligned q, codes and out; dev_err required.  A length outside its range sets

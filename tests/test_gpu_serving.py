@@ -1184,3 +1184,31 @@ def test_eager_calls_behind_a_capture_have_their_own_workspace(dev):
     assert ops._workspaces[key] is not of_graph
     s.synchronize()
     ops.raise_device_errors(dev)
+
+
+# ---- softmax scales --------------------------------------------------------------------
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_attention_q8_largest_scale(dev, fp8):
+    """Under the largest scale the softmax takes the largest score's value alone, and equal
+    ones alike; zero scores (a zero query) still weigh all values the same."""
+    rng = np.random.default_rng(71)
+    q, k, v, ks, vs, table = attention_case(dev, rng, [100], 1, 8, 2, 64, 16, fp8)
+    ks[:] = 0.5 if fp8 else 700.0
+    q[0, 0, 3] = 0
+    a = [to(q, dev)] + [t.to(dev) for t in (k, v, ks, vs)] + [to(table, dev), to(np.array([100], np.int32), dev)]
+    out = ops.gqa_decode_q8(*a, scale=2.0 ** 64).cpu().numpy().astype(np.float64)
+    ops.raise_device_errors(dev)
+    kv, vv = so.pool_values(k, ks), so.pool_values(v, vs)
+    at = [so.physical(e) for e in table[0]]
+    flat = lambda p: p[at].transpose(0, 2, 1, 3).reshape(-1, 2, 64)[:100]
+    kv, vv = flat(kv), flat(vv)
+    for h in range(8):
+        if h == 3:
+            want, tol = vv[:, 0].mean(axis=0), 2 * HALF * (1 + 2.0 ** -6) * np.abs(vv[:, 0]).mean(axis=0)
+        else:
+            x = kv[:, h // 4] @ q[0, 0, h].astype(np.float64)
+            assert np.sort(x)[-1] - np.sort(x)[-2] > 2.0 ** -18 * np.abs(kv).max() * np.abs(q[0, 0, h]).sum()
+            want = vv[x.argmax(), h // 4]
+            tol = 2 * HALF * (1 + 2.0 ** -6) * np.abs(want)
+        assert (np.abs(out[0, 0, h] - want) <= tol + 2.0 ** -24).all(), h

@@ -169,3 +169,9 @@ def test_logits_front_end(change):
     a.update(change)
     with pytest.raises(ValueError):
         ops.logits_process(**a)
+
+
+@pytest.mark.parametrize("scale", [float("-inf"), 2.0 ** 64 * (1 + 2.0 ** -23), 1e35])
+def test_attention_scale_refused(scale):
+    """Scales that are not finite, and those whose product with an int8 block's scale is not."""
+    assert _lib.load().anvilq_gqa_decode_q8(*{**ATTN, "scale": scale}.values()) == EINVAL
