@@ -85,5 +85,11 @@ __device__ __forceinline__ float scale_for(float top) {
   return __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
 }
 
+// Whether two runs of bytes share any (an empty one shares none).
+inline bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na && nb && x < y + nb && y < x + na;
+}
+
 }  // namespace q8
 }  // namespace anvilq

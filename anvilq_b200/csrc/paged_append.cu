@@ -34,6 +34,7 @@
 // items, a row or two, it takes several heads at once.
 #include <algorithm>
 #include <cmath>
+#include <iterator>
 
 #include "kv_q8.cuh"
 
@@ -41,6 +42,7 @@ namespace anvilq {
 namespace append {
 
 using q8::kBlock;
+using q8::overlap;
 constexpr int kBinary16 = -1;   // the pool's type: binary16, q8::kInt8 or q8::kE4m3
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
@@ -442,10 +444,6 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* k, const uin
   }
 }
 
-static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + nb && y < x + na;
-}
 static bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename... KArgs, typename... Args>
@@ -466,6 +464,11 @@ static int launch(void (*kernel)(KArgs...), dim3 grid, int threads, cudaStream_t
   return ANVILQ_OK;
 }
 
+struct Span {
+  const void* start;
+  size_t bytes;
+};
+
 // type: kBinary16 or an ANVILQ_KV_Q8_* code type (scales then given)
 static int run(const uint16_t* qkv, long long stride, const int32_t* starts, const int32_t* seqlens,
                const uint32_t* page_table, uint16_t* q_out, void* k, void* v, float* k_scales, float* v_scales,
@@ -482,11 +485,19 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
     return ANVILQ_ESHAPE;
   const int heads = Hq + 2 * Hkv;
   if (stride < (long long)heads * D) return ANVILQ_EINVAL;
+  const long long positions = (long long)num_pages * page_tokens;
+  if (positions > (1LL << 40) / Hkv) return ANVILQ_ESHAPE;
   if (!a16(qkv) || !a16(q_out) || !a16(k) || !a16(v) || stride % 8) return ANVILQ_EALIGN;
   if (T == 0) return ANVILQ_OK;
-  // an item's q is written while others' rows are still to be read
-  if (overlap(qkv, ((size_t)(T - 1) * stride + (size_t)heads * D) * 2, q_out, (size_t)T * Hq * D * 2))
-    return ANVILQ_EINVAL;
+  // an item's q is written while others' rows are still to be read, and every pool by
+  // warps of its own
+  const size_t pool = (size_t)positions * Hkv * D * (type == kBinary16 ? 2 : 1);
+  const size_t scales = type == kBinary16 ? 0 : (size_t)positions / kBlock * Hkv * sizeof(float);
+  const Span spans[] = {{qkv, ((size_t)(T - 1) * stride + (size_t)heads * D) * 2}, {q_out, (size_t)T * Hq * D * 2},
+                        {k, pool}, {v, pool}, {k_scales, scales}, {v_scales, scales}};
+  for (const Span& a : spans)
+    for (const Span* b = &a + 1; b != std::end(spans); ++b)
+      if (overlap(a.start, a.bytes, b->start, b->bytes)) return ANVILQ_EINVAL;
   Params p{};
   p.qkv = reinterpret_cast<const __half*>(qkv);
   p.stride = stride;

@@ -658,7 +658,8 @@ int anvilq_gqa_decode_paged(const uint16_t* q, const uint16_t* k_pool, const uin
  * token ANVILQ_DEV_ERR_PAGE; nothing is then written for it (for that page).
  * D in {64, 128}, page_tokens % 16 == 0, qkv_stride % 8 == 0, 16-byte aligned
  * qkv, q_out and pools; dev_err required; T == 0 does nothing (qkv and q_out
- * may then be NULL); q_out lies outside the span of qkv's rows. */
+ * may then be NULL); the span of qkv's rows, q_out and the pools (with their
+ * scales) are apart from each other. */
 int anvilq_paged_kv_append(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
                            const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, uint16_t* k_pool,
                            uint16_t* v_pool, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages,

@@ -175,3 +175,27 @@ def test_logits_front_end(change):
 def test_attention_scale_refused(scale):
     """Scales that are not finite, and those whose product with an int8 block's scale is not."""
     assert _lib.load().anvilq_gqa_decode_q8(*{**ATTN, "scale": scale}.values()) == EINVAL
+
+
+# 4 tokens, 12 heads of 128: 12288 bytes of qkv, 8192 of q; 8 pages x 16 x 2 x 128: 65536
+# bytes of a binary16 pool, 32768 of codes, 64 of scales
+APART = dict(APPEND, qkv=at(0), q=at(1 << 14), k=at(1 << 17), v=at(1 << 18))
+APART_Q8 = dict(APPEND_Q8, qkv=at(0), q=at(1 << 14), k=at(1 << 17), v=at(1 << 18), ks=at(1 << 19), vs=at(1 << 20))
+
+
+@pytest.mark.parametrize("name,base,change", [
+    *(("anvilq_paged_kv_append", APART, c) for c in (
+        dict(v=at(1 << 17)), dict(v=at((1 << 17) + 65536 - 16)), dict(v=at((1 << 17) - 65536 + 16)), dict(k=at(0)),
+        dict(v=at(16)), dict(q=at((1 << 17) + 1024)), dict(k=at((1 << 14) + 8192 - 16)))),
+    *(("anvilq_paged_kv_append_q8", APART_Q8, c) for c in (
+        dict(v=at(1 << 17)), dict(v=at((1 << 17) + 32768 - 16)), dict(vs=at(1 << 19)), dict(vs=at((1 << 19) + 60)),
+        dict(ks=at((1 << 17) + 64)), dict(vs=at((1 << 18) + 32764)), dict(ks=at(1 << 14)), dict(vs=at(12284)))),
+], ids=lambda v: v if isinstance(v, str) else None)
+def test_append_outputs_that_overlap_are_refused(name, base, change):
+    assert getattr(_lib.load(), name)(*{**base, **change}.values()) == EINVAL
+
+
+def test_append_pools_beyond_memory_are_refused():
+    big = dict(pages=2**31 - 1, page=1 << 26, max_pages=1)
+    assert _lib.load().anvilq_paged_kv_append(*{**APART, **big}.values()) == ESHAPE
+    assert _lib.load().anvilq_paged_kv_append_q8(*{**APART_Q8, **big}.values()) == ESHAPE
