@@ -1141,6 +1141,13 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
   const double tiles = all_pairs * ((double)max_pages * page_tokens / kTile + 1);   // that the table has room for
   if (tiles > (double)(1u << 31)) return ANVILQ_ESHAPE;   // they are counted in 32 bits
   if (!a16(q) || !a16(k_codes) || !a16(v_codes) || !a16(out) || !a16(workspace)) return ANVILQ_EALIGN;
+  // out may be q: a pair's rows are written when all that read them have done so
+  const size_t rows_bytes = (size_t)B * Q * Hq * D * 2, codes = (size_t)rows * D, scales = (size_t)rows / kBlock * 4;
+  if ((out != q && q8::overlap(out, rows_bytes, q, rows_bytes)) || q8::overlap(out, rows_bytes, k_codes, codes) ||
+      q8::overlap(out, rows_bytes, v_codes, codes) || q8::overlap(out, rows_bytes, k_scales, scales) ||
+      q8::overlap(out, rows_bytes, v_scales, scales) ||
+      (workspace && q8::overlap(out, rows_bytes, workspace, workspace_bytes)))
+    return ANVILQ_EINVAL;
   const int sms = sm_count();
   if (sms <= 0) return ANVILQ_ECUDA;
   if (!workspace || workspace_bytes < anvilq_gqa_decode_q8_workspace_size(B, Q, Hq, Hkv, D)) return ANVILQ_EWORKSPACE;

@@ -805,7 +805,7 @@ def gqa_decode_q8(q, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, 
     chunk), each seeing the positions up to its own.  seqlens int32 [B] counts all
     tokens, the queries' included; a sequence of length 0 gives zeros.  scale (finite, at
     most 2^64): of the scores, 0 or less for 1/sqrt(D).  Returns fp16
-    in q's shape.  workspace: a uint8 tensor zero-filled once, for callers that keep
+    in q's shape (out may be q itself).  workspace: a uint8 tensor zero-filled once, for callers that keep
     their own (default: the current stream's).
 
     attention(q, keys, values) of anvil-q1-fp/tests/fp64_reference.py:164-170, batched."""

@@ -699,7 +699,8 @@ int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k
  * 2^64) <= 0 selects 1/sqrt(D).  Hq % Hkv == 0, Hq <= 1024, Q <= 64, B <= 65535, at most 2^31 - 1
  * rows (num_pages * page_tokens * Hkv) in a pool; the tables' positions over
  * 32, times Hkv and the groups of 8 or 16 query rows of a head, at most 2^31;
- * 16-byte aligned q, codes and out; dev_err required.  A length outside its range sets
+ * 16-byte aligned q, codes and out; out is q itself or apart from all inputs;
+ * dev_err required.  A length outside its range sets
  * ANVILQ_DEV_ERR_SEQLEN and counts as 0; an absent live page sets
  * ANVILQ_DEV_ERR_PAGE (the output is then not to be used).  workspace: at least
  * anvilq_gqa_decode_q8_workspace_size(...) bytes (0: shape not supported),

@@ -1212,3 +1212,18 @@ def test_attention_q8_largest_scale(dev, fp8):
             want = vv[x.argmax(), h // 4]
             tol = 2 * HALF * (1 + 2.0 ** -6) * np.abs(want)
         assert (np.abs(out[0, 0, h] - want) <= tol + 2.0 ** -24).all(), h
+
+
+@pytest.mark.parametrize("lens,Q", [([5000, 0, 40], 1), ([900, 3, 70], 4), ([33] * 40, 1)])
+def test_attention_q8_in_place(dev, lens, Q):
+    rng = np.random.default_rng(81)
+    q, k, v, ks, vs, table = attention_case(dev, rng, lens, Q, 8, 2, 128, 16, False)
+    a = [t.to(dev) for t in (k, v, ks, vs)] + [to(table, dev), to(np.array(lens, np.int32), dev)]
+    ref = ops.gqa_decode_q8(to(q, dev), *a)
+    for _ in range(5):
+        x = to(q, dev)
+        assert ops.gqa_decode_q8(x, *a, out=x) is x and torch.equal(x, ref)
+    ops.raise_device_errors(dev)
+    both = torch.zeros((2 * x.numel(),), dtype=torch.float16, device=dev)
+    with pytest.raises(AnvilqError):
+        ops.gqa_decode_q8(both[:x.numel()].view_as(x), *a, out=both[64:64 + x.numel()].view_as(x))

@@ -199,3 +199,16 @@ def test_append_pools_beyond_memory_are_refused():
     big = dict(pages=2**31 - 1, page=1 << 26, max_pages=1)
     assert _lib.load().anvilq_paged_kv_append(*{**APART, **big}.values()) == ESHAPE
     assert _lib.load().anvilq_paged_kv_append_q8(*{**APART_Q8, **big}.values()) == ESHAPE
+
+
+# 2 queries of 8 heads of 128: 4096 bytes of q and of out
+ATTN_APART = dict(ATTN, q=at(0), out=at(1 << 14), k=at(1 << 17), v=at(1 << 18), ks=at(1 << 19), vs=at(1 << 20),
+                  ws=at(1 << 21))
+
+
+@pytest.mark.parametrize("change", [
+    dict(out=at(16)), dict(out=at(4080)), dict(out=at(-4080)), dict(out=at(1 << 17)), dict(out=at((1 << 18) + 32752)),
+    dict(out=at((1 << 17) - 4080)), dict(out=at((1 << 19) + 48)), dict(out=at((1 << 20) - 16)), dict(out=at(1 << 22)),
+])
+def test_attention_output_over_inputs_refused(change):
+    assert _lib.load().anvilq_gqa_decode_q8(*{**ATTN_APART, **change}.values()) == EINVAL
