@@ -1227,3 +1227,76 @@ def test_attention_q8_in_place(dev, lens, Q):
     both = torch.zeros((2 * x.numel(),), dtype=torch.float16, device=dev)
     with pytest.raises(AnvilqError):
         ops.gqa_decode_q8(both[:x.numel()].view_as(x), *a, out=both[64:64 + x.numel()].view_as(x))
+
+
+@pytest.mark.parametrize("lens,Q,Hq,Hkv,page,fp8", [
+    ([900, 40], 8, 8, 2, 16, False),           # 32 query rows a kv head: two groups
+    ([300, 0, 2000], 8, 28, 4, 32, True),      # 56: four groups, the last half full
+    ([700], 64, 32, 8, 64, False),             # 256
+    ([5000], 16, 4, 1, 16, True),              # 64 rows of one kv head over many CTAs
+])
+def test_attention_q8_row_groups(dev, lens, Q, Hq, Hkv, page, fp8):
+    """More query rows a kv head than one group holds, heads of 128."""
+    rng = np.random.default_rng(Q + Hq)
+    q, k, v, ks, vs, table = attention_case(dev, rng, lens, Q, Hq, Hkv, 128, page, fp8)
+    a = [t.to(dev) for t in (k, v, ks, vs)] + [to(table, dev), to(np.array(lens, np.int32), dev)]
+    qd = to(q, dev)
+    out = ops.gqa_decode_q8(qd, *a)
+    again = ops.gqa_decode_q8(qd, *a, out=torch.full_like(qd, float("nan")))
+    ops.raise_device_errors(dev)
+    assert torch.equal(out, again)
+    check_attention(out.cpu().numpy(), q, k, v, ks, vs, table, lens)
+
+
+def test_append_rotations_of_several_thetas(dev):
+    """Calls that take turns in theta and head size, in one thread: each rotates by its own."""
+    rng = np.random.default_rng(91)
+    Hq, Hkv, page = 4, 2, 16
+    cases = []
+    for D in (64, 128):
+        qkv, table, starts, lens, pages = append_case(rng, [3000, 0], [5, 20], Hq, Hkv, D, page, spare_rows=0)
+        cases.append((D, qkv, to(table, dev), to(lens, dev), to(starts, dev), pages, rows_of(starts, lens)))
+    for i, theta in ((0, 1e4), (0, 5e5), (0, 1e6), (1, 1e6), (1, 1e4), (0, 1e4), (0, 5e5), (1, 5e5)):   # one changes
+        D, qkv, table, lens, starts, pages, rows = cases[i]
+        x = qkv.reshape(len(rows), Hq + 2 * Hkv, D)[:, :Hq]
+        turned = so.rotate(x, [p for _, p in rows], theta)
+        pair = np.abs(x.astype(np.float64))
+        tol = HALF * np.abs(turned) + 2.0 ** -22 * (pair + np.roll(pair, D // 2, axis=2)) + 2.0 ** -25
+        k = torch.zeros((pages, page, Hkv, D), dtype=torch.float16, device=dev)
+        q = ops.paged_kv_append(to(qkv, dev), k, torch.zeros_like(k), table, lens, starts, Hq, theta)
+        assert (np.abs(q.cpu().numpy() - turned) <= tol).all(), (D, theta)
+        codes, scales = torch.zeros((pages, Hkv, page, D), dtype=torch.int8, device=dev), torch.zeros((pages, Hkv, 1), device=dev)
+        assert torch.equal(ops.paged_kv_append_q8(to(qkv, dev), codes, codes.clone(), scales, scales.clone(), table, lens,
+                                                  starts, Hq, theta), q)
+    ops.raise_device_errors(dev)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_drafts_rejected_and_appended_over(dev, fp8):
+    """Drafts of large values, cut back by seqlens and appended over: the accepted rows stay
+    coded to the scale that the drafts raised, later rows of the block use it too, and a block
+    that was cut back to its start takes a scale of its own."""
+    rng = np.random.default_rng(95)
+    Hq, Hkv, D, page, dtype = 4, 2, 64, 32, code_dtype(fp8)
+    table = so.make_table([1], 2, rng)
+    pg = so.physical(table[0, 0])
+    k = torch.zeros((2, Hkv, page, D), device=dev).to(dtype)
+    v, ks, vs = k.clone(), *(torch.zeros((2, Hkv, page // BLOCK), device=dev) for _ in range(2))
+    t = to(table, dev)
+    codes, scales = [torch.zeros((0, D)).to(dtype)] * Hkv, torch.zeros(Hkv)      # of the block in work
+    kept = 0
+    for first, n, size in ((0, 5, 1.0), (5, 4, 50.0), (6, 3, 1.0), (9, 7, 2.0),  # one draft of four accepted
+                           (16, 3, 90.0), (16, 4, 0.5), (18, 2, 8.0)):           # none of three; half of four
+        qkv = (rng.standard_normal((n, (Hq + 2 * Hkv) * D)) * size).astype(np.float16)
+        lens = to(np.array([first + n], np.int32), dev)
+        q = ops.paged_kv_append_q8(to(qkv, dev), k, v, ks, vs, t, lens, to(np.array([0, n], np.int32), dev), Hq)
+        x = torch.from_numpy(qkv.astype(np.float32)).view(n, Hq + 2 * Hkv, D)[:, Hq + Hkv:]
+        block, kept = first // BLOCK, first % BLOCK
+        for h in range(Hkv):
+            codes[h], s = step_codes(x[:, h], kept, codes[h], scales[h], dtype)
+            scales[h] = s
+            assert vs[pg, h, block].item() == s.item(), (first, h)
+            assert torch.equal(v[pg, h, block * BLOCK:first + n].cpu().float(), codes[h].float()), (first, h)
+        out = ops.gqa_decode_q8(q.view(1, n, Hq, D), k, v, ks, vs, t, lens)
+        check_attention(out.cpu().numpy(), q.cpu().numpy()[None], k, v, ks, vs, table, [first + n])
+    ops.raise_device_errors(dev)
