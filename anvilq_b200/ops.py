@@ -61,19 +61,21 @@ def raise_device_errors(device=None):
         if value & 1:
             what.append("invalid AWQ scale (negative nonzero or nonfinite)")
         if value & 2:
-            what.append("sequence length outside [1, Tmax]")
+            what.append("sequence or history length, bias range or mask row outside its bounds")
         if value & 4:
             what.append("bounded wait expired inside a kernel")
         if value & 8:
             what.append("token id outside [0, V)")
         if value & 16:
-            what.append("nonfinite binary16 parameter (bias)")
+            what.append("nonfinite value (a bias, a key or value to be coded, or an escaped row without its buffer)")
         if value & 32:
             what.append("page-table entry of a live page absent or out of range")
         if value & 64:
             what.append("draft-node ancestor mask breaks the tree contract")
         if value & 128:
             what.append("legacy cache block with a forbidden code, padding or metadata")
+        if value & 256:
+            what.append("tensor of a layer table that is not 16-byte aligned")
         raise _lib.AnvilqError(f"device error bits 0x{value:x}: " + "; ".join(what))
 
 

@@ -48,10 +48,13 @@ typedef struct CUstream_st* anvilq_stream_t; /* same type as cudaStream_t */
 
 /* Bits OR-ed into *dev_err by a kernel. */
 #define ANVILQ_DEV_ERR_SCALE 1   /* an AWQ scale was negative-nonzero or nonfinite */
-#define ANVILQ_DEV_ERR_SEQLEN 2  /* a sequence length outside [1, Tmax] */
+#define ANVILQ_DEV_ERR_SEQLEN 2  /* a sequence length or position outside the call's range (most: [1, Tmax]), a
+                                    sequence with more new tokens than its length, a history length, bias range or
+                                    mask row outside its bounds */
 #define ANVILQ_DEV_ERR_TIMEOUT 4 /* a bounded wait inside a kernel expired */
 #define ANVILQ_DEV_ERR_TOKEN 8   /* a token id outside [0, V) */
-#define ANVILQ_DEV_ERR_NONFINITE 16 /* a binary16 parameter (bias) was Inf or NaN */
+#define ANVILQ_DEV_ERR_NONFINITE 16 /* a binary16 parameter (bias) or a key or value to be coded was Inf or NaN, or a
+                                       cached row was escaped without an escape buffer */
 #define ANVILQ_DEV_ERR_PAGE 32     /* a page-table entry of a live page was absent or out of range */
 #define ANVILQ_DEV_ERR_TREE 64     /* a draft node's ancestor mask broke the tree contract */
 #define ANVILQ_DEV_ERR_CODEC 128   /* a legacy cache block held a forbidden code, padding or metadata */
@@ -653,9 +656,10 @@ int anvilq_gqa_decode_paged(const uint16_t* q, const uint16_t* k_pool, const uin
  * goes to q_out fp16 [T][Hq][D], k and v to row position % page_tokens of
  * physical page page_table[b][position / page_tokens] of the pools of
  * anvilq_gqa_decode_paged.  No two new tokens may share a cache row.
- * A sequence with more new tokens than seqlens[b], or longer than
- * page_tokens * max_pages, sets ANVILQ_DEV_ERR_SEQLEN, an absent page of a new
- * token ANVILQ_DEV_ERR_PAGE; nothing is then written for it (for that page).
+ * Of the sequences with new tokens, one with more of them than seqlens[b], or
+ * longer than page_tokens * max_pages, sets ANVILQ_DEV_ERR_SEQLEN, an absent page
+ * of a new token ANVILQ_DEV_ERR_PAGE; nothing is then written for it (for that
+ * page).
  * D in {64, 128}, page_tokens % 16 == 0, qkv_stride % 8 == 0, 16-byte aligned
  * qkv, q_out and pools; dev_err required; T == 0 does nothing (qkv and q_out
  * may then be NULL); the span of qkv's rows, q_out and the pools (with their
@@ -673,8 +677,12 @@ int anvilq_paged_kv_append(const uint16_t* qkv, long long qkv_stride, const int3
  * row is among the new ones; new rows are stored as round(value * fp32(1 / s)),
  * and where s > s_kept the block's earlier rows become
  * round(code * fp32(s_kept / s)) -- so one int8 code is off by at most half a
- * step of every scale its block has had.  Rows behind the new ones keep their
- * codes.  A value that is not finite sets ANVILQ_DEV_ERR_NONFINITE and is
+ * step of every scale its block has had.  A sequence may be cut back (seqlens
+ * lowered, as when drafted tokens are rejected) and appended to again: rows that
+ * stay keep the scale that rejected rows of their block had raised, and later
+ * rows of the block use it too; a block cut back to its start takes a new one.
+ * The codes of the same tokens therefore depend on how they arrived.  Rows behind
+ * the new ones keep their codes.  A value that is not finite sets ANVILQ_DEV_ERR_NONFINITE and is
  * stored as 0.  Two sequences must not append to the same page in one call. */
 int anvilq_paged_kv_append_q8(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
                               const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, void* k_codes,
