@@ -515,7 +515,7 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   const long long by_place = T / kBlock + 2LL * B;
   p.by_token = T <= by_place;
   const int items = (int)(p.by_token ? (long long)T : by_place);
-  // Slices of the heads, at least 8 heads each, only until there are four CTAs an SM
+  // Slices of the heads, more than 4 heads each, only until there are four CTAs an SM
   // (three with 8-bit pages, whose CTAs take more registers): every slice looks up
   // its tokens and computes their cosines again.  32/8 heads of 128, one slice and
   // two: 560 items into binary16 47.5 and 39.9 us, 350 items into 8 bits 32.0 and
