@@ -838,6 +838,11 @@ def gqa_decode_q8(q, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, 
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _logits_workspace_size(B, V):
+    return _lib.load().anvilq_logits_process_workspace_size(B, V)
+
+
 def logits_process(logits, history=None, history_lens=None, prompt_lens=None, repetition=None, presence=None,
                    frequency=None, bias_starts=None, bias_ids=None, bias_values=None, allowed=None, allowed_rows=None,
                    out=None, write_logits: bool = True, choose: bool = True, dev_err=None, workspace=None,
@@ -933,9 +938,10 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
     tokens = logits.new_empty(B, dtype=torch.int32) if choose else None
     _on_device(name, dev, history, history_lens, prompt_lens, repetition, presence, frequency, bias_starts, bias_ids,
                bias_values, allowed, allowed_rows, out)
-    if B > 4096 or V > 1 << 30:
+    need = _logits_workspace_size(B, V)
+    if need == 0:
         raise ValueError(f"{name}: unsupported shape B={B} V={V}")
-    ws = _call_workspace(dev, WORKSPACE_COUNTER_BYTES, workspace) if choose else None
+    ws = _call_workspace(dev, need, workspace) if choose else None
     err = _error_word(dev, dev_err)
     _call("anvilq_logits_process", dev, _ptr(logits), half, pitch if B > 1 else V, _ptr(out), out_pitch, _ptr(tokens),
           B, V, _ptr(history) if L else _ptr(history_lens), history_pitch, _ptr(history_lens), _ptr(prompt_lens), L,
