@@ -701,10 +701,14 @@ int anvilq_kv_q8_values(const void* k_codes, const void* v_codes, const float* k
  * b is its token at position seqlens[b] - Q + i and sees every position up to
  * its own (Q = 1: the decode step; more: drafted tokens or a chunk, appended
  * before).  q and out fp16 [B][Q][Hq][D], seqlens int32 [B] (device, 0 ..
- * page_tokens * max_pages <= 2^30).  A query that sees nothing -- an empty sequence, or
- * a position below 0 -- gives zeros.  Scores and the softmax run in fp32, the
- * probabilities enter the tensor cores as binary16.  scale (finite, at most
- * 2^64) <= 0 selects 1/sqrt(D).  Hq % Hkv == 0, Hq <= 1024, Q <= 64, B <= 65535, at most 2^31 - 1
+ * page_tokens * max_pages <= 2^30).  Codes of the tokens that a sequence holds
+ * are numbers and their scales finite and >= 0, as the append writes them (a NaN
+ * among the values of drafted tokens would reach the queries before them too);
+ * what lies behind a sequence's last token may be anything.  A query that sees
+ * nothing -- an empty sequence, or a position below 0 -- gives zeros.  Scores and
+ * the softmax run in fp32, the probabilities enter the tensor cores as binary16.
+ * scale (finite, at most 2^64) <= 0 selects 1/sqrt(D).  Hq % Hkv == 0,
+ * Hq <= 1024, Q <= 64, B <= 65535, at most 2^31 - 1
  * rows (num_pages * page_tokens * Hkv) in a pool; the tables' positions over
  * 32, times Hkv and the groups of 8 or 16 query rows of a head, at most 2^31;
  * 16-byte aligned q, codes and out; out is q itself or apart from all inputs;
