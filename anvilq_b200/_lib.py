@@ -70,6 +70,10 @@ SIGNATURES = {
     "anvilq_paged_kv_append": (I, [P, LL, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, P, ctypes.c_uint, P]),
     "anvilq_paged_kv_append_q8": (I, [P, LL, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, ctypes.c_uint,
                                       P]),
+    "anvilq_paged_kv_append_rope": (I, [P, LL, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P, I, I, F, P, ctypes.c_uint,
+                                        P]),
+    "anvilq_paged_kv_append_q8_rope": (I, [P, LL, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, I, I, F, P,
+                                           ctypes.c_uint, P]),
     "anvilq_kv_q8_values": (I, [P, P, P, P, I, P, P, I, I, I, I, ctypes.c_uint, P]),
     "anvilq_gqa_decode_q8_workspace_size": (SZ, [I, I, I, I, I]),
     "anvilq_gqa_decode_q8": (I, [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, P, SZ, P, ctypes.c_uint, P]),

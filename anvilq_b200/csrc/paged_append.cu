@@ -15,6 +15,10 @@
 // with a new row).  Where s > s_kept the kept rows are re-coded,
 //   code' = round(code * fp32(s_kept / s)).
 // Values are coded from binary32, not from a binary16 rounding of them.
+// With frequencies of the caller's (ROPE), angle_i = fp32(p * inv_freq[i]) for the
+// first R dims of a head only, in split halves of them (i, i + R/2) or in neighbouring
+// pairs (2i, 2i + 1); cos and sin are multiplied by a factor (binary32, rounded).  A
+// thread takes 8 pairs all the same, so only where its 16 dims lie differs.
 //
 // What bounds it: bytes (2 B in, 2 or 1 B out for every element; a few binary32
 // operations each), and for a decode step, one token a sequence, the latency of
@@ -35,6 +39,7 @@
 #include <algorithm>
 #include <cmath>
 #include <iterator>
+#include <type_traits>
 
 #include "kv_q8.cuh"
 
@@ -47,9 +52,20 @@ constexpr int kBinary16 = -1;   // the pool's type: binary16, q8::kInt8 or q8::k
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxPairs = 64;   // D <= 128
+// of a caller's rotation: 8-bit blocks' scales then stay below 2^26, which attention's
+// scores, with its largest softmax scale, take without leaving binary32's range
+constexpr float kMaxFactor = 65536.0f;
 
 struct Freq {
   double inv[kMaxPairs];   // theta^(-2i/D), binary64, computed on the host
+};
+
+// Frequencies of the caller's, in device memory: no copy of them is made at a call.
+struct Rope {
+  const double* inv;   // [dims / 2]; null: Freq, the whole head in split halves
+  int dims;            // R: a multiple of 16
+  int pairs;           // neighbouring dims turn together
+  float factor;
 };
 
 struct Params {
@@ -67,6 +83,7 @@ struct Params {
   int T, B, Hq, Hkv, page_tokens, max_pages, num_pages;
   int by_token;                 // how blockIdx.x names an item, see find_item
   int heads_per_cta;
+  Rope rope;
 };
 
 // The item of a CTA: rows [row, row + count) of qkv, positions pos .. of sequence b.
@@ -147,18 +164,43 @@ __device__ __forceinline__ void load8(const float* src, float* v) {   // 16-byte
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
-// 8 dims of both halves of a row, rotated: (a, b) -> (a cos - b sin, b cos + a sin)
-__device__ __forceinline__ void rotate8(float* a, float* b, const float* co, const float* si) {
+// (a, b) -> (a cos - b sin, b cos + a sin)
+__device__ __forceinline__ void rotate_pair(float& a, float& b, float co, float si) {
+  const float u = a, v = b;
+  a = __fsub_rn(__fmul_rn(u, co), __fmul_rn(v, si));
+  b = __fadd_rn(__fmul_rn(v, co), __fmul_rn(u, si));
+}
+
+// How a head is rotated: whole, in split halves, by Freq; or by Params::rope in split
+// halves of its first dims or in neighbouring pairs of them.
+enum { kTheta, kHalves, kPairs };
+
+// Where the 8 pairs of a row's lane `c` lie: 8 dims from lo on, 8 from hi on.
+struct Dims {
+  int lo, hi;
+  bool turns;   // else they are copied
+};
+template <int D, int ROPE>
+__device__ __forceinline__ Dims dims_of(const Rope& r, int c) {
+  if (!ROPE) return {8 * c, 8 * c + D / 2, true};
+  const bool turns = 16 * c < r.dims;
+  if (!turns || ROPE == kPairs) return {16 * c, 16 * c + 8, turns};
+  return {8 * c, 8 * c + r.dims / 2, true};
+}
+// The 16 values of such a lane, rotated.
+template <int ROPE>
+__device__ __forceinline__ void turn16(float* x, const float* co, const float* si) {
+  if (ROPE == kPairs) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float u = a[e], v = b[e];
-    a[e] = __fsub_rn(__fmul_rn(u, co[e]), __fmul_rn(v, si[e]));
-    b[e] = __fadd_rn(__fmul_rn(v, co[e]), __fmul_rn(u, si[e]));
+    for (int e = 0; e < 8; ++e) rotate_pair(x[2 * e], x[2 * e + 1], co[e], si[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) rotate_pair(x[e], x[8 + e], co[e], si[e]);
   }
 }
 
 // FEW: with a path for items of a row or two (run has the rule)
-template <int D, int TYPE, bool FEW>
+template <int D, int TYPE, bool FEW, int ROPE>
 __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
     append_kernel(const __grid_constant__ Params p, const __grid_constant__ Freq freq) {
   constexpr int kHalf = D / 2;
@@ -175,27 +217,40 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
   // are a power of two of rows; the other threads take other heads.
   const int end16 = TYPE == kBinary16 ? head1 : min(head1, p.Hq);
   const int log_rows = 32 - __clz(it.count - 1);   // 0 for one row
-  const int d16 = 8 * (threadIdx.x % kLanes), r16 = (threadIdx.x / kLanes) & ((1 << log_rows) - 1);
+  const int c16 = threadIdx.x % kLanes, r16 = (threadIdx.x / kLanes) & ((1 << log_rows) - 1);
+  const Dims at16 = dims_of<D, ROPE>(p.rope, c16);
   const int step = (kThreads / kLanes) >> log_rows;
-  const __half* src16 = p.qkv + (size_t)(it.row + r16) * p.stride + d16;
+  const __half* src16 = p.qkv + (size_t)(it.row + r16) * p.stride;
   constexpr int kAhead = 3;   // heads a thread loads at a time
   uint4 lo[kAhead], hi[kAhead];
   auto load = [&](int h0) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       if (r16 < it.count && h0 + k * step < end16) {
-        lo[k] = *reinterpret_cast<const uint4*>(src16 + (h0 + k * step) * D);
-        hi[k] = *reinterpret_cast<const uint4*>(src16 + (h0 + k * step) * D + kHalf);
+        lo[k] = *reinterpret_cast<const uint4*>(src16 + (h0 + k * step) * D + at16.lo);
+        hi[k] = *reinterpret_cast<const uint4*>(src16 + (h0 + k * step) * D + at16.hi);
       }
   };
   int h0 = head0 + ((threadIdx.x / kLanes) >> log_rows);
   load(h0);   // the first heads' rows travel with the page-table word, while the cosines are computed
 
   const int page = q8::page_of(p.page_table, p.max_pages, p.num_pages, it.b, it.pos / p.page_tokens);
-  for (int i = threadIdx.x; i < it.count * kHalf; i += kThreads) {
-    const int r = i / kHalf, pair = i % kHalf;
-    const float angle = (float)((double)(it.pos + r) * freq.inv[pair]);
-    sincosf(angle, &s_sin[r][pair], &s_cos[r][pair]);
+  if (ROPE) {
+    const int n = p.rope.dims / 2;
+    for (int i = threadIdx.x; i < it.count * n; i += kThreads) {
+      const int r = i / n, pair = i % n;
+      const float angle = (float)((double)(it.pos + r) * p.rope.inv[pair]);
+      float si, co;
+      sincosf(angle, &si, &co);
+      s_sin[r][pair] = __fmul_rn(si, p.rope.factor);
+      s_cos[r][pair] = __fmul_rn(co, p.rope.factor);
+    }
+  } else {
+    for (int i = threadIdx.x; i < it.count * kHalf; i += kThreads) {
+      const int r = i / kHalf, pair = i % kHalf;
+      const float angle = (float)((double)(it.pos + r) * freq.inv[pair]);
+      sincosf(angle, &s_sin[r][pair], &s_cos[r][pair]);
+    }
   }
   if (page < 0) {
     if (threadIdx.x == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
@@ -205,32 +260,32 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
   const int slot = it.pos % p.page_tokens;    // row of the page of the item's first token
   {
     float co[8], si[8];
-    load8(s_cos[r16] + d16, co);   // of a row behind the item's: not used
-    load8(s_sin[r16] + d16, si);
+    load8(s_cos[r16] + 8 * c16, co);   // of a row behind the item's, of pairs that are not: not used
+    load8(s_sin[r16] + 8 * c16, si);
 #pragma unroll 1
     for (; h0 < end16; h0 += kAhead * step) {
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int head = h0 + k * step;
         if (r16 >= it.count || head >= end16) break;
-        if (TYPE != kBinary16 || head < p.Hq + p.Hkv) {
-          float a[8], b[8];
-          unpack8(lo[k], a);
-          unpack8(hi[k], b);
-          rotate8(a, b, co, si);
-          lo[k] = pack8(a);
-          hi[k] = pack8(b);
+        if ((TYPE != kBinary16 || head < p.Hq + p.Hkv) && (!ROPE || at16.turns)) {
+          float x[16];
+          unpack8(lo[k], x);
+          unpack8(hi[k], x + 8);
+          turn16<ROPE>(x, co, si);
+          lo[k] = pack8(x);
+          hi[k] = pack8(x + 8);
         }
         __half* dst;
         if (TYPE != kBinary16 || head < p.Hq) {
-          dst = p.q_out + ((size_t)(it.row + r16) * p.Hq + head) * D + d16;
+          dst = p.q_out + ((size_t)(it.row + r16) * p.Hq + head) * D;
         } else {
           const bool is_k = head < p.Hq + p.Hkv;
           dst = static_cast<__half*>(is_k ? p.k : p.v) +
-                (((size_t)page * p.page_tokens + slot + r16) * p.Hkv + head - p.Hq - (is_k ? 0 : p.Hkv)) * D + d16;
+                (((size_t)page * p.page_tokens + slot + r16) * p.Hkv + head - p.Hq - (is_k ? 0 : p.Hkv)) * D;
         }
-        *reinterpret_cast<uint4*>(dst) = lo[k];
-        *reinterpret_cast<uint4*>(dst + kHalf) = hi[k];
+        *reinterpret_cast<uint4*>(dst + at16.lo) = lo[k];
+        *reinterpret_cast<uint4*>(dst + at16.hi) = hi[k];
       }
       load(h0 + kAhead * step);
     }
@@ -241,7 +296,8 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
   constexpr int kCode = TYPE == q8::kE4m3 ? q8::kE4m3 : q8::kInt8;
   constexpr int kRows = 32 / kLanes;          // rows of a pass of a warp
   constexpr int kPasses = kBlock / kRows;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r0 = lane / kLanes, d0 = 8 * (lane % kLanes);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r0 = lane / kLanes, c0 = lane % kLanes;
+  const Dims at0 = dims_of<D, ROPE>(p.rope, c0);
   const int kept = it.pos % kBlock;           // rows of the block that were there before
   auto finite = [](float v) { return fabsf(v) <= 3.4028234664e38f ? v : 0.0f; };
   // the block's earlier codes in the lane's dims, rows first, first + step ..., times ratio
@@ -250,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
     for (int r = first; r < kept; r += step) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint2* at = reinterpret_cast<uint2*>(rows + r * D + d0 + h * kHalf);
+        uint2* at = reinterpret_cast<uint2*>(rows + r * D + (h ? at0.hi : at0.lo));
         uint2 w = *at;
         float v[8];
         q8::codes_to_float4<kCode>(w.x, v);
@@ -275,19 +331,19 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
       uint4 a = make_uint4(0, 0, 0, 0), b = a;
       float s_kept = 0.0f;
       if (mine) {
-        const __half* src = p.qkv + (size_t)(it.row + row) * p.stride + head * D + d0;
-        a = *reinterpret_cast<const uint4*>(src);
-        b = *reinterpret_cast<const uint4*>(src + kHalf);
+        const __half* src = p.qkv + (size_t)(it.row + row) * p.stride + head * D;
+        a = *reinterpret_cast<const uint4*>(src + at0.lo);
+        b = *reinterpret_cast<const uint4*>(src + at0.hi);
       }
       if (live && kept) s_kept = *scale_at;
       float x[16];
       unpack8(a, x);
       unpack8(b, x + 8);
-      if (is_k && mine) {
+      if (is_k && mine && (!ROPE || at0.turns)) {
         float co[8], si[8];
-        load8(s_cos[row] + d0, co);
-        load8(s_sin[row] + d0, si);
-        rotate8(x, x + 8, co, si);
+        load8(s_cos[row] + 8 * c0, co);
+        load8(s_sin[row] + 8 * c0, si);
+        turn16<ROPE>(x, co, si);
       }
       float top = 0.0f, probe = 0.0f;   // probe: NaN after a value that is not finite
 #pragma unroll
@@ -317,9 +373,9 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
         if (mine)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<uint2*>(rows + (kept + row) * D + d0 + h * kHalf) =
+            *reinterpret_cast<uint2*>(rows + (kept + row) * D + (h ? at0.hi : at0.lo)) =
                 make_uint2(q8::float4_to_codes<kCode>(x + 8 * h), q8::float4_to_codes<kCode>(x + 8 * h + 4));
-        if (row == 0 && d0 == 0) *scale_at = s;
+        if (row == 0 && c0 == 0) *scale_at = s;
       }
     }
     return;
@@ -329,23 +385,23 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
     const bool is_k = head < p.Hq + p.Hkv;
     const int kvh = head - p.Hq - (is_k ? 0 : p.Hkv);
     uint4 raw[kPasses][2];
-    const __half* src = p.qkv + (size_t)(it.row + r0) * p.stride + head * D + d0;
+    const __half* src = p.qkv + (size_t)(it.row + r0) * p.stride + head * D;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
       if (i * kRows + r0 < it.count) {
-        raw[i][0] = *reinterpret_cast<const uint4*>(src + (size_t)i * kRows * p.stride);
-        raw[i][1] = *reinterpret_cast<const uint4*>(src + (size_t)i * kRows * p.stride + kHalf);
+        raw[i][0] = *reinterpret_cast<const uint4*>(src + (size_t)i * kRows * p.stride + at0.lo);
+        raw[i][1] = *reinterpret_cast<const uint4*>(src + (size_t)i * kRows * p.stride + at0.hi);
       }
     }
     auto values = [&](int i, float* x) {   // of pass i
       unpack8(raw[i][0], x);
       unpack8(raw[i][1], x + 8);
-      if (is_k && i * kRows + r0 < it.count) {
+      if (is_k && i * kRows + r0 < it.count && (!ROPE || at0.turns)) {
         float co[8], si[8];
-        load8(s_cos[i * kRows + r0] + d0, co);
-        load8(s_sin[i * kRows + r0] + d0, si);
-        rotate8(x, x + 8, co, si);
+        load8(s_cos[i * kRows + r0] + 8 * c0, co);
+        load8(s_sin[i * kRows + r0] + 8 * c0, si);
+        turn16<ROPE>(x, co, si);
       }
     };
     float top = 0.0f, probe = 0.0f;   // probe: NaN after a value that is not finite
@@ -396,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, TYPE == kBinary16 ? 8 : 5)
       if (r < it.count)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint2*>(rows + (kept + r) * D + d0 + h * kHalf) =
+          *reinterpret_cast<uint2*>(rows + (kept + r) * D + (h ? at0.hi : at0.lo)) =
               make_uint2(q8::float4_to_codes<kCode>(x + 8 * h), q8::float4_to_codes<kCode>(x + 8 * h + 4));
     }
     __syncwarp();   // every lane has read the scale
@@ -469,32 +525,37 @@ struct Span {
   size_t bytes;
 };
 
-// type: kBinary16 or an ANVILQ_KV_Q8_* code type (scales then given)
+// type: kBinary16 or an ANVILQ_KV_Q8_* code type (scales then given); rope null: by theta
 static int run(const uint16_t* qkv, long long stride, const int32_t* starts, const int32_t* seqlens,
                const uint32_t* page_table, uint16_t* q_out, void* k, void* v, float* k_scales, float* v_scales,
                int type, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages, int num_pages,
-               float theta, int* dev_err, unsigned flags, cudaStream_t st) {
+               float theta, const Rope* rope, int* dev_err, unsigned flags, cudaStream_t st) {
   if ((T != 0 && (!qkv || !q_out)) || !starts || !seqlens || !page_table || !k || !v || !dev_err) return ANVILQ_EINVAL;
   if (type != kBinary16 && (!k_scales || !v_scales)) return ANVILQ_EINVAL;
   if (flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) return ANVILQ_EINVAL;
-  if (T < 0 || B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || !(theta > 0.0f) || !std::isfinite(theta))
+  if (T < 0 || B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv) return ANVILQ_EINVAL;
+  if (rope ? !rope->inv || (rope->pairs != 0 && rope->pairs != 1) || !(rope->factor > 0.0f && rope->factor <= kMaxFactor)
+           : !(theta > 0.0f) || !std::isfinite(theta))
     return ANVILQ_EINVAL;
   if (type != kBinary16 && type != q8::kInt8 && type != q8::kE4m3) return ANVILQ_EINVAL;
   if ((D != 64 && D != 128) || page_tokens < kBlock || page_tokens % kBlock || max_pages < 1 || num_pages < 1 ||
       (long long)page_tokens * max_pages > (1LL << 30) || B > (1 << 24) || Hq > (1 << 16) || T > (1 << 30))
     return ANVILQ_ESHAPE;
+  if (rope && (rope->dims < 16 || rope->dims % 16 || rope->dims > D)) return ANVILQ_ESHAPE;
   const int heads = Hq + 2 * Hkv;
   if (stride < (long long)heads * D) return ANVILQ_EINVAL;
   const long long positions = (long long)num_pages * page_tokens;
   if (positions > (1LL << 40) / Hkv) return ANVILQ_ESHAPE;
   if (!a16(qkv) || !a16(q_out) || !a16(k) || !a16(v) || stride % 8) return ANVILQ_EALIGN;
+  if (rope && (reinterpret_cast<uintptr_t>(rope->inv) & 7u)) return ANVILQ_EALIGN;
   if (T == 0) return ANVILQ_OK;
   // an item's q is written while others' rows are still to be read, and every pool by
   // warps of its own
   const size_t pool = (size_t)positions * Hkv * D * (type == kBinary16 ? 2 : 1);
   const size_t scales = type == kBinary16 ? 0 : (size_t)positions / kBlock * Hkv * sizeof(float);
   const Span spans[] = {{qkv, ((size_t)(T - 1) * stride + (size_t)heads * D) * 2}, {q_out, (size_t)T * Hq * D * 2},
-                        {k, pool}, {v, pool}, {k_scales, scales}, {v_scales, scales}};
+                        {k, pool}, {v, pool}, {k_scales, scales}, {v_scales, scales},
+                        {rope ? rope->inv : nullptr, rope ? (size_t)rope->dims * 4 : 0}};
   for (const Span& a : spans)
     for (const Span* b = &a + 1; b != std::end(spans); ++b)
       if (overlap(a.start, a.bytes, b->start, b->bytes)) return ANVILQ_EINVAL;
@@ -531,7 +592,9 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   thread_local Freq freq;
   thread_local float freq_theta = 0.0f;
   thread_local int freq_d = 0;
-  if (theta != freq_theta || D != freq_d) {
+  if (rope) {
+    p.rope = *rope;
+  } else if (theta != freq_theta || D != freq_d) {
     for (int i = 0; i < D / 2; ++i) freq.inv[i] = std::pow((double)theta, -2.0 * i / D);
     freq_theta = theta;
     freq_d = D;
@@ -543,13 +606,19 @@ static int run(const uint16_t* qkv, long long stride, const int32_t* starts, con
   // against 50.3, of two 30.2 against 58.  It takes 10 % longer where items are full (4096
   // tokens of one sequence 44.2 against 38.6), though those items go the same way in both.
   const bool few = T <= 2LL * B;
-  if (type == kBinary16)
-    return D == 64 ? go(append_kernel<64, kBinary16, false>) : go(append_kernel<128, kBinary16, false>);
-  if (D == 64)
-    return type == q8::kInt8 ? (few ? go(append_kernel<64, q8::kInt8, true>) : go(append_kernel<64, q8::kInt8, false>))
-                             : (few ? go(append_kernel<64, q8::kE4m3, true>) : go(append_kernel<64, q8::kE4m3, false>));
-  return type == q8::kInt8 ? (few ? go(append_kernel<128, q8::kInt8, true>) : go(append_kernel<128, q8::kInt8, false>))
-                           : (few ? go(append_kernel<128, q8::kE4m3, true>) : go(append_kernel<128, q8::kE4m3, false>));
+  auto by = [&](auto d, auto rotation) {
+    constexpr int kD = decltype(d)::value;
+    constexpr int kRope = decltype(rotation)::value;
+    if (type == kBinary16) return go(append_kernel<kD, kBinary16, false, kRope>);
+    if (type == q8::kInt8)
+      return few ? go(append_kernel<kD, q8::kInt8, true, kRope>) : go(append_kernel<kD, q8::kInt8, false, kRope>);
+    return few ? go(append_kernel<kD, q8::kE4m3, true, kRope>) : go(append_kernel<kD, q8::kE4m3, false, kRope>);
+  };
+  auto dims = [&](auto d) {
+    if (!rope) return by(d, std::integral_constant<int, kTheta>{});
+    return rope->pairs ? by(d, std::integral_constant<int, kPairs>{}) : by(d, std::integral_constant<int, kHalves>{});
+  };
+  return D == 64 ? dims(std::integral_constant<int, 64>{}) : dims(std::integral_constant<int, 128>{});
 }
 
 }  // namespace append
@@ -563,7 +632,19 @@ int anvilq_paged_kv_append(const uint16_t* qkv, long long qkv_stride, const int3
                            int num_pages, float theta, int* dev_err, unsigned flags, anvilq_stream_t stream) {
   using namespace anvilq::append;
   return run(qkv, qkv_stride, token_starts, seqlens, page_table, q_out, k_pool, v_pool, nullptr, nullptr, kBinary16,
-             T, B, Hq, Hkv, D, page_tokens, max_pages, num_pages, theta, dev_err, flags,
+             T, B, Hq, Hkv, D, page_tokens, max_pages, num_pages, theta, nullptr, dev_err, flags,
+             reinterpret_cast<cudaStream_t>(stream));
+}
+
+int anvilq_paged_kv_append_rope(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
+                                const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, uint16_t* k_pool,
+                                uint16_t* v_pool, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages,
+                                int num_pages, const double* inv_freq, int rotary_dim, int interleaved, float factor,
+                                int* dev_err, unsigned flags, anvilq_stream_t stream) {
+  using namespace anvilq::append;
+  const Rope rope{inv_freq, rotary_dim, interleaved, factor};
+  return run(qkv, qkv_stride, token_starts, seqlens, page_table, q_out, k_pool, v_pool, nullptr, nullptr, kBinary16,
+             T, B, Hq, Hkv, D, page_tokens, max_pages, num_pages, 0.0f, &rope, dev_err, flags,
              reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -575,7 +656,21 @@ int anvilq_paged_kv_append_q8(const uint16_t* qkv, long long qkv_stride, const i
   using namespace anvilq::append;
   if (code_type != ANVILQ_KV_Q8_INT8 && code_type != ANVILQ_KV_Q8_E4M3) return ANVILQ_EINVAL;
   return run(qkv, qkv_stride, token_starts, seqlens, page_table, q_out, k_codes, v_codes, k_scales, v_scales,
-             code_type, T, B, Hq, Hkv, D, page_tokens, max_pages, num_pages, theta, dev_err, flags,
+             code_type, T, B, Hq, Hkv, D, page_tokens, max_pages, num_pages, theta, nullptr, dev_err, flags,
+             reinterpret_cast<cudaStream_t>(stream));
+}
+
+int anvilq_paged_kv_append_q8_rope(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
+                                   const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, void* k_codes,
+                                   void* v_codes, float* k_scales, float* v_scales, int code_type, int T, int B,
+                                   int Hq, int Hkv, int D, int page_tokens, int max_pages, int num_pages,
+                                   const double* inv_freq, int rotary_dim, int interleaved, float factor,
+                                   int* dev_err, unsigned flags, anvilq_stream_t stream) {
+  using namespace anvilq::append;
+  if (code_type != ANVILQ_KV_Q8_INT8 && code_type != ANVILQ_KV_Q8_E4M3) return ANVILQ_EINVAL;
+  const Rope rope{inv_freq, rotary_dim, interleaved, factor};
+  return run(qkv, qkv_stride, token_starts, seqlens, page_table, q_out, k_codes, v_codes, k_scales, v_scales,
+             code_type, T, B, Hq, Hkv, D, page_tokens, max_pages, num_pages, 0.0f, &rope, dev_err, flags,
              reinterpret_cast<cudaStream_t>(stream));
 }
 

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import threading
 
 import torch
@@ -726,8 +727,60 @@ def _check_append(name, qkv, Hq, Hkv, D, page_table, seqlens, token_starts, q_ou
     return T, B, max_pages, (stride if T > 1 else width), q_out
 
 
+def rope_frequencies(rotary_dim: int, theta: float = 1e6, scaling: dict | None = None, device="cuda"):
+    """(inv_freq float64 [rotary_dim / 2] on `device`, rope_factor) for the appends' rotation:
+    theta^(-2i / rotary_dim), for contexts beyond the trained one scaled by `scaling`:
+      {"kind": "linear", "factor": s}   every frequency divided by s (position interpolation);
+      {"kind": "ntk", "factor": s}      theta raised so that the slowest pair turns s times slower;
+      {"kind": "yarn", "factor": s, "original": n, "fast": 32, "slow": 1}   (Peng et al. 2023) pairs of over
+          `fast` turns in n tokens stay, those of less than `slow` are divided by s, a ramp over the pairs
+          between; rope_factor 0.1 ln(s) + 1;
+      {"kind": "bands", "factor": s, "original": n, "low": 1, "high": 4}   the same with limits on n over the
+          wavelength, a ramp over that, rope_factor 1.
+    Computed on the host, once; not for a graph's capture."""
+    R = int(rotary_dim)
+    if R < 2 or R % 2 or not (theta > 1.0 and math.isfinite(theta)):
+        raise ValueError("rope_frequencies: an even rotary_dim and a finite theta above 1 expected")
+    known = {"linear": (), "ntk": (), "yarn": ("original", "fast", "slow"), "bands": ("original", "low", "high")}
+    scaling = dict(scaling or {"kind": "linear", "factor": 1.0})
+    kind, s = scaling.pop("kind", None), float(scaling.pop("factor", 0.0))
+    if kind not in known or set(scaling) - set(known[kind]) or not (s >= 1.0 and math.isfinite(s)):
+        raise ValueError(f"rope_frequencies: kind one of {list(known)}, its own options and a factor >= 1 expected")
+    inv, factor = [float(theta) ** (-2.0 * i / R) for i in range(R // 2)], 1.0
+    if kind == "linear":
+        inv = [f / s for f in inv]
+    elif kind == "ntk":
+        base = float(theta) * s ** (R / (R - 2)) if R > 2 else float(theta)
+        inv = [base ** (-2.0 * i / R) for i in range(R // 2)]
+    else:
+        n = float(scaling.get("original", 0))
+        least, most = ((float(scaling.get("slow", 1)), float(scaling.get("fast", 32))) if kind == "yarn" else
+                       (float(scaling.get("low", 1)), float(scaling.get("high", 4))))
+        if n < 1 or not 0 < least < most:
+            raise ValueError("rope_frequencies: original >= 1 and limits with 0 < lower < upper expected")
+        if kind == "yarn":
+            at = lambda turns: R * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(theta))
+            lo, hi = max(0, math.floor(at(most))), min(R // 2 - 1, math.ceil(at(least)))
+            slow = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(R // 2)]
+            factor = 0.1 * math.log(s) + 1.0
+        else:
+            slow = [1.0 - min(1.0, max(0.0, (n * f / (2 * math.pi) - least) / (most - least))) for f in inv]
+        inv = [f * (1.0 - w) + f / s * w for f, w in zip(inv, slow)]
+    return torch.tensor(inv, dtype=torch.float64, device=device), factor
+
+
+def _check_rope(name, inv_freq, D):
+    R = 2 * inv_freq.numel()
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError(f"{name}: inv_freq must be a contiguous float64 vector")
+    if R < 16 or R % 16 or R > D:
+        raise ValueError(f"{name}: inv_freq turns {R} dims: a multiple of 16, at most {D}, expected")
+    return R
+
+
 def paged_kv_append(qkv, k_pool, v_pool, page_table, seqlens, token_starts, Hq: int, theta: float = 1e6, q_out=None,
-                    dev_err=None, overlap_prior: bool = False):
+                    dev_err=None, overlap_prior: bool = False, inv_freq=None, interleaved: bool = False,
+                    rope_factor: float = 1.0):
     """Append the new tokens of a ragged batch to a paged fp16 cache, rotating q and
     k on the way.  qkv fp16 [T, (Hq + 2 Hkv) D] (rows may be strided) holds the new
     tokens' [q | k | v] rows, sequence after sequence: those of sequence b are rows
@@ -735,6 +788,11 @@ def paged_kv_append(qkv, k_pool, v_pool, page_table, seqlens, token_starts, Hq: 
     (int32 [B]) counting them already.  Pools and page_table as for
     ``gqa_decode_paged``, written in place.  Returns the rotated q, fp16 [T, Hq, D]
     (rows of no sequence are left as they are).
+
+    inv_freq (float64 [R / 2] on the device, ``rope_frequencies``): only the first R dims
+    of a head are rotated, pair i at position p by fp32(p * inv_freq[i]), theta unused;
+    pairs are dims (i, i + R / 2), or (2i, 2i + 1) with interleaved; cosines and sines are
+    multiplied by rope_factor.
 
     The rotation and cache write of FP32Model.token (anvil-q1/tests/official_weights.py:439-449,
     466-470) for many tokens, over the Anvil-Q4 page table (anvil-q4/design/SPEC.md:205-208);
@@ -749,6 +807,16 @@ def paged_kv_append(qkv, k_pool, v_pool, page_table, seqlens, token_starts, Hq: 
     dev = qkv.device
     _on_device(name, dev, k_pool, v_pool, page_table, seqlens, token_starts, q_out)
     err = _error_word(dev, dev_err)
+    if inv_freq is not None:
+        R = _check_rope(name, inv_freq, D)
+        _on_device(name, dev, inv_freq)
+        _call("anvilq_paged_kv_append_rope", dev, qkv.data_ptr(), stride, token_starts.data_ptr(), seqlens.data_ptr(),
+              page_table.data_ptr(), q_out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), T, B, Hq, Hkv, D, page,
+              max_pages, pages, inv_freq.data_ptr(), R, 1 if interleaved else 0, float(rope_factor), err.data_ptr(),
+              GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+        return q_out
+    if interleaved or rope_factor != 1.0:
+        raise ValueError(f"{name}: interleaved and rope_factor come with inv_freq")
     _call("anvilq_paged_kv_append", dev, qkv.data_ptr(), stride, token_starts.data_ptr(), seqlens.data_ptr(),
           page_table.data_ptr(), q_out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), T, B, Hq, Hkv, D, page,
           max_pages, pages, float(theta), err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
@@ -756,20 +824,32 @@ def paged_kv_append(qkv, k_pool, v_pool, page_table, seqlens, token_starts, Hq: 
 
 
 def paged_kv_append_q8(qkv, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, token_starts, Hq: int,
-                       theta: float = 1e6, q_out=None, dev_err=None, overlap_prior: bool = False):
+                       theta: float = 1e6, q_out=None, dev_err=None, overlap_prior: bool = False, inv_freq=None,
+                       interleaved: bool = False, rope_factor: float = 1.0):
     """``paged_kv_append`` into 8-bit pages: codes int8 or float8_e4m3fn
     [num_pages, Hkv, page_tokens, D], scales float32 [num_pages, Hkv, page_tokens / 16],
     one for each block of 16 tokens and head, all written in place.  A block's scale
     fits its largest value; when a later token of the block needs a larger one, the
     block's earlier codes are rounded again to it (anvilq_paged_kv_append_q8 in
     include/anvilq.h has the formulas).  Values that are not finite set a device error
-    and are stored as 0."""
+    and are stored as 0.  inv_freq, interleaved, rope_factor: as for ``paged_kv_append``."""
     name = "paged_kv_append_q8"
     pages, Hkv, page, D, code = _check_q8(name, k_codes, v_codes, k_scales, v_scales)
     T, B, max_pages, stride, q_out = _check_append(name, qkv, Hq, Hkv, D, page_table, seqlens, token_starts, q_out)
     dev = qkv.device
     _on_device(name, dev, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, token_starts, q_out)
     err = _error_word(dev, dev_err)
+    if inv_freq is not None:
+        R = _check_rope(name, inv_freq, D)
+        _on_device(name, dev, inv_freq)
+        _call("anvilq_paged_kv_append_q8_rope", dev, qkv.data_ptr(), stride, token_starts.data_ptr(),
+              seqlens.data_ptr(), page_table.data_ptr(), q_out.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(),
+              k_scales.data_ptr(), v_scales.data_ptr(), code, T, B, Hq, Hkv, D, page, max_pages, pages,
+              inv_freq.data_ptr(), R, 1 if interleaved else 0, float(rope_factor), err.data_ptr(),
+              GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+        return q_out
+    if interleaved or rope_factor != 1.0:
+        raise ValueError(f"{name}: interleaved and rope_factor come with inv_freq")
     _call("anvilq_paged_kv_append_q8", dev, qkv.data_ptr(), stride, token_starts.data_ptr(), seqlens.data_ptr(),
           page_table.data_ptr(), q_out.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(),
           v_scales.data_ptr(), code, T, B, Hq, Hkv, D, page, max_pages, pages, float(theta), err.data_ptr(),

@@ -690,6 +690,28 @@ int anvilq_paged_kv_append_q8(const uint16_t* qkv, long long qkv_stride, const i
                               int Hkv, int D, int page_tokens, int max_pages, int num_pages, float theta,
                               int* dev_err, unsigned flags, anvilq_stream_t stream);
 
+/* The two appends with frequencies of the caller's: of every q and k head the first
+ * rotary_dim dims R are rotated, the others are copied.  Pair i (0 <= i < R / 2) is
+ * dims (i, i + R / 2), or with interleaved = 1 dims (2 i, 2 i + 1); at position p its
+ * angle is fp32(p * inv_freq[i]) (binary64 product), and
+ *   (a, b) -> (a c - b s, b c + a s),  c = factor * cos(angle), s = factor * sin(angle)
+ * (binary32, each operation rounded).  inv_freq: device double [R / 2], 8-byte
+ * aligned, apart from what the call writes; it is read when the call runs, after the
+ * preceding work on the stream.  R % 16 == 0, 16 <= R <= D; 0 < factor <= 65536.  With
+ * inv_freq[i] = theta^(-2i/D), R = D and factor 1 this is the append by theta, bit for
+ * bit.  All else as above. */
+int anvilq_paged_kv_append_rope(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
+                                const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, uint16_t* k_pool,
+                                uint16_t* v_pool, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages,
+                                int num_pages, const double* inv_freq, int rotary_dim, int interleaved, float factor,
+                                int* dev_err, unsigned flags, anvilq_stream_t stream);
+int anvilq_paged_kv_append_q8_rope(const uint16_t* qkv, long long qkv_stride, const int32_t* token_starts,
+                                   const int32_t* seqlens, const uint32_t* page_table, uint16_t* q_out, void* k_codes,
+                                   void* v_codes, float* k_scales, float* v_scales, int code_type, int T, int B,
+                                   int Hq, int Hkv, int D, int page_tokens, int max_pages, int num_pages,
+                                   const double* inv_freq, int rotary_dim, int interleaved, float factor,
+                                   int* dev_err, unsigned flags, anvilq_stream_t stream);
+
 /* The values of whole 8-bit pools in binary16: out[page][head][token][d] =
  * fp16(code * scale), same layout as the codes (to move pages into binary16, or
  * to look at them).  16-byte aligned codes and outputs, which do not overlap. */
