@@ -80,6 +80,13 @@ SIGNATURES = {
     "anvilq_logits_process_workspace_size": (SZ, [I, I]),
     "anvilq_logits_process": (I, [P, I, LL, P, LL, P, I, I, P, LL, P, P, I, P, P, P, P, P, P, I, P, LL, P, I, P, SZ, P,
                                   ctypes.c_uint, P]),
+    "anvilq_pages_fork": (I, [P, P, P, P, I, I, I, I, I, P, ctypes.c_uint, P]),
+    "anvilq_pages_reserve_workspace_size": (SZ, [I, I]),
+    "anvilq_pages_reserve": (I, [P, P, P, P, P, P, I, I, I, I, I, P, SZ, P, ctypes.c_uint, P]),
+    "anvilq_pages_release": (I, [P, P, P, I, I, I, I, P, ctypes.c_uint, P]),
+    "anvilq_pages_compact_workspace_size": (SZ, [I]),
+    "anvilq_pages_compact": (I, [P, P, P, P, P, P, I, I, I, I, I, P, SZ, P, ctypes.c_uint, P]),
+    "anvilq_pages_copy": (I, [P, I, P, P, P, P, I, I, I, P, ctypes.c_uint, P]),
     "anvilq_tree_attention_workspace_size": (SZ, [I, I, I, I, I]),
     "anvilq_tree_attention": (I, [P, P, P, P, I, P, I, I, I, I, I, F, P, SZ, P, P]),
     "anvilq_rmsnorm_rows": (I, [P, P, F, P, I, I, ctypes.c_uint, P]),
@@ -104,6 +111,11 @@ class GemvPlan(ctypes.Structure):
 
     def as_dict(self):
         return {name: getattr(self, name) for name, _ in self._fields_}
+
+
+class PagePool(ctypes.Structure):
+    """anvilq_page_pool: how a page lies in a pool."""
+    _fields_ = [("base", P), ("segments", I), ("segment_bytes", I), ("unit_tokens", I)]
 
 
 _lib = None

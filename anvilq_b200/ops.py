@@ -77,6 +77,8 @@ def raise_device_errors(device=None):
             what.append("legacy cache block with a forbidden code, padding or metadata")
         if value & 256:
             what.append("tensor of a layer table that is not 16-byte aligned")
+        if value & 512:
+            what.append("fewer free pages than a call needs")
         raise _lib.AnvilqError(f"device error bits 0x{value:x}: " + "; ".join(what))
 
 
@@ -1029,3 +1031,191 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
           n_bias, _ptr(allowed), mask_pitch, _ptr(allowed_rows), masks, _ptr(ws), 0 if ws is None else ws.numel(),
           _ptr(err), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return out, tokens
+
+
+# ---- pages that sequences share ----------------------------------------------------
+
+class PagePools:
+    """The tensors of a paged cache whose pages the calls below copy: for every layer the
+    pair of float16 pools [num_pages, page_tokens, Hkv, D], or of 8-bit codes [num_pages,
+    Hkv, page_tokens, D] with their float32 scales [num_pages, Hkv, page_tokens / 16], in
+    any order.  A program that keeps its pools keeps one of these; the calls also take a
+    plain list of tensors and check it each time."""
+
+    def __init__(self, pools, page_tokens: int):
+        name = "PagePools"
+        self.pools, self.page_tokens = list(pools), int(page_tokens)
+        self.num_pages = self.device = self.array = None
+        n, pt = len(self.pools), self.page_tokens
+        if not n:
+            return
+        self.num_pages, self.device = self.pools[0].shape[0], self.pools[0].device
+        index, known = self.pools[0].get_device(), {}     # (type, shape) -> how its pages lie
+        if index < 0:
+            raise ValueError(f"{name}: pools must be on a CUDA device")
+        self.array = (_lib.PagePool * n)()
+        for a, t in zip(self.array, self.pools):
+            kind = (t.dtype, t.shape)
+            how = known.get(kind)
+            if how is None:
+                how = known[kind] = self._layout(name, t, pt)
+            if not t.is_contiguous() or t.get_device() != index:
+                raise ValueError(f"{name}: pools must be contiguous and on one device")
+            a.base = t.data_ptr()
+            a.segments, a.segment_bytes, a.unit_tokens = how
+
+    def _layout(self, name, t, pt):
+        shape = tuple(t.shape)
+        if t.dtype == torch.float16 and len(shape) == 4 and shape[1] == pt:
+            how = 1, pt * shape[2] * shape[3] * 2, 1
+        elif t.dtype in (torch.int8, torch.float8_e4m3fn) and len(shape) == 4 and shape[2] == pt:
+            how = shape[1], pt * shape[3], 1
+        elif t.dtype == torch.float32 and len(shape) == 3 and shape[2] * _lib.KV_Q8_BLOCK == pt:
+            how = shape[1], shape[2] * 4, _lib.KV_Q8_BLOCK
+        else:
+            raise ValueError(f"{name}: {t.dtype} {list(shape)} is no pool of pages of {pt} tokens")
+        if shape[0] != self.num_pages or 0 in shape:
+            raise ValueError(f"{name}: all pools must hold the same number of pages")
+        return how
+
+
+def _page_pools(name, pools, page_tokens, device, num_pages):
+    p = pools if isinstance(pools, PagePools) else PagePools(pools, page_tokens)
+    if p.page_tokens != page_tokens:
+        raise ValueError(f"{name}: the pools' pages hold {p.page_tokens} tokens, not {page_tokens}")
+    if p.array is not None and (p.device != device or p.num_pages != num_pages):
+        raise ValueError(f"{name}: pools of {num_pages} pages on {device} expected")
+    return p
+
+
+def _check_pages(name, page_table, refs, *vectors):
+    """(rows, max_pages, num_pages, device) of a table, the pages' counts and int32 vectors of a row each."""
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+        raise ValueError(f"{name}: page_table must be a contiguous int32 tensor [rows, max_pages]")
+    if refs.dtype != torch.int32 or refs.dim() != 1 or not refs.is_contiguous():
+        raise ValueError(f"{name}: refs must be a contiguous int32 tensor [num_pages]")
+    rows, max_pages = page_table.shape
+    for t in vectors:
+        if t.dtype != torch.int32 or t.shape != (rows,) or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous int32 tensors [{rows}] expected")
+    dev = page_table.device
+    _on_device(name, dev, refs, *vectors)
+    return rows, max_pages, refs.shape[0], dev
+
+
+def pages_fork(page_table, refs, parents, out=None, dev_err=None, overlap_prior: bool = False):
+    """Rows of a page table by their parents, as beams go on: out[n] = page_table[parents[n]],
+    an empty row for -1; refs (int32 [num_pages], how many entries of all tables name a page,
+    0: free) follows, the rows of page_table being given up.  parents int32 [new_rows], or
+    [items, N] naming rows of their own item (page_table then has items * K rows, as
+    ``beam_select`` gives them).  Returns out, int32 [new_rows, max_pages]; it shares all
+    pages, also half-filled ones: ``pages_reserve`` before the next tokens are written."""
+    name = "pages_fork"
+    rows, max_pages, pages, dev = _check_pages(name, page_table, refs)
+    if parents.dtype != torch.int32 or parents.dim() not in (1, 2) or not parents.is_contiguous():
+        raise ValueError(f"{name}: parents must be contiguous int32 [new_rows] or [items, N]")
+    new_rows, groups = parents.numel(), parents.shape[0] if parents.dim() == 2 else 1
+    if groups < 1 or rows % groups:
+        raise ValueError(f"{name}: {rows} rows for {groups} items")
+    if out is None:
+        out = page_table.new_empty((new_rows, max_pages))
+    elif out.dtype != torch.int32 or out.shape != (new_rows, max_pages) or not out.is_contiguous():
+        raise ValueError(f"{name}: out must be contiguous int32 [{new_rows}, {max_pages}]")
+    _on_device(name, dev, parents, out)
+    err = _error_word(dev, dev_err)
+    _call("anvilq_pages_fork", dev, page_table.data_ptr(), out.data_ptr(), refs.data_ptr(), parents.data_ptr(), rows,
+          new_rows, groups, max_pages, pages, err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0,
+          _stream_ptr(dev))
+    return out
+
+
+def pages_reserve(page_table, refs, before, after, page_tokens: int, pools, lacking=None, dev_err=None,
+                  workspace=None, overlap_prior: bool = False):
+    """Make the positions before[b] .. after[b] (int32 [rows]) of every row writable, in place:
+    absent pages are allocated, the lowest free ones first, and pages that other entries
+    name too are replaced by new ones, their rows below before[b] copied in all `pools` (a
+    ``PagePools`` or a list of tensors: all that this table pages).  Returns lacking, int32
+    [1]: 0, or how many free pages were missing; nothing has changed then, and a device
+    error is set.  workspace: as for ``gqa_decode_q8``."""
+    name = "pages_reserve"
+    rows, max_pages, pages, dev = _check_pages(name, page_table, refs, before, after)
+    p = _page_pools(name, pools, page_tokens, dev, pages)
+    if lacking is None:
+        lacking = refs.new_empty(1)
+    elif lacking.dtype != torch.int32 or lacking.numel() < 1 or lacking.device != dev:
+        raise ValueError(f"{name}: lacking must be an int32 tensor on {dev}")
+    need = _lib.load().anvilq_pages_reserve_workspace_size(rows, pages)
+    ws = _call_workspace(dev, need, workspace)
+    err = _error_word(dev, dev_err)
+    _call("anvilq_pages_reserve", dev, page_table.data_ptr(), refs.data_ptr(), before.data_ptr(), after.data_ptr(),
+          lacking.data_ptr(), p.array, len(p.pools), rows, page_tokens, max_pages, pages, ws.data_ptr(), ws.numel(),
+          err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    return lacking
+
+
+def pages_release(page_table, refs, keep, page_tokens: int, dev_err=None, overlap_prior: bool = False):
+    """Drop the entries behind every row's first keep[b] tokens (int32 [rows], 0: the whole
+    row), in place: sequences that ended, drafts that were rejected."""
+    name = "pages_release"
+    rows, max_pages, pages, dev = _check_pages(name, page_table, refs, keep)
+    err = _error_word(dev, dev_err)
+    _call("anvilq_pages_release", dev, page_table.data_ptr(), refs.data_ptr(), keep.data_ptr(), rows, page_tokens,
+          max_pages, pages, err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+
+
+def pages_compact(page_table, refs, pools, page_tokens: int | None = None, out=None, out_refs=None, used=None,
+                  dev_err=None, workspace=None, overlap_prior: bool = False):
+    """Bring the n pages in use to the front of all `pools`: those at n and above move, in
+    order, to the free ones below n.  page_table has to hold every entry over the pool.
+    Returns (out, out_refs, used): the table and counts after it (by default in place) and
+    n, int32 [1].  page_tokens: needed with an empty list of pools only."""
+    name = "pages_compact"
+    rows, max_pages, pages, dev = _check_pages(name, page_table, refs)
+    if page_tokens is None:
+        if isinstance(pools, PagePools):
+            page_tokens = pools.page_tokens
+        elif pools:
+            t = pools[0]
+            page_tokens = t.shape[1] if t.dtype == torch.float16 else \
+                t.shape[2] * (1 if t.dim() == 4 else _lib.KV_Q8_BLOCK) if t.dim() > 2 else 1
+        else:
+            raise ValueError(f"{name}: page_tokens or pools expected")
+    p = _page_pools(name, pools, page_tokens, dev, pages)
+    out, out_refs = page_table if out is None else out, refs if out_refs is None else out_refs
+    used = refs.new_empty(1) if used is None else used
+    for t, like in ((out, page_table), (out_refs, refs)):
+        if t.dtype != torch.int32 or t.shape != like.shape or not t.is_contiguous():
+            raise ValueError(f"{name}: out and out_refs must be contiguous int32 {list(like.shape)}")
+    if used.dtype != torch.int32 or used.numel() < 1:
+        raise ValueError(f"{name}: used must be an int32 tensor")
+    _on_device(name, dev, out, out_refs, used)
+    ws = _call_workspace(dev, _lib.load().anvilq_pages_compact_workspace_size(pages), workspace)
+    err = _error_word(dev, dev_err)
+    _call("anvilq_pages_compact", dev, page_table.data_ptr(), out.data_ptr(), refs.data_ptr(), out_refs.data_ptr(),
+          used.data_ptr(), p.array, len(p.pools), rows, page_tokens, max_pages, pages, ws.data_ptr(), ws.numel(),
+          err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    return out, out_refs, used
+
+
+def pages_copy(pools, src, dst, page_tokens: int, rows=None, count=None, dev_err=None, overlap_prior: bool = False):
+    """Copy page src[i] onto page dst[i] (int32 [n]) in all `pools`: its first rows[i] tokens
+    (int32 [n]; None or negative: all), for i < count[0] (int32 [1]; None: n).  Pairs with a
+    negative page are passed over.  No page may be a destination twice, nor both source
+    and destination."""
+    name = "pages_copy"
+    p = _page_pools(name, pools, page_tokens, src.device, pools.num_pages if isinstance(pools, PagePools) else
+                    pools[0].shape[0] if pools else 0)
+    if src.dtype != torch.int32 or src.dim() != 1 or not src.is_contiguous():
+        raise ValueError(f"{name}: src must be a contiguous int32 vector")
+    n, dev = src.shape[0], src.device
+    for t in (dst, rows):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError(f"{name}: dst and rows must be contiguous int32 [{n}]")
+    if count is not None and (count.dtype != torch.int32 or count.numel() < 1):
+        raise ValueError(f"{name}: count must be an int32 tensor")
+    _on_device(name, dev, src, dst, rows, count)
+    if p.array is None:
+        return
+    err = _error_word(dev, dev_err)
+    _call("anvilq_pages_copy", dev, p.array, len(p.pools), src.data_ptr(), dst.data_ptr(), _ptr(rows), _ptr(count), n,
+          page_tokens, p.num_pages, err.data_ptr(), GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))

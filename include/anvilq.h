@@ -59,6 +59,7 @@ typedef struct CUstream_st* anvilq_stream_t; /* same type as cudaStream_t */
 #define ANVILQ_DEV_ERR_TREE 64     /* a draft node's ancestor mask broke the tree contract */
 #define ANVILQ_DEV_ERR_CODEC 128   /* a legacy cache block held a forbidden code, padding or metadata */
 #define ANVILQ_DEV_ERR_ALIGN 256   /* a tensor named by a device-side table was not 16-byte aligned */
+#define ANVILQ_DEV_ERR_NOPAGE 512  /* a paged cache had fewer free pages than a call needed */
 
 /* Workspace layout shared by every entry point that takes one: the first
  * ANVILQ_WORKSPACE_COUNTER_BYTES hold arrival counters that must be zero
@@ -783,6 +784,85 @@ int anvilq_logits_process(const void* logits, int logits_half, long long logits_
                           int bias_total, const uint32_t* allowed, long long allowed_stride,
                           const int32_t* allowed_rows, int masks, void* workspace, size_t workspace_bytes,
                           int* dev_err, unsigned flags, anvilq_stream_t stream);
+
+/* ---- pages that sequences share -----------------------------------------------
+ *
+ * Beams of a search, several answers to one prompt, prompts with a common start:
+ * rows of page tables that name the same pages.  The state is the tables (uint32,
+ * bit 31 valid, bits 30:0 the page, as everywhere) and refs int32 [num_pages]: how
+ * many entries of all tables over the pool name a page, 0 for a free one.  All of it
+ * lies on the device and the calls read nothing back; each can be captured.  An entry
+ * that names a page >= num_pages sets ANVILQ_DEV_ERR_PAGE and is passed over (by the
+ * fork dropped), as is a page whose count is less than its entries.  Tables hold at most
+ * 16384 rows and 2^30 entries; arrays are apart from each other, workspace included,
+ * unless said otherwise.  flags: ANVILQ_GEMM_OVERLAP_PRIOR.  No counterpart in the
+ * reference, whose page table (anvil-q4/design/SPEC.md:205-208) has one owner.
+ *
+ * A pool that the calls copy pages in: a page is `segments` runs of segment_bytes, each
+ * of them the page's tokens in order, unit_tokens tokens in every piece of
+ *   segment_bytes / (page_tokens / unit_tokens)  bytes (a multiple of 4);
+ * base 4-byte aligned (16 is faster), a page at most 2^31 - 1 bytes.
+ *   binary16 [num_pages][page_tokens][Hkv][D]:          1,   2 page_tokens Hkv D,  1
+ *   8-bit codes [num_pages][Hkv][page_tokens][D]:       Hkv, page_tokens D,        1
+ *   their scales [num_pages][Hkv][page_tokens / 16]:    Hkv, page_tokens / 4,      16 */
+typedef struct anvilq_page_pool {
+  void* base;          /* device */
+  int segments;
+  int segment_bytes;
+  int unit_tokens;
+} anvilq_page_pool;    /* arrays of these are host memory, read before the call returns */
+
+/* out[n] = the row parents[n] of page_table, an empty row for parents[n] = -1; refs
+ * follows: + the entries of out, - the entries of page_table, whose rows are then
+ * given up.  page_table [old_rows], out [new_rows] rows of max_pages entries; rows
+ * are in `groups` equal groups and parents name rows of their own group (1 group: any
+ * row).  A parent outside [-1, old_rows / groups) sets ANVILQ_DEV_ERR_SEQLEN and
+ * counts as -1. */
+int anvilq_pages_fork(const uint32_t* page_table, uint32_t* out, int32_t* refs, const int32_t* parents, int old_rows,
+                      int new_rows, int groups, int max_pages, int num_pages, int* dev_err, unsigned flags,
+                      anvilq_stream_t stream);
+
+/* Makes the positions before[b] .. after[b] of every row b writable (nothing where
+ * after[b] <= before[b]; the two arrays may overlap): entries of theirs that are
+ * absent get a new page, entries whose page other entries name too get a new one, to
+ * which the page's rows below before[b] are copied in every pool.  Entries ask
+ * in (row, index) order and get the lowest free pages in order; where all entries
+ * that name a page ask for it, the last of them keeps it.  With too few free pages
+ * nothing changes, ANVILQ_DEV_ERR_NOPAGE is set and *lacking (device) is how many
+ * were missing, else 0.  before < 0 or after > page_tokens * max_pages (at most
+ * 2^30) sets ANVILQ_DEV_ERR_SEQLEN, the row is passed over.  workspace: 16-byte
+ * aligned, anvilq_pages_reserve_workspace_size bytes, layout as described at
+ * ANVILQ_WORKSPACE_COUNTER_BYTES. */
+size_t anvilq_pages_reserve_workspace_size(int rows, int num_pages);
+int anvilq_pages_reserve(uint32_t* page_table, int32_t* refs, const int32_t* before, const int32_t* after,
+                         int32_t* lacking, const anvilq_page_pool* pools, int pool_count, int rows, int page_tokens,
+                         int max_pages, int num_pages, void* workspace, size_t workspace_bytes, int* dev_err,
+                         unsigned flags, anvilq_stream_t stream);
+
+/* Drops the entries of every row b behind its first keep[b] tokens (0: all), refs
+ * following: sequences that ended, drafts that were rejected.  Dropped entries become
+ * 0.  keep[b] < 0 sets ANVILQ_DEV_ERR_SEQLEN, the row is passed over. */
+int anvilq_pages_release(uint32_t* page_table, int32_t* refs, const int32_t* keep, int rows, int page_tokens,
+                         int max_pages, int num_pages, int* dev_err, unsigned flags, anvilq_stream_t stream);
+
+/* Brings the n pages in use to the places 0 .. n - 1 of every pool: those at n and
+ * above move, in order, to the free ones below n.  out and out_refs (each may be its
+ * input) are the table and the counts after it, *used (device) is n.  The table has
+ * to hold every entry that names a page of the pool. */
+size_t anvilq_pages_compact_workspace_size(int num_pages);
+int anvilq_pages_compact(const uint32_t* page_table, uint32_t* out, const int32_t* refs, int32_t* out_refs,
+                         int32_t* used, const anvilq_page_pool* pools, int pool_count, int rows, int page_tokens,
+                         int max_pages, int num_pages, void* workspace, size_t workspace_bytes, int* dev_err,
+                         unsigned flags, anvilq_stream_t stream);
+
+/* Copies page src[i] onto page dst[i] in every pool, for i < min(*count, most) (count
+ * NULL: most): its first rows[i] tokens, or all of it (rows NULL or rows[i] < 0).
+ * most = 0 does nothing (the lists may then be NULL).  A pair with a negative page is
+ * passed over, a page >= num_pages sets
+ * ANVILQ_DEV_ERR_PAGE.  No page may be a destination twice, nor source and destination. */
+int anvilq_pages_copy(const anvilq_page_pool* pools, int pool_count, const int32_t* src, const int32_t* dst,
+                      const int32_t* rows, const int32_t* count, int most, int page_tokens, int num_pages,
+                      int* dev_err, unsigned flags, anvilq_stream_t stream);
 
 /* ---- tree attention of speculative draft nodes -----------------------------
  *
