@@ -80,6 +80,9 @@ SIGNATURES = {
     "anvilq_logits_process_workspace_size": (SZ, [I, I]),
     "anvilq_logits_process": (I, [P, I, LL, P, LL, P, I, I, P, LL, P, P, I, P, P, P, P, P, P, I, P, LL, P, I, P, SZ, P,
                                   ctypes.c_uint, P]),
+    "anvilq_beam_select_workspace_size": (SZ, [I, I, I, I]),
+    "anvilq_beam_select": (I, [P, I, LL, P, P, F, P, P, I, I, P, P, P, P, P, I, I, I, I, P, SZ, P, ctypes.c_uint, P]),
+    "anvilq_beam_reorder": (I, [P, I, P, I, I, I, P, ctypes.c_uint, P]),
     "anvilq_pages_fork": (I, [P, P, P, P, I, I, I, I, I, P, ctypes.c_uint, P]),
     "anvilq_pages_reserve_workspace_size": (SZ, [I, I]),
     "anvilq_pages_reserve": (I, [P, P, P, P, P, P, I, I, I, I, I, P, SZ, P, ctypes.c_uint, P]),
@@ -116,6 +119,11 @@ class GemvPlan(ctypes.Structure):
 class PagePool(ctypes.Structure):
     """anvilq_page_pool: how a page lies in a pool."""
     _fields_ = [("base", P), ("segments", I), ("segment_bytes", I), ("unit_tokens", I)]
+
+
+class BeamState(ctypes.Structure):
+    """anvilq_beam_state: a state's rows before and after."""
+    _fields_ = [("input", P), ("output", P), ("row_bytes", LL)]
 
 
 _lib = None

@@ -1,0 +1,668 @@
+// beam_select.cu -- a beam search's step: the best N continuations of an item's K
+// beams over the vocabulary, and the reordering of per-beam rows by their parents.
+//
+// Mathematics.  For a beam k with score S_k and logits l_kv,
+//   lse_k = log sum_v exp(l_kv),   s_kv = S_k + (l_kv - lse_k),
+//   rank  = s_kv / (length_k + 1)^alpha.
+// An ended beam has one candidate, its own score with rank S_k / max(length_k, 1)^alpha,
+// at its first place.  The N candidates of the largest ranks win, ties by the lowest
+// place k V + v.
+//
+// Within a beam the order is that of the logits, which is exact; across beams it hangs
+// on the lse, so that is held to about 1e-8: the exponent of exp2((l - c) log2 e) is
+// formed from a difference and a product in two parts, a thread's partial sums are
+// short, and everything from a span's sum on is binary64.  Candidates of different
+// beams whose ranks differ by less may come in either order.
+//
+// What bounds it: the logits are read once (HBM); about 7 instructions a logit.  A
+// small call is bound by latency: load, threshold, merge.
+//
+// Work split.  A CTA takes a span of a beam's vocabulary (splits so that the device is
+// full), in tiles that stay in registers.  Its first tile's N-th largest thread
+// maximum bounds its N-th best logit from below; what beats the bound goes to a list
+// in shared memory, as do later tiles' logits that beat the list's N-th.  After a tile
+// of random logits that is seldom any (N log of the span over the tile in all), so the
+// passes over the list do not show.  The span's sum and N best go to the workspace,
+// and the item's last CTA (by a ticket) merges them.
+#include <algorithm>
+#include <cmath>
+
+#include "kv_q8.cuh"
+
+namespace anvilq {
+namespace beam {
+
+using q8::overlap;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxBeams = 64, kMaxBest = 128;   // K, N
+constexpr int kMaxItems = 4096;
+constexpr int kUnits = 4;                       // 16-byte units of a thread in a tile
+constexpr int kList = 1024;                     // candidates in shared memory
+constexpr int kMaxSplits = 64;
+constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596299e-8f;   // log2 e in two parts
+
+struct Params {
+  const void* logits;        // [B K] rows of V, `stride` elements apart
+  long long stride;
+  const float* scores;       // [B][K]
+  const int* lengths;        // [B][K], null: no length penalty, no lengths out
+  const uint8_t* finished;   // [B][K], null: none
+  const int* eos;            // [eos_count]
+  int* tokens;               // [B][N]
+  int* parents;
+  float* new_scores;
+  int* new_lengths;          // null where lengths is
+  uint8_t* new_finished;
+  int* tickets;              // [B]
+  double2* sums;             // [B][K][splits]: the largest logit, sum of exp(logit - it)
+  unsigned long long* best;  // [B][K][splits][N]: keys, best first
+  int* dev_err;
+  float alpha;
+  int B, K, V, N, splits, eos_count, pad;
+};
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A logit and its place as one number that grows with the logit and, among equals,
+// with smaller places; 0 is below every logit but those of -inf, which get 0 too.
+__device__ __forceinline__ unsigned long long key_of(float v, int at) {
+  const uint32_t u = __float_as_uint(v + 0.0f);   // -0 as +0
+  const uint32_t order = (u >> 31) ? ~u : u | 0x80000000u;
+  return v == -INFINITY ? 0 : ((unsigned long long)order << 32) | (0xFFFFFFFFu - (uint32_t)at);
+}
+__device__ __forceinline__ float logit_of(unsigned long long key) {
+  const uint32_t order = (uint32_t)(key >> 32);
+  return __uint_as_float((order >> 31) ? order & 0x7FFFFFFFu : ~order);
+}
+__device__ __forceinline__ int place_of(unsigned long long key) { return (int)(0xFFFFFFFFu - (uint32_t)key); }
+
+// A beam that goes on or has ended; scores of NaN and +inf are reported and count as none.
+__device__ __forceinline__ bool is_live(float score) { return score > -INFINITY && score < INFINITY; }
+
+// A span's list of candidates.  `bar`: keys must be above it.
+struct List {
+  unsigned long long key[kList];
+  unsigned long long sorted[kMaxBest];
+  unsigned long long bar;
+  int count;
+};
+
+// The list's N best, best first, in its front; bar: the N-th where there are N.  All
+// threads; every key is unique.
+__device__ __forceinline__ void prune(List& s, int N) {
+  __syncthreads();
+  const int n = s.count;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const unsigned long long mine = s.key[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += s.key[j] > mine;
+    if (above < N) s.sorted[above] = mine;
+  }
+  __syncthreads();
+  const int left = min(n, N);
+  for (int i = threadIdx.x; i < left; i += kThreads) s.key[i] = s.sorted[i];
+  if (threadIdx.x == 0) {
+    s.count = left;
+    if (n >= N) s.bar = s.sorted[N - 1];
+  }
+  __syncthreads();
+}
+
+// The final candidates: rank, and the place k V + v (-1: none).
+struct Candidate {
+  double rank;
+  long long place;
+  __device__ __forceinline__ bool beats(const Candidate& o) const {
+    return rank > o.rank || (rank == o.rank && place < o.place);
+  }
+};
+struct Merge {
+  double score[kMaxBeams];
+  double top[kMaxBeams];      // lse = top + log_sum: kept apart, as a logit minus top is exact however
+  double log_sum[kMaxBeams];  // large both are
+  double scale[kMaxBeams];    // the rank's divisor
+  Candidate list[kList];
+  Candidate sorted[kMaxBest];
+  Candidate bar;
+  int count;
+};
+
+__device__ __forceinline__ void prune(Merge& s, int N) {
+  __syncthreads();
+  const int n = s.count;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const Candidate mine = s.list[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += s.list[j].beats(mine);
+    if (above < N) s.sorted[above] = mine;
+  }
+  __syncthreads();
+  const int left = min(n, N);
+  for (int i = threadIdx.x; i < left; i += kThreads) s.list[i] = s.sorted[i];
+  if (threadIdx.x == 0) {
+    s.count = left;
+    if (n >= N) s.bar = s.sorted[N - 1];
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void widen(const uint4& w, float* v, __half) {
+  const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void widen(const uint4& w, float* v, float) {
+  v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y);
+  v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+}
+// 16 bytes of a row that starts on a multiple of `align` bytes
+__device__ __forceinline__ uint4 load_unit(const void* p, int align) {
+  uint4 w;
+  if (align == 16) {
+    w = __ldcs(static_cast<const uint4*>(p));
+  } else if (align == 8) {
+    const uint2 a = __ldg(static_cast<const uint2*>(p)), b = __ldg(static_cast<const uint2*>(p) + 1);
+    w = make_uint4(a.x, a.y, b.x, b.y);
+  } else if (align == 4) {
+    const uint32_t* q = static_cast<const uint32_t*>(p);
+    w = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
+  } else {
+    const unsigned short* q = static_cast<const unsigned short*>(p);
+    uint32_t* o = &w.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __ldg(q + 2 * i) | (uint32_t)__ldg(q + 2 * i + 1) << 16;
+  }
+  return w;
+}
+
+template <typename T>
+__device__ void span_pass(const Params& p, List& s, int row, int split) {
+  constexpr int kVec = 16 / sizeof(T), kEach = kUnits * kVec;
+  const int tid = threadIdx.x;
+  const T* x = static_cast<const T*>(p.logits) + (long long)row * p.stride;
+  // Units of kVec places, wherever the row starts: two equal rows give equal sums, so
+  // that their candidates tie.
+  const int units = (p.V + kVec - 1) / kVec;
+  const uintptr_t start = reinterpret_cast<uintptr_t>(x);
+  const int align = start % 16 == 0 ? 16 : start % 8 == 0 ? 8 : start % 4 == 0 ? 4 : 2;
+  const int u0 = (int)((long long)units * split / p.splits), u1 = (int)((long long)units * (split + 1) / p.splits);
+  if (tid == 0) {
+    s.count = 0;
+    s.bar = 0;
+  }
+  __syncthreads();
+  float c = -INFINITY, sum = 0.0f;    // sum of exp2(log2 e (l - c)), c the thread's largest
+  bool odd = false;                   // a logit of +inf or NaN was left out
+  for (int t0 = u0; t0 < u1; t0 += kThreads * kUnits) {
+    float v[kEach];
+    uint4 raw[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int u = t0 + i * kThreads + tid;
+      if (u < u1 && u * kVec + kVec <= p.V) raw[i] = load_unit(x + u * kVec, align);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int u = t0 + i * kThreads + tid, at = u * kVec;
+      if (u < u1 && at + kVec <= p.V) {
+        widen(raw[i], v + i * kVec, T());
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[i * kVec + e] = u < u1 && at + e < p.V ? (float)x[at + e] : -INFINITY;
+      }
+    }
+    auto place = [&](int i) { return (t0 + (i / kVec) * kThreads + tid) * kVec + i % kVec; };
+    float top = v[0], probe = 0.0f;
+#pragma unroll
+    for (int i = 1; i < kEach; ++i) top = fmaxf(top, v[i]);
+    auto add = [&]() {   // the tile's sum relative to the largest so far
+      const float now = fmaxf(c, top);
+      if (now == -INFINITY) return 0.0f;
+      if (now > c) {
+        const float d = c - now;
+        sum *= c == -INFINITY ? 0.0f : fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
+        c = now;
+      }
+      float part = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const float d = v[i] - c;
+        part += fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
+      }
+      return part;
+    };
+    const float c_was = c, sum_was = sum;
+    probe = add();
+    if (!(probe < INFINITY)) {   // +inf or NaN among them: they count as -inf, and are reported
+      odd = true;
+      top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (!(v[i] < INFINITY)) v[i] = -INFINITY;
+        top = fmaxf(top, v[i]);
+      }
+      c = c_was;
+      sum = sum_was;
+      probe = add();
+    } else if (top == INFINITY || top != top) {   // (all of the thread's logits are NaN)
+      odd = true;
+    }
+    sum += probe;
+    // ---- candidates ----
+    if (t0 == u0) {
+      // the N-th largest of the threads' largest: at least N logits are no smaller
+      unsigned long long mine = 0;
+      if (top > -INFINITY) {
+        int where = 0;
+#pragma unroll
+        for (int i = kEach - 1; i >= 0; --i)
+          if (v[i] == top) where = place(i);
+        mine = key_of(top, where);
+      }
+      s.key[tid] = mine;
+      __syncthreads();
+      int above = 0;
+      for (int j = 0; j < kThreads; ++j) above += s.key[j] > mine;
+      __syncthreads();
+      if (above == p.N - 1 && mine) s.bar = mine - 1;   // only one thread, unless it is of no logit
+      __syncthreads();
+    }
+    // may this thread have any, and how many at most
+    const unsigned long long bar = s.bar;
+    const float least = bar ? logit_of(bar) : -INFINITY;
+    int mine = 0;
+    if (top >= least && top > -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) mine += v[i] >= least && key_of(v[i], place(i)) > bar;
+    }
+    const int many = __syncthreads_or(mine > 0);
+    if (!many) continue;
+    // all at once where they are sure to fit, else a column of the tile at a time
+    __shared__ int total;
+    if (tid == 0) total = 0;
+    __syncthreads();
+    if (mine) atomicAdd(&total, mine);
+    __syncthreads();
+    const bool fit = s.count + total <= kList;
+    __syncthreads();
+    if (fit) {
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const unsigned long long key = v[i] >= least ? key_of(v[i], place(i)) : 0;
+          if (key > bar) s.key[atomicAdd(&s.count, 1)] = key;
+        }
+      }
+      prune(s, p.N);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kEach; ++i) {
+        // (an index into registers that the compiler cannot see: by selection)
+        float mine_v = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) mine_v = e == i ? v[e] : mine_v;
+        if (s.count + kThreads > kList) prune(s, p.N);   // the same for all: the count stands still here
+        const unsigned long long key = key_of(mine_v, place(i)), now = s.bar;
+        __syncthreads();
+        if (key > now) s.key[atomicAdd(&s.count, 1)] = key;
+        __syncthreads();
+      }
+      prune(s, p.N);
+    }
+  }
+  // ---- the span's sum, in binary64 from the threads' on ----
+  __shared__ float tops[kWarps];
+  __shared__ double parts[kWarps];
+  float top = c;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (tid % 32 == 0) tops[tid / 32] = top;
+  __syncthreads();
+  top = tops[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) top = fmaxf(top, tops[w]);
+  double mine = 0.0;
+  if (c > -INFINITY) mine = (double)sum * exp((double)c - (double)top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (tid % 32 == 0) parts[tid / 32] = mine;
+  if (odd) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
+  __syncthreads();
+  const size_t at = (size_t)row * p.splits + split;
+  if (tid == 0) {
+    double all = 0.0;
+    for (int w = 0; w < kWarps; ++w) all += parts[w];
+    __stcg(p.sums + at, make_double2(top, all));
+  }
+  for (int i = tid; i < p.N; i += kThreads) __stcg(p.best + at * p.N + i, i < s.count ? s.key[i] : 0ull);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(16) unsigned char room[];   // a List, then a Merge
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, b = row / p.K;
+  // a beam that is dead or ended has no logits to be read
+  const bool live = is_live(p.scores[row]) && !(p.finished && p.finished[row]);
+  if (live) span_pass<T>(p, *reinterpret_cast<List*>(room), row, split);
+  // ---- the item's last CTA goes on ----
+  __shared__ int last;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    const int arrived = atomicAdd(p.tickets + b, 1);
+    last = arrived == p.K * p.splits - 1;
+    if (last) p.tickets[b] = 0;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  Merge& m = *reinterpret_cast<Merge*>(room);
+  for (int k = tid / 32; k < p.K; k += kWarps) {   // a beam a warp
+    const int r = b * p.K + k, lane = tid % 32;
+    const float score = p.scores[r];
+    const bool ended = p.finished && p.finished[r];
+    const int length = p.lengths ? max(p.lengths[r], 0) : 0;
+    double largest = 0.0, log_sum = 0.0;
+    if (is_live(score) && !ended) {
+      static_assert(kMaxSplits <= 64, "two spans a lane");
+      const double2 none = make_double2(-INFINITY, 0.0);
+      const double2* at = p.sums + (size_t)r * p.splits;
+      const double2 one = lane < p.splits ? __ldcg(at + lane) : none;
+      const double2 two = lane + 32 < p.splits ? __ldcg(at + lane + 32) : none;
+      double top = fmax(one.x, two.x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+      double all = 0.0;
+      if (one.y > 0.0) all = one.y * exp(one.x - top);
+      if (two.y > 0.0) all += two.y * exp(two.x - top);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+      largest = top;            // of a beam without candidates: not used
+      log_sum = log(all);
+    }
+    if (lane == 0) {
+      if (!(score < INFINITY)) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
+      m.score[k] = score;
+      m.top[k] = largest;
+      m.log_sum[k] = log_sum;
+      const int steps = ended ? max(length, 1) : length + 1;
+      m.scale[k] = p.alpha == 0.0f ? 1.0 : pow((double)steps, (double)p.alpha);
+    }
+  }
+  if (tid == 0) {
+    m.count = 0;
+    m.bar = Candidate{-INFINITY, 0};
+  }
+  __syncthreads();
+  auto score_of = [&](int k, float logit) { return m.score[k] + (((double)logit - m.top[k]) - m.log_sum[k]); };
+  const int per = p.splits * p.N, all = p.K * per;
+  for (int i0 = 0; i0 < all; i0 += kThreads) {
+    const int i = i0 + tid;
+    Candidate mine{-INFINITY, -1};
+    if (i < all) {
+      const int k = i / per, r = b * p.K + k;
+      if (is_live(p.scores[r])) {
+        if (p.finished && p.finished[r]) {
+          if (i % per == 0) mine = Candidate{m.score[k] / m.scale[k], (long long)k * p.V};
+        } else if (const unsigned long long key = __ldcg(p.best + (size_t)r * per + i % per)) {
+          mine = Candidate{score_of(k, logit_of(key)) / m.scale[k], (long long)k * p.V + place_of(key)};
+        }
+      }
+    }
+    if (m.count + kThreads > kList) prune(m, p.N);
+    const Candidate bar = m.bar;
+    __syncthreads();
+    if (mine.place >= 0 && mine.rank > -INFINITY && mine.beats(bar)) m.list[atomicAdd(&m.count, 1)] = mine;
+    __syncthreads();
+  }
+  prune(m, p.N);
+  for (int i = tid; i < p.N; i += kThreads) {
+    const int at = b * p.N + i;
+    if (i >= m.count) {
+      p.tokens[at] = p.parents[at] = -1;
+      p.new_scores[at] = -INFINITY;
+      p.new_finished[at] = 1;
+      if (p.new_lengths) p.new_lengths[at] = 0;
+      continue;
+    }
+    const Candidate c = m.list[i];
+    const int k = (int)(c.place / p.V), r = b * p.K + k;
+    const bool ended = p.finished && p.finished[r];
+    const int token = ended ? p.pad : (int)(c.place % p.V);
+    bool over = ended;
+    for (int e = 0; e < p.eos_count; ++e) over |= p.eos[e] == token;
+    p.tokens[at] = token;
+    p.parents[at] = k;
+    // the score itself, not the rank times its divisor
+    double score = p.scores[r];
+    if (!ended) {
+      const T* x = static_cast<const T*>(p.logits) + (long long)r * p.stride;
+      score = score_of(k, (float)x[token]);
+    }
+    p.new_scores[at] = (float)score;
+    p.new_finished[at] = over;
+    if (p.new_lengths) p.new_lengths[at] = p.lengths[r] + !ended;
+  }
+}
+
+// ---- rows by their parents ---------------------------------------------------------
+
+constexpr int kMaxStates = 32;
+struct State {
+  const char* in;
+  char* out;
+  long long row_bytes;
+};
+struct Reorder {
+  const int* parents;   // [B][N]
+  int* dev_err;
+  int B, K, N, states;
+  State state[kMaxStates];
+};
+
+template <typename W>
+__device__ __forceinline__ void move_row(const char* from, char* to, long long bytes) {
+  constexpr int kAhead = 4;
+  const long long n = bytes / (long long)sizeof(W), step = (long long)gridDim.x * kThreads;
+  for (long long i0 = (long long)blockIdx.x * kThreads + threadIdx.x; i0 < n; i0 += kAhead * step) {
+    W w[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      w[a] = W{};
+      if (from && i0 + a * step < n) w[a] = reinterpret_cast<const W*>(from)[i0 + a * step];
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+      if (i0 + a * step < n) reinterpret_cast<W*>(to)[i0 + a * step] = w[a];
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) reorder_kernel(const __grid_constant__ Reorder p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const State& s = p.state[blockIdx.z];
+  for (int row = blockIdx.y; row < p.B * p.N; row += gridDim.y) {
+    int parent = p.parents[row];
+    if (parent < -1 || parent >= p.K) {
+      if (threadIdx.x == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+      parent = -1;
+    }
+    const char* from = parent < 0 ? nullptr : s.in + ((long long)(row / p.N) * p.K + parent) * s.row_bytes;
+    char* to = s.out + (long long)row * s.row_bytes;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(s.in) | reinterpret_cast<uintptr_t>(s.out) | s.row_bytes;
+    if (all % 16 == 0) move_row<uint4>(from, to, s.row_bytes);
+    else if (all % 4 == 0) move_row<uint32_t>(from, to, s.row_bytes);
+    else move_row<uint8_t>(from, to, s.row_bytes);
+  }
+}
+
+template <typename P>
+static int launch(void (*kernel)(P), dim3 grid, size_t smem, cudaStream_t s, unsigned flags, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = (flags & ANVILQ_GEMM_OVERLAP_PRIOR) ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+    cudaGetLastError();
+    return ANVILQ_ECUDA;
+  }
+  return ANVILQ_OK;
+}
+
+static bool shape_ok(int B, int K, int V, int N) {
+  return B >= 1 && B <= kMaxItems && K >= 1 && K <= kMaxBeams && N >= 1 && N <= kMaxBest && V >= 1 && V <= (1 << 30) &&
+         B * K <= 65535;
+}
+// Spans of a row: about 8 CTAs an SM in all, of at least a tile each.
+static int splits_for(int B, int K, int V) {
+  const long long rows = (long long)B * K, tile = kThreads * kUnits * 4;
+  return (int)std::min<long long>(kMaxSplits, std::max<long long>(1, std::min((148 * 8 + rows - 1) / rows,
+                                                                              (V + tile - 1) / tile)));
+}
+
+}  // namespace beam
+}  // namespace anvilq
+
+extern "C" {
+
+size_t anvilq_beam_select_workspace_size(int B, int K, int V, int N) {
+  using namespace anvilq::beam;
+  if (!shape_ok(B, K, V, N)) return 0;
+  const size_t spans = (size_t)B * K * splits_for(B, K, V);
+  return ANVILQ_WORKSPACE_COUNTER_BYTES + spans * (sizeof(double2) + (size_t)N * 8);
+}
+
+int anvilq_beam_select(const void* logits, int logits_half, long long logits_stride, const float* scores,
+                       const int32_t* lengths, float length_penalty, const uint8_t* finished, const int32_t* eos_ids,
+                       int eos_count, int pad_id, int32_t* tokens, int32_t* parents, float* new_scores,
+                       int32_t* new_lengths, uint8_t* new_finished, int B, int K, int V, int N, void* workspace,
+                       size_t workspace_bytes, int* dev_err, unsigned flags, anvilq_stream_t stream) {
+  using namespace anvilq;
+  using namespace anvilq::beam;
+  if (!logits || !scores || !tokens || !parents || !new_scores || !new_finished || !dev_err) return ANVILQ_EINVAL;
+  if ((logits_half != 0 && logits_half != 1) || eos_count < 0 || (eos_count && !eos_ids)) return ANVILQ_EINVAL;
+  if ((lengths == nullptr) != (new_lengths == nullptr) || (!lengths && length_penalty != 0.0f)) return ANVILQ_EINVAL;
+  if (!(std::fabs(length_penalty) <= 16.0f)) return ANVILQ_EINVAL;
+  if (flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) return ANVILQ_EINVAL;
+  if (!shape_ok(B, K, V, N) || eos_count > 1024) return ANVILQ_ESHAPE;
+  if (logits_stride < V) return ANVILQ_EINVAL;
+  const uintptr_t ints = reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(lengths) |
+                         reinterpret_cast<uintptr_t>(eos_ids) | reinterpret_cast<uintptr_t>(tokens) |
+                         reinterpret_cast<uintptr_t>(parents) | reinterpret_cast<uintptr_t>(new_scores) |
+                         reinterpret_cast<uintptr_t>(new_lengths);
+  if (ints % 4 || reinterpret_cast<uintptr_t>(logits) % (logits_half ? 2 : 4) ||
+      reinterpret_cast<uintptr_t>(workspace) % 16)
+    return ANVILQ_EALIGN;
+  // an item's results are written while other items are still to be read
+  const size_t in = (size_t)B * K, out = (size_t)B * N;
+  struct Span {
+    const void* start;
+    size_t bytes;
+  };
+  const Span reads[] = {{logits, ((in - 1) * (size_t)logits_stride + V) * (logits_half ? 2 : 4)}, {scores, in * 4},
+                        {lengths, lengths ? in * 4 : 0}, {finished, finished ? in : 0}, {eos_ids, eos_count * 4u},
+                        {workspace, workspace ? workspace_bytes : 0}};
+  const Span writes[] = {{tokens, out * 4}, {parents, out * 4}, {new_scores, out * 4},
+                         {new_lengths, new_lengths ? out * 4 : 0}, {new_finished, out}};
+  for (int i = 0; i < 5; ++i) {
+    for (const Span& r : reads)
+      if (overlap(writes[i].start, writes[i].bytes, r.start, r.bytes)) return ANVILQ_EINVAL;
+    for (int j = 0; j < i; ++j)
+      if (overlap(writes[i].start, writes[i].bytes, writes[j].start, writes[j].bytes)) return ANVILQ_EINVAL;
+    if (workspace && i < 4 && overlap(reads[i].start, reads[i].bytes, workspace, workspace_bytes)) return ANVILQ_EINVAL;
+  }
+  if (!workspace || workspace_bytes < anvilq_beam_select_workspace_size(B, K, V, N)) return ANVILQ_EWORKSPACE;
+  Params p{};
+  p.logits = logits;
+  p.stride = logits_stride;
+  p.scores = scores;
+  p.lengths = lengths;
+  p.finished = finished;
+  p.eos = eos_ids;
+  p.tokens = tokens;
+  p.parents = parents;
+  p.new_scores = new_scores;
+  p.new_lengths = new_lengths;
+  p.new_finished = new_finished;
+  p.dev_err = dev_err;
+  p.alpha = length_penalty;
+  p.B = B; p.K = K; p.V = V; p.N = N;
+  p.splits = splits_for(B, K, V);
+  p.eos_count = eos_count;
+  p.pad = pad_id;
+  char* at = static_cast<char*>(workspace) + ANVILQ_WORKSPACE_COUNTER_BYTES;
+  p.tickets = static_cast<int*>(workspace);
+  p.sums = reinterpret_cast<double2*>(at);
+  p.best = reinterpret_cast<unsigned long long*>(at + (size_t)B * K * p.splits * sizeof(double2));
+  const size_t smem = std::max(sizeof(List), sizeof(Merge));
+  const dim3 grid(p.splits, B * K);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return logits_half ? launch(beam_kernel<__half>, grid, smem, st, flags, p)
+                     : launch(beam_kernel<float>, grid, smem, st, flags, p);
+}
+
+int anvilq_beam_reorder(const anvilq_beam_state* states, int count, const int32_t* parents, int B, int K, int N,
+                        int* dev_err, unsigned flags, anvilq_stream_t stream) {
+  using namespace anvilq;
+  using namespace anvilq::beam;
+  if (!parents || !dev_err || count < 0 || (count && !states)) return ANVILQ_EINVAL;
+  if (flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) return ANVILQ_EINVAL;
+  if (B < 1 || K < 1 || N < 1 || (long long)B * std::max(K, N) > (1 << 24)) return ANVILQ_ESHAPE;
+  if (reinterpret_cast<uintptr_t>(parents) % 4) return ANVILQ_EALIGN;
+  for (int i = 0; i < count; ++i) {
+    const anvilq_beam_state& a = states[i];
+    if (!a.in || !a.out || a.row_bytes < 1) return ANVILQ_EINVAL;
+    if (a.row_bytes > (1LL << 40) / (B * (long long)std::max(K, N))) return ANVILQ_ESHAPE;
+  }
+  for (int i = 0; i < count; ++i) {
+    const anvilq_beam_state& a = states[i];
+    const size_t out = (size_t)B * N * a.row_bytes;
+    if (overlap(a.out, out, parents, (size_t)B * N * 4)) return ANVILQ_EINVAL;
+    for (int j = 0; j < count; ++j) {
+      const anvilq_beam_state& o = states[j];
+      if (overlap(a.out, out, o.in, (size_t)B * K * o.row_bytes) ||
+          (j != i && overlap(a.out, out, o.out, (size_t)B * N * o.row_bytes)))
+        return ANVILQ_EINVAL;
+    }
+  }
+  for (int done = 0; done < count; done += kMaxStates) {
+    Reorder p{};
+    p.parents = parents;
+    p.dev_err = dev_err;
+    p.B = B; p.K = K; p.N = N;
+    p.states = std::min(kMaxStates, count - done);
+    long long widest = 0;
+    for (int i = 0; i < p.states; ++i) {
+      const anvilq_beam_state& a = states[done + i];
+      p.state[i] = State{static_cast<const char*>(a.in), static_cast<char*>(a.out), a.row_bytes};
+      widest = std::max<long long>(widest, a.row_bytes);
+    }
+    // CTAs of a row: 16 KB each, no more than fill the device
+    const int rows = std::min(B * N, 65535);
+    const long long fill = (148 * 8 + (long long)rows * p.states - 1) / ((long long)rows * p.states);
+    const int ctas = (int)std::max<long long>(1, std::min<long long>((widest + 16383) / 16384, fill));
+    if (const int rc = launch(reorder_kernel, dim3(ctas, rows, p.states), 0, reinterpret_cast<cudaStream_t>(stream),
+                              done ? flags | ANVILQ_GEMM_OVERLAP_PRIOR : flags, p))
+      return rc;
+  }
+  return ANVILQ_OK;
+}
+
+}  // extern "C"

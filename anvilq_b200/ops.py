@@ -1033,6 +1033,107 @@ def logits_process(logits, history=None, history_lens=None, prompt_lens=None, re
     return out, tokens
 
 
+# ---- beam search -------------------------------------------------------------------
+
+@functools.lru_cache(maxsize=1024)
+def _beam_workspace_size(B, K, V, N):
+    return _lib.load().anvilq_beam_select_workspace_size(B, K, V, N)
+
+
+def beam_select(logits, scores, N: int | None = None, lengths=None, length_penalty: float = 0.0, finished=None,
+                eos_ids=None, pad_id: int = 0, dev_err=None, workspace=None, overlap_prior: bool = False):
+    """The best N (default K) continuations of every item's K beams over the vocabulary.
+    logits fp32 or fp16 [B, K, V] or [B * K, V] (rows may be strided; ``logits_process``'s
+    masks are kept), scores fp32 [B, K] (the beams' log probabilities, -inf: none), lengths
+    int32 [B, K], finished bool [B, K], eos_ids int32 [E].  A token's score is its beam's
+    plus its log probability, its rank that over (length + 1)^length_penalty; a finished
+    beam stays as one candidate with pad_id.  Returns (tokens, parents, scores, lengths,
+    finished), [B, N] each, best first, ties by the lowest beam and token: int32, int32
+    (beams of the item, for ``beam_reorder`` and ``pages_fork``), fp32, int32 (None without
+    lengths), bool; -1, -1, -inf, 0, True where candidates are fewer.  include/anvilq.h has
+    the formulas.  workspace: as for ``gqa_decode_q8``."""
+    name = "beam_select"
+    if scores.dtype != torch.float32 or scores.dim() != 2 or not scores.is_contiguous():
+        raise ValueError(f"{name}: scores must be contiguous float32 [B, K]")
+    B, K = scores.shape
+    half = logits.dtype == torch.float16
+    if not half and logits.dtype != torch.float32:
+        raise ValueError(f"{name}: logits must be float32 or float16")
+    shape, strides = logits.shape, logits.stride()
+    if len(shape) not in (2, 3) or (shape[:2] != (B, K) if len(shape) == 3 else shape[0] != B * K):
+        raise ValueError(f"{name}: logits must be [{B}, {K}, V] or [{B * K}, V]")
+    V, rows = shape[-1], B * K
+    stride = strides[-2] if rows > 1 else V
+    if len(shape) == 3 and B > 1:
+        stride = strides[1] if K > 1 else strides[0]
+        if K > 1 and strides[0] != K * strides[1]:
+            raise ValueError(f"{name}: logits' rows must be equally far apart")
+    if (V > 1 and strides[-1] != 1) or stride < V:
+        raise ValueError(f"{name}: rows of logits must be contiguous and must not overlap")
+    N = K if N is None else int(N)
+    for t, kind in ((lengths, torch.int32), (finished, torch.bool)):
+        if t is not None and (t.dtype != kind or t.shape != (B, K) or not t.is_contiguous()):
+            raise ValueError(f"{name}: lengths must be contiguous int32 and finished bool, [{B}, {K}]")
+    if eos_ids is not None and (eos_ids.dtype != torch.int32 or eos_ids.dim() != 1 or not eos_ids.is_contiguous()):
+        raise ValueError(f"{name}: eos_ids must be a contiguous int32 vector")
+    if lengths is None and length_penalty:
+        raise ValueError(f"{name}: a length penalty needs lengths")
+    dev = logits.device
+    _on_device(name, dev, scores, lengths, finished, eos_ids)
+    need = _beam_workspace_size(B, K, V, N)
+    if need == 0:
+        raise ValueError(f"{name}: unsupported shape B={B} K={K} V={V} N={N}")
+    ws = _call_workspace(dev, need, workspace)
+    err = _error_word(dev, dev_err)
+    ints = scores.new_empty((2 if lengths is None else 3, B, N), dtype=torch.int32)
+    new_scores, new_finished = scores.new_empty((B, N)), scores.new_empty((B, N), dtype=torch.bool)
+    tokens, parents, *new_lengths = ints.unbind(0)
+    _call("anvilq_beam_select", dev, logits.data_ptr(), 1 if half else 0, stride, scores.data_ptr(), _ptr(lengths),
+          float(length_penalty), _ptr(finished), _ptr(eos_ids), 0 if eos_ids is None else eos_ids.shape[0], int(pad_id),
+          tokens.data_ptr(), parents.data_ptr(), new_scores.data_ptr(), new_lengths[0].data_ptr() if new_lengths else
+          None, new_finished.data_ptr(), B, K, V, N, ws.data_ptr(), ws.numel(), err.data_ptr(),
+          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    return tokens, parents, new_scores, new_lengths[0] if new_lengths else None, new_finished
+
+
+def beam_reorder(states, parents, outs=None, dev_err=None, overlap_prior: bool = False):
+    """Per-beam rows by their parents: for each of `states` ([B, K, ...] of any type,
+    contiguous) a tensor [B, N, ...] whose row n of item b is row parents[b, n]
+    (int32 [B, N], ``beam_select``'s) of the item's, zeros for -1.  outs: tensors of that
+    shape to write to, apart from the states.  Page tables go by ``pages_fork``, which
+    keeps the pages' counts."""
+    name = "beam_reorder"
+    if parents.dtype != torch.int32 or parents.dim() != 2 or not parents.is_contiguous():
+        raise ValueError(f"{name}: parents must be contiguous int32 [B, N]")
+    (B, N), dev, K = parents.shape, parents.device, None
+    states = list(states)
+    if outs is not None and len(outs) != len(states):
+        raise ValueError(f"{name}: as many outs as states expected")
+    results, array = [], (_lib.BeamState * len(states))()
+    for i, t in enumerate(states):
+        shape = t.shape
+        K = shape[1] if K is None and len(shape) > 1 else K
+        if shape[:2] != (B, K) or 0 in shape or not t.is_contiguous():
+            raise ValueError(f"{name}: states must be contiguous [{B}, K, ...] with one K")
+        rest = shape[2:]
+        if outs is None:
+            o = t.new_empty((B, N, *rest))
+        else:
+            o = outs[i]
+            if o.dtype != t.dtype or o.shape != (B, N, *rest) or not o.is_contiguous():
+                raise ValueError(f"{name}: out {i} must be contiguous {t.dtype} {[B, N, *rest]}")
+        results.append(o)
+        array[i].input, array[i].output = t.data_ptr(), o.data_ptr()
+        array[i].row_bytes = t.numel() // (B * K) * t.element_size()
+    _on_device(name, dev, *states, *results)
+    if not states:
+        return results
+    err = _error_word(dev, dev_err)
+    _call("anvilq_beam_reorder", dev, array, len(states), parents.data_ptr(), B, K, N, err.data_ptr(),
+          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    return results
+
+
 # ---- pages that sequences share ----------------------------------------------------
 
 class PagePools:

@@ -785,6 +785,49 @@ int anvilq_logits_process(const void* logits, int logits_half, long long logits_
                           const int32_t* allowed_rows, int masks, void* workspace, size_t workspace_bytes,
                           int* dev_err, unsigned flags, anvilq_stream_t stream);
 
+/* ---- beam search ----------------------------------------------------------------
+ *
+ * The best N continuations of each of B items with K beams: beam k of item b has the
+ * score S = scores[b][k] (fp32; -inf: none yet), the logits row b K + k (fp32, or fp16
+ * with logits_half; V of them, rows logits_stride elements apart) and, with lengths
+ * (int32 [B][K]), a number of tokens n.  Its candidates are its tokens v with a
+ * logit l > -inf,
+ *   s = S + (l - log sum_v exp(l)),   rank = s / (n + 1)^length_penalty,
+ * or, where finished[b][k] is not 0, one candidate, pad_id with s = S and
+ * rank = S / max(n, 1)^length_penalty, standing at v = 0.  The N largest ranks win,
+ * equal ones by the lowest k V + v; sums are held to about 1e-8, ranks of different
+ * beams that are closer may come in either order.  Results, best first, [B][N]:
+ *   tokens, parents (the beam k), new_scores (s), new_lengths (n + 1, n of a finished
+ *   beam), new_finished (1: of a finished beam, or one of the eos_count eos_ids)
+ * and where there are fewer candidates -1, -1, -inf, 0, 1.  A logit of +inf or NaN
+ * counts as -inf, a score of +inf or NaN as none, both set ANVILQ_DEV_ERR_NONFINITE.
+ * lengths, finished, eos_ids may be NULL (new_lengths with lengths; without them
+ * length_penalty is 0); lengths below 0 count as 0; |length_penalty| <= 16.  B <= 4096,
+ * K <= 64, B K <= 65535, N <= 128, V <= 2^30, eos_count <= 1024; results, inputs and
+ * workspace apart from each other; flags: ANVILQ_GEMM_OVERLAP_PRIOR; workspace: 16-byte
+ * aligned, anvilq_beam_select_workspace_size bytes, layout as described at
+ * ANVILQ_WORKSPACE_COUNTER_BYTES.  No counterpart in the reference, which decodes
+ * greedily (anvil-q4/tests/transformer_reference.py:212-217). */
+size_t anvilq_beam_select_workspace_size(int B, int K, int V, int N);
+int anvilq_beam_select(const void* logits, int logits_half, long long logits_stride, const float* scores,
+                       const int32_t* lengths, float length_penalty, const uint8_t* finished, const int32_t* eos_ids,
+                       int eos_count, int pad_id, int32_t* tokens, int32_t* parents, float* new_scores,
+                       int32_t* new_lengths, uint8_t* new_finished, int B, int K, int V, int N, void* workspace,
+                       size_t workspace_bytes, int* dev_err, unsigned flags, anvilq_stream_t stream);
+
+/* A beam's row of every state by its parent: out row b N + n = in row b K +
+ * parents[b][n], zeros for -1 (a parent outside [-1, K) sets ANVILQ_DEV_ERR_SEQLEN and
+ * counts as -1).  Rows of any number of bytes, without gaps (16-byte multiples are
+ * faster); outs apart from all else.  The array of states is host memory, read before
+ * the call returns. */
+typedef struct anvilq_beam_state {
+  const void* in;        /* device, [B K] rows */
+  void* out;             /* device, [B N] rows */
+  long long row_bytes;
+} anvilq_beam_state;
+int anvilq_beam_reorder(const anvilq_beam_state* states, int count, const int32_t* parents, int B, int K, int N,
+                        int* dev_err, unsigned flags, anvilq_stream_t stream);
+
 /* ---- pages that sequences share -----------------------------------------------
  *
  * Beams of a search, several answers to one prompt, prompts with a common start:
