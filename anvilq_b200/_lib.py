@@ -77,6 +77,8 @@ SIGNATURES = {
     "anvilq_kv_q8_values": (I, [P, P, P, P, I, P, P, I, I, I, I, ctypes.c_uint, P]),
     "anvilq_gqa_decode_q8_workspace_size": (SZ, [I, I, I, I, I]),
     "anvilq_gqa_decode_q8": (I, [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, F, P, SZ, P, ctypes.c_uint, P]),
+    "anvilq_gqa_chunk_paged_workspace_size": (SZ, [I, I, I, I, I, I, I]),
+    "anvilq_gqa_chunk_paged": (I, [P, LL, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, P, SZ, P, ctypes.c_uint, P]),
     "anvilq_logits_process_workspace_size": (SZ, [I, I]),
     "anvilq_logits_process": (I, [P, I, LL, P, LL, P, I, I, P, LL, P, P, I, P, P, P, P, P, P, I, P, LL, P, I, P, SZ, P,
                                   ctypes.c_uint, P]),

@@ -1,0 +1,930 @@
+// gqa_chunk.cu -- attention of many new tokens a sequence over a paged binary16
+// cache: prompts in chunks, questions about long documents, batches that mix them
+// with decode steps.  Fifth-generation tensor cores (tcgen05), softmax in registers.
+//
+// Mathematics.  Token t of sequence b is at position pos = seqlens[b] - n_b + (t -
+// start_b) (its n_b new tokens are its last, in the cache already); query head h reads
+// kv head h / g, g = Hq / Hkv, and
+//   out = sum_{s <= pos} p_s v_s / sum p_s,   p_s = exp2(scale log2(e) q.k_s - m)
+// with a running reference m of each row that is at least the row's largest exponent
+// minus 8: p stays below 2^8, so m seldom moves and the sums are rescaled only then.
+// Scores, sums and outputs are binary32; p enters the tensor cores as binary16 (half a
+// step, 2^-11 of each), which they need as the operand beside binary16 values.
+//
+// Tiles.  A pair of 128-row tiles holds 2 tpt tokens of one kv head's g query heads,
+// tpt = 128 / g (row r: token r / g, head r % g; rows behind tpt g are padding), and
+// walks over the keys up to its last token's position, 128 a step: S = Q K^T into TMEM,
+// softmax by a warpgroup (a thread a row), P back into TMEM over S, O += P V.  Two
+// tiles in turn keep the tensor cores at one's products while the other's softmax runs.
+//
+// Work split (stream-K).  All (pair, key tile) units in a row, pairs in the order
+// (sequence, kv head, pair), are cut into equal stretches, one a CTA, so lengths do not
+// matter to the balance and few rows over a long axis are split over it.  A pair that
+// several CTAs share leaves binary32 partial sums in the workspace; a second kernel,
+// launched with the first's end overlapped, merges them in CTA order (bit-reproducible).
+// How many units there are is a sum of rounded linear functions, computed in closed form
+// (floor_sum) by every CTA from the lengths on the device.
+//
+// Warp roles (12 warps, one CTA an SM):
+//   0-3, 4-7   softmax of tile 0 and tile 1: also load its Q, rescale and store its O
+//   8, 9       TMA of K and of V (their boxes are issued side by side: pages of 16
+//              tokens take 16 copies a tile)
+//   10         MMA issuer, TMEM owner; zeroes V's rows behind a sequence's last token
+// K and V tiles share a ring: [half of 64 dims][128 keys][128 bytes], 128-byte swizzle.
+// K is the K-major B operand of S, V the MN-major one of O.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+
+#include "kv_q8.cuh"
+
+namespace anvilq {
+namespace chunk {
+
+using q8::overlap;
+using u64 = unsigned long long;
+constexpr int kRows = 128;                 // of a tile: MMA M, a TMEM lane each
+constexpr int kKeys = 128;                 // of a step
+constexpr int kThreads = 384;
+constexpr int kWarps = kThreads / 32;
+constexpr int kKWarp = 8, kVWarp = 9, kMmaWarp = 10;
+constexpr int kMaxCtas = 148;
+constexpr int kMaxBatch = 65536;
+constexpr float kNone = -1e30f;            // a reference below every exponent
+constexpr float kSlack = 8.0f;             // how far (log2) the reference may lag behind the largest
+constexpr u64 kWaitLimitNs = 1000000000ull;
+constexpr uint32_t kTmemCols = 512, kTmemO = 256;   // S of tile t at 128 t, O at 256 + 128 t
+
+template <int D>
+struct Cfg {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTileBytes = kKeys * D * 2;                 // a K, V or Q tile
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr int kOffQ = kStages * kTileBytes;
+  static constexpr int kOffBar = kOffQ + 2 * kTileBytes;
+  static constexpr int kBars = 2 * kStages + 2 * 4 + 1;
+  static constexpr int kOffMisc = kOffBar + kBars * 8;
+  static constexpr int kSmem = kOffMisc + 128 + 1024;              // + slack to align the base
+  static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
+  static_assert(kMaxBatch / 32 * 8 <= kOffQ, "the groups' counts lie in the ring before its first copy");
+};
+
+struct Params {
+  const __half* q;              // [T] tokens of Hq D, `q_stride` elements apart
+  long long q_stride;
+  const int* starts;            // [B + 1]
+  const int* seqlens;           // [B]
+  const uint32_t* page_table;   // [B][max_pages]
+  __half* out;                  // [T][Hq][D]
+  float* partials;              // [CTAs][2][256 (D + 2)]
+  struct Open* open;            // [CTAs]
+  int* dev_err;
+  float scale_log2;
+  int T, B, Hq, Hkv, group, tpt, page_tokens, max_pages, num_pages, box;
+};
+
+// What the merge needs to know of a CTA's first pair.
+struct Open {
+  u64 begin, end;               // its units; the CTA's own begin at `at`
+  u64 at, chunk;
+  int token, tokens, head, mid; // first token, tokens left in the sequence from it on; mid: begun by an earlier CTA
+};
+
+// ---- PTX ------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ u64 globaltimer() {
+  u64 t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Waits for the phase of `parity`; gives up after kWaitLimitNs, or once another role has.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const u64 t0 = globaltimer();
+  for (;;) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag || globaltimer() - t0 > kWaitLimitNs) return false;
+  }
+}
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+  const u64 t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer() - t0 > kWaitLimitNs) return;
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile("{\n .reg .pred e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}"
+               : "=r"(pred));
+  return pred != 0;
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]^T and D[tmem] (+)= A[tmem] B[smem]^T, binary16 operands
+__device__ __forceinline__ void mma_ss(uint32_t d, u64 a, u64 b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, u64 b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0)
+      : "memory");
+}
+#define ANVILQ_R32(r)                                                                                              \
+  r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),           \
+      "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),       \
+      "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),      \
+      "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]
+// 32 consecutive columns of the thread's lane; wait_ld() before the registers are used
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(ANVILQ_R32(r))
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
+      "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
+      "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Shared-memory matrix descriptor: start, leading and stride byte offsets in 16-byte
+// units, version 1, 128-byte swizzle.  K-major: stride between 8-row groups (leading
+// unused).  MN-major: leading between blocks of 64 dims, stride between 8-key groups.
+__device__ __forceinline__ u64 smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return (u64)((addr >> 4) & 0x3FFFu) | ((u64)((lbo >> 4) & 0x3FFFu) << 16) | ((u64)((sbo >> 4) & 0x3FFFu) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// Instruction descriptor, kind::f16: binary32 accumulator, binary16 operands, M 128;
+// bit 16: B is MN-major
+__host__ __device__ constexpr uint32_t instr_desc(int n, bool b_mn_major) {
+  return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+
+// ---- the plan -----------------------------------------------------------------------
+
+// sum of floor((a i + b) / m), i = 0 .. n - 1
+__device__ __forceinline__ u64 floor_sum(u64 n, u64 m, u64 a, u64 b) {
+  u64 sum = 0;
+  while (n) {
+    if (a >= m) {
+      sum += (n - 1) * n / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      sum += n * (b / m);
+      b %= m;
+    }
+    const u64 top = a * n + b;
+    if (top < m) break;
+    n = top / m;
+    b = top % m;
+    const u64 t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+
+// A sequence's new tokens: rows [start, start + n) at positions before and on.
+struct Seq {
+  int start, n, before;
+};
+__device__ __forceinline__ Seq sequence(const Params& p, int b) {
+  const int s0 = p.starts[b], s1 = p.starts[b + 1], len = p.seqlens[b];
+  const long long n = (long long)s1 - s0;
+  if (n <= 0) return Seq{0, 0, 0};
+  if (s0 < 0 || s1 > p.T || n > len || len > (long long)p.page_tokens * p.max_pages) {
+    atomicOr(p.dev_err, ANVILQ_DEV_ERR_SEQLEN);
+    return Seq{0, 0, 0};
+  }
+  return Seq{s0, (int)n, len - (int)n};
+}
+__device__ __forceinline__ int pairs_of(const Params& p, const Seq& s) { return (s.n + 2 * p.tpt - 1) / (2 * p.tpt); }
+// key tiles of the first `tokens` (> 0) new tokens
+__device__ __forceinline__ int tiles_to(const Seq& s, int tokens) {
+  return (s.before + min(tokens, s.n) + kKeys - 1) / kKeys;
+}
+// units of a head's first i pairs, i < pairs_of
+__device__ __forceinline__ u64 units_before(const Params& p, const Seq& s, int i) {
+  return floor_sum(i, kKeys, 2 * p.tpt, (u64)s.before + 2 * p.tpt + kKeys - 1);
+}
+__device__ __forceinline__ u64 units_of(const Params& p, const Seq& s) {   // of a head
+  return s.n ? units_before(p, s, pairs_of(p, s) - 1) + tiles_to(s, s.n) : 0;
+}
+
+// Where a stretch is: every role walks the same way.
+struct Walk {
+  Seq s;
+  int b, h, i, j;
+  u64 left;
+};
+// A stretch's share of a pair: key tiles [j0, j1) of nk.
+struct Segment {
+  Seq s;
+  int b, h, i, j0, j1, nk;
+  // tile t's part of them ends here
+  __device__ __forceinline__ int end(const Params& p, int t) const {
+    const int first = (2 * i + t) * p.tpt;
+    return first < s.n ? min(j1, tiles_to(s, first + p.tpt)) : j0;
+  }
+};
+// The next segment; the whole warp calls it.
+__device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& g) {
+  if (w.left == 0) return false;
+  g.s = w.s;
+  g.b = w.b; g.h = w.h; g.i = w.i; g.j0 = w.j;
+  g.nk = tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
+  g.j1 = (int)min((u64)g.nk, w.j + w.left);
+  w.left -= g.j1 - g.j0;
+  w.j = 0;
+  if (w.left == 0 || ++w.i < pairs_of(p, w.s)) return true;
+  w.i = 0;
+  if (++w.h < p.Hkv) return true;
+  w.h = 0;
+  const int lane = threadIdx.x % 32;
+  for (int b0 = w.b + 1; b0 < p.B; b0 += 32) {   // the next sequence with new tokens
+    const Seq s = b0 + lane < p.B ? sequence(p, b0 + lane) : Seq{0, 0, 0};
+    const uint32_t some = __ballot_sync(0xffffffffu, s.n > 0);
+    if (!some) continue;
+    const int l = __ffs(some) - 1;
+    w.b = b0 + l;
+    w.s.start = __shfl_sync(0xffffffffu, s.start, l);
+    w.s.n = __shfl_sync(0xffffffffu, s.n, l);
+    w.s.before = __shfl_sync(0xffffffffu, s.before, l);
+    return true;
+  }
+  w.left = 0;
+  return true;
+}
+
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+struct Shared {
+  Walk first;
+  u64 at, chunk;
+  uint32_t tmem;
+  volatile int abort;
+};
+
+// The CTA's stretch, from the lengths: all threads; `groups` holds a number for every 32
+// sequences.
+__device__ __forceinline__ void plan(const Params& p, u64* groups, Shared& sh) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = (p.B + 31) / 32;
+  for (int i = warp; i < n; i += kWarps) {
+    const int b = 32 * i + lane;
+    const u64 units = warp_sum(b < p.B ? units_of(p, sequence(p, b)) * p.Hkv : 0);
+    if (lane == 0) groups[i] = units;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    u64 total = 0;
+    for (int i = lane; i < n; i += 32) total += groups[i];
+    total = warp_sum(total);
+    const u64 chunk = max((total + gridDim.x - 1) / gridDim.x, (u64)1);
+    const u64 at = min(total, blockIdx.x * chunk);
+    Walk w{};
+    w.left = min(chunk, total - at);
+    if (w.left) {
+      u64 rest = at;   // units between the ones passed over and `at`
+      // of 32 runs, the first that holds `rest`, which becomes its offset there; 32: none
+      auto holds = [&](u64 run) {
+        u64 incl = run;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 up = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += up;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, incl > rest);
+        const int l = past ? __ffs(past) - 1 : 32;
+        rest -= __shfl_sync(0xffffffffu, past ? incl - run : incl, min(l, 31));
+        return l;
+      };
+      int g = 0, l = 32;
+      for (; l == 32 && g < n; g += l == 32 ? 32 : l) l = holds(g + lane < n ? groups[g + lane] : 0);
+      const int b = 32 * g + lane;
+      Seq s = b < p.B ? sequence(p, b) : Seq{0, 0, 0};
+      u64 units = units_of(p, s);   // of a head
+      l = min(holds(units * p.Hkv), 31);
+      w.b = 32 * g + l;
+      w.s.start = __shfl_sync(0xffffffffu, s.start, l);
+      w.s.n = __shfl_sync(0xffffffffu, s.n, l);
+      w.s.before = __shfl_sync(0xffffffffu, s.before, l);
+      units = __shfl_sync(0xffffffffu, units, l);
+      w.h = (int)(rest / units);
+      rest -= w.h * units;
+      int lo = 0, span = pairs_of(p, w.s);   // the pair is one of [lo, lo + span)
+      while (span > 1) {
+        const int step = (span + 31) / 32, i = lo + lane * step;
+        const bool le = lane * step < span && units_before(p, w.s, i) <= rest;
+        const int k = 31 - __clz(__ballot_sync(0xffffffffu, le));
+        lo += k * step;
+        span = min(step, span - k * step);
+      }
+      w.i = lo;
+      w.j = (int)(rest - units_before(p, w.s, lo));
+    }
+    if (lane == 0) {
+      sh.first = w;
+      sh.at = at;
+      sh.chunk = chunk;
+      // for the merge: the pair that the stretch begins in
+      Open o{};
+      if (w.left) {
+        o.begin = at - w.j;
+        o.end = o.begin + tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
+        o.at = at;
+        o.chunk = chunk;
+        o.token = w.s.start + w.i * 2 * p.tpt;
+        o.tokens = w.s.n - w.i * 2 * p.tpt;
+        o.head = w.h;
+        o.mid = w.j > 0;
+      }
+      p.open[blockIdx.x] = o;
+    }
+  }
+  // the counts' place is the ring's, which asynchronous copies write next
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+}
+
+// ---- the kernel ----------------------------------------------------------------------
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                 const __grid_constant__ Params p) {
+  using C = Cfg<D>;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ Shared sh;
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  unsigned char* smem = smem_raw + (base - raw);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t bars = base + C::kOffBar;
+  auto kv_full = [&](int s) { return bars + 8u * s; };
+  auto kv_empty = [&](int s) { return bars + 8u * (C::kStages + s); };
+  auto q_full = [&](int t) { return bars + 8u * (2 * C::kStages + t); };
+  auto s_full = [&](int t) { return bars + 8u * (2 * C::kStages + 2 + t); };
+  auto p_full = [&](int t) { return bars + 8u * (2 * C::kStages + 4 + t); };
+  auto pv_done = [&](int t) { return bars + 8u * (2 * C::kStages + 6 + t); };
+  const uint32_t drained = bars + 8u * (2 * C::kStages + 8);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(kv_full(s), 1);
+      mbar_init(kv_empty(s), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(q_full(t), 4);
+      mbar_init(s_full(t), 1);
+      mbar_init(p_full(t), 4);
+      mbar_init(pv_done(t), 1);
+    }
+    mbar_init(drained, 1);
+    sh.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  plan(p, reinterpret_cast<u64*>(smem), sh);   // ends with a barrier
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  Walk w = sh.first;
+  Segment g;
+  auto fail = [&]() {
+    sh.abort = 1;
+    atomicOr(p.dev_err, ANVILQ_DEV_ERR_TIMEOUT);
+  };
+  auto wait = [&](uint32_t bar, uint32_t parity) {   // the whole warp; false: leave
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, &sh.abort));
+    if (!ok && lane == 0) fail();
+    return ok;
+  };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == kKWarp || warp == kVWarp) {
+      // ------------------------------------------------------------------ TMA
+      const CUtensorMap* map = warp == kKWarp ? &mk : &mv;
+      const int boxes = kKeys / p.box, box_bytes = p.box * 128;
+      const int my_box = lane % boxes, my_half = lane / boxes;   // at most 8 x 2 copies
+      unsigned seq = warp - kKWarp, issued = 0;                  // K and V tiles alternate in the ring
+      bool ok = true;
+      while (ok && next_segment(p, w, g)) {
+        const int len = g.s.before + g.s.n;
+        for (int j = g.j0; j < g.j1; ++j, seq += 2) {
+          const int stage = seq % C::kStages;
+          // the lane's box: its page is looked up while the stage is waited for
+          const int key = j * kKeys + my_box * p.box;
+          const bool live = my_half < C::kHalves && key < len;
+          int page = live ? q8::page_of(p.page_table, p.max_pages, p.num_pages, g.b, key / p.page_tokens) : 0;
+          if (page < 0) {   // the output is not to be used
+            atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
+            page = 0;
+          }
+          ok = wait(kv_empty(stage), ((seq / C::kStages) & 1) ^ 1);
+          if (!ok) break;
+          const int copies = __popc(__ballot_sync(0xffffffffu, live));
+          if (lane == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kv_full(stage)),
+                         "r"(copies * box_bytes)
+                         : "memory");
+          __syncwarp();
+          if (live)
+            tma_2d(base + stage * C::kTileBytes + my_half * (kKeys * 128) + my_box * box_bytes, map,
+                   g.h * D + my_half * 64, page * p.page_tokens + key % p.page_tokens, kv_full(stage));
+          __syncwarp();
+          issued = seq + 1;
+        }
+      }
+      if (sh.abort && lane == 0) {   // let the copies in flight land before the CTA exits
+        for (int i = 0; i < C::kStages; i += 2) {
+          const int s = (int)issued - 1 - i;
+          if (s >= 0) mbar_drain(kv_full(s % C::kStages), (s / C::kStages) & 1);
+        }
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------------ MMA
+      constexpr uint32_t idesc_s = instr_desc(kKeys, false), idesc_o = instr_desc(D, true);
+      unsigned seq = 0;                      // of K; V's is the next
+      unsigned segments[2] = {0, 0}, steps[2] = {0, 0};   // of a tile so far
+      bool ok = true;
+      auto score = [&](int t, int stage) {   // S_t = Q_t K^T
+        if (elect_one()) {
+          const uint32_t a = base + C::kOffQ + t * C::kTileBytes, b = base + stage * C::kTileBytes;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = (k / 4) * (kKeys * 128) + (k % 4) * 32;
+            mma_ss(tmem + t * kKeys, smem_desc(a + at, 16, 1024), smem_desc(b + at, 16, 1024), idesc_s, k > 0);
+          }
+          tc_commit(s_full(t));
+        }
+        __syncwarp();
+      };
+      while (ok && next_segment(p, w, g)) {
+        const int end[2] = {g.end(p, 0), g.end(p, 1)};
+        for (int j = g.j0 - 1; ok && j < g.j1; ++j) {
+          // products of tile j (none before the first), scores of tile j + 1
+          const bool products = j >= g.j0, scores = j + 1 < g.j1;
+          const int vs = (seq - 1) % C::kStages, ks = seq % C::kStages;   // V of j, K of j + 1
+          if (scores) ok = wait(kv_full(ks), (seq / C::kStages) & 1);
+          if (ok && products) {
+            ok = wait(kv_full(vs), ((seq - 1) / C::kStages) & 1);
+            // rows behind the sequence's last token may hold anything: times p = 0 they must be 0
+            const int live = g.s.before + g.s.n - j * kKeys;
+            if (ok && live < kKeys) {
+              const uint32_t v = base + vs * C::kTileBytes;
+              for (int i = live * 8 + lane; i < kKeys * 8; i += 32)
+#pragma unroll
+                for (int h = 0; h < C::kHalves; ++h)
+                  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * (kKeys * 128) + i * 16), "r"(0)
+                               : "memory");
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok) break;
+            if (products && j < end[t]) {
+              ok = wait(p_full(t), steps[t] & 1);
+              if (!ok) break;
+              tc_fence_after();
+              if (elect_one()) {
+                const uint32_t v = base + vs * C::kTileBytes;
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k)
+                  mma_ts(tmem + kTmemO + t * 128, tmem + t * kKeys + k * 8, smem_desc(v + k * 2048, kKeys * 128, 1024),
+                         idesc_o, (j > g.j0 || k > 0) ? 1u : 0u);
+                tc_commit(pv_done(t));
+              }
+              __syncwarp();
+              ++steps[t];
+            }
+            if (scores && j + 1 < end[t]) {
+              if (!products) {
+                ok = wait(q_full(t), segments[t] & 1);
+                ++segments[t];
+              }
+              // S goes where the products of the tile's last step read P
+              if (ok && steps[t]) ok = wait(pv_done(t), (steps[t] - 1) & 1);
+              if (!ok) break;
+              tc_fence_after();
+              score(t, ks);
+            }
+          }
+          if (ok && elect_one()) {
+            if (products) tc_commit(kv_empty(vs));
+            if (scores) tc_commit(kv_empty(ks));
+          }
+          __syncwarp();
+          if (scores) seq += 2;
+        }
+      }
+      if (sh.abort) {   // MMAs still running write TMEM
+        if (elect_one()) tc_commit(drained);
+        __syncwarp();
+        mbar_drain(drained, 0);
+      }
+    }
+  } else {
+    // -------------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp / 4, row = threadIdx.x % kRows;
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
+    const uint32_t s_at = tmem + t * kKeys + lanes, o_at = tmem + kTmemO + t * 128 + lanes;
+    const int of_token = row / p.group, of_head = row % p.group;
+    unsigned steps = 0;
+    bool ok = true, first_seg = true;
+    while (ok && next_segment(p, w, g)) {
+      const int end = g.end(p, t), first = (2 * g.i + t) * p.tpt;   // the tile's first token
+      const bool mine = of_token < p.tpt && first + of_token < g.s.n;
+      const bool whole = g.j0 == 0 && g.j1 == g.nk;
+      float m = kNone, sum = 0.0f;
+      if (end > g.j0) {
+        // ---- Q: 16 lanes a row, into the swizzled tile ----
+        const uint32_t qt = base + C::kOffQ + t * C::kTileBytes;
+        constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks;     // 16-byte pieces of a row; rows of a pass
+        for (int r0 = warp % 4 * 32; r0 < warp % 4 * 32 + 32; r0 += kAtOnce) {
+          const int r = r0 + lane / kChunks, c = lane % kChunks, token = r / p.group;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (token < p.tpt && first + token < g.s.n)
+            v = *reinterpret_cast<const uint4*>(p.q + (long long)(g.s.start + first + token) * p.q_stride +
+                                                (g.h * p.group + r % p.group) * D + c * 8);
+          const uint32_t at = qt + (c / 8) * (kKeys * 128) + r * 128 + (((c % 8) ^ (r & 7)) * 16);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                       : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full(t));
+      }
+      const int pos = g.s.before + min(first + of_token, g.s.n - 1);
+      for (int j = g.j0; j < end; ++j, ++steps) {
+        ok = wait(s_full(t), steps & 1);
+        if (!ok) break;
+        tc_fence_after();
+        float s[kKeys];
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 32) tmem_ld32(s_at + c, reinterpret_cast<uint32_t*>(s) + c);
+        wait_ld();
+        const int visible = pos + 1 - j * kKeys;   // keys of the tile that the row sees
+        if (__any_sync(0xffffffffu, visible < kKeys)) {
+#pragma unroll
+          for (int c = 0; c < kKeys; ++c) s[c] = c < visible ? s[c] : -INFINITY;
+        }
+        float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < kKeys; ++c) tops[c % 4] = fmaxf(tops[c % 4], s[c]);
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;
+        const bool moves = top > m + kSlack;
+        if (__any_sync(0xffffffffu, moves)) {
+          const float now = moves ? top : m, f = fast_exp2(m - now);
+          m = now;
+          sum *= f;
+          if (j > g.j0) {
+            ok = wait(pv_done(t), (steps - 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_at + c, o);
+              wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(o_at + c, o);
+            }
+          }
+        }
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 64) {
+          uint32_t half[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float a = fast_exp2(fmaf(s[c + 2 * e], p.scale_log2, -m));
+            const float b = fast_exp2(fmaf(s[c + 2 * e + 1], p.scale_log2, -m));
+            part[e % 4] += a + b;
+            const __half2 h = __floats2half2_rn(a, b);
+            half[e] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          tmem_st32(s_at + c / 2, half);
+        }
+        wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(t));
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+      }
+      if (!ok) break;
+      // ---- O: the rows' outputs, or their sums for the merge ----
+      float* slot = nullptr;
+      if (!whole) {
+        slot = p.partials + ((size_t)blockIdx.x * 2 + (first_seg && g.j0 > 0 ? 0 : 1)) * (2 * kRows * (D + 2));
+        if (mine) reinterpret_cast<float2*>(slot + 2 * kRows * D)[t * kRows + row] = make_float2(m, sum);
+      }
+      first_seg = false;
+      if (end > g.j0) {
+        ok = wait(pv_done(t), (steps - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // (nothing but scores of -inf: zeros)
+        __half* out = p.out + ((long long)(g.s.start + first + of_token) * p.Hq + g.h * p.group + of_head) * D;
+        float* part = whole ? nullptr : slot + (t * kRows + row) * D;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_at + c, o);
+          wait_ld();
+          if (!mine) continue;
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 v;
+              __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                h[k] = __floats2half2_rn(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
+              *reinterpret_cast<uint4*>(out + c + e) = v;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              __stcg(reinterpret_cast<uint4*>(part + c + e), make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+          }
+        }
+        tc_fence_before();
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ---- the merge of pairs that several CTAs share ---------------------------------------
+
+constexpr int kMergeRows = 32, kMergeThreads = 256;
+
+template <int D>
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // block y is of the pair that CTA y + 1 goes on with, if CTA y began it
+  const int second = blockIdx.y + 1;
+  const Open o = p.open[second];
+  if (!o.mid || o.begin + o.chunk < o.at) return;
+  const int last = (int)((o.end - 1) / o.chunk);   // the CTA that ends it
+  constexpr int kVec = D / 4, kMine = kMergeRows * kVec / kMergeThreads;
+  constexpr size_t kSlot = 2 * kRows * (D + 2);
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = i * kMergeThreads + threadIdx.x, r = blockIdx.x * kMergeRows + at / kVec, d = at % kVec * 4;
+    const int token = r / kRows * p.tpt + r % kRows / p.group;
+    if (r % kRows / p.group >= p.tpt || token >= o.tokens) continue;
+    float m = kNone, sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c = second - 1; c <= last; ++c) {
+      // the pair is the last of the CTA that began it, the first of the others
+      const float* slot = p.partials + ((size_t)c * 2 + (c < second)) * kSlot;
+      const float2 state = __ldcg(reinterpret_cast<const float2*>(slot + 2 * kRows * D) + r);
+      if (!(state.y > 0.0f) && state.y == state.y) continue;   // the row saw nothing there
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(slot + (size_t)r * D + d));
+      const float now = fmaxf(m, state.x), f = fast_exp2(m - now), e = fast_exp2(state.x - now);
+      m = now;
+      sum = sum * f + state.y * e;
+      acc.x = acc.x * f + v.x * e;
+      acc.y = acc.y * f + v.y * e;
+      acc.z = acc.z * f + v.z * e;
+      acc.w = acc.w * f + v.w * e;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint2 w;
+    __half2* h = reinterpret_cast<__half2*>(&w);
+    h[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
+    h[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(p.out + ((long long)(o.token + token) * p.Hq + o.head * p.group + r % kRows % p.group) * D + d) = w;
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------
+static bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// 128 products of two binary16 values, times it, stay far above kNone
+constexpr float kMaxScale = 0x1p32f;
+
+static bool shape_ok(int T, int B, int Hq, int Hkv, int D) {
+  return T >= 0 && T <= (1 << 30) && B >= 1 && B < kMaxBatch && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hq <= 1024 &&
+         Hq / Hkv <= kRows && (D == 64 || D == 128);
+}
+
+constexpr int kMaxDevices = 64;
+static int g_sms[kMaxDevices];
+static std::once_flag g_once[kMaxDevices];
+static int sm_count() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  std::call_once(g_once[dev], [dev] {
+    cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    cudaFuncSetAttribute(chunk_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<64>::kSmem);
+    cudaFuncSetAttribute(chunk_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<128>::kSmem);
+    cudaGetLastError();
+  });
+  return g_sms[dev];
+}
+
+static std::once_flag g_encode_once;
+static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+
+// A pool as a matrix of positions, each a row of all heads: a box is 64 dims of `box` of them.
+static bool pool_map(CUtensorMap* map, const void* pool, long long rows, int width, int box) {
+  std::call_once(g_encode_once, [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    cudaGetLastError();
+  });
+  if (!g_encode) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)width * 2};
+  const cuuint32_t boxes[2] = {64, (cuuint32_t)box};
+  const cuuint32_t estr[2] = {1, 1};
+  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(pool), dims, strides, boxes, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+static int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int ctas, unsigned flags,
+                  cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<D>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = (flags & ANVILQ_GEMM_OVERLAP_PRIOR) ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, chunk_kernel<D>, mk, mv, p) != cudaSuccess) {
+    cudaGetLastError();
+    return ANVILQ_ECUDA;
+  }
+  if (ctas == 1) return ANVILQ_OK;   // nothing is shared
+  cfg.gridDim = dim3(2 * kRows / kMergeRows, ctas - 1);
+  cfg.blockDim = dim3(kMergeThreads);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, merge_kernel<D>, p) != cudaSuccess) {
+    cudaGetLastError();
+    return ANVILQ_ECUDA;
+  }
+  return ANVILQ_OK;
+}
+
+// CTAs of a call: one an SM, no more than there can be units.
+static int ctas_for(int sms, int T, int B, int Hq, int Hkv, long long capacity) {
+  const int tpt = kRows / (Hq / Hkv);
+  const double pairs = ((double)T / (2 * tpt) + std::min(T, B)) * Hkv;
+  return (int)std::max(1.0, std::min({(double)std::min(sms, kMaxCtas), pairs * (double)((capacity + kKeys - 1) / kKeys)}));
+}
+static size_t partial_bytes(int ctas, int D) { return (size_t)ctas * 2 * 2 * kRows * (D + 2) * sizeof(float); }
+
+}  // namespace chunk
+}  // namespace anvilq
+
+extern "C" {
+
+size_t anvilq_gqa_chunk_paged_workspace_size(int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages) {
+  using namespace anvilq::chunk;
+  if (!shape_ok(T, B, Hq, Hkv, D) || page_tokens < 16 || page_tokens % 16 || max_pages < 1 ||
+      (long long)page_tokens * max_pages > (1LL << 30))
+    return 0;
+  const int sms = sm_count();
+  if (sms <= 0) return 0;
+  const int ctas = ctas_for(sms, T, B, Hq, Hkv, (long long)page_tokens * max_pages);
+  return ANVILQ_WORKSPACE_COUNTER_BYTES + partial_bytes(ctas, D) + ctas * sizeof(Open);
+}
+
+int anvilq_gqa_chunk_paged(const uint16_t* q, long long q_stride, const uint16_t* k_pool, const uint16_t* v_pool,
+                           const uint32_t* page_table, const int32_t* seqlens, const int32_t* token_starts,
+                           uint16_t* out, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages,
+                           int num_pages, float scale, void* workspace, size_t workspace_bytes, int* dev_err,
+                           unsigned flags, anvilq_stream_t stream) {
+  using namespace anvilq;
+  using namespace anvilq::chunk;
+  if ((T != 0 && (!q || !out)) || !k_pool || !v_pool || !page_table || !seqlens || !token_starts || !dev_err)
+    return ANVILQ_EINVAL;
+  if (flags & ~(unsigned)ANVILQ_GEMM_OVERLAP_PRIOR) return ANVILQ_EINVAL;
+  if (!std::isfinite(scale) || scale > kMaxScale) return ANVILQ_EINVAL;
+  if (T < 0 || (T > 0 && q_stride < (long long)Hq * D)) return ANVILQ_EINVAL;
+  if (!shape_ok(T, B, Hq, Hkv, D) || page_tokens < 16 || page_tokens % 16 || max_pages < 1 || num_pages < 1 ||
+      (long long)page_tokens * max_pages > (1LL << 30))
+    return ANVILQ_ESHAPE;
+  const long long positions = (long long)num_pages * page_tokens;
+  if (positions > 0x7FFFFFFFLL) return ANVILQ_ESHAPE;   // a TMA coordinate is an int
+  if (!a16(q) || !a16(k_pool) || !a16(v_pool) || !a16(out) || !a16(workspace) || q_stride % 8) return ANVILQ_EALIGN;
+  if (T == 0) return ANVILQ_OK;
+  const size_t pool = (size_t)positions * Hkv * D * 2, rows = (size_t)T * Hq * D * 2;
+  const size_t read = ((size_t)(T - 1) * q_stride + (size_t)Hq * D) * 2;
+  if (overlap(out, rows, q, read) || overlap(out, rows, k_pool, pool) || overlap(out, rows, v_pool, pool) ||
+      overlap(out, rows, page_table, (size_t)B * max_pages * 4) || overlap(out, rows, seqlens, (size_t)B * 4) ||
+      overlap(out, rows, token_starts, (size_t)(B + 1) * 4) ||
+      (workspace && overlap(out, rows, workspace, workspace_bytes)))
+    return ANVILQ_EINVAL;
+  const int sms = sm_count();
+  if (sms <= 0) return ANVILQ_ECUDA;
+  const size_t need = anvilq_gqa_chunk_paged_workspace_size(T, B, Hq, Hkv, D, page_tokens, max_pages);
+  if (!workspace || workspace_bytes < need) return ANVILQ_EWORKSPACE;
+  const int ctas = ctas_for(sms, T, B, Hq, Hkv, (long long)page_tokens * max_pages);
+  Params p{};
+  p.q = reinterpret_cast<const __half*>(q);
+  p.q_stride = q_stride;
+  p.starts = token_starts;
+  p.seqlens = seqlens;
+  p.page_table = page_table;
+  p.out = reinterpret_cast<__half*>(out);
+  char* at = static_cast<char*>(workspace) + ANVILQ_WORKSPACE_COUNTER_BYTES;
+  p.partials = reinterpret_cast<float*>(at);
+  p.open = reinterpret_cast<Open*>(at + partial_bytes(ctas, D));
+  p.dev_err = dev_err;
+  p.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
+  p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
+  p.group = Hq / Hkv;
+  p.tpt = kRows / p.group;
+  p.page_tokens = page_tokens; p.max_pages = max_pages; p.num_pages = num_pages;
+  p.box = 16;
+  while (p.box < kKeys && page_tokens % (2 * p.box) == 0) p.box *= 2;
+  CUtensorMap mk, mv;
+  if (!pool_map(&mk, k_pool, positions, Hkv * D, p.box) || !pool_map(&mv, v_pool, positions, Hkv * D, p.box))
+    return ANVILQ_ECUDA;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return D == 64 ? launch<64>(mk, mv, p, ctas, flags, st) : launch<128>(mk, mv, p, ctas, flags, st);
+}
+
+}  // extern "C"

@@ -920,6 +920,56 @@ def gqa_decode_q8(q, k_codes, v_codes, k_scales, v_scales, page_table, seqlens, 
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _chunk_workspace_size(index, *shape):
+    with torch.cuda.device(index):     # by its number of SMs
+        return _lib.load().anvilq_gqa_chunk_paged_workspace_size(*shape)
+
+
+def gqa_chunk_paged(q, k_pool, v_pool, page_table, seqlens, token_starts, scale: float = 0.0, out=None, dev_err=None,
+                    workspace=None, overlap_prior: bool = False):
+    """GQA attention of a ragged batch's new tokens over a paged fp16 cache: prompts in
+    chunks, questions about long documents, decode steps among them.  q fp16 [T, Hq, D]
+    (tokens may be strided), ``paged_kv_append``'s result; token_starts int32 [B + 1] and
+    seqlens int32 [B] as for it, pools and page_table as for ``gqa_decode_paged``.  Every
+    token sees the positions up to its own.  scale (finite, at most 2^32): of the scores,
+    0 or less for 1/sqrt(D).  Returns out, fp16 [T, Hq, D] (rows of no sequence are left
+    as they are).  workspace: as for ``gqa_decode_q8``.
+
+    attention(q, keys, values) of anvil-q1-fp/tests/fp64_reference.py:164-170, batched."""
+    name = "gqa_chunk_paged"
+    if q.dtype != torch.float16 or k_pool.dtype != torch.float16 or v_pool.dtype != torch.float16:
+        raise TypeError(f"{name}: q and the KV pools must be float16")
+    if q.dim() != 3 or k_pool.dim() != 4 or v_pool.shape != k_pool.shape or not k_pool.is_contiguous() or \
+            not v_pool.is_contiguous():
+        raise ValueError(f"{name}: q [T, Hq, D], k_pool/v_pool contiguous [num_pages, page_tokens, Hkv, D]")
+    (T, Hq, D), (pages, page, Hkv, Dk) = q.shape, k_pool.shape
+    if Dk != D:
+        raise ValueError(f"{name}: head_dim of q and the pools differ")
+    stride, head, inner = q.stride()
+    if (D > 1 and inner != 1) or (Hq > 1 and head != D) or (T > 1 and stride < Hq * D):
+        raise ValueError(f"{name}: heads of q must be contiguous and tokens must not overlap")
+    B, max_pages = _check_table(name, page_table, seqlens)
+    if token_starts.dtype != torch.int32 or token_starts.shape != (B + 1,) or not token_starts.is_contiguous():
+        raise ValueError(f"{name}: token_starts must be a contiguous int32 tensor [{B + 1}]")
+    if out is None:
+        out = q.new_empty((T, Hq, D))
+    elif out.dtype != torch.float16 or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError(f"{name}: out must be contiguous float16 in q's shape")
+    dev = q.device
+    _on_device(name, dev, k_pool, v_pool, page_table, seqlens, token_starts, out)
+    need = _chunk_workspace_size(dev.index, T, B, Hq, Hkv, D, page, max_pages)
+    if need == 0:
+        raise ValueError(f"{name}: unsupported shape T={T} B={B} Hq={Hq} Hkv={Hkv} D={D} pages of {page} tokens")
+    ws = _call_workspace(dev, need, workspace)
+    err = _error_word(dev, dev_err)
+    _call("anvilq_gqa_chunk_paged", dev, q.data_ptr(), stride if T > 1 else Hq * D, k_pool.data_ptr(),
+          v_pool.data_ptr(), page_table.data_ptr(), seqlens.data_ptr(), token_starts.data_ptr(), out.data_ptr(), T, B,
+          Hq, Hkv, D, page, max_pages, pages, float(scale), ws.data_ptr(), ws.numel(), err.data_ptr(),
+          GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
+    return out
+
+
 @functools.lru_cache(maxsize=1024)
 def _logits_workspace_size(B, V):
     return _lib.load().anvilq_logits_process_workspace_size(B, V)

@@ -753,6 +753,34 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
                          int num_pages, float scale, void* workspace, size_t workspace_bytes, int* dev_err,
                          unsigned flags, anvilq_stream_t stream);
 
+/* Attention of the new tokens of a ragged batch over binary16 pages: prompts in chunks,
+ * questions about long documents, decode steps among them.  Token t of sequence b
+ * (token_starts[b] <= t < token_starts[b + 1], as for anvilq_paged_kv_append, which
+ * puts its key and value into the pages before) is at position seqlens[b] -
+ * token_starts[b + 1] + t and sees every position up to its own.  q and out fp16 [T]
+ * tokens of [Hq][D], q's q_stride elements apart (a multiple of 8), out's without
+ * gaps; rows of no sequence are neither read nor written.  Scores, sums and outputs in
+ * fp32, the probabilities enter the tensor cores as binary16.  What lies behind a
+ * sequence's last token may be anything; a NaN or an infinity among the values of new
+ * tokens would reach the queries before them too.  A query whose scores are all -inf
+ * gives zeros.  scale (finite, at most 2^32) <= 0 selects 1/sqrt(D).  Hq % Hkv == 0,
+ * Hq <= 1024, Hq / Hkv <= 128, B <= 65535, T <= 2^30; D, page_tokens and positions as
+ * for the append, at most 2^31 - 1 positions in a pool; 16-byte aligned q, pools, out
+ * and workspace; out apart from all inputs; dev_err required; T == 0 does nothing.
+ * Of the sequences with new tokens, one with more of them than seqlens[b], or longer
+ * than page_tokens * max_pages, sets ANVILQ_DEV_ERR_SEQLEN and its rows are not
+ * written; an absent live page sets ANVILQ_DEV_ERR_PAGE (the output is then not to be
+ * used).  Waits are bounded by ~1 s each; one that expires sets
+ * ANVILQ_DEV_ERR_TIMEOUT, and the output is not to be used.
+ * workspace: anvilq_gqa_chunk_paged_workspace_size bytes (0: not supported), layout as
+ * described at ANVILQ_WORKSPACE_COUNTER_BYTES; its counters are not used. */
+size_t anvilq_gqa_chunk_paged_workspace_size(int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages);
+int anvilq_gqa_chunk_paged(const uint16_t* q, long long q_stride, const uint16_t* k_pool, const uint16_t* v_pool,
+                           const uint32_t* page_table, const int32_t* seqlens, const int32_t* token_starts,
+                           uint16_t* out, int T, int B, int Hq, int Hkv, int D, int page_tokens, int max_pages,
+                           int num_pages, float scale, void* workspace, size_t workspace_bytes, int* dev_err,
+                           unsigned flags, anvilq_stream_t stream);
+
 /* Penalties, biases and grammar masks on B rows of V logits (fp32, or fp16 with
  * logits_half; logits_stride elements apart), and the greedy choice.  For token
  * v of row b, in fp32, each operation rounded:
