@@ -68,7 +68,7 @@ struct Cfg {
   static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kOffQ = kStages * kTileBytes;
   static constexpr int kOffBar = kOffQ + 2 * kTileBytes;
-  static constexpr int kBars = 2 * kStages + 2 * 4 + 1;
+  static constexpr int kBars = 2 * kStages + 2 * 5 + 1;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kSmem = kOffMisc + 128 + 1024;              // + slack to align the base
   static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
@@ -196,6 +196,33 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// two binary32 values at a time
+__device__ __forceinline__ u64 pair(float a, float b) {
+  u64 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 unpair(u64 v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // Shared-memory matrix descriptor: start, leading and stride byte offsets in 16-byte
 // units, version 1, 128-byte swizzle.  K-major: stride between 8-row groups (leading
 // unused).  MN-major: leading between blocks of 64 dims, stride between 8-key groups.
@@ -211,23 +238,25 @@ __host__ __device__ constexpr uint32_t instr_desc(int n, bool b_mn_major) {
 
 // ---- the plan -----------------------------------------------------------------------
 
-// sum of floor((a i + b) / m), i = 0 .. n - 1
-__device__ __forceinline__ u64 floor_sum(u64 n, u64 m, u64 a, u64 b) {
+// sum of floor((a i + b) / m), i = 0 .. n - 1; a n + b below 2^32
+__device__ __forceinline__ u64 floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   u64 sum = 0;
   while (n) {
     if (a >= m) {
-      sum += (n - 1) * n / 2 * (a / m);
-      a %= m;
+      const uint32_t d = a / m;
+      sum += (u64)(n - 1) * n / 2 * d;
+      a -= d * m;
     }
     if (b >= m) {
-      sum += n * (b / m);
-      b %= m;
+      const uint32_t d = b / m;
+      sum += (u64)n * d;
+      b -= d * m;
     }
-    const u64 top = a * n + b;
+    const uint32_t top = a * n + b;
     if (top < m) break;
     n = top / m;
-    b = top % m;
-    const u64 t = m;
+    b = top - n * m;
+    const uint32_t t = m;
     m = a;
     a = t;
   }
@@ -255,7 +284,7 @@ __device__ __forceinline__ int tiles_to(const Seq& s, int tokens) {
 }
 // units of a head's first i pairs, i < pairs_of
 __device__ __forceinline__ u64 units_before(const Params& p, const Seq& s, int i) {
-  return floor_sum(i, kKeys, 2 * p.tpt, (u64)s.before + 2 * p.tpt + kKeys - 1);
+  return floor_sum(i, kKeys, 2 * p.tpt, s.before + 2 * p.tpt + kKeys - 1);
 }
 __device__ __forceinline__ u64 units_of(const Params& p, const Seq& s) {   // of a head
   return s.n ? units_before(p, s, pairs_of(p, s) - 1) + tiles_to(s, s.n) : 0;
@@ -277,18 +306,18 @@ struct Segment {
     return first < s.n ? min(j1, tiles_to(s, first + p.tpt)) : j0;
   }
 };
-// The next segment; the whole warp calls it.
-__device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& g) {
-  if (w.left == 0) return false;
+// The next segment; the whole warp calls it.  Both lie in shared memory, as the softmax
+// needs the registers.
+__device__ __forceinline__ void advance(const Params& p, Walk& w, Segment& g) {
   g.s = w.s;
   g.b = w.b; g.h = w.h; g.i = w.i; g.j0 = w.j;
   g.nk = tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
   g.j1 = (int)min((u64)g.nk, w.j + w.left);
   w.left -= g.j1 - g.j0;
   w.j = 0;
-  if (w.left == 0 || ++w.i < pairs_of(p, w.s)) return true;
+  if (w.left == 0 || ++w.i < pairs_of(p, w.s)) return;
   w.i = 0;
-  if (++w.h < p.Hkv) return true;
+  if (++w.h < p.Hkv) return;
   w.h = 0;
   const int lane = threadIdx.x % 32;
   for (int b0 = w.b + 1; b0 < p.B; b0 += 32) {   // the next sequence with new tokens
@@ -300,9 +329,22 @@ __device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& 
     w.s.start = __shfl_sync(0xffffffffu, s.start, l);
     w.s.n = __shfl_sync(0xffffffffu, s.n, l);
     w.s.before = __shfl_sync(0xffffffffu, s.before, l);
-    return true;
+    return;
   }
   w.left = 0;
+}
+__device__ __forceinline__ bool next_segment(const Params& p, Walk& walk, Segment& seg) {
+  __syncwarp();
+  Walk w = walk;
+  if (w.left == 0) return false;
+  Segment g;
+  advance(p, w, g);
+  __syncwarp();
+  if (threadIdx.x % 32 == 0) {
+    walk = w;
+    seg = g;
+  }
+  __syncwarp();
   return true;
 }
 
@@ -313,8 +355,8 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
 }
 
 struct Shared {
-  Walk first;
-  u64 at, chunk;
+  Walk walk[kWarps];
+  Segment seg[kWarps][2];
   uint32_t tmem;
   volatile int abort;
 };
@@ -323,15 +365,24 @@ struct Shared {
 // sequences.
 __device__ __forceinline__ void plan(const Params& p, u64* groups, Shared& sh) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n = (p.B + 31) / 32;
-  for (int i = warp; i < n; i += kWarps) {
-    const int b = 32 * i + lane;
-    const u64 units = warp_sum(b < p.B ? units_of(p, sequence(p, b)) * p.Hkv : 0);
-    if (lane == 0) groups[i] = units;
+  if (n > 1) {
+    for (int i = warp; i < n; i += kWarps) {
+      const int b = 32 * i + lane;
+      const u64 units = warp_sum(b < p.B ? units_of(p, sequence(p, b)) * p.Hkv : 0);
+      if (lane == 0) groups[i] = units;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (warp == 0) {
-    u64 total = 0;
-    for (int i = lane; i < n; i += 32) total += groups[i];
+    Seq s{0, 0, 0};          // of a group's sequences, the lane's
+    u64 units = 0, total = 0;
+    if (n == 1) {
+      if (lane < p.B) s = sequence(p, lane);
+      units = units_of(p, s);
+      total = units * p.Hkv;
+    } else {
+      for (int i = lane; i < n; i += 32) total += groups[i];
+    }
     total = warp_sum(total);
     const u64 chunk = max((total + gridDim.x - 1) / gridDim.x, (u64)1);
     const u64 at = min(total, blockIdx.x * chunk);
@@ -353,33 +404,35 @@ __device__ __forceinline__ void plan(const Params& p, u64* groups, Shared& sh) {
         return l;
       };
       int g = 0, l = 32;
-      for (; l == 32 && g < n; g += l == 32 ? 32 : l) l = holds(g + lane < n ? groups[g + lane] : 0);
-      const int b = 32 * g + lane;
-      Seq s = b < p.B ? sequence(p, b) : Seq{0, 0, 0};
-      u64 units = units_of(p, s);   // of a head
+      if (n > 1) {
+        for (; l == 32 && g < n; g += l == 32 ? 32 : l) l = holds(g + lane < n ? groups[g + lane] : 0);
+        const int b = 32 * g + lane;
+        s = b < p.B ? sequence(p, b) : Seq{0, 0, 0};
+        units = units_of(p, s);   // of a head
+      }
       l = min(holds(units * p.Hkv), 31);
       w.b = 32 * g + l;
       w.s.start = __shfl_sync(0xffffffffu, s.start, l);
       w.s.n = __shfl_sync(0xffffffffu, s.n, l);
       w.s.before = __shfl_sync(0xffffffffu, s.before, l);
       units = __shfl_sync(0xffffffffu, units, l);
-      w.h = (int)(rest / units);
+      w.h = p.Hkv == 1 ? 0 : (int)(rest / units);
       rest -= w.h * units;
       int lo = 0, span = pairs_of(p, w.s);   // the pair is one of [lo, lo + span)
+      u64 before = 0;                        // units before pair lo
       while (span > 1) {
         const int step = (span + 31) / 32, i = lo + lane * step;
-        const bool le = lane * step < span && units_before(p, w.s, i) <= rest;
-        const int k = 31 - __clz(__ballot_sync(0xffffffffu, le));
+        const u64 mine = lane * step < span ? units_before(p, w.s, i) : rest + 1;
+        const int k = 31 - __clz(__ballot_sync(0xffffffffu, mine <= rest));
+        before = __shfl_sync(0xffffffffu, mine, k);
         lo += k * step;
         span = min(step, span - k * step);
       }
       w.i = lo;
-      w.j = (int)(rest - units_before(p, w.s, lo));
+      w.j = (int)(rest - before);
     }
+    if (lane < kWarps) sh.walk[lane] = w;
     if (lane == 0) {
-      sh.first = w;
-      sh.at = at;
-      sh.chunk = chunk;
       // for the merge: the pair that the stretch begins in
       Open o{};
       if (w.left) {
@@ -417,9 +470,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto kv_empty = [&](int s) { return bars + 8u * (C::kStages + s); };
   auto q_full = [&](int t) { return bars + 8u * (2 * C::kStages + t); };
   auto s_full = [&](int t) { return bars + 8u * (2 * C::kStages + 2 + t); };
-  auto p_full = [&](int t) { return bars + 8u * (2 * C::kStages + 4 + t); };
-  auto pv_done = [&](int t) { return bars + 8u * (2 * C::kStages + 6 + t); };
-  const uint32_t drained = bars + 8u * (2 * C::kStages + 8);
+  auto p_full = [&](int t, int half) { return bars + 8u * (2 * C::kStages + 4 + 2 * t + half); };   // 64 keys each
+  auto pv_done = [&](int t) { return bars + 8u * (2 * C::kStages + 8 + t); };
+  const uint32_t drained = bars + 8u * (2 * C::kStages + 10);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(kv_full(s), 1);
@@ -428,7 +481,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(q_full(t), 4);
       mbar_init(s_full(t), 1);
-      mbar_init(p_full(t), 4);
+      mbar_init(p_full(t, 0), 4);
+      mbar_init(p_full(t, 1), 4);
       mbar_init(pv_done(t), 1);
     }
     mbar_init(drained, 1);
@@ -449,8 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   plan(p, reinterpret_cast<u64*>(smem), sh);   // ends with a barrier
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  Walk w = sh.first;
-  Segment g;
+  Walk& w = sh.walk[warp];
   auto fail = [&]() {
     sh.abort = 1;
     atomicOr(p.dev_err, ANVILQ_DEV_ERR_TIMEOUT);
@@ -470,6 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int my_box = lane % boxes, my_half = lane / boxes;   // at most 8 x 2 copies
       unsigned seq = warp - kKWarp, issued = 0;                  // K and V tiles alternate in the ring
       bool ok = true;
+      Segment& g = sh.seg[warp][0];
       while (ok && next_segment(p, w, g)) {
         const int len = g.s.before + g.s.n;
         for (int j = g.j0; j < g.j1; ++j, seq += 2) {
@@ -521,6 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       };
+      Segment& g = sh.seg[warp][0];
       while (ok && next_segment(p, w, g)) {
         const int end[2] = {g.end(p, 0), g.end(p, 1)};
         for (int j = g.j0 - 1; ok && j < g.j1; ++j) {
@@ -547,18 +602,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int t = 0; t < 2; ++t) {
             if (!ok) break;
             if (products && j < end[t]) {
-              ok = wait(p_full(t), steps[t] & 1);
-              if (!ok) break;
-              tc_fence_after();
-              if (elect_one()) {
-                const uint32_t v = base + vs * C::kTileBytes;
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                  mma_ts(tmem + kTmemO + t * 128, tmem + t * kKeys + k * 8, smem_desc(v + k * 2048, kKeys * 128, 1024),
-                         idesc_o, (j > g.j0 || k > 0) ? 1u : 0u);
-                tc_commit(pv_done(t));
+              for (int half = 0; half < 2; ++half) {
+                ok = ok && wait(p_full(t, half), steps[t] & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                  const uint32_t v = base + vs * C::kTileBytes;
+#pragma unroll
+                  for (int k = 4 * half; k < 4 * half + 4; ++k)
+                    mma_ts(tmem + kTmemO + t * 128, tmem + t * kKeys + k * 8,
+                           smem_desc(v + k * 2048, kKeys * 128, 1024), idesc_o, (j > g.j0 || k > 0) ? 1u : 0u);
+                  if (half) tc_commit(pv_done(t));
+                }
+                __syncwarp();
               }
-              __syncwarp();
+              if (!ok) break;
               ++steps[t];
             }
             if (scores && j + 1 < end[t]) {
@@ -595,30 +654,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_at = tmem + t * kKeys + lanes, o_at = tmem + kTmemO + t * 128 + lanes;
     const int of_token = row / p.group, of_head = row % p.group;
     unsigned steps = 0;
-    bool ok = true, first_seg = true;
-    while (ok && next_segment(p, w, g)) {
+    // Q of a segment: 16 lanes a row, into the swizzled tile.  It may be sent for when the
+    // scores of the segment before it are all there.
+    const uint32_t qt = base + C::kOffQ + t * C::kTileBytes;
+    auto send_for_q = [&](const Segment& g) {
+      const int first = (2 * g.i + t) * p.tpt;
+      constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks;     // 16-byte pieces of a row; rows of a pass
+      const int c = lane % kChunks;
+      int r = warp % 4 * 32 + lane / kChunks, token = r / p.group, head = r % p.group;
+      for (int pass = 0; pass < kChunks; ++pass, r += kAtOnce) {
+        const bool live = token < p.tpt && first + token < g.s.n;
+        const __half* from = p.q + (live ? (long long)(g.s.start + first + token) * p.q_stride +
+                                               (g.h * p.group + head) * D + c * 8 : 0);
+        const uint32_t at = qt + (c / 8) * (kKeys * 128) + r * 128 + (((c % 8) ^ (r & 7)) * 16);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(live ? 16 : 0)
+                     : "memory");   // zeros where it is not live
+        for (head += kAtOnce; head >= p.group; head -= p.group) ++token;
+      }
+    };
+    auto q_is_there = [&]() {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full(t));
+    };
+    int slot_of = 0;
+    bool ok = true, first_seg = true, more = next_segment(p, w, sh.seg[warp][0]);
+    if (more && sh.seg[warp][0].end(p, t) > sh.seg[warp][0].j0) {
+      send_for_q(sh.seg[warp][0]);
+      q_is_there();
+    }
+    while (more) {
+      const Segment& g = sh.seg[warp][slot_of];
       const int end = g.end(p, t), first = (2 * g.i + t) * p.tpt;   // the tile's first token
       const bool mine = of_token < p.tpt && first + of_token < g.s.n;
       const bool whole = g.j0 == 0 && g.j1 == g.nk;
       float m = kNone, sum = 0.0f;
-      if (end > g.j0) {
-        // ---- Q: 16 lanes a row, into the swizzled tile ----
-        const uint32_t qt = base + C::kOffQ + t * C::kTileBytes;
-        constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks;     // 16-byte pieces of a row; rows of a pass
-        for (int r0 = warp % 4 * 32; r0 < warp % 4 * 32 + 32; r0 += kAtOnce) {
-          const int r = r0 + lane / kChunks, c = lane % kChunks, token = r / p.group;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (token < p.tpt && first + token < g.s.n)
-            v = *reinterpret_cast<const uint4*>(p.q + (long long)(g.s.start + first + token) * p.q_stride +
-                                                (g.h * p.group + r % p.group) * D + c * 8);
-          const uint32_t at = qt + (c / 8) * (kKeys * 128) + r * 128 + (((c % 8) ^ (r & 7)) * 16);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                       : "memory");
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full(t));
-      }
       const int pos = g.s.before + min(first + of_token, g.s.n - 1);
       for (int j = g.j0; j < end; ++j, ++steps) {
         ok = wait(s_full(t), steps & 1);
@@ -635,8 +706,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < kKeys; ++c) tops[c % 4] = fmaxf(tops[c % 4], s[c]);
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;
+        for (int c = 4; c + 1 < kKeys; c += 2) tops[c / 2 % 4] = max3(tops[c / 2 % 4], s[c], s[c + 1]);
+        const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * p.scale_log2;
         const bool moves = top > m + kSlack;
         if (__any_sync(0xffffffffu, moves)) {
           const float now = moves ? top : m, f = fast_exp2(m - now);
@@ -657,25 +728,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const u64 scale2 = pair(p.scale_log2, p.scale_log2), ref2 = pair(-m, -m);
+        u64 part[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < kKeys; c += 64) {
           uint32_t half[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float a = fast_exp2(fmaf(s[c + 2 * e], p.scale_log2, -m));
-            const float b = fast_exp2(fmaf(s[c + 2 * e + 1], p.scale_log2, -m));
-            part[e % 4] += a + b;
+            const float2 x = unpair(fma2(pair(s[c + 2 * e], s[c + 2 * e + 1]), scale2, ref2));
+            const float a = fast_exp2(x.x), b = fast_exp2(x.y);
+            part[e % 2] = add2(part[e % 2], pair(a, b));
             const __half2 h = __floats2half2_rn(a, b);
             half[e] = *reinterpret_cast<const uint32_t*>(&h);
           }
           tmem_st32(s_at + c / 2, half);
+          wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full(t, c / 64));
         }
-        wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(t));
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        const float2 both = unpair(add2(part[0], part[1]));
+        sum += both.x + both.y;
       }
       if (!ok) break;
       // ---- O: the rows' outputs, or their sums for the merge ----
@@ -685,10 +758,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (mine) reinterpret_cast<float2*>(slot + 2 * kRows * D)[t * kRows + row] = make_float2(m, sum);
       }
       first_seg = false;
+      // the next segment's Q on its way, and there before O is stored
+      const Segment& next = sh.seg[warp][slot_of ^ 1];
+      more = next_segment(p, w, sh.seg[warp][slot_of ^ 1]);
+      const bool next_q = more && next.end(p, t) > next.j0;
+      if (next_q) send_for_q(next);
       if (end > g.j0) {
         ok = wait(pv_done(t), (steps - 1) & 1);
         if (!ok) break;
         tc_fence_after();
+      }
+      if (next_q) q_is_there();
+      if (end > g.j0) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // (nothing but scores of -inf: zeros)
         __half* out = p.out + ((long long)(g.s.start + first + of_token) * p.Hq + g.h * p.group + of_head) * D;
         float* part = whole ? nullptr : slot + (t * kRows + row) * D;
@@ -716,6 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before();
       }
+      slot_of ^= 1;
     }
   }
   __syncthreads();
@@ -727,46 +809,84 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ---- the merge of pairs that several CTAs share ---------------------------------------
 
-constexpr int kMergeRows = 32, kMergeThreads = 256;
+constexpr int kMergeThreads = 256;
 
+// Resident blocks over (shared pair, rows of a block).  A thread has 4 dims of a row: the
+// states and sums of 16 CTAs on their way at once, then merged as a softmax goes on.
 template <int D>
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ Params p, int ctas) {
+  constexpr int kVec = D / 4, kBlockRows = kMergeThreads / kVec, kSlices = 2 * kRows / kBlockRows, kAtOnce = 16;
+  constexpr size_t kSlot = 2 * kRows * (D + 2);
+  __shared__ int seconds[kMaxCtas];   // the CTAs that go on with a pair that the CTA before them began
+  __shared__ int count[kMergeThreads / 32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  // block y is of the pair that CTA y + 1 goes on with, if CTA y began it
-  const int second = blockIdx.y + 1;
-  const Open o = p.open[second];
-  if (!o.mid || o.begin + o.chunk < o.at) return;
-  const int last = (int)((o.end - 1) / o.chunk);   // the CTA that ends it
-  constexpr int kVec = D / 4, kMine = kMergeRows * kVec / kMergeThreads;
-  constexpr size_t kSlot = 2 * kRows * (D + 2);
+  static_assert(kMaxCtas <= kMergeThreads, "a CTA a thread");
+  bool shared = false;
+  if (threadIdx.x < ctas) {
+    const Open& o = p.open[threadIdx.x];
+    shared = o.mid && o.begin + o.chunk >= o.at;
+  }
+  const uint32_t some = __ballot_sync(0xffffffffu, shared);
+  if (threadIdx.x % 32 == 0) count[threadIdx.x / 32] = __popc(some);
+  __syncthreads();
+  int at = __popc(some & ((1u << threadIdx.x % 32) - 1)), pairs = 0;
 #pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    const int at = i * kMergeThreads + threadIdx.x, r = blockIdx.x * kMergeRows + at / kVec, d = at % kVec * 4;
-    const int token = r / kRows * p.tpt + r % kRows / p.group;
-    if (r % kRows / p.group >= p.tpt || token >= o.tokens) continue;
+  for (int w = 0; w < kMergeThreads / 32; ++w) {
+    if (w < threadIdx.x / 32) at += count[w];
+    pairs += count[w];
+  }
+  if (shared) seconds[at] = threadIdx.x;
+  __syncthreads();
+  const int d = threadIdx.x % kVec * 4;
+  for (int work = blockIdx.x; work < pairs * kSlices; work += gridDim.x) {
+    const int second = seconds[work / kSlices], r = work % kSlices * kBlockRows + threadIdx.x / kVec;
+    const Open o = p.open[second];
+    const int of = r % kRows / p.group, token = r / kRows * p.tpt + of, head = r % kRows % p.group;
+    if (of >= p.tpt || token >= o.tokens) continue;
+    const int n = (int)((o.end - 1) / o.chunk) - second + 2;   // CTAs
+    // the pair is the last of the CTA that began it, the first of the others
+    const float* begin = p.partials + ((size_t)(second - 1) * 2 + 1) * kSlot;
+    const float* others = p.partials + (size_t)second * 2 * kSlot;
     float m = kNone, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int c = second - 1; c <= last; ++c) {
-      // the pair is the last of the CTA that began it, the first of the others
-      const float* slot = p.partials + ((size_t)c * 2 + (c < second)) * kSlot;
-      const float2 state = __ldcg(reinterpret_cast<const float2*>(slot + 2 * kRows * D) + r);
-      if (!(state.y > 0.0f) && state.y == state.y) continue;   // the row saw nothing there
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(slot + (size_t)r * D + d));
-      const float now = fmaxf(m, state.x), f = fast_exp2(m - now), e = fast_exp2(state.x - now);
+    for (int c0 = 0; c0 < n; c0 += kAtOnce) {
+      float2 state[kAtOnce];
+      float4 v[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        state[k] = make_float2(kNone, 0.0f);
+        v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float* slot = c0 + k ? others + (size_t)(c0 + k - 1) * 2 * kSlot : begin;
+        if (c0 + k < n) {
+          state[k] = __ldcg(reinterpret_cast<const float2*>(slot + 2 * kRows * D) + r);
+          v[k] = __ldcg(reinterpret_cast<const float4*>(slot + (size_t)r * D + d));
+        }
+      }
+      float now = m;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) now = fmaxf(now, state[k].x);
+      const float f = fast_exp2(m - now);
       m = now;
-      sum = sum * f + state.y * e;
-      acc.x = acc.x * f + v.x * e;
-      acc.y = acc.y * f + v.y * e;
-      acc.z = acc.z * f + v.z * e;
-      acc.w = acc.w * f + v.w * e;
+      sum *= f;
+      acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        if (state[k].y == 0.0f) continue;   // the row saw nothing there, and there may be no sums either
+        const float e = fast_exp2(state[k].x - now);
+        sum += state[k].y * e;
+        acc.x += v[k].x * e;
+        acc.y += v[k].y * e;
+        acc.z += v[k].z * e;
+        acc.w += v[k].w * e;
+      }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     uint2 w;
     __half2* h = reinterpret_cast<__half2*>(&w);
     h[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
     h[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(p.out + ((long long)(o.token + token) * p.Hq + o.head * p.group + r % kRows % p.group) * D + d) = w;
+    *reinterpret_cast<uint2*>(p.out + ((long long)(o.token + token) * p.Hq + o.head * p.group + head) * D + d) = w;
   }
 }
 
@@ -836,11 +956,11 @@ static int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,
     return ANVILQ_ECUDA;
   }
   if (ctas == 1) return ANVILQ_OK;   // nothing is shared
-  cfg.gridDim = dim3(2 * kRows / kMergeRows, ctas - 1);
+  cfg.gridDim = dim3(std::min(ctas * 32, kMaxCtas * 2));
   cfg.blockDim = dim3(kMergeThreads);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, merge_kernel<D>, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, merge_kernel<D>, p, ctas) != cudaSuccess) {
     cudaGetLastError();
     return ANVILQ_ECUDA;
   }
