@@ -18,18 +18,19 @@
 // tiles in turn keep the tensor cores at one's products while the other's softmax runs.
 //
 // Work split (stream-K).  All (pair, key tile) units in a row, pairs in the order
-// (sequence, kv head, pair), are cut into equal stretches, one a CTA, so lengths do not
+// (sequence, kv head, pair), a unit for each pair's beginning, are cut into equal stretches, one a CTA, so lengths do not
 // matter to the balance and few rows over a long axis are split over it.  A pair that
 // several CTAs share leaves binary32 partial sums in the workspace; a second kernel,
 // launched with the first's end overlapped, merges them in CTA order (bit-reproducible).
 // How many units there are is a sum of rounded linear functions, computed in closed form
 // (floor_sum) by every CTA from the lengths on the device.
 //
-// Warp roles (12 warps, one CTA an SM):
-//   0-3, 4-7   softmax of tile 0 and tile 1: also load its Q, rescale and store its O
-//   8, 9       TMA of K and of V (their boxes are issued side by side: pages of 16
-//              tokens take 16 copies a tile)
-//   10         MMA issuer, TMEM owner; zeroes V's rows behind a sequence's last token
+// Warp roles (16 warps, one CTA an SM):
+//   0-3, 4-7   softmax of tile 0 and tile 1; they rescale its O where they must
+//   8-11       store O, while the next pair's scores are under way
+//   12, 13     TMA of K and of V (side by side: pages of 16 tokens take 16 copies a tile)
+//   14         MMA issuer, TMEM owner; zeroes V's rows behind a sequence's last token
+//   15         TMA of Q
 // K and V tiles share a ring: [half of 64 dims][128 keys][128 bytes], 128-byte swizzle.
 // K is the K-major B operand of S, V the MN-major one of O.
 #include <cuda.h>
@@ -51,9 +52,10 @@ using q8::overlap;
 using u64 = unsigned long long;
 constexpr int kRows = 128;                 // of a tile: MMA M, a TMEM lane each
 constexpr int kKeys = 128;                 // of a step
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kKWarp = 8, kVWarp = 9, kMmaWarp = 10;
+constexpr int kStoreWarp = 8, kKWarp = 12, kVWarp = 13, kMmaWarp = 14, kQWarp = 15;
+constexpr int kSetup = 1;                  // what a pair's beginning costs, in key tiles
 constexpr int kMaxCtas = 148;
 constexpr int kMaxBatch = 65536;
 constexpr float kNone = -1e30f;            // a reference below every exponent
@@ -68,10 +70,8 @@ struct Cfg {
   static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kOffQ = kStages * kTileBytes;
   static constexpr int kOffBar = kOffQ + 2 * kTileBytes;
-  static constexpr int kBars = 2 * kStages + 2 * 5 + 1;
-  static constexpr int kOffMisc = kOffBar + kBars * 8;
-  static constexpr int kSmem = kOffMisc + 128 + 1024;              // + slack to align the base
-  static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
+  static constexpr int kBars = 2 * kStages + 2 * 8 + 1;
+  static constexpr int kOffShared = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static_assert(kMaxBatch / 32 * 8 <= kOffQ, "the groups' counts lie in the ring before its first copy");
 };
 
@@ -91,7 +91,7 @@ struct Params {
 
 // What the merge needs to know of a CTA's first pair.
 struct Open {
-  u64 begin, end;               // its units; the CTA's own begin at `at`
+  u64 begin, end;               // its key tiles' units; the CTA's own begin at `at`
   u64 at, chunk;
   int token, tokens, head, mid; // first token, tokens left in the sequence from it on; mid: begun by an earlier CTA
 };
@@ -145,6 +145,13 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
@@ -186,6 +193,21 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
       "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
       "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -282,18 +304,19 @@ __device__ __forceinline__ int pairs_of(const Params& p, const Seq& s) { return 
 __device__ __forceinline__ int tiles_to(const Seq& s, int tokens) {
   return (s.before + min(tokens, s.n) + kKeys - 1) / kKeys;
 }
-// units of a head's first i pairs, i < pairs_of
+// A pair's units are kSetup for its beginning and one a key tile: of a head's first i
+// pairs, i < pairs_of
 __device__ __forceinline__ u64 units_before(const Params& p, const Seq& s, int i) {
-  return floor_sum(i, kKeys, 2 * p.tpt, s.before + 2 * p.tpt + kKeys - 1);
+  return (u64)i * kSetup + floor_sum(i, kKeys, 2 * p.tpt, s.before + 2 * p.tpt + kKeys - 1);
 }
 __device__ __forceinline__ u64 units_of(const Params& p, const Seq& s) {   // of a head
-  return s.n ? units_before(p, s, pairs_of(p, s) - 1) + tiles_to(s, s.n) : 0;
+  return s.n ? units_before(p, s, pairs_of(p, s) - 1) + kSetup + tiles_to(s, s.n) : 0;
 }
 
 // Where a stretch is: every role walks the same way.
 struct Walk {
   Seq s;
-  int b, h, i, j;
+  int b, h, i, x;   // pair i of head h of sequence b, x units into it
   u64 left;
 };
 // A stretch's share of a pair: key tiles [j0, j1) of nk.
@@ -310,11 +333,13 @@ struct Segment {
 // needs the registers.
 __device__ __forceinline__ void advance(const Params& p, Walk& w, Segment& g) {
   g.s = w.s;
-  g.b = w.b; g.h = w.h; g.i = w.i; g.j0 = w.j;
+  g.b = w.b; g.h = w.h; g.i = w.i;
   g.nk = tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
-  g.j1 = (int)min((u64)g.nk, w.j + w.left);
-  w.left -= g.j1 - g.j0;
-  w.j = 0;
+  const int end = (int)min((u64)(kSetup + g.nk), w.x + w.left);
+  g.j0 = max(0, w.x - kSetup);
+  g.j1 = max(0, end - kSetup);
+  w.left -= end - w.x;
+  w.x = 0;
   if (w.left == 0 || ++w.i < pairs_of(p, w.s)) return;
   w.i = 0;
   if (++w.h < p.Hkv) return;
@@ -345,7 +370,7 @@ __device__ __forceinline__ bool next_segment(const Params& p, Walk& walk, Segmen
     seg = g;
   }
   __syncwarp();
-  return true;
+  return g.j1 > g.j0;   // else the stretch ends in a pair's beginning
 }
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -356,7 +381,8 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
 
 struct Shared {
   Walk walk[kWarps];
-  Segment seg[kWarps][2];
+  Segment seg[kWarps + 1];   // the MMA issuer has two
+  float sums[2][kRows];
   uint32_t tmem;
   volatile int abort;
 };
@@ -429,21 +455,21 @@ __device__ __forceinline__ void plan(const Params& p, u64* groups, Shared& sh) {
         span = min(step, span - k * step);
       }
       w.i = lo;
-      w.j = (int)(rest - before);
+      w.x = (int)(rest - before);
     }
     if (lane < kWarps) sh.walk[lane] = w;
     if (lane == 0) {
       // for the merge: the pair that the stretch begins in
       Open o{};
       if (w.left) {
-        o.begin = at - w.j;
+        o.begin = at - w.x + kSetup;
         o.end = o.begin + tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
         o.at = at;
         o.chunk = chunk;
         o.token = w.s.start + w.i * 2 * p.tpt;
         o.tokens = w.s.n - w.i * 2 * p.tpt;
         o.head = w.h;
-        o.mid = w.j > 0;
+        o.mid = w.x > kSetup;
       }
       p.open[blockIdx.x] = o;
     }
@@ -457,37 +483,44 @@ __device__ __forceinline__ void plan(const Params& p, u64* groups, Shared& sh) {
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    chunk_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                 const __grid_constant__ Params p) {
+    chunk_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ Params p) {
   using C = Cfg<D>;
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ Shared sh;
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  unsigned char* smem = smem_raw + (base - raw);
+  extern __shared__ __align__(1024) unsigned char smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem + C::kOffShared);
+  const uint32_t base = smem_u32(smem);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t bars = base + C::kOffBar;
   auto kv_full = [&](int s) { return bars + 8u * s; };
   auto kv_empty = [&](int s) { return bars + 8u * (C::kStages + s); };
-  auto q_full = [&](int t) { return bars + 8u * (2 * C::kStages + t); };
-  auto s_full = [&](int t) { return bars + 8u * (2 * C::kStages + 2 + t); };
-  auto p_full = [&](int t, int half) { return bars + 8u * (2 * C::kStages + 4 + 2 * t + half); };   // 64 keys each
-  auto pv_done = [&](int t) { return bars + 8u * (2 * C::kStages + 8 + t); };
-  const uint32_t drained = bars + 8u * (2 * C::kStages + 10);
+  auto bar_of = [&](int kind, int t) { return bars + 8u * (2 * C::kStages + 2 * kind + t); };
+  auto q_full = [&](int t) { return bar_of(0, t); };
+  auto q_empty = [&](int t) { return bar_of(1, t); };
+  auto s_full = [&](int t) { return bar_of(2, t); };
+  auto p_full = [&](int t, int half) { return bar_of(3 + half, t); };   // 64 keys each
+  auto pv_done = [&](int t) { return bar_of(5, t); };
+  auto sums_full = [&](int t) { return bar_of(6, t); };
+  auto o_empty = [&](int t) { return bar_of(7, t); };
+  const uint32_t drained = bar_of(8, 0);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(kv_full(s), 1);
       mbar_init(kv_empty(s), 1);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(q_full(t), 4);
+      mbar_init(q_full(t), 1);
+      mbar_init(q_empty(t), 1);
       mbar_init(s_full(t), 1);
       mbar_init(p_full(t, 0), 4);
       mbar_init(p_full(t, 1), 4);
       mbar_init(pv_done(t), 1);
+      mbar_init(sums_full(t), 4);
+      mbar_init(o_empty(t), 4);
     }
     mbar_init(drained, 1);
     sh.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
   }
@@ -504,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   Walk& w = sh.walk[warp];
+  Segment& g = sh.seg[warp];
   auto fail = [&]() {
     sh.abort = 1;
     atomicOr(p.dev_err, ANVILQ_DEV_ERR_TIMEOUT);
@@ -513,17 +547,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) fail();
     return ok;
   };
+  auto expect = [&](uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  };
+  // `uses` of a tile: the segments that it has a part in
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  if (warp >= kStoreWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == kKWarp || warp == kVWarp) {
-      // ------------------------------------------------------------------ TMA
+      // ------------------------------------------------------------------ K and V
       const CUtensorMap* map = warp == kKWarp ? &mk : &mv;
       const int boxes = kKeys / p.box, box_bytes = p.box * 128;
       const int my_box = lane % boxes, my_half = lane / boxes;   // at most 8 x 2 copies
       unsigned seq = warp - kKWarp, issued = 0;                  // K and V tiles alternate in the ring
       bool ok = true;
-      Segment& g = sh.seg[warp][0];
       while (ok && next_segment(p, w, g)) {
         const int len = g.s.before + g.s.n;
         for (int j = g.j0; j < g.j1; ++j, seq += 2) {
@@ -539,10 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = wait(kv_empty(stage), ((seq / C::kStages) & 1) ^ 1);
           if (!ok) break;
           const int copies = __popc(__ballot_sync(0xffffffffu, live));
-          if (lane == 0)
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kv_full(stage)),
-                         "r"(copies * box_bytes)
-                         : "memory");
+          if (lane == 0) expect(kv_full(stage), copies * box_bytes);
           __syncwarp();
           if (live)
             tma_2d(base + stage * C::kTileBytes + my_half * (kKeys * 128) + my_box * box_bytes, map,
@@ -557,87 +591,123 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (s >= 0) mbar_drain(kv_full(s % C::kStages), (s / C::kStages) & 1);
         }
       }
-    } else if (warp == kMmaWarp) {
-      // ------------------------------------------------------------------ MMA
-      constexpr uint32_t idesc_s = instr_desc(kKeys, false), idesc_o = instr_desc(D, true);
-      unsigned seq = 0;                      // of K; V's is the next
-      unsigned segments[2] = {0, 0}, steps[2] = {0, 0};   // of a tile so far
+    } else if (warp == kQWarp) {
+      // ------------------------------------------------------------------ Q
+      // A box is tpt tokens of g heads; tokens behind the sequence's are other rows, that
+      // are not stored, tokens behind the last zeros.
+      unsigned uses[2] = {0, 0};
       bool ok = true;
-      auto score = [&](int t, int stage) {   // S_t = Q_t K^T
-        if (elect_one()) {
-          const uint32_t a = base + C::kOffQ + t * C::kTileBytes, b = base + stage * C::kTileBytes;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t at = (k / 4) * (kKeys * 128) + (k % 4) * 32;
-            mma_ss(tmem + t * kKeys, smem_desc(a + at, 16, 1024), smem_desc(b + at, 16, 1024), idesc_s, k > 0);
-          }
-          tc_commit(s_full(t));
-        }
-        __syncwarp();
-      };
-      Segment& g = sh.seg[warp][0];
       while (ok && next_segment(p, w, g)) {
-        const int end[2] = {g.end(p, 0), g.end(p, 1)};
-        for (int j = g.j0 - 1; ok && j < g.j1; ++j) {
-          // products of tile j (none before the first), scores of tile j + 1
-          const bool products = j >= g.j0, scores = j + 1 < g.j1;
-          const int vs = (seq - 1) % C::kStages, ks = seq % C::kStages;   // V of j, K of j + 1
-          if (scores) ok = wait(kv_full(ks), (seq / C::kStages) & 1);
-          if (ok && products) {
-            ok = wait(kv_full(vs), ((seq - 1) / C::kStages) & 1);
-            // rows behind the sequence's last token may hold anything: times p = 0 they must be 0
-            const int live = g.s.before + g.s.n - j * kKeys;
-            if (ok && live < kKeys) {
-              const uint32_t v = base + vs * C::kTileBytes;
-              for (int i = live * 8 + lane; i < kKeys * 8; i += 32)
 #pragma unroll
-                for (int h = 0; h < C::kHalves; ++h)
-                  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * (kKeys * 128) + i * 16), "r"(0)
-                               : "memory");
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-            }
-          }
+        for (int t = 0; t < 2; ++t) {
+          if (g.end(p, t) <= g.j0) continue;
+          ok = ok && wait(q_empty(t), (uses[t] & 1) ^ 1);
+          if (!ok) break;
+          if (elect_one()) {
+            expect(q_full(t), C::kHalves * p.group * p.tpt * 128);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (!ok) break;
-            if (products && j < end[t]) {
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                ok = ok && wait(p_full(t, half), steps[t] & 1);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-                  const uint32_t v = base + vs * C::kTileBytes;
-#pragma unroll
-                  for (int k = 4 * half; k < 4 * half + 4; ++k)
-                    mma_ts(tmem + kTmemO + t * 128, tmem + t * kKeys + k * 8,
-                           smem_desc(v + k * 2048, kKeys * 128, 1024), idesc_o, (j > g.j0 || k > 0) ? 1u : 0u);
-                  if (half) tc_commit(pv_done(t));
-                }
-                __syncwarp();
-              }
-              if (!ok) break;
-              ++steps[t];
-            }
-            if (scores && j + 1 < end[t]) {
-              if (!products) {
-                ok = wait(q_full(t), segments[t] & 1);
-                ++segments[t];
-              }
-              // S goes where the products of the tile's last step read P
-              if (ok && steps[t]) ok = wait(pv_done(t), (steps[t] - 1) & 1);
-              if (!ok) break;
-              tc_fence_after();
-              score(t, ks);
-            }
-          }
-          if (ok && elect_one()) {
-            if (products) tc_commit(kv_empty(vs));
-            if (scores) tc_commit(kv_empty(ks));
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_3d(base + C::kOffQ + t * C::kTileBytes + h * (kRows * 128), &mq, h * 64, g.h * p.group,
+                     g.s.start + (2 * g.i + t) * p.tpt, q_full(t));
           }
           __syncwarp();
-          if (scores) seq += 2;
+          ++uses[t];
+        }
+      }
+      if (sh.abort && lane == 0)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (uses[t]) mbar_drain(q_full(t), (uses[t] - 1) & 1);
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------------ MMA
+      // Step by step through all segments: the products of one key tile beside the scores
+      // of the next, of the next pair where it is the last.
+      constexpr uint32_t idesc_s = instr_desc(kKeys, false), idesc_o = instr_desc(D, true);
+      unsigned seq = 0;                                    // of the scores' K; its V is the next
+      unsigned steps[2] = {0, 0}, q_uses[2] = {0, 0}, o_uses[2] = {0, 0};
+      int slot = 0;
+      auto seg = [&](int i) -> Segment& { return sh.seg[i ? kWarps : kMmaWarp]; };
+      bool ok = true, products = false, scores = next_segment(p, w, seg(0));
+      int j = 0, j0 = 0, end[2] = {0, 0}, live = 0;        // of the products
+      int sj = seg(0).j0, s_end[2] = {seg(0).end(p, 0), seg(0).end(p, 1)};   // of the scores
+      while (ok && (products || scores)) {
+        const Segment& n = seg(slot);
+        const int vs = (seq - 1) % C::kStages, ks = seq % C::kStages;
+        if (scores) ok = wait(kv_full(ks), (seq / C::kStages) & 1);
+        if (ok && products) {
+          ok = wait(kv_full(vs), ((seq - 1) / C::kStages) & 1);
+          // rows behind the sequence's last token may hold anything: times p = 0 they must be 0
+          if (ok && live < kKeys) {
+            const uint32_t v = base + vs * C::kTileBytes;
+            for (int i = live * 8 + lane; i < kKeys * 8; i += 32)
+#pragma unroll
+              for (int h = 0; h < C::kHalves; ++h)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * (kKeys * 128) + i * 16), "r"(0)
+                             : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (ok && products && j < end[t]) {
+            if (j == j0) ok = wait(o_empty(t), (o_uses[t]++ & 1) ^ 1);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              ok = ok && wait(p_full(t, half), steps[t] & 1);
+              if (!ok) break;
+              tc_fence_after();
+              if (elect_one()) {
+                const uint32_t v = base + vs * C::kTileBytes;
+#pragma unroll
+                for (int k = 4 * half; k < 4 * half + 4; ++k)
+                  mma_ts(tmem + kTmemO + t * 128, tmem + t * kKeys + k * 8,
+                         smem_desc(v + k * 2048, kKeys * 128, 1024), idesc_o, (j > j0 || k > 0) ? 1u : 0u);
+                if (half) tc_commit(pv_done(t));
+              }
+              __syncwarp();
+            }
+            ++steps[t];
+          }
+          if (ok && scores && sj < s_end[t]) {
+            if (sj == n.j0) ok = wait(q_full(t), q_uses[t]++ & 1);
+            // S goes where the products of the tile's last step read P
+            if (ok && steps[t]) ok = wait(pv_done(t), (steps[t] - 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {   // S_t = Q_t K^T
+              const uint32_t a = base + C::kOffQ + t * C::kTileBytes, b = base + ks * C::kTileBytes;
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t at = (k / 4) * (kKeys * 128) + (k % 4) * 32;
+                mma_ss(tmem + t * kKeys, smem_desc(a + at, 16, 1024), smem_desc(b + at, 16, 1024), idesc_s, k > 0);
+              }
+              tc_commit(s_full(t));
+              if (sj + 1 == s_end[t]) tc_commit(q_empty(t));
+            }
+            __syncwarp();
+          }
+        }
+        if (ok && elect_one()) {
+          if (products) tc_commit(kv_empty(vs));
+          if (scores) tc_commit(kv_empty(ks));
+        }
+        __syncwarp();
+        // on to the next step
+        products = scores;
+        if (!scores) break;
+        seq += 2;
+        j = sj;
+        j0 = n.j0;
+        live = n.s.before + n.s.n - j * kKeys;
+        end[0] = s_end[0];
+        end[1] = s_end[1];
+        if (++sj == n.j1) {
+          slot ^= 1;
+          scores = next_segment(p, w, seg(slot));
+          sj = seg(slot).j0;
+          s_end[0] = seg(slot).end(p, 0);
+          s_end[1] = seg(slot).end(p, 1);
         }
       }
       if (sh.abort) {   // MMAs still running write TMEM
@@ -645,53 +715,77 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         mbar_drain(drained, 0);
       }
+    } else {
+      // ------------------------------------------------------------------ stores
+      const int row = warp % 4 * 32 + lane, of_token = row / p.group, of_head = row % p.group;
+      unsigned steps[2] = {0, 0}, uses[2] = {0, 0};
+      bool ok = true, first_seg = true;
+      while (ok && next_segment(p, w, g)) {
+        const bool whole = g.j0 == 0 && g.j1 == g.nk;
+        float4* slot = reinterpret_cast<float4*>(
+            p.partials + ((size_t)blockIdx.x * 2 + (first_seg && g.j0 > 0 ? 0 : 1)) * (2 * kRows * (D + 2)));
+        first_seg = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int end = g.end(p, t), first = (2 * g.i + t) * p.tpt;
+          if (!ok || end <= g.j0) continue;
+          const bool mine = of_token < p.tpt && first + of_token < g.s.n;
+          steps[t] += end - g.j0;
+          ok = wait(sums_full(t), uses[t]++ & 1) && wait(pv_done(t), (steps[t] - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const float sum = sh.sums[t][row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // (only scores of -inf: zeros)
+          __half* out = p.out + ((long long)(g.s.start + first + of_token) * p.Hq + g.h * p.group + of_head) * D;
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(tmem + kTmemO + t * 128 + ((uint32_t)(warp % 4 * 32) << 16) + c, o);
+            wait_ld();
+            if (c + 32 == D) {   // the tile's sums are out of TMEM
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(o_empty(t));
+            }
+            if (!mine) continue;
+            if (whole) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 16) {   // a sector at a time
+                uint32_t v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  const __half2 h = __floats2half2_rn(__uint_as_float(o[e + 2 * k]) * inv,
+                                                      __uint_as_float(o[e + 2 * k + 1]) * inv);
+                  v[k] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c + e), "r"(v[0]),
+                             "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                             : "memory");
+              }
+            } else {   // [dims / 4][row]
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                __stcg(slot + (c + e) / 4 * (2 * kRows) + t * kRows + row,
+                       make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                   __uint_as_float(o[e + 3])));
+            }
+          }
+        }
+      }
     }
   } else {
     // -------------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int t = warp / 4, row = threadIdx.x % kRows;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t s_at = tmem + t * kKeys + lanes, o_at = tmem + kTmemO + t * 128 + lanes;
-    const int of_token = row / p.group, of_head = row % p.group;
-    unsigned steps = 0;
-    // Q of a segment: 16 lanes a row, into the swizzled tile.  It may be sent for when the
-    // scores of the segment before it are all there.
-    const uint32_t qt = base + C::kOffQ + t * C::kTileBytes;
-    auto send_for_q = [&](const Segment& g) {
-      const int first = (2 * g.i + t) * p.tpt;
-      constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks;     // 16-byte pieces of a row; rows of a pass
-      const int c = lane % kChunks;
-      int r = warp % 4 * 32 + lane / kChunks, token = r / p.group, head = r % p.group;
-      for (int pass = 0; pass < kChunks; ++pass, r += kAtOnce) {
-        const bool live = token < p.tpt && first + token < g.s.n;
-        const __half* from = p.q + (live ? (long long)(g.s.start + first + token) * p.q_stride +
-                                               (g.h * p.group + head) * D + c * 8 : 0);
-        const uint32_t at = qt + (c / 8) * (kKeys * 128) + r * 128 + (((c % 8) ^ (r & 7)) * 16);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(live ? 16 : 0)
-                     : "memory");   // zeros where it is not live
-        for (head += kAtOnce; head >= p.group; head -= p.group) ++token;
-      }
-    };
-    auto q_is_there = [&]() {
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full(t));
-    };
-    int slot_of = 0;
-    bool ok = true, first_seg = true, more = next_segment(p, w, sh.seg[warp][0]);
-    if (more && sh.seg[warp][0].end(p, t) > sh.seg[warp][0].j0) {
-      send_for_q(sh.seg[warp][0]);
-      q_is_there();
-    }
-    while (more) {
-      const Segment& g = sh.seg[warp][slot_of];
-      const int end = g.end(p, t), first = (2 * g.i + t) * p.tpt;   // the tile's first token
-      const bool mine = of_token < p.tpt && first + of_token < g.s.n;
-      const bool whole = g.j0 == 0 && g.j1 == g.nk;
+    unsigned steps = 0, uses = 0;
+    bool ok = true, first_seg = true;
+    while (ok && next_segment(p, w, g)) {
+      const int end = g.end(p, t), j0 = g.j0;
+      // the last position that the row sees (of a row that is none, some)
+      const int pos = g.s.before + min((2 * g.i + t) * p.tpt + row / p.group, g.s.n - 1);
       float m = kNone, sum = 0.0f;
-      const int pos = g.s.before + min(first + of_token, g.s.n - 1);
-      for (int j = g.j0; j < end; ++j, ++steps) {
+      for (int j = j0; j < end; ++j, ++steps) {
         ok = wait(s_full(t), steps & 1);
         if (!ok) break;
         tc_fence_after();
@@ -713,18 +807,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float now = moves ? top : m, f = fast_exp2(m - now);
           m = now;
           sum *= f;
-          if (j > g.j0) {
+          if (j > j0) {
             ok = wait(pv_done(t), (steps - 1) & 1);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_at + c, o);
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_at + c, o);
               wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st32(o_at + c, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(o_at + c, o);
             }
           }
         }
@@ -751,53 +845,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         sum += both.x + both.y;
       }
       if (!ok) break;
-      // ---- O: the rows' outputs, or their sums for the merge ----
-      float* slot = nullptr;
-      if (!whole) {
-        slot = p.partials + ((size_t)blockIdx.x * 2 + (first_seg && g.j0 > 0 ? 0 : 1)) * (2 * kRows * (D + 2));
-        if (mine) reinterpret_cast<float2*>(slot + 2 * kRows * D)[t * kRows + row] = make_float2(m, sum);
+      if (g.j0 > 0 || g.j1 < g.nk) {   // for the merge
+        float* slot = p.partials + ((size_t)blockIdx.x * 2 + (first_seg && g.j0 > 0 ? 0 : 1)) * (2 * kRows * (D + 2));
+        __stcg(reinterpret_cast<float2*>(slot + 2 * kRows * D) + t * kRows + row, make_float2(m, sum));
       }
       first_seg = false;
-      // the next segment's Q on its way, and there before O is stored
-      const Segment& next = sh.seg[warp][slot_of ^ 1];
-      more = next_segment(p, w, sh.seg[warp][slot_of ^ 1]);
-      const bool next_q = more && next.end(p, t) > next.j0;
-      if (next_q) send_for_q(next);
-      if (end > g.j0) {
-        ok = wait(pv_done(t), (steps - 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
+      if (end > j0) {
+        ok = wait(o_empty(t), (uses++ & 1) ^ 1);   // the sums of the segment before are read
+        sh.sums[t][row] = sum;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sums_full(t));
       }
-      if (next_q) q_is_there();
-      if (end > g.j0) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // (nothing but scores of -inf: zeros)
-        __half* out = p.out + ((long long)(g.s.start + first + of_token) * p.Hq + g.h * p.group + of_head) * D;
-        float* part = whole ? nullptr : slot + (t * kRows + row) * D;
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_at + c, o);
-          wait_ld();
-          if (!mine) continue;
-          if (whole) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint4 v;
-              __half2* h = reinterpret_cast<__half2*>(&v);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                h[k] = __floats2half2_rn(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
-              *reinterpret_cast<uint4*>(out + c + e) = v;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              __stcg(reinterpret_cast<uint4*>(part + c + e), make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
-          }
-        }
-        tc_fence_before();
-      }
-      slot_of ^= 1;
     }
   }
   __syncthreads();
@@ -811,56 +869,66 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 constexpr int kMergeThreads = 256;
 
-// Resident blocks over (shared pair, rows of a block).  A thread has 4 dims of a row: the
-// states and sums of 16 CTAs on their way at once, then merged as a softmax goes on.
+// Resident blocks over (shared pair, 32 of its rows).  A thread has a row and 4 dims in
+// D / 32 places of it, so that a warp reads whole lines; several CTAs' states and sums are
+// on their way at once and merged as a softmax goes on.  The outputs are turned in shared
+// memory into rows.
 template <int D>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ Params p, int ctas) {
-  constexpr int kVec = D / 4, kBlockRows = kMergeThreads / kVec, kSlices = 2 * kRows / kBlockRows, kAtOnce = 16;
+  constexpr int kVec = D / 4, kMine = kVec / (kMergeThreads / 32), kSlices = 2 * kRows / 32, kAtOnce = 4;
   constexpr size_t kSlot = 2 * kRows * (D + 2);
   __shared__ int seconds[kMaxCtas];   // the CTAs that go on with a pair that the CTA before them began
   __shared__ int count[kMergeThreads / 32];
+  __shared__ uint2 turned[32][kVec + 1];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   static_assert(kMaxCtas <= kMergeThreads, "a CTA a thread");
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   bool shared = false;
   if (threadIdx.x < ctas) {
     const Open& o = p.open[threadIdx.x];
     shared = o.mid && o.begin + o.chunk >= o.at;
   }
   const uint32_t some = __ballot_sync(0xffffffffu, shared);
-  if (threadIdx.x % 32 == 0) count[threadIdx.x / 32] = __popc(some);
+  if (lane == 0) count[warp] = __popc(some);
   __syncthreads();
-  int at = __popc(some & ((1u << threadIdx.x % 32) - 1)), pairs = 0;
+  int at = __popc(some & ((1u << lane) - 1)), pairs = 0;
 #pragma unroll
   for (int w = 0; w < kMergeThreads / 32; ++w) {
-    if (w < threadIdx.x / 32) at += count[w];
+    if (w < warp) at += count[w];
     pairs += count[w];
   }
   if (shared) seconds[at] = threadIdx.x;
   __syncthreads();
-  const int d = threadIdx.x % kVec * 4;
   for (int work = blockIdx.x; work < pairs * kSlices; work += gridDim.x) {
-    const int second = seconds[work / kSlices], r = work % kSlices * kBlockRows + threadIdx.x / kVec;
+    const int second = seconds[work / kSlices], r0 = work % kSlices * 32, r = r0 + lane;
     const Open o = p.open[second];
-    const int of = r % kRows / p.group, token = r / kRows * p.tpt + of, head = r % kRows % p.group;
-    if (of >= p.tpt || token >= o.tokens) continue;
+    // token of a row in the pair, -1: none
+    auto token_of = [&](int row) {
+      const int of = row % kRows / p.group, token = row / kRows * p.tpt + of;
+      return of < p.tpt && token < o.tokens ? token : -1;
+    };
+    const bool mine = token_of(r) >= 0;
     const int n = (int)((o.end - 1) / o.chunk) - second + 2;   // CTAs
     // the pair is the last of the CTA that began it, the first of the others
     const float* begin = p.partials + ((size_t)(second - 1) * 2 + 1) * kSlot;
     const float* others = p.partials + (size_t)second * 2 * kSlot;
     float m = kNone, sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int c0 = 0; c0 < n; c0 += kAtOnce) {
+    float4 acc[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c0 = 0; c0 < n && mine; c0 += kAtOnce) {
       float2 state[kAtOnce];
-      float4 v[kAtOnce];
+      float4 v[kAtOnce][kMine];
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
         state[k] = make_float2(kNone, 0.0f);
-        v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float* slot = c0 + k ? others + (size_t)(c0 + k - 1) * 2 * kSlot : begin;
         if (c0 + k < n) {
+          const float* slot = c0 + k ? others + (size_t)(c0 + k - 1) * 2 * kSlot : begin;
           state[k] = __ldcg(reinterpret_cast<const float2*>(slot + 2 * kRows * D) + r);
-          v[k] = __ldcg(reinterpret_cast<const float4*>(slot + (size_t)r * D + d));
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+            v[k][i] = __ldcg(reinterpret_cast<const float4*>(slot) + (warp * kMine + i) * (2 * kRows) + r);
         }
       }
       float now = m;
@@ -869,24 +937,41 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       const float f = fast_exp2(m - now);
       m = now;
       sum *= f;
-      acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        acc[i].x *= f; acc[i].y *= f; acc[i].z *= f; acc[i].w *= f;
+      }
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
         if (state[k].y == 0.0f) continue;   // the row saw nothing there, and there may be no sums either
         const float e = fast_exp2(state[k].x - now);
         sum += state[k].y * e;
-        acc.x += v[k].x * e;
-        acc.y += v[k].y * e;
-        acc.z += v[k].z * e;
-        acc.w += v[k].w * e;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          acc[i].x += v[k][i].x * e;
+          acc[i].y += v[k][i].y * e;
+          acc[i].z += v[k][i].z * e;
+          acc[i].w += v[k][i].w * e;
+        }
       }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint2 w;
-    __half2* h = reinterpret_cast<__half2*>(&w);
-    h[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
-    h[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(p.out + ((long long)(o.token + token) * p.Hq + o.head * p.group + head) * D + d) = w;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      uint2 w;
+      __half2* h = reinterpret_cast<__half2*>(&w);
+      h[0] = __floats2half2_rn(acc[i].x * inv, acc[i].y * inv);
+      h[1] = __floats2half2_rn(acc[i].z * inv, acc[i].w * inv);
+      turned[lane][warp * kMine + i] = w;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * kVec; i += kMergeThreads) {
+      const int row = r0 + i / kVec, token = token_of(row);
+      if (token >= 0)
+        reinterpret_cast<uint2*>(p.out + ((long long)(o.token + token) * p.Hq + o.head * p.group +
+                                          row % kRows % p.group) * D)[i % kVec] = turned[i / kVec][i % kVec];
+    }
+    __syncthreads();
   }
 }
 
@@ -900,6 +985,12 @@ static bool shape_ok(int T, int B, int Hq, int Hkv, int D) {
          Hq / Hkv <= kRows && (D == 64 || D == 128);
 }
 
+template <int D>
+constexpr int smem_bytes() {
+  static_assert(Cfg<D>::kOffShared + sizeof(Shared) <= 227 * 1024, "shared memory per CTA");
+  return Cfg<D>::kOffShared + sizeof(Shared);
+}
+
 constexpr int kMaxDevices = 64;
 static int g_sms[kMaxDevices];
 static std::once_flag g_once[kMaxDevices];
@@ -908,8 +999,8 @@ static int sm_count() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
   std::call_once(g_once[dev], [dev] {
     cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev);
-    cudaFuncSetAttribute(chunk_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<64>::kSmem);
-    cudaFuncSetAttribute(chunk_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<128>::kSmem);
+    cudaFuncSetAttribute(chunk_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<64>());
+    cudaFuncSetAttribute(chunk_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<128>());
     cudaGetLastError();
   });
   return g_sms[dev];
@@ -918,8 +1009,8 @@ static int sm_count() {
 static std::once_flag g_encode_once;
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
-// A pool as a matrix of positions, each a row of all heads: a box is 64 dims of `box` of them.
-static bool pool_map(CUtensorMap* map, const void* pool, long long rows, int width, int box) {
+static bool encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                   const cuuint32_t* box) {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -928,35 +1019,44 @@ static bool pool_map(CUtensorMap* map, const void* pool, long long rows, int wid
       g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     cudaGetLastError();
   });
-  if (!g_encode) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)width * 2};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return g_encode && g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), dims, strides, box,
+                              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// A pool as a matrix of positions, each a row of all heads: a box is 64 dims of `box` of them.
+static bool pool_map(CUtensorMap* map, const void* pool, long long rows, int width, int box) {
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)width * 2};
   const cuuint32_t boxes[2] = {64, (cuuint32_t)box};
-  const cuuint32_t estr[2] = {1, 1};
-  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(pool), dims, strides, boxes, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode(map, pool, 2, dims, strides, boxes);
+}
+// Queries: a box is 64 dims of a group's heads of a tile's tokens.
+static bool query_map(CUtensorMap* map, const Params& p, int D) {
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.Hq, (cuuint64_t)p.T};
+  const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)p.q_stride * 2};
+  const cuuint32_t boxes[3] = {64, (cuuint32_t)p.group, (cuuint32_t)p.tpt};
+  return encode(map, p.q, 3, dims, strides, boxes);
 }
 
 template <int D>
-static int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int ctas, unsigned flags,
-                  cudaStream_t st) {
+static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int ctas,
+                  unsigned flags, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<D>::kSmem;
+  cfg.dynamicSmemBytes = smem_bytes<D>();
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (flags & ANVILQ_GEMM_OVERLAP_PRIOR) ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, chunk_kernel<D>, mk, mv, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, chunk_kernel<D>, mq, mk, mv, p) != cudaSuccess) {
     cudaGetLastError();
     return ANVILQ_ECUDA;
   }
   if (ctas == 1) return ANVILQ_OK;   // nothing is shared
-  cfg.gridDim = dim3(std::min(ctas * 32, kMaxCtas * 2));
+  cfg.gridDim = dim3(std::min(ctas * 8, kMaxCtas * 3));
   cfg.blockDim = dim3(kMergeThreads);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
@@ -1040,11 +1140,11 @@ int anvilq_gqa_chunk_paged(const uint16_t* q, long long q_stride, const uint16_t
   p.page_tokens = page_tokens; p.max_pages = max_pages; p.num_pages = num_pages;
   p.box = 16;
   while (p.box < kKeys && page_tokens % (2 * p.box) == 0) p.box *= 2;
-  CUtensorMap mk, mv;
-  if (!pool_map(&mk, k_pool, positions, Hkv * D, p.box) || !pool_map(&mv, v_pool, positions, Hkv * D, p.box))
+  CUtensorMap mq, mk, mv;
+  if (!query_map(&mq, p, D) || !pool_map(&mk, k_pool, positions, Hkv * D, p.box) || !pool_map(&mv, v_pool, positions, Hkv * D, p.box))
     return ANVILQ_ECUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return D == 64 ? launch<64>(mk, mv, p, ctas, flags, st) : launch<128>(mk, mv, p, ctas, flags, st);
+  return D == 64 ? launch<64>(mq, mk, mv, p, ctas, flags, st) : launch<128>(mq, mk, mv, p, ctas, flags, st);
 }
 
 }  // extern "C"
