@@ -28,9 +28,9 @@
 // Warp roles (16 warps, one CTA an SM):
 //   0-3, 4-7   softmax of tile 0 and tile 1; they rescale its O where they must
 //   8-11       store O, while the next pair's scores are under way
-//   12, 13     TMA of K and of V (side by side: pages of 16 tokens take 16 copies a tile)
-//   14         MMA issuer, TMEM owner; zeroes V's rows behind a sequence's last token
-//   15         TMA of Q
+//   12, 13     TMA of Q and K, and of V (side by side: pages of 16 tokens take 16 copies
+//              a tile); the latter zeroes V's rows behind a sequence's last token
+//   14, 15     MMA of tile 0 and tile 1 (14 owns the TMEM)
 // K and V tiles share a ring: [half of 64 dims][128 keys][128 bytes], 128-byte swizzle.
 // K is the K-major B operand of S, V the MN-major one of O.
 #include <cuda.h>
@@ -54,7 +54,7 @@ constexpr int kRows = 128;                 // of a tile: MMA M, a TMEM lane each
 constexpr int kKeys = 128;                 // of a step
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kStoreWarp = 8, kKWarp = 12, kVWarp = 13, kMmaWarp = 14, kQWarp = 15;
+constexpr int kStoreWarp = 8, kKWarp = 12, kVWarp = 13, kMmaWarp = 14;
 constexpr int kSetup = 1;                  // what a pair's beginning costs, in key tiles
 constexpr int kMaxCtas = 148;
 constexpr int kMaxBatch = 65536;
@@ -70,7 +70,7 @@ struct Cfg {
   static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kOffQ = kStages * kTileBytes;
   static constexpr int kOffBar = kOffQ + 2 * kTileBytes;
-  static constexpr int kBars = 2 * kStages + 2 * 8 + 1;
+  static constexpr int kBars = 2 * kStages + 2 * 9 + 1;
   static constexpr int kOffShared = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static_assert(kMaxBatch / 32 * 8 <= kOffQ, "the groups' counts lie in the ring before its first copy");
 };
@@ -381,9 +381,10 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
 
 struct Shared {
   Walk walk[kWarps];
-  Segment seg[kWarps + 1];   // the MMA issuer has two
+  Segment seg[kWarps];
   float sums[2][kRows];
   uint32_t tmem;
+  int turn;                  // 1: one of the tiles has its products and its next scores issued
   volatile int abort;
 };
 
@@ -501,11 +502,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto pv_done = [&](int t) { return bar_of(5, t); };
   auto sums_full = [&](int t) { return bar_of(6, t); };
   auto o_empty = [&](int t) { return bar_of(7, t); };
-  const uint32_t drained = bar_of(8, 0);
+  auto drained = [&](int t) { return bar_of(8, t); };
+  const uint32_t landed = bar_of(9, 0);   // a V tile whose last rows are still to be zeroed
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(kv_full(s), 1);
-      mbar_init(kv_empty(s), 1);
+      mbar_init(kv_empty(s), 2);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(q_full(t), 1);
@@ -516,8 +518,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(pv_done(t), 1);
       mbar_init(sums_full(t), 4);
       mbar_init(o_empty(t), 4);
+      mbar_init(drained(t), 1);
     }
-    mbar_init(drained, 1);
+    mbar_init(landed, 1);
+    sh.turn = 0;
     sh.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
@@ -552,19 +556,37 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   // `uses` of a tile: the segments that it has a part in
 
-  if (warp >= kStoreWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  if (warp >= kKWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == kKWarp || warp == kVWarp) {
-      // ------------------------------------------------------------------ K and V
-      const CUtensorMap* map = warp == kKWarp ? &mk : &mv;
+      // ------------------------------------------------------------------ Q, K and V
+      const bool is_v = warp == kVWarp;
+      const CUtensorMap* map = is_v ? &mv : &mk;
       const int boxes = kKeys / p.box, box_bytes = p.box * 128;
       const int my_box = lane % boxes, my_half = lane / boxes;   // at most 8 x 2 copies
-      unsigned seq = warp - kKWarp, issued = 0;                  // K and V tiles alternate in the ring
+      int stage = is_v ? 1 : 0;                                  // K and V tiles alternate in the ring
+      uint32_t phase = 0, q_uses[2] = {0, 0}, tails = 0, issued = 0;   // issued: a bit a stage, its phase in the upper half
       bool ok = true;
       while (ok && next_segment(p, w, g)) {
+        if (!is_v) {
+          // Q: a box is tpt tokens of g heads.  Tokens behind the sequence's are other rows,
+          // which are not stored, tokens behind the last zeros.
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || g.end(p, t) <= g.j0) continue;
+            ok = wait(q_empty(t), (q_uses[t]++ & 1) ^ 1);
+            if (ok && lane == 0) {
+              expect(q_full(t), C::kHalves * p.group * p.tpt * 128);
+#pragma unroll
+              for (int h = 0; h < C::kHalves; ++h)
+                tma_3d(base + C::kOffQ + t * C::kTileBytes + h * (kRows * 128), &mq, h * 64, g.h * p.group,
+                       g.s.start + (2 * g.i + t) * p.tpt, q_full(t));
+            }
+            __syncwarp();
+          }
+        }
         const int len = g.s.before + g.s.n;
-        for (int j = g.j0; j < g.j1; ++j, seq += 2) {
-          const int stage = seq % C::kStages;
+        for (int j = g.j0; ok && j < g.j1; ++j) {
           // the lane's box: its page is looked up while the stage is waited for
           const int key = j * kKeys + my_box * p.box;
           const bool live = my_half < C::kHalves && key < len;
@@ -573,149 +595,160 @@ __global__ void __launch_bounds__(kThreads, 1)
             atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
             page = 0;
           }
-          ok = wait(kv_empty(stage), ((seq / C::kStages) & 1) ^ 1);
+          ok = wait(kv_empty(stage), phase ^ 1);
           if (!ok) break;
+          // V's rows behind the sequence's last token may hold anything: times p = 0 they must be 0
+          const int rows = len - j * kKeys;
+          const bool tail = is_v && rows < kKeys;
+          const uint32_t at = base + stage * C::kTileBytes, full = tail ? landed : kv_full(stage);
           const int copies = __popc(__ballot_sync(0xffffffffu, live));
-          if (lane == 0) expect(kv_full(stage), copies * box_bytes);
+          if (lane == 0) expect(full, copies * box_bytes);
           __syncwarp();
           if (live)
-            tma_2d(base + stage * C::kTileBytes + my_half * (kKeys * 128) + my_box * box_bytes, map,
-                   g.h * D + my_half * 64, page * p.page_tokens + key % p.page_tokens, kv_full(stage));
+            tma_2d(at + my_half * (kKeys * 128) + my_box * box_bytes, map, g.h * D + my_half * 64,
+                   page * p.page_tokens + key % p.page_tokens, full);
           __syncwarp();
-          issued = seq + 1;
-        }
-      }
-      if (sh.abort && lane == 0) {   // let the copies in flight land before the CTA exits
-        for (int i = 0; i < C::kStages; i += 2) {
-          const int s = (int)issued - 1 - i;
-          if (s >= 0) mbar_drain(kv_full(s % C::kStages), (s / C::kStages) & 1);
-        }
-      }
-    } else if (warp == kQWarp) {
-      // ------------------------------------------------------------------ Q
-      // A box is tpt tokens of g heads; tokens behind the sequence's are other rows, that
-      // are not stored, tokens behind the last zeros.
-      unsigned uses[2] = {0, 0};
-      bool ok = true;
-      while (ok && next_segment(p, w, g)) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (g.end(p, t) <= g.j0) continue;
-          ok = ok && wait(q_empty(t), (uses[t] & 1) ^ 1);
-          if (!ok) break;
-          if (elect_one()) {
-            expect(q_full(t), C::kHalves * p.group * p.tpt * 128);
-#pragma unroll
-            for (int h = 0; h < C::kHalves; ++h)
-              tma_3d(base + C::kOffQ + t * C::kTileBytes + h * (kRows * 128), &mq, h * 64, g.h * p.group,
-                     g.s.start + (2 * g.i + t) * p.tpt, q_full(t));
-          }
-          __syncwarp();
-          ++uses[t];
-        }
-      }
-      if (sh.abort && lane == 0)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (uses[t]) mbar_drain(q_full(t), (uses[t] - 1) & 1);
-    } else if (warp == kMmaWarp) {
-      // ------------------------------------------------------------------ MMA
-      // Step by step through all segments: the products of one key tile beside the scores
-      // of the next, of the next pair where it is the last.
-      constexpr uint32_t idesc_s = instr_desc(kKeys, false), idesc_o = instr_desc(D, true);
-      unsigned seq = 0;                                    // of the scores' K; its V is the next
-      unsigned steps[2] = {0, 0}, q_uses[2] = {0, 0}, o_uses[2] = {0, 0};
-      int slot = 0;
-      auto seg = [&](int i) -> Segment& { return sh.seg[i ? kWarps : kMmaWarp]; };
-      bool ok = true, products = false, scores = next_segment(p, w, seg(0));
-      int j = 0, j0 = 0, end[2] = {0, 0}, live = 0;        // of the products
-      int sj = seg(0).j0, s_end[2] = {seg(0).end(p, 0), seg(0).end(p, 1)};   // of the scores
-      while (ok && (products || scores)) {
-        const Segment& n = seg(slot);
-        const int vs = (seq - 1) % C::kStages, ks = seq % C::kStages;
-        if (scores) ok = wait(kv_full(ks), (seq / C::kStages) & 1);
-        if (ok && products) {
-          ok = wait(kv_full(vs), ((seq - 1) / C::kStages) & 1);
-          // rows behind the sequence's last token may hold anything: times p = 0 they must be 0
-          if (ok && live < kKeys) {
-            const uint32_t v = base + vs * C::kTileBytes;
-            for (int i = live * 8 + lane; i < kKeys * 8; i += 32)
+          if (tail) {
+            ok = wait(landed, tails++ & 1);
+            if (!ok) break;
+            for (int i = rows * 8 + lane; i < kKeys * 8; i += 32)
 #pragma unroll
               for (int h = 0; h < C::kHalves; ++h)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + h * (kKeys * 128) + i * 16), "r"(0)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at + h * (kKeys * 128) + i * 16), "r"(0)
                              : "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
+            if (lane == 0) mbar_arrive(kv_full(stage));
           }
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (ok && products && j < end[t]) {
-            if (j == j0) ok = wait(o_empty(t), (o_uses[t]++ & 1) ^ 1);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              ok = ok && wait(p_full(t, half), steps[t] & 1);
-              if (!ok) break;
-              tc_fence_after();
-              if (elect_one()) {
-                const uint32_t v = base + vs * C::kTileBytes;
-#pragma unroll
-                for (int k = 4 * half; k < 4 * half + 4; ++k)
-                  mma_ts(tmem + kTmemO + t * 128, tmem + t * kKeys + k * 8,
-                         smem_desc(v + k * 2048, kKeys * 128, 1024), idesc_o, (j > j0 || k > 0) ? 1u : 0u);
-                if (half) tc_commit(pv_done(t));
-              }
-              __syncwarp();
-            }
-            ++steps[t];
+          issued = (issued & ~(0x10001u << stage)) | ((1u | phase << 16) << stage);
+          stage += 2;
+          if (stage >= C::kStages) {
+            stage -= C::kStages;
+            phase ^= 1;
           }
-          if (ok && scores && sj < s_end[t]) {
-            if (sj == n.j0) ok = wait(q_full(t), q_uses[t]++ & 1);
-            // S goes where the products of the tile's last step read P
-            if (ok && steps[t]) ok = wait(pv_done(t), (steps[t] - 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {   // S_t = Q_t K^T
-              const uint32_t a = base + C::kOffQ + t * C::kTileBytes, b = base + ks * C::kTileBytes;
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint32_t at = (k / 4) * (kKeys * 128) + (k % 4) * 32;
-                mma_ss(tmem + t * kKeys, smem_desc(a + at, 16, 1024), smem_desc(b + at, 16, 1024), idesc_s, k > 0);
-              }
-              tc_commit(s_full(t));
-              if (sj + 1 == s_end[t]) tc_commit(q_empty(t));
-            }
-            __syncwarp();
-          }
-        }
-        if (ok && elect_one()) {
-          if (products) tc_commit(kv_empty(vs));
-          if (scores) tc_commit(kv_empty(ks));
-        }
-        __syncwarp();
-        // on to the next step
-        products = scores;
-        if (!scores) break;
-        seq += 2;
-        j = sj;
-        j0 = n.j0;
-        live = n.s.before + n.s.n - j * kKeys;
-        end[0] = s_end[0];
-        end[1] = s_end[1];
-        if (++sj == n.j1) {
-          slot ^= 1;
-          scores = next_segment(p, w, seg(slot));
-          sj = seg(slot).j0;
-          s_end[0] = seg(slot).end(p, 0);
-          s_end[1] = seg(slot).end(p, 1);
         }
       }
-      if (sh.abort) {   // MMAs still running write TMEM
-        if (elect_one()) tc_commit(drained);
-        __syncwarp();
-        mbar_drain(drained, 0);
+      if (sh.abort && lane == 0) {   // let the copies in flight land before the CTA exits
+        for (int s = 0; s < C::kStages; ++s)
+          if (issued >> s & 1) mbar_drain(kv_full(s), issued >> (16 + s) & 1);
+        if (is_v && tails) mbar_drain(landed, (tails - 1) & 1);
+        for (int t = 0; t < 2; ++t)
+          if (q_uses[t]) mbar_drain(q_full(t), (q_uses[t] - 1) & 1);
       }
     } else {
+      // ------------------------------------------------------------------ MMA
+      // A thread a tile issues its products: S = Q K^T when a K tile is there, O += P V when
+      // its P and the V tile are.  A tile's last products and its next scores go together,
+      // one tile at a time (`turn`): so the tiles' softmax run in turns, each beside the
+      // other's products.  Left alone, both ran at once and both waited at once.
+      const int t = warp - kMmaWarp;
+      constexpr uint32_t idesc_s = instr_desc(kKeys, false), idesc_o = instr_desc(D, true);
+      // low words of the descriptors (start, leading offset); the high one is all tiles'
+      constexpr uint32_t kHigh = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);
+      constexpr uint32_t kHalf = kKeys * 128 / 16, kTile = C::kTileBytes / 16;
+      auto low = [](uint32_t at, uint32_t lbo) { return at >> 4 | (lbo >> 4) << 16; };
+      const uint32_t q_low = low(base + C::kOffQ + t * C::kTileBytes, 16), k_low = low(base, 16),
+                     v_low = low(base, kKeys * 128);
+      auto desc = [](uint32_t lo) {
+        u64 d;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(kHigh));
+        return d;
+      };
+      const uint32_t s_at = tmem + t * kKeys, o_at = tmem + kTmemO + t * 128;
+      int stage = 0;                           // the ring's next tile: K, V, K, V ...
+      uint32_t phase = 0, steps = 0, uses = 0;
+      bool ok = true;
+      auto wait1 = [&](uint32_t bar, uint32_t parity) {   // by the one thread
+        if (mbar_wait(bar, parity, &sh.abort)) return true;
+        fail();
+        return false;
+      };
+      auto next_stage = [&]() {
+        if (++stage == C::kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      };
+      auto take_turn = [&]() {
+        if (atomicCAS(&sh.turn, 0, 1) == 0) return true;
+        const u64 t0 = globaltimer();
+        while (atomicCAS(&sh.turn, 0, 1) != 0)
+          if (sh.abort || globaltimer() - t0 > kWaitLimitNs) {
+            fail();
+            return false;
+          }
+        return true;
+      };
+      auto scores = [&](int ks) {              // S_t = Q_t K^T
+        tc_fence_after();
+        const uint32_t k = k_low + ks * kTile;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          mma_ss(s_at, desc(q_low + (i / 4 * kHalf + i % 4 * 2)), desc(k + (i / 4 * kHalf + i % 4 * 2)), idesc_s, i > 0);
+        tc_commit(s_full(t));
+      };
+      // the tile's steps [j0, end) of a segment, none of them: passed over
+      auto run = [&](int j0, int end, int j1) {
+        if (end > j0) {
+          if (!wait1(kv_full(stage), phase) || !wait1(q_full(t), uses & 1)) return false;
+          if (steps && !wait1(pv_done(t), (steps - 1) & 1)) return false;
+          scores(stage);
+          if (j0 + 1 == end) tc_commit(q_empty(t));
+          tc_commit(kv_empty(stage));
+          next_stage();
+          for (int j = j0; j < end; ++j, ++steps) {
+            const int vs = stage;
+            const bool more = j + 1 < end;
+            if (!wait1(kv_full(vs), phase)) return false;
+            next_stage();
+            const uint32_t v = v_low + vs * kTile;
+            if (j == j0 && !wait1(o_empty(t), (uses & 1) ^ 1)) return false;
+            if (!wait1(p_full(t, 0), steps & 1)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma_ts(o_at, s_at + i * 8, desc(v + i * 128), idesc_o, (j > j0 || i > 0) ? 1u : 0u);
+            if (more && !wait1(kv_full(stage), phase)) return false;
+            if (!wait1(p_full(t, 1), steps & 1) || !take_turn()) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int i = 4; i < 8; ++i) mma_ts(o_at, s_at + i * 8, desc(v + i * 128), idesc_o, 1u);
+            tc_commit(pv_done(t));
+            if (more) {   // S goes where the products read P
+              if (!wait1(pv_done(t), steps & 1)) return false;
+              scores(stage);
+            }
+            atomicExch(&sh.turn, 0);
+            tc_commit(kv_empty(vs));
+            if (more) {
+              tc_commit(kv_empty(stage));
+              if (j + 2 == end) tc_commit(q_empty(t));
+              next_stage();
+            }
+          }
+          ++uses;
+        }
+        for (int i = 2 * (j1 - max(end, j0)); i > 0; --i) {
+          if (!wait1(kv_full(stage), phase)) return false;
+          mbar_arrive(kv_empty(stage));
+          next_stage();
+        }
+        return true;
+      };
+      while (ok && next_segment(p, w, g)) {
+        if (lane == 0) ok = run(g.j0, g.end(p, t), g.j1);
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+      }
+      if (sh.abort) {   // MMAs still running write TMEM
+        if (lane == 0) {
+          tc_commit(drained(t));
+          mbar_drain(drained(t), 0);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp >= kStoreWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    {
       // ------------------------------------------------------------------ stores
       const int row = warp % 4 * 32 + lane, of_token = row / p.group, of_head = row % p.group;
       unsigned steps[2] = {0, 0}, uses[2] = {0, 0};
@@ -774,7 +807,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // -------------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     const int t = warp / 4, row = threadIdx.x % kRows;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t s_at = tmem + t * kKeys + lanes, o_at = tmem + kTmemO + t * 128 + lanes;
