@@ -17,13 +17,13 @@
 // softmax by a warpgroup (a thread a row), P back into TMEM over S, O += P V.  Two
 // tiles in turn keep the tensor cores at one's products while the other's softmax runs.
 //
-// Work split (stream-K).  All (pair, key tile) units in a row, pairs in the order
-// (sequence, kv head, pair), a unit for each pair's beginning, are cut into equal stretches, one a CTA, so lengths do not
-// matter to the balance and few rows over a long axis are split over it.  A pair that
+// Work split (stream-K).  All pairs' keys in a row, in the order (sequence, kv head,
+// pair), with 128 units more for a pair's beginning, are cut into equal stretches, one a
+// CTA; a key tile is the CTA's in whose stretch it begins.  So lengths do not matter to the
+// balance and few rows over a long axis are split over it.  A pair that
 // several CTAs share leaves binary32 partial sums in the workspace; a second kernel,
 // launched with the first's end overlapped, merges them in CTA order (bit-reproducible).
-// How many units there are is a sum of rounded linear functions, computed in closed form
-// (floor_sum) by every CTA from the lengths on the device.
+// Every CTA finds its stretch from the lengths on the device, by sums in closed form.
 //
 // Warp roles (16 warps, one CTA an SM):
 //   0-3, 4-7   softmax of tile 0 and tile 1; they rescale its O where they must
@@ -55,7 +55,8 @@ constexpr int kKeys = 128;                 // of a step
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kStoreWarp = 8, kKWarp = 12, kVWarp = 13, kMmaWarp = 14;
-constexpr int kSetup = 1;                  // what a pair's beginning costs, in key tiles
+constexpr int kSetup = 192;                // what a pair's beginning costs, in keys
+constexpr int kLeast = 1;                  // key tiles' worth of units of a stretch, at least
 constexpr int kMaxCtas = 148;
 constexpr int kMaxBatch = 65536;
 constexpr float kNone = -1e30f;            // a reference below every exponent
@@ -91,7 +92,7 @@ struct Params {
 
 // What the merge needs to know of a CTA's first pair.
 struct Open {
-  u64 begin, end;               // its key tiles' units; the CTA's own begin at `at`
+  u64 begin, end;               // the units of its first and last key tile; the CTA's own begin at `at`
   u64 at, chunk;
   int token, tokens, head, mid; // first token, tokens left in the sequence from it on; mid: begun by an earlier CTA
 };
@@ -260,31 +261,6 @@ __host__ __device__ constexpr uint32_t instr_desc(int n, bool b_mn_major) {
 
 // ---- the plan -----------------------------------------------------------------------
 
-// sum of floor((a i + b) / m), i = 0 .. n - 1; a n + b below 2^32
-__device__ __forceinline__ u64 floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-  u64 sum = 0;
-  while (n) {
-    if (a >= m) {
-      const uint32_t d = a / m;
-      sum += (u64)(n - 1) * n / 2 * d;
-      a -= d * m;
-    }
-    if (b >= m) {
-      const uint32_t d = b / m;
-      sum += (u64)n * d;
-      b -= d * m;
-    }
-    const uint32_t top = a * n + b;
-    if (top < m) break;
-    n = top / m;
-    b = top - n * m;
-    const uint32_t t = m;
-    m = a;
-    a = t;
-  }
-  return sum;
-}
-
 // A sequence's new tokens: rows [start, start + n) at positions before and on.
 struct Seq {
   int start, n, before;
@@ -304,14 +280,17 @@ __device__ __forceinline__ int pairs_of(const Params& p, const Seq& s) { return 
 __device__ __forceinline__ int tiles_to(const Seq& s, int tokens) {
   return (s.before + min(tokens, s.n) + kKeys - 1) / kKeys;
 }
-// A pair's units are kSetup for its beginning and one a key tile: of a head's first i
-// pairs, i < pairs_of
+// A pair's units are kSetup for its beginning, then its keys.  Those of a head's first i
+// pairs, i < pairs_of: their keys are an arithmetic series.
 __device__ __forceinline__ u64 units_before(const Params& p, const Seq& s, int i) {
-  return (u64)i * kSetup + floor_sum(i, kKeys, 2 * p.tpt, s.before + 2 * p.tpt + kKeys - 1);
+  return (u64)i * (kSetup + s.before) + (u64)i * (i + 1) / 2 * (2 * p.tpt);
 }
 __device__ __forceinline__ u64 units_of(const Params& p, const Seq& s) {   // of a head
-  return s.n ? units_before(p, s, pairs_of(p, s) - 1) + kSetup + tiles_to(s, s.n) : 0;
+  return s.n ? units_before(p, s, pairs_of(p, s) - 1) + kSetup + s.before + s.n : 0;
 }
+// A key tile belongs to the stretch that its first key is in: of a pair's tiles, those whose
+// first key lies below the pair's unit x.
+__device__ __forceinline__ int tiles_below(int x) { return max(0, x - kSetup + kKeys - 1) / kKeys; }
 
 // Where a stretch is: every role walks the same way.
 struct Walk {
@@ -329,48 +308,48 @@ struct Segment {
     return first < s.n ? min(j1, tiles_to(s, first + p.tpt)) : j0;
   }
 };
-// The next segment; the whole warp calls it.  Both lie in shared memory, as the softmax
-// needs the registers.
-__device__ __forceinline__ void advance(const Params& p, Walk& w, Segment& g) {
-  g.s = w.s;
-  g.b = w.b; g.h = w.h; g.i = w.i;
-  g.nk = tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
-  const int end = (int)min((u64)(kSetup + g.nk), w.x + w.left);
-  g.j0 = max(0, w.x - kSetup);
-  g.j1 = max(0, end - kSetup);
-  w.left -= end - w.x;
-  w.x = 0;
-  if (w.left == 0 || ++w.i < pairs_of(p, w.s)) return;
-  w.i = 0;
-  if (++w.h < p.Hkv) return;
-  w.h = 0;
-  const int lane = threadIdx.x % 32;
-  for (int b0 = w.b + 1; b0 < p.B; b0 += 32) {   // the next sequence with new tokens
-    const Seq s = b0 + lane < p.B ? sequence(p, b0 + lane) : Seq{0, 0, 0};
-    const uint32_t some = __ballot_sync(0xffffffffu, s.n > 0);
-    if (!some) continue;
-    const int l = __ffs(some) - 1;
-    w.b = b0 + l;
-    w.s.start = __shfl_sync(0xffffffffu, s.start, l);
-    w.s.n = __shfl_sync(0xffffffffu, s.n, l);
-    w.s.before = __shfl_sync(0xffffffffu, s.before, l);
-    return;
-  }
-  w.left = 0;
-}
+// The next segment that has a key tile; the whole warp calls it.  Both lie in shared
+// memory, as the softmax needs the registers.
 __device__ __forceinline__ bool next_segment(const Params& p, Walk& walk, Segment& seg) {
   __syncwarp();
   Walk w = walk;
-  if (w.left == 0) return false;
   Segment g;
-  advance(p, w, g);
+  g.j0 = g.j1 = 0;
+  while (w.left && g.j1 <= g.j0) {
+    g.s = w.s;
+    g.b = w.b; g.h = w.h; g.i = w.i;
+    g.nk = tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
+    const int end = (int)min((u64)(kSetup + w.s.before + min((w.i + 1) * 2 * p.tpt, w.s.n)), w.x + w.left);
+    g.j0 = min(g.nk, tiles_below(w.x));
+    g.j1 = tiles_below(end);
+    w.left -= end - w.x;
+    w.x = 0;
+    if (w.left == 0 || ++w.i < pairs_of(p, w.s)) continue;
+    w.i = 0;
+    if (++w.h < p.Hkv) continue;
+    w.h = 0;
+    const int lane = threadIdx.x % 32;
+    int b0 = w.b + 1;
+    for (; b0 < p.B; b0 += 32) {   // the next sequence with new tokens
+      const Seq s = b0 + lane < p.B ? sequence(p, b0 + lane) : Seq{0, 0, 0};
+      const uint32_t some = __ballot_sync(0xffffffffu, s.n > 0);
+      if (!some) continue;
+      const int l = __ffs(some) - 1;
+      w.b = b0 + l;
+      w.s.start = __shfl_sync(0xffffffffu, s.start, l);
+      w.s.n = __shfl_sync(0xffffffffu, s.n, l);
+      w.s.before = __shfl_sync(0xffffffffu, s.before, l);
+      break;
+    }
+    if (b0 >= p.B) w.left = 0;
+  }
   __syncwarp();
   if (threadIdx.x % 32 == 0) {
     walk = w;
     seg = g;
   }
   __syncwarp();
-  return g.j1 > g.j0;   // else the stretch ends in a pair's beginning
+  return g.j1 > g.j0;
 }
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -411,7 +390,7 @@ __device__ __forceinline__ void plan(const Params& p, u64* groups, Shared& sh) {
       for (int i = lane; i < n; i += 32) total += groups[i];
     }
     total = warp_sum(total);
-    const u64 chunk = max((total + gridDim.x - 1) / gridDim.x, (u64)1);
+    const u64 chunk = max((total + gridDim.x - 1) / gridDim.x, (u64)(kLeast * kKeys));
     const u64 at = min(total, blockIdx.x * chunk);
     Walk w{};
     w.left = min(chunk, total - at);
@@ -463,14 +442,15 @@ __device__ __forceinline__ void plan(const Params& p, u64* groups, Shared& sh) {
       // for the merge: the pair that the stretch begins in
       Open o{};
       if (w.left) {
+        const int nk = tiles_to(w.s, (w.i + 1) * 2 * p.tpt), j0 = tiles_below(w.x);
         o.begin = at - w.x + kSetup;
-        o.end = o.begin + tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
+        o.end = o.begin + (u64)(nk - 1) * kKeys;
         o.at = at;
         o.chunk = chunk;
         o.token = w.s.start + w.i * 2 * p.tpt;
         o.tokens = w.s.n - w.i * 2 * p.tpt;
         o.head = w.h;
-        o.mid = w.x > kSetup;
+        o.mid = j0 > 0 && j0 < nk;
       }
       p.open[blockIdx.x] = o;
     }
@@ -942,7 +922,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       return of < p.tpt && token < o.tokens ? token : -1;
     };
     const bool mine = token_of(r) >= 0;
-    const int n = (int)((o.end - 1) / o.chunk) - second + 2;   // CTAs
+    const int n = (int)(o.end / o.chunk) - second + 2;   // CTAs
     // the pair is the last of the CTA that began it, the first of the others
     const float* begin = p.partials + ((size_t)(second - 1) * 2 + 1) * kSlot;
     const float* others = p.partials + (size_t)second * 2 * kSlot;
