@@ -18,12 +18,12 @@
 // small call is bound by latency: load, threshold, merge.
 //
 // Work split.  A CTA takes a span of a beam's vocabulary (splits so that the device is
-// full), in tiles that stay in registers.  Its first tile's N-th largest thread
-// maximum bounds its N-th best logit from below; what beats the bound goes to a list
-// in shared memory, as do later tiles' logits that beat the list's N-th.  After a tile
-// of random logits that is seldom any (N log of the span over the tile in all), so the
-// passes over the list do not show.  The span's sum and N best go to the workspace,
-// and the item's last CTA (by a ticket) merges them.
+// full, splits_for), its warps tiles of 32 x 4 x 16 bytes in turn, without a barrier: a
+// warp adds a tile up, and looks for candidates only where a 16-byte unit's largest beats
+// the span's bar.  Where every warp has N / warps keys, there are N: the first tiles' lanes
+// set it so, lists that fill raise it, for all warps of the CTA.  Of random logits few beat it (N log of the span over
+// the tile in all).  The span's sum and N best go to the workspace, and the item's last
+// CTA (by a ticket) merges them.
 #include <algorithm>
 #include <cmath>
 
@@ -38,8 +38,10 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBeams = 64, kMaxBest = 128;   // K, N
 constexpr int kMaxItems = 4096;
 constexpr int kUnits = 4;                       // 16-byte units of a thread in a tile
-constexpr int kList = 1024;                     // candidates in shared memory
+constexpr int kList = 1024;                     // final candidates in shared memory
+constexpr int kWarpList = 192;                  // a warp's
 constexpr int kMaxSplits = 64;
+constexpr int kResident = 4;                    // CTAs an SM
 constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596299e-8f;   // log2 e in two parts
 
 struct Params {
@@ -84,43 +86,61 @@ __device__ __forceinline__ int place_of(unsigned long long key) { return (int)(0
 // A beam that goes on or has ended; scores of NaN and +inf are reported and count as none.
 __device__ __forceinline__ bool is_live(float score) { return score > -INFINITY && score < INFINITY; }
 
-// A span's list of candidates.  `bar`: keys must be above it.
+// A span's candidates: a list a warp, and what any of them has to beat.
 struct List {
-  unsigned long long key[kList];
-  unsigned long long sorted[kMaxBest];
-  unsigned long long bar;
-  int count;
+  unsigned long long key[kWarps][kWarpList];
+  unsigned long long all[kWarps * kMaxBest];
+  unsigned long long bar;   // at least N keys of the span are above it, or it is the N-th
+  uint32_t share[kWarps];   // the warp has its share of N keys, N / warps, of this order or above
+  int count[kWarps];
 };
-
-// The list's N best, best first, in its front; bar: the N-th where there are N.  All
-// threads; every key is unique.
-__device__ __forceinline__ void prune(List& s, int N) {
-  __syncthreads();
-  const int n = s.count;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const unsigned long long mine = s.key[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += s.key[j] > mine;
-    if (above < N) s.sorted[above] = mine;
-  }
-  __syncthreads();
-  const int left = min(n, N);
-  for (int i = threadIdx.x; i < left; i += kThreads) s.key[i] = s.sorted[i];
-  if (threadIdx.x == 0) {
-    s.count = left;
-    if (n >= N) s.bar = s.sorted[N - 1];
-  }
-  __syncthreads();
+// What a key has to be above: the bar, or what all warps have their shares of.
+__device__ __forceinline__ unsigned long long bar_of(const List& s, int warps) {
+  const int lane = threadIdx.x % 32;
+  const uint32_t mine = lane < warps ? *reinterpret_cast<const volatile uint32_t*>(&s.share[lane]) : 0xFFFFFFFFu;
+  const unsigned long long all = (unsigned long long)__reduce_min_sync(0xffffffffu, mine) << 32;
+  const unsigned long long bar = *reinterpret_cast<const volatile unsigned long long*>(&s.bar);
+  return all > bar ? all : bar;
 }
 
-// The final candidates: rank, and the place k V + v (-1: none).
+// The n keys' best N, best first, in `to`: every thread of the group (thread `me` of
+// `threads`) calls it, all keys differ.
+__device__ __forceinline__ void best_of(const unsigned long long* key, int n, unsigned long long* to, int N, int me,
+                                        int threads) {
+  for (int i = me; i < n; i += threads) {
+    const unsigned long long mine = key[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += key[j] > mine;
+    if (above < N) to[above] = mine;
+  }
+}
+
+// The lanes' values in descending order, by exchanges (Batcher's bitonic network).
+__device__ __forceinline__ float sorted(float v) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int o = size / 2; o > 0; o /= 2) {
+      const float other = __shfl_xor_sync(0xffffffffu, v, o);
+      const bool larger = ((lane & o) == 0) == ((lane & size) == 0);   // this lane keeps the larger one
+      v = larger ? fmaxf(v, other) : fminf(v, other);
+    }
+  return v;
+}
+
+// The final candidates, by rank, then by place k V + v.
 struct Candidate {
-  double rank;
+  unsigned long long rank;    // a binary64 number in its order
   long long place;
   __device__ __forceinline__ bool beats(const Candidate& o) const {
     return rank > o.rank || (rank == o.rank && place < o.place);
   }
 };
+__device__ __forceinline__ unsigned long long order_of(double r) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(r + 0.0);   // -0 as +0
+  return (u >> 63) ? ~u : u | 1ull << 63;
+}
 struct Merge {
   double score[kMaxBeams];
   double top[kMaxBeams];      // lse = top + log_sum: kept apart, as a logit minus top is exact however
@@ -151,6 +171,39 @@ __device__ __forceinline__ void prune(Merge& s, int N) {
   __syncthreads();
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// two binary32 values at a time
+using u64 = unsigned long long;
+__device__ __forceinline__ u64 pair(float a, float b) {
+  u64 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 unpair(u64 v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 __device__ __forceinline__ void widen(const uint4& w, float* v, __half) {
   const __half2* h = reinterpret_cast<const __half2*>(&w);
 #pragma unroll
@@ -164,24 +217,65 @@ __device__ __forceinline__ void widen(const uint4& w, float* v, float) {
   v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y);
   v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
 }
-// 16 bytes of a row that starts on a multiple of `align` bytes
-__device__ __forceinline__ uint4 load_unit(const void* p, int align) {
+// What seldom runs is kept out of the loops, whose instructions would not fit the
+// instruction cache (beam batch 148 us with all of it unrolled in place).
+
+// 16 bytes of a row, of which `n` values are in it (all where it holds a whole unit); the
+// others are -inf.
+template <typename T>
+__device__ __noinline__ uint4 load_odd_unit(const T* p, int n) {
   uint4 w;
-  if (align == 16) {
-    w = __ldcs(static_cast<const uint4*>(p));
-  } else if (align == 8) {
-    const uint2 a = __ldg(static_cast<const uint2*>(p)), b = __ldg(static_cast<const uint2*>(p) + 1);
-    w = make_uint4(a.x, a.y, b.x, b.y);
-  } else if (align == 4) {
-    const uint32_t* q = static_cast<const uint32_t*>(p);
-    w = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
-  } else {
-    const unsigned short* q = static_cast<const unsigned short*>(p);
-    uint32_t* o = &w.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __ldg(q + 2 * i) | (uint32_t)__ldg(q + 2 * i + 1) << 16;
+  uint32_t* o = &w.x;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    if (sizeof(T) == 4) {
+      o[i] = i < n ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0xFF800000u;
+    } else {
+      const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+      const uint32_t a = 2 * i < n ? __ldg(q + 2 * i) : 0xFC00u, b = 2 * i + 1 < n ? __ldg(q + 2 * i + 1) : 0xFC00u;
+      o[i] = a | b << 16;
+    }
   }
   return w;
+}
+
+// A warp's list cut to its N best, of which `share` are its share; returns their number.
+__device__ __noinline__ int cut_list(List& s, int count, int N, int share) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  unsigned long long *mine = s.key[warp], *room = s.all + warp * kMaxBest;
+  __syncwarp();
+  best_of(mine, count, room, N, lane, 32);
+  __syncwarp();
+  const int left = min(count, N);
+  for (int i = lane; i < left; i += 32) mine[i] = room[i];
+  if (lane == 0) {
+    if (count >= N) atomicMax(&s.bar, room[N - 1]);
+    if (count >= share) s.share[warp] = max(s.share[warp], (uint32_t)(room[share - 1] >> 32));
+  }
+  __syncwarp();
+  return left;
+}
+
+// The candidates of a warp's units, of which lane l has unit u + l, in the lanes of `hits`:
+// appended to its list, whose new length is returned.  Read again, as the values'
+// registers have no index: a lane takes a value of a unit.
+template <typename T>
+__device__ __noinline__ int scan_units(List& s, const T* x, int u, uint32_t hits, int V, int count, int N, int warps) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int lane = threadIdx.x % 32;
+  unsigned long long* mine = s.key[threadIdx.x / 32];
+#pragma unroll 1
+  for (; hits; hits &= hits - 1) {
+    const int at = (u + __ffs(hits) - 1) * kVec + lane;
+    const float l = lane < kVec && at < V ? (float)x[at] : -INFINITY;
+    const unsigned long long key = l < INFINITY ? key_of(l, at) : 0;   // 0: no candidate
+    const uint32_t some = __ballot_sync(0xffffffffu, key > bar_of(s, warps));
+    if (some >> lane & 1) mine[count + __popc(some & ((1u << lane) - 1))] = key;
+    count += __popc(some);
+    if (count > min(N + 32, kWarpList - kVec)) count = cut_list(s, count, N, (N + warps - 1) / warps);
+  }
+  __syncwarp();
+  return count;
 }
 
 template <typename T>
@@ -192,150 +286,128 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
   // Units of kVec places, wherever the row starts: two equal rows give equal sums, so
   // that their candidates tie.
   const int units = (p.V + kVec - 1) / kVec;
-  const uintptr_t start = reinterpret_cast<uintptr_t>(x);
-  const int align = start % 16 == 0 ? 16 : start % 8 == 0 ? 8 : start % 4 == 0 ? 4 : 2;
+  const bool aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0;
   const int u0 = (int)((long long)units * split / p.splits), u1 = (int)((long long)units * (split + 1) / p.splits);
-  if (tid == 0) {
-    s.count = 0;
-    s.bar = 0;
-  }
+  const int warp = tid / 32, lane = tid % 32;
+  // the warps that have a tile, and of each the keys that make N in all
+  const int warps = min(kWarps, (u1 - u0 + 31) / 32), share = (p.N + warps - 1) / warps;
+  if (tid == 0) s.bar = 0;
+  if (tid < kWarps) s.share[tid] = 0;
   __syncthreads();
+  int count = 0;                      // of the warp's list
   float c = -INFINITY, sum = 0.0f;    // sum of exp2(log2 e (l - c)), c the thread's largest
   bool odd = false;                   // a logit of +inf or NaN was left out
-  for (int t0 = u0; t0 < u1; t0 += kThreads * kUnits) {
-    float v[kEach];
-    uint4 raw[kUnits];
+  bool begun = false;
+  for (int t0 = u0 + warp * 32; t0 < u1; t0 += kThreads * kUnits) {
+    float v[kEach], tops[kUnits];     // tops: of the units
+    {
+      uint4 raw[kUnits];
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int u = t0 + i * kThreads + tid;
-      if (u < u1 && u * kVec + kVec <= p.V) raw[i] = load_unit(x + u * kVec, align);
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = t0 + i * kThreads + lane, n = u < u1 ? p.V - u * kVec : 0;
+        if (aligned && n >= kVec) raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + u * kVec));
+        else raw[i] = load_odd_unit(x + (n > 0 ? u * kVec : 0), n);
+      }
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) widen(raw[i], v + i * kVec, T());
     }
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int u = t0 + i * kThreads + tid, at = u * kVec;
-      if (u < u1 && at + kVec <= p.V) {
-        widen(raw[i], v + i * kVec, T());
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) v[i * kVec + e] = u < u1 && at + e < p.V ? (float)x[at + e] : -INFINITY;
-      }
-    }
-    auto place = [&](int i) { return (t0 + (i / kVec) * kThreads + tid) * kVec + i % kVec; };
-    float top = v[0], probe = 0.0f;
-#pragma unroll
-    for (int i = 1; i < kEach; ++i) top = fmaxf(top, v[i]);
-    auto add = [&]() {   // the tile's sum relative to the largest so far
-      const float now = fmaxf(c, top);
-      if (now == -INFINITY) return 0.0f;
-      if (now > c) {
-        const float d = c - now;
-        sum *= c == -INFINITY ? 0.0f : fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
-        c = now;
-      }
-      float part = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const float d = v[i] - c;
-        part += fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
-      }
-      return part;
-    };
+    static_assert(kUnits == 4, "four units' largest");
     const float c_was = c, sum_was = sum;
-    probe = add();
-    if (!(probe < INFINITY)) {   // +inf or NaN among them: they count as -inf, and are reported
-      odd = true;
-      top = -INFINITY;
+    float top;
+#pragma unroll 1
+    for (bool again = false;; again = true) {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        if (!(v[i] < INFINITY)) v[i] = -INFINITY;
-        top = fmaxf(top, v[i]);
+      for (int i = 0; i < kUnits; ++i) {
+        float a = fmaxf(v[i * kVec], v[i * kVec + 1]);
+#pragma unroll
+        for (int e = 2; e < kVec; e += 2) a = max3(a, v[i * kVec + e], v[i * kVec + e + 1]);
+        tops[i] = a;
       }
+      top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+      // the tile's sum relative to the largest so far
+      const float now = fmaxf(c, top);
+      float part = 0.0f;
+      if (now != -INFINITY) {
+        if (now > c) {
+          const float d = c - now;
+          sum *= c == -INFINITY ? 0.0f : fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
+          c = now;
+        }
+        const u64 minus = pair(-c, -c), high = pair(kLog2e, kLog2e), low = pair(kLog2eLow, kLog2eLow);
+        u64 parts[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < kEach; i += 2) {
+          const u64 d = add2(pair(v[i], v[i + 1]), minus);
+          const float2 e = unpair(fma2(d, high, mul2(d, low)));
+          parts[i / 2 % 2] = add2(parts[i / 2 % 2], pair(fast_exp2(e.x), fast_exp2(e.y)));
+        }
+        const float2 a = unpair(add2(parts[0], parts[1]));
+        part = a.x + a.y;
+      }
+      if ((part < INFINITY && top == top) || again) {
+        sum += part;
+        break;
+      }
+      // +inf or NaN among them: they count as -inf, and are reported
+      odd = true;
       c = c_was;
       sum = sum_was;
-      probe = add();
-    } else if (top == INFINITY || top != top) {   // (all of the thread's logits are NaN)
-      odd = true;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (!(v[i] < INFINITY)) v[i] = -INFINITY;
     }
-    sum += probe;
     // ---- candidates ----
-    if (t0 == u0) {
-      // the N-th largest of the threads' largest: at least N logits are no smaller
-      unsigned long long mine = 0;
-      if (top > -INFINITY) {
-        int where = 0;
-#pragma unroll
-        for (int i = kEach - 1; i >= 0; --i)
-          if (v[i] == top) where = place(i);
-        mine = key_of(top, where);
+    if (!begun) {
+      // the lanes' largest bound the warp's share, and its N-th, from below
+      const float order = sorted(top), a = __shfl_sync(0xffffffffu, order, share - 1),
+                  b = __shfl_sync(0xffffffffu, order, min(p.N, 32) - 1);
+      if (lane == 0) {
+        s.share[warp] = (uint32_t)(key_of(a, 0) >> 32);
+        if (p.N <= 32 && b > -INFINITY) atomicMax(&s.bar, key_of(b, 0) & ~0xFFFFFFFFull);
       }
-      s.key[tid] = mine;
-      __syncthreads();
-      int above = 0;
-      for (int j = 0; j < kThreads; ++j) above += s.key[j] > mine;
-      __syncthreads();
-      if (above == p.N - 1 && mine) s.bar = mine - 1;   // only one thread, unless it is of no logit
-      __syncthreads();
+      asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
+      begun = true;
     }
-    // may this thread have any, and how many at most
-    const unsigned long long bar = s.bar;
+    const unsigned long long bar = bar_of(s, warps);
     const float least = bar ? logit_of(bar) : -INFINITY;
-    int mine = 0;
-    if (top >= least && top > -INFINITY) {
+    if (!__any_sync(0xffffffffu, top >= least && top > -INFINITY)) continue;
+    uint32_t hits[kUnits];
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) mine += v[i] >= least && key_of(v[i], place(i)) > bar;
-    }
-    const int many = __syncthreads_or(mine > 0);
-    if (!many) continue;
-    // all at once where they are sure to fit, else a column of the tile at a time
-    __shared__ int total;
-    if (tid == 0) total = 0;
-    __syncthreads();
-    if (mine) atomicAdd(&total, mine);
-    __syncthreads();
-    const bool fit = s.count + total <= kList;
-    __syncthreads();
-    if (fit) {
-      if (mine) {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          const unsigned long long key = v[i] >= least ? key_of(v[i], place(i)) : 0;
-          if (key > bar) s.key[atomicAdd(&s.count, 1)] = key;
-        }
-      }
-      prune(s, p.N);
-    } else {
+    for (int i = 0; i < kUnits; ++i) hits[i] = __ballot_sync(0xffffffffu, tops[i] >= least && tops[i] > -INFINITY);
 #pragma unroll 1
-      for (int i = 0; i < kEach; ++i) {
-        // (an index into registers that the compiler cannot see: by selection)
-        float mine_v = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) mine_v = e == i ? v[e] : mine_v;
-        if (s.count + kThreads > kList) prune(s, p.N);   // the same for all: the count stands still here
-        const unsigned long long key = key_of(mine_v, place(i)), now = s.bar;
-        __syncthreads();
-        if (key > now) s.key[atomicAdd(&s.count, 1)] = key;
-        __syncthreads();
-      }
-      prune(s, p.N);
+    for (int i = 0; i < kUnits; ++i) {
+      const uint32_t h = i == 0 ? hits[0] : i == 1 ? hits[1] : i == 2 ? hits[2] : hits[3];
+      if (h) count = scan_units(s, x, t0 + i * kThreads, h, p.V, count, p.N, warps);
     }
   }
-  // ---- the span's sum, in binary64 from the threads' on ----
+  if (count > p.N) count = cut_list(s, count, p.N, share);
+  if (lane == 0) s.count[warp] = count;
+  // ---- the span's sum, in binary64 from the threads' on, and its N best ----
   __shared__ float tops[kWarps];
   __shared__ double parts[kWarps];
   float top = c;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (tid % 32 == 0) tops[tid / 32] = top;
+  if (lane == 0) tops[warp] = top;
   __syncthreads();
   top = tops[0];
+  int total = 0, before = 0;
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) top = fmaxf(top, tops[w]);
-  double mine = 0.0;
-  if (c > -INFINITY) mine = (double)sum * exp((double)c - (double)top);
+  for (int w = 0; w < kWarps; ++w) {
+    top = fmaxf(top, tops[w]);
+    if (w < warp) before += s.count[w];
+    total += s.count[w];
+  }
+  double term = 0.0;
+  if (c > -INFINITY) {
+    const float d = c - top;
+    term = (double)(sum * fast_exp2(fmaf(d, kLog2e, d * kLog2eLow)));
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (tid % 32 == 0) parts[tid / 32] = mine;
+  for (int o = 16; o > 0; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
+  if (lane == 0) parts[warp] = term;
   if (odd) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
+  for (int i = lane; i < count; i += 32) s.all[before + i] = s.key[warp][i];
   __syncthreads();
   const size_t at = (size_t)row * p.splits + split;
   if (tid == 0) {
@@ -343,11 +415,17 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
     for (int w = 0; w < kWarps; ++w) all += parts[w];
     __stcg(p.sums + at, make_double2(top, all));
   }
-  for (int i = tid; i < p.N; i += kThreads) __stcg(p.best + at * p.N + i, i < s.count ? s.key[i] : 0ull);
+  for (int i = tid; i < total; i += kThreads) {   // ranked among all
+    const unsigned long long key = s.all[i];
+    int above = 0;
+    for (int j = 0; j < total; ++j) above += s.all[j] > key;
+    if (above < p.N) __stcg(p.best + at * p.N + above, key);
+  }
+  for (int i = total + tid; i < p.N; i += kThreads) __stcg(p.best + at * p.N + i, 0ull);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, kResident) beam_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) unsigned char room[];   // a List, then a Merge
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -402,28 +480,49 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
   }
   if (tid == 0) {
     m.count = 0;
-    m.bar = Candidate{-INFINITY, 0};
+    m.bar = Candidate{0, 0};
   }
   __syncthreads();
   auto score_of = [&](int k, float logit) { return m.score[k] + (((double)logit - m.top[k]) - m.log_sum[k]); };
+  // candidate `i` of span `split` of beam k; rank 0: none
+  auto candidate = [&](int k, int split, int i) {
+    const int r = b * p.K + k;
+    Candidate none{0, -1};
+    if (!is_live(p.scores[r])) return none;
+    double rank;
+    long long place = (long long)k * p.V;
+    if (p.finished && p.finished[r]) {
+      if (split || i) return none;
+      rank = m.score[k] / m.scale[k];
+    } else {
+      const unsigned long long key = __ldcg(p.best + ((size_t)r * p.splits + split) * p.N + i);
+      if (!key) return none;
+      rank = score_of(k, logit_of(key)) / m.scale[k];
+      place += place_of(key);
+    }
+    return rank > -INFINITY ? Candidate{order_of(rank), place} : none;
+  };
+  // the N-th of the spans' best bounds all others
+  const int spans = p.K * p.splits;
+  if (spans >= p.N && spans <= kList) {
+    for (int i = tid; i < spans; i += kThreads) m.list[i] = candidate(i / p.splits, i % p.splits, 0);
+    __syncthreads();
+    for (int i = tid; i < spans; i += kThreads) {
+      const Candidate mine = m.list[i];
+      int above = 0;
+      for (int j = 0; j < spans; ++j) above += m.list[j].beats(mine);
+      if (above == p.N - 1 && mine.rank) m.bar = Candidate{mine.rank, mine.place + 1};   // itself beats that
+    }
+    __syncthreads();
+  }
   const int per = p.splits * p.N, all = p.K * per;
   for (int i0 = 0; i0 < all; i0 += kThreads) {
     const int i = i0 + tid;
-    Candidate mine{-INFINITY, -1};
-    if (i < all) {
-      const int k = i / per, r = b * p.K + k;
-      if (is_live(p.scores[r])) {
-        if (p.finished && p.finished[r]) {
-          if (i % per == 0) mine = Candidate{m.score[k] / m.scale[k], (long long)k * p.V};
-        } else if (const unsigned long long key = __ldcg(p.best + (size_t)r * per + i % per)) {
-          mine = Candidate{score_of(k, logit_of(key)) / m.scale[k], (long long)k * p.V + place_of(key)};
-        }
-      }
-    }
+    const Candidate mine = i < all ? candidate(i / per, i % per / p.N, i % p.N) : Candidate{0, -1};
     if (m.count + kThreads > kList) prune(m, p.N);
     const Candidate bar = m.bar;
     __syncthreads();
-    if (mine.place >= 0 && mine.rank > -INFINITY && mine.beats(bar)) m.list[atomicAdd(&m.count, 1)] = mine;
+    if (mine.rank && mine.beats(bar)) m.list[atomicAdd(&m.count, 1)] = mine;
     __syncthreads();
   }
   prune(m, p.N);
@@ -530,11 +629,20 @@ static bool shape_ok(int B, int K, int V, int N) {
   return B >= 1 && B <= kMaxItems && K >= 1 && K <= kMaxBeams && N >= 1 && N <= kMaxBest && V >= 1 && V <= (1 << 30) &&
          B * K <= 65535;
 }
-// Spans of a row: about 8 CTAs an SM in all, of at least a tile each.
+// Spans of a row: the number of least cost, in waves of resident CTAs, of a span's
+// logits and what it costs besides (about 4000 logits).
 static int splits_for(int B, int K, int V) {
-  const long long rows = (long long)B * K, tile = kThreads * kUnits * 4;
-  return (int)std::min<long long>(kMaxSplits, std::max<long long>(1, std::min((148 * 8 + rows - 1) / rows,
-                                                                              (V + tile - 1) / tile)));
+  const long long rows = (long long)B * K, resident = 148 * kResident;
+  int best = 1;
+  long long least = 0;
+  for (int s = 1; s <= kMaxSplits && (s == 1 || V / s >= 2048); ++s) {
+    const long long cost = (rows * s + resident - 1) / resident * (V / s + 4000);
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
 }
 
 }  // namespace beam
