@@ -38,8 +38,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBeams = 64, kMaxBest = 128;   // K, N
 constexpr int kMaxItems = 4096;
 constexpr int kUnits = 4;                       // 16-byte units of a thread in a tile
-constexpr int kList = 1024;                     // final candidates in shared memory
+constexpr int kKeys = 1536;                     // of the merge in shared memory, at most
 constexpr int kWarpList = 192;                  // a warp's
+constexpr int kPending = 160;                   // units a warp has put off, at most
 constexpr int kMaxSplits = 64;
 constexpr int kResident = 4;                    // CTAs an SM
 constexpr float kLog2e = 1.44269504f, kLog2eLow = 1.92596299e-8f;   // log2 e in two parts
@@ -57,6 +58,7 @@ struct Params {
   int* new_lengths;          // null where lengths is
   uint8_t* new_finished;
   int* tickets;              // [B]
+  double* scales;            // [B][K]: the ranks' divisors
   double2* sums;             // [B][K][splits]: the largest logit, sum of exp(logit - it)
   unsigned long long* best;  // [B][K][splits][N]: keys, best first
   int* dev_err;
@@ -91,6 +93,7 @@ struct List {
   unsigned long long key[kWarps][kWarpList];
   unsigned long long all[kWarps * kMaxBest];
   unsigned long long bar;   // at least N keys of the span are above it, or it is the N-th
+  int pending[kWarps][kPending];   // units that may hold candidates
   uint32_t share[kWarps];   // the warp has its share of N keys, N / warps, of this order or above
   int count[kWarps];
 };
@@ -129,14 +132,7 @@ __device__ __forceinline__ float sorted(float v) {
   return v;
 }
 
-// The final candidates, by rank, then by place k V + v.
-struct Candidate {
-  unsigned long long rank;    // a binary64 number in its order
-  long long place;
-  __device__ __forceinline__ bool beats(const Candidate& o) const {
-    return rank > o.rank || (rank == o.rank && place < o.place);
-  }
-};
+// A binary64 number as one that compares alike; 0 stays free for "none".
 __device__ __forceinline__ unsigned long long order_of(double r) {
   const unsigned long long u = (unsigned long long)__double_as_longlong(r + 0.0);   // -0 as +0
   return (u >> 63) ? ~u : u | 1ull << 63;
@@ -146,29 +142,19 @@ struct Merge {
   double top[kMaxBeams];      // lse = top + log_sum: kept apart, as a logit minus top is exact however
   double log_sum[kMaxBeams];  // large both are
   double scale[kMaxBeams];    // the rank's divisor
-  Candidate list[kList];
-  Candidate sorted[kMaxBest];
-  Candidate bar;
-  int count;
+  int ended[kMaxBeams];
+  unsigned long long key[kKeys];    // the spans' lists, where they fit
+  unsigned long long best[kKeys];   // [K][N]: the beams' lists, where they fit
+  unsigned long long rank[kKeys];   // their ranks' orders
+  int taken[kMaxBest];              // beam, candidate of it
 };
 
-__device__ __forceinline__ void prune(Merge& s, int N) {
-  __syncthreads();
-  const int n = s.count;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const Candidate mine = s.list[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += s.list[j].beats(mine);
-    if (above < N) s.sorted[above] = mine;
-  }
-  __syncthreads();
-  const int left = min(n, N);
-  for (int i = threadIdx.x; i < left; i += kThreads) s.list[i] = s.sorted[i];
-  if (threadIdx.x == 0) {
-    s.count = left;
-    if (n >= N) s.bar = s.sorted[N - 1];
-  }
-  __syncthreads();
+// The largest of the lanes' numbers and the lowest lane that has it; -1 where all are 0.
+__device__ __forceinline__ int largest_lane(unsigned long long v) {
+  const uint32_t high = (uint32_t)(v >> 32), top = __reduce_max_sync(0xffffffffu, high);
+  const uint32_t low = high == top ? (uint32_t)v : 0u, rest = __reduce_max_sync(0xffffffffu, low);
+  const uint32_t who = __ballot_sync(0xffffffffu, high == top && low == rest);
+  return top | rest ? __ffs(who) - 1 : -1;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -256,23 +242,31 @@ __device__ __noinline__ int cut_list(List& s, int count, int N, int share) {
   return left;
 }
 
-// The candidates of a warp's units, of which lane l has unit u + l, in the lanes of `hits`:
-// appended to its list, whose new length is returned.  Read again, as the values'
-// registers have no index: a lane takes a value of a unit.
+// The candidates of a warp's pending units, appended to its list, whose new length is
+// returned.  A lane takes a unit and reads it again.
 template <typename T>
-__device__ __noinline__ int scan_units(List& s, const T* x, int u, uint32_t hits, int V, int count, int N, int warps) {
+__device__ __noinline__ int scan_pending(List& s, const T* x, bool aligned, int pending, int V, int count, int N,
+                                         int warps, int share) {
   constexpr int kVec = 16 / sizeof(T);
-  const int lane = threadIdx.x % 32;
-  unsigned long long* mine = s.key[threadIdx.x / 32];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  unsigned long long* mine = s.key[warp];
+  __syncwarp();
 #pragma unroll 1
-  for (; hits; hits &= hits - 1) {
-    const int at = (u + __ffs(hits) - 1) * kVec + lane;
-    const float l = lane < kVec && at < V ? (float)x[at] : -INFINITY;
-    const unsigned long long key = l < INFINITY ? key_of(l, at) : 0;   // 0: no candidate
-    const uint32_t some = __ballot_sync(0xffffffffu, key > bar_of(s, warps));
-    if (some >> lane & 1) mine[count + __popc(some & ((1u << lane) - 1))] = key;
-    count += __popc(some);
-    if (count > min(N + 32, kWarpList - kVec)) count = cut_list(s, count, N, (N + warps - 1) / warps);
+  for (int i = 0; i < pending; i += 32) {
+    const bool some = i + lane < pending;
+    const int at = some ? s.pending[warp][i + lane] * kVec : 0, n = some ? V - at : 0;
+    const uint4 w = aligned && n >= kVec ? *reinterpret_cast<const uint4*>(x + at) : load_odd_unit(x + at, n);
+    float v[kVec];
+    widen(w, v, T());
+    const unsigned long long bar = bar_of(s, warps);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const unsigned long long key = v[e] < INFINITY ? key_of(v[e], at + e) : 0;   // 0, of -inf too: none
+      const uint32_t hits = __ballot_sync(0xffffffffu, key > bar);
+      if (hits >> lane & 1) mine[count + __popc(hits & ((1u << lane) - 1))] = key;
+      count += __popc(hits);
+      if (count > kWarpList - 32) count = cut_list(s, count, N, share);
+    }
   }
   __syncwarp();
   return count;
@@ -294,10 +288,12 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
   if (tid == 0) s.bar = 0;
   if (tid < kWarps) s.share[tid] = 0;
   __syncthreads();
-  int count = 0;                      // of the warp's list
+  int count = 0, pending = 0;         // of the warp's lists
   float c = -INFINITY, sum = 0.0f;    // sum of exp2(log2 e (l - c)), c the thread's largest
   bool odd = false;                   // a logit of +inf or NaN was left out
   bool begun = false;
+  auto sync_warps = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory"); };   // that have a tile
+  const bool more = u1 - u0 > kThreads * kUnits;
   for (int t0 = u0 + warp * 32; t0 < u1; t0 += kThreads * kUnits) {
     float v[kEach], tops[kUnits];     // tops: of the units
     {
@@ -311,7 +307,6 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) widen(raw[i], v + i * kVec, T());
     }
-    static_assert(kUnits == 4, "four units' largest");
     const float c_was = c, sum_was = sum;
     float top;
 #pragma unroll 1
@@ -323,7 +318,9 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
         for (int e = 2; e < kVec; e += 2) a = max3(a, v[i * kVec + e], v[i * kVec + e + 1]);
         tops[i] = a;
       }
-      top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+      top = tops[0];
+#pragma unroll
+      for (int i = 1; i < kUnits; ++i) top = fmaxf(top, tops[i]);
       // the tile's sum relative to the largest so far
       const float now = fmaxf(c, top);
       float part = 0.0f;
@@ -357,7 +354,8 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
         if (!(v[i] < INFINITY)) v[i] = -INFINITY;
     }
     // ---- candidates ----
-    if (!begun) {
+    const bool first = !begun;
+    if (first) {
       // the lanes' largest bound the warp's share, and its N-th, from below
       const float order = sorted(top), a = __shfl_sync(0xffffffffu, order, share - 1),
                   b = __shfl_sync(0xffffffffu, order, min(p.N, 32) - 1);
@@ -365,21 +363,48 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
         s.share[warp] = (uint32_t)(key_of(a, 0) >> 32);
         if (p.N <= 32 && b > -INFINITY) atomicMax(&s.bar, key_of(b, 0) & ~0xFFFFFFFFull);
       }
-      asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
+      sync_warps();
       begun = true;
     }
     const unsigned long long bar = bar_of(s, warps);
     const float least = bar ? logit_of(bar) : -INFINITY;
-    if (!__any_sync(0xffffffffu, top >= least && top > -INFINITY)) continue;
-    uint32_t hits[kUnits];
+    if (!first && !__any_sync(0xffffffffu, top >= least && top > -INFINITY)) continue;
+    // units that may hold candidates are put off: looking at each at once took 20 us of 67
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) hits[i] = __ballot_sync(0xffffffffu, tops[i] >= least && tops[i] > -INFINITY);
-#pragma unroll 1
     for (int i = 0; i < kUnits; ++i) {
-      const uint32_t h = i == 0 ? hits[0] : i == 1 ? hits[1] : i == 2 ? hits[2] : hits[3];
-      if (h) count = scan_units(s, x, t0 + i * kThreads, h, p.V, count, p.N, warps);
+      const bool hit = tops[i] >= least && tops[i] > -INFINITY;
+      const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+      if (hit) s.pending[warp][pending + __popc(hits & ((1u << lane) - 1))] = t0 + i * kThreads + lane;
+      pending += __popc(hits);
+    }
+    if (first || pending > kPending - 32 * kUnits) {
+      count = scan_pending(s, x, aligned, pending, p.V, count, p.N, warps, share);
+      if (!first && count > p.N) count = cut_list(s, count, p.N, share);   // it raises the bar
+      pending = 0;
+    }
+    // The N-th of all that the first tiles gave: few later logits beat it, where the bar so
+    // far lets through several a tile (48 x 8 beams 67 us without it).
+    if (first && more) {
+      if (count > p.N) count = cut_list(s, count, p.N, share);
+      if (lane == 0) s.count[warp] = count;
+      sync_warps();
+      int total = 0, before = 0;
+      for (int w = 0; w < warps; ++w) {
+        if (w < warp) before += s.count[w];
+        total += s.count[w];
+      }
+      for (int i = lane; i < count; i += 32) s.all[before + i] = s.key[warp][i];
+      sync_warps();
+      for (int i = tid; i < total; i += 32 * warps) {
+        const unsigned long long key = s.all[i];
+        int above = 0;
+        for (int j = 0; j < total; ++j) above += s.all[j] > key;
+        if (above == p.N - 1) atomicMax(&s.bar, key);
+      }
+      sync_warps();   // (the room is used again)
     }
   }
+  if (pending) count = scan_pending(s, x, aligned, pending, p.V, count, p.N, warps, share);
   if (count > p.N) count = cut_list(s, count, p.N, share);
   if (lane == 0) s.count[warp] = count;
   // ---- the span's sum, in binary64 from the threads' on, and its N best ----
@@ -432,6 +457,12 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_kernel(const __grid_
   const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, b = row / p.K;
   // a beam that is dead or ended has no logits to be read
   const bool live = is_live(p.scores[row]) && !(p.finished && p.finished[row]);
+  if (split == 0 && tid == kThreads - 1) {   // (a power in binary64 takes 2 us)
+    const int length = p.lengths ? max(p.lengths[row], 0) : 0;
+    const int steps = p.finished && p.finished[row] ? max(length, 1) : length + 1;
+    __stcg(p.scales + row, p.alpha == 0.0f ? 1.0 : pow((double)steps, (double)p.alpha));
+    if (!(p.scores[row] < INFINITY)) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
+  }
   if (live) span_pass<T>(p, *reinterpret_cast<List*>(room), row, split);
   // ---- the item's last CTA goes on ----
   __shared__ int last;
@@ -446,13 +477,29 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_kernel(const __grid_
   if (!last) return;
   __threadfence();
   Merge& m = *reinterpret_cast<Merge*>(room);
-  for (int k = tid / 32; k < p.K; k += kWarps) {   // a beam a warp
-    const int r = b * p.K + k, lane = tid % 32;
+  const int warp = tid / 32, lane = tid % 32;
+  const int per = p.splits * p.N;                                    // keys of a beam
+  const bool keys_fit = p.K * per <= kKeys, best_fit = p.K * p.N <= kKeys;
+  unsigned long long* spans = p.best + (size_t)b * p.K * per;
+  if (keys_fit)
+    for (int i = tid; i < p.K * per; i += kThreads) m.key[i] = __ldcg(spans + i);
+  __syncthreads();
+  // ---- a beam a warp: its sum, and its N best, the heads of its spans' lists compared ----
+  for (int k = warp; k < p.K; k += kWarps) {
+    const int r = b * p.K + k;
     const float score = p.scores[r];
     const bool ended = p.finished && p.finished[r];
-    const int length = p.lengths ? max(p.lengths[r], 0) : 0;
-    double largest = 0.0, log_sum = 0.0;
-    if (is_live(score) && !ended) {
+    unsigned long long* to = best_fit ? m.best + k * p.N : spans + (size_t)k * per;   // (in place: see below)
+    if (lane == 0) {
+      m.score[k] = score;
+      m.scale[k] = __ldcg(p.scales + r);
+      m.ended[k] = ended;
+    }
+    int found = 0;
+    if (is_live(score) && ended) {
+      if (lane == 0) to[0] = 1;   // any key will do
+      found = 1;
+    } else if (is_live(score)) {
       static_assert(kMaxSplits <= 64, "two spans a lane");
       const double2 none = make_double2(-INFINITY, 0.0);
       const double2* at = p.sums + (size_t)r * p.splits;
@@ -461,97 +508,118 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_kernel(const __grid_
       double top = fmax(one.x, two.x);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-      double all = 0.0;
-      if (one.y > 0.0) all = one.y * exp(one.x - top);
-      if (two.y > 0.0) all += two.y * exp(two.x - top);
+      // (binary32 exponents of binary32 differences, as in a span)
+      auto part = [&](double2 v) {
+        const float d = (float)(v.x - top);
+        return v.y > 0.0 ? v.y * (double)fast_exp2(fmaf(d, kLog2e, d * kLog2eLow)) : 0.0;
+      };
+      double all = part(one) + part(two);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-      largest = top;            // of a beam without candidates: not used
-      log_sum = log(all);
+      if (lane == 0) {
+        m.top[k] = top;           // of a beam without candidates: not used
+        m.log_sum[k] = log(all);
+      }
+      auto key_at = [&](int span, int i) {
+        if (span >= p.splits || i >= p.N) return 0ull;
+        return keys_fit ? m.key[k * per + span * p.N + i] : __ldcg(spans + (size_t)k * per + span * p.N + i);
+      };
+      if (p.splits == 1) {
+        if (best_fit)   // else it is there
+          for (int i = lane; i < p.N; i += 32) to[i] = key_at(0, i);
+        found = p.N;
+      } else {
+        // Keys differ, so a head is at one lane only.  The list grows in registers' place:
+        // results go out behind the loop where they would overwrite lists still to be read.
+        int i0 = 0, i1 = 0;
+        unsigned long long h0 = key_at(lane, 0), h1 = key_at(lane + 32, 0), kept[kMaxBest / 32];
+#pragma unroll
+        for (int q = 0; q < kMaxBest / 32; ++q) kept[q] = 0;
+        for (; found < p.N; ++found) {
+          const unsigned long long mine = h0 > h1 ? h0 : h1;
+          const int l = largest_lane(mine);
+          if (l < 0) break;
+          const unsigned long long best = __shfl_sync(0xffffffffu, mine, l);
+#pragma unroll
+          for (int q = 0; q < kMaxBest / 32; ++q)
+            if (found == 32 * q + lane) kept[q] = best;
+          if (lane == l) {
+            if (h0 > h1) h0 = key_at(lane, ++i0);
+            else h1 = key_at(lane + 32, ++i1);
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < kMaxBest / 32; ++q)
+          if (32 * q + lane < found) to[32 * q + lane] = kept[q];
+      }
     }
-    if (lane == 0) {
-      if (!(score < INFINITY)) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
-      m.score[k] = score;
-      m.top[k] = largest;
-      m.log_sum[k] = log_sum;
-      const int steps = ended ? max(length, 1) : length + 1;
-      m.scale[k] = p.alpha == 0.0f ? 1.0 : pow((double)steps, (double)p.alpha);
-    }
-  }
-  if (tid == 0) {
-    m.count = 0;
-    m.bar = Candidate{0, 0};
+    __syncwarp();
+    for (int i = found + lane; i < p.N; i += 32) to[i] = 0;
   }
   __syncthreads();
-  auto score_of = [&](int k, float logit) { return m.score[k] + (((double)logit - m.top[k]) - m.log_sum[k]); };
-  // candidate `i` of span `split` of beam k; rank 0: none
-  auto candidate = [&](int k, int split, int i) {
-    const int r = b * p.K + k;
-    Candidate none{0, -1};
-    if (!is_live(p.scores[r])) return none;
-    double rank;
-    long long place = (long long)k * p.V;
-    if (p.finished && p.finished[r]) {
-      if (split || i) return none;
-      rank = m.score[k] / m.scale[k];
-    } else {
-      const unsigned long long key = __ldcg(p.best + ((size_t)r * p.splits + split) * p.N + i);
-      if (!key) return none;
-      rank = score_of(k, logit_of(key)) / m.scale[k];
-      place += place_of(key);
-    }
-    return rank > -INFINITY ? Candidate{order_of(rank), place} : none;
+  // ---- ranks, and the N best of all ----
+  auto key_of_beam = [&](int k, int i) {
+    return best_fit ? m.best[k * p.N + i] : *reinterpret_cast<volatile unsigned long long*>(spans + (size_t)k * per + i);
   };
-  // the N-th of the spans' best bounds all others
-  const int spans = p.K * p.splits;
-  if (spans >= p.N && spans <= kList) {
-    for (int i = tid; i < spans; i += kThreads) m.list[i] = candidate(i / p.splits, i % p.splits, 0);
-    __syncthreads();
-    for (int i = tid; i < spans; i += kThreads) {
-      const Candidate mine = m.list[i];
-      int above = 0;
-      for (int j = 0; j < spans; ++j) above += m.list[j].beats(mine);
-      if (above == p.N - 1 && mine.rank) m.bar = Candidate{mine.rank, mine.place + 1};   // itself beats that
+  auto score_of = [&](int k, unsigned long long key) {
+    return m.ended[k] ? m.score[k] : m.score[k] + (((double)logit_of(key) - m.top[k]) - m.log_sum[k]);
+  };
+  auto order_at = [&](int k, int i) {   // 0: no candidate, or one of a rank that is none
+    const unsigned long long key = key_of_beam(k, i);
+    if (!key) return 0ull;
+    const double rank = score_of(k, key) / m.scale[k];
+    return rank > -INFINITY ? order_of(rank) : 0ull;
+  };
+  if (best_fit)
+    for (int i = tid; i < p.K * p.N; i += kThreads) m.rank[i] = order_at(i / p.N, i % p.N);
+  __syncthreads();
+  __shared__ int chosen;
+  if (warp == 0) {
+    static_assert(kMaxBeams <= 64, "two beams a lane");
+    // lane l has beams 2 l and 2 l + 1: of equal ranks the lowest lane's lower beam is first
+    auto head = [&](int k, int i) {
+      if (k >= p.K || i >= p.N) return 0ull;
+      return best_fit ? m.rank[k * p.N + i] : order_at(k, i);
+    };
+    int i0 = 0, i1 = 0, n = 0;
+    unsigned long long h0 = head(2 * lane, 0), h1 = head(2 * lane + 1, 0);
+    for (; n < p.N; ++n) {
+      const int l = largest_lane(h0 >= h1 ? h0 : h1);
+      if (l < 0) break;
+      if (lane == l) {
+        if (h0 >= h1) {
+          m.taken[n] = 2 * lane << 16 | i0;
+          h0 = head(2 * lane, ++i0);
+        } else {
+          m.taken[n] = (2 * lane + 1) << 16 | i1;
+          h1 = head(2 * lane + 1, ++i1);
+        }
+      }
     }
-    __syncthreads();
+    if (lane == 0) chosen = n;
   }
-  const int per = p.splits * p.N, all = p.K * per;
-  for (int i0 = 0; i0 < all; i0 += kThreads) {
-    const int i = i0 + tid;
-    const Candidate mine = i < all ? candidate(i / per, i % per / p.N, i % p.N) : Candidate{0, -1};
-    if (m.count + kThreads > kList) prune(m, p.N);
-    const Candidate bar = m.bar;
-    __syncthreads();
-    if (mine.rank && mine.beats(bar)) m.list[atomicAdd(&m.count, 1)] = mine;
-    __syncthreads();
-  }
-  prune(m, p.N);
+  __syncthreads();
   for (int i = tid; i < p.N; i += kThreads) {
     const int at = b * p.N + i;
-    if (i >= m.count) {
+    if (i >= chosen) {
       p.tokens[at] = p.parents[at] = -1;
       p.new_scores[at] = -INFINITY;
       p.new_finished[at] = 1;
       if (p.new_lengths) p.new_lengths[at] = 0;
       continue;
     }
-    const Candidate c = m.list[i];
-    const int k = (int)(c.place / p.V), r = b * p.K + k;
-    const bool ended = p.finished && p.finished[r];
-    const int token = ended ? p.pad : (int)(c.place % p.V);
+    const int k = m.taken[i] >> 16;
+    const unsigned long long key = key_of_beam(k, m.taken[i] & 0xffff);
+    const bool ended = m.ended[k];
+    const int token = ended ? p.pad : place_of(key);
     bool over = ended;
     for (int e = 0; e < p.eos_count; ++e) over |= p.eos[e] == token;
     p.tokens[at] = token;
     p.parents[at] = k;
-    // the score itself, not the rank times its divisor
-    double score = p.scores[r];
-    if (!ended) {
-      const T* x = static_cast<const T*>(p.logits) + (long long)r * p.stride;
-      score = score_of(k, (float)x[token]);
-    }
-    p.new_scores[at] = (float)score;
+    p.new_scores[at] = (float)score_of(k, key);
     p.new_finished[at] = over;
-    if (p.new_lengths) p.new_lengths[at] = p.lengths[r] + !ended;
+    if (p.new_lengths) p.new_lengths[at] = max(p.lengths[b * p.K + k], 0) + !ended;
   }
 }
 
@@ -654,7 +722,7 @@ size_t anvilq_beam_select_workspace_size(int B, int K, int V, int N) {
   using namespace anvilq::beam;
   if (!shape_ok(B, K, V, N)) return 0;
   const size_t spans = (size_t)B * K * splits_for(B, K, V);
-  return ANVILQ_WORKSPACE_COUNTER_BYTES + spans * (sizeof(double2) + (size_t)N * 8);
+  return ANVILQ_WORKSPACE_COUNTER_BYTES + spans * (sizeof(double2) + (size_t)N * 8) + (size_t)B * K * sizeof(double);
 }
 
 int anvilq_beam_select(const void* logits, int logits_half, long long logits_stride, const float* scores,
@@ -719,6 +787,7 @@ int anvilq_beam_select(const void* logits, int logits_half, long long logits_str
   p.tickets = static_cast<int*>(workspace);
   p.sums = reinterpret_cast<double2*>(at);
   p.best = reinterpret_cast<unsigned long long*>(at + (size_t)B * K * p.splits * sizeof(double2));
+  p.scales = reinterpret_cast<double*>(p.best + (size_t)B * K * p.splits * N);
   const size_t smem = std::max(sizeof(List), sizeof(Merge));
   const dim3 grid(p.splits, B * K);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
