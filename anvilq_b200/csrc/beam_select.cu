@@ -272,6 +272,15 @@ __device__ __noinline__ int scan_pending(List& s, const T* x, bool aligned, int 
   return count;
 }
 
+// The divisor of a beam's ranks, for the merge: a power in binary64 takes 2 us, here beside
+// other threads' work.
+__device__ __noinline__ void write_divisor(const Params& p, int row) {
+  const int length = p.lengths ? max(p.lengths[row], 0) : 0;
+  const int steps = p.finished && p.finished[row] ? max(length, 1) : length + 1;
+  __stcg(p.scales + row, p.alpha == 0.0f ? 1.0 : p.alpha == 1.0f ? (double)steps : pow((double)steps, (double)p.alpha));
+  if (!(p.scores[row] < INFINITY)) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
+}
+
 template <typename T>
 __device__ void span_pass(const Params& p, List& s, int row, int split) {
   constexpr int kVec = 16 / sizeof(T), kEach = kUnits * kVec;
@@ -293,7 +302,7 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
   bool odd = false;                   // a logit of +inf or NaN was left out
   bool begun = false;
   auto sync_warps = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory"); };   // that have a tile
-  const bool more = u1 - u0 > kThreads * kUnits;
+  const bool more = u1 - u0 > 3 * kThreads * kUnits;
   for (int t0 = u0 + warp * 32; t0 < u1; t0 += kThreads * kUnits) {
     float v[kEach], tops[kUnits];     // tops: of the units
     {
@@ -440,6 +449,7 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
     for (int w = 0; w < kWarps; ++w) all += parts[w];
     __stcg(p.sums + at, make_double2(top, all));
   }
+  if (split == 0 && tid == kThreads - 1) write_divisor(p, row);
   for (int i = tid; i < total; i += kThreads) {   // ranked among all
     const unsigned long long key = s.all[i];
     int above = 0;
@@ -457,25 +467,19 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_kernel(const __grid_
   const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, b = row / p.K;
   // a beam that is dead or ended has no logits to be read
   const bool live = is_live(p.scores[row]) && !(p.finished && p.finished[row]);
-  if (split == 0 && tid == kThreads - 1) {   // (a power in binary64 takes 2 us)
-    const int length = p.lengths ? max(p.lengths[row], 0) : 0;
-    const int steps = p.finished && p.finished[row] ? max(length, 1) : length + 1;
-    __stcg(p.scales + row, p.alpha == 0.0f ? 1.0 : pow((double)steps, (double)p.alpha));
-    if (!(p.scores[row] < INFINITY)) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
-  }
+  if (!live && split == 0 && tid == kThreads - 1) write_divisor(p, row);
   if (live) span_pass<T>(p, *reinterpret_cast<List*>(room), row, split);
   // ---- the item's last CTA goes on ----
   __shared__ int last;
-  __threadfence();
-  __syncthreads();
+  __syncthreads();   // the thread that takes the ticket releases, and acquires, for all
   if (tid == 0) {
-    const int arrived = atomicAdd(p.tickets + b, 1);
+    int arrived;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(arrived) : "l"(p.tickets + b) : "memory");
     last = arrived == p.K * p.splits - 1;
     if (last) p.tickets[b] = 0;
   }
   __syncthreads();
   if (!last) return;
-  __threadfence();
   Merge& m = *reinterpret_cast<Merge*>(room);
   const int warp = tid / 32, lane = tid % 32;
   const int per = p.splits * p.N;                                    // keys of a beam
