@@ -40,7 +40,7 @@ constexpr int kPlan = 1024;            // threads of a planning CTA
 constexpr int kMaxRows = 16384;        // rows of a table: their first entries' numbers lie in shared memory
 constexpr int kMaxPools = 128;         // pools of one copy launch (more: several)
 constexpr int kCopyThreads = 256;
-constexpr int kAhead = 8;              // 16-byte pieces of a thread on their way
+constexpr int kAhead = 8;              // loads of a thread on their way
 constexpr uint32_t kValid = 1u << 31;
 
 // A moved page: rows < 0 means the whole page.
@@ -423,55 +423,56 @@ struct Copy {
   const int* rows;         // may be null: whole pages
   const int* count;        // may be null: `most`
   int* dev_err;
-  int most, pools, pieces, num_pages;
+  int most, num_pages, pools;
+  int stretches;   // of a page
   Pool pool[kMaxPools];
 };
 
-// Resident CTAs, a piece of a page of a pool at a time: kAhead loads a thread, then
-// their stores.
+// Resident CTAs over stretches of a moved page of a pool, each a team's: a CTA of TEAM = 256
+// threads takes 32 KB at a time, a warp 4 KB where pages are smaller, so that kAhead loads
+// of every thread are on their way before their stores.  W: 16 bytes, or 4 where pools are
+// not aligned to more.
+template <typename W, int TEAM>
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ Copy p) {
   prologue();
+  constexpr unsigned kStep = TEAM * sizeof(W), kRounds = 16 / sizeof(W);
+  constexpr int kTeams = kCopyThreads / TEAM;
+  const unsigned team = TEAM == kCopyThreads ? 0 : threadIdx.x / TEAM, me = threadIdx.x % TEAM;
   const int count = p.count ? min(max(*p.count, 0), p.most) : p.most;
-  const long long units = (long long)count * p.pools * p.pieces;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int piece = (int)(u % p.pieces);
-    const int t = (int)(u / p.pieces);
+  const long long units = (long long)count * p.pools * p.stretches;
+  for (long long u = (long long)blockIdx.x * kTeams + team; u < units; u += (long long)gridDim.x * kTeams) {
+    const int stretch = (int)(u % p.stretches);
+    const int t = (int)(u / p.stretches);
     const int i = t / p.pools;
     const Pool& pool = p.pool[t % p.pools];
     const Move m = p.moves ? p.moves[i] : Move{p.src[i], p.dst[i], p.rows ? p.rows[i] : -1};
     if (m.src < 0 || m.dst < 0) continue;
     if (m.src >= p.num_pages || m.dst >= p.num_pages) {
-      if (threadIdx.x == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
+      if (me == 0) atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
       continue;
     }
+    // of a segment of the page, what the move's rows take
     const unsigned live = m.rows < 0 ? pool.segment_bytes
                                      : min(pool.segment_bytes,
-                                           ((unsigned)m.rows + pool.unit_tokens - 1) / pool.unit_tokens *
-                                               pool.unit_bytes);   // of a segment, to be copied
+                                           ((unsigned)m.rows + pool.unit_tokens - 1) / pool.unit_tokens * pool.unit_bytes);
     const unsigned page_bytes = pool.segments * pool.segment_bytes;   // below 2^31
     const char* from = pool.base + (size_t)m.src * page_bytes;
     char* to = pool.base + (size_t)m.dst * page_bytes;
-    auto run = [&](auto word) {
-      using W = decltype(word);
-      const unsigned begin = (unsigned)piece * (kCopyThreads * kAhead * 16);   // below 2^31 + 2^15
-      constexpr int kRounds = 16 / sizeof(W);
-      for (int round = 0; round < kRounds; ++round) {
-        W w[kAhead];
-        bool on[kAhead];
-        const unsigned o0 = begin + (round * kAhead * kCopyThreads + threadIdx.x) * (unsigned)sizeof(W);
+#pragma unroll 1
+    for (unsigned round = 0; round < kRounds; ++round) {
+      const unsigned o0 = (stretch * kRounds + round) * (kAhead * kStep) + me * (unsigned)sizeof(W);
+      W w[kAhead];
+      bool on[kAhead];
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-          const unsigned o = o0 + a * kCopyThreads * (unsigned)sizeof(W);
-          on[a] = o < page_bytes && (pool.segments == 1 ? o : o % pool.segment_bytes) < live;
-          if (on[a]) w[a] = *reinterpret_cast<const W*>(from + o);
-        }
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a)
-          if (on[a]) *reinterpret_cast<W*>(to + o0 + a * kCopyThreads * (unsigned)sizeof(W)) = w[a];
+      for (int a = 0; a < kAhead; ++a) {
+        const unsigned o = o0 + a * kStep;
+        on[a] = o < page_bytes && (pool.segments == 1 ? o : o % pool.segment_bytes) < live;
+        if (on[a]) w[a] = *reinterpret_cast<const W*>(from + o);
       }
-    };
-    if (((reinterpret_cast<uintptr_t>(pool.base) | pool.segment_bytes | pool.unit_bytes) & 15) == 0) run(uint4{});
-    else run(uint32_t{});
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+        if (on[a]) *reinterpret_cast<W*>(to + o0 + a * kStep) = w[a];
+    }
   }
 }
 
@@ -519,22 +520,32 @@ static int check_pools(const anvilq_page_pool* pools, int n, int num_pages, int 
   return ANVILQ_OK;
 }
 
-// The copies of `moves` (or of the lists) in all pools.
+// The copies of `moves` (or of the lists) in all pools: those aligned to 16 bytes, then the
+// others.
 static int copy_all(Copy& c, const anvilq_page_pool* pools, int n, int page_tokens, bool overlaps, cudaStream_t st) {
-  for (int done = 0; done < n; done += kMaxPools) {
-    c.pools = std::min(kMaxPools, n - done);
-    size_t widest = 0;
-    for (int i = 0; i < c.pools; ++i) {
-      const anvilq_page_pool& a = pools[done + i];
-      c.pool[i] = Pool{static_cast<char*>(a.base), (unsigned)a.segments, (unsigned)a.segment_bytes,
-                       (unsigned)(a.segment_bytes / (page_tokens / a.unit_tokens)), (unsigned)a.unit_tokens};
-      widest = std::max(widest, (size_t)a.segments * a.segment_bytes);
+  for (int odd = 0; odd < 2; ++odd) {
+    for (int next = 0; next < n;) {
+      size_t widest = 0;
+      for (c.pools = 0; next < n && c.pools < kMaxPools; ++next) {
+        const anvilq_page_pool& a = pools[next];
+        const int unit = a.segment_bytes / (page_tokens / a.unit_tokens);
+        if ((aligned(a.base, 16) && a.segment_bytes % 16 == 0 && unit % 16 == 0) == (bool)odd) continue;
+        c.pool[c.pools++] = Pool{static_cast<char*>(a.base), (unsigned)a.segments, (unsigned)a.segment_bytes,
+                                 (unsigned)unit, (unsigned)a.unit_tokens};
+        widest = std::max(widest, (size_t)a.segments * a.segment_bytes);
+      }
+      if (!c.pools) continue;
+      const bool small = widest < (size_t)kCopyThreads * kAhead * 16;
+      const size_t stretch = (size_t)(small ? 32 : kCopyThreads) * kAhead * 16;
+      c.stretches = (int)((widest + stretch - 1) / stretch);
+      const double units = (double)c.most * c.pools * c.stretches;
+      const int ctas = (int)std::min(std::max(small ? units / (kCopyThreads / 32) : units, 1.0), 148.0 * 6);
+      auto go = [&](auto kernel) { return launch(kernel, ctas, kCopyThreads, 0, st, overlaps, c); };
+      const int rc = odd ? (small ? go(copy_kernel<uint32_t, 32>) : go(copy_kernel<uint32_t, kCopyThreads>))
+                         : (small ? go(copy_kernel<uint4, 32>) : go(copy_kernel<uint4, kCopyThreads>));
+      if (rc) return rc;
+      overlaps = true;   // the next one waits for this one's stores all the same
     }
-    c.pieces = (int)((widest + kCopyThreads * kAhead * 16 - 1) / (kCopyThreads * kAhead * 16));
-    const double units = (double)c.most * c.pools * c.pieces;
-    const int ctas = (int)std::min(units, 148.0 * 6);
-    if (const int rc = launch(copy_kernel, std::max(ctas, 1), kCopyThreads, 0, st, overlaps, c)) return rc;
-    overlaps = true;   // the next one waits for this one's stores all the same
   }
   return ANVILQ_OK;
 }

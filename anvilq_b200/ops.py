@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 import threading
 
 import torch
@@ -1197,23 +1198,23 @@ class PagePools:
         name = "PagePools"
         self.pools, self.page_tokens = list(pools), int(page_tokens)
         self.num_pages = self.device = self.array = None
-        n, pt = len(self.pools), self.page_tokens
-        if not n:
+        if not self.pools:
             return
-        self.num_pages, self.device = self.pools[0].shape[0], self.pools[0].device
-        index, known = self.pools[0].get_device(), {}     # (type, shape) -> how its pages lie
+        first = self.pools[0]
+        self.num_pages, self.device = first.shape[0], first.device
+        index = first.get_device()
         if index < 0:
             raise ValueError(f"{name}: pools must be on a CUDA device")
-        self.array = (_lib.PagePool * n)()
-        for a, t in zip(self.array, self.pools):
-            kind = (t.dtype, t.shape)
-            how = known.get(kind)
-            if how is None:
-                how = known[kind] = self._layout(name, t, pt)
+        fields, kind, shape = [], None, None         # pools of a kind come one after the other
+        for t in self.pools:
+            if t.dtype is not kind or t.shape != shape:
+                kind, shape = t.dtype, t.shape
+                segments, size, unit = self._layout(name, t, self.page_tokens)
             if not t.is_contiguous() or t.get_device() != index:
                 raise ValueError(f"{name}: pools must be contiguous and on one device")
-            a.base = t.data_ptr()
-            a.segments, a.segment_bytes, a.unit_tokens = how
+            fields += (t.data_ptr(), segments, size, unit)
+        # an array of anvilq_page_pool
+        self.array = struct.pack("Qiii4x" * len(self.pools), *fields)
 
     def _layout(self, name, t, pt):
         shape = tuple(t.shape)
@@ -1227,6 +1228,8 @@ class PagePools:
             raise ValueError(f"{name}: {t.dtype} {list(shape)} is no pool of pages of {pt} tokens")
         if shape[0] != self.num_pages or 0 in shape:
             raise ValueError(f"{name}: all pools must hold the same number of pages")
+        if how[0] * how[1] >= 1 << 31:
+            raise ValueError(f"{name}: a page of {how[0] * how[1]} bytes")
         return how
 
 
