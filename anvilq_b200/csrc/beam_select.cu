@@ -25,6 +25,7 @@
 // the tile in all).  The span's sum and N best go to the workspace, and the item's last
 // CTA (by a ticket) merges them.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "kv_q8.cuh"
@@ -276,8 +277,8 @@ __device__ __noinline__ int scan_pending(List& s, const T* x, bool aligned, int 
 // other threads' work.
 __device__ __noinline__ void write_divisor(const Params& p, int row) {
   const int length = p.lengths ? max(p.lengths[row], 0) : 0;
-  const int steps = p.finished && p.finished[row] ? max(length, 1) : length + 1;
-  __stcg(p.scales + row, p.alpha == 0.0f ? 1.0 : p.alpha == 1.0f ? (double)steps : pow((double)steps, (double)p.alpha));
+  const double steps = p.finished && p.finished[row] ? (double)max(length, 1) : (double)length + 1.0;
+  __stcg(p.scales + row, p.alpha == 0.0f ? 1.0 : p.alpha == 1.0f ? steps : pow(steps, (double)p.alpha));
   if (!(p.scores[row] < INFINITY)) atomicOr(p.dev_err, ANVILQ_DEV_ERR_NONFINITE);
 }
 
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_kernel(const __grid_
     p.parents[at] = k;
     p.new_scores[at] = (float)score_of(k, key);
     p.new_finished[at] = over;
-    if (p.new_lengths) p.new_lengths[at] = max(p.lengths[b * p.K + k], 0) + !ended;
+    if (p.new_lengths) p.new_lengths[at] = ended ? max(p.lengths[b * p.K + k], 0) : min(max(p.lengths[b * p.K + k], 0), INT_MAX - 1) + 1;
   }
 }
 

@@ -1120,7 +1120,7 @@ int anvilq_gqa_chunk_paged(const uint16_t* q, long long q_stride, const uint16_t
       (long long)page_tokens * max_pages > (1LL << 30))
     return ANVILQ_ESHAPE;
   const long long positions = (long long)num_pages * page_tokens;
-  if (positions > 0x7FFFFFFFLL) return ANVILQ_ESHAPE;   // a TMA coordinate is an int
+  if (positions > 0x7FFFFFFFLL || (T > 0 && q_stride > 1LL << 38)) return ANVILQ_ESHAPE;   // of a tensor map
   if (!a16(q) || !a16(k_pool) || !a16(v_pool) || !a16(out) || !a16(workspace) || q_stride % 8) return ANVILQ_EALIGN;
   if (T == 0) return ANVILQ_OK;
   const size_t pool = (size_t)positions * Hkv * D * 2, rows = (size_t)T * Hq * D * 2;

@@ -758,7 +758,7 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
  * (token_starts[b] <= t < token_starts[b + 1], as for anvilq_paged_kv_append, which
  * puts its key and value into the pages before) is at position seqlens[b] -
  * token_starts[b + 1] + t and sees every position up to its own.  q and out fp16 [T]
- * tokens of [Hq][D], q's q_stride elements apart (a multiple of 8), out's without
+ * tokens of [Hq][D], q's q_stride elements apart (a multiple of 8, at most 2^38), out's without
  * gaps; rows of no sequence are neither read nor written.  Scores, sums and outputs in
  * fp32, the probabilities enter the tensor cores as binary16.  What lies behind a
  * sequence's last token may be anything; a NaN or an infinity among the values of new
