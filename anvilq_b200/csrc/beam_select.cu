@@ -308,11 +308,17 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
     float v[kEach], tops[kUnits];     // tops: of the units
     {
       uint4 raw[kUnits];
+      const int end = t0 + (kUnits - 1) * kThreads + 32;   // of the tile's units
+      if (aligned && end <= u1 && end <= p.V / kVec) {     // the same for all lanes
 #pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-        const int u = t0 + i * kThreads + lane, n = u < u1 ? p.V - u * kVec : 0;
-        if (aligned && n >= kVec) raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + u * kVec));
-        else raw[i] = load_odd_unit(x + (n > 0 ? u * kVec : 0), n);
+        for (int i = 0; i < kUnits; ++i)
+          raw[i] = __ldcs(reinterpret_cast<const uint4*>(x) + (t0 + i * kThreads + lane));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int u = t0 + i * kThreads + lane, n = u < u1 ? p.V - u * kVec : 0;
+          raw[i] = load_odd_unit(x + (n > 0 ? u * kVec : 0), n);
+        }
       }
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) widen(raw[i], v + i * kVec, T());
@@ -702,14 +708,16 @@ static bool shape_ok(int B, int K, int V, int N) {
   return B >= 1 && B <= kMaxItems && K >= 1 && K <= kMaxBeams && N >= 1 && N <= kMaxBest && V >= 1 && V <= (1 << 30) &&
          B * K <= 65535;
 }
-// Spans of a row: the number of least cost, in waves of resident CTAs, of a span's
-// logits and what it costs besides (about 4000 logits).
+// Spans of a row: the number of least cost, in waves of resident CTAs, of a span's logits
+// and what it costs besides.  (8 us: as much as 60000 logits, so that a second wave seldom
+// pays.  48 x 8 rows of 151936 fp16 logits as one span 58.6 us, as three 60.7; 64 rows as
+// nine 22.9, as two 26.3.)
 static int splits_for(int B, int K, int V) {
   const long long rows = (long long)B * K, resident = 148 * kResident;
   int best = 1;
   long long least = 0;
   for (int s = 1; s <= kMaxSplits && (s == 1 || V / s >= 2048); ++s) {
-    const long long cost = (rows * s + resident - 1) / resident * (V / s + 4000);
+    const long long cost = (rows * s + resident - 1) / resident * (V / s + 60000);
     if (s == 1 || cost < least) {
       least = cost;
       best = s;
