@@ -376,7 +376,7 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
       const float order = sorted(top), a = __shfl_sync(0xffffffffu, order, share - 1),
                   b = __shfl_sync(0xffffffffu, order, min(p.N, 32) - 1);
       if (lane == 0) {
-        s.share[warp] = (uint32_t)(key_of(a, 0) >> 32);
+        if (share <= 32) s.share[warp] = (uint32_t)(key_of(a, 0) >> 32);   // else there are too few lanes to tell
         if (p.N <= 32 && b > -INFINITY) atomicMax(&s.bar, key_of(b, 0) & ~0xFFFFFFFFull);
       }
       sync_warps();

@@ -111,6 +111,17 @@ def test_select(dev, B, K, V, N, half):
 
 
 @pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("V,N", [(64, 64), (128, 128), (126, 100), (256, 128), (256, 70), (384, 100), (512, 128), (768, 97)])
+def test_more_candidates_than_a_warps_lanes(dev, V, N, half):
+    """Rows of whole warps' units, of which a warp has to give more candidates than it has lanes."""
+    x, scores, lengths, _ = inputs(V * N, 3, 2, V, half, dev)
+    check(x, scores, N, got=ops.beam_select(x, scores, N))
+    scores[:, 1] = -float("inf")   # the other beam gives them all
+    check(x, scores, N, lengths, 1.0, got=ops.beam_select(x, scores, N, lengths=lengths, length_penalty=1.0))
+    ops.raise_device_errors(dev)
+
+
+@pytest.mark.parametrize("half", [False, True])
 def test_ties_go_to_the_lowest_place(dev, half):
     """Rows of few values, rows all alike, and equal beams of equal scores, at odd rows too."""
     for V in (5000, 9001):
