@@ -214,12 +214,14 @@ __global__ void __launch_bounds__(kPlan) reserve_kernel(const __grid_constant__ 
   auto needs = [&](const Entry& x, int e) {
     if (x.page < 0) return x.page == -1;
     const Writers w = p.writers[x.page];
-    return w.refs > 1 && !(w.refs == w.count && w.last == e);
+    return w.refs > 1 && w.refs >= w.count && !(w.refs == w.count && w.last == e);   // (below: miscounted, passed over)
   };
   int wanted = 0;
   for (int e0 = 0; e0 < entries; e0 += kPlan) {
     const int e = e0 + tid;
-    wanted += __syncthreads_count(needs(entry(e), e));
+    const Entry x = entry(e);
+    if (x.page >= 0 && p.writers[x.page].refs < p.writers[x.page].count) atomicOr(p.dev_err, ANVILQ_DEV_ERR_PAGE);
+    wanted += __syncthreads_count(needs(x, e));
   }
   // ---- that many of the free pages, the lowest ----
   int found = 0;
@@ -453,8 +455,9 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
     }
     // of a segment of the page, what the move's rows take
     const unsigned live = m.rows < 0 ? pool.segment_bytes
-                                     : min(pool.segment_bytes,
-                                           ((unsigned)m.rows + pool.unit_tokens - 1) / pool.unit_tokens * pool.unit_bytes);
+                                     : (unsigned)min((unsigned long long)pool.segment_bytes,
+                                                     (unsigned long long)(((unsigned)m.rows + pool.unit_tokens - 1) /
+                                                                          pool.unit_tokens) * pool.unit_bytes);
     const unsigned page_bytes = pool.segments * pool.segment_bytes;   // below 2^31
     const char* from = pool.base + (size_t)m.src * page_bytes;
     char* to = pool.base + (size_t)m.dst * page_bytes;
@@ -503,9 +506,10 @@ struct Span {
   const void* start;
   size_t bytes;
 };
-static int check_pools(const anvilq_page_pool* pools, int n, int num_pages, int page_tokens,
+static int check_pools(const anvilq_page_pool* pools, int n, int num_pages, int moves, int page_tokens,
                        std::initializer_list<Span> others) {
   if (n < 0 || (n && !pools)) return ANVILQ_EINVAL;
+  if ((long long)std::min(n, kMaxPools) * moves > INT_MAX) return ANVILQ_ESHAPE;   // a copy launch's numbers of them
   for (int i = 0; i < n; ++i) {
     const anvilq_page_pool& a = pools[i];
     if (!a.base || a.segments < 1 || a.segment_bytes < 1 || a.unit_tokens < 1) return ANVILQ_EINVAL;
@@ -607,7 +611,7 @@ int anvilq_pages_reserve(uint32_t* page_table, int32_t* refs, const int32_t* bef
     for (const Span* b = &a + 1; b != std::end(spans); ++b)
       if (!(a.start == before && b->start == after) && overlap(a.start, a.bytes, b->start, b->bytes))
         return ANVILQ_EINVAL;
-  if (const int rc = check_pools(pools, pool_count, num_pages, page_tokens,
+  if (const int rc = check_pools(pools, pool_count, num_pages, rows, page_tokens,
                                  {spans[0], spans[1], spans[2], spans[3], spans[4], spans[5]}))
     return rc;
   if (!workspace || workspace_bytes < anvilq_pages_reserve_workspace_size(rows, num_pages)) return ANVILQ_EWORKSPACE;
@@ -679,7 +683,7 @@ int anvilq_pages_compact(const uint32_t* page_table, uint32_t* out, const int32_
   for (const Span& a : spans)
     for (const Span* b = &a + 1; b != std::end(spans); ++b)
       if (overlap(a.start, a.bytes, b->start, b->bytes)) return ANVILQ_EINVAL;
-  if (const int rc = check_pools(pools, pool_count, num_pages, page_tokens,
+  if (const int rc = check_pools(pools, pool_count, num_pages, num_pages / 2 + 1, page_tokens,
                                  {spans[0], spans[1], spans[2], spans[3], spans[4], spans[5]}))
     return rc;
   if (!workspace || workspace_bytes < anvilq_pages_compact_workspace_size(num_pages)) return ANVILQ_EWORKSPACE;
@@ -714,7 +718,7 @@ int anvilq_pages_copy(const anvilq_page_pool* pools, int pool_count, const int32
   if (num_pages < 1 || page_tokens < 1) return ANVILQ_ESHAPE;
   if (!aligned(src, 4) || !aligned(dst, 4) || !aligned(rows, 4) || !aligned(count, 4)) return ANVILQ_EALIGN;
   const size_t list = (size_t)most * 4;
-  if (const int rc = check_pools(pools, pool_count, num_pages, page_tokens,
+  if (const int rc = check_pools(pools, pool_count, num_pages, most, page_tokens,
                                  {{src, list}, {dst, list}, {rows, rows ? list : 0}, {count, count ? 4u : 0u}}))
     return rc;
   if (most == 0) return ANVILQ_OK;

@@ -864,8 +864,10 @@ int anvilq_beam_reorder(const anvilq_beam_state* states, int count, const int32_
  * many entries of all tables over the pool name a page, 0 for a free one.  All of it
  * lies on the device and the calls read nothing back; each can be captured.  An entry
  * that names a page >= num_pages sets ANVILQ_DEV_ERR_PAGE and is passed over (by the
- * fork dropped), as is a page whose count is less than its entries.  Tables hold at most
- * 16384 rows and 2^30 entries; arrays are apart from each other, workspace included,
+ * fork dropped), as is a page that reserve and release find named more often than its
+ * count says.  Tables hold at most
+ * 16384 rows and 2^30 entries, the pages that a call may copy times 128 pools (or
+ * fewer) stay below 2^31; arrays are apart from each other, workspace included,
  * unless said otherwise.  flags: ANVILQ_GEMM_OVERLAP_PRIOR.  No counterpart in the
  * reference, whose page table (anvil-q4/design/SPEC.md:205-208) has one owner.
  *

@@ -177,6 +177,30 @@ def test_copy_lists(dev):
     ops.raise_device_errors(dev)
 
 
+def test_copies_of_more_rows_than_a_page_has(dev):
+    """They are the whole page, also where their bytes pass 32 bits (2^24 tokens of 256 bytes)."""
+    t = torch.arange(12 * 16 * 2 * 64, device=dev).reshape(12, 16, 2, 64).half()
+    want = t.clone()
+    src, dst, rows = [0, 1, 2, 3, 4], [6, 7, 8, 9, 10], [16, 17, 1 << 24, (1 << 24) + 3, (1 << 31) - 1]
+    want[6:11] = want[:5]
+    ops.pages_copy([t], ints(src, dev), ints(dst, dev), 16, rows=ints(rows, dev))
+    assert torch.equal(t, want)
+    ops.raise_device_errors(dev)
+
+
+def test_reserve_passes_over_pages_that_more_entries_name_than_counted(dev):
+    """Page 1 is named three times and counted twice: its entries and its count stay, the rest is done."""
+    table = to(po.words([[0, 1], [2, 1], [3, 1]], 3), dev)
+    refs = ints([1, 2, 1, 1, 0, 0, 0], dev)
+    pool = torch.randn(7, 16, 1, 64, device=dev).half()
+    want = pool.clone()
+    lacking = ops.pages_reserve(table, refs, ints([20, 20, 20], dev), ints([40, 21, 21], dev), 16, [pool])
+    assert po.rows(table.cpu().numpy()) == [[0, 1, 4], [2, 1, None], [3, 1, None]]
+    assert refs.tolist() == [1, 2, 1, 1, 1, 0, 0] and int(lacking) == 0 and torch.equal(pool, want)
+    with pytest.raises(AnvilqError):
+        ops.raise_device_errors(dev)
+
+
 def test_unaligned_pools(dev):
     """Pools that start on a 4-byte border only, and heads whose runs are odd multiples of 4 bytes."""
     rng = np.random.default_rng(9)

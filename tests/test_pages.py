@@ -108,3 +108,7 @@ def test_too_few_pages_has_a_text(monkeypatch):
     monkeypatch.setattr(ops, "device_error_word", lambda device: word)
     with pytest.raises(AnvilqError, match="free pages"):
         ops.raise_device_errors("cpu")
+
+
+def test_more_copies_than_a_launch_numbers():
+    assert _lib.load().anvilq_pages_copy(*{**COPY, "n": 128, "most": 1 << 25}.values()) == ESHAPE
