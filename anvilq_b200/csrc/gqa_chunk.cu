@@ -162,15 +162,15 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
 __device__ __forceinline__ void mma_ss(uint32_t d, u64 a, u64 b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0)
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, u64 b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0)
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 #define ANVILQ_R32(r)                                                                                              \
@@ -617,8 +617,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else {
       // ------------------------------------------------------------------ MMA
-      // A thread a tile issues its products: S = Q K^T when a K tile is there, O += P V when
-      // its P and the V tile are.  A tile's last products and its next scores go together,
+      // A warp a tile issues its products, one thread of it (`leader`) the instructions: S = Q K^T
+      // when a K tile is there, O += P V when its P and the V tile are.  The whole warp walks and
+      // waits, so that descriptors are uniform values; with one thread alone each came from
+      // its registers (4096 tokens after 12288, 32/8 heads: 950 us, so 907).  A tile's last products and its next scores go together,
       // one tile at a time (`turn`): so the tiles' softmax run in turns, each beside the
       // other's products.  Left alone, both ran at once and both waited at once.
       const int t = warp - kMmaWarp;
@@ -638,11 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0;                           // the ring's next tile: K, V, K, V ...
       uint32_t phase = 0, steps = 0, uses = 0;
       bool ok = true;
-      auto wait1 = [&](uint32_t bar, uint32_t parity) {   // by the one thread
-        if (mbar_wait(bar, parity, &sh.abort)) return true;
-        fail();
-        return false;
-      };
+      const bool leader = elect_one();
       auto next_stage = [&]() {
         if (++stage == C::kStages) {
           stage = 0;
@@ -650,76 +648,83 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       auto take_turn = [&]() {
-        if (atomicCAS(&sh.turn, 0, 1) == 0) return true;
-        const u64 t0 = globaltimer();
-        while (atomicCAS(&sh.turn, 0, 1) != 0)
-          if (sh.abort || globaltimer() - t0 > kWaitLimitNs) {
-            fail();
-            return false;
-          }
-        return true;
+        bool mine = !leader || atomicCAS(&sh.turn, 0, 1) == 0;
+        if (!mine) {
+          const u64 t0 = globaltimer();
+          do {
+            mine = atomicCAS(&sh.turn, 0, 1) == 0;
+          } while (!mine && !sh.abort && globaltimer() - t0 <= kWaitLimitNs);
+          if (!mine) fail();
+        }
+        return __all_sync(0xffffffffu, mine) != 0;
       };
       auto scores = [&](int ks) {              // S_t = Q_t K^T
         tc_fence_after();
         const uint32_t k = k_low + ks * kTile;
+        if (leader) {
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          mma_ss(s_at, desc(q_low + (i / 4 * kHalf + i % 4 * 2)), desc(k + (i / 4 * kHalf + i % 4 * 2)), idesc_s, i > 0);
-        tc_commit(s_full(t));
+          for (int i = 0; i < D / 16; ++i)
+            mma_ss(s_at, desc(q_low + (i / 4 * kHalf + i % 4 * 2)), desc(k + (i / 4 * kHalf + i % 4 * 2)), idesc_s, i > 0);
+          tc_commit(s_full(t));
+        }
       };
       // the tile's steps [j0, end) of a segment, none of them: passed over
       auto run = [&](int j0, int end, int j1) {
         if (end > j0) {
-          if (!wait1(kv_full(stage), phase) || !wait1(q_full(t), uses & 1)) return false;
-          if (steps && !wait1(pv_done(t), (steps - 1) & 1)) return false;
+          if (!wait(kv_full(stage), phase) || !wait(q_full(t), uses & 1)) return false;
+          if (steps && !wait(pv_done(t), (steps - 1) & 1)) return false;
           scores(stage);
-          if (j0 + 1 == end) tc_commit(q_empty(t));
-          tc_commit(kv_empty(stage));
+          if (leader) {
+            if (j0 + 1 == end) tc_commit(q_empty(t));
+            tc_commit(kv_empty(stage));
+          }
           next_stage();
           for (int j = j0; j < end; ++j, ++steps) {
             const int vs = stage;
             const bool more = j + 1 < end;
-            if (!wait1(kv_full(vs), phase)) return false;
+            if (!wait(kv_full(vs), phase)) return false;
             next_stage();
             const uint32_t v = v_low + vs * kTile;
-            if (j == j0 && !wait1(o_empty(t), (uses & 1) ^ 1)) return false;
-            if (!wait1(p_full(t, 0), steps & 1)) return false;
+            if (j == j0 && !wait(o_empty(t), (uses & 1) ^ 1)) return false;
+            if (!wait(p_full(t, 0), steps & 1)) return false;
             tc_fence_after();
+            if (leader)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma_ts(o_at, s_at + i * 8, desc(v + i * 128), idesc_o, (j > j0 || i > 0) ? 1u : 0u);
-            if (more && !wait1(kv_full(stage), phase)) return false;
-            if (!wait1(p_full(t, 1), steps & 1) || !take_turn()) return false;
+              for (int i = 0; i < 4; ++i) mma_ts(o_at, s_at + i * 8, desc(v + i * 128), idesc_o, (j > j0 || i > 0) ? 1u : 0u);
+            if (more && !wait(kv_full(stage), phase)) return false;
+            if (!wait(p_full(t, 1), steps & 1) || !take_turn()) return false;
             tc_fence_after();
+            if (leader) {
 #pragma unroll
-            for (int i = 4; i < 8; ++i) mma_ts(o_at, s_at + i * 8, desc(v + i * 128), idesc_o, 1u);
-            tc_commit(pv_done(t));
+              for (int i = 4; i < 8; ++i) mma_ts(o_at, s_at + i * 8, desc(v + i * 128), idesc_o, 1u);
+              tc_commit(pv_done(t));
+            }
             if (more) {   // S goes where the products read P
-              if (!wait1(pv_done(t), steps & 1)) return false;
+              if (!wait(pv_done(t), steps & 1)) return false;
               scores(stage);
             }
-            atomicExch(&sh.turn, 0);
-            tc_commit(kv_empty(vs));
-            if (more) {
-              tc_commit(kv_empty(stage));
+            if (leader) {
+              atomicExch(&sh.turn, 0);
+              tc_commit(kv_empty(vs));
+              if (more) tc_commit(kv_empty(stage));
               if (j + 2 == end) tc_commit(q_empty(t));
-              next_stage();
             }
+            if (more) next_stage();
           }
           ++uses;
         }
         for (int i = 2 * (j1 - max(end, j0)); i > 0; --i) {
-          if (!wait1(kv_full(stage), phase)) return false;
-          mbar_arrive(kv_empty(stage));
+          if (!wait(kv_full(stage), phase)) return false;
+          if (leader) mbar_arrive(kv_empty(stage));
           next_stage();
         }
         return true;
       };
-      while (ok && next_segment(p, w, g)) {
-        if (lane == 0) ok = run(g.j0, g.end(p, t), g.j1);
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-      }
+      while (ok && next_segment(p, w, g))
+        ok = run(__shfl_sync(0xffffffffu, g.j0, 0), __shfl_sync(0xffffffffu, g.end(p, t), 0),
+                 __shfl_sync(0xffffffffu, g.j1, 0));
       if (sh.abort) {   // MMAs still running write TMEM
-        if (lane == 0) {
+        if (leader) {
           tc_commit(drained(t));
           mbar_drain(drained(t), 0);
         }
