@@ -18,7 +18,7 @@
 // tiles in turn keep the tensor cores at one's products while the other's softmax runs.
 //
 // Work split (stream-K).  All pairs' keys in a row, in the order (sequence, kv head,
-// pair), with 128 units more for a pair's beginning, are cut into equal stretches, one a
+// pair), with kSetup units more for a pair's beginning, are cut into equal stretches, one a
 // CTA; a key tile is the CTA's in whose stretch it begins.  So lengths do not matter to the
 // balance and few rows over a long axis are split over it.  A pair that
 // several CTAs share leaves binary32 partial sums in the workspace; a second kernel,
@@ -30,9 +30,17 @@
 //   8-11       store O, while the next pair's scores are under way
 //   12, 13     TMA of Q and K, and of V (side by side: pages of 16 tokens take 16 copies
 //              a tile); the latter zeroes V's rows behind a sequence's last token
-//   14, 15     MMA of tile 0 and tile 1 (14 owns the TMEM)
+//   14, 15     MMA of tile 0 and tile 1 (14 owns the TMEM); one thread of each issues
 // K and V tiles share a ring: [half of 64 dims][128 keys][128 bytes], 128-byte swizzle.
 // K is the K-major B operand of S, V the MN-major one of O.
+//
+// What bounds it: two tiles' step of 128 keys is 2048 cycles of the tensor cores and as
+// many of the MUFU (an exponential a score), and takes 4100, as a tile's chain does: softmax
+// 1830, its products and next scores 1400, hand-overs.  With D = 128 two S and two O fill the
+// TMEM, so there is no second S to take the chain apart.  Measured, 32/8 heads of 128: 4096
+// tokens after 12288 in 869 us (1107 TFLOP/s of the causal products; 1012 us when run on end,
+// under the power cap), 60 tokens after 60001 in 86 us with the merge (2.9 TB/s); 13 tokens
+// after 150 of 14/2 heads of 64 in 12 us: plan 3, first copies 3.5, two steps, merge.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -55,7 +63,9 @@ constexpr int kKeys = 128;                 // of a step
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kStoreWarp = 8, kKWarp = 12, kVWarp = 13, kMmaWarp = 14;
-constexpr int kSetup = 192;                // what a pair's beginning costs, in keys
+// What a pair's beginning costs, in keys: queries, first scores, outputs.  (12 sequences of which
+// six take a step, the others chunks up to 500: without it 149 us, with 128 keys 129, 192 123.)
+constexpr int kSetup = 192;
 constexpr int kLeast = 1;                  // key tiles' worth of units of a stretch, at least
 constexpr int kMaxCtas = 148;
 constexpr int kMaxBatch = 65536;
@@ -620,9 +630,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       // A warp a tile issues its products, one thread of it (`leader`) the instructions: S = Q K^T
       // when a K tile is there, O += P V when its P and the V tile are.  The whole warp walks and
       // waits, so that descriptors are uniform values; with one thread alone each came from
-      // its registers (4096 tokens after 12288, 32/8 heads: 950 us, so 907).  A tile's last products and its next scores go together,
-      // one tile at a time (`turn`): so the tiles' softmax run in turns, each beside the
-      // other's products.  Left alone, both ran at once and both waited at once.
+      // its registers (4096 tokens after 12288, 32/8 heads: 950 us, so 907).  A tile's last
+      // products and its next scores go together, one tile at a time (`turn`): so the tiles'
+      // softmax run in turns, each beside the other's products.  Left alone, both ran at once
+      // and both waited at once (955 us).
       const int t = warp - kMmaWarp;
       constexpr uint32_t idesc_s = instr_desc(kKeys, false), idesc_o = instr_desc(D, true);
       // low words of the descriptors (start, leading offset); the high one is all tiles'

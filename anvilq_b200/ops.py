@@ -933,7 +933,9 @@ def gqa_chunk_paged(q, k_pool, v_pool, page_table, seqlens, token_starts, scale:
     chunks, questions about long documents, decode steps among them.  q fp16 [T, Hq, D]
     (tokens may be strided), ``paged_kv_append``'s result; token_starts int32 [B + 1] and
     seqlens int32 [B] as for it, pools and page_table as for ``gqa_decode_paged``.  Every
-    token sees the positions up to its own.  scale (finite, at most 2^32): of the scores,
+    token sees the positions up to its own (a new token whose value is NaN or infinite may
+    spoil the tokens before it in its sequence; what lies behind a sequence's end may be
+    anything).  scale (finite, at most 2^32): of the scores,
     0 or less for 1/sqrt(D).  Returns out, fp16 [T, Hq, D] (rows of no sequence are left
     as they are).  workspace: as for ``gqa_decode_q8``.
 
