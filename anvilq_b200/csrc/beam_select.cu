@@ -163,9 +163,15 @@ __device__ __forceinline__ int largest_lane(unsigned long long v) {
   return top | rest ? __ffs(who) - 1 : -1;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// The largest, or NaN where one of them is (fmaxf would pass it over).
+__device__ __forceinline__ float max_or_nan(float a, float b) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // two binary32 values at a time
@@ -334,16 +340,16 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
     for (bool again = false;; again = true) {
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
-        float a = fmaxf(v[i * kVec], v[i * kVec + 1]);
+        float a = max_or_nan(v[i * kVec], v[i * kVec + 1]);
 #pragma unroll
-        for (int e = 2; e < kVec; e += 2) a = max3(a, v[i * kVec + e], v[i * kVec + e + 1]);
+        for (int e = 2; e < kVec; e += 2) a = max_or_nan(a, v[i * kVec + e], v[i * kVec + e + 1]);
         tops[i] = a;
       }
       top = tops[0];
 #pragma unroll
-      for (int i = 1; i < kUnits; ++i) top = fmaxf(top, tops[i]);
+      for (int i = 1; i < kUnits; ++i) top = max_or_nan(top, tops[i]);
       // the tile's sum relative to the largest so far
-      const float now = fmaxf(c, top);
+      const float now = fmaxf(c, top);   // c where top is NaN: the tile is then taken again
       float part = 0.0f;
       if (now != -INFINITY) {
         if (now > c) {
@@ -366,7 +372,7 @@ __device__ void span_pass(const Params& p, List& s, int row, int split) {
         sum += part;
         break;
       }
-      // +inf or NaN among them: they count as -inf, and are reported
+      // +inf (the sum is then no number) or NaN among them: they count as -inf, and are reported
       odd = true;
       c = c_was;
       sum = sum_was;
