@@ -71,6 +71,10 @@ constexpr int kMaxCtas = 148;
 constexpr int kMaxBatch = 65536;
 constexpr float kNone = -1e30f;            // a reference below every exponent
 constexpr float kSlack = 8.0f;             // how far (log2) the reference may lag behind the largest
+// An exponent is a product less the reference, rounded once, so of a row's largest it is half a step of
+// the reference off: up to here at most 8, which binary16 takes.  From here on different scores are 16
+// or more apart, so that only the largest count, and a power of two as the scale gives their exponents exactly.
+constexpr float kLarge = 0x1p28f;
 constexpr u64 kWaitLimitNs = 1000000000ull;
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;   // S of tile t at 128 t, O at 256 + 128 t
 
@@ -96,7 +100,7 @@ struct Params {
   float* partials;              // [CTAs][2][256 (D + 2)]
   struct Open* open;            // [CTAs]
   int* dev_err;
-  float scale_log2;
+  float scale_log2, scale_large;   // the latter a power of two, 16 to 32 times the former
   int T, B, Hq, Hkv, group, tpt, page_tokens, max_pages, num_pages, box;
   int sectors;                  // out lies on 32 bytes, and with it every 16 dims of a row
 };
@@ -819,7 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int end = g.end(p, t), j0 = g.j0;
       // the last position that the row sees (of a row that is none, some)
       const int pos = g.s.before + min((2 * g.i + t) * p.tpt + row / p.group, g.s.n - 1);
-      float m = kNone, sum = 0.0f;
+      float m = kNone, sum = 0.0f, scale = p.scale_log2;
       for (int j = j0; j < end; ++j, ++steps) {
         ok = wait(s_full(t), steps & 1);
         if (!ok) break;
@@ -836,10 +840,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
         for (int c = 4; c + 1 < kKeys; c += 2) tops[c / 2 % 4] = max3(tops[c / 2 % 4], s[c], s[c + 1]);
-        const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * p.scale_log2;
-        const bool moves = top > m + kSlack;
+        const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]), bound = top * scale;
+        const bool moves = bound > __fadd_rd(m, kSlack);
         if (__any_sync(0xffffffffu, moves)) {
-          const float now = moves ? top : m, f = fast_exp2(m - now);
+          const float other = fabsf(top * p.scale_log2) < kLarge ? p.scale_log2 : p.scale_large;
+          scale = moves ? other : scale;
+          const float now = moves ? top * scale : m;
+          const float f = fast_exp2(m - now);
           m = now;
           sum *= f;
           if (j > j0) {
@@ -857,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const u64 scale2 = pair(p.scale_log2, p.scale_log2), ref2 = pair(-m, -m);
+        const u64 scale2 = pair(scale, scale), ref2 = pair(-m, -m);
         u64 part[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < kKeys; c += 64) {
@@ -882,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (g.j0 > 0 || g.j1 < g.nk) {   // for the merge
         float* slot = p.partials + ((size_t)blockIdx.x * 2 + (first_seg && g.j0 > 0 ? 0 : 1)) * (2 * kRows * (D + 2));
-        __stcg(reinterpret_cast<float2*>(slot + 2 * kRows * D) + t * kRows + row, make_float2(m, sum));
+        __stcg(reinterpret_cast<float2*>(slot + 2 * kRows * D) + t * kRows + row, make_float2(scale == p.scale_log2 ? m : m / scale * p.scale_log2, sum));
       }
       first_seg = false;
       if (end > j0) {
@@ -1169,6 +1176,7 @@ int anvilq_gqa_chunk_paged(const uint16_t* q, long long q_stride, const uint16_t
   p.open = reinterpret_cast<Open*>(at + partial_bytes(ctas, D));
   p.dev_err = dev_err;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
+  p.scale_large = std::ldexp(1.0f, std::ilogb(p.scale_log2) + 5);
   p.T = T; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
   p.group = Hq / Hkv;
   p.tpt = kRows / p.group;

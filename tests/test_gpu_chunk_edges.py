@@ -1,11 +1,14 @@
-"""Chunk attention at the edges of what it accepts: outputs on any 16 bytes.
+"""Chunk attention at the edges of what it accepts: outputs on any 16 bytes, scores of any size.
 
 Tolerances and cases' makers: ``test_gpu_chunk``."""
+import numpy as np
 import pytest
 import torch
 
+import serving_oracle as so
 from anvilq_b200 import ops
 from test_gpu_chunk import Case, dev  # noqa: F401
+from test_gpu_serving import to
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +28,42 @@ def test_outputs_on_any_16_bytes(dev, first, D):
     ops.raise_device_errors(dev)
     assert torch.equal(out, want)
     assert (room[:first] == 5.0).all() and (room[first + want.numel():] == 5.0).all()
+
+
+def set_keys(c, b, k):
+    """Other keys of sequence b, [positions, heads, D], in the pages too."""
+    page = c.args[1].shape[1]
+    c.k[b] = k.astype(np.float16)
+    for j in range(-(-len(k) // page)):
+        part = to(c.k[b][j * page:(j + 1) * page], c.dev)
+        c.args[1][so.physical(c.np_table[b, j]), :len(part)] = part
+
+
+@pytest.mark.parametrize("sign", [1, -1, 0])
+@pytest.mark.parametrize("scale", [2.0 ** 12, 2.0 ** 19, 2.0 ** 22, 2.0 ** 25, 2.0 ** 32])
+def test_scores_of_any_size(dev, scale, sign):
+    """Scores are whole numbers times a large scale, all above 0, all below, or of both signs: the keys of a
+    row's largest share it, the others' weights, exp(-4096) or less, are nothing.  Equal keys have equal
+    probabilities, so the tolerance is their rounding, 2^-11 of sum p |v|, the output's, and 2^-20 for
+    the products' and the sums' few additions."""
+    c = Case(dev, 50, [300, 0, 40], [150, 77, 1], 8, 2, 64, 16, scale=scale, spare=0)
+    rng = np.random.default_rng(51)
+    whole = lambda *shape: rng.integers(1 if sign else -3, 4, size=shape)
+    c.q[:] = whole(*c.q.shape)
+    c.args[0][:] = to(c.q, dev)
+    for b in range(3):
+        set_keys(c, b, whole(*c.k[b].shape) * (sign or 1))
+    got = c.run().cpu().numpy().astype(np.float64)
+    ops.raise_device_errors(dev)
+    for b, n in enumerate(c.new):
+        q = c.q[c.starts_list[b]:c.starts_list[b + 1]].astype(np.float64)
+        hidden = np.arange(len(c.k[b]))[None] > c.before[b] + np.arange(n)[:, None]
+        for i in range(8):
+            k, v = c.k[b][:, i // 4].astype(np.float64), c.v[b][:, i // 4].astype(np.float64)
+            x = q[:, i] @ k.T
+            x[hidden] = -np.inf
+            p = (x == x.max(axis=1, keepdims=True)).astype(np.float64)
+            p /= p.sum(axis=1, keepdims=True)
+            want = p @ v
+            tol = 2.0 ** -11 * np.abs(want) + (2.0 ** -11 + 2.0 ** -20) * (p @ np.abs(v)) + 2.0 ** -25
+            assert (np.abs(got[c.starts_list[b]:c.starts_list[b + 1], i] - want) <= tol).all(), (b, i)
