@@ -6,10 +6,11 @@
 // start_b) (its n_b new tokens are its last, in the cache already); query head h reads
 // kv head h / g, g = Hq / Hkv, and
 //   out = sum_{s <= pos} p_s v_s / sum p_s,   p_s = exp2(scale log2(e) q.k_s - m)
-// with a running reference m of each row that is at least the row's largest exponent
-// minus 8: p stays below 2^8, so m seldom moves and the sums are rescaled only then.
-// Scores, sums and outputs are binary32; p enters the tensor cores as binary16 (half a
-// step, 2^-11 of each), which they need as the operand beside binary16 values.
+// with a running reference m of each row, 7 below the row's largest exponent when it is
+// set, moved where p would pass 2^15: so it seldom moves and the sums are rescaled only then.
+// Scores, sums and outputs are binary32; p enters the tensor cores as binary16, which they
+// need as the operand beside binary16 values: half a step, 2^-11 of p, and below 2^-14
+// 2^-25, which is 2^-32 of the row's largest or less.
 //
 // Tiles.  A pair of 128-row tiles holds 2 tpt tokens of one kv head's g query heads,
 // tpt = 128 / g (row r: token r / g, head r % g; rows behind tpt g are padding), and
@@ -70,9 +71,11 @@ constexpr int kLeast = 1;                  // key tiles' worth of units of a str
 constexpr int kMaxCtas = 148;
 constexpr int kMaxBatch = 65536;
 constexpr float kNone = -1e30f;            // a reference below every exponent
-constexpr float kSlack = 8.0f;             // how far (log2) the reference may lag behind the largest
+// How far (log2) the reference is below a row's largest when it is set, and may lag behind it later: the
+// largest p is from 2^7 to 2^15, so that binary16 has normal numbers down to 2^-21 of it or less.
+constexpr float kBelow = 7.0f, kSlack = 15.0f;
 // An exponent is a product less the reference, rounded once, so of a row's largest it is half a step of
-// the reference off: up to here at most 8, which binary16 takes.  From here on different scores are 16
+// the reference off: up to here it stays below 2^15.5, which binary16 takes.  From here on different scores are 16
 // or more apart, so that only the largest count, and a power of two as the scale gives their exponents exactly.
 constexpr float kLarge = 0x1p28f;
 constexpr u64 kWaitLimitNs = 1000000000ull;
@@ -845,7 +848,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (__any_sync(0xffffffffu, moves)) {
           const float other = fabsf(top * p.scale_log2) < kLarge ? p.scale_log2 : p.scale_large;
           scale = moves ? other : scale;
-          const float now = moves ? top * scale : m;
+          const float now = moves ? top * scale - kBelow : m;
           const float f = fast_exp2(m - now);
           m = now;
           sum *= f;

@@ -1,4 +1,5 @@
-"""Chunk attention at the edges of what it accepts: outputs on any 16 bytes, scores of any size.
+"""Chunk attention at the edges of what it accepts: outputs on any 16 bytes, scores of any size, weights
+far below a row's largest.
 
 Tolerances and cases' makers: ``test_gpu_chunk``."""
 import numpy as np
@@ -67,3 +68,39 @@ def test_scores_of_any_size(dev, scale, sign):
             want = p @ v
             tol = 2.0 ** -11 * np.abs(want) + (2.0 ** -11 + 2.0 ** -20) * (p @ np.abs(v)) + 2.0 ** -25
             assert (np.abs(got[c.starts_list[b]:c.starts_list[b + 1], i] - want) <= tol).all(), (b, i)
+
+
+@pytest.mark.parametrize("below", [12, 20, 26, 28])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_keys_far_below_the_largest(dev, below, D):
+    """One key takes most of a row, 2^17 others lie some `below` powers of two under it and have a share
+    all the same.  Binary16 takes a probability to 2^-11 of it, or 2^-32 of the row's largest; a CTA has all
+    keys of a pair of tokens, n / 16 accumulation steps of 2^-22; scores as in ``test_gpu_chunk``."""
+    n, T, heads, page, kinds = 1 << 17, 296, 128, 256, 8
+    rng = np.random.default_rng(below + D)
+    q, k = rng.standard_normal((T, heads, D)) / 8, rng.standard_normal((1 + kinds, page, 1, D)) / 8
+    v = 1 + rng.standard_normal(k.shape) / 4
+    q[..., 0], k[..., 0] = 8, 0
+    k[0], v[0] = k[1], v[1]
+    k[0, 0, 0, 0], v[0, 0] = below / (8 * np.log2(np.e)) * np.sqrt(D), rng.standard_normal((1, D)) / 64
+    q, k, v = (x.astype(np.float16) for x in (q, k, v))
+    # page 0 first, the others in turn
+    names = np.concatenate([[0], 1 + np.arange(n // page - 1) % kinds])
+    table = (names.astype(np.uint32) | np.uint32(so.VALID)).view(np.int32)[None]
+    out = ops.gqa_chunk_paged(*(to(a, dev) for a in (q, k, v, table, np.array([n], np.int32), np.array([0, T], np.int32))))
+    ops.raise_device_errors(dev)
+    got = out.cpu().numpy().astype(np.float64)
+    keys, values = k.reshape(-1, D).astype(np.float64), v.reshape(-1, D).astype(np.float64)
+    for t in (0, 1, 150, 295):
+        seen = n - T + t + 1
+        count = np.bincount(names[np.arange(seen) // page] * page + np.arange(seen) % page, minlength=len(keys))
+        for h in (0, 77):
+            x = keys @ q[t, h].astype(np.float64) / np.sqrt(D)
+            p = np.exp(x - x.max())
+            total = (p * count).sum()
+            want, mass = p * count @ values / total, p * count @ np.abs(values) / total
+            reach = np.abs(q[t, h].astype(np.float64)).sum() * np.abs(keys).max() / np.sqrt(D)
+            tol = 2.0 ** -11 * np.abs(want) + mass * (2.0 ** -11 + 2.0 ** -18 * reach + n / 16 * 2.0 ** -22) + \
+                2.0 ** -32 * (count @ np.abs(values)) / total + 2.0 ** -25
+            off = np.abs(got[t, h] - want)
+            assert (off <= tol).all(), (t, h, float(off.max()), float(tol.max()), float(want.mean()))
