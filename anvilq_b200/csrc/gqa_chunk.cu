@@ -24,6 +24,7 @@
 // balance and few rows over a long axis are split over it.  A pair that
 // several CTAs share leaves binary32 partial sums in the workspace; a second kernel,
 // launched with the first's end overlapped, merges them in CTA order (bit-reproducible).
+// A share of more than 128 key tiles is taken in segments, added up there by the CTA itself.
 // Every CTA finds its stretch from the lengths on the device, by sums in closed form.
 //
 // Warp roles (16 warps, one CTA an SM):
@@ -69,6 +70,11 @@ constexpr int kStoreWarp = 8, kKWarp = 12, kVWarp = 13, kMmaWarp = 14;
 constexpr int kSetup = 192;
 constexpr int kLeast = 1;                  // key tiles' worth of units of a stretch, at least
 constexpr int kMaxCtas = 148;
+// Key tiles of a segment, at most.  The tensor cores add to binary32 by cutting off, up to 2^-23 of the sum at
+// each 16 keys and always downwards: over 2^20 keys of equal weights 6.7e-3.  So after a segment the
+// products begin anew, and its outputs are added to those before by rounded operations: 1e-4 at any length.
+// (4096 tokens at the end of 65536 positions, 32/8 heads: with heads of 64 3.3 ms as without, of 128 4.0 and 3.8.)
+constexpr int kPiece = 128;
 constexpr int kMaxBatch = 65536;
 constexpr float kNone = -1e30f;            // a reference below every exponent
 // How far (log2) the reference is below a row's largest when it is set, and may lag behind it later: the
@@ -100,7 +106,10 @@ struct Params {
   const int* seqlens;           // [B]
   const uint32_t* page_table;   // [B][max_pages]
   __half* out;                  // [T][Hq][D]
-  float* partials;              // [CTAs][2][256 (D + 2)]
+  // [CTAs][2][256 (D + 2)]: sums of a share that is not all of a pair, or not one segment; a share that an
+  // earlier CTA's goes before is the stretch's first, and has the first place
+  float* partials;
+  float2* fresh;                // [CTAs][256]: references and sums of a segment that others of its share came before
   struct Open* open;            // [CTAs]
   int* dev_err;
   float scale_log2, scale_large;   // the latter a power of two, 16 to 32 times the former
@@ -314,13 +323,17 @@ __device__ __forceinline__ int tiles_below(int x) { return max(0, x - kSetup + k
 struct Walk {
   Seq s;
   int b, h, i, x;   // pair i of head h of sequence b, x units into it
+  int part;         // kOn, kMid of the segment that comes next
   u64 left;
 };
-// A stretch's share of a pair: key tiles [j0, j1) of nk.
+// What a segment is of a pair: kOn, not the first of its stretch's share of it; kMid, that share is not
+// the pair's first; kShared, another CTA has a share too; kOne, it is all of the pair.
+enum { kOn = 1, kMid = 2, kShared = 4, kOne = 8 };
+// Key tiles [j0, j1) of a pair, at most kPiece.
 struct Segment {
   Seq s;
-  int b, h, i, j0, j1, nk;
-  // tile t's part of them ends here
+  int b, h, i, j0, j1, part;
+  // tile t's part of them ends here, at j0 or before where it has none
   __device__ __forceinline__ int end(const Params& p, int t) const {
     const int first = (2 * i + t) * p.tpt;
     return first < s.n ? min(j1, tiles_to(s, first + p.tpt)) : j0;
@@ -336,13 +349,19 @@ __device__ __forceinline__ bool next_segment(const Params& p, Walk& walk, Segmen
   while (w.left && g.j1 <= g.j0) {
     g.s = w.s;
     g.b = w.b; g.h = w.h; g.i = w.i;
-    g.nk = tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
-    const int end = (int)min((u64)(kSetup + w.s.before + min((w.i + 1) * 2 * p.tpt, w.s.n)), w.x + w.left);
-    g.j0 = min(g.nk, tiles_below(w.x));
-    g.j1 = tiles_below(end);
+    const int nk = tiles_to(w.s, (w.i + 1) * 2 * p.tpt);
+    int end = (int)min((u64)(kSetup + w.s.before + min((w.i + 1) * 2 * p.tpt, w.s.n)), w.x + w.left);
+    const int to = tiles_below(end);
+    g.j0 = min(nk, tiles_below(w.x));
+    g.j1 = min(g.j0 + kPiece, to);
+    if (!w.part && g.j0 > 0) w.part = kMid;
+    g.part = w.part | (w.part & kMid || to < nk ? kShared : 0) | (g.j0 == 0 && g.j1 == nk ? kOne : 0);
+    const bool on = g.j1 < to;   // the next segment begins there
+    if (on) end = kSetup + g.j1 * kKeys;
     w.left -= end - w.x;
-    w.x = 0;
-    if (w.left == 0 || ++w.i < pairs_of(p, w.s)) continue;
+    w.x = on ? end : 0;
+    w.part = on ? w.part | kOn : 0;
+    if (w.left == 0 || on || ++w.i < pairs_of(p, w.s)) continue;
     w.i = 0;
     if (++w.h < p.Hkv) continue;
     w.h = 0;
@@ -555,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // `uses` of a tile: the segments that it has a part in
 
   if (warp >= kKWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == kKWarp || warp == kVWarp) {
       // ------------------------------------------------------------------ Q, K and V
       const bool is_v = warp == kVWarp;
@@ -751,40 +770,96 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp >= kStoreWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     {
       // ------------------------------------------------------------------ stores
       const int row = warp % 4 * 32 + lane, of_token = row / p.group, of_head = row % p.group;
-      unsigned steps[2] = {0, 0}, uses[2] = {0, 0};
-      bool ok = true, first_seg = true;
+      auto leave = [&](int t) {   // tile t's outputs are out of TMEM
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_empty(t));
+      };
+      unsigned phases = 0;   // of the next sums (bit t) and of the products (bit 2 + t) of tile t
+      bool ok = true;
       while (ok && next_segment(p, w, g)) {
-        const bool whole = g.j0 == 0 && g.j1 == g.nk;
+        // sums of a share that others merge, or that goes on in another segment
         float4* slot = reinterpret_cast<float4*>(
-            p.partials + ((size_t)blockIdx.x * 2 + (first_seg && g.j0 > 0 ? 0 : 1)) * (2 * kRows * (D + 2)));
-        first_seg = false;
-#pragma unroll
+            p.partials + ((size_t)blockIdx.x * 2 + (g.part & kMid ? 0 : 1)) * (2 * kRows * (D + 2)));
+#pragma unroll 1
         for (int t = 0; t < 2; ++t) {
           const int end = g.end(p, t), first = (2 * g.i + t) * p.tpt;
-          if (!ok || end <= g.j0) continue;
+          if (!ok) continue;
+          float2* state = reinterpret_cast<float2*>(slot + 2 * kRows * (D / 4)) + t * kRows + row;
+          if (end <= g.j0) {
+            if ((g.part & (kShared | kOn)) == kShared) __stcg(state, make_float2(kNone, 0.0f));   // the merge reads both tiles'
+            continue;
+          }
           const bool mine = of_token < p.tpt && first + of_token < g.s.n;
-          steps[t] += end - g.j0;
-          ok = wait(sums_full(t), uses[t]++ & 1) && wait(pv_done(t), (steps[t] - 1) & 1);
+          phases ^= (unsigned)(end - g.j0 & 1) << (2 + t);
+          ok = wait(sums_full(t), phases >> t & 1) && wait(pv_done(t), ~phases >> (2 + t) & 1);
+          phases ^= 1u << t;
           if (!ok) break;
           tc_fence_after();
-          const float sum = sh.sums[t][row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // (only scores of -inf: zeros)
+          const bool last = !(g.part & kShared) && tiles_to(g.s, first + p.tpt) <= g.j1;   // the outputs are whole
+          const uint32_t o_at = tmem + kTmemO + t * 128 + ((uint32_t)(warp % 4 * 32) << 16);
+          float4* at = slot + t * kRows + row;   // [dims / 4][row]
           __half* out = p.out + ((long long)(g.s.start + first + of_token) * p.Hq + g.h * p.group + of_head) * D;
+          if (g.part & kOn) {   // added to the segments before
+            float f_then = 0.0f, f = 0.0f;
+            if (mine) {
+              const float2 then = __ldcg(state), now = __ldcg(p.fresh + blockIdx.x * (2 * kRows) + t * kRows + row);
+              const float top = fmaxf(then.x, now.x);
+              f_then = fast_exp2(then.x - top);
+              f = fast_exp2(now.x - top);
+              const float sum = then.y * f_then + now.y * f, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+              if (last) {
+                f_then *= inv;
+                f *= inv;
+              } else {
+                __stcg(state, make_float2(top, sum));
+              }
+            }
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_at + c, o);
+              wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16 && mine; e += 8) {
+                float4 v[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const uint32_t* n = o + e + 4 * k;
+                  v[k] = __ldcg(at + ((c + e) / 4 + k) * (2 * kRows));
+                  v[k].x = v[k].x * f_then + __uint_as_float(n[0]) * f;
+                  v[k].y = v[k].y * f_then + __uint_as_float(n[1]) * f;
+                  v[k].z = v[k].z * f_then + __uint_as_float(n[2]) * f;
+                  v[k].w = v[k].w * f_then + __uint_as_float(n[3]) * f;
+                  if (!last) __stcg(at + ((c + e) / 4 + k) * (2 * kRows), v[k]);
+                }
+                if (last) {
+                  uint4 w;
+                  __half2* h = reinterpret_cast<__half2*>(&w);
+                  h[0] = __floats2half2_rn(v[0].x, v[0].y);
+                  h[1] = __floats2half2_rn(v[0].z, v[0].w);
+                  h[2] = __floats2half2_rn(v[1].x, v[1].y);
+                  h[3] = __floats2half2_rn(v[1].z, v[1].w);
+                  *reinterpret_cast<uint4*>(out + c + e) = w;
+                }
+              }
+            }
+            leave(t);
+            continue;
+          }
+          const float sum = sh.sums[t][row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // (only scores of -inf: zeros)
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
-            tmem_ld32(tmem + kTmemO + t * 128 + ((uint32_t)(warp % 4 * 32) << 16) + c, o);
+            tmem_ld32(o_at + c, o);
             wait_ld();
-            if (c + 32 == D) {   // the tile's sums are out of TMEM
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(o_empty(t));
-            }
+            if (c + 32 == D) leave(t);
             if (!mine) continue;
-            if (whole) {
+            if (last) {
 #pragma unroll
               for (int e = 0; e < 32; e += 16) {   // a sector at a time
                 uint32_t v[8];
@@ -803,12 +878,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                   *reinterpret_cast<uint4*>(out + c + e + 8) = make_uint4(v[4], v[5], v[6], v[7]);
                 }
               }
-            } else {   // [dims / 4][row]
+            } else {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
-                __stcg(slot + (c + e) / 4 * (2 * kRows) + t * kRows + row,
-                       make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
-                                   __uint_as_float(o[e + 3])));
+                __stcg(at + (c + e) / 4 * (2 * kRows), make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]),
+                                                                   __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])));
             }
           }
         }
@@ -820,15 +894,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = warp / 4, row = threadIdx.x % kRows;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t s_at = tmem + t * kKeys + lanes, o_at = tmem + kTmemO + t * 128 + lanes;
-    unsigned steps = 0, uses = 0;
-    bool ok = true, first_seg = true;
+    unsigned phases = 0;   // of the next scores and (bit 1) of the outputs' place
+    bool ok = true;
     while (ok && next_segment(p, w, g)) {
       const int end = g.end(p, t), j0 = g.j0;
       // the last position that the row sees (of a row that is none, some)
       const int pos = g.s.before + min((2 * g.i + t) * p.tpt + row / p.group, g.s.n - 1);
       float m = kNone, sum = 0.0f, scale = p.scale_log2;
-      for (int j = j0; j < end; ++j, ++steps) {
-        ok = wait(s_full(t), steps & 1);
+      for (int j = j0; j < end; ++j, phases ^= 1) {
+        ok = wait(s_full(t), phases & 1);
         if (!ok) break;
         tc_fence_after();
         float s[kKeys];
@@ -853,7 +927,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = now;
           sum *= f;
           if (j > j0) {
-            ok = wait(pv_done(t), (steps - 1) & 1);
+            ok = wait(pv_done(t), ~phases & 1);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -890,14 +964,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         sum += both.x + both.y;
       }
       if (!ok) break;
-      if (g.j0 > 0 || g.j1 < g.nk) {   // for the merge
-        float* slot = p.partials + ((size_t)blockIdx.x * 2 + (first_seg && g.j0 > 0 ? 0 : 1)) * (2 * kRows * (D + 2));
-        __stcg(reinterpret_cast<float2*>(slot + 2 * kRows * D) + t * kRows + row, make_float2(scale == p.scale_log2 ? m : m / scale * p.scale_log2, sum));
-      }
-      first_seg = false;
       if (end > j0) {
-        ok = wait(o_empty(t), (uses++ & 1) ^ 1);   // the sums of the segment before are read
+        ok = wait(o_empty(t), ~phases >> 1 & 1);   // the sums of the segment before are read
+        phases ^= 2;
         sh.sums[t][row] = sum;
+        if (!(g.part & kOne)) {   // for the merge, or the stores
+          float* slot = p.partials + ((size_t)blockIdx.x * 2 + (g.part & kMid ? 0 : 1)) * (2 * kRows * (D + 2));
+          float2* to = g.part & kOn ? p.fresh + blockIdx.x * (2 * kRows) : reinterpret_cast<float2*>(slot + 2 * kRows * D);
+          __stcg(to + t * kRows + row, make_float2(scale == p.scale_log2 ? m : m / scale * p.scale_log2, sum));
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(sums_full(t));
       }
@@ -1133,7 +1208,7 @@ size_t anvilq_gqa_chunk_paged_workspace_size(int T, int B, int Hq, int Hkv, int 
   const int sms = sm_count();
   if (sms <= 0) return 0;
   const int ctas = ctas_for(sms, T, B, Hq, Hkv, (long long)page_tokens * max_pages);
-  return ANVILQ_WORKSPACE_COUNTER_BYTES + partial_bytes(ctas, D) + ctas * sizeof(Open);
+  return ANVILQ_WORKSPACE_COUNTER_BYTES + partial_bytes(ctas, D) + ctas * (2 * kRows * sizeof(float2) + sizeof(Open));
 }
 
 int anvilq_gqa_chunk_paged(const uint16_t* q, long long q_stride, const uint16_t* k_pool, const uint16_t* v_pool,
@@ -1176,7 +1251,8 @@ int anvilq_gqa_chunk_paged(const uint16_t* q, long long q_stride, const uint16_t
   p.out = reinterpret_cast<__half*>(out);
   char* at = static_cast<char*>(workspace) + ANVILQ_WORKSPACE_COUNTER_BYTES;
   p.partials = reinterpret_cast<float*>(at);
-  p.open = reinterpret_cast<Open*>(at + partial_bytes(ctas, D));
+  p.fresh = reinterpret_cast<float2*>(at + partial_bytes(ctas, D));
+  p.open = reinterpret_cast<Open*>(p.fresh + (size_t)ctas * 2 * kRows);
   p.dev_err = dev_err;
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
   p.scale_large = std::ldexp(1.0f, std::ilogb(p.scale_log2) + 5);

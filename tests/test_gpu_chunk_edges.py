@@ -1,5 +1,5 @@
 """Chunk attention at the edges of what it accepts: outputs on any 16 bytes, scores of any size, weights
-far below a row's largest.
+far below a row's largest, contexts of many segments.
 
 Tolerances and cases' makers: ``test_gpu_chunk``."""
 import numpy as np
@@ -104,3 +104,80 @@ def test_many_keys_far_below_the_largest(dev, below, D):
                 2.0 ** -32 * (count @ np.abs(values)) / total + 2.0 ** -25
             off = np.abs(got[t, h] - want)
             assert (off <= tol).all(), (t, h, float(off.max()), float(tol.max()), float(want.mean()))
+
+
+def long_case(dev, seed, before, new, Hq, Hkv, D, page, kinds=None):
+    """(arguments, positions' page rows of every sequence) of a batch whose contexts are long; with `kinds`
+    their pages are that many, named in turn."""
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    need = [-(-(p + n) // page) for p, n in zip(before, new)]
+    pages = kinds or sum(need)
+    order = torch.randperm(pages, generator=g, device=dev).repeat(-(-sum(need) // pages))
+    table = torch.zeros((len(new), max(need)), dtype=torch.int64, device=dev)
+    rows, at = [], 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n] - (1 << 31)
+        rows.append((order[at:at + n, None] * page + torch.arange(page, device=dev)).reshape(-1))
+        at += n
+    half = lambda *shape: torch.randn(shape, generator=g, device=dev).half()
+    starts = np.concatenate([[0], np.cumsum(new)])
+    q, k, v = half(int(starts[-1]), Hq, D), half(pages, page, Hkv, D), half(pages, page, Hkv, D)
+    lens = torch.tensor([p + n for p, n in zip(before, new)], dtype=torch.int32, device=dev)
+    return [q, k, v, table.to(torch.int32), lens, to(starts.astype(np.int32), dev)], rows
+
+
+def exactly(args, rows, b, t, h):
+    """(output, sum p |v|, scores' reach) of token t and head h of sequence b, in 64 bits."""
+    q, k, v, _, lens, starts = args
+    Hq, D = q.shape[1:]
+    kv = h // (Hq // k.shape[2])
+    seen = rows[b][:int(lens[b] - starts[b + 1] + starts[b]) + t + 1]
+    query = q[int(starts[b]) + t, h].double()
+    keys, values = k.flatten(0, 1)[:, kv].double(), v.flatten(0, 1)[:, kv].double()
+    x = keys @ query / D ** 0.5
+    p = torch.exp(x - x[seen].max()) * torch.bincount(seen, minlength=len(x))
+    p /= p.sum()
+    return p @ values, p @ values.abs(), query.abs().sum() * keys.abs().max() / D ** 0.5
+
+
+@pytest.mark.parametrize("before,new,Hq,Hkv,D,page", [
+    ([50000], [2600], 8, 8, 64, 64),                       # stretches inside pairs of several segments
+    ([20000, 60000, 0], [700, 260, 5], 32, 8, 128, 16),    # and across them
+    ([33000], [300], 128, 1, 64, 256),                     # whole pairs of several segments
+    ([16384 - 151], [300], 128, 1, 128, 128),              # a segment's end between a pair's tiles
+    ([16384, 16380, 16256], [1, 9, 3], 16, 16, 64, 32),    # a tile or a key more than a segment
+])
+def test_contexts_of_many_segments(dev, before, new, Hq, Hkv, D, page):
+    """As ``test_gpu_chunk``, for chosen tokens and heads; a segment's products are 1024 accumulation steps of
+    at most 2^-22 of sum p |v|."""
+    args, rows = long_case(dev, len(before) + D, before, new, Hq, Hkv, D, page)
+    out = ops.gqa_chunk_paged(*args)
+    assert torch.equal(out, ops.gqa_chunk_paged(*args)), "bit-reproducible"
+    ops.raise_device_errors(dev)
+    for b, n in enumerate(new):
+        for t in sorted({0, min(1, n - 1), n // 3, n // 2, 151 % n, max(n - 2, 0), n - 1}):
+            for h in sorted({0, Hq // 2 + 1, Hq - 1}):
+                want, mass, reach = exactly(args, rows, b, t, h)
+                tol = 2.0 ** -11 * want.abs() + mass * (2.0 ** -11 + 2.0 ** -18 * reach + 2.0 ** -12) + 2.0 ** -25
+                off = (out[int(args[5][b]) + t, h].double() - want).abs()
+                assert (off <= tol).all(), (b, t, h, float(off.max()), float(tol.min()))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_contexts_are_not_biased(dev, D):
+    """2^18 keys of nearly equal weights and values above 0, which a CTA adds up: additions that cut off,
+    at most 2^-23 of the sum in each of a segment's 1024, would all err downwards.  Of the other roundings the
+    mean over 100 rows of D values is far below 2^-14."""
+    args, rows = long_case(dev, D, [1 << 18], [296], 128, 1, D, 256, kinds=16)
+    args[0] *= 0.25
+    args[2][:] = (torch.rand(args[2].shape, device=dev) * 0.5 + torch.linspace(0.3, 0.7, D, device=dev)).half()
+    out = ops.gqa_chunk_paged(*args)
+    ops.raise_device_errors(dev)
+    off = []
+    for t in range(0, 296, 30):
+        for h in range(0, 128, 13):
+            want, *_ = exactly(args, rows, 0, t, h)
+            off.append((out[t, h].double() - want) / want)
+    mean = float(torch.cat(off).mean())
+    assert abs(mean) <= 2.0 ** -13 + 2.0 ** -14, mean
