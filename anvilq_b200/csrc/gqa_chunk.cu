@@ -1232,11 +1232,16 @@ int anvilq_gqa_chunk_paged(const uint16_t* q, long long q_stride, const uint16_t
   if (T == 0) return ANVILQ_OK;
   const size_t pool = (size_t)positions * Hkv * D * 2, rows = (size_t)T * Hq * D * 2;
   const size_t read = ((size_t)(T - 1) * q_stride + (size_t)Hq * D) * 2;
-  if (overlap(out, rows, q, read) || overlap(out, rows, k_pool, pool) || overlap(out, rows, v_pool, pool) ||
-      overlap(out, rows, page_table, (size_t)B * max_pages * 4) || overlap(out, rows, seqlens, (size_t)B * 4) ||
-      overlap(out, rows, token_starts, (size_t)(B + 1) * 4) ||
-      (workspace && overlap(out, rows, workspace, workspace_bytes)))
-    return ANVILQ_EINVAL;
+  // the outputs and the workspace are written while all else is still to be read
+  const struct {
+    const void* start;
+    size_t bytes;
+  } reads[] = {{q, read}, {k_pool, pool}, {v_pool, pool}, {page_table, (size_t)B * max_pages * 4},
+               {seqlens, (size_t)B * 4}, {token_starts, (size_t)(B + 1) * 4}};
+  const size_t scratch = workspace ? workspace_bytes : 0;
+  for (const auto& r : reads)
+    if (overlap(out, rows, r.start, r.bytes) || overlap(workspace, scratch, r.start, r.bytes)) return ANVILQ_EINVAL;
+  if (overlap(out, rows, workspace, scratch)) return ANVILQ_EINVAL;
   const int sms = sm_count();
   if (sms <= 0) return ANVILQ_ECUDA;
   const size_t need = anvilq_gqa_chunk_paged_workspace_size(T, B, Hq, Hkv, D, page_tokens, max_pages);

@@ -766,7 +766,8 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
  * gives zeros.  scale (finite, at most 2^32) <= 0 selects 1/sqrt(D).  Hq % Hkv == 0,
  * Hq <= 1024, Hq / Hkv <= 128, B <= 65535, T <= 2^30; D, page_tokens and positions as
  * for the append, at most 2^31 - 1 positions in a pool; 16-byte aligned q, pools, out
- * and workspace; out apart from all inputs; dev_err required; T == 0 does nothing.
+ * and workspace; out and workspace apart from all inputs and each other; dev_err required; T == 0
+ * does nothing.
  * Of the sequences with new tokens, one with more of them than seqlens[b], or longer
  * than page_tokens * max_pages, sets ANVILQ_DEV_ERR_SEQLEN and its rows are not
  * written; an absent live page sets ANVILQ_DEV_ERR_PAGE (the output is then not to be
