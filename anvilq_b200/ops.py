@@ -1152,7 +1152,7 @@ def beam_select(logits, scores, N: int | None = None, lengths=None, length_penal
 def beam_reorder(states, parents, outs=None, dev_err=None, overlap_prior: bool = False):
     """Per-beam rows by their parents: for each of `states` ([B, K, ...] of any type,
     contiguous) a tensor [B, N, ...] whose row n of item b is row parents[b, n]
-    (int32 [B, N], ``beam_select``'s) of the item's, zeros for -1.  outs: tensors of that
+    (int32 [B, N], ``beam_select``'s) of the item's, zeros for -1; rows may be empty.  outs: tensors of that
     shape to write to, apart from the states.  Page tables go by ``pages_fork``, which
     keeps the pages' counts."""
     name = "beam_reorder"
@@ -1162,11 +1162,11 @@ def beam_reorder(states, parents, outs=None, dev_err=None, overlap_prior: bool =
     states = list(states)
     if outs is not None and len(outs) != len(states):
         raise ValueError(f"{name}: as many outs as states expected")
-    results, array = [], (_lib.BeamState * len(states))()
+    results, array, count = [], (_lib.BeamState * len(states))(), 0
     for i, t in enumerate(states):
         shape = t.shape
         K = shape[1] if K is None and len(shape) > 1 else K
-        if shape[:2] != (B, K) or 0 in shape or not t.is_contiguous():
+        if shape[:2] != (B, K) or 0 in shape[:2] or not t.is_contiguous():
             raise ValueError(f"{name}: states must be contiguous [{B}, K, ...] with one K")
         rest = shape[2:]
         if outs is None:
@@ -1176,13 +1176,15 @@ def beam_reorder(states, parents, outs=None, dev_err=None, overlap_prior: bool =
             if o.dtype != t.dtype or o.shape != (B, N, *rest) or not o.is_contiguous():
                 raise ValueError(f"{name}: out {i} must be contiguous {t.dtype} {[B, N, *rest]}")
         results.append(o)
-        array[i].input, array[i].output = t.data_ptr(), o.data_ptr()
-        array[i].row_bytes = t.numel() // (B * K) * t.element_size()
+        if t.numel():                        # rows of no elements (a history before its first token): nothing to move
+            array[count].input, array[count].output = t.data_ptr(), o.data_ptr()
+            array[count].row_bytes = t.numel() // (B * K) * t.element_size()
+            count += 1
     _on_device(name, dev, *states, *results)
-    if not states:
+    if not count:
         return results
     err = _error_word(dev, dev_err)
-    _call("anvilq_beam_reorder", dev, array, len(states), parents.data_ptr(), B, K, N, err.data_ptr(),
+    _call("anvilq_beam_reorder", dev, array, count, parents.data_ptr(), B, K, N, err.data_ptr(),
           GEMM_OVERLAP_PRIOR if overlap_prior else 0, _stream_ptr(dev))
     return results
 

@@ -1,4 +1,5 @@
-"""Beam selection at the edges of what it accepts: values that are not finite among masked ones.
+"""Beam selection at the edges of what it accepts: values that are not finite among masked ones,
+rows of no elements.
 
 Tolerances and the definition: ``test_gpu_beam``."""
 import pytest
@@ -30,3 +31,19 @@ def test_bad_values_among_masked_ones_are_reported(dev, V, at, left, bad, half):
     check(clean, scores, 6, got=got)
     ops.beam_select(clean, scores, 6)
     ops.raise_device_errors(dev)             # masks alone are no error
+
+
+def test_reorder_of_empty_rows(dev):
+    """A search's first step: histories of no tokens among other states, or alone, given outputs or not."""
+    parents = torch.tensor([[1, 0, -1], [2, 2, 1]], dtype=torch.int32, device=dev)
+    scores = torch.arange(6, device=dev).reshape(2, 3).float()
+    history, wide = (torch.empty((2, 3, *rest), dtype=torch.int32, device=dev) for rest in ((0,), (4, 0)))
+    a, b, c = ops.beam_reorder([history, scores, wide], parents)
+    assert a.shape == (2, 3, 0) and a.dtype == torch.int32 and c.shape == (2, 3, 4, 0)
+    assert b.tolist() == [[1, 0, 0], [5, 5, 4]]
+    assert ops.beam_reorder([history], parents)[0].shape == (2, 3, 0)
+    out = torch.empty((2, 3, 0), dtype=torch.int32, device=dev)
+    assert ops.beam_reorder([history], parents, outs=[out])[0] is out
+    with pytest.raises(ValueError):
+        ops.beam_reorder([history, torch.zeros((2, 4), device=dev)], parents)      # another K all the same
+    ops.raise_device_errors(dev)
