@@ -763,8 +763,9 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e6, scaling: dict | None =
             raise ValueError("rope_frequencies: original >= 1 and limits with 0 < lower < upper expected")
         if kind == "yarn":
             at = lambda turns: R * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(theta))
-            lo, hi = max(0, math.floor(at(most))), min(R // 2 - 1, math.ceil(at(least)))
-            slow = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(R // 2)]
+            # the ramp may end behind the last pair, where that still turns fast enough
+            lo, hi = max(0, math.floor(at(most))), min(R - 1, math.ceil(at(least)))
+            slow = [1.0 if i >= hi else 0.0 if i <= lo else (i - lo) / (hi - lo) for i in range(R // 2)]
             factor = 0.1 * math.log(s) + 1.0
         else:
             slow = [1.0 - min(1.0, max(0.0, (n * f / (2 * math.pi) - least) / (most - least))) for f in inv]
