@@ -9,10 +9,16 @@
 // place k V + v.
 //
 // Within a beam the order is that of the logits, which is exact; across beams it hangs
-// on the lse, so that is held to about 1e-8: the exponent of exp2((l - c) log2 e) is
-// formed from a difference and a product in two parts, a thread's partial sums are
-// short, and everything from a span's sum on is binary64.  Candidates of different
-// beams whose ranks differ by less may come in either order.
+// on the lse.  The exponent of exp2((l - c) log2 e) is formed from a difference and a product
+// in two parts, a thread's partial sums are short, and everything from a span's sum on is
+// binary64.  The lse is off by at most
+//   3 2^-22 (ex2.approx, of a logit to its thread's largest, that to the span's, that to the row's)
+//   + 2^-23 d (their exponents' two roundings; d: the logits' mean distance to the row's largest,
+//     weighted by their exponentials) + 32 2^-24 (a tile's additions of a thread)
+//   + V / 4096 (2^-22 + 2 2^-24) (for each of a thread's tiles its addition, and the sum taken
+//     to a new largest, if every tile has one),
+// below 3e-6 + 2^-23 d + 4e-7 V / 4096.  Random logits' sums were 2e-8 off.  Candidates of
+// different beams whose scores are closer than that may come in either order.
 //
 // What bounds it: the logits are read once (HBM); about 7 instructions a logit.  A
 // small call is bound by latency: load, threshold, merge.

@@ -824,8 +824,11 @@ int anvilq_logits_process(const void* logits, int logits_half, long long logits_
  *   s = S + (l - log sum_v exp(l)),   rank = s / (n + 1)^length_penalty,
  * or, where finished[b][k] is not 0, one candidate, pad_id with s = S and
  * rank = S / max(n, 1)^length_penalty, standing at v = 0.  The N largest ranks win,
- * equal ones by the lowest k V + v; sums are held to about 1e-8, ranks of different
- * beams that are closer may come in either order.  Results, best first, [B][N]:
+ * equal ones by the lowest k V + v.  The order within a beam is exact.  A beam's log sum is
+ * off by at most 3e-6 + 2^-23 d + 4e-7 V / 4096, d the mean distance of its logits to the
+ * largest, each weighted by its exponential (fp32 exponentials and partial sums; 2e-8 on random
+ * logits), new_scores besides by half a step; candidates of different beams whose scores are
+ * closer than that may come in either order.  Equal rows have equal sums.  Results, best first, [B][N]:
  *   tokens, parents (the beam k), new_scores (s), new_lengths (n + 1, n of a finished
  *   beam), new_finished (1: of a finished beam, or one of the eos_count eos_ids)
  * and where there are fewer candidates -1, -1, -inf, 0, 1.  A logit of +inf or NaN

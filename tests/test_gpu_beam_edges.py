@@ -1,5 +1,5 @@
 """Beam selection at the edges of what it accepts: values that are not finite among masked ones,
-rows of no elements.
+rows of no elements, log sums of rows that do not average.
 
 Tolerances and the definition: ``test_gpu_beam``."""
 import pytest
@@ -47,3 +47,41 @@ def test_reorder_of_empty_rows(dev):
     with pytest.raises(ValueError):
         ops.beam_reorder([history, torch.zeros((2, 4), device=dev)], parents)      # another K all the same
     ops.raise_device_errors(dev)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("kind", ["two", "three", "ten", "rising", "steep"])
+def test_scores_of_rows_that_do_not_average(dev, kind, half):
+    """Rows of a few live logits, and rows whose largest so far moves with every tile: the log sums are within
+    3e-6 + 2^-23 d + 4e-7 V / 4096, which include/anvilq.h states, the scores within half a step more."""
+    V = 151936
+    g = torch.Generator(device=dev)
+    g.manual_seed(len(kind))
+    x = torch.full((3, 4, V), -float("inf"), device=dev)
+    if kind in ("rising", "steep"):
+        x[:] = torch.arange(V, device=dev) * ((1 if kind == "rising" else 30) / V)
+        x += torch.rand((3, 4, 1), generator=g, device=dev)
+    else:
+        n = {"two": 2, "three": 3, "ten": 10}[kind]
+        for b in range(3):
+            for k in range(4):
+                at = torch.randperm(V, generator=g, device=dev)[:n]
+                x[b, k, at] = torch.randn(n, generator=g, device=dev) * 2 ** (b - 1) + 5 * k
+    x = x.half() if half else x
+    scores = -torch.rand((3, 4), generator=g, device=dev) * 10
+    tokens, parents, new, *_ = ops.beam_select(x, scores, 8)
+    ops.raise_device_errors(dev)
+    y = x.double()
+    top = y.amax(dim=2, keepdim=True)
+    e = torch.exp(y - top)
+    total = e.sum(dim=2)
+    d = torch.where(e > 0, e * (top - y), 0.0).sum(dim=2) / total
+    lse = top[..., 0] + torch.log(total)
+    for b in range(3):
+        for i in range(8):
+            if int(tokens[b, i]) < 0:
+                continue
+            k = int(parents[b, i])
+            want = float(scores[b, k].double() + y[b, k, int(tokens[b, i])] - lse[b, k])
+            bound = 3e-6 + 2.0 ** -23 * float(d[b, k]) + 4e-7 * V / 4096 + 2.0 ** -24 * abs(want)
+            assert abs(float(new[b, i]) - want) <= bound, (b, i, float(new[b, i]) - want, bound)
