@@ -72,9 +72,11 @@ constexpr int kLeast = 1;                  // key tiles' worth of units of a str
 constexpr int kMaxCtas = 148;
 // Key tiles of a segment, at most.  The tensor cores add to binary32 by cutting off, up to 2^-23 of the sum at
 // each 16 keys and always downwards: over 2^20 keys of equal weights 6.7e-3.  So after a segment the
-// products begin anew, and its outputs are added to those before by rounded operations: 1e-4 at any length.
-// (4096 tokens at the end of 65536 positions, 32/8 heads: with heads of 64 3.3 ms as without, of 128 4.0 and 3.8.)
+// products begin anew, and its outputs are added to those before by rounded operations, when the products go
+// on: 1e-4 at any length.  (4096 tokens after 61440, 32/8 heads: of 128 4.20 ms, 4.08 without, of 64 3.48 as without;
+// with outputs added before the products go on 4.43 and 3.64.)
 constexpr int kPiece = 128;
+constexpr int kSlots = 3;
 constexpr int kMaxBatch = 65536;
 constexpr float kNone = -1e30f;            // a reference below every exponent
 // How far (log2) the reference is below a row's largest when it is set, and may lag behind it later: the
@@ -106,8 +108,8 @@ struct Params {
   const int* seqlens;           // [B]
   const uint32_t* page_table;   // [B][max_pages]
   __half* out;                  // [T][Hq][D]
-  // [CTAs][2][256 (D + 2)]: sums of a share that is not all of a pair, or not one segment; a share that an
-  // earlier CTA's goes before is the stretch's first, and has the first place
+  // [CTAs][kSlots][256 (D + 2)]: sums of a share that is not all of a pair, or not one segment; the first place is
+  // for a stretch's first share where an earlier CTA's goes before it, the last for a segment's yet to be added
   float* partials;
   float2* fresh;                // [CTAs][256]: references and sums of a segment that others of its share came before
   struct Open* open;            // [CTAs]
@@ -773,93 +775,71 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     {
       // ------------------------------------------------------------------ stores
-      const int row = warp % 4 * 32 + lane, of_token = row / p.group, of_head = row % p.group;
+      const int row = warp % 4 * 32 + lane, of_token = row / p.group;
       auto leave = [&](int t) {   // tile t's outputs are out of TMEM
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(o_empty(t));
       };
+      // A place's outputs [dims / 4][row] of tile t, and its states [row].
+      auto place = [&](int i, int t) {
+        return reinterpret_cast<float4*>(p.partials + ((size_t)blockIdx.x * kSlots + i) * (2 * kRows * (D + 2))) + t * kRows + row;
+      };
+      auto state_at = [&](int i, int t) {
+        return reinterpret_cast<float2*>(p.partials + ((size_t)blockIdx.x * kSlots + i) * (2 * kRows * (D + 2)) + 2 * kRows * D) +
+               t * kRows + row;
+      };
+      auto token_of = [&](int t) { return (2 * g.i + t) * p.tpt + of_token; };   // of the sequence's new ones
+      auto is_token = [&](int t) { return of_token < p.tpt && token_of(t) < g.s.n; };
+      auto out_at = [&](int t) {
+        return p.out + ((long long)(g.s.start + token_of(t)) * p.Hq + g.h * p.group + row - of_token * p.group) * D;
+      };
+      // no other segment and no other CTA has more of the tile
+      auto is_last = [&](int t) { return !(g.part & kShared) && tiles_to(g.s, (2 * g.i + t + 1) * p.tpt) <= g.j1; };
       unsigned phases = 0;   // of the next sums (bit t) and of the products (bit 2 + t) of tile t
       bool ok = true;
       while (ok && next_segment(p, w, g)) {
-        // sums of a share that others merge, or that goes on in another segment
-        float4* slot = reinterpret_cast<float4*>(
-            p.partials + ((size_t)blockIdx.x * 2 + (g.part & kMid ? 0 : 1)) * (2 * kRows * (D + 2)));
-#pragma unroll 1
+        const int own = g.part & kMid ? 0 : 1;   // the place of the share's sums
+        const bool on = g.part & kOn;
+#pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int end = g.end(p, t), first = (2 * g.i + t) * p.tpt;
-          if (!ok) continue;
-          float2* state = reinterpret_cast<float2*>(slot + 2 * kRows * (D / 4)) + t * kRows + row;
+          const int end = g.end(p, t);
           if (end <= g.j0) {
-            if ((g.part & (kShared | kOn)) == kShared) __stcg(state, make_float2(kNone, 0.0f));   // the merge reads both tiles'
+            if ((g.part & (kShared | kOn)) == kShared) __stcg(state_at(own, t), make_float2(kNone, 0.0f));   // the merge reads both tiles'
             continue;
           }
-          const bool mine = of_token < p.tpt && first + of_token < g.s.n;
+          const bool mine = is_token(t), last = is_last(t);
+          // the outputs of a segment that others came before go out of the way, to be added below
+          float4* to = place(on ? kSlots - 1 : own, t);
+          __half* out = out_at(t);
           phases ^= (unsigned)(end - g.j0 & 1) << (2 + t);
           ok = wait(sums_full(t), phases >> t & 1) && wait(pv_done(t), ~phases >> (2 + t) & 1);
           phases ^= 1u << t;
           if (!ok) break;
           tc_fence_after();
-          const bool last = !(g.part & kShared) && tiles_to(g.s, first + p.tpt) <= g.j1;   // the outputs are whole
-          const uint32_t o_at = tmem + kTmemO + t * 128 + ((uint32_t)(warp % 4 * 32) << 16);
-          float4* at = slot + t * kRows + row;   // [dims / 4][row]
-          __half* out = p.out + ((long long)(g.s.start + first + of_token) * p.Hq + g.h * p.group + of_head) * D;
-          if (g.part & kOn) {   // added to the segments before
-            float f_then = 0.0f, f = 0.0f;
-            if (mine) {
-              const float2 then = __ldcg(state), now = __ldcg(p.fresh + blockIdx.x * (2 * kRows) + t * kRows + row);
-              const float top = fmaxf(then.x, now.x);
-              f_then = fast_exp2(then.x - top);
-              f = fast_exp2(now.x - top);
-              const float sum = then.y * f_then + now.y * f, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-              if (last) {
-                f_then *= inv;
-                f *= inv;
-              } else {
-                __stcg(state, make_float2(top, sum));
-              }
+          if (on && mine) {
+            const float2 then = __ldcg(state_at(own, t)), now = __ldcg(p.fresh + blockIdx.x * (2 * kRows) + t * kRows + row);
+            const float top = fmaxf(then.x, now.x);
+            float f_then = fast_exp2(then.x - top), f = fast_exp2(now.x - top);
+            const float sum = then.y * f_then + now.y * f;
+            if (last) {
+              const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+              f_then *= inv;
+              f *= inv;
+            } else {
+              __stcg(state_at(own, t), make_float2(top, sum));
             }
-#pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              uint32_t o[16];
-              tmem_ld16(o_at + c, o);
-              wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16 && mine; e += 8) {
-                float4 v[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const uint32_t* n = o + e + 4 * k;
-                  v[k] = __ldcg(at + ((c + e) / 4 + k) * (2 * kRows));
-                  v[k].x = v[k].x * f_then + __uint_as_float(n[0]) * f;
-                  v[k].y = v[k].y * f_then + __uint_as_float(n[1]) * f;
-                  v[k].z = v[k].z * f_then + __uint_as_float(n[2]) * f;
-                  v[k].w = v[k].w * f_then + __uint_as_float(n[3]) * f;
-                  if (!last) __stcg(at + ((c + e) / 4 + k) * (2 * kRows), v[k]);
-                }
-                if (last) {
-                  uint4 w;
-                  __half2* h = reinterpret_cast<__half2*>(&w);
-                  h[0] = __floats2half2_rn(v[0].x, v[0].y);
-                  h[1] = __floats2half2_rn(v[0].z, v[0].w);
-                  h[2] = __floats2half2_rn(v[1].x, v[1].y);
-                  h[3] = __floats2half2_rn(v[1].z, v[1].w);
-                  *reinterpret_cast<uint4*>(out + c + e) = w;
-                }
-              }
-            }
-            leave(t);
-            continue;
+            __stcg(state_at(kSlots - 1, t), make_float2(f_then, f));   // factors of the outputs before, and of these
           }
           const float sum = sh.sums[t][row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // (only scores of -inf: zeros)
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
-            tmem_ld32(o_at + c, o);
+            tmem_ld32(tmem + kTmemO + t * 128 + ((uint32_t)(warp % 4 * 32) << 16) + c, o);
             wait_ld();
             if (c + 32 == D) leave(t);
             if (!mine) continue;
-            if (last) {
+            if (last && !on) {
 #pragma unroll
               for (int e = 0; e < 32; e += 16) {   // a sector at a time
                 uint32_t v[8];
@@ -881,8 +861,47 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
-                __stcg(at + (c + e) / 4 * (2 * kRows), make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]),
+                __stcg(to + (c + e) / 4 * (2 * kRows), make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]),
                                                                    __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])));
+            }
+          }
+        }
+        if (!on || !ok) continue;
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {   // added to the outputs before
+          if (g.end(p, t) <= g.j0 || !is_token(t)) continue;
+          const bool last = is_last(t);
+          const float2 factor = __ldcg(state_at(kSlots - 1, t));
+          float4* at = place(own, t);
+          const float4* more = place(kSlots - 1, t);
+          __half* out = out_at(t);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            float4 a[4], b[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              a[k] = __ldcg(at + (c / 4 + k) * (2 * kRows));
+              b[k] = __ldcg(more + (c / 4 + k) * (2 * kRows));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              a[k].x = a[k].x * factor.x + b[k].x * factor.y;
+              a[k].y = a[k].y * factor.x + b[k].y * factor.y;
+              a[k].z = a[k].z * factor.x + b[k].z * factor.y;
+              a[k].w = a[k].w * factor.x + b[k].w * factor.y;
+              if (!last) __stcg(at + (c / 4 + k) * (2 * kRows), a[k]);
+            }
+            if (!last) continue;
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+              uint4 v;
+              __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                h[2 * e] = __floats2half2_rn(a[k + e].x, a[k + e].y);
+                h[2 * e + 1] = __floats2half2_rn(a[k + e].z, a[k + e].w);
+              }
+              *reinterpret_cast<uint4*>(out + c + 4 * k) = v;
             }
           }
         }
@@ -969,7 +988,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         phases ^= 2;
         sh.sums[t][row] = sum;
         if (!(g.part & kOne)) {   // for the merge, or the stores
-          float* slot = p.partials + ((size_t)blockIdx.x * 2 + (g.part & kMid ? 0 : 1)) * (2 * kRows * (D + 2));
+          float* slot = p.partials + ((size_t)blockIdx.x * kSlots + (g.part & kMid ? 0 : 1)) * (2 * kRows * (D + 2));
           float2* to = g.part & kOn ? p.fresh + blockIdx.x * (2 * kRows) : reinterpret_cast<float2*>(slot + 2 * kRows * D);
           __stcg(to + t * kRows + row, make_float2(scale == p.scale_log2 ? m : m / scale * p.scale_log2, sum));
         }
@@ -1031,8 +1050,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
     const bool mine = token_of(r) >= 0;
     const int n = (int)(o.end / o.chunk) - second + 2;   // CTAs
     // the pair is the last of the CTA that began it, the first of the others
-    const float* begin = p.partials + ((size_t)(second - 1) * 2 + 1) * kSlot;
-    const float* others = p.partials + (size_t)second * 2 * kSlot;
+    const float* begin = p.partials + ((size_t)(second - 1) * kSlots + 1) * kSlot;
+    const float* others = p.partials + (size_t)second * kSlots * kSlot;
     float m = kNone, sum = 0.0f;
     float4 acc[kMine];
 #pragma unroll
@@ -1044,7 +1063,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       for (int k = 0; k < kAtOnce; ++k) {
         state[k] = make_float2(kNone, 0.0f);
         if (c0 + k < n) {
-          const float* slot = c0 + k ? others + (size_t)(c0 + k - 1) * 2 * kSlot : begin;
+          const float* slot = c0 + k ? others + (size_t)(c0 + k - 1) * kSlots * kSlot : begin;
           state[k] = __ldcg(reinterpret_cast<const float2*>(slot + 2 * kRows * D) + r);
 #pragma unroll
           for (int i = 0; i < kMine; ++i)
@@ -1193,7 +1212,7 @@ static int ctas_for(int sms, int T, int B, int Hq, int Hkv, long long capacity) 
   const double pairs = ((double)T / (2 * tpt) + std::min(T, B)) * Hkv;
   return (int)std::max(1.0, std::min({(double)std::min(sms, kMaxCtas), pairs * (double)((capacity + kKeys - 1) / kKeys)}));
 }
-static size_t partial_bytes(int ctas, int D) { return (size_t)ctas * 2 * 2 * kRows * (D + 2) * sizeof(float); }
+static size_t partial_bytes(int ctas, int D) { return (size_t)ctas * kSlots * 2 * kRows * (D + 2) * sizeof(float); }
 
 }  // namespace chunk
 }  // namespace anvilq
