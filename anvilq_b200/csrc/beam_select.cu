@@ -20,8 +20,9 @@
 // below 3e-6 + 2^-23 d + 4e-7 V / 4096.  Random logits' sums were 2e-8 off.  Candidates of
 // different beams whose scores are closer than that may come in either order.
 //
-// What bounds it: the logits are read once (HBM); about 7 instructions a logit.  A
-// small call is bound by latency: load, threshold, merge.
+// What bounds it: the logits are read once (HBM), 13 instructions a fp16 logit, 27 a fp32 one
+// in spans of 7 tiles a warp, whose beginning and end count.  A small call is bound by
+// latency: load, threshold, merge.
 //
 // Work split.  A CTA takes a span of a beam's vocabulary (splits so that the device is
 // full, splits_for), its warps tiles of 32 x 4 x 16 bytes in turn, without a barrier: a
@@ -31,10 +32,11 @@
 // the tile in all).  The span's sum and N best go to the workspace, and the item's last
 // CTA (by a ticket) merges them.
 //
-// Measured: 48 x 8 beams over 151936 fp16 logits, some masked, some beams ended, 59 us (2.0
+// Measured: 48 x 8 beams over 151936 fp16 logits, some masked, some beams ended, 60 us (1.9
 // TB/s: a tile's dependent instructions at 21 warps an SM, issue slots 30 % busy; 8 us of a
-// CTA's beginning and end); 100 x 5 over 32000 fp32 logits, N = 10, 34 us; one item's 4 beams
-// over 151936 15 us with the reordering.
+// CTA's beginning and end); 100 x 5 over 32000 fp32 logits, N = 10, 35 us; one item's 4 beams
+// over 151936 17 us with the reordering.  Rows off 16 bytes are loaded logit by logit: 48 x 8 over
+// 50257 fp16 logits 40.5 us, over 50256 30.2; fp32 66 and 35.
 #include <algorithm>
 #include <climits>
 #include <cmath>

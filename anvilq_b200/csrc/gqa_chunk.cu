@@ -39,10 +39,12 @@
 // What bounds it: two tiles' step of 128 keys is 2048 cycles of the tensor cores and as
 // many of the MUFU (an exponential a score), and takes 4100, as a tile's chain does: softmax
 // 1830, its products and next scores 1400, hand-overs.  With D = 128 two S and two O fill the
-// TMEM, so there is no second S to take the chain apart.  Measured, 32/8 heads of 128: 4096
-// tokens after 12288 in 869 us (1107 TFLOP/s of the causal products; 1012 us when run on end,
-// under the power cap), 60 tokens after 60001 in 86 us with the merge (2.9 TB/s); 13 tokens
-// after 150 of 14/2 heads of 64 in 12 us: plan 3, first copies 3.5, two steps, merge.
+// TMEM, so there is no second S to take the chain apart; with D = 64 a quarter of it is left,
+// which this kernel does not use.  Measured, 32/8 heads of 128: 4096 tokens after 12288 in
+// 890 us (1080 TFLOP/s of the causal products; 1001 us when run on end, under the power cap),
+// 60 tokens after 60001 in 88 us with the merge (2.8 TB/s); 14/2 heads of 64: eight prompts of
+// 117 to 2000 tokens after 133 to 1000 in 104 us (390 TFLOP/s), 13 tokens after 150 in 12 us: plan 3,
+// first copies 3.5, two steps, merge.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

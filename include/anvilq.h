@@ -759,8 +759,10 @@ int anvilq_gqa_decode_q8(const uint16_t* q, const void* k_codes, const void* v_c
  * puts its key and value into the pages before) is at position seqlens[b] -
  * token_starts[b + 1] + t and sees every position up to its own.  q and out fp16 [T]
  * tokens of [Hq][D], q's q_stride elements apart (a multiple of 8, at most 2^38), out's without
- * gaps; rows of no sequence are neither read nor written.  Scores, sums and outputs in
- * fp32, the probabilities enter the tensor cores as binary16.  What lies behind a
+ * gaps; rows of no sequence are not written, and what they hold does not matter.  Scores, sums
+ * and outputs in fp32, the probabilities enter the tensor cores as binary16, off by 2^-11 of each, or
+ * 2^-32 of the row's largest; sums over any length lose at most 2^-13 of them to the tensor
+ * cores' cutting off.  What lies behind a
  * sequence's last token may be anything; a NaN or an infinity among the values of new
  * tokens would reach the queries before them too.  A query whose scores are all -inf
  * gives zeros.  scale (finite, at most 2^32) <= 0 selects 1/sqrt(D).  Hq % Hkv == 0,
