@@ -78,7 +78,7 @@ constexpr int kMaxCtas = 148;
 // on: 1e-4 at any length.  (4096 tokens after 61440, 32/8 heads: of 128 4.20 ms, 4.08 without, of 64 3.48 as without;
 // with outputs added before the products go on 4.43 and 3.64.)
 constexpr int kPiece = 128;
-constexpr int kSlots = 3;
+constexpr int kSlots = 3;                  // of partial sums a CTA
 constexpr int kMaxBatch = 65536;
 constexpr float kNone = -1e30f;            // a reference below every exponent
 // How far (log2) the reference is below a row's largest when it is set, and may lag behind it later: the
@@ -784,12 +784,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(o_empty(t));
       };
       // A place's outputs [dims / 4][row] of tile t, and its states [row].
-      auto place = [&](int i, int t) {
-        return reinterpret_cast<float4*>(p.partials + ((size_t)blockIdx.x * kSlots + i) * (2 * kRows * (D + 2))) + t * kRows + row;
-      };
+      auto start_of = [&](int i) { return p.partials + ((size_t)blockIdx.x * kSlots + i) * (2 * kRows * (D + 2)); };
+      auto place = [&](int i, int t) { return reinterpret_cast<float4*>(start_of(i)) + t * kRows + row; };
       auto state_at = [&](int i, int t) {
-        return reinterpret_cast<float2*>(p.partials + ((size_t)blockIdx.x * kSlots + i) * (2 * kRows * (D + 2)) + 2 * kRows * D) +
-               t * kRows + row;
+        return reinterpret_cast<float2*>(start_of(i) + 2 * kRows * D) + t * kRows + row;
       };
       auto token_of = [&](int t) { return (2 * g.i + t) * p.tpt + of_token; };   // of the sequence's new ones
       auto is_token = [&](int t) { return of_token < p.tpt && token_of(t) < g.s.n; };
@@ -807,7 +805,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = 0; t < 2; ++t) {
           const int end = g.end(p, t);
           if (end <= g.j0) {
-            if ((g.part & (kShared | kOn)) == kShared) __stcg(state_at(own, t), make_float2(kNone, 0.0f));   // the merge reads both tiles'
+            // the merge reads both tiles'
+            if ((g.part & (kShared | kOn)) == kShared) __stcg(state_at(own, t), make_float2(kNone, 0.0f));
             continue;
           }
           const bool mine = is_token(t), last = is_last(t);
@@ -820,7 +819,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           tc_fence_after();
           if (on && mine) {
-            const float2 then = __ldcg(state_at(own, t)), now = __ldcg(p.fresh + blockIdx.x * (2 * kRows) + t * kRows + row);
+            const float2 then = __ldcg(state_at(own, t));
+            const float2 now = __ldcg(p.fresh + (blockIdx.x * 2 + t) * kRows + row);
             const float top = fmaxf(then.x, now.x);
             float f_then = fast_exp2(then.x - top), f = fast_exp2(now.x - top);
             const float sum = then.y * f_then + now.y * f;
@@ -863,8 +863,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
-                __stcg(to + (c + e) / 4 * (2 * kRows), make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]),
-                                                                   __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])));
+                __stcg(to + (c + e) / 4 * (2 * kRows),
+                       make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                   __uint_as_float(o[e + 3])));
             }
           }
         }
@@ -991,7 +992,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         sh.sums[t][row] = sum;
         if (!(g.part & kOne)) {   // for the merge, or the stores
           float* slot = p.partials + ((size_t)blockIdx.x * kSlots + (g.part & kMid ? 0 : 1)) * (2 * kRows * (D + 2));
-          float2* to = g.part & kOn ? p.fresh + blockIdx.x * (2 * kRows) : reinterpret_cast<float2*>(slot + 2 * kRows * D);
+          float2* to = reinterpret_cast<float2*>(slot + 2 * kRows * D);
+          if (g.part & kOn) to = p.fresh + blockIdx.x * (2 * kRows);
           __stcg(to + t * kRows + row, make_float2(scale == p.scale_log2 ? m : m / scale * p.scale_log2, sum));
         }
         __syncwarp();

@@ -87,7 +87,8 @@ def test_many_keys_far_below_the_largest(dev, below, D):
     # page 0 first, the others in turn
     names = np.concatenate([[0], 1 + np.arange(n // page - 1) % kinds])
     table = (names.astype(np.uint32) | np.uint32(so.VALID)).view(np.int32)[None]
-    out = ops.gqa_chunk_paged(*(to(a, dev) for a in (q, k, v, table, np.array([n], np.int32), np.array([0, T], np.int32))))
+    lens, starts = np.array([n], np.int32), np.array([0, T], np.int32)
+    out = ops.gqa_chunk_paged(*(to(a, dev) for a in (q, k, v, table, lens, starts)))
     ops.raise_device_errors(dev)
     got = out.cpu().numpy().astype(np.float64)
     keys, values = k.reshape(-1, D).astype(np.float64), v.reshape(-1, D).astype(np.float64)
